@@ -140,6 +140,8 @@ _SIGNATURES = {
     "pb_recurrence_workspace": [_I, _I, _I, _I, _I, _I],
     "pb_matrix_memory": [_I, _P, _L, _P, _P, _F, _P, _F, _F, _F, _P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "pb_state_space": [_I, _P, _L, _P, _P, _I, _P, _P, _P, _P, _I, _F, _P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P],
+    "pb_copy_pages": [_I, _P, _P, _P, _P, _P, _I, _P],
+    "pb_token_scores": [_I, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P],
 }
 _RETURNS = {"pb_recurrence_workspace": _L}        # the others return an int
 _fns = {}
@@ -152,7 +154,8 @@ _LAUNCHERS = {"embed", "scale_cap", "move_ids", "add_rmsnorm", "rope_table", "qk
               "paged_attention_general", "paged_attention_general_tiled", "paged_attention_general_tc", "qkv_split_write", "heads_linear", "latent_prepare", "latent_norms", "latent_expand_keys", "sigmoid_gate", "causal_conv_silu",
               "selective_scan", "selective_scan_prompt", "selective_scan_chunked", "post_norm_add", "clamped_glu",
               "post_norm_add_bias", "glu_bias", "qk_prepare", "qk_prepare_whole", "sigmoid_gate_strided", "add_bias", "moe_route", "moe_gate_up", "moe_up", "moe_down", "moe_grouped",
-              "norm_shift", "parallel_add", "activation", "min_gru", "diff_combine", "retention", "scaled_sum", "concat_streams", "normed_sum", "matrix_memory", "state_space"}
+              "norm_shift", "parallel_add", "activation", "min_gru", "diff_combine", "retention", "scaled_sum", "concat_streams", "normed_sum", "matrix_memory", "state_space",
+              "copy_pages", "token_scores"}
 
 
 class KernelError(RuntimeError):
@@ -1905,3 +1908,82 @@ def concat_streams(residual: torch.Tensor, delta: Optional[torch.Tensor], origin
     assert residual.dtype == origin.dtype == torch.float32 and origin.shape == (n, width) and out.shape == (n, 2 * width)
     assert delta is None or (delta.shape == (n, width) and delta.dtype == out.dtype)
     check(fn("pb_concat_streams")(code(out.dtype), _p(residual), _p(delta), _p(origin), _p(out), n, width, stream()), "concat_streams")
+
+
+# ------------------------------------------------------------------ several scored continuations of one prompt
+_MOST_POOLS = 16                  # of one launch (csrc/pages.cu)
+
+
+def _page_run(pool: torch.Tensor) -> None:
+    """Refuses a pool whose pages are not one run of bytes each ([entries, pages, ...], the entries at any distance)."""
+    if not pool.is_cuda:
+        raise KernelError(f"kernel arguments must be CUDA tensors (found device {pool.device}); there is no CPU path")
+    if pool.dim() < 2:
+        raise KernelError(f"copy_pages: a pool is [entries, pages, ...], found {tuple(pool.shape)}")
+    if pool.numel() and not pool[0].is_contiguous():
+        raise KernelError("copy_pages: the pages of an entry must lie one behind the other")
+
+
+def copy_pages(src_pools, dst_pools, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """dst_pools[k][:, dst[i]] = src_pools[k][:, src[i]] for all pools k and pairs i.  A pool is [entries, pages, ...] (a cache's, or
+    fixed-size states as one entry); ``dst_pools`` may be ``src_pools``.  ``src``, ``dst`` int32 [n] on the device.  The pairs are not
+    ordered: no page may be both read and written, none written twice.  A pair with an id outside a pool is left out there."""
+    src_pools, dst_pools = list(src_pools), list(dst_pools)
+    _cuda(src, dst)
+    if src.dtype != torch.int32 or dst.dtype != torch.int32 or src.numel() != dst.numel():
+        raise KernelError("copy_pages: the page ids must be int32, as many to read as to write")
+    if len(src_pools) != len(dst_pools):
+        raise KernelError(f"copy_pages: {len(src_pools)} pools to read, {len(dst_pools)} to write")
+    for a, b in zip(src_pools, dst_pools):
+        _page_run(a)
+        _page_run(b)
+        if a.dtype != b.dtype or a.shape[0] != b.shape[0] or a.shape[2:] != b.shape[2:]:
+            raise KernelError(f"copy_pages: pools of {a.dtype} {tuple(a.shape)} and {b.dtype} {tuple(b.shape)} do not have the same pages")
+        if a.device != src.device or b.device != src.device or dst.device != src.device:
+            raise KernelError("copy_pages: pools and page ids must be on one device")
+    for at in range(0, len(src_pools), _MOST_POOLS):
+        some = list(zip(src_pools[at:at + _MOST_POOLS], dst_pools[at:at + _MOST_POOLS]))
+        n, shapes = len(some), []
+        for a, b in some:
+            size = a.element_size()
+            page = a[0, 0].numel() if a.shape[0] and a.shape[1] else 0
+            shapes += [a.stride(0) * size, b.stride(0) * size, page * size, a.shape[1], b.shape[1], a.shape[0]]
+        check(fn("pb_copy_pages")(n, (ctypes.c_void_p * n)(*[a.data_ptr() for a, _ in some]), (ctypes.c_void_p * n)(*[b.data_ptr() for _, b in some]),
+                                  (ctypes.c_longlong * len(shapes))(*shapes), _p(src), _p(dst), src.numel(), stream()), "copy_pages")
+
+
+MOST_ALTERNATIVES = 32            # one per lane of a warp (csrc/token_scores.cu)
+
+
+def token_scores(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tensor, entropy: torch.Tensor, rank: Optional[torch.Tensor] = None,
+                 top_ids: Optional[torch.Tensor] = None, top_logprob: Optional[torch.Tensor] = None) -> None:
+    """What a row of ``logits`` [R, V] (float32 or bfloat16, rows at any distance) says of the token ``tokens[r]`` (int32):
+    ``logprob[r]`` its log probability, ``rank[r]`` (int32) how many tokens are likelier (of equal ones the lower id is),
+    ``entropy[r]`` of the row in nats, and the n likeliest tokens in order with their log probabilities, ``top_ids`` (int32) and
+    ``top_logprob`` [R, n], n <= 32.  Results are float32.  A logit of -inf is a token that cannot come; a row of nothing else, or with a
+    NaN or +inf, has NaN where the formulas have it.  A token outside the vocabulary (-1 for none) has log probability NaN and rank -1."""
+    _cuda(tokens, logprob, entropy, rank, top_ids, top_logprob)
+    if not logits.is_cuda or logits.dim() != 2 or (logits.numel() and logits.stride(1) != 1):
+        raise KernelError(f"token_scores: logits must be CUDA rows of neighbouring elements, found {tuple(logits.shape)} with strides "
+                          f"{tuple(logits.stride())} on {logits.device}; there is no CPU path")
+    rows, vocab = logits.shape
+    kind = code(logits.dtype)
+    for t, dtype, shape, name in ((tokens, torch.int32, (rows,), "tokens"), (logprob, torch.float32, (rows,), "logprob"),
+                                  (entropy, torch.float32, (rows,), "entropy"), (rank, torch.int32, (rows,), "rank")):
+        if t is not None and (t.dtype != dtype or tuple(t.shape) != shape):
+            raise KernelError(f"token_scores: {name} must be {dtype} {shape}, found {t.dtype} {tuple(t.shape)}")
+    if (top_ids is None) != (top_logprob is None):
+        raise KernelError("token_scores: the alternatives' ids and log probabilities go together")
+    n = 0
+    if top_ids is not None:
+        n = top_ids.shape[-1]
+        if top_ids.dtype != torch.int32 or top_logprob.dtype != torch.float32 or tuple(top_ids.shape) != (rows, n) or top_logprob.shape != top_ids.shape:
+            raise KernelError(f"token_scores: alternatives must be int32 and float32 [{rows}, n], found {tuple(top_ids.shape)} and {tuple(top_logprob.shape)}")
+        if n > MOST_ALTERNATIVES or n > vocab:
+            raise KernelError(f"token_scores: at most {MOST_ALTERNATIVES} alternatives and no more than the vocabulary's {vocab}, found {n}")
+    if rows == 0:
+        return
+    if vocab == 0:
+        raise KernelError("token_scores: an empty vocabulary")
+    check(fn("pb_token_scores")(kind, _p(logits), logits.stride(0) if rows > 1 else vocab, rows, vocab, _p(tokens), _p(logprob), _p(entropy), _p(rank),
+                                _p(top_ids) if n else None, _p(top_logprob) if n else None, n, stream()), "token_scores")
