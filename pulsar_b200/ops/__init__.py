@@ -141,6 +141,7 @@ _SIGNATURES = {
     "pb_matrix_memory": [_I, _P, _L, _P, _P, _F, _P, _F, _F, _F, _P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "pb_state_space": [_I, _P, _L, _P, _P, _I, _P, _P, _P, _P, _I, _F, _P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "pb_copy_pages": [_I, _P, _P, _P, _P, _P, _I, _P],
+    "pb_paged_attention_shared": [_I] + [_P] * 6 + [_I] + [_P] * 4 + [_I] * 8 + [_F, _I, _I, _P],
     "pb_token_scores": [_I, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P],
 }
 _RETURNS = {"pb_recurrence_workspace": _L}        # the others return an int
@@ -155,7 +156,7 @@ _LAUNCHERS = {"embed", "scale_cap", "move_ids", "add_rmsnorm", "rope_table", "qk
               "selective_scan", "selective_scan_prompt", "selective_scan_chunked", "post_norm_add", "clamped_glu",
               "post_norm_add_bias", "glu_bias", "qk_prepare", "qk_prepare_whole", "sigmoid_gate_strided", "add_bias", "moe_route", "moe_gate_up", "moe_up", "moe_down", "moe_grouped",
               "norm_shift", "parallel_add", "activation", "min_gru", "diff_combine", "retention", "scaled_sum", "concat_streams", "normed_sum", "matrix_memory", "state_space",
-              "copy_pages", "token_scores"}
+              "copy_pages", "token_scores", "paged_attention_shared"}
 
 
 class KernelError(RuntimeError):
@@ -1987,3 +1988,66 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tens
         raise KernelError("token_scores: an empty vocabulary")
     check(fn("pb_token_scores")(kind, _p(logits), logits.stride(0) if rows > 1 else vocab, rows, vocab, _p(tokens), _p(logprob), _p(entropy), _p(rank),
                                 _p(top_ids) if n else None, _p(top_logprob) if n else None, n, stream()), "token_scores")
+
+
+def shared_splits(rows: int, n_kv_heads: int, keys: int, tile_rows: int) -> int:
+    """Parts that the keys of one side are cut into: so many that its blocks (row tiles x kv heads x parts) fill the SMs twice, none
+    shorter than 256 keys."""
+    blocks = max(1, -(-rows // tile_rows)) * n_kv_heads
+    return max(1, min(32, keys // 256, _DECODE_SLOTS // blocks))
+
+
+def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, out: torch.Tensor, block_table: torch.Tensor,
+                           kv_len: torch.Tensor, shared_len: torch.Tensor, members: torch.Tensor, family_start: torch.Tensor, most_members: int,
+                           most_shared: int, scale: float, partial: Optional[torch.Tensor] = None) -> None:
+    """Attention of one query token per sequence over a cache in which families of sequences share pages: q, out [S, Hq, D], pools
+    [pages, Hkv, page, D], ``block_table`` [S, width], ``kv_len`` [S].  Family f is the sequences ``members[family_start[f]:family_start[f + 1]]``;
+    they all have the same pages for their first ``shared_len[s]`` keys (whole pages, at most ``kv_len[s]``), which are read once for all
+    of them.  A sequence in no family has ``shared_len`` 0; one with ``kv_len`` 0 gets zeros.  All arrays int32 on the device.
+    ``most_members`` and ``most_shared`` are the largest family's size and the longest shared length as the host knows them (more members
+    than that are not served).  ``partial``: float32 scratch of ``shared_scratch`` elements, made here where it is not given."""
+    _cuda(q, k_pool, v_pool, out, block_table, kv_len, shared_len, members, family_start, partial)
+    _check_against(k_pool)
+    if q.dim() != 3 or k_pool.dim() != 4:
+        raise KernelError(f"paged_attention_shared: q is [S, heads, D] and pools [pages, kv heads, page, D], found {tuple(q.shape)}, {tuple(k_pool.shape)}")
+    s, hq, d = q.shape
+    _, hkv, page_size, d2 = k_pool.shape
+    if d2 != d or v_pool.shape != k_pool.shape or out.shape != q.shape or hkv == 0 or hq % hkv:
+        raise KernelError(f"paged_attention_shared: q {tuple(q.shape)}, out {tuple(out.shape)} and pools {tuple(k_pool.shape)}, {tuple(v_pool.shape)} do not fit")
+    if not (q.dtype == k_pool.dtype == v_pool.dtype == out.dtype):
+        raise KernelError("paged_attention_shared: q, out and the pools must have one dtype")
+    if d % 16 or d > 256:
+        raise KernelError(f"paged_attention_shared: head size {d} must be a multiple of 16, at most 256")
+    for t in (block_table, kv_len, shared_len, members, family_start):
+        if t.dtype != torch.int32:
+            raise KernelError(f"paged_attention_shared: index arrays must be int32, found {t.dtype}")
+    if block_table.dim() != 2 or block_table.shape[0] != s or kv_len.numel() != s or shared_len.numel() != s or family_start.numel() == 0:
+        raise KernelError(f"paged_attention_shared: {s} sequences need a table row, a length and a shared length each, and family_start one more "
+                          "element than there are families")
+    if most_members < 0 or most_shared < 0 or most_members > s:
+        raise KernelError(f"paged_attention_shared: most_members must lie in [0, {s}] and most_shared must not be negative, found {most_members}, {most_shared}")
+    kind = code(q.dtype)
+    if s == 0:
+        return
+    families = family_start.numel() - 1 if most_members > 0 and most_shared > 0 else 0
+    n_shared, n_own = shared_cut(s, families, int(most_members), int(most_shared), block_table.shape[1] * page_size, hq, hkv)
+    need = s * hq * (n_shared + n_own) * (d + 2)
+    if partial is None:
+        partial = torch.empty(need, dtype=torch.float32, device=q.device)
+    elif partial.dtype != torch.float32 or partial.numel() < need:
+        raise KernelError(f"paged_attention_shared: partial must be float32 of at least {need} elements, found {partial.numel()} of {partial.dtype}")
+    check(fn("pb_paged_attention_shared")(kind, _p(q), _p(k_pool), _p(v_pool), _p(out), _p(partial), _p(block_table), block_table.shape[1], _p(kv_len),
+                                          _p(shared_len), _p(members), _p(family_start), s, members.numel(), families, int(most_members), hq, hkv, d,
+                                          page_size, float(scale), n_shared, n_own, stream()), "paged_attention_shared", kernels=2)
+
+
+def shared_cut(n_seqs: int, n_families: int, most_members: int, most_shared: int, table_tokens: int, n_heads: int, n_kv_heads: int) -> Tuple[int, int]:
+    """(parts of the shared keys, parts of the own keys) that ``paged_attention_shared`` works in."""
+    group = n_heads // n_kv_heads
+    n_own = shared_splits(n_seqs * max(1, group), n_kv_heads, max(1, table_tokens - (most_shared if n_families else 0)), max(1, group))
+    return (shared_splits(n_families * most_members * group, n_kv_heads, most_shared, 16) if n_families else 0), n_own
+
+
+def shared_scratch(n_seqs: int, n_families: int, most_members: int, most_shared: int, table_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    """Elements of ``paged_attention_shared``'s scratch."""
+    return n_seqs * n_heads * sum(shared_cut(n_seqs, n_families, most_members, most_shared, table_tokens, n_heads, n_kv_heads)) * (head_dim + 2)
