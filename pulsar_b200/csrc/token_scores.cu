@@ -1,16 +1,12 @@
 // What rows of logits say of given tokens: log probability, rank, the row's entropy and its likeliest tokens.
 //
-// With m the row's maximum, s = sum exp(x - m) and t = sum exp(x - m) (x - m) over the row,
-//     log p(i) = (x_i - m) - log s,      entropy = -sum p log p = log s - t / s   (both terms are >= 0: nothing cancels).
-// All come from one pass: every thread keeps (m, s, t) of what it has seen and, when its maximum rises by delta, carries them over with
-// f = exp(-delta): t <- f (t - s delta), s <- f s.  The rank of the given token is a count of comparisons against its logit.
+// One pass: every thread keeps the maximum and the sums (scores.cuh) of what it has seen.  The rank of the given token is a count of
+// comparisons against its logit.
 // The n likeliest (n <= 32) are kept by each warp as a list with one entry per lane, in order: a key of 64 bits holds the logit's
 // bits, made to compare as unsigned numbers, above the complement of its index, so of equal logits the lower index is larger.  A
 // logit enters only when it is beyond the list's last, which soon is rare.
-//
-// Differences below -1000 count as -1000, where exp is 0 already: a logit of -inf, or of the type's lowest number, then adds 0 to s and
-// to t.  NaN and +inf make s and t NaN, as they do in the formulas; in the order of tokens a NaN is below every number.
-#include "common.cuh"
+// In the order of tokens a NaN is below every number.
+#include "scores.cuh"
 
 namespace {
 
@@ -18,21 +14,6 @@ using namespace pb;
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kFar = -1000.0f;         // exp of it is 0, and times any sum of 32 bits' worth of elements it stays finite
-
-struct Stats {
-    float m, s, t;
-};
-
-// Brings `a` and `b` under the larger of their maxima.  A part without a finite or infinite number has m = -inf, and s = t = 0 (or NaN).
-__device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
-    const float m = fmaxf(a.m, b.m);
-    const float da = a.m == -INFINITY ? 0.0f : fmaxf(a.m - m, kFar), db = b.m == -INFINITY ? 0.0f : fmaxf(b.m - m, kFar);
-    const float fa = exp2f(da * kLog2e), fb = exp2f(db * kLog2e);
-    return Stats{m, a.s * fa + b.s * fb, fa * (a.t + a.s * da) + fb * (b.t + b.s * db)};
-}
-
 typedef unsigned long long Key;
 
 __device__ __forceinline__ Key key_of(float x, int index) {
@@ -72,14 +53,14 @@ token_scores_kernel(const T* __restrict__ logits, long long row_stride, int voca
         if (in) {
             if (x > st.m) {
                 if (st.m > -INFINITY) {
-                    const float delta = fmaxf(st.m - x, kFar), f = exp2f(delta * kLog2e);
+                    const float delta = fmaxf(st.m - x, kFar), f = exp2f(delta * kScoreLog2e);
                     st.t = f * (st.t + st.s * delta);
                     st.s *= f;
                 }
                 st.m = x;
             }
             const float d = x - (st.m == -INFINITY ? 0.0f : st.m);
-            const float e = exp2f(d * kLog2e);
+            const float e = exp2f(d * kScoreLog2e);
             st.s += e;
             st.t += e * fmaxf(d, kFar);
             likelier += (x > given || (x == given && i < token)) ? 1 : 0;

@@ -142,9 +142,13 @@ _SIGNATURES = {
     "pb_state_space": [_I, _P, _L, _P, _P, _I, _P, _P, _P, _P, _I, _F, _P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "pb_copy_pages": [_I, _P, _P, _P, _P, _P, _I, _P],
     "pb_paged_attention_shared": [_I] + [_P] * 6 + [_I] + [_P] * 4 + [_I] * 8 + [_F, _I, _I, _P],
+    "pb_head_scores_supported": [_I, _I, _I],
+    "pb_head_scores_scratch": [_I, _I],
+    "pb_head_scores_wait_limit": [ctypes.c_longlong],
+    "pb_head_scores": [_P] * 5 + [_I, _I, _I, _F, _F, _P, _P, _P],
     "pb_token_scores": [_I, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P],
 }
-_RETURNS = {"pb_recurrence_workspace": _L}        # the others return an int
+_RETURNS = {"pb_recurrence_workspace": _L, "pb_head_scores_scratch": _L}        # the others return an int
 _fns = {}
 # the entry points that launch kernels (the others answer questions on the host): what PULSAR_PROF=1 times
 _LAUNCHERS = {"embed", "scale_cap", "move_ids", "add_rmsnorm", "rope_table", "qk_norm_rope_write", "silu_mul", "gather_words",
@@ -156,7 +160,7 @@ _LAUNCHERS = {"embed", "scale_cap", "move_ids", "add_rmsnorm", "rope_table", "qk
               "selective_scan", "selective_scan_prompt", "selective_scan_chunked", "post_norm_add", "clamped_glu",
               "post_norm_add_bias", "glu_bias", "qk_prepare", "qk_prepare_whole", "sigmoid_gate_strided", "add_bias", "moe_route", "moe_gate_up", "moe_up", "moe_down", "moe_grouped",
               "norm_shift", "parallel_add", "activation", "min_gru", "diff_combine", "retention", "scaled_sum", "concat_streams", "normed_sum", "matrix_memory", "state_space",
-              "copy_pages", "token_scores", "paged_attention_shared"}
+              "copy_pages", "token_scores", "paged_attention_shared", "head_scores"}
 
 
 class KernelError(RuntimeError):
@@ -692,7 +696,8 @@ def set_wait_limit(cycles: int) -> None:
         raise ValueError("the wait limit must be positive")
     if fn("pb_gemm_tcgen05_wait_control")(int(cycles), -1, None) != 0 or \
             fn("pb_prefill_tcgen05_wait_control")(int(cycles), -1, None) != 0 or \
-            fn("pb_gemm_tcgen05_stream_wait_control")(int(cycles), -1, None) != 0:
+            fn("pb_gemm_tcgen05_stream_wait_control")(int(cycles), -1, None) != 0 or \
+            fn("pb_head_scores_wait_limit")(int(cycles)) != 0:
         raise KernelError("the wait limit could not be set")
 
 
@@ -2051,3 +2056,44 @@ def shared_cut(n_seqs: int, n_families: int, most_members: int, most_shared: int
 def shared_scratch(n_seqs: int, n_families: int, most_members: int, most_shared: int, table_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int) -> int:
     """Elements of ``paged_attention_shared``'s scratch."""
     return n_seqs * n_heads * sum(shared_cut(n_seqs, n_families, most_members, most_shared, table_tokens, n_heads, n_kv_heads)) * (head_dim + 2)
+
+
+_LOGITS_AT_ONCE = 1 << 26         # elements of float32 logits that ``head_scores`` keeps where it cannot do without them
+
+
+def head_scores(h: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tensor, entropy: torch.Tensor, scale: float = 1.0,
+                cap: Optional[float] = None) -> None:
+    """``token_scores`` of the logits x = scale * (h @ w.T), capped as cap * tanh(x / cap) where a cap is given, that never have to
+    exist: ``logprob[r]`` of ``tokens[r]`` and ``entropy[r]``, float32.  ``h`` [R, K] hidden rows behind the final norm, ``w`` [V, K] the
+    head's weight, both bfloat16 or both float32, ``tokens`` int32 [R] (outside the vocabulary: log probability NaN).
+
+    bfloat16 takes the fused tcgen05 kernel (a wait that it gives up is reported in the tcgen05 product's error word).  float32, and
+    rows that are no multiple of 16 bytes, take the CUDA-core product and ``token_scores`` over as many rows at a time as 256 MiB
+    of logits hold."""
+    _cuda(h, w, tokens, logprob, entropy)
+    if h.dim() != 2 or w.dim() != 2 or h.shape[1] != w.shape[1] or h.dtype != w.dtype:
+        raise KernelError(f"head_scores: h [R, K] and w [V, K] of one dtype, found {h.dtype} {tuple(h.shape)} and {w.dtype} {tuple(w.shape)}")
+    code(h.dtype)
+    (rows, k), vocab = h.shape, w.shape[0]
+    for t, dtype, name in ((tokens, torch.int32, "tokens"), (logprob, torch.float32, "logprob"), (entropy, torch.float32, "entropy")):
+        if t.dtype != dtype or tuple(t.shape) != (rows,):
+            raise KernelError(f"head_scores: {name} must be {dtype} ({rows},), found {t.dtype} {tuple(t.shape)}")
+    if cap is not None and not cap > 0.0:
+        raise KernelError(f"head_scores: the cap on the logits must be positive, found {cap}")
+    if vocab == 0 or k == 0:
+        raise KernelError("head_scores: an empty vocabulary or hidden rows without elements")
+    if rows == 0:
+        return
+    if h.dtype == torch.bfloat16 and (h.data_ptr() | w.data_ptr()) % 16 == 0 and fn("pb_head_scores_supported")(rows, vocab, k):
+        scratch = torch.empty(int(fn("pb_head_scores_scratch")(rows, vocab)), dtype=torch.float32, device=h.device)
+        check(fn("pb_head_scores")(_p(h), _p(w), _p(tokens), _p(logprob), _p(entropy), rows, vocab, k, float(scale), float(cap or 0.0), _p(scratch),
+                                   wait_word_addresses()[0], stream()), "head_scores", kernels=2)
+        return
+    some = max(1, min(rows, _LOGITS_AT_ONCE // vocab))
+    logits = torch.empty((some, vocab), dtype=torch.float32, device=h.device)
+    for at in range(0, rows, some):
+        n = min(some, rows - at)
+        gemm_simt(h[at:at + n], w, logits[:n])
+        if scale != 1.0 or cap is not None:
+            scale_cap(logits[:n], scale, cap)
+        token_scores(logits[:n], tokens[at:at + n], logprob[at:at + n], entropy[at:at + n])
