@@ -1,19 +1,34 @@
 // What rows of logits say of given tokens: log probability, rank, the row's entropy and its likeliest tokens.
 //
-// One pass: every thread keeps the maximum and the sums (scores.cuh) of what it has seen.  The rank of the given token is a count of
-// comparisons against its logit.
-// The n likeliest (n <= 32) are kept by each warp as a list with one entry per lane, in order: a key of 64 bits holds the logit's
-// bits, made to compare as unsigned numbers, above the complement of its index, so of equal logits the lower index is larger.  A
-// logit enters only when it is beyond the list's last, which soon is rare.
-// In the order of tokens a NaN is below every number.
+// One pass over the row: every thread keeps the maximum and the sums (scores.cuh) of what it has seen, and counts the logits beyond the
+// given token's.  Bound by the bytes of the logits where there are rows enough, by latency where there are few: a row is cut among the
+// blocks of a cluster (up to eight), whose results meet in the first block's hands through distributed shared memory, so there is one
+// launch, no scratch memory and no order of atomics that a result could depend on.
+//
+// The n likeliest (n <= 32) cost the pass nothing but the number of the chunk in which a thread's maximum rose last.  A key of 64 bits
+// holds a logit's bits, made to compare as unsigned numbers, above the complement of its index: of equal logits the lower index is the larger
+// key, and no two keys are equal.  The n-th largest of the threads' (or pairs of threads') largest keys is reached by n keys at least, so
+// no key below it is among the n likeliest, and only the few threads whose largest reaches it can hold any that are: their elements are read
+// once more (2 to 15 % of the row, from L2), what reaches the threshold is ranked by counting.  Should more than kMostCandidates reach it (a
+// row made so that few threads hold all its large logits), the likeliest are found one by one.  In the order of tokens a NaN is below
+// every number; a thread that met one is always read again.
 #include "scores.cuh"
+
+#include <cooperative_groups.h>
+
+namespace cg = cooperative_groups;
 
 namespace {
 
 using namespace pb;
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+constexpr int kMostThreads = 512;
+constexpr int kMostWarps = kMostThreads / 32;
+constexpr int kGroups = 256;                 // threads, or pairs of them, whose largest keys are compared
+constexpr int kMostCandidates = 1024;
+constexpr int kMostCluster = 8;              // the portable limit
+constexpr int kMostTop = 32;
+
 typedef unsigned long long Key;
 
 __device__ __forceinline__ Key key_of(float x, int index) {
@@ -22,95 +37,313 @@ __device__ __forceinline__ Key key_of(float x, int index) {
     return ((Key)up << 32) | (uint32_t)~(uint32_t)index;
 }
 __device__ __forceinline__ int index_of(Key k) { return (int)~(uint32_t)k; }
-
-// Puts the warp's candidate (the same in all lanes, beyond the list's last) in its place.
-__device__ __forceinline__ void insert(Key& list, Key candidate, int lane) {
-    const int place = __popc(__ballot_sync(0xffffffffu, list > candidate));
-    const Key above = __shfl_up_sync(0xffffffffu, list, 1);
-    if (lane >= place) list = lane == place ? candidate : above;
+__device__ __forceinline__ float logit_of(Key k) {
+    const uint32_t up = (uint32_t)(k >> 32);
+    return up == 0 ? nanf("") : __uint_as_float((up >> 31) ? up ^ 0x80000000u : ~up);
 }
 
+// 16 bytes of a row as float32.
+template <typename T> constexpr int kPerVector = 16 / (int)sizeof(T);
+__device__ __forceinline__ void widen(const uint4& u, const float*, float* x) {
+    x[0] = __uint_as_float(u.x); x[1] = __uint_as_float(u.y); x[2] = __uint_as_float(u.z); x[3] = __uint_as_float(u.w);
+}
+__device__ __forceinline__ void widen(const uint4& u, const __nv_bfloat16*, float* x) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+__device__ __forceinline__ uint4 load_once(const uint4* p) {                  // (a row is read once: it need not stay in L1)
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+struct Scores {
+    const void* logits;
+    long long row_stride;
+    const int* tokens;
+    float *logprob, *entropy, *top_logprob;
+    int *rank, *top_ids;
+    int vocab, n_top;
+};
+
+// What a block hands to the first of its cluster.
+struct Result {
+    Stats st;
+    int likelier;
+    Key keys[kMostTop];
+};
+
+// The row as 16-byte vectors, with the elements in front of the first whole one and behind the last; this block's are [begin, end).
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-token_scores_kernel(const T* __restrict__ logits, long long row_stride, int vocab, const int* __restrict__ tokens, float* __restrict__ logprob,
-                    float* __restrict__ entropy, int* __restrict__ rank, int* __restrict__ top_ids, float* __restrict__ top_logprob, int n_top) {
-    __shared__ Stats stats_s[kWarps];
-    __shared__ int count_s[kWarps];
-    __shared__ Key keys_s[kWarps * 32];
-    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const T* row = logits + (long long)r * row_stride;
-    const int token = tokens[r];
-    const bool known = token >= 0 && token < vocab;
-    const float given = known ? to_float(row[token]) : 0.0f;
+struct Slice {
+    const T* row;
+    const uint4* vectors;
+    int before, behind, first_behind;        // odd elements: [0, before) and [first_behind, first_behind + behind)
+    int begin, end;
+    bool odd;                                // whether the odd elements are this block's
+
+    __device__ __forceinline__ Slice(const Scores& p, long long r, int block, int blocks) {
+        constexpr int N = kPerVector<T>;
+        row = static_cast<const T*>(p.logits) + r * p.row_stride;
+        before = min(p.vocab, (int)(((16 - ((uintptr_t)row & 15)) & 15) / sizeof(T)));
+        const int n = (p.vocab - before) / N;
+        vectors = reinterpret_cast<const uint4*>(row + before);
+        first_behind = before + n * N;
+        behind = p.vocab - first_behind;
+        const int each = ((n + blocks - 1) / blocks + 31) & ~31;
+        begin = min(n, block * each);
+        end = min(n, begin + each);
+        odd = block == 0;
+    }
+    // the index of a vector's first element
+    __device__ __forceinline__ int index(int vector) const { return before + vector * kPerVector<T>; }
+    // the lane's odd element, or -1
+    __device__ __forceinline__ int odd_index(int lane) const {
+        if (!odd) return -1;
+        return lane < before ? lane : lane - before < behind ? first_behind + lane - before : -1;
+    }
+};
+
+template <typename T, bool RANK>
+__global__ void __launch_bounds__(kMostThreads)
+token_scores_kernel(const Scores p) {
+    constexpr int N = kPerVector<T>, V = 16 / N, E = N * V;                   // elements of a vector, vectors and elements of a thread's chunk
+    __shared__ Result result;
+    __shared__ Stats stats_s[kMostWarps];
+    __shared__ int count_s[kMostWarps];
+    __shared__ __align__(16) Key keys_s[kMostCandidates];                                  // the groups' largest, then the candidates
+    __shared__ unsigned short hot_s[kGroups];
+    __shared__ Key threshold_s, best_s[kMostWarps];
+    __shared__ int n_hot_s, n_candidates_s;
+
+    cg::cluster_group cluster = cg::this_cluster();
+    const int blocks = cluster.num_blocks(), block = cluster.block_rank();
+    const long long r = blockIdx.x / blocks;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    const Slice<T> slice(p, r, block, blocks);
+    const int step = warps * 32 * V;                                          // vectors of a turn of the whole block
+    const int my_first = slice.begin + warp * 32 * V + lane;                  // + turn * step + j * 32
+
+    uint4 next[V];
+    auto fetch = [&](int first) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (first + j * 32 < slice.end) next[j] = load_once(slice.vectors + first + j * 32);
+    };
+    fetch(my_first);
+    const int token = p.tokens[r];
+    const bool known = token >= 0 && token < p.vocab;
+    const float given = known ? to_float(slice.row[token]) : 0.0f;
 
     Stats st = {-INFINITY, 0.0f, 0.0f};
-    int likelier = 0;
-    Key list = 0, last = 0;
-    for (int base = warp * 32; base < vocab; base += kThreads) {
-        const int i = base + lane;
-        const bool in = i < vocab;
-        const float x = in ? to_float(row[i]) : -INFINITY;
-        if (in) {
-            if (x > st.m) {
-                if (st.m > -INFINITY) {
-                    const float delta = fmaxf(st.m - x, kFar), f = exp2f(delta * kScoreLog2e);
-                    st.t = f * (st.t + st.s * delta);
-                    st.s *= f;
-                }
-                st.m = x;
+    int likelier = 0, risen = my_first;
+    for (int first = my_first; first - lane < slice.end; first += step) {
+        float x[E];
+        const bool whole = first - lane + 32 * V <= slice.end;                // the warp's chunk ends inside the slice
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            widen(next[j], slice.row, x + j * N);
+            if (!whole && first + j * 32 >= slice.end) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) x[j * N + i] = -INFINITY;
             }
-            const float d = x - (st.m == -INFINITY ? 0.0f : st.m);
-            const float e = exp2f(d * kScoreLog2e);
-            st.s += e;
-            st.t += e * fmaxf(d, kFar);
-            likelier += (x > given || (x == given && i < token)) ? 1 : 0;
         }
-        if (n_top > 0) {
-            const Key key = in ? key_of(x, i) : 0;
-            unsigned beyond = __ballot_sync(0xffffffffu, key > last);
-            while (beyond) {
-                const Key candidate = __shfl_sync(0xffffffffu, key, __ffs(beyond) - 1);
-                insert(list, candidate, lane);
-                last = __shfl_sync(0xffffffffu, list, n_top - 1);
-                beyond &= beyond - 1;
-                beyond &= __ballot_sync(0xffffffffu, key > last);
+        fetch(first + step);
+        const float before = st.m;
+        add_logits(st, x);
+        if (st.m > before) risen = first;
+        if (RANK) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int index = slice.index(first + j * 32);
+                if (!whole && first + j * 32 >= slice.end) continue;
+                if (token >= index + N) {                                     // equal logits count in front of the given token only
+#pragma unroll
+                    for (int i = 0; i < N; ++i) likelier += x[j * N + i] >= given ? 1 : 0;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) likelier += x[j * N + i] > given || (x[j * N + i] == given && index + i < token) ? 1 : 0;
+                }
             }
+        }
+    }
+    const bool met_nan = st.s != st.s;
+    if (warp == 0) {
+        const int i = slice.odd_index(lane);
+        if (i >= 0) {
+            const float x[1] = {to_float(slice.row[i])};
+            Stats one = {-INFINITY, 0.0f, 0.0f};
+            add_logits(one, x);
+            st = join(st, one);
+            if (RANK) likelier += x[0] > given || (x[0] == given && i < token) ? 1 : 0;
         }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const Stats other = {__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.t, o)};
         st = join(st, other);
-        likelier += __shfl_xor_sync(0xffffffffu, likelier, o);
+        if (RANK) likelier += __shfl_xor_sync(0xffffffffu, likelier, o);
     }
     if (lane == 0) { stats_s[warp] = st; count_s[warp] = likelier; }
-    if (n_top > 0) keys_s[warp * 32 + lane] = lane < n_top ? list : 0;
-    __syncthreads();
-    st = stats_s[0];
-    likelier = count_s[0];
-    for (int w = 1; w < kWarps; ++w) {
-        st = join(st, stats_s[w]);
-        likelier += count_s[w];
-    }
-    const float log_s = logf(st.s);
-    if (tid == 0) {
-        logprob[r] = known ? (given - st.m) - log_s : nanf("");
-        entropy[r] = log_s - st.t / st.s;
-        if (rank != nullptr) rank[r] = known ? likelier : -1;
-    }
-    // a key's place among all warps' lists is the number of larger ones (no two are equal but the empty ones, which are smallest)
-    for (int i = tid; i < kWarps * n_top; i += kThreads) {
-        const Key key = keys_s[i / n_top * 32 + i % n_top];
-        if (key == 0) continue;
-        int place = 0;
-        for (int w = 0; w < kWarps; ++w)
-            for (int j = 0; j < n_top && keys_s[w * 32 + j] > key; ++j) ++place;
-        if (place < n_top) {
-            const int index = index_of(key);
-            top_ids[(long long)r * n_top + place] = index;
-            top_logprob[(long long)r * n_top + place] = (to_float(row[index]) - st.m) - log_s;
+
+    if (p.n_top > 0) {
+        // the groups' largest keys
+        Key key = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int vector = risen + j * 32;
+            if (vector < slice.end) {
+                float x[N];
+                widen(slice.vectors[vector], slice.row, x);
+#pragma unroll
+                for (int i = 0; i < N; ++i) key = max(key, key_of(x[i], slice.index(vector) + i));
+            }
+        }
+        bool again = met_nan;
+        int group = tid;
+        const bool pairs = blockDim.x > kGroups;
+        if (pairs) {
+            key = max(key, __shfl_xor_sync(0xffffffffu, key, 1));
+            const int other_again = __shfl_xor_sync(0xffffffffu, (int)again, 1);       // (every lane takes part, whatever its own is)
+            again = again || other_again;
+            group = tid >> 1;
+        }
+        const bool speaks = !pairs || !(tid & 1);
+        if (tid == 0) { threshold_s = 0; n_hot_s = 0; n_candidates_s = 0; }
+        if (tid < kMostTop) result.keys[tid] = 0;
+        if (speaks) keys_s[group] = key;
+        __syncthreads();
+        const int groups = pairs ? blockDim.x >> 1 : blockDim.x;
+        if (tid < groups) {
+            const Key mine = keys_s[tid];
+            int larger = 0;
+            for (int g = 0; g < groups; g += 2) {
+                const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(keys_s + g);
+                larger += (two.x > mine ? 1 : 0) + (two.y > mine ? 1 : 0);
+            }
+            if (mine != 0 && larger == p.n_top - 1) threshold_s = mine;
+        }
+        __syncthreads();
+        const Key threshold = threshold_s;                                    // 0: fewer groups have elements than are asked for
+        if (speaks && ((key != 0 && key >= threshold) || again)) hot_s[atomicAdd(&n_hot_s, 1)] = (unsigned short)group;
+        __syncthreads();
+        const int turns = (slice.end - slice.begin + step - 1) / step, per_group = pairs ? 2 : 1;
+        auto candidate = [&](Key k) {
+            if (k >= threshold) {
+                const int at = atomicAdd(&n_candidates_s, 1);                 // (ranked below: their order here does not matter)
+                if (at < kMostCandidates) keys_s[at] = k;
+            }
+        };
+        for (int h = warp; h < n_hot_s; h += warps) {
+            for (int q = lane; q < turns * V * per_group; q += 32) {
+                const int owner = hot_s[h] * per_group + q % per_group, chunk = q / per_group;
+                const int vector = slice.begin + (owner >> 5) * 32 * V + (owner & 31) + chunk / V * step + chunk % V * 32;
+                if (vector < slice.end) {
+                    float x[N];
+                    widen(slice.vectors[vector], slice.row, x);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) candidate(key_of(x[i], slice.index(vector) + i));
+                }
+            }
+        }
+        if (warp == 0) {
+            const int i = slice.odd_index(lane);
+            if (i >= 0) candidate(key_of(to_float(slice.row[i]), i));
+        }
+        __syncthreads();
+        const int n = n_candidates_s;
+        if (n <= kMostCandidates) {
+            for (int i = tid; i < n; i += blockDim.x) {
+                const Key mine = keys_s[i];
+                int larger = 0;
+                for (int g = 0; g < n; ++g) larger += keys_s[g] > mine ? 1 : 0;
+                if (larger < p.n_top) result.keys[larger] = mine;
+            }
+        } else {
+            Key below = ~(Key)0;
+            for (int i = 0; i < p.n_top && below != 0; ++i) {
+                Key best = 0;
+                for (int vector = slice.begin + tid; vector < slice.end; vector += blockDim.x) {
+                    float x[N];
+                    widen(slice.vectors[vector], slice.row, x);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        const Key k = key_of(x[e], slice.index(vector) + e);
+                        if (k < below) best = max(best, k);
+                    }
+                }
+                if (warp == 0 && slice.odd_index(lane) >= 0) {
+                    const Key k = key_of(to_float(slice.row[slice.odd_index(lane)]), slice.odd_index(lane));
+                    if (k < below) best = max(best, k);
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+                __syncthreads();
+                if (lane == 0) best_s[warp] = best;
+                __syncthreads();
+                below = 0;
+                for (int w = 0; w < warps; ++w) below = max(below, best_s[w]);
+                if (tid == 0) result.keys[i] = below;
+            }
         }
     }
+    __syncthreads();
+    if (tid == 0) {
+        st = stats_s[0];
+        likelier = count_s[0];
+        for (int w = 1; w < warps; ++w) {
+            st = join(st, stats_s[w]);
+            likelier += count_s[w];
+        }
+        result.st = st;
+        result.likelier = likelier;
+    }
+    if (blocks > 1) cluster.sync();
+    else __syncthreads();
+    if (block == 0) {
+        for (int i = tid; i < blocks * p.n_top; i += blockDim.x) keys_s[i] = cluster.map_shared_rank(&result, i / p.n_top)->keys[i % p.n_top];
+        st = result.st;
+        likelier = result.likelier;
+        for (int b = 1; b < blocks; ++b) {
+            const Result* other = cluster.map_shared_rank(&result, b);
+            st = join(st, other->st);
+            likelier += other->likelier;
+        }
+        __syncthreads();
+        const float log_s = logf(st.s);
+        if (tid == 0) {
+            p.logprob[r] = known ? (given - st.m) - log_s : nanf("");
+            p.entropy[r] = log_s - st.t / st.s;
+            if (RANK) p.rank[r] = known ? likelier : -1;
+        }
+        for (int i = tid; i < blocks * p.n_top; i += blockDim.x) {
+            const Key mine = keys_s[i];
+            int larger = 0;
+            for (int g = 0; g < blocks * p.n_top; ++g) larger += keys_s[g] > mine ? 1 : 0;
+            if (mine != 0 && larger < p.n_top) {
+                p.top_ids[r * p.n_top + larger] = index_of(mine);
+                p.top_logprob[r * p.n_top + larger] = (logit_of(mine) - st.m) - log_s;
+            }
+        }
+    }
+    if (blocks > 1) cluster.sync();                                           // no block leaves while the first still reads its result
+}
+
+template <typename T, bool RANK>
+int launch(const Scores& p, int rows, int threads, int cluster, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)rows * cluster);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, token_scores_kernel<T, RANK>, p);
 }
 
 }  // namespace
@@ -120,15 +353,17 @@ token_scores_kernel(const T* __restrict__ logits, long long row_stride, int voca
 PB_EXPORT int pb_token_scores(int dtype, const void* logits, long row_stride, int rows, int vocab, const int* tokens, float* logprob, float* entropy,
                               int* rank, int* top_ids, float* top_logprob, int n_top, cudaStream_t stream) {
     if (rows <= 0) return 0;
-    if (vocab <= 0 || n_top < 0 || n_top > 32 || n_top > vocab || row_stride < 0) return PB_ERR_BAD_SIZE;
+    if (dtype != PB_F32 && dtype != PB_BF16) return PB_ERR_BAD_DTYPE;
+    if (vocab <= 0 || n_top < 0 || n_top > kMostTop || n_top > vocab || row_stride < 0) return PB_ERR_BAD_SIZE;
     if (n_top > 0 && (top_ids == nullptr || top_logprob == nullptr)) return PB_ERR_BAD_SIZE;
+    const Scores p = {logits, row_stride, tokens, logprob, entropy, top_logprob, rank, top_ids, vocab, n_top};
+    // Blocks for four of 256 threads on each SM, none with less than 4,096 logits; where even eight a row are few, of 512 threads.
+    int cluster = 1;
+    while (cluster < kMostCluster && (long long)rows * cluster * 2 <= 4 * 148 && vocab / (cluster * 2) >= 4096) cluster *= 2;
+    if ((long long)rows * cluster > 0x7fffffff) return PB_ERR_TOO_LARGE;
+    const int threads = (long long)rows * cluster <= 148 ? 512 : 256;
     if (dtype == PB_F32)
-        token_scores_kernel<float><<<rows, kThreads, 0, stream>>>((const float*)logits, row_stride, vocab, tokens, logprob, entropy, rank, top_ids,
-                                                                  top_logprob, n_top);
-    else if (dtype == PB_BF16)
-        token_scores_kernel<__nv_bfloat16><<<rows, kThreads, 0, stream>>>((const __nv_bfloat16*)logits, row_stride, vocab, tokens, logprob, entropy,
-                                                                          rank, top_ids, top_logprob, n_top);
-    else
-        return PB_ERR_BAD_DTYPE;
-    return launch_status();
+        return rank != nullptr ? launch<float, true>(p, rows, threads, cluster, stream) : launch<float, false>(p, rows, threads, cluster, stream);
+    return rank != nullptr ? launch<__nv_bfloat16, true>(p, rows, threads, cluster, stream)
+                           : launch<__nv_bfloat16, false>(p, rows, threads, cluster, stream);
 }

@@ -210,6 +210,35 @@ def test_offsets_beyond_32_bits():
 
 
 @cuda
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 30, 800])
+@pytest.mark.parametrize("run_of", [1, 4, 8, 16, 512, 2048, 4096])
+def test_large_logits_lie_close_together(dtype, rows, run_of):
+    """Runs of large logits, so many apart from each other as a thread's or a block's elements may be: the likeliest lie with few threads."""
+    vocab = 60000
+    g = torch.Generator().manual_seed(run_of)
+    logits = (torch.randn(rows, vocab, generator=g) * 0.5).to(dtype)
+    at = torch.arange(vocab)
+    logits[:, at % (run_of * 37) < run_of] += 20.0
+    logits[::2, at % (run_of * 64) < max(1, run_of // 4)] = 40.0
+    tokens = torch.randint(0, vocab, (rows,), generator=g).to(torch.int32).cuda()
+    check(logits.cuda(), tokens, 32)
+
+
+@cuda
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [8192, 16389, 33001, 151937])
+def test_the_rank_of_forbidden_tokens(dtype, vocab):
+    """The given token is one of many of logit -inf, at the places where a row is cut among blocks and around them."""
+    cuts = sorted({min(vocab - 1, max(0, round(vocab * i / 8) + d)) for i in range(9) for d in (-130, -9, -8, -4, -1, 0, 1, 3, 7, 120)})
+    logits = torch.full((1, vocab), -math.inf, dtype=dtype)
+    logits[0, 5:vocab:1000] = 1.0
+    tokens = torch.tensor(cuts, dtype=torch.int32).cuda()
+    for some in (tokens[i:i + 1] for i in range(len(cuts))):
+        check(logits.cuda(), some, 2)
+
+
+@cuda
 def test_refusals():
     logits, tokens = logits_of(4, 100, torch.float32, 11)
     lp, en = torch.empty(4, device="cuda"), torch.empty(4, device="cuda")
