@@ -19,12 +19,29 @@ struct Stats {
     float m, s, t;
 };
 
+// 2^x by the special-function unit alone: 2 ulp like exp2f, results below 2^-126 are 0 (beside a sum that holds exp(0) = 1).
+__device__ __forceinline__ float pow2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Brings `a` and `b` under the larger of their maxima.  A part without a number has m = -inf, and s = t = 0 (or NaN).
 __device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
     const float m = fmaxf(a.m, b.m);
     const float da = a.m == -INFINITY ? 0.0f : fmaxf(a.m - m, kFar), db = b.m == -INFINITY ? 0.0f : fmaxf(b.m - m, kFar);
-    const float fa = exp2f(da * kScoreLog2e), fb = exp2f(db * kScoreLog2e);
+    const float fa = pow2(da * kScoreLog2e), fb = pow2(db * kScoreLog2e);
     return Stats{m, a.s * fa + b.s * fb, fa * (a.t + a.s * da) + fb * (b.t + b.s * db)};
+}
+
+// The lanes' sums as one, the same in all lanes.
+__device__ __forceinline__ Stats warp_join(Stats st) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const Stats other = {__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.t, o)};
+        st = join(st, other);
+    }
+    return st;
 }
 
 // Adds N logits.  Four sums of each kind are kept apart, so that additions do not wait for one another.
@@ -35,7 +52,7 @@ __device__ __forceinline__ void add_logits(Stats& st, const float (&x)[N]) {
     for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
     if (top > st.m) {
         if (st.m > -INFINITY) {
-            const float delta = fmaxf(st.m - top, kFar), f = exp2f(delta * kScoreLog2e);
+            const float delta = fmaxf(st.m - top, kFar), f = pow2(delta * kScoreLog2e);
             st.t = f * (st.t + st.s * delta);
             st.s *= f;
         }
@@ -46,7 +63,7 @@ __device__ __forceinline__ void add_logits(Stats& st, const float (&x)[N]) {
     float s[kApart] = {}, t[kApart] = {};
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const float d = x[i] - base, e = exp2f(d * kScoreLog2e);
+        const float d = x[i] - base, e = pow2(d * kScoreLog2e);
         s[i % kApart] += e;
         t[i % kApart] = fmaf(e, fmaxf(d, kFar), t[i % kApart]);
     }

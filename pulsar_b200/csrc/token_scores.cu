@@ -24,7 +24,7 @@ using namespace pb;
 
 constexpr int kMostThreads = 512;
 constexpr int kMostWarps = kMostThreads / 32;
-constexpr int kGroups = 256;                 // threads, or pairs of them, whose largest keys are compared
+constexpr int kGroups = 128;                 // pairs of threads, or quads of a block of 512, whose largest keys are compared
 constexpr int kMostCandidates = 1024;
 constexpr int kMostCluster = 8;              // the portable limit
 constexpr int kMostTop = 32;
@@ -169,56 +169,52 @@ token_scores_kernel(const Scores p) {
         }
     }
     const bool met_nan = st.s != st.s;
+    Stats odd = {-INFINITY, 0.0f, 0.0f};
     if (warp == 0) {
         const int i = slice.odd_index(lane);
         if (i >= 0) {
             const float x[1] = {to_float(slice.row[i])};
-            Stats one = {-INFINITY, 0.0f, 0.0f};
-            add_logits(one, x);
-            st = join(st, one);
+            add_logits(odd, x);
             if (RANK) likelier += x[0] > given || (x[0] == given && i < token) ? 1 : 0;
         }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const Stats other = {__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.t, o)};
-        st = join(st, other);
-        if (RANK) likelier += __shfl_xor_sync(0xffffffffu, likelier, o);
-    }
+    const float highest = st.m;                                               // of this thread's chunks
+    st = warp_join(warp == 0 ? join(st, odd) : st);
+    if (RANK) likelier = __reduce_add_sync(0xffffffffu, likelier);
     if (lane == 0) { stats_s[warp] = st; count_s[warp] = likelier; }
 
     if (p.n_top > 0) {
-        // the groups' largest keys
+        // the groups' largest keys: a thread's is its highest logit's first place in the chunk where the maximum rose last
         Key key = 0;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
+        for (int j = V - 1; j >= 0; --j) {
             const int vector = risen + j * 32;
             if (vector < slice.end) {
                 float x[N];
                 widen(slice.vectors[vector], slice.row, x);
 #pragma unroll
-                for (int i = 0; i < N; ++i) key = max(key, key_of(x[i], slice.index(vector) + i));
+                for (int i = N - 1; i >= 0; --i)
+                    if (x[i] == highest) key = (Key)(slice.index(vector) + i + 1);
             }
         }
-        bool again = met_nan;
-        int group = tid;
-        const bool pairs = blockDim.x > kGroups;
-        if (pairs) {
-            key = max(key, __shfl_xor_sync(0xffffffffu, key, 1));
-            const int other_again = __shfl_xor_sync(0xffffffffu, (int)again, 1);       // (every lane takes part, whatever its own is)
-            again = again || other_again;
-            group = tid >> 1;
+        if (key != 0) key = key_of(highest, (int)key - 1);
+        int again = met_nan;
+        const int per_group = blockDim.x / kGroups;                           // 2 or 4
+        for (int o = 1; o < per_group; o <<= 1) {
+            key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+            again |= __shfl_xor_sync(0xffffffffu, again, o);
         }
-        const bool speaks = !pairs || !(tid & 1);
+        const bool speaks = tid % per_group == 0;
+        const int group = tid / per_group;
         if (tid == 0) { threshold_s = 0; n_hot_s = 0; n_candidates_s = 0; }
         if (tid < kMostTop) result.keys[tid] = 0;
         if (speaks) keys_s[group] = key;
         __syncthreads();
-        const int groups = pairs ? blockDim.x >> 1 : blockDim.x;
-        if (tid < groups) {
+        if (tid < kGroups) {
             const Key mine = keys_s[tid];
             int larger = 0;
-            for (int g = 0; g < groups; g += 2) {
+#pragma unroll 4
+            for (int g = 0; g < kGroups; g += 2) {
                 const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(keys_s + g);
                 larger += (two.x > mine ? 1 : 0) + (two.y > mine ? 1 : 0);
             }
@@ -228,8 +224,11 @@ token_scores_kernel(const Scores p) {
         const Key threshold = threshold_s;                                    // 0: fewer groups have elements than are asked for
         if (speaks && ((key != 0 && key >= threshold) || again)) hot_s[atomicAdd(&n_hot_s, 1)] = (unsigned short)group;
         __syncthreads();
-        const int turns = (slice.end - slice.begin + step - 1) / step, per_group = pairs ? 2 : 1;
-        auto candidate = [&](Key k) {
+        const int turns = (slice.end - slice.begin + step - 1) / step;
+        const float threshold_logit = logit_of(threshold);                    // (NaN where there is no threshold: then no logit is below it)
+        auto candidate = [&](float x, int index) {
+            if (x < threshold_logit) return;
+            const Key k = key_of(x, index);
             if (k >= threshold) {
                 const int at = atomicAdd(&n_candidates_s, 1);                 // (ranked below: their order here does not matter)
                 if (at < kMostCandidates) keys_s[at] = k;
@@ -243,13 +242,13 @@ token_scores_kernel(const Scores p) {
                     float x[N];
                     widen(slice.vectors[vector], slice.row, x);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) candidate(key_of(x[i], slice.index(vector) + i));
+                    for (int i = 0; i < N; ++i) candidate(x[i], slice.index(vector) + i);
                 }
             }
         }
         if (warp == 0) {
             const int i = slice.odd_index(lane);
-            if (i >= 0) candidate(key_of(to_float(slice.row[i]), i));
+            if (i >= 0) candidate(to_float(slice.row[i]), i);
         }
         __syncthreads();
         const int n = n_candidates_s;
@@ -289,27 +288,17 @@ token_scores_kernel(const Scores p) {
         }
     }
     __syncthreads();
-    if (tid == 0) {
-        st = stats_s[0];
-        likelier = count_s[0];
-        for (int w = 1; w < warps; ++w) {
-            st = join(st, stats_s[w]);
-            likelier += count_s[w];
-        }
-        result.st = st;
-        result.likelier = likelier;
+    if (warp == 0) {
+        st = warp_join(lane < warps ? stats_s[lane] : Stats{-INFINITY, 0.0f, 0.0f});
+        likelier = __reduce_add_sync(0xffffffffu, lane < warps ? count_s[lane] : 0);
+        if (lane == 0) { result.st = st; result.likelier = likelier; }
     }
     if (blocks > 1) cluster.sync();
     else __syncthreads();
     if (block == 0) {
         for (int i = tid; i < blocks * p.n_top; i += blockDim.x) keys_s[i] = cluster.map_shared_rank(&result, i / p.n_top)->keys[i % p.n_top];
-        st = result.st;
-        likelier = result.likelier;
-        for (int b = 1; b < blocks; ++b) {
-            const Result* other = cluster.map_shared_rank(&result, b);
-            st = join(st, other->st);
-            likelier += other->likelier;
-        }
+        st = warp_join(lane < blocks ? cluster.map_shared_rank(&result, lane)->st : Stats{-INFINITY, 0.0f, 0.0f});
+        likelier = __reduce_add_sync(0xffffffffu, lane < blocks ? cluster.map_shared_rank(&result, lane)->likelier : 0);
         __syncthreads();
         const float log_s = logf(st.s);
         if (tid == 0) {
@@ -320,7 +309,8 @@ token_scores_kernel(const Scores p) {
         for (int i = tid; i < blocks * p.n_top; i += blockDim.x) {
             const Key mine = keys_s[i];
             int larger = 0;
-            for (int g = 0; g < blocks * p.n_top; ++g) larger += keys_s[g] > mine ? 1 : 0;
+            for (int b = 0; b < blocks && larger < p.n_top; ++b)              // (every block's keys are in order)
+                for (int j = 0; j < p.n_top && keys_s[b * p.n_top + j] > mine; ++j) ++larger;
             if (mine != 0 && larger < p.n_top) {
                 p.top_ids[r * p.n_top + larger] = index_of(mine);
                 p.top_logprob[r * p.n_top + larger] = (logit_of(mine) - st.m) - log_s;

@@ -1920,14 +1920,22 @@ def concat_streams(residual: torch.Tensor, delta: Optional[torch.Tensor], origin
 _MOST_POOLS = 16                  # of one launch (csrc/pages.cu)
 
 
-def _page_run(pool: torch.Tensor) -> None:
-    """Refuses a pool whose pages are not one run of bytes each ([entries, pages, ...], the entries at any distance)."""
+def _page_run(pool: torch.Tensor) -> Tuple[torch.Size, int, int]:
+    """(shape, elements from an entry to the next, elements of a page) of a pool [entries, pages, ...] whose pages are one run of bytes
+    each, one behind the other; the entries may lie at any distance.  Refuses others."""
     if not pool.is_cuda:
         raise KernelError(f"kernel arguments must be CUDA tensors (found device {pool.device}); there is no CPU path")
-    if pool.dim() < 2:
-        raise KernelError(f"copy_pages: a pool is [entries, pages, ...], found {tuple(pool.shape)}")
-    if pool.numel() and not pool[0].is_contiguous():
+    shape = pool.shape
+    if len(shape) < 2:
+        raise KernelError(f"copy_pages: a pool is [entries, pages, ...], found {tuple(shape)}")
+    strides, page = pool.stride(), 1
+    fits = True
+    for size, stride in zip(reversed(shape[2:]), reversed(strides[2:])):
+        fits = fits and (size == 1 or stride == page)
+        page *= size
+    if pool.numel() and not (fits and (shape[1] == 1 or strides[1] == page)):
         raise KernelError("copy_pages: the pages of an entry must lie one behind the other")
+    return shape, strides[0], page
 
 
 def copy_pages(src_pools, dst_pools, src: torch.Tensor, dst: torch.Tensor) -> None:
@@ -1936,29 +1944,40 @@ def copy_pages(src_pools, dst_pools, src: torch.Tensor, dst: torch.Tensor) -> No
     ordered: no page may be both read and written, none written twice.  A pair with an id outside a pool is left out there."""
     src_pools, dst_pools = list(src_pools), list(dst_pools)
     _cuda(src, dst)
-    if src.dtype != torch.int32 or dst.dtype != torch.int32 or src.numel() != dst.numel():
+    n_pairs = src.numel()
+    if src.dtype != torch.int32 or dst.dtype != torch.int32 or n_pairs != dst.numel():
         raise KernelError("copy_pages: the page ids must be int32, as many to read as to write")
     if len(src_pools) != len(dst_pools):
         raise KernelError(f"copy_pages: {len(src_pools)} pools to read, {len(dst_pools)} to write")
+    where, of, to, shapes = src.device, [], [], []
     for a, b in zip(src_pools, dst_pools):
-        _page_run(a)
-        _page_run(b)
-        if a.dtype != b.dtype or a.shape[0] != b.shape[0] or a.shape[2:] != b.shape[2:]:
-            raise KernelError(f"copy_pages: pools of {a.dtype} {tuple(a.shape)} and {b.dtype} {tuple(b.shape)} do not have the same pages")
-        if a.device != src.device or b.device != src.device or dst.device != src.device:
+        (a_shape, a_stride, page), size = _page_run(a), a.element_size()
+        b_shape, b_stride, _ = (a_shape, a_stride, page) if b is a else _page_run(b)
+        if b is not a:
+            if a.dtype != b.dtype or a_shape[0] != b_shape[0] or a_shape[2:] != b_shape[2:]:
+                raise KernelError(f"copy_pages: pools of {a.dtype} {tuple(a_shape)} and {b.dtype} {tuple(b_shape)} do not have the same pages")
+            if b.device != where:
+                raise KernelError("copy_pages: pools and page ids must be on one device")
+        if a.device != where:
             raise KernelError("copy_pages: pools and page ids must be on one device")
-    for at in range(0, len(src_pools), _MOST_POOLS):
-        some = list(zip(src_pools[at:at + _MOST_POOLS], dst_pools[at:at + _MOST_POOLS]))
-        n, shapes = len(some), []
-        for a, b in some:
-            size = a.element_size()
-            page = a[0, 0].numel() if a.shape[0] and a.shape[1] else 0
-            shapes += [a.stride(0) * size, b.stride(0) * size, page * size, a.shape[1], b.shape[1], a.shape[0]]
-        check(fn("pb_copy_pages")(n, (ctypes.c_void_p * n)(*[a.data_ptr() for a, _ in some]), (ctypes.c_void_p * n)(*[b.data_ptr() for _, b in some]),
-                                  (ctypes.c_longlong * len(shapes))(*shapes), _p(src), _p(dst), src.numel(), stream()), "copy_pages")
+        of.append(a.data_ptr())
+        to.append(b.data_ptr())
+        shapes += (a_stride * size, b_stride * size, page * size, a_shape[1], b_shape[1], a_shape[0])
+    if dst.device != where:
+        raise KernelError("copy_pages: pools and page ids must be on one device")
+    for at in range(0, len(of), _MOST_POOLS):
+        n = min(_MOST_POOLS, len(of) - at)
+        pointers, numbers = ctypes.c_void_p * n, ctypes.c_longlong * (6 * n)
+        check(fn("pb_copy_pages")(n, pointers(*of[at:at + n]), pointers(*to[at:at + n]), numbers(*shapes[6 * at:6 * (at + n)]), src.data_ptr(),
+                                  dst.data_ptr(), n_pairs, stream()), "copy_pages")
 
 
 MOST_ALTERNATIVES = 32            # one per lane of a warp (csrc/token_scores.cu)
+
+
+def _rows_of(name: str, what: str, t: torch.Tensor, dtype: torch.dtype, rows: int) -> None:
+    if t.dtype != dtype or t.dim() != 1 or t.numel() != rows:
+        raise KernelError(f"{name}: {what} must be {dtype} [{rows}], found {t.dtype} {tuple(t.shape)}")
 
 
 def token_scores(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tensor, entropy: torch.Tensor, rank: Optional[torch.Tensor] = None,
@@ -1969,15 +1988,17 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tens
     ``top_logprob`` [R, n], n <= 32.  Results are float32.  A logit of -inf is a token that cannot come; a row of nothing else, or with a
     NaN or +inf, has NaN where the formulas have it.  A token outside the vocabulary (-1 for none) has log probability NaN and rank -1."""
     _cuda(tokens, logprob, entropy, rank, top_ids, top_logprob)
-    if not logits.is_cuda or logits.dim() != 2 or (logits.numel() and logits.stride(1) != 1):
-        raise KernelError(f"token_scores: logits must be CUDA rows of neighbouring elements, found {tuple(logits.shape)} with strides "
+    shape = logits.shape
+    if not logits.is_cuda or len(shape) != 2 or (logits.stride(1) != 1 and logits.numel()):
+        raise KernelError(f"token_scores: logits must be CUDA rows of neighbouring elements, found {tuple(shape)} with strides "
                           f"{tuple(logits.stride())} on {logits.device}; there is no CPU path")
-    rows, vocab = logits.shape
+    rows, vocab = shape
     kind = code(logits.dtype)
-    for t, dtype, shape, name in ((tokens, torch.int32, (rows,), "tokens"), (logprob, torch.float32, (rows,), "logprob"),
-                                  (entropy, torch.float32, (rows,), "entropy"), (rank, torch.int32, (rows,), "rank")):
-        if t is not None and (t.dtype != dtype or tuple(t.shape) != shape):
-            raise KernelError(f"token_scores: {name} must be {dtype} {shape}, found {t.dtype} {tuple(t.shape)}")
+    _rows_of("token_scores", "tokens", tokens, torch.int32, rows)
+    _rows_of("token_scores", "logprob", logprob, torch.float32, rows)
+    _rows_of("token_scores", "entropy", entropy, torch.float32, rows)
+    if rank is not None:
+        _rows_of("token_scores", "rank", rank, torch.int32, rows)
     if (top_ids is None) != (top_logprob is None):
         raise KernelError("token_scores: the alternatives' ids and log probabilities go together")
     n = 0
@@ -2075,9 +2096,9 @@ def head_scores(h: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, logprob:
         raise KernelError(f"head_scores: h [R, K] and w [V, K] of one dtype, found {h.dtype} {tuple(h.shape)} and {w.dtype} {tuple(w.shape)}")
     code(h.dtype)
     (rows, k), vocab = h.shape, w.shape[0]
-    for t, dtype, name in ((tokens, torch.int32, "tokens"), (logprob, torch.float32, "logprob"), (entropy, torch.float32, "entropy")):
-        if t.dtype != dtype or tuple(t.shape) != (rows,):
-            raise KernelError(f"head_scores: {name} must be {dtype} ({rows},), found {t.dtype} {tuple(t.shape)}")
+    _rows_of("head_scores", "tokens", tokens, torch.int32, rows)
+    _rows_of("head_scores", "logprob", logprob, torch.float32, rows)
+    _rows_of("head_scores", "entropy", entropy, torch.float32, rows)
     if cap is not None and not cap > 0.0:
         raise KernelError(f"head_scores: the cap on the logits must be positive, found {cap}")
     if vocab == 0 or k == 0:
@@ -2090,6 +2111,8 @@ def head_scores(h: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, logprob:
                                    wait_word_addresses()[0], stream()), "head_scores", kernels=2)
         return
     some = max(1, min(rows, _LOGITS_AT_ONCE // vocab))
+    if 4 < some < rows:
+        some -= some % 4             # a row then starts as far from a multiple of 16 bytes as it would in one piece: the same sums
     logits = torch.empty((some, vocab), dtype=torch.float32, device=h.device)
     for at in range(0, rows, some):
         n = min(some, rows - at)
