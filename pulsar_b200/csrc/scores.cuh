@@ -44,7 +44,31 @@ __device__ __forceinline__ Stats warp_join(Stats st) {
     return st;
 }
 
-// Adds N logits.  Four sums of each kind are kept apart, so that additions do not wait for one another.
+// Two float32 at a time (one instruction each on sm_100).
+typedef unsigned long long Two;
+__device__ __forceinline__ Two two(float a, float b) {
+    Two v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ void apart(Two v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ Two add2(Two a, Two b) {
+    Two v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    Two v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+
+// Adds N logits (N even).  Two pairs of sums of each kind are kept apart, so that additions do not wait for one another.
 template <int N>
 __device__ __forceinline__ void add_logits(Stats& st, const float (&x)[N]) {
     float top = x[0];
@@ -59,18 +83,29 @@ __device__ __forceinline__ void add_logits(Stats& st, const float (&x)[N]) {
         st.m = top;
     }
     const float base = st.m == -INFINITY ? 0.0f : st.m;
-    constexpr int kApart = N < 4 ? N : 4;
-    float s[kApart] = {}, t[kApart] = {};
+    const Two lower = two(-base, -base), log2e = two(kScoreLog2e, kScoreLog2e);
+    Two s[2] = {0, 0}, t[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float d = x[i] - base, e = pow2(d * kScoreLog2e);
-        s[i % kApart] += e;
-        t[i % kApart] = fmaf(e, fmaxf(d, kFar), t[i % kApart]);
+    for (int i = 0; i < N; i += 2) {
+        const Two d = add2(two(x[i], x[i + 1]), lower), y = mul2(d, log2e);
+        float d0, d1, y0, y1;
+        apart(d, d0, d1);
+        apart(y, y0, y1);
+        const Two e = two(pow2(y0), pow2(y1));
+        s[i / 2 % 2] = add2(s[i / 2 % 2], e);
+        t[i / 2 % 2] = fma2(e, two(fmaxf(d0, kFar), fmaxf(d1, kFar)), t[i / 2 % 2]);
     }
-#pragma unroll
-    for (int i = 1; i < kApart; ++i) { s[0] += s[i]; t[0] += t[i]; }
-    st.s += s[0];
-    st.t += t[0];
+    float s0, s1, t0, t1;
+    apart(add2(s[0], s[1]), s0, s1);
+    apart(add2(t[0], t[1]), t0, t1);
+    st.s += s0 + s1;
+    st.t += t0 + t1;
+}
+
+// The sums of one logit.
+__device__ __forceinline__ Stats one_logit(float x) {
+    const float d = x == -INFINITY ? x : x - x, e = pow2(d);                  // x - x: 0, or NaN for NaN and +inf
+    return Stats{x == x ? x : -INFINITY, e, e * fmaxf(d, kFar)};
 }
 
 }  // namespace pb

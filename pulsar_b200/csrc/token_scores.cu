@@ -24,7 +24,7 @@ using namespace pb;
 
 constexpr int kMostThreads = 512;
 constexpr int kMostWarps = kMostThreads / 32;
-constexpr int kGroups = 128;                 // pairs of threads, or quads of a block of 512, whose largest keys are compared
+constexpr int kGroups = 128;                 // threads, pairs or quads (of a block of 128, 256, 512) whose largest keys are compared
 constexpr int kMostCandidates = 1024;
 constexpr int kMostCluster = 8;              // the portable limit
 constexpr int kMostTop = 32;
@@ -106,7 +106,7 @@ struct Slice {
 };
 
 template <typename T, bool RANK>
-__global__ void __launch_bounds__(kMostThreads)
+__global__ void __launch_bounds__(kMostThreads, 2)
 token_scores_kernel(const Scores p) {
     constexpr int N = kPerVector<T>, V = 16 / N, E = N * V;                   // elements of a vector, vectors and elements of a thread's chunk
     __shared__ Result result;
@@ -161,6 +161,9 @@ token_scores_kernel(const Scores p) {
                 if (token >= index + N) {                                     // equal logits count in front of the given token only
 #pragma unroll
                     for (int i = 0; i < N; ++i) likelier += x[j * N + i] >= given ? 1 : 0;
+                } else if (token < index) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) likelier += x[j * N + i] > given ? 1 : 0;
                 } else {
 #pragma unroll
                     for (int i = 0; i < N; ++i) likelier += x[j * N + i] > given || (x[j * N + i] == given && index + i < token) ? 1 : 0;
@@ -169,16 +172,22 @@ token_scores_kernel(const Scores p) {
         }
     }
     const bool met_nan = st.s != st.s;
+    const float highest = st.m;                                               // of this thread's chunks
+    uint4 last[V];                                                            // the chunk where it rose last, for the likeliest (asked for ahead of the sums)
+    if (p.n_top > 0) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (risen + j * 32 < slice.end) last[j] = slice.vectors[risen + j * 32];
+    }
     Stats odd = {-INFINITY, 0.0f, 0.0f};
     if (warp == 0) {
         const int i = slice.odd_index(lane);
         if (i >= 0) {
-            const float x[1] = {to_float(slice.row[i])};
-            add_logits(odd, x);
-            if (RANK) likelier += x[0] > given || (x[0] == given && i < token) ? 1 : 0;
+            const float x = to_float(slice.row[i]);
+            odd = one_logit(x);
+            if (RANK) likelier += x > given || (x == given && i < token) ? 1 : 0;
         }
     }
-    const float highest = st.m;                                               // of this thread's chunks
     st = warp_join(warp == 0 ? join(st, odd) : st);
     if (RANK) likelier = __reduce_add_sync(0xffffffffu, likelier);
     if (lane == 0) { stats_s[warp] = st; count_s[warp] = likelier; }
@@ -191,7 +200,7 @@ token_scores_kernel(const Scores p) {
             const int vector = risen + j * 32;
             if (vector < slice.end) {
                 float x[N];
-                widen(slice.vectors[vector], slice.row, x);
+                widen(last[j], slice.row, x);
 #pragma unroll
                 for (int i = N - 1; i >= 0; --i)
                     if (x[i] == highest) key = (Key)(slice.index(vector) + i + 1);
@@ -199,7 +208,7 @@ token_scores_kernel(const Scores p) {
         }
         if (key != 0) key = key_of(highest, (int)key - 1);
         int again = met_nan;
-        const int per_group = blockDim.x / kGroups;                           // 2 or 4
+        const int per_group = blockDim.x / kGroups;                           // 1, 2 or 4
         for (int o = 1; o < per_group; o <<= 1) {
             key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
             again |= __shfl_xor_sync(0xffffffffu, again, o);
@@ -210,15 +219,17 @@ token_scores_kernel(const Scores p) {
         if (tid < kMostTop) result.keys[tid] = 0;
         if (speaks) keys_s[group] = key;
         __syncthreads();
-        if (tid < kGroups) {
-            const Key mine = keys_s[tid];
+        {
+            // the threads of a group share its comparisons
+            const Key mine = keys_s[group];
             int larger = 0;
 #pragma unroll 4
-            for (int g = 0; g < kGroups; g += 2) {
-                const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(keys_s + g);
-                larger += (two.x > mine ? 1 : 0) + (two.y > mine ? 1 : 0);
+            for (int g = 2 * (tid % per_group); g < kGroups; g += 2 * per_group) {
+                const ulonglong2 some = *reinterpret_cast<const ulonglong2*>(keys_s + g);
+                larger += (some.x > mine ? 1 : 0) + (some.y > mine ? 1 : 0);
             }
-            if (mine != 0 && larger == p.n_top - 1) threshold_s = mine;
+            for (int o = 1; o < per_group; o <<= 1) larger += __shfl_xor_sync(0xffffffffu, larger, o);
+            if (speaks && mine != 0 && larger == p.n_top - 1) threshold_s = mine;
         }
         __syncthreads();
         const Key threshold = threshold_s;                                    // 0: fewer groups have elements than are asked for
@@ -234,15 +245,29 @@ token_scores_kernel(const Scores p) {
                 if (at < kMostCandidates) keys_s[at] = k;
             }
         };
-        for (int h = warp; h < n_hot_s; h += warps) {
-            for (int q = lane; q < turns * V * per_group; q += 32) {
-                const int owner = hot_s[h] * per_group + q % per_group, chunk = q / per_group;
-                const int vector = slice.begin + (owner >> 5) * 32 * V + (owner & 31) + chunk / V * step + chunk % V * 32;
-                if (vector < slice.end) {
-                    float x[N];
-                    widen(slice.vectors[vector], slice.row, x);
+        // the hot groups' vectors, all of them side by side; a thread asks for four before it looks at one
+        const int of_one = turns * V * per_group, of_all = n_hot_s * of_one;
+        for (int item0 = tid; item0 < of_all; item0 += 4 * blockDim.x) {
+            uint4 v[4];
+            int at[4];
 #pragma unroll
-                    for (int i = 0; i < N; ++i) candidate(x[i], slice.index(vector) + i);
+            for (int u = 0; u < 4; ++u) {
+                const int item = item0 + u * blockDim.x;
+                at[u] = slice.end;
+                if (item < of_all) {
+                    const int h = item / of_one, q = item - h * of_one;
+                    const int owner = hot_s[h] * per_group + q % per_group, chunk = q / per_group;
+                    at[u] = slice.begin + (owner >> 5) * 32 * V + (owner & 31) + chunk / V * step + chunk % V * 32;
+                    if (at[u] < slice.end) v[u] = slice.vectors[at[u]];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (at[u] < slice.end) {
+                    float x[N];
+                    widen(v[u], slice.row, x);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) candidate(x[i], slice.index(at[u]) + i);
                 }
             }
         }
@@ -256,6 +281,7 @@ token_scores_kernel(const Scores p) {
             for (int i = tid; i < n; i += blockDim.x) {
                 const Key mine = keys_s[i];
                 int larger = 0;
+#pragma unroll 4
                 for (int g = 0; g < n; ++g) larger += keys_s[g] > mine ? 1 : 0;
                 if (larger < p.n_top) result.keys[larger] = mine;
             }
@@ -297,27 +323,34 @@ token_scores_kernel(const Scores p) {
     else __syncthreads();
     if (block == 0) {
         for (int i = tid; i < blocks * p.n_top; i += blockDim.x) keys_s[i] = cluster.map_shared_rank(&result, i / p.n_top)->keys[i % p.n_top];
-        st = warp_join(lane < blocks ? cluster.map_shared_rank(&result, lane)->st : Stats{-INFINITY, 0.0f, 0.0f});
-        likelier = __reduce_add_sync(0xffffffffu, lane < blocks ? cluster.map_shared_rank(&result, lane)->likelier : 0);
+        if (warp == 0) {
+            st = warp_join(lane < blocks ? cluster.map_shared_rank(&result, lane)->st : Stats{-INFINITY, 0.0f, 0.0f});
+            likelier = __reduce_add_sync(0xffffffffu, lane < blocks ? cluster.map_shared_rank(&result, lane)->likelier : 0);
+            if (lane == 0) stats_s[0] = Stats{st.m, logf(st.s), st.t / st.s};
+        }
         __syncthreads();
-        const float log_s = logf(st.s);
+        if (blocks > 1) cluster.barrier_arrive();                             // the others' results are here: they may leave
+        const float m = stats_s[0].m, log_s = stats_s[0].s;
         if (tid == 0) {
-            p.logprob[r] = known ? (given - st.m) - log_s : nanf("");
-            p.entropy[r] = log_s - st.t / st.s;
+            p.logprob[r] = known ? (given - m) - log_s : nanf("");
+            p.entropy[r] = log_s - stats_s[0].t;
             if (RANK) p.rank[r] = known ? likelier : -1;
         }
         for (int i = tid; i < blocks * p.n_top; i += blockDim.x) {
             const Key mine = keys_s[i];
             int larger = 0;
-            for (int b = 0; b < blocks && larger < p.n_top; ++b)              // (every block's keys are in order)
-                for (int j = 0; j < p.n_top && keys_s[b * p.n_top + j] > mine; ++j) ++larger;
+#pragma unroll 4
+            for (int g = 0; g < blocks * p.n_top; ++g) larger += keys_s[g] > mine ? 1 : 0;
             if (mine != 0 && larger < p.n_top) {
                 p.top_ids[r * p.n_top + larger] = index_of(mine);
-                p.top_logprob[r * p.n_top + larger] = (logit_of(mine) - st.m) - log_s;
+                p.top_logprob[r * p.n_top + larger] = (logit_of(mine) - m) - log_s;
             }
         }
     }
-    if (blocks > 1) cluster.sync();                                           // no block leaves while the first still reads its result
+    if (blocks > 1) {                                                         // no block leaves while the first still reads its result
+        if (block != 0) cluster.barrier_arrive();
+        cluster.barrier_wait();
+    }
 }
 
 template <typename T, bool RANK>
@@ -351,7 +384,7 @@ PB_EXPORT int pb_token_scores(int dtype, const void* logits, long row_stride, in
     int cluster = 1;
     while (cluster < kMostCluster && (long long)rows * cluster * 2 <= 4 * 148 && vocab / (cluster * 2) >= 4096) cluster *= 2;
     if ((long long)rows * cluster > 0x7fffffff) return PB_ERR_TOO_LARGE;
-    const int threads = (long long)rows * cluster <= 148 ? 512 : 256;
+    const int threads = (long long)rows * cluster <= 148 ? 512 : (long long)rows * cluster <= 4 * 148 ? 256 : 128;
     if (dtype == PB_F32)
         return rank != nullptr ? launch<float, true>(p, rows, threads, cluster, stream) : launch<float, false>(p, rows, threads, cluster, stream);
     return rank != nullptr ? launch<__nv_bfloat16, true>(p, rows, threads, cluster, stream)
