@@ -105,10 +105,11 @@ struct Slice {
     }
 };
 
-template <typename T, bool RANK>
-__global__ void __launch_bounds__(kMostThreads, 2)
+// Registers for as many blocks on an SM as the launch counts on: one of 512 threads, two of 256, six of 128.
+template <typename T, bool RANK, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : THREADS == 256 ? 2 : 6)
 token_scores_kernel(const Scores p) {
-    constexpr int N = kPerVector<T>, V = 16 / N, E = N * V;                   // elements of a vector, vectors and elements of a thread's chunk
+    constexpr int N = kPerVector<T>, V = 16 / N;                              // elements of a vector, vectors of a thread's chunk of sixteen
     __shared__ Result result;
     __shared__ Stats stats_s[kMostWarps];
     __shared__ int count_s[kMostWarps];
@@ -120,44 +121,45 @@ token_scores_kernel(const Scores p) {
     cg::cluster_group cluster = cg::this_cluster();
     const int blocks = cluster.num_blocks(), block = cluster.block_rank();
     const long long r = blockIdx.x / blocks;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int warps = THREADS / 32;
     const Slice<T> slice(p, r, block, blocks);
     const int step = warps * 32 * V;                                          // vectors of a turn of the whole block
     const int my_first = slice.begin + warp * 32 * V + lane;                  // + turn * step + j * 32
 
-    uint4 next[V];
-    auto fetch = [&](int first) {
+    uint4 next[2][V];                                                         // the next two chunks are on their way
+    auto fetch = [&](uint4 (&into)[V], int first) {
 #pragma unroll
         for (int j = 0; j < V; ++j)
-            if (first + j * 32 < slice.end) next[j] = load_once(slice.vectors + first + j * 32);
+            if (first + j * 32 < slice.end) into[j] = load_once(slice.vectors + first + j * 32);
     };
-    fetch(my_first);
+    fetch(next[0], my_first);
+    fetch(next[1], my_first + step);
     const int token = p.tokens[r];
     const bool known = token >= 0 && token < p.vocab;
     const float given = known ? to_float(slice.row[token]) : 0.0f;
 
     Stats st = {-INFINITY, 0.0f, 0.0f};
     int likelier = 0, risen = my_first;
-    for (int first = my_first; first - lane < slice.end; first += step) {
-        float x[E];
+    auto take = [&](uint4 (&now)[V], int first) {
         const bool whole = first - lane + 32 * V <= slice.end;                // the warp's chunk ends inside the slice
+        float x[16];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            widen(next[j], slice.row, x + j * N);
+            widen(now[j], slice.row, x + j * N);
             if (!whole && first + j * 32 >= slice.end) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) x[j * N + i] = -INFINITY;
             }
         }
-        fetch(first + step);
+        fetch(now, first + 2 * step);
         const float before = st.m;
         add_logits(st, x);
-        if (st.m > before) risen = first;
         if (RANK) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const int index = slice.index(first + j * 32);
-                if (!whole && first + j * 32 >= slice.end) continue;
+                const int vector = first + j * 32, index = slice.index(vector);
+                if (!whole && vector >= slice.end) continue;
                 if (token >= index + N) {                                     // equal logits count in front of the given token only
 #pragma unroll
                     for (int i = 0; i < N; ++i) likelier += x[j * N + i] >= given ? 1 : 0;
@@ -170,6 +172,11 @@ token_scores_kernel(const Scores p) {
                 }
             }
         }
+        if (st.m > before) risen = first;
+    };
+    for (int first = my_first; first - lane < slice.end; first += 2 * step) {
+        take(next[0], first);
+        if (first - lane + step < slice.end) take(next[1], first + step);
     }
     const bool met_nan = st.s != st.s;
     const float highest = st.m;                                               // of this thread's chunks
@@ -208,7 +215,7 @@ token_scores_kernel(const Scores p) {
         }
         if (key != 0) key = key_of(highest, (int)key - 1);
         int again = met_nan;
-        const int per_group = blockDim.x / kGroups;                           // 1, 2 or 4
+        constexpr int per_group = THREADS / kGroups;                              // 1, 2 or 4
         for (int o = 1; o < per_group; o <<= 1) {
             key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
             again |= __shfl_xor_sync(0xffffffffu, again, o);
@@ -247,15 +254,16 @@ token_scores_kernel(const Scores p) {
         };
         // the hot groups' vectors, all of them side by side; a thread asks for four before it looks at one
         const int of_one = turns * V * per_group, of_all = n_hot_s * of_one;
-        for (int item0 = tid; item0 < of_all; item0 += 4 * blockDim.x) {
+        const float share = 1.0f / of_one;                                    // (item + 1/2) share has the whole part of item / of_one below 2^20 items
+        for (int item0 = tid; item0 < of_all; item0 += 4 * THREADS) {
             uint4 v[4];
             int at[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const int item = item0 + u * blockDim.x;
+                const int item = item0 + u * THREADS;
                 at[u] = slice.end;
                 if (item < of_all) {
-                    const int h = item / of_one, q = item - h * of_one;
+                    const int h = of_all < (1 << 20) ? (int)((item + 0.5f) * share) : item / of_one, q = item - h * of_one;
                     const int owner = hot_s[h] * per_group + q % per_group, chunk = q / per_group;
                     at[u] = slice.begin + (owner >> 5) * 32 * V + (owner & 31) + chunk / V * step + chunk % V * 32;
                     if (at[u] < slice.end) v[u] = slice.vectors[at[u]];
@@ -278,7 +286,7 @@ token_scores_kernel(const Scores p) {
         __syncthreads();
         const int n = n_candidates_s;
         if (n <= kMostCandidates) {
-            for (int i = tid; i < n; i += blockDim.x) {
+            for (int i = tid; i < n; i += THREADS) {
                 const Key mine = keys_s[i];
                 int larger = 0;
 #pragma unroll 4
@@ -289,7 +297,7 @@ token_scores_kernel(const Scores p) {
             Key below = ~(Key)0;
             for (int i = 0; i < p.n_top && below != 0; ++i) {
                 Key best = 0;
-                for (int vector = slice.begin + tid; vector < slice.end; vector += blockDim.x) {
+                for (int vector = slice.begin + tid; vector < slice.end; vector += THREADS) {
                     float x[N];
                     widen(slice.vectors[vector], slice.row, x);
 #pragma unroll
@@ -322,11 +330,13 @@ token_scores_kernel(const Scores p) {
     if (blocks > 1) cluster.sync();
     else __syncthreads();
     if (block == 0) {
-        for (int i = tid; i < blocks * p.n_top; i += blockDim.x) keys_s[i] = cluster.map_shared_rank(&result, i / p.n_top)->keys[i % p.n_top];
         if (warp == 0) {
             st = warp_join(lane < blocks ? cluster.map_shared_rank(&result, lane)->st : Stats{-INFINITY, 0.0f, 0.0f});
             likelier = __reduce_add_sync(0xffffffffu, lane < blocks ? cluster.map_shared_rank(&result, lane)->likelier : 0);
             if (lane == 0) stats_s[0] = Stats{st.m, logf(st.s), st.t / st.s};
+        } else {
+            for (int i = tid - 32; i < blocks * p.n_top; i += THREADS - 32)
+                keys_s[i] = cluster.map_shared_rank(&result, i / p.n_top)->keys[i % p.n_top];
         }
         __syncthreads();
         if (blocks > 1) cluster.barrier_arrive();                             // the others' results are here: they may leave
@@ -336,11 +346,20 @@ token_scores_kernel(const Scores p) {
             p.entropy[r] = log_s - stats_s[0].t;
             if (RANK) p.rank[r] = known ? likelier : -1;
         }
-        for (int i = tid; i < blocks * p.n_top; i += blockDim.x) {
+        for (int i = tid; i < blocks * p.n_top; i += THREADS) {
             const Key mine = keys_s[i];
-            int larger = 0;
-#pragma unroll 4
-            for (int g = 0; g < blocks * p.n_top; ++g) larger += keys_s[g] > mine ? 1 : 0;
+            int larger = i;                                                   // its own block's keys are in order
+            if (blocks > 1) {                                                 // and so are the others': searched all at once
+                int more[kMostCluster] = {};
+#pragma unroll
+                for (int jump = kMostTop; jump > 0; jump >>= 1)
+#pragma unroll
+                    for (int b = 0; b < kMostCluster; ++b)
+                        if (b < blocks && more[b] + jump <= p.n_top && keys_s[b * p.n_top + more[b] + jump - 1] > mine) more[b] += jump;
+                larger = 0;
+#pragma unroll
+                for (int b = 0; b < kMostCluster; ++b) larger += more[b];
+            }
             if (mine != 0 && larger < p.n_top) {
                 p.top_ids[r * p.n_top + larger] = index_of(mine);
                 p.top_logprob[r * p.n_top + larger] = (logit_of(mine) - m) - log_s;
@@ -353,11 +372,11 @@ token_scores_kernel(const Scores p) {
     }
 }
 
-template <typename T, bool RANK>
-int launch(const Scores& p, int rows, int threads, int cluster, cudaStream_t stream) {
+template <typename T, bool RANK, int THREADS>
+int launch(const Scores& p, int rows, int cluster, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows * cluster);
-    cfg.blockDim = dim3(threads);
+    cfg.blockDim = dim3(THREADS);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -366,7 +385,20 @@ int launch(const Scores& p, int rows, int threads, int cluster, cudaStream_t str
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, token_scores_kernel<T, RANK>, p);
+    return (int)cudaLaunchKernelEx(&cfg, token_scores_kernel<T, RANK, THREADS>, p);
+}
+
+template <typename T, bool RANK>
+int launch(const Scores& p, int rows, cudaStream_t stream) {
+    // What follows the pass over a row costs every block of it the same work: so no more blocks than two of 256 threads an SM, none with
+    // less than 4,096 logits.
+    int cluster = 1;
+    while (cluster < kMostCluster && (long long)rows * cluster * 2 <= 2 * 148 && p.vocab / (cluster * 2) >= 4096) cluster *= 2;
+    const long long blocks = (long long)rows * cluster;
+    if (blocks > 0x7fffffff) return PB_ERR_TOO_LARGE;
+    if (blocks <= 148) return launch<T, RANK, 512>(p, rows, cluster, stream);
+    if (blocks <= 2 * 148) return launch<T, RANK, 256>(p, rows, cluster, stream);
+    return launch<T, RANK, 128>(p, rows, cluster, stream);
 }
 
 }  // namespace
@@ -380,13 +412,6 @@ PB_EXPORT int pb_token_scores(int dtype, const void* logits, long row_stride, in
     if (vocab <= 0 || n_top < 0 || n_top > kMostTop || n_top > vocab || row_stride < 0) return PB_ERR_BAD_SIZE;
     if (n_top > 0 && (top_ids == nullptr || top_logprob == nullptr)) return PB_ERR_BAD_SIZE;
     const Scores p = {logits, row_stride, tokens, logprob, entropy, top_logprob, rank, top_ids, vocab, n_top};
-    // Blocks for four of 256 threads on each SM, none with less than 4,096 logits; where even eight a row are few, of 512 threads.
-    int cluster = 1;
-    while (cluster < kMostCluster && (long long)rows * cluster * 2 <= 4 * 148 && vocab / (cluster * 2) >= 4096) cluster *= 2;
-    if ((long long)rows * cluster > 0x7fffffff) return PB_ERR_TOO_LARGE;
-    const int threads = (long long)rows * cluster <= 148 ? 512 : (long long)rows * cluster <= 4 * 148 ? 256 : 128;
-    if (dtype == PB_F32)
-        return rank != nullptr ? launch<float, true>(p, rows, threads, cluster, stream) : launch<float, false>(p, rows, threads, cluster, stream);
-    return rank != nullptr ? launch<__nv_bfloat16, true>(p, rows, threads, cluster, stream)
-                           : launch<__nv_bfloat16, false>(p, rows, threads, cluster, stream);
+    if (dtype == PB_F32) return rank != nullptr ? launch<float, true>(p, rows, stream) : launch<float, false>(p, rows, stream);
+    return rank != nullptr ? launch<__nv_bfloat16, true>(p, rows, stream) : launch<__nv_bfloat16, false>(p, rows, stream);
 }
