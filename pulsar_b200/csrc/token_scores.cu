@@ -7,11 +7,11 @@
 //
 // The n likeliest (n <= 32) cost the pass nothing but the number of the chunk in which a thread's maximum rose last.  A key of 64 bits
 // holds a logit's bits, made to compare as unsigned numbers, above the complement of its index: of equal logits the lower index is the larger
-// key, and no two keys are equal.  The n-th largest of the threads' (or pairs of threads') largest keys is reached by n keys at least, so
-// no key below it is among the n likeliest, and only the few threads whose largest reaches it can hold any that are: their elements are read
-// once more (2 to 15 % of the row, from L2), what reaches the threshold is ranked by counting.  Should more than kMostCandidates reach it (a
-// row made so that few threads hold all its large logits), the likeliest are found one by one.  In the order of tokens a NaN is below
-// every number; a thread that met one is always read again.
+// key, and no two keys are equal.  The n-th largest of the thread groups' largest keys is reached by n keys at least, so no key below it is
+// among the n likeliest, and only the few threads whose own largest reaches it can hold any that are: their elements are read once more (some 5
+// to 10 % of the row, from L2), what reaches the threshold is ranked by counting.  Should more than kMostCandidates reach it (a row made
+// so that few threads hold all its large logits), the likeliest are found one by one.  In the order of tokens a NaN is below every
+// number; a thread that met one is always read again.
 #include "scores.cuh"
 
 #include <cooperative_groups.h>
@@ -24,7 +24,7 @@ using namespace pb;
 
 constexpr int kMostThreads = 512;
 constexpr int kMostWarps = kMostThreads / 32;
-constexpr int kGroups = 128;                 // threads, pairs or quads (of a block of 128, 256, 512) whose largest keys are compared
+constexpr int kGroups = 64;                  // of neighbouring threads, whose largest keys are compared
 constexpr int kMostCandidates = 1024;
 constexpr int kMostCluster = 8;              // the portable limit
 constexpr int kMostTop = 32;
@@ -114,7 +114,7 @@ token_scores_kernel(const Scores p) {
     __shared__ Stats stats_s[kMostWarps];
     __shared__ int count_s[kMostWarps];
     __shared__ __align__(16) Key keys_s[kMostCandidates];                                  // the groups' largest, then the candidates
-    __shared__ unsigned short hot_s[kGroups];
+    __shared__ unsigned short hot_s[THREADS];
     __shared__ Key threshold_s, best_s[kMostWarps];
     __shared__ int n_hot_s, n_candidates_s;
 
@@ -135,6 +135,8 @@ token_scores_kernel(const Scores p) {
     };
     fetch(next[0], my_first);
     fetch(next[1], my_first + step);
+    const int odd_index = warp == 0 ? slice.odd_index(lane) : -1;
+    const float odd_logit = odd_index >= 0 ? to_float(slice.row[odd_index]) : 0.0f;
     const int token = p.tokens[r];
     const bool known = token >= 0 && token < p.vocab;
     const float given = known ? to_float(slice.row[token]) : 0.0f;
@@ -187,13 +189,9 @@ token_scores_kernel(const Scores p) {
             if (risen + j * 32 < slice.end) last[j] = slice.vectors[risen + j * 32];
     }
     Stats odd = {-INFINITY, 0.0f, 0.0f};
-    if (warp == 0) {
-        const int i = slice.odd_index(lane);
-        if (i >= 0) {
-            const float x = to_float(slice.row[i]);
-            odd = one_logit(x);
-            if (RANK) likelier += x > given || (x == given && i < token) ? 1 : 0;
-        }
+    if (odd_index >= 0) {
+        odd = one_logit(odd_logit);
+        if (RANK) likelier += odd_logit > given || (odd_logit == given && odd_index < token) ? 1 : 0;
     }
     st = warp_join(warp == 0 ? join(st, odd) : st);
     if (RANK) likelier = __reduce_add_sync(0xffffffffu, likelier);
@@ -214,12 +212,10 @@ token_scores_kernel(const Scores p) {
             }
         }
         if (key != 0) key = key_of(highest, (int)key - 1);
-        int again = met_nan;
-        constexpr int per_group = THREADS / kGroups;                              // 1, 2 or 4
-        for (int o = 1; o < per_group; o <<= 1) {
-            key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
-            again |= __shfl_xor_sync(0xffffffffu, again, o);
-        }
+        const Key own = key;
+        constexpr int per_group = THREADS / kGroups;
+#pragma unroll
+        for (int o = 1; o < per_group; o <<= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
         const bool speaks = tid % per_group == 0;
         const int group = tid / per_group;
         if (tid == 0) { threshold_s = 0; n_hot_s = 0; n_candidates_s = 0; }
@@ -240,7 +236,7 @@ token_scores_kernel(const Scores p) {
         }
         __syncthreads();
         const Key threshold = threshold_s;                                    // 0: fewer groups have elements than are asked for
-        if (speaks && ((key != 0 && key >= threshold) || again)) hot_s[atomicAdd(&n_hot_s, 1)] = (unsigned short)group;
+        if ((own != 0 && own >= threshold) || met_nan) hot_s[atomicAdd(&n_hot_s, 1)] = (unsigned short)tid;
         __syncthreads();
         const int turns = (slice.end - slice.begin + step - 1) / step;
         const float threshold_logit = logit_of(threshold);                    // (NaN where there is no threshold: then no logit is below it)
@@ -252,8 +248,8 @@ token_scores_kernel(const Scores p) {
                 if (at < kMostCandidates) keys_s[at] = k;
             }
         };
-        // the hot groups' vectors, all of them side by side; a thread asks for four before it looks at one
-        const int of_one = turns * V * per_group, of_all = n_hot_s * of_one;
+        // the hot threads' vectors, all of them side by side; a thread asks for four before it looks at one
+        const int of_one = turns * V, of_all = n_hot_s * of_one;
         const float share = 1.0f / of_one;                                    // (item + 1/2) share has the whole part of item / of_one below 2^20 items
         for (int item0 = tid; item0 < of_all; item0 += 4 * THREADS) {
             uint4 v[4];
@@ -264,8 +260,8 @@ token_scores_kernel(const Scores p) {
                 at[u] = slice.end;
                 if (item < of_all) {
                     const int h = of_all < (1 << 20) ? (int)((item + 0.5f) * share) : item / of_one, q = item - h * of_one;
-                    const int owner = hot_s[h] * per_group + q % per_group, chunk = q / per_group;
-                    at[u] = slice.begin + (owner >> 5) * 32 * V + (owner & 31) + chunk / V * step + chunk % V * 32;
+                    const int owner = hot_s[h];
+                    at[u] = slice.begin + (owner >> 5) * 32 * V + (owner & 31) + q / V * step + q % V * 32;
                     if (at[u] < slice.end) v[u] = slice.vectors[at[u]];
                 }
             }
@@ -279,10 +275,7 @@ token_scores_kernel(const Scores p) {
                 }
             }
         }
-        if (warp == 0) {
-            const int i = slice.odd_index(lane);
-            if (i >= 0) candidate(to_float(slice.row[i]), i);
-        }
+        if (odd_index >= 0) candidate(odd_logit, odd_index);
         __syncthreads();
         const int n = n_candidates_s;
         if (n <= kMostCandidates) {
@@ -306,8 +299,8 @@ token_scores_kernel(const Scores p) {
                         if (k < below) best = max(best, k);
                     }
                 }
-                if (warp == 0 && slice.odd_index(lane) >= 0) {
-                    const Key k = key_of(to_float(slice.row[slice.odd_index(lane)]), slice.odd_index(lane));
+                if (odd_index >= 0) {
+                    const Key k = key_of(odd_logit, odd_index);
                     if (k < below) best = max(best, k);
                 }
 #pragma unroll
