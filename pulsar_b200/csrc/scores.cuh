@@ -68,12 +68,8 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
     return v;
 }
 
-// Adds N logits (N even).  Two pairs of sums of each kind are kept apart, so that additions do not wait for one another.
-template <int N>
-__device__ __forceinline__ void add_logits(Stats& st, const float (&x)[N]) {
-    float top = x[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
+// Brings the sums under `top` where that is beyond their maximum.
+__device__ __forceinline__ void raise(Stats& st, float top) {
     if (top > st.m) {
         if (st.m > -INFINITY) {
             const float delta = fmaxf(st.m - top, kFar), f = pow2(delta * kScoreLog2e);
@@ -82,24 +78,46 @@ __device__ __forceinline__ void add_logits(Stats& st, const float (&x)[N]) {
         }
         st.m = top;
     }
-    const float base = st.m == -INFINITY ? 0.0f : st.m;
+}
+
+// Adds N logits (N even) to sums under `base`; BOUNDED: none is so far below it that the difference overflows.  Two pairs of sums of each
+// kind are kept apart, so that additions do not wait for one another.
+template <bool BOUNDED, int N>
+__device__ __forceinline__ void add_under(Stats& st, float base, const float (&x)[N]) {
     const Two lower = two(-base, -base), log2e = two(kScoreLog2e, kScoreLog2e);
     Two s[2] = {0, 0}, t[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-        const Two d = add2(two(x[i], x[i + 1]), lower), y = mul2(d, log2e);
-        float d0, d1, y0, y1;
-        apart(d, d0, d1);
+        Two d = add2(two(x[i], x[i + 1]), lower);
+        const Two y = mul2(d, log2e);
+        float y0, y1;
         apart(y, y0, y1);
         const Two e = two(pow2(y0), pow2(y1));
+        if (!BOUNDED) {
+            float d0, d1;
+            apart(d, d0, d1);
+            d = two(fmaxf(d0, kFar), fmaxf(d1, kFar));
+        }
         s[i / 2 % 2] = add2(s[i / 2 % 2], e);
-        t[i / 2 % 2] = fma2(e, two(fmaxf(d0, kFar), fmaxf(d1, kFar)), t[i / 2 % 2]);
+        t[i / 2 % 2] = fma2(e, d, t[i / 2 % 2]);
     }
     float s0, s1, t0, t1;
     apart(add2(s[0], s[1]), s0, s1);
     apart(add2(t[0], t[1]), t0, t1);
     st.s += s0 + s1;
     st.t += t0 + t1;
+}
+template <int N>
+__device__ __forceinline__ void add_bounded(Stats& st, float base, const float (&x)[N]) { add_under<true>(st, base, x); }
+
+// Adds N logits.
+template <int N>
+__device__ __forceinline__ void add_logits(Stats& st, const float (&x)[N]) {
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
+    raise(st, top);
+    add_under<false>(st, st.m == -INFINITY ? 0.0f : st.m, x);
 }
 
 // The sums of one logit.

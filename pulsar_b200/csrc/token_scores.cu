@@ -58,6 +58,70 @@ __device__ __forceinline__ uint4 load_once(const uint4* p) {                  //
     return v;
 }
 
+// A chunk of sixteen logits joins the sums.
+__device__ __forceinline__ void add_chunk(Stats& st, const uint4 (&v)[4], const float* tag) {
+    float x[16];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) widen(v[j], tag, x + 4 * j);
+    add_logits(st, x);
+}
+// bfloat16: the maximum, and the bound that keeps differences finite, are found on pairs as they are (half the instructions, which is what
+// a row of bfloat16 is bound by).  The bound is 1,000 below the maximum, or a 64th of it, which is more than bfloat16's step, and is rounded
+// down: no number that weighs anything is raised to it.
+__device__ __forceinline__ void add_chunk(Stats& st, const uint4 (&v)[2], const __nv_bfloat16* tag) {
+    const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+    __nv_bfloat162 pair[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) pair[i] = *reinterpret_cast<const __nv_bfloat162*>(&w[i]);
+    const __nv_bfloat162 high = __hmax2(__hmax2(__hmax2(pair[0], pair[1]), __hmax2(pair[2], pair[3])),
+                                        __hmax2(__hmax2(pair[4], pair[5]), __hmax2(pair[6], pair[7])));
+    raise(st, fmaxf(__low2float(high), __high2float(high)));
+    if (st.m < -1e38f && st.m > -INFINITY) {             // there is no room below such a maximum for the bound
+        float x[16];
+        widen(v[0], tag, x);
+        widen(v[1], tag, x + 8);
+        add_logits(st, x);
+        return;
+    }
+    const float base = st.m == -INFINITY ? 0.0f : st.m;
+    const __nv_bfloat162 bound = __bfloat162bfloat162(__float2bfloat16_rd(base - fmaxf(-kFar, fabsf(base) * 0.015625f)));
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const __nv_bfloat162 up = __hmax2_nan(pair[i], bound);
+        x[2 * i] = __low2float(up);
+        x[2 * i + 1] = __high2float(up);
+    }
+    add_bounded(st, base, x);
+}
+
+// How many logits of a vector are beyond `given` (EQUAL: or equal to it).
+template <bool EQUAL>
+__device__ __forceinline__ int beyond(const uint4& v, float given, const float* tag) {
+    float x[4];
+    widen(v, tag, x);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n += (EQUAL ? x[i] >= given : x[i] > given) ? 1 : 0;
+    return n;
+}
+template <bool EQUAL>
+__device__ __forceinline__ int beyond(const uint4& v, float given, const __nv_bfloat16*) {
+    const __nv_bfloat162 bar = __float2bfloat162_rn(given);                   // (given is one of the row's own)
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    __nv_bfloat162 n[4];                                                      // ones and zeros: whole numbers up to 256 are exact
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&w[i]);
+        n[i] = EQUAL ? __hge2(x, bar) : __hgt2(x, bar);
+    }
+    const __nv_bfloat162 sum = __hadd2(__hadd2(n[0], n[1]), __hadd2(n[2], n[3]));
+    return (int)(__low2float(sum) + __high2float(sum));
+}
+// A vector of logits that are not there.
+__device__ __forceinline__ uint4 nothing(const float*) { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+__device__ __forceinline__ uint4 nothing(const __nv_bfloat16*) { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+
 struct Scores {
     const void* logits;
     long long row_stride;
@@ -145,32 +209,26 @@ token_scores_kernel(const Scores p) {
     int likelier = 0, risen = my_first;
     auto take = [&](uint4 (&now)[V], int first) {
         const bool whole = first - lane + 32 * V <= slice.end;                // the warp's chunk ends inside the slice
-        float x[16];
+        uint4 v[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            widen(now[j], slice.row, x + j * N);
-            if (!whole && first + j * 32 >= slice.end) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) x[j * N + i] = -INFINITY;
-            }
-        }
+        for (int j = 0; j < V; ++j) v[j] = !whole && first + j * 32 >= slice.end ? nothing(slice.row) : now[j];
         fetch(now, first + 2 * step);
         const float before = st.m;
-        add_logits(st, x);
+        add_chunk(st, v, slice.row);
         if (RANK) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const int vector = first + j * 32, index = slice.index(vector);
                 if (!whole && vector >= slice.end) continue;
                 if (token >= index + N) {                                     // equal logits count in front of the given token only
-#pragma unroll
-                    for (int i = 0; i < N; ++i) likelier += x[j * N + i] >= given ? 1 : 0;
+                    likelier += beyond<true>(v[j], given, slice.row);
                 } else if (token < index) {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) likelier += x[j * N + i] > given ? 1 : 0;
+                    likelier += beyond<false>(v[j], given, slice.row);
                 } else {
+                    float x[N];
+                    widen(v[j], slice.row, x);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) likelier += x[j * N + i] > given || (x[j * N + i] == given && index + i < token) ? 1 : 0;
+                    for (int i = 0; i < N; ++i) likelier += x[i] > given || (x[i] == given && index + i < token) ? 1 : 0;
                 }
             }
         }

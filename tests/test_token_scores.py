@@ -36,6 +36,7 @@ def plain(logits, tokens, top):
     ids = torch.argsort(order, dim=1, descending=True, stable=True)
     behind = torch.isnan(x).gather(1, ids)
     ids = ids.gather(1, torch.argsort(behind.int(), dim=1, stable=True))[:, :top]
+    log_p = torch.where(log_p < torch.finfo(torch.float32).min, -math.inf, log_p)      # results are float32
     logprob = torch.where(known, log_p.gather(1, t0.view(-1, 1)).squeeze(1), torch.full((len(t),), math.nan, dtype=torch.float64))
     return dict(logprob=logprob, entropy=entropy, rank=torch.where(known, rank, torch.full_like(rank, -1)), top_ids=ids, top_logprob=log_p.gather(1, ids))
 
@@ -170,6 +171,25 @@ def test_rows_at_any_distance_and_address(dtype, offset, stride, rows):
     logits = torch.as_strided(base, (rows, 1003), (stride, 1), offset)
     tokens = torch.randint(0, 1003, (rows,), generator=g).to(torch.int32).cuda()
     check(logits, tokens, 6)
+
+
+@cuda
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("top", [1e3, 5e4, 3e6, 1e20, 3e38, -2e38])
+def test_maxima_of_any_size_with_numbers_just_below(dtype, top):
+    """The step below a large maximum is a whole number or more: nothing below it weighs anything, and -inf beside the lowest numbers."""
+    vocab = 3003
+    logits = torch.full((4, vocab), -math.inf, dtype=dtype)
+    high = torch.tensor(top, dtype=dtype)
+    below = torch.nextafter(high.float(), torch.tensor(-math.inf)).to(dtype) if dtype == torch.float32 else (high.view(torch.int16) + (1 if top < 0 else -1)).view(dtype)
+    logits[0, ::3] = below
+    logits[0, 1500] = high
+    logits[1, ::2] = high
+    logits[2, 5::7] = torch.finfo(dtype).min
+    logits[3, 5::7] = torch.finfo(dtype).min
+    logits[3, 1000] = high
+    tokens = torch.tensor([1500, 2000, 5, 1000], dtype=torch.int32)
+    check(logits.cuda(), tokens.cuda(), 8)
 
 
 @cuda
