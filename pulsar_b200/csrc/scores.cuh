@@ -36,12 +36,9 @@ __device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
 
 // The lanes' sums as one, the same in all lanes.
 __device__ __forceinline__ Stats warp_join(Stats st) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const Stats other = {__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.t, o)};
-        st = join(st, other);
-    }
-    return st;
+    const float m = warp_max(st.m);
+    const float delta = st.m == -INFINITY ? 0.0f : fmaxf(st.m - m, kFar), f = pow2(delta * kScoreLog2e);
+    return Stats{m, warp_sum(st.s * f), warp_sum(f * (st.t + st.s * delta))};
 }
 
 // Two float32 at a time (one instruction each on sm_100).

@@ -95,28 +95,51 @@ __device__ __forceinline__ void add_chunk(Stats& st, const uint4 (&v)[2], const 
     add_bounded(st, base, x);
 }
 
-// How many logits of a vector are beyond `given` (EQUAL: or equal to it).
-template <bool EQUAL>
-__device__ __forceinline__ int beyond(const uint4& v, float given, const float* tag) {
-    float x[4];
-    widen(v, tag, x);
-    int n = 0;
+// Counts the logits of a chunk that are not below a bar of their vector's (NaN: none is counted), in ones and zeros of the logits' own type,
+// two an instruction.  float32 counts a thread's whole share (below 2^24), bfloat16 a chunk (below 2^8): exact.
+struct Count32 {
+    Two n = 0;
+    __device__ __forceinline__ void add(const uint4& v, float bar) {
+        float x[4], one[4];
+        widen(v, (const float*)nullptr, x);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) n += (EQUAL ? x[i] >= given : x[i] > given) ? 1 : 0;
-    return n;
-}
-template <bool EQUAL>
-__device__ __forceinline__ int beyond(const uint4& v, float given, const __nv_bfloat16*) {
-    const __nv_bfloat162 bar = __float2bfloat162_rn(given);                   // (given is one of the row's own)
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    __nv_bfloat162 n[4];                                                      // ones and zeros: whole numbers up to 256 are exact
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&w[i]);
-        n[i] = EQUAL ? __hge2(x, bar) : __hgt2(x, bar);
+        for (int i = 0; i < 4; ++i) asm("set.ge.f32.f32 %0, %1, %2;" : "=f"(one[i]) : "f"(x[i]), "f"(bar));
+        n = add2(n, add2(two(one[0], one[1]), two(one[2], one[3])));
     }
-    const __nv_bfloat162 sum = __hadd2(__hadd2(n[0], n[1]), __hadd2(n[2], n[3]));
-    return (int)(__low2float(sum) + __high2float(sum));
+    __device__ __forceinline__ void end_chunk() {}
+    __device__ __forceinline__ int total() const {
+        float a, b;
+        apart(n, a, b);
+        return (int)a + (int)b;
+    }
+};
+struct Count16 {
+    __nv_bfloat162 n = __float2bfloat162_rn(0.0f);
+    int sum = 0;
+    __device__ __forceinline__ void add(const uint4& v, float bar) {
+        const __nv_bfloat162 at = __float2bfloat162_rn(bar);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n = __hadd2(n, __hge2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), at));
+    }
+    __device__ __forceinline__ void end_chunk() {
+        sum += (int)(__low2float(n) + __high2float(n));
+        n = __float2bfloat162_rn(0.0f);
+    }
+    __device__ __forceinline__ int total() const { return sum; }
+};
+template <typename T> struct CountOf { typedef Count32 type; };
+template <> struct CountOf<__nv_bfloat16> { typedef Count16 type; };
+// The next larger number of the logits' type (NaN behind +inf and NaN): what a logit has to reach to be beyond x.
+__device__ __forceinline__ float next_up(float x, const float*) {
+    if (x != x) return x;
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    return __uint_as_float(x == 0.0f ? 1u : (b >> 31) ? b - 1 : b + 1);
+}
+__device__ __forceinline__ float next_up(float x, const __nv_bfloat16*) {
+    if (x != x) return x;
+    const uint32_t b = __float_as_uint(x + 0.0f) >> 16;
+    return __uint_as_float((x == 0.0f ? 1u : (b >> 15) ? b - 1 : b + 1) << 16);
 }
 // A vector of logits that are not there.
 __device__ __forceinline__ uint4 nothing(const float*) { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
@@ -205,8 +228,13 @@ token_scores_kernel(const Scores p) {
     const bool known = token >= 0 && token < p.vocab;
     const float given = known ? to_float(slice.row[token]) : 0.0f;
 
+    const float beyond = next_up(given, slice.row);
+    // the first element of the vector that holds the given token (an odd element in front of all: 0, behind all: the first of those)
+    const int token_vector = token < slice.before ? 0 : token >= slice.first_behind ? slice.first_behind : token - (token - slice.before) % N;
+
     Stats st = {-INFINITY, 0.0f, 0.0f};
-    int likelier = 0, risen = my_first;
+    typename CountOf<T>::type beaten;
+    int risen = my_first;
     auto take = [&](uint4 (&now)[V], int first) {
         const bool whole = first - lane + 32 * V <= slice.end;                // the warp's chunk ends inside the slice
         uint4 v[V];
@@ -218,19 +246,12 @@ token_scores_kernel(const Scores p) {
         if (RANK) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const int vector = first + j * 32, index = slice.index(vector);
-                if (!whole && vector >= slice.end) continue;
-                if (token >= index + N) {                                     // equal logits count in front of the given token only
-                    likelier += beyond<true>(v[j], given, slice.row);
-                } else if (token < index) {
-                    likelier += beyond<false>(v[j], given, slice.row);
-                } else {
-                    float x[N];
-                    widen(v[j], slice.row, x);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) likelier += x[i] > given || (x[i] == given && index + i < token) ? 1 : 0;
-                }
+                const int vector = first + j * 32;
+                // in front of the given token's vector equal logits count too
+                const float bar = slice.index(vector) < token_vector ? given : beyond;
+                beaten.add(v[j], !whole && vector >= slice.end ? nanf("") : bar);
             }
+            beaten.end_chunk();
         }
         if (st.m > before) risen = first;
     };
@@ -246,6 +267,10 @@ token_scores_kernel(const Scores p) {
         for (int j = 0; j < V; ++j)
             if (risen + j * 32 < slice.end) last[j] = slice.vectors[risen + j * 32];
     }
+    int likelier = beaten.total();
+    // logits equal to the given token's that stand in front of it in its own vector
+    if (RANK && block == 0 && warp == warps - 1 && token_vector + lane < token && token >= slice.before && token < slice.first_behind)
+        likelier += to_float(slice.row[token_vector + lane]) == given ? 1 : 0;
     Stats odd = {-INFINITY, 0.0f, 0.0f};
     if (odd_index >= 0) {
         odd = one_logit(odd_logit);
