@@ -40,49 +40,48 @@ struct Item {
     __device__ __forceinline__ int head_of(int kvh, int i, int G) const { return kvh * G + (row0 + i) % G; }
 };
 
-// Blocks 0 .. n_families * family_tiles * n_shared - 1 are the shared sides', the rest the sequences' own.  False: nothing to do.
-template <int ROWS, int TILE>
-__device__ __forceinline__ bool item_of(const Shared& p, int block, int G, Item& it) {
-    const int family_tiles = (p.most_members * G + ROWS - 1) / ROWS, own_tiles = (G + ROWS - 1) / ROWS;
-    int keys, split, splits;
-    const int shared_blocks = p.n_families * family_tiles * p.n_shared;
-    if (block < shared_blocks) {
-        split = block % p.n_shared;
-        const int tile = block / p.n_shared % family_tiles, family = block / p.n_shared / family_tiles;
-        it.first_member = p.family_start[family];
-        const int count = min(min(p.family_start[family + 1], p.n_members) - it.first_member, p.most_members);
-        if (it.first_member < 0 || count <= 0) return false;
-        it.row0 = tile * ROWS;
-        it.rows = min(ROWS, count * G - it.row0);
-        if (it.rows <= 0) return false;
-        const int first = p.members[it.first_member];
-        if (first < 0 || first >= p.n_seqs) return false;
-        it.table = p.block_table + (size_t)first * p.table_stride;
-        it.begin = 0;
-        keys = p.shared_len[first];
-        it.seq = -1;
-        it.part = split;
-        splits = p.n_shared;
-    } else {
-        block -= shared_blocks;
-        split = block % p.n_own;
-        it.seq = block / p.n_own / own_tiles;
-        it.row0 = block / p.n_own % own_tiles * ROWS;
-        it.rows = min(ROWS, G - it.row0);
-        it.first_member = 0;
-        it.table = p.block_table + (size_t)it.seq * p.table_stride;
-        it.begin = p.shared_len[it.seq];
-        keys = p.kv_len[it.seq] - it.begin;
-        it.part = p.n_shared + split;
-        splits = p.n_own;
-    }
-    keys = max(0, min(keys, p.table_stride * p.page_size - it.begin));          // never beyond the table
+// Split `split` of `splits` of the keys from it.begin on, never beyond the table.
+template <int TILE>
+__device__ __forceinline__ void cut(const Shared& p, Item& it, int keys, int split, int splits) {
+    keys = max(0, min(keys, p.table_stride * p.page_size - it.begin));
     int chunk = (keys + splits - 1) / splits;
     chunk = (chunk + TILE - 1) / TILE * TILE;
     const int end = it.begin + keys;
     it.begin = min(end, it.begin + split * chunk);
     it.end = min(end, it.begin + chunk);
+}
+// Block `block` of the shared sides.  False: nothing to do.
+template <int ROWS, int TILE>
+__device__ __forceinline__ bool family_item(const Shared& p, int block, int G, Item& it) {
+    const int tiles = (p.most_members * G + ROWS - 1) / ROWS;
+    const int split = block % p.n_shared, tile = block / p.n_shared % tiles, family = block / p.n_shared / tiles;
+    it.first_member = p.family_start[family];
+    const int count = min(min(p.family_start[family + 1], p.n_members) - it.first_member, p.most_members);
+    if (it.first_member < 0 || count <= 0) return false;
+    it.row0 = tile * ROWS;
+    it.rows = min(ROWS, count * G - it.row0);
+    if (it.rows <= 0) return false;
+    const int first = p.members[it.first_member];
+    if (first < 0 || first >= p.n_seqs) return false;
+    it.table = p.block_table + (size_t)first * p.table_stride;
+    it.begin = 0;
+    it.seq = -1;
+    it.part = split;
+    cut<TILE>(p, it, p.shared_len[first], split, p.n_shared);
     return true;
+}
+// Block `block` of the sequences' own sides.
+template <int ROWS, int TILE>
+__device__ __forceinline__ void own_item(const Shared& p, int block, int G, Item& it) {
+    const int tiles = (G + ROWS - 1) / ROWS, split = block % p.n_own;
+    it.seq = block / p.n_own / tiles;
+    it.row0 = block / p.n_own % tiles * ROWS;
+    it.rows = min(ROWS, G - it.row0);
+    it.first_member = 0;
+    it.table = p.block_table + (size_t)it.seq * p.table_stride;
+    it.begin = p.shared_len[it.seq];
+    it.part = p.n_shared + split;
+    cut<TILE>(p, it, p.kv_len[it.seq] - it.begin, split, p.n_own);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -95,7 +94,7 @@ constexpr int kWarpRows = kRows / (kThreads / 32);
 template <typename T, int QUADS /* groups of 128 dimensions */>
 __global__ void __launch_bounds__(kThreads)
 shared_general_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, const T* __restrict__ v_pool, float* __restrict__ partial,
-                      const Shared p, int D, const PoolBounds bounds) {
+                      const Shared p, int shared_blocks, int D, const PoolBounds bounds) {
     extern __shared__ __align__(16) float smem[];
     const int row_floats = D + 4;                        // 16-byte reads of 32 neighbouring rows then meet no bank twice
     float* q_s = smem;                                   // [kRows][D]
@@ -104,7 +103,9 @@ shared_general_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, con
     const int kvh = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int G = p.Hq / p.Hkv;
     Item it;
-    if (!item_of<kRows, kKeys>(p, blockIdx.x, G, it)) return;
+    pdl_trigger();                                       // (the join waits for this kernel's end)
+    if ((int)blockIdx.x >= shared_blocks) own_item<kRows, kKeys>(p, blockIdx.x - shared_blocks, G, it);
+    else if (!family_item<kRows, kKeys>(p, blockIdx.x, G, it)) return;
     const int quads = D / 4;
     for (int i = tid; i < kRows * quads; i += kThreads) {
         const int r = i / quads, d = (i - r * quads) * 4;
@@ -205,6 +206,197 @@ shared_general_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, con
     }
 }
 
+// ---------------------------------------------------------------------------------------------
+// bfloat16, head size 64 or 128, pages of a power of two up to 64 keys: on the tensor cores (mma.m16n8k16, float32 sums).  Tiles of 64
+// keys and values come through a ring of cp.async stages; ROW_TILES x 16 query rows meet each tile.  The four warps share the work as
+// ROW_TILES row tiles x 4 / ROW_TILES parts of the tile's keys: with one row tile (a sequence's own keys) each warp has 16 keys, with four
+// each has all 64 for its own rows, so that shared memory is read no more often than rows need.  What limits it is bytes in flight, two
+// blocks of three stages (128 KB on their way) an SM.
+constexpr int kTile = 64, kStages = 3, kWarps = 4;
+
+template <int D, int ROW_TILES>
+__device__ __forceinline__ void attend(const bf16* __restrict__ q, const bf16* __restrict__ k_pool, const bf16* __restrict__ v_pool,
+                                       float* __restrict__ partial, const Shared& p, const Item& it, int kvh, int page_shift,
+                                       const PoolBounds& bounds, unsigned char* smem) {
+    constexpr int kTileBytes = kTile * D * 2, kKSteps = D / 16, kNTiles = D / 8;
+    constexpr int kKeyParts = kWarps / ROW_TILES, kGroups = ROW_TILES;           // groups of 16 keys that a warp has of a tile
+    const uint32_t smem_base = smem_u32(smem);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int row_tile = warp % ROW_TILES, key_part = warp / ROW_TILES;
+    const int G = p.Hq / p.Hkv;
+    const int tile0 = it.begin / kTile, n_tiles = it.begin < it.end ? (it.end - 1) / kTile - tile0 + 1 : 0;
+    auto issue = [&](int i) {
+        const uint32_t k_dst = smem_base + i % kStages * 2 * kTileBytes;
+        if (i < n_tiles)
+            load_kv_tile<D, kWarps * 32>(k_dst, k_dst + kTileBytes, k_pool, v_pool, it.table, (tile0 + i) * kTile, it.begin, it.end - 1, kvh, p.Hkv,
+                                         page_shift, tid, 0, bounds);
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue(i);
+
+    // the warp's query rows: row_tile * 16 + g and + 8
+    long long row_of[2];                                                          // sequence * Hq + head, or -1
+    uint32_t qa[kKSteps][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int i = row_tile * 16 + g + 8 * r;
+        row_of[r] = -1;
+        if (i < it.rows) {
+            const int seq = it.seq_of(p, i, G);
+            if (seq >= 0 && seq < p.n_seqs) row_of[r] = (long long)seq * p.Hq + it.head_of(kvh, i, G);
+        }
+        const bf16* from = q + row_of[r] * D + 2 * t;
+#pragma unroll
+        for (int ks = 0; ks < kKSteps; ++ks) {
+            qa[ks][r] = row_of[r] >= 0 ? *reinterpret_cast<const uint32_t*>(from + ks * 16) : 0u;
+            qa[ks][r + 2] = row_of[r] >= 0 ? *reinterpret_cast<const uint32_t*>(from + ks * 16 + 8) : 0u;
+        }
+    }
+    float o[kNTiles][4];
+#pragma unroll
+    for (int i = 0; i < kNTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    const bool has_rows = row_tile * 16 < it.rows;
+
+    for (int i = 0; i < n_tiles; ++i) {
+        cp_async_wait<kStages - 2>();
+        __syncthreads();                                                          // tile i has landed; the stage of tile i - 1 is free
+        issue(i + kStages - 1);
+        const uint32_t k_s = smem_base + i % kStages * 2 * kTileBytes, v_s = k_s + kTileBytes;
+        const int in_tile = key_part * kGroups * 16, key0 = (tile0 + i) * kTile + in_tile;
+        if (!has_rows || key0 >= it.end || key0 + kGroups * 16 <= it.begin) continue;
+
+        float s[2 * kGroups][4];
+#pragma unroll
+        for (int n = 0; n < 2 * kGroups; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < kKSteps; ++ks)
+#pragma unroll
+            for (int n = 0; n < kGroups; ++n) {
+                uint32_t kb[4];
+                ldmatrix_x4(kb, k_s + tile_offset<D>(in_tile + n * 16 + (lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
+                mma_bf16(s[2 * n], qa[ks], kb[0], kb[1]);
+                mma_bf16(s[2 * n + 1], qa[ks], kb[2], kb[3]);
+            }
+        const bool inside = key0 >= it.begin && key0 + kGroups * 16 <= it.end;
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < 2 * kGroups; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int key = key0 + n * 8 + 2 * t + (e & 1);
+                s[n][e] = inside || (key >= it.begin && key < it.end) ? s[n][e] * p.scale_log2 : -INFINITY;
+                top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+            }
+        float f[2], base[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+            const float m_new = fmaxf(m[r], top[r]);
+            base[r] = m_new == -INFINITY ? 0.0f : m_new;                          // scores of -inf alone weigh nothing
+            f[r] = exp2f(m[r] - base[r]);
+            m[r] = m_new;
+            l[r] *= f[r];
+        }
+#pragma unroll
+        for (int n = 0; n < 2 * kGroups; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[n][e] = exp2f(s[n][e] - base[e >> 1]);
+                l[e >> 1] += s[n][e];
+            }
+#pragma unroll
+        for (int j = 0; j < kNTiles; ++j) { o[j][0] *= f[0]; o[j][1] *= f[0]; o[j][2] *= f[1]; o[j][3] *= f[1]; }
+#pragma unroll
+        for (int n = 0; n < kGroups; ++n) {
+            // weights in [0, 1], rounded to bfloat16 for the product (2^-9 of each); their sum is of the unrounded ones
+            const uint32_t pa[4] = {pack_bf16(s[2 * n][0], s[2 * n][1]), pack_bf16(s[2 * n][2], s[2 * n][3]), pack_bf16(s[2 * n + 1][0], s[2 * n + 1][1]),
+                                    pack_bf16(s[2 * n + 1][2], s[2 * n + 1][3])};
+#pragma unroll
+            for (int j = 0; j < kNTiles; j += 2) {
+                uint32_t vb[4];
+                ldmatrix_x4_trans(vb, v_s + tile_offset<D>(in_tile + n * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), j + (lane >> 4)));
+                mma_bf16(o[j], pa, vb[0], vb[1]);
+                mma_bf16(o[j + 1], pa, vb[2], vb[3]);
+            }
+        }
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    }
+    const int stride = D + 2, parts = p.n_shared + p.n_own;
+    if (kKeyParts == 1) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            if (row_of[r] < 0) continue;
+            float* dst = partial + ((size_t)row_of[r] * parts + it.part) * stride;
+#pragma unroll
+            for (int j = 0; j < kNTiles; ++j) *reinterpret_cast<float2*>(dst + j * 8 + 2 * t) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
+            if (t == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m[r], l[r]);
+        }
+        return;
+    }
+    // the warps that had other keys of the same rows meet in shared memory
+    __syncthreads();
+    float* o_s = reinterpret_cast<float*>(smem);                                  // [kWarps][16][D]
+    float* m_s = o_s + kWarps * 16 * D;                                           // [kWarps][16]
+    float* l_s = m_s + kWarps * 16;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+        for (int j = 0; j < kNTiles; ++j)
+            *reinterpret_cast<float2*>(o_s + (warp * 16 + g + 8 * r) * D + j * 8 + 2 * t) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
+        if (t == 0) { m_s[warp * 16 + g + 8 * r] = m[r]; l_s[warp * 16 + g + 8 * r] = l[r]; }
+    }
+    __syncthreads();
+    for (int i = tid; i < it.rows * (D / 4); i += kWarps * 32) {
+        const int row = i / (D / 4), d = (i - row * (D / 4)) * 4, at = (row / 16) * 16 + row % 16;       // warp row / 16 is its first key part
+        const int seq = it.seq_of(p, row, G);
+        if (seq < 0 || seq >= p.n_seqs) continue;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kKeyParts; ++w) top = fmaxf(top, m_s[w * ROW_TILES * 16 + at]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kKeyParts; ++w) {
+            const int from = w * ROW_TILES * 16 + at;
+            const float f = exp2f(m_s[from] - base);
+            const float4 v = *reinterpret_cast<const float4*>(o_s + from * D + d);
+            acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+            sum = fmaf(l_s[from], f, sum);
+        }
+        float* dst = partial + (((size_t)seq * p.Hq + it.head_of(kvh, row, G)) * parts + it.part) * stride;
+        *reinterpret_cast<float2*>(dst + d) = make_float2(acc.x, acc.y);
+        *reinterpret_cast<float2*>(dst + d + 2) = make_float2(acc.z, acc.w);
+        if (d == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(top, sum);
+    }
+}
+
+// ROW_TILES: of the shared sides' blocks; a sequence's own keys meet tiles of 16 rows.
+template <int D, int ROW_TILES>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+shared_tc_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pool, const bf16* __restrict__ v_pool, float* __restrict__ partial,
+                 const Shared p, int shared_blocks, int page_shift, const PoolBounds bounds) {
+    extern __shared__ __align__(128) unsigned char smem_tc[];
+    pdl_trigger();                                                                // (the join waits for this kernel's end)
+    const int G = p.Hq / p.Hkv;
+    Item it;
+    if ((int)blockIdx.x < shared_blocks) {
+        if (family_item<ROW_TILES * 16, kTile>(p, blockIdx.x, G, it))
+            attend<D, ROW_TILES>(q, k_pool, v_pool, partial, p, it, blockIdx.y, page_shift, bounds, smem_tc);
+    } else {
+        own_item<16, kTile>(p, blockIdx.x - shared_blocks, G, it);
+        attend<D, 1>(q, k_pool, v_pool, partial, p, it, blockIdx.y, page_shift, bounds, smem_tc);
+    }
+}
+
 // Joins a row's parts: a warp per row.  A sequence outside the families has no shared parts.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
@@ -212,6 +404,7 @@ shared_join_kernel(const float* __restrict__ partial, T* __restrict__ out, const
                    int n_own) {
     const int row = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (row >= rows) return;
+    pdl_wait();
     const int parts = n_shared + n_own, stride = D + 2;
     const int first = shared_len[row / Hq] > 0 ? 0 : n_shared;
     const float* base = partial + (size_t)row * parts * stride;
@@ -228,26 +421,55 @@ shared_join_kernel(const float* __restrict__ partial, T* __restrict__ out, const
     }
 }
 
-template <typename T>
+// Blocks of the shared sides and of all; 0 for all: too many for a grid.
+struct Grid {
+    int shared, all;
+};
+Grid grid_of(const Shared& p, int G, int shared_rows, int own_rows) {
+    const long long shared = (long long)p.n_families * ((p.most_members * G + shared_rows - 1) / shared_rows) * p.n_shared;
+    const long long all = shared + (long long)p.n_seqs * ((G + own_rows - 1) / own_rows) * p.n_own;
+    return all > 0x7fffffff ? Grid{0, 0} : Grid{(int)shared, (int)all};
+}
+
+template <typename T, int QUADS>
 int launch_general(const void* q, const void* k_pool, const void* v_pool, float* partial, const Shared& p, int D, int G, cudaStream_t stream) {
-    const long long blocks = (long long)p.n_families * ((p.most_members * G + kRows - 1) / kRows) * p.n_shared +
-                             (long long)p.n_seqs * ((G + kRows - 1) / kRows) * p.n_own;
-    if (blocks > 0x7fffffff) return PB_ERR_TOO_LARGE;
+    const Grid grid = grid_of(p, G, kRows, kRows);
+    if (grid.all == 0) return PB_ERR_TOO_LARGE;
     const size_t smem = (size_t)(kRows * D + kKeys * (D + 4) + kKeys * D) * sizeof(float);
-    const dim3 grid((unsigned)blocks, p.Hkv);
-    if (D <= 128) {
-        static SmemLimit limit;
-        if (const int rc = limit.allow(shared_general_kernel<T, 1>, smem)) return rc;
-        shared_general_kernel<T, 1><<<grid, kThreads, smem, stream>>>((const T*)q, (const T*)k_pool, (const T*)v_pool, partial, p, D, pool_bounds_now());
-    } else {
-        static SmemLimit limit;
-        if (const int rc = limit.allow(shared_general_kernel<T, 2>, smem)) return rc;
-        shared_general_kernel<T, 2><<<grid, kThreads, smem, stream>>>((const T*)q, (const T*)k_pool, (const T*)v_pool, partial, p, D, pool_bounds_now());
-    }
+    static SmemLimit limit;
+    if (const int rc = limit.allow(shared_general_kernel<T, QUADS>, smem)) return rc;
+    shared_general_kernel<T, QUADS><<<dim3(grid.all, p.Hkv), kThreads, smem, stream>>>((const T*)q, (const T*)k_pool, (const T*)v_pool, partial, p, grid.shared, D,
+                                                                                       pool_bounds_now());
     return launch_status();
 }
 
+template <int D, int ROW_TILES>
+int launch_tc(const void* q, const void* k_pool, const void* v_pool, float* partial, const Shared& p, int G, cudaStream_t stream) {
+    const Grid grid = grid_of(p, G, ROW_TILES * 16, 16);
+    if (grid.all == 0) return PB_ERR_TOO_LARGE;
+    constexpr int ring = kStages * 2 * kTile * D * 2, merge = (kWarps * 16 * D + 2 * kWarps * 16) * 4, smem = ring > merge ? ring : merge;
+    static SmemLimit limit;
+    if (const int rc = limit.allow(shared_tc_kernel<D, ROW_TILES>, smem)) return rc;
+    shared_tc_kernel<D, ROW_TILES><<<dim3(grid.all, p.Hkv), kWarps * 32, smem, stream>>>((const bf16*)q, (const bf16*)k_pool, (const bf16*)v_pool, partial, p,
+                                                                                         grid.shared, log2_exact(p.page_size), pool_bounds_now());
+    return launch_status();
+}
+template <int D>
+int launch_tc(const void* q, const void* k_pool, const void* v_pool, float* partial, const Shared& p, int G, cudaStream_t stream) {
+    const int rows = p.most_members * G;                  // as many row tiles as the largest family fills
+    if (rows <= 16) return launch_tc<D, 1>(q, k_pool, v_pool, partial, p, G, stream);
+    if (rows <= 32) return launch_tc<D, 2>(q, k_pool, v_pool, partial, p, G, stream);
+    return launch_tc<D, 4>(q, k_pool, v_pool, partial, p, G, stream);
+}
+
+bool tc_takes(int dtype, int D, int page_size) {
+    return dtype == PB_BF16 && (D == 64 || D == 128) && log2_exact(page_size) >= 0 && page_size <= kTile;
+}
+
 }  // namespace
+
+// Query rows that a block of the shared sides works on: what the caller cuts the keys by.
+PB_EXPORT int pb_shared_rows(int dtype, int rows, int D, int page_size) { return !tc_takes(dtype, D, page_size) ? kRows : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
 // q, out [n_seqs, Hq, D], pools [pages, Hkv, page_size, D] (dtype 0 float32, 1 bfloat16); block_table int32 [n_seqs, table_stride];
 // kv_len, shared_len int32 [n_seqs]; members int32 [n_members], family_start int32 [n_families + 1]; partial float32
@@ -264,13 +486,15 @@ PB_EXPORT int pb_paged_attention_shared(int dtype, const void* q, const void* k_
     const int G = Hq / Hkv;
     Shared p{block_table, kv_len, shared_len, members, family_start, n_seqs, n_members, n_families, most_members, table_stride, Hq, Hkv, page_size, n_shared, n_own,
              scale * kLog2e};
-    const int rc = dtype == PB_F32 ? launch_general<float>(q, k_pool, v_pool, partial, p, D, G, stream)
-                                   : launch_general<bf16>(q, k_pool, v_pool, partial, p, D, G, stream);
+    int rc;
+    if (tc_takes(dtype, D, page_size))
+        rc = D == 64 ? launch_tc<64>(q, k_pool, v_pool, partial, p, G, stream) : launch_tc<128>(q, k_pool, v_pool, partial, p, G, stream);
+    else if (dtype == PB_F32)
+        rc = D <= 128 ? launch_general<float, 1>(q, k_pool, v_pool, partial, p, D, G, stream) : launch_general<float, 2>(q, k_pool, v_pool, partial, p, D, G, stream);
+    else
+        rc = D <= 128 ? launch_general<bf16, 1>(q, k_pool, v_pool, partial, p, D, G, stream) : launch_general<bf16, 2>(q, k_pool, v_pool, partial, p, D, G, stream);
     if (rc != 0) return rc;
     const int rows = n_seqs * Hq, blocks = (rows + kThreads / 32 - 1) / (kThreads / 32);
-    if (dtype == PB_F32)
-        shared_join_kernel<float><<<blocks, kThreads, 0, stream>>>(partial, (float*)out, shared_len, rows, Hq, D, n_shared, n_own);
-    else
-        shared_join_kernel<bf16><<<blocks, kThreads, 0, stream>>>(partial, (bf16*)out, shared_len, rows, Hq, D, n_shared, n_own);
-    return launch_status();
+    if (dtype == PB_F32) return launch_pdl(shared_join_kernel<float>, dim3(blocks), dim3(kThreads), 0, stream, partial, (float*)out, shared_len, rows, Hq, D, n_shared, n_own);
+    return launch_pdl(shared_join_kernel<bf16>, dim3(blocks), dim3(kThreads), 0, stream, partial, (bf16*)out, shared_len, rows, Hq, D, n_shared, n_own);
 }

@@ -142,6 +142,7 @@ _SIGNATURES = {
     "pb_state_space": [_I, _P, _L, _P, _P, _I, _P, _P, _P, _P, _I, _F, _P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "pb_copy_pages": [_I, _P, _P, _P, _P, _P, _I, _P],
     "pb_paged_attention_shared": [_I] + [_P] * 6 + [_I] + [_P] * 4 + [_I] * 8 + [_F, _I, _I, _P],
+    "pb_shared_rows": [_I, _I, _I, _I],
     "pb_head_scores_supported": [_I, _I, _I],
     "pb_head_scores_scratch": [_I, _I],
     "pb_head_scores_wait_limit": [ctypes.c_longlong],
@@ -2016,13 +2017,6 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tens
                                 _p(top_ids) if n else None, _p(top_logprob) if n else None, n, stream()), "token_scores")
 
 
-def shared_splits(rows: int, n_kv_heads: int, keys: int, tile_rows: int) -> int:
-    """Parts that the keys of one side are cut into: so many that its blocks (row tiles x kv heads x parts) fill the SMs twice, none
-    shorter than 256 keys."""
-    blocks = max(1, -(-rows // tile_rows)) * n_kv_heads
-    return max(1, min(32, keys // 256, _DECODE_SLOTS // blocks))
-
-
 def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, out: torch.Tensor, block_table: torch.Tensor,
                            kv_len: torch.Tensor, shared_len: torch.Tensor, members: torch.Tensor, family_start: torch.Tensor, most_members: int,
                            most_shared: int, scale: float, partial: Optional[torch.Tensor] = None) -> None:
@@ -2056,7 +2050,7 @@ def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     if s == 0:
         return
     families = family_start.numel() - 1 if most_members > 0 and most_shared > 0 else 0
-    n_shared, n_own = shared_cut(s, families, int(most_members), int(most_shared), block_table.shape[1] * page_size, hq, hkv)
+    n_shared, n_own = shared_cut(s, families, int(most_members), int(most_shared), block_table.shape[1] * page_size, hq, hkv, d, page_size, q.dtype)
     need = s * hq * (n_shared + n_own) * (d + 2)
     if partial is None:
         partial = torch.empty(need, dtype=torch.float32, device=q.device)
@@ -2067,16 +2061,25 @@ def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
                                           page_size, float(scale), n_shared, n_own, stream()), "paged_attention_shared", kernels=2)
 
 
-def shared_cut(n_seqs: int, n_families: int, most_members: int, most_shared: int, table_tokens: int, n_heads: int, n_kv_heads: int) -> Tuple[int, int]:
+@functools.lru_cache(maxsize=1024)
+def shared_cut(n_seqs: int, n_families: int, most_members: int, most_shared: int, table_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int,
+               page_size: int, dtype: torch.dtype) -> Tuple[int, int]:
     """(parts of the shared keys, parts of the own keys) that ``paged_attention_shared`` works in."""
     group = n_heads // n_kv_heads
-    n_own = shared_splits(n_seqs * max(1, group), n_kv_heads, max(1, table_tokens - (most_shared if n_families else 0)), max(1, group))
-    return (shared_splits(n_families * most_members * group, n_kv_heads, most_shared, 16) if n_families else 0), n_own
+    rows = most_members * group
+    tile = fn("pb_shared_rows")(code(dtype), rows, head_dim, page_size)
+    blocks = n_families * -(-rows // tile) * n_kv_heads
+    n_shared = max(1, min(32, most_shared // 256, _DECODE_SLOTS // max(1, blocks))) if n_families else 0
+    own_blocks = n_seqs * -(-group // 16) * n_kv_heads
+    n_own = max(1, min(32, (table_tokens - (most_shared if n_families else 0)) // 256, _DECODE_SLOTS // max(1, own_blocks)))
+    return n_shared, n_own
 
 
-def shared_scratch(n_seqs: int, n_families: int, most_members: int, most_shared: int, table_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+def shared_scratch(n_seqs: int, n_families: int, most_members: int, most_shared: int, table_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int,
+                   page_size: int, dtype: torch.dtype) -> int:
     """Elements of ``paged_attention_shared``'s scratch."""
-    return n_seqs * n_heads * sum(shared_cut(n_seqs, n_families, most_members, most_shared, table_tokens, n_heads, n_kv_heads)) * (head_dim + 2)
+    return n_seqs * n_heads * sum(shared_cut(n_seqs, n_families, most_members, most_shared, table_tokens, n_heads, n_kv_heads, head_dim, page_size,
+                                             dtype)) * (head_dim + 2)
 
 
 _LOGITS_AT_ONCE = 1 << 26         # elements of float32 logits that ``head_scores`` keeps where it cannot do without them

@@ -136,7 +136,7 @@ def test_a_family_gives_what_its_members_give_alone(dtype):
 @cuda
 def test_wide_tables_scratch_of_the_caller_and_the_same_bits():
     c = Cache(FAMILIES["eight"], 8, 2, 128, 16, torch.bfloat16, 8)
-    need = ops.shared_scratch(8, 1, 8, max(c.shared), 400 * 16, 8, 2, 128)
+    need = ops.shared_scratch(8, 1, 8, max(c.shared), 400 * 16, 8, 2, 128, 16, torch.bfloat16)
     partial = torch.full((need,), float("nan"), device="cuda")
     first = c.run(width=400, partial=partial)
     assert torch.equal(first, c.run(width=400, partial=partial)) and torch.equal(first, c.run(width=400))
