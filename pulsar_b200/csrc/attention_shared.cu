@@ -10,10 +10,18 @@
 //
 // partial [n_seqs * Hq][n_shared + n_own][D + 2] float32: a part's o, then m (in units of log2) and l.
 #include "mma_common.cuh"
+#include "tcgen05_common.cuh"
 
 namespace {
 
 using namespace pb;
+
+// 2^x by the special-function unit alone; results below 2^-126 are 0.
+__device__ __forceinline__ float pow2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 struct Shared {
     const int* block_table;
@@ -207,134 +215,197 @@ shared_general_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, con
 }
 
 // ---------------------------------------------------------------------------------------------
-// bfloat16, head size 64 or 128, pages of a power of two up to 64 keys: on the tensor cores (mma.m16n8k16, float32 sums).  Tiles of 64
-// keys and values come through a ring of cp.async stages; ROW_TILES x 16 query rows meet each tile.  The four warps share the work as
-// ROW_TILES row tiles x 4 / ROW_TILES parts of the tile's keys: with one row tile (a sequence's own keys) each warp has 16 keys, with four
-// each has all 64 for its own rows, so that shared memory is read no more often than rows need.  What limits it is bytes in flight, two
-// blocks of three stages (128 KB on their way) an SM.
-constexpr int kTile = 64, kStages = 3, kWarps = 4;
+// bfloat16, head size 64 or 128, pages of 8, 16, 32 or 64 keys: on the tensor cores (mma.m16n8k16, float32 sums).  Tiles of 64 keys and
+// values come page by page through TMA (boxes of a page x 64 dimensions, 128-byte swizzle) into a ring of 96 KB that a warp of its own
+// fills, two blocks an SM: what limits the kernel is bytes in flight, and instructions that gather a tile would cost the other warps as
+// much as its products (cp.async by all warps: 2,300 cycles a tile and block, 77 against 48 us for 101 sequences).  ROW_TILES x 16 query
+// rows meet each tile; the four warps share the work as ROW_TILES row tiles x 4 / ROW_TILES parts of the tile's keys: with one row tile (a
+// sequence's own keys) each warp has 16 keys, with four each has all 64 for its own rows, so that shared memory is read no more often than
+// rows need.
+//
+// Rows of a tile that no key of the item fills hold what lies in the page, or an earlier tile: their scores are masked, and their values
+// are overwritten with zeros, for zero weights do not silence a NaN.  Every wait is bounded; a block that gives up sets the error
+// word, lets its copies land and returns.
+constexpr int kTile = 64, kWarps = 4, kTcThreads = (kWarps + 1) * 32;
+constexpr int kRing = 96 * 1024;
+template <int D> constexpr int kTileBytes = kTile * D * 2;                    // of keys, and of values
+template <int D> constexpr int kStages = kRing / (2 * kTileBytes<D>);
+
+// Byte offset of 16-byte chunk `chunk` of row `row` in a tile: halves of 64 dimensions, rows of 128 bytes, swizzled as TMA leaves them.
+__device__ __forceinline__ uint32_t tma_offset(int row, int chunk) {
+    return (uint32_t)((chunk >> 3) * (kTile * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+}
+
+struct Ring {
+    uint64_t full[8], empty[8];
+    int rows[64];                // the item's query rows: sequence * Hq + head, or -1
+    int gave_up;
+};
+
+// The warp that fills the ring: a lane per page of a tile.
+template <int D>
+__device__ __forceinline__ void fill(const CUtensorMap* map_k, const CUtensorMap* map_v, const Shared& p, const Item& it, int tile0, int n_tiles, int kvh,
+                                     int page_shift, const PoolBounds& bounds, uint32_t ring, Ring& sync, unsigned int* error) {
+    const int lane = threadIdx.x & 31;
+    for (int i = 0; i < n_tiles; ++i) {
+        const int stage = i % kStages<D>, key0 = (tile0 + i) * kTile;
+        const int first = max(it.begin, key0) >> page_shift, last = (min(it.end, key0 + kTile) - 1) >> page_shift;      // pages of the tile
+        int page = first + lane <= last ? it.table[first + lane] : 0;
+        if (!page_ok(page, bounds)) page = 0;
+        const uint32_t full = smem_addr(&sync.full[stage]);
+        bool ok = true;
+        if (lane == 0) {
+            ok = mbar_wait(smem_addr(&sync.empty[stage]), ((i / kStages<D>)&1) ^ 1, &sync.gave_up);
+            if (ok) mbar_expect_tx(full, (uint32_t)((last - first + 1) << page_shift) * D * 4);
+        }
+        if (!__shfl_sync(0xffffffffu, (int)ok, 0)) {
+            if (lane == 0) { *(volatile int*)&sync.gave_up = 1; atomicMax(error, 2u); }
+            return;
+        }
+        if (first + lane <= last) {
+            const uint32_t dst = ring + stage * 2 * kTileBytes<D> + (((first + lane) << page_shift) - key0) * 128;
+            const int row = (page * p.Hkv + kvh) << page_shift;
+#pragma unroll
+            for (int half = 0; half < D / 64; ++half) {
+                tma_load_2d(dst + half * kTile * 128, map_k, full, half * 64, row);
+                tma_load_2d(dst + kTileBytes<D> + half * kTile * 128, map_v, full, half * 64, row);
+            }
+        }
+        __syncwarp();
+    }
+}
 
 template <int D, int ROW_TILES>
-__device__ __forceinline__ void attend(const bf16* __restrict__ q, const bf16* __restrict__ k_pool, const bf16* __restrict__ v_pool,
-                                       float* __restrict__ partial, const Shared& p, const Item& it, int kvh, int page_shift,
-                                       const PoolBounds& bounds, unsigned char* smem) {
-    constexpr int kTileBytes = kTile * D * 2, kKSteps = D / 16, kNTiles = D / 8;
+__device__ __forceinline__ void attend(const bf16* __restrict__ q, const CUtensorMap* map_k, const CUtensorMap* map_v, float* __restrict__ partial,
+                                       const Shared& p, const Item& it, int kvh, int page_shift, const PoolBounds& bounds, unsigned char* smem,
+                                       Ring& sync, unsigned int* error) {
+    constexpr int kKSteps = D / 16, kNTiles = D / 8;
     constexpr int kKeyParts = kWarps / ROW_TILES, kGroups = ROW_TILES;           // groups of 16 keys that a warp has of a tile
-    const uint32_t smem_base = smem_u32(smem);
+    const uint32_t ring = smem_addr(smem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int row_tile = warp % ROW_TILES, key_part = warp / ROW_TILES;
-    const int G = p.Hq / p.Hkv;
     const int tile0 = it.begin / kTile, n_tiles = it.begin < it.end ? (it.end - 1) / kTile - tile0 + 1 : 0;
-    auto issue = [&](int i) {
-        const uint32_t k_dst = smem_base + i % kStages * 2 * kTileBytes;
-        if (i < n_tiles)
-            load_kv_tile<D, kWarps * 32>(k_dst, k_dst + kTileBytes, k_pool, v_pool, it.table, (tile0 + i) * kTile, it.begin, it.end - 1, kvh, p.Hkv,
-                                         page_shift, tid, 0, bounds);
-        cp_async_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue(i);
-
-    // the warp's query rows: row_tile * 16 + g and + 8
-    long long row_of[2];                                                          // sequence * Hq + head, or -1
-    uint32_t qa[kKSteps][4];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const int i = row_tile * 16 + g + 8 * r;
-        row_of[r] = -1;
-        if (i < it.rows) {
-            const int seq = it.seq_of(p, i, G);
-            if (seq >= 0 && seq < p.n_seqs) row_of[r] = (long long)seq * p.Hq + it.head_of(kvh, i, G);
-        }
-        const bf16* from = q + row_of[r] * D + 2 * t;
-#pragma unroll
-        for (int ks = 0; ks < kKSteps; ++ks) {
-            qa[ks][r] = row_of[r] >= 0 ? *reinterpret_cast<const uint32_t*>(from + ks * 16) : 0u;
-            qa[ks][r + 2] = row_of[r] >= 0 ? *reinterpret_cast<const uint32_t*>(from + ks * 16 + 8) : 0u;
-        }
-    }
     float o[kNTiles][4];
-#pragma unroll
-    for (int i = 0; i < kNTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    const bool has_rows = row_tile * 16 < it.rows;
-
-    for (int i = 0; i < n_tiles; ++i) {
-        cp_async_wait<kStages - 2>();
-        __syncthreads();                                                          // tile i has landed; the stage of tile i - 1 is free
-        issue(i + kStages - 1);
-        const uint32_t k_s = smem_base + i % kStages * 2 * kTileBytes, v_s = k_s + kTileBytes;
-        const int in_tile = key_part * kGroups * 16, key0 = (tile0 + i) * kTile + in_tile;
-        if (!has_rows || key0 >= it.end || key0 + kGroups * 16 <= it.begin) continue;
-
-        float s[2 * kGroups][4];
-#pragma unroll
-        for (int n = 0; n < 2 * kGroups; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-#pragma unroll
-        for (int ks = 0; ks < kKSteps; ++ks)
-#pragma unroll
-            for (int n = 0; n < kGroups; ++n) {
-                uint32_t kb[4];
-                ldmatrix_x4(kb, k_s + tile_offset<D>(in_tile + n * 16 + (lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
-                mma_bf16(s[2 * n], qa[ks], kb[0], kb[1]);
-                mma_bf16(s[2 * n + 1], qa[ks], kb[2], kb[3]);
-            }
-        const bool inside = key0 >= it.begin && key0 + kGroups * 16 <= it.end;
-        float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int n = 0; n < 2 * kGroups; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int key = key0 + n * 8 + 2 * t + (e & 1);
-                s[n][e] = inside || (key >= it.begin && key < it.end) ? s[n][e] * p.scale_log2 : -INFINITY;
-                top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
-            }
-        float f[2], base[2];
+    if (warp == kWarps) {
+        fill<D>(map_k, map_v, p, it, tile0, n_tiles, kvh, page_shift, bounds, ring, sync, error);
+    } else {
+        // the warp's query rows: row_tile * 16 + g and + 8
+        uint32_t qa[kKSteps][4];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-            const float m_new = fmaxf(m[r], top[r]);
-            base[r] = m_new == -INFINITY ? 0.0f : m_new;                          // scores of -inf alone weigh nothing
-            f[r] = exp2f(m[r] - base[r]);
-            m[r] = m_new;
-            l[r] *= f[r];
+            const int row = sync.rows[row_tile * 16 + g + 8 * r];
+            const bf16* from = q + (size_t)max(row, 0) * D + 2 * t;
+#pragma unroll
+            for (int ks = 0; ks < kKSteps; ++ks) {
+                qa[ks][r] = row >= 0 ? *reinterpret_cast<const uint32_t*>(from + ks * 16) : 0u;
+                qa[ks][r + 2] = row >= 0 ? *reinterpret_cast<const uint32_t*>(from + ks * 16 + 8) : 0u;
+            }
         }
 #pragma unroll
-        for (int n = 0; n < 2 * kGroups; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s[n][e] = exp2f(s[n][e] - base[e >> 1]);
-                l[e >> 1] += s[n][e];
+        for (int i = 0; i < kNTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        const bool has_rows = row_tile * 16 < it.rows;
+
+        for (int i = 0; i < n_tiles; ++i) {
+            const int stage = i % kStages<D>;
+            if (!mbar_wait(smem_addr(&sync.full[stage]), (i / kStages<D>)&1, &sync.gave_up)) {
+                if (lane == 0) { *(volatile int*)&sync.gave_up = 1; atomicMax(error, 4u); }
+                break;
             }
+            __syncwarp();
+            const uint32_t k_s = ring + stage * 2 * kTileBytes<D>, v_s = k_s + kTileBytes<D>;
+            const int in_tile = key_part * kGroups * 16, key0 = (tile0 + i) * kTile + in_tile;
+            if (has_rows && key0 < it.end && key0 + kGroups * 16 > it.begin) {
+                const bool inside = key0 >= it.begin && key0 + kGroups * 16 <= it.end;
+                if (!inside) {
+                    // values of rows without a key become zeros (warps with the same rows write the same)
+                    for (int c = lane; c < kGroups * 16 * (D / 8); c += 32) {
+                        const int row = c / (D / 8), key = key0 + row;
+                        if (key < it.begin || key >= it.end)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_s + tma_offset(in_tile + row, c % (D / 8))), "r"(0) : "memory");
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");          // before TMA fills the stage again
+                    __syncwarp();
+                }
+                float s[2 * kGroups][4];
 #pragma unroll
-        for (int j = 0; j < kNTiles; ++j) { o[j][0] *= f[0]; o[j][1] *= f[0]; o[j][2] *= f[1]; o[j][3] *= f[1]; }
+                for (int n = 0; n < 2 * kGroups; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
 #pragma unroll
-        for (int n = 0; n < kGroups; ++n) {
-            // weights in [0, 1], rounded to bfloat16 for the product (2^-9 of each); their sum is of the unrounded ones
-            const uint32_t pa[4] = {pack_bf16(s[2 * n][0], s[2 * n][1]), pack_bf16(s[2 * n][2], s[2 * n][3]), pack_bf16(s[2 * n + 1][0], s[2 * n + 1][1]),
-                                    pack_bf16(s[2 * n + 1][2], s[2 * n + 1][3])};
+                for (int ks = 0; ks < kKSteps; ++ks)
 #pragma unroll
-            for (int j = 0; j < kNTiles; j += 2) {
-                uint32_t vb[4];
-                ldmatrix_x4_trans(vb, v_s + tile_offset<D>(in_tile + n * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), j + (lane >> 4)));
-                mma_bf16(o[j], pa, vb[0], vb[1]);
-                mma_bf16(o[j + 1], pa, vb[2], vb[3]);
+                    for (int n = 0; n < kGroups; ++n) {
+                        uint32_t kb[4];
+                        ldmatrix_x4(kb, k_s + tma_offset(in_tile + n * 16 + (lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
+                        mma_bf16(s[2 * n], qa[ks], kb[0], kb[1]);
+                        mma_bf16(s[2 * n + 1], qa[ks], kb[2], kb[3]);
+                    }
+                float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int n = 0; n < 2 * kGroups; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = key0 + n * 8 + 2 * t + (e & 1);
+                        s[n][e] = inside || (key >= it.begin && key < it.end) ? s[n][e] * p.scale_log2 : -INFINITY;
+                        top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+                    }
+                float f[2], base[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                    const float m_new = fmaxf(m[r], top[r]);
+                    base[r] = m_new == -INFINITY ? 0.0f : m_new;                  // scores of -inf alone weigh nothing
+                    f[r] = pow2(m[r] - base[r]);
+                    m[r] = m_new;
+                    l[r] *= f[r];
+                }
+#pragma unroll
+                for (int n = 0; n < 2 * kGroups; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[n][e] = pow2(s[n][e] - base[e >> 1]);
+                        l[e >> 1] += s[n][e];
+                    }
+                if (__any_sync(0xffffffffu, f[0] != 1.0f || f[1] != 1.0f)) {      // a maximum rose, which soon is rare
+#pragma unroll
+                    for (int j = 0; j < kNTiles; ++j) { o[j][0] *= f[0]; o[j][1] *= f[0]; o[j][2] *= f[1]; o[j][3] *= f[1]; }
+                }
+#pragma unroll
+                for (int n = 0; n < kGroups; ++n) {
+                    // weights in [0, 1], rounded to bfloat16 for the product (2^-9 of each); their sum is of the unrounded ones
+                    const uint32_t pa[4] = {pack_bf16(s[2 * n][0], s[2 * n][1]), pack_bf16(s[2 * n][2], s[2 * n][3]),
+                                            pack_bf16(s[2 * n + 1][0], s[2 * n + 1][1]), pack_bf16(s[2 * n + 1][2], s[2 * n + 1][3])};
+#pragma unroll
+                    for (int j = 0; j < kNTiles; j += 2) {
+                        uint32_t vb[4];
+                        ldmatrix_x4_trans(vb, v_s + tma_offset(in_tile + n * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), j + (lane >> 4)));
+                        mma_bf16(o[j], pa, vb[0], vb[1]);
+                        mma_bf16(o[j + 1], pa, vb[2], vb[3]);
+                    }
+                }
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_addr(&sync.empty[stage]));
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
         }
     }
-    cp_async_wait<0>();
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    __syncthreads();                                                              // all tiles have been read
+    if (*(volatile int*)&sync.gave_up) {
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);                         // copies in flight land before this block's memory is reused
+        return;
     }
     const int stride = D + 2, parts = p.n_shared + p.n_own;
     if (kKeyParts == 1) {
+        if (warp == kWarps) return;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            if (row_of[r] < 0) continue;
-            float* dst = partial + ((size_t)row_of[r] * parts + it.part) * stride;
+            const int row = sync.rows[row_tile * 16 + g + 8 * r];
+            if (row < 0) continue;
+            float* dst = partial + ((size_t)row * parts + it.part) * stride;
 #pragma unroll
             for (int j = 0; j < kNTiles; ++j) *reinterpret_cast<float2*>(dst + j * 8 + 2 * t) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
             if (t == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m[r], l[r]);
@@ -342,37 +413,39 @@ __device__ __forceinline__ void attend(const bf16* __restrict__ q, const bf16* _
         return;
     }
     // the warps that had other keys of the same rows meet in shared memory
-    __syncthreads();
-    float* o_s = reinterpret_cast<float*>(smem);                                  // [kWarps][16][D]
-    float* m_s = o_s + kWarps * 16 * D;                                           // [kWarps][16]
+    constexpr int kPitch = D + 8;                                                 // floats of a row: eight rows of a warp then meet different banks
+    float* o_s = reinterpret_cast<float*>(smem);                                  // [kWarps][16][kPitch]
+    float* m_s = o_s + kWarps * 16 * kPitch;                                      // [kWarps][16]
     float* l_s = m_s + kWarps * 16;
+    if (warp < kWarps) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+        for (int r = 0; r < 2; ++r) {
 #pragma unroll
-        for (int j = 0; j < kNTiles; ++j)
-            *reinterpret_cast<float2*>(o_s + (warp * 16 + g + 8 * r) * D + j * 8 + 2 * t) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
-        if (t == 0) { m_s[warp * 16 + g + 8 * r] = m[r]; l_s[warp * 16 + g + 8 * r] = l[r]; }
+            for (int j = 0; j < kNTiles; ++j)
+                *reinterpret_cast<float2*>(o_s + (warp * 16 + g + 8 * r) * kPitch + j * 8 + 2 * t) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
+            if (t == 0) { m_s[warp * 16 + g + 8 * r] = m[r]; l_s[warp * 16 + g + 8 * r] = l[r]; }
+        }
     }
     __syncthreads();
-    for (int i = tid; i < it.rows * (D / 4); i += kWarps * 32) {
-        const int row = i / (D / 4), d = (i - row * (D / 4)) * 4, at = (row / 16) * 16 + row % 16;       // warp row / 16 is its first key part
-        const int seq = it.seq_of(p, row, G);
-        if (seq < 0 || seq >= p.n_seqs) continue;
+    for (int i = tid; i < it.rows * (D / 4); i += kTcThreads) {
+        const int row = i / (D / 4), d = i % (D / 4) * 4;                         // the row's first key part is warp row / 16
+        const int to = sync.rows[row];
+        if (to < 0) continue;
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kKeyParts; ++w) top = fmaxf(top, m_s[w * ROW_TILES * 16 + at]);
+        for (int w = 0; w < kKeyParts; ++w) top = fmaxf(top, m_s[w * ROW_TILES * 16 + row]);
         const float base = top == -INFINITY ? 0.0f : top;
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         float sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kKeyParts; ++w) {
-            const int from = w * ROW_TILES * 16 + at;
-            const float f = exp2f(m_s[from] - base);
-            const float4 v = *reinterpret_cast<const float4*>(o_s + from * D + d);
+            const int from = w * ROW_TILES * 16 + row;
+            const float f = pow2(m_s[from] - base);
+            const float4 v = *reinterpret_cast<const float4*>(o_s + from * kPitch + d);
             acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
             sum = fmaf(l_s[from], f, sum);
         }
-        float* dst = partial + (((size_t)seq * p.Hq + it.head_of(kvh, row, G)) * parts + it.part) * stride;
+        float* dst = partial + ((size_t)to * parts + it.part) * stride;
         *reinterpret_cast<float2*>(dst + d) = make_float2(acc.x, acc.y);
         *reinterpret_cast<float2*>(dst + d + 2) = make_float2(acc.z, acc.w);
         if (d == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(top, sum);
@@ -381,43 +454,84 @@ __device__ __forceinline__ void attend(const bf16* __restrict__ q, const bf16* _
 
 // ROW_TILES: of the shared sides' blocks; a sequence's own keys meet tiles of 16 rows.
 template <int D, int ROW_TILES>
-__global__ void __launch_bounds__(kWarps * 32, 2)
-shared_tc_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_pool, const bf16* __restrict__ v_pool, float* __restrict__ partial,
-                 const Shared p, int shared_blocks, int page_shift, const PoolBounds bounds) {
-    extern __shared__ __align__(128) unsigned char smem_tc[];
+__global__ void __launch_bounds__(kTcThreads, 2)
+shared_tc_kernel(const bf16* __restrict__ q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                 float* __restrict__ partial, const Shared p, int shared_blocks, int page_shift, const PoolBounds bounds, unsigned int* error) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ Ring sync;
     pdl_trigger();                                                                // (the join waits for this kernel's end)
-    const int G = p.Hq / p.Hkv;
+    const int G = p.Hq / p.Hkv, tid = threadIdx.x;
+    const bool family = (int)blockIdx.x < shared_blocks;
     Item it;
-    if ((int)blockIdx.x < shared_blocks) {
-        if (family_item<ROW_TILES * 16, kTile>(p, blockIdx.x, G, it))
-            attend<D, ROW_TILES>(q, k_pool, v_pool, partial, p, it, blockIdx.y, page_shift, bounds, smem_tc);
+    if (family) {
+        if (!family_item<ROW_TILES * 16, kTile>(p, blockIdx.x, G, it)) return;
     } else {
         own_item<16, kTile>(p, blockIdx.x - shared_blocks, G, it);
-        attend<D, 1>(q, k_pool, v_pool, partial, p, it, blockIdx.y, page_shift, bounds, smem_tc);
     }
+    if (tid == kWarps * 32) {
+        for (int i = 0; i < kStages<D>; ++i) {
+            mbar_init(smem_addr(&sync.full[i]), 1);
+            mbar_init(smem_addr(&sync.empty[i]), kWarps);
+        }
+        sync.gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    } else if (tid < 64) {
+        int row = -1;
+        if (tid < it.rows) {
+            const int seq = it.seq_of(p, tid, G);
+            if (seq >= 0 && seq < p.n_seqs) row = seq * p.Hq + it.head_of(blockIdx.y, tid, G);
+        }
+        sync.rows[tid] = row;
+    }
+    __syncthreads();
+    if (family) attend<D, ROW_TILES>(q, &map_k, &map_v, partial, p, it, blockIdx.y, page_shift, bounds, smem, sync, error);
+    else attend<D, 1>(q, &map_k, &map_v, partial, p, it, blockIdx.y, page_shift, bounds, smem, sync, error);
 }
 
-// Joins a row's parts: a warp per row.  A sequence outside the families has no shared parts.
+// Joins a row's parts: a warp per row, a lane per part for their weights and per four dimensions for the sums.  A sequence outside
+// the families has no shared parts.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 shared_join_kernel(const float* __restrict__ partial, T* __restrict__ out, const int* __restrict__ shared_len, int rows, int Hq, int D, int n_shared,
                    int n_own) {
     const int row = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (row >= rows) return;
-    pdl_wait();
     const int parts = n_shared + n_own, stride = D + 2;
-    const int first = shared_len[row / Hq] > 0 ? 0 : n_shared;
+    const int first = shared_len[row / Hq] > 0 ? 0 : n_shared;                    // (the host wrote it, before the kernel ahead began)
     const float* base = partial + (size_t)row * parts * stride;
-    float m = -INFINITY;
-    for (int i = first; i < parts; ++i) m = fmaxf(m, base[i * stride + D]);
-    if (m == -INFINITY) m = 0.0f;                        // nothing to attend to (or NaN, which l carries)
-    float l = 0.0f;
-    for (int i = first; i < parts; ++i) l += base[i * stride + D + 1] * exp2f(base[i * stride + D] - m);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;       // a sequence without keys: zeros
-    for (int d = lane; d < D; d += 32) {
-        float acc = 0.0f;
-        for (int i = first; i < parts; ++i) acc = fmaf(base[i * stride + d], exp2f(base[i * stride + D] - m), acc);
-        out[(size_t)row * D + d] = from_float<T>(acc * inv);
+    pdl_wait();
+    float m[2], l[2];                                                             // up to 64 parts
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int i = first + lane + 32 * h;
+        const float2 ml = i < parts ? *reinterpret_cast<const float2*>(base + (size_t)i * stride + D) : make_float2(-INFINITY, 0.0f);
+        m[h] = ml.x;
+        l[h] = ml.y;
+    }
+    float top = warp_max(fmaxf(m[0], m[1]));
+    if (top == -INFINITY) top = 0.0f;                    // nothing to attend to (or NaN, which l carries)
+    m[0] = pow2(m[0] - top);
+    m[1] = pow2(m[1] - top);
+    const float sum = warp_sum(l[0] * m[0] + l[1] * m[1]);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // a sequence without keys: zeros
+    for (int d0 = 0; d0 < D; d0 += 128) {
+        const int d = d0 + lane * 4;
+        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int i = first; i < parts; ++i) {
+            const int at = i - first;
+            const float f = __shfl_sync(0xffffffffu, at < 32 ? m[0] : m[1], at & 31);
+            if (d < D) {
+                const float2 a = *reinterpret_cast<const float2*>(base + (size_t)i * stride + d), b = *reinterpret_cast<const float2*>(base + (size_t)i * stride + d + 2);
+                acc[0] = fmaf(a.x, f, acc[0]); acc[1] = fmaf(a.y, f, acc[1]); acc[2] = fmaf(b.x, f, acc[2]); acc[3] = fmaf(b.y, f, acc[3]);
+            }
+        }
+        if (d < D) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[k] *= inv;
+            store_quad(out + (size_t)row * D + d, acc);
+        }
     }
 }
 
@@ -443,27 +557,52 @@ int launch_general(const void* q, const void* k_pool, const void* v_pool, float*
     return launch_status();
 }
 
+// A pool as rows of D dimensions, a box a page of 64 of them.
+int make_map(CUtensorMap* map, const void* pool, long long rows, int D, int page_size) {
+    EncodeTiledFn encode = encode_fn();
+    if (!encode) return (int)cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)D * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)page_size};
+    const cuuint32_t elem[2] = {1, 1};
+    const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(pool), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return rc == CUDA_SUCCESS ? 0 : PB_ERR_BAD_SIZE;
+}
+
+struct Maps {
+    CUtensorMap k, v;
+    unsigned int* error;
+};
+
 template <int D, int ROW_TILES>
-int launch_tc(const void* q, const void* k_pool, const void* v_pool, float* partial, const Shared& p, int G, cudaStream_t stream) {
+int launch_tc(const void* q, const Maps& maps, float* partial, const Shared& p, int G, cudaStream_t stream) {
     const Grid grid = grid_of(p, G, ROW_TILES * 16, 16);
     if (grid.all == 0) return PB_ERR_TOO_LARGE;
-    constexpr int ring = kStages * 2 * kTile * D * 2, merge = (kWarps * 16 * D + 2 * kWarps * 16) * 4, smem = ring > merge ? ring : merge;
+    constexpr int smem = kRing + 1024;
     static SmemLimit limit;
     if (const int rc = limit.allow(shared_tc_kernel<D, ROW_TILES>, smem)) return rc;
-    shared_tc_kernel<D, ROW_TILES><<<dim3(grid.all, p.Hkv), kWarps * 32, smem, stream>>>((const bf16*)q, (const bf16*)k_pool, (const bf16*)v_pool, partial, p,
-                                                                                         grid.shared, log2_exact(p.page_size), pool_bounds_now());
+    shared_tc_kernel<D, ROW_TILES><<<dim3(grid.all, p.Hkv), kTcThreads, smem, stream>>>((const bf16*)q, maps.k, maps.v, partial, p, grid.shared,
+                                                                                        log2_exact(p.page_size), pool_bounds_now(), maps.error);
     return launch_status();
 }
 template <int D>
-int launch_tc(const void* q, const void* k_pool, const void* v_pool, float* partial, const Shared& p, int G, cudaStream_t stream) {
+int launch_tc(const void* q, const void* k_pool, const void* v_pool, float* partial, const Shared& p, int G, int n_pages, unsigned int* error, cudaStream_t stream) {
+    Maps maps;
+    maps.error = error;
+    const long long pool_rows = (long long)n_pages * p.Hkv * p.page_size;
+    if (pool_rows > 0x7fffffff) return PB_ERR_TOO_LARGE;
+    int rc = make_map(&maps.k, k_pool, pool_rows, D, p.page_size);
+    if (rc == 0) rc = make_map(&maps.v, v_pool, pool_rows, D, p.page_size);
+    if (rc != 0) return rc;
     const int rows = p.most_members * G;                  // as many row tiles as the largest family fills
-    if (rows <= 16) return launch_tc<D, 1>(q, k_pool, v_pool, partial, p, G, stream);
-    if (rows <= 32) return launch_tc<D, 2>(q, k_pool, v_pool, partial, p, G, stream);
-    return launch_tc<D, 4>(q, k_pool, v_pool, partial, p, G, stream);
+    if (rows <= 16) return launch_tc<D, 1>(q, maps, partial, p, G, stream);
+    if (rows <= 32) return launch_tc<D, 2>(q, maps, partial, p, G, stream);
+    return launch_tc<D, 4>(q, maps, partial, p, G, stream);
 }
 
 bool tc_takes(int dtype, int D, int page_size) {
-    return dtype == PB_BF16 && (D == 64 || D == 128) && log2_exact(page_size) >= 0 && page_size <= kTile;
+    return dtype == PB_BF16 && (D == 64 || D == 128) && log2_exact(page_size) >= 3 && page_size <= kTile;
 }
 
 }  // namespace
@@ -473,22 +612,24 @@ PB_EXPORT int pb_shared_rows(int dtype, int rows, int D, int page_size) { return
 
 // q, out [n_seqs, Hq, D], pools [pages, Hkv, page_size, D] (dtype 0 float32, 1 bfloat16); block_table int32 [n_seqs, table_stride];
 // kv_len, shared_len int32 [n_seqs]; members int32 [n_members], family_start int32 [n_families + 1]; partial float32
-// [n_seqs * Hq * (n_shared + n_own) * (D + 2)].
+// [n_seqs * Hq * (n_shared + n_own) * (D + 2)], all 16-byte aligned; n_pages: of the pools; error: the word that a block sets which gave up
+// a bounded wait; n_shared + n_own <= 64.
 PB_EXPORT int pb_paged_attention_shared(int dtype, const void* q, const void* k_pool, const void* v_pool, void* out, float* partial,
                                         const int* block_table, int table_stride, const int* kv_len, const int* shared_len, const int* members,
                                         const int* family_start, int n_seqs, int n_members, int n_families, int most_members, int Hq, int Hkv, int D,
-                                        int page_size, float scale, int n_shared, int n_own, cudaStream_t stream) {
+                                        int page_size, float scale, int n_shared, int n_own, int n_pages, unsigned int* error, cudaStream_t stream) {
     if (n_seqs <= 0) return 0;
     if (dtype != PB_F32 && dtype != PB_BF16) return PB_ERR_BAD_DTYPE;
     if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || D <= 0 || D % 16 || D > 256 || page_size <= 0 || table_stride <= 0) return PB_ERR_BAD_SIZE;
     if (n_families < 0 || most_members < 0 || n_members < 0 || n_own <= 0 || n_shared < 0 || (n_families > 0 && n_shared == 0)) return PB_ERR_BAD_SIZE;
-    if (Hkv > 65535 || n_shared + n_own > 256 || (long long)n_seqs * Hq > 0x7fffffff) return PB_ERR_TOO_LARGE;
+    if (Hkv > 65535 || n_shared + n_own > 64 || (long long)n_seqs * Hq > 0x7fffffff) return PB_ERR_TOO_LARGE;
     const int G = Hq / Hkv;
     Shared p{block_table, kv_len, shared_len, members, family_start, n_seqs, n_members, n_families, most_members, table_stride, Hq, Hkv, page_size, n_shared, n_own,
              scale * kLog2e};
     int rc;
-    if (tc_takes(dtype, D, page_size))
-        rc = D == 64 ? launch_tc<64>(q, k_pool, v_pool, partial, p, G, stream) : launch_tc<128>(q, k_pool, v_pool, partial, p, G, stream);
+    if ((((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out | (uintptr_t)partial) & 15) != 0) return PB_ERR_BAD_SIZE;
+    if (tc_takes(dtype, D, page_size) && n_pages > 0 && error != nullptr)
+        rc = D == 64 ? launch_tc<64>(q, k_pool, v_pool, partial, p, G, n_pages, error, stream) : launch_tc<128>(q, k_pool, v_pool, partial, p, G, n_pages, error, stream);
     else if (dtype == PB_F32)
         rc = D <= 128 ? launch_general<float, 1>(q, k_pool, v_pool, partial, p, D, G, stream) : launch_general<float, 2>(q, k_pool, v_pool, partial, p, D, G, stream);
     else
@@ -497,4 +638,9 @@ PB_EXPORT int pb_paged_attention_shared(int dtype, const void* q, const void* k_
     const int rows = n_seqs * Hq, blocks = (rows + kThreads / 32 - 1) / (kThreads / 32);
     if (dtype == PB_F32) return launch_pdl(shared_join_kernel<float>, dim3(blocks), dim3(kThreads), 0, stream, partial, (float*)out, shared_len, rows, Hq, D, n_shared, n_own);
     return launch_pdl(shared_join_kernel<bf16>, dim3(blocks), dim3(kThreads), 0, stream, partial, (bf16*)out, shared_len, rows, Hq, D, n_shared, n_own);
+}
+
+// A new limit of this kernel's bounded waits in clock cycles.
+PB_EXPORT int pb_shared_wait_limit(long long limit) {
+    return limit > 0 && cudaMemcpyToSymbol(g_wait_limit, &limit, sizeof(limit)) == cudaSuccess ? 0 : -1;
 }

@@ -141,7 +141,8 @@ _SIGNATURES = {
     "pb_matrix_memory": [_I, _P, _L, _P, _P, _F, _P, _F, _F, _F, _P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "pb_state_space": [_I, _P, _L, _P, _P, _I, _P, _P, _P, _P, _I, _F, _P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "pb_copy_pages": [_I, _P, _P, _P, _P, _P, _I, _P],
-    "pb_paged_attention_shared": [_I] + [_P] * 6 + [_I] + [_P] * 4 + [_I] * 8 + [_F, _I, _I, _P],
+    "pb_paged_attention_shared": [_I] + [_P] * 6 + [_I] + [_P] * 4 + [_I] * 8 + [_F, _I, _I, _I, _P, _P],
+    "pb_shared_wait_limit": [ctypes.c_longlong],
     "pb_shared_rows": [_I, _I, _I, _I],
     "pb_head_scores_supported": [_I, _I, _I],
     "pb_head_scores_scratch": [_I, _I],
@@ -698,7 +699,7 @@ def set_wait_limit(cycles: int) -> None:
     if fn("pb_gemm_tcgen05_wait_control")(int(cycles), -1, None) != 0 or \
             fn("pb_prefill_tcgen05_wait_control")(int(cycles), -1, None) != 0 or \
             fn("pb_gemm_tcgen05_stream_wait_control")(int(cycles), -1, None) != 0 or \
-            fn("pb_head_scores_wait_limit")(int(cycles)) != 0:
+            fn("pb_head_scores_wait_limit")(int(cycles)) != 0 or fn("pb_shared_wait_limit")(int(cycles)) != 0:
         raise KernelError("the wait limit could not be set")
 
 
@@ -2024,6 +2025,8 @@ def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     [pages, Hkv, page, D], ``block_table`` [S, width], ``kv_len`` [S].  Family f is the sequences ``members[family_start[f]:family_start[f + 1]]``;
     they all have the same pages for their first ``shared_len[s]`` keys (whole pages, at most ``kv_len[s]``), which are read once for all
     of them.  A sequence in no family has ``shared_len`` 0; one with ``kv_len`` 0 gets zeros.  All arrays int32 on the device.
+    (bfloat16 with pages of 8, 16, 32 or 64 keys and heads of 64 or 128 runs on the tensor cores; a wait that it gives up is reported in
+    the tcgen05 attention's error word.)
     ``most_members`` and ``most_shared`` are the largest family's size and the longest shared length as the host knows them (more members
     than that are not served).  ``partial``: float32 scratch of ``shared_scratch`` elements, made here where it is not given."""
     _cuda(q, k_pool, v_pool, out, block_table, kv_len, shared_len, members, family_start, partial)
@@ -2049,16 +2052,18 @@ def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     kind = code(q.dtype)
     if s == 0:
         return
+    if (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr() | out.data_ptr()) % 16:
+        raise KernelError("paged_attention_shared: q, out and the pools must start at a multiple of 16 bytes")
     families = family_start.numel() - 1 if most_members > 0 and most_shared > 0 else 0
     n_shared, n_own = shared_cut(s, families, int(most_members), int(most_shared), block_table.shape[1] * page_size, hq, hkv, d, page_size, q.dtype)
     need = s * hq * (n_shared + n_own) * (d + 2)
     if partial is None:
         partial = torch.empty(need, dtype=torch.float32, device=q.device)
-    elif partial.dtype != torch.float32 or partial.numel() < need:
-        raise KernelError(f"paged_attention_shared: partial must be float32 of at least {need} elements, found {partial.numel()} of {partial.dtype}")
+    elif partial.dtype != torch.float32 or partial.numel() < need or partial.data_ptr() % 16:
+        raise KernelError(f"paged_attention_shared: partial must be float32 of at least {need} elements at a multiple of 16 bytes, found {partial.numel()} of {partial.dtype}")
     check(fn("pb_paged_attention_shared")(kind, _p(q), _p(k_pool), _p(v_pool), _p(out), _p(partial), _p(block_table), block_table.shape[1], _p(kv_len),
                                           _p(shared_len), _p(members), _p(family_start), s, members.numel(), families, int(most_members), hq, hkv, d,
-                                          page_size, float(scale), n_shared, n_own, stream()), "paged_attention_shared", kernels=2)
+                                          page_size, float(scale), n_shared, n_own, k_pool.shape[0], wait_word_addresses()[1], stream()), "paged_attention_shared", kernels=2)
 
 
 @functools.lru_cache(maxsize=1024)
