@@ -9,6 +9,7 @@
 // Bytes bound it: a key and a value of the shared part are read once per kv head and row tile, whatever the number of members.
 //
 // partial [n_seqs * Hq][n_shared + n_own][D + 2] float32: a part's o, then m (in units of log2) and l.
+#include "attention_shared.cuh"
 #include "mma_common.cuh"
 #include "tcgen05_common.cuh"
 
@@ -16,81 +17,7 @@ namespace {
 
 using namespace pb;
 
-// 2^x by the special-function unit alone; results below 2^-126 are 0.
-__device__ __forceinline__ float pow2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-struct Shared {
-    const int* block_table;
-    const int* kv_len;          // [n_seqs]
-    const int* shared_len;      // [n_seqs]: keys [0, shared_len) are read with the family; 0: no family
-    const int* members;         // the families' sequences, one family behind the other
-    const int* family_start;    // [n_families + 1]
-    int n_seqs, n_members, n_families, most_members;
-    int table_stride;
-    int Hq, Hkv, page_size;
-    int n_shared, n_own;        // splits of either side
-    float scale_log2;
-};
-
-// What a block works on: keys [begin, end) read through `table`, and `rows` query rows from row `row0` of its family or sequence on.
-struct Item {
-    const int* table;
-    int begin, end, rows, row0, first_member, seq, part;
-
-    // row i of the item: its sequence and head
-    __device__ __forceinline__ int seq_of(const Shared& p, int i, int G) const {
-        return seq >= 0 ? seq : p.members[first_member + (row0 + i) / G];
-    }
-    __device__ __forceinline__ int head_of(int kvh, int i, int G) const { return kvh * G + (row0 + i) % G; }
-};
-
-// Split `split` of `splits` of the keys from it.begin on, never beyond the table.
-template <int TILE>
-__device__ __forceinline__ void cut(const Shared& p, Item& it, int keys, int split, int splits) {
-    keys = max(0, min(keys, p.table_stride * p.page_size - it.begin));
-    int chunk = (keys + splits - 1) / splits;
-    chunk = (chunk + TILE - 1) / TILE * TILE;
-    const int end = it.begin + keys;
-    it.begin = min(end, it.begin + split * chunk);
-    it.end = min(end, it.begin + chunk);
-}
-// Block `block` of the shared sides.  False: nothing to do.
-template <int ROWS, int TILE>
-__device__ __forceinline__ bool family_item(const Shared& p, int block, int G, Item& it) {
-    const int tiles = (p.most_members * G + ROWS - 1) / ROWS;
-    const int split = block % p.n_shared, tile = block / p.n_shared % tiles, family = block / p.n_shared / tiles;
-    it.first_member = p.family_start[family];
-    const int count = min(min(p.family_start[family + 1], p.n_members) - it.first_member, p.most_members);
-    if (it.first_member < 0 || count <= 0) return false;
-    it.row0 = tile * ROWS;
-    it.rows = min(ROWS, count * G - it.row0);
-    if (it.rows <= 0) return false;
-    const int first = p.members[it.first_member];
-    if (first < 0 || first >= p.n_seqs) return false;
-    it.table = p.block_table + (size_t)first * p.table_stride;
-    it.begin = 0;
-    it.seq = -1;
-    it.part = split;
-    cut<TILE>(p, it, p.shared_len[first], split, p.n_shared);
-    return true;
-}
-// Block `block` of the sequences' own sides.
-template <int ROWS, int TILE>
-__device__ __forceinline__ void own_item(const Shared& p, int block, int G, Item& it) {
-    const int tiles = (G + ROWS - 1) / ROWS, split = block % p.n_own;
-    it.seq = block / p.n_own / tiles;
-    it.row0 = block / p.n_own % tiles * ROWS;
-    it.rows = min(ROWS, G - it.row0);
-    it.first_member = 0;
-    it.table = p.block_table + (size_t)it.seq * p.table_stride;
-    it.begin = p.shared_len[it.seq];
-    it.part = p.n_shared + split;
-    cut<TILE>(p, it, p.kv_len[it.seq] - it.begin, split, p.n_own);
-}
+using namespace pb::shared_attention;
 
 // ---------------------------------------------------------------------------------------------
 // Any head size that is a multiple of 16 (up to 256), any page size, float32 or bfloat16, on the CUDA cores in float32.  Four warps take
@@ -216,8 +143,8 @@ shared_general_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, con
 
 // ---------------------------------------------------------------------------------------------
 // bfloat16, head size 64 or 128, pages of 8, 16, 32 or 64 keys: on the tensor cores (mma.m16n8k16, float32 sums).  Tiles of 64 keys and
-// values come page by page through TMA (boxes of a page x 64 dimensions, 128-byte swizzle) into a ring of 96 KB that a warp of its own
-// fills, two blocks an SM: what limits the kernel is bytes in flight, and instructions that gather a tile would cost the other warps as
+// values come page by page through TMA (boxes of a page x 64 dimensions, 128-byte swizzle) into a ring that a warp of its own fills,
+// two or three blocks an SM: what limits the kernel is bytes in flight, and instructions that gather a tile would cost the other warps as
 // much as its products (cp.async by all warps: 2,300 cycles a tile and block, 77 against 48 us for 101 sequences).  ROW_TILES x 16 query
 // rows meet each tile; the four warps share the work as ROW_TILES row tiles x 4 / ROW_TILES parts of the tile's keys: with one row tile (a
 // sequence's own keys) each warp has 16 keys, with four each has all 64 for its own rows, so that shared memory is read no more often than
@@ -227,9 +154,10 @@ shared_general_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, con
 // are overwritten with zeros, for zero weights do not silence a NaN.  Every wait is bounded; a block that gives up sets the error
 // word, lets its copies land and returns.
 constexpr int kTile = 64, kWarps = 4, kTcThreads = (kWarps + 1) * 32;
-constexpr int kRing = 96 * 1024;
+// Blocks of one row tile (a sequence's own keys: short walks, whose starts and ends others have to hide) run three to an SM, others two.
+template <int ROW_TILES> constexpr int kBlocks = ROW_TILES == 1 ? 3 : 2;
+template <int ROW_TILES> constexpr int kRing = (ROW_TILES == 1 ? 64 : 96) * 1024;
 template <int D> constexpr int kTileBytes = kTile * D * 2;                    // of keys, and of values
-template <int D> constexpr int kStages = kRing / (2 * kTileBytes<D>);
 
 // Byte offset of 16-byte chunk `chunk` of row `row` in a tile: halves of 64 dimensions, rows of 128 bytes, swizzled as TMA leaves them.
 __device__ __forceinline__ uint32_t tma_offset(int row, int chunk) {
@@ -243,19 +171,19 @@ struct Ring {
 };
 
 // The warp that fills the ring: a lane per page of a tile.
-template <int D>
-__device__ __forceinline__ void fill(const CUtensorMap* map_k, const CUtensorMap* map_v, const Shared& p, const Item& it, int tile0, int n_tiles, int kvh,
+template <int D, int STAGES>
+__device__ __forceinline__ void fill(const CUtensorMap* map_k, const CUtensorMap* map_v, const Shared& p, const Item& it, int n_tiles, int kvh,
                                      int page_shift, const PoolBounds& bounds, uint32_t ring, Ring& sync, unsigned int* error) {
     const int lane = threadIdx.x & 31;
     for (int i = 0; i < n_tiles; ++i) {
-        const int stage = i % kStages<D>, key0 = (tile0 + i) * kTile;
-        const int first = max(it.begin, key0) >> page_shift, last = (min(it.end, key0 + kTile) - 1) >> page_shift;      // pages of the tile
+        const int stage = i % STAGES, key0 = it.begin + i * kTile;                // (an item begins with a page)
+        const int first = key0 >> page_shift, last = (min(it.end, key0 + kTile) - 1) >> page_shift;      // pages of the tile
         int page = first + lane <= last ? it.table[first + lane] : 0;
         if (!page_ok(page, bounds)) page = 0;
         const uint32_t full = smem_addr(&sync.full[stage]);
         bool ok = true;
         if (lane == 0) {
-            ok = mbar_wait(smem_addr(&sync.empty[stage]), ((i / kStages<D>)&1) ^ 1, &sync.gave_up);
+            ok = mbar_wait(smem_addr(&sync.empty[stage]), ((i / STAGES) & 1) ^ 1, &sync.gave_up);
             if (ok) mbar_expect_tx(full, (uint32_t)((last - first + 1) << page_shift) * D * 4);
         }
         if (!__shfl_sync(0xffffffffu, (int)ok, 0)) {
@@ -263,7 +191,7 @@ __device__ __forceinline__ void fill(const CUtensorMap* map_k, const CUtensorMap
             return;
         }
         if (first + lane <= last) {
-            const uint32_t dst = ring + stage * 2 * kTileBytes<D> + (((first + lane) << page_shift) - key0) * 128;
+            const uint32_t dst = ring + stage * 2 * kTileBytes<D> + (lane << page_shift) * 128;
             const int row = (page * p.Hkv + kvh) << page_shift;
 #pragma unroll
             for (int half = 0; half < D / 64; ++half) {
@@ -275,7 +203,7 @@ __device__ __forceinline__ void fill(const CUtensorMap* map_k, const CUtensorMap
     }
 }
 
-template <int D, int ROW_TILES>
+template <int D, int ROW_TILES, int STAGES>
 __device__ __forceinline__ void attend(const bf16* __restrict__ q, const CUtensorMap* map_k, const CUtensorMap* map_v, float* __restrict__ partial,
                                        const Shared& p, const Item& it, int kvh, int page_shift, const PoolBounds& bounds, unsigned char* smem,
                                        Ring& sync, unsigned int* error) {
@@ -284,11 +212,11 @@ __device__ __forceinline__ void attend(const bf16* __restrict__ q, const CUtenso
     const uint32_t ring = smem_addr(smem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int row_tile = warp % ROW_TILES, key_part = warp / ROW_TILES;
-    const int tile0 = it.begin / kTile, n_tiles = it.begin < it.end ? (it.end - 1) / kTile - tile0 + 1 : 0;
+    const int n_tiles = (it.end - it.begin + kTile - 1) / kTile;
     float o[kNTiles][4];
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
     if (warp == kWarps) {
-        fill<D>(map_k, map_v, p, it, tile0, n_tiles, kvh, page_shift, bounds, ring, sync, error);
+        fill<D, STAGES>(map_k, map_v, p, it, n_tiles, kvh, page_shift, bounds, ring, sync, error);
     } else {
         // the warp's query rows: row_tile * 16 + g and + 8
         uint32_t qa[kKSteps][4];
@@ -307,21 +235,21 @@ __device__ __forceinline__ void attend(const bf16* __restrict__ q, const CUtenso
         const bool has_rows = row_tile * 16 < it.rows;
 
         for (int i = 0; i < n_tiles; ++i) {
-            const int stage = i % kStages<D>;
-            if (!mbar_wait(smem_addr(&sync.full[stage]), (i / kStages<D>)&1, &sync.gave_up)) {
+            const int stage = i % STAGES;
+            if (!mbar_wait(smem_addr(&sync.full[stage]), (i / STAGES) & 1, &sync.gave_up)) {
                 if (lane == 0) { *(volatile int*)&sync.gave_up = 1; atomicMax(error, 4u); }
                 break;
             }
             __syncwarp();
             const uint32_t k_s = ring + stage * 2 * kTileBytes<D>, v_s = k_s + kTileBytes<D>;
-            const int in_tile = key_part * kGroups * 16, key0 = (tile0 + i) * kTile + in_tile;
-            if (has_rows && key0 < it.end && key0 + kGroups * 16 > it.begin) {
-                const bool inside = key0 >= it.begin && key0 + kGroups * 16 <= it.end;
+            const int in_tile = key_part * kGroups * 16, key0 = it.begin + i * kTile + in_tile;
+            if (has_rows && key0 < it.end) {
+                const bool inside = key0 + kGroups * 16 <= it.end;
                 if (!inside) {
                     // values of rows without a key become zeros (warps with the same rows write the same)
                     for (int c = lane; c < kGroups * 16 * (D / 8); c += 32) {
-                        const int row = c / (D / 8), key = key0 + row;
-                        if (key < it.begin || key >= it.end)
+                        const int row = c / (D / 8);
+                        if (key0 + row >= it.end)
                             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_s + tma_offset(in_tile + row, c % (D / 8))), "r"(0) : "memory");
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");          // before TMA fills the stage again
@@ -345,7 +273,7 @@ __device__ __forceinline__ void attend(const bf16* __restrict__ q, const CUtenso
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int key = key0 + n * 8 + 2 * t + (e & 1);
-                        s[n][e] = inside || (key >= it.begin && key < it.end) ? s[n][e] * p.scale_log2 : -INFINITY;
+                        s[n][e] = inside || key < it.end ? s[n][e] * p.scale_log2 : -INFINITY;
                         top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
                     }
                 float f[2], base[2];
@@ -452,14 +380,16 @@ __device__ __forceinline__ void attend(const bf16* __restrict__ q, const CUtenso
     }
 }
 
-// ROW_TILES: of the shared sides' blocks; a sequence's own keys meet tiles of 16 rows.
+// ROW_TILES: of the shared sides' blocks; a sequence's own keys meet tiles of 16 rows.  beside: the kernel before it on the stream has the
+// shared sides; it was launched the ordinary way, lets this one in at its start, and the two write different parts.
 template <int D, int ROW_TILES>
-__global__ void __launch_bounds__(kTcThreads, 2)
+__global__ void __launch_bounds__(kTcThreads, kBlocks<ROW_TILES>)
 shared_tc_kernel(const bf16* __restrict__ q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                 float* __restrict__ partial, const Shared p, int shared_blocks, int page_shift, const PoolBounds bounds, unsigned int* error) {
+                 float* __restrict__ partial, const Shared p, int shared_blocks, int page_shift, const PoolBounds bounds, unsigned int* error, bool beside) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ Ring sync;
+    constexpr int kStages = kRing<ROW_TILES> / (2 * kTileBytes<D>);
     pdl_trigger();                                                                // (the join waits for this kernel's end)
     const int G = p.Hq / p.Hkv, tid = threadIdx.x;
     const bool family = (int)blockIdx.x < shared_blocks;
@@ -470,7 +400,7 @@ shared_tc_kernel(const bf16* __restrict__ q, const __grid_constant__ CUtensorMap
         own_item<16, kTile>(p, blockIdx.x - shared_blocks, G, it);
     }
     if (tid == kWarps * 32) {
-        for (int i = 0; i < kStages<D>; ++i) {
+        for (int i = 0; i < kStages; ++i) {
             mbar_init(smem_addr(&sync.full[i]), 1);
             mbar_init(smem_addr(&sync.empty[i]), kWarps);
         }
@@ -485,8 +415,10 @@ shared_tc_kernel(const bf16* __restrict__ q, const __grid_constant__ CUtensorMap
         sync.rows[tid] = row;
     }
     __syncthreads();
-    if (family) attend<D, ROW_TILES>(q, &map_k, &map_v, partial, p, it, blockIdx.y, page_shift, bounds, smem, sync, error);
-    else attend<D, 1>(q, &map_k, &map_v, partial, p, it, blockIdx.y, page_shift, bounds, smem, sync, error);
+    if (family) attend<D, ROW_TILES, kStages>(q, &map_k, &map_v, partial, p, it, blockIdx.y, page_shift, bounds, smem, sync, error);
+    else attend<D, 1, kStages>(q, &map_k, &map_v, partial, p, it, blockIdx.y, page_shift, bounds, smem, sync, error);
+    // complete no sooner than the kernel it ran beside: the last block alone waits, the others leave their places to those behind them
+    if (beside && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1) pdl_wait();
 }
 
 // Joins a row's parts: a warp per row, a lane per part for their weights and per four dimensions for the sums.  A sequence outside
@@ -576,18 +508,25 @@ struct Maps {
 };
 
 template <int D, int ROW_TILES>
-int launch_tc(const void* q, const Maps& maps, float* partial, const Shared& p, int G, cudaStream_t stream) {
+int launch_tc(const void* q, const Maps& maps, float* partial, const Shared& p, int G, bool beside, cudaStream_t stream) {
     const Grid grid = grid_of(p, G, ROW_TILES * 16, 16);
     if (grid.all == 0) return PB_ERR_TOO_LARGE;
-    constexpr int smem = kRing + 1024;
+    constexpr int smem = kRing<ROW_TILES> + 1024;
     static SmemLimit limit;
+    static DeviceLimit most;
     if (const int rc = limit.allow(shared_tc_kernel<D, ROW_TILES>, smem)) return rc;
-    shared_tc_kernel<D, ROW_TILES><<<dim3(grid.all, p.Hkv), kTcThreads, smem, stream>>>((const bf16*)q, maps.k, maps.v, partial, p, grid.shared,
-                                                                                        log2_exact(p.page_size), pool_bounds_now(), maps.error);
-    return launch_status();
+    if (const int rc = share_most(most, shared_tc_kernel<D, ROW_TILES>)) return rc;
+    return launch_early(beside, shared_tc_kernel<D, ROW_TILES>, dim3(grid.all, p.Hkv), dim3(kTcThreads), smem, stream, (const bf16*)q, maps.k, maps.v, partial, p,
+                        grid.shared, log2_exact(p.page_size), pool_bounds_now(), maps.error, beside);
 }
-template <int D>
-int launch_tc(const void* q, const void* k_pool, const void* v_pool, float* partial, const Shared& p, int G, int n_pages, unsigned int* error, cudaStream_t stream) {
+
+// Families of up to 16 rows meet their keys as a sequence its own.  Beyond that heads of 128 take the tcgen05 kernel for the shared sides
+// (8 members of 4 heads: 13 against 21 us in all, 64 members: 26 against 104), which takes no other; heads of 64 as many row tiles as the
+// largest family fills.
+bool tcgen05_takes(int rows, int D) { return D == 128 && rows > 16; }
+
+int launch_tc(const void* q, const void* k_pool, const void* v_pool, float* partial, Shared p, int G, int D, int n_pages, unsigned int* error,
+              cudaStream_t stream) {
     Maps maps;
     maps.error = error;
     const long long pool_rows = (long long)n_pages * p.Hkv * p.page_size;
@@ -595,10 +534,17 @@ int launch_tc(const void* q, const void* k_pool, const void* v_pool, float* part
     int rc = make_map(&maps.k, k_pool, pool_rows, D, p.page_size);
     if (rc == 0) rc = make_map(&maps.v, v_pool, pool_rows, D, p.page_size);
     if (rc != 0) return rc;
-    const int rows = p.most_members * G;                  // as many row tiles as the largest family fills
-    if (rows <= 16) return launch_tc<D, 1>(q, maps, partial, p, G, stream);
-    if (rows <= 32) return launch_tc<D, 2>(q, maps, partial, p, G, stream);
-    return launch_tc<D, 4>(q, maps, partial, p, G, stream);
+    const int rows = p.n_families > 0 ? p.most_members * G : 0;
+    if (tcgen05_takes(rows, D)) {
+        rc = launch_tcgen05(q, k_pool, v_pool, partial, p, n_pages, error, stream);
+        if (rc != 0) return rc;
+        p.n_families = 0;                                 // (n_shared stays: it is where a sequence's own parts begin)
+        return launch_tc<128, 1>(q, maps, partial, p, G, true, stream);
+    }
+    if (D == 128) return launch_tc<128, 1>(q, maps, partial, p, G, false, stream);
+    if (rows <= 16) return launch_tc<64, 1>(q, maps, partial, p, G, false, stream);
+    if (rows <= 32) return launch_tc<64, 2>(q, maps, partial, p, G, false, stream);
+    return launch_tc<64, 4>(q, maps, partial, p, G, false, stream);
 }
 
 bool tc_takes(int dtype, int D, int page_size) {
@@ -608,7 +554,10 @@ bool tc_takes(int dtype, int D, int page_size) {
 }  // namespace
 
 // Query rows that a block of the shared sides works on: what the caller cuts the keys by.
-PB_EXPORT int pb_shared_rows(int dtype, int rows, int D, int page_size) { return !tc_takes(dtype, D, page_size) ? kRows : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+PB_EXPORT int pb_shared_rows(int dtype, int rows, int D, int page_size) {
+    if (!tc_takes(dtype, D, page_size)) return kRows;
+    return tcgen05_takes(rows, D) ? kTcgen05Rows : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+}
 
 // q, out [n_seqs, Hq, D], pools [pages, Hkv, page_size, D] (dtype 0 float32, 1 bfloat16); block_table int32 [n_seqs, table_stride];
 // kv_len, shared_len int32 [n_seqs]; members int32 [n_members], family_start int32 [n_families + 1]; partial float32
@@ -629,7 +578,7 @@ PB_EXPORT int pb_paged_attention_shared(int dtype, const void* q, const void* k_
     int rc;
     if ((((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out | (uintptr_t)partial) & 15) != 0) return PB_ERR_BAD_SIZE;
     if (tc_takes(dtype, D, page_size) && n_pages > 0 && error != nullptr)
-        rc = D == 64 ? launch_tc<64>(q, k_pool, v_pool, partial, p, G, n_pages, error, stream) : launch_tc<128>(q, k_pool, v_pool, partial, p, G, n_pages, error, stream);
+        rc = launch_tc(q, k_pool, v_pool, partial, p, G, D, n_pages, error, stream);
     else if (dtype == PB_F32)
         rc = D <= 128 ? launch_general<float, 1>(q, k_pool, v_pool, partial, p, D, G, stream) : launch_general<float, 2>(q, k_pool, v_pool, partial, p, D, G, stream);
     else

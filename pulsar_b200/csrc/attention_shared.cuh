@@ -1,0 +1,102 @@
+// What the kernels of the attention over shared pages have in common: the call's arrays, and the piece of work that a block finds in them.
+#pragma once
+
+#include "common.cuh"
+
+namespace pb {
+namespace shared_attention {
+
+// 2^x by the special-function unit alone; results below 2^-126 are 0.
+__device__ __forceinline__ float pow2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+struct Shared {
+    const int* block_table;
+    const int* kv_len;          // [n_seqs]
+    const int* shared_len;      // [n_seqs]: keys [0, shared_len) are read with the family; 0: no family
+    const int* members;         // the families' sequences, one family behind the other
+    const int* family_start;    // [n_families + 1]
+    int n_seqs, n_members, n_families, most_members;
+    int table_stride;
+    int Hq, Hkv, page_size;
+    int n_shared, n_own;        // splits of either side
+    float scale_log2;
+};
+
+// What a block works on: keys [begin, end) read through `table`, and `rows` query rows from row `row0` of its family or sequence on.
+struct Item {
+    const int* table;
+    int begin, end, rows, row0, first_member, seq, part;
+
+    // row i of the item: its sequence and head
+    __device__ __forceinline__ int seq_of(const Shared& p, int i, int G) const {
+        return seq >= 0 ? seq : p.members[first_member + (row0 + i) / G];
+    }
+    __device__ __forceinline__ int head_of(int kvh, int i, int G) const { return kvh * G + (row0 + i) % G; }
+};
+
+// Split `split` of `splits` of the keys from it.begin on, never beyond the table.
+template <int TILE>
+__device__ __forceinline__ void cut(const Shared& p, Item& it, int keys, int split, int splits) {
+    keys = max(0, min(keys, p.table_stride * p.page_size - it.begin));
+    int chunk = (keys + splits - 1) / splits;
+    chunk = (chunk + TILE - 1) / TILE * TILE;
+    const int end = it.begin + keys;
+    it.begin = min(end, it.begin + split * chunk);
+    it.end = min(end, it.begin + chunk);
+}
+// Block `block` of the shared sides.  False: nothing to do.
+template <int ROWS, int TILE>
+__device__ __forceinline__ bool family_item(const Shared& p, int block, int G, Item& it) {
+    const int tiles = (p.most_members * G + ROWS - 1) / ROWS;
+    const int split = block % p.n_shared, tile = block / p.n_shared % tiles, family = block / p.n_shared / tiles;
+    it.first_member = p.family_start[family];
+    const int count = min(min(p.family_start[family + 1], p.n_members) - it.first_member, p.most_members);
+    if (it.first_member < 0 || count <= 0) return false;
+    it.row0 = tile * ROWS;
+    it.rows = min(ROWS, count * G - it.row0);
+    if (it.rows <= 0) return false;
+    const int first = p.members[it.first_member];
+    if (first < 0 || first >= p.n_seqs) return false;
+    it.table = p.block_table + (size_t)first * p.table_stride;
+    it.begin = 0;
+    it.seq = -1;
+    it.part = split;
+    cut<TILE>(p, it, p.shared_len[first], split, p.n_shared);
+    return true;
+}
+// Block `block` of the sequences' own sides.
+template <int ROWS, int TILE>
+__device__ __forceinline__ void own_item(const Shared& p, int block, int G, Item& it) {
+    const int tiles = (G + ROWS - 1) / ROWS, split = block % p.n_own;
+    it.seq = block / p.n_own / tiles;
+    it.row0 = block / p.n_own % tiles * ROWS;
+    it.rows = min(ROWS, G - it.row0);
+    it.first_member = 0;
+    it.table = p.block_table + (size_t)it.seq * p.table_stride;
+    it.begin = max(0, p.shared_len[it.seq]) / p.page_size * p.page_size;      // (whole pages already, unless the caller erred)
+    it.part = p.n_shared + split;
+    cut<TILE>(p, it, p.kv_len[it.seq] - it.begin, split, p.n_own);
+}
+
+// Lets an SM that runs `kernel` have as much of its memory shared as can be, so that a block of another kernel finds room beside it (once per device).
+template <typename... KArgs>
+int share_most(DeviceLimit& done, void (*kernel)(KArgs...)) {
+    return done.allow(1, [](int* dev) { return (int)cudaGetDevice(dev); }, [&](size_t) {
+        return (int)cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    });
+}
+
+// Blocks of the shared sides.
+inline long long family_blocks(const Shared& p, int G, int rows) { return (long long)p.n_families * ((p.most_members * G + rows - 1) / rows) * p.n_shared; }
+
+// The shared sides on the fifth-generation tensor cores (attention_shared_tcgen05.cu): head size 128, pages of 8 to 64 keys.
+constexpr int kTcgen05Rows = 128;
+int launch_tcgen05(const void* q, const void* k_pool, const void* v_pool, float* partial, const Shared& p, int n_pages, unsigned int* error,
+                   cudaStream_t stream);
+
+}  // namespace shared_attention
+}  // namespace pb

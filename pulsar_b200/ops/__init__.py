@@ -143,6 +143,7 @@ _SIGNATURES = {
     "pb_copy_pages": [_I, _P, _P, _P, _P, _P, _I, _P],
     "pb_paged_attention_shared": [_I] + [_P] * 6 + [_I] + [_P] * 4 + [_I] * 8 + [_F, _I, _I, _I, _P, _P],
     "pb_shared_wait_limit": [ctypes.c_longlong],
+    "pb_shared_tcgen05_wait_limit": [ctypes.c_longlong],
     "pb_shared_rows": [_I, _I, _I, _I],
     "pb_head_scores_supported": [_I, _I, _I],
     "pb_head_scores_scratch": [_I, _I],
@@ -699,7 +700,8 @@ def set_wait_limit(cycles: int) -> None:
     if fn("pb_gemm_tcgen05_wait_control")(int(cycles), -1, None) != 0 or \
             fn("pb_prefill_tcgen05_wait_control")(int(cycles), -1, None) != 0 or \
             fn("pb_gemm_tcgen05_stream_wait_control")(int(cycles), -1, None) != 0 or \
-            fn("pb_head_scores_wait_limit")(int(cycles)) != 0 or fn("pb_shared_wait_limit")(int(cycles)) != 0:
+            fn("pb_head_scores_wait_limit")(int(cycles)) != 0 or fn("pb_shared_wait_limit")(int(cycles)) != 0 or \
+            fn("pb_shared_tcgen05_wait_limit")(int(cycles)) != 0:
         raise KernelError("the wait limit could not be set")
 
 
@@ -2074,7 +2076,10 @@ def shared_cut(n_seqs: int, n_families: int, most_members: int, most_shared: int
     rows = most_members * group
     tile = fn("pb_shared_rows")(code(dtype), rows, head_dim, page_size)
     blocks = n_families * -(-rows // tile) * n_kv_heads
-    n_shared = max(1, min(32, most_shared // 256, _DECODE_SLOTS // max(1, blocks))) if n_families else 0
+    # As many parts as the SMs hold at once (one block of the tcgen05 kernel each, two of the others); more blocks than that run in
+    # rounds, and cutting their keys further only makes more of them.
+    slots = _DECODE_SLOTS // 2 if tile == 128 else _DECODE_SLOTS
+    n_shared = max(1, min(32, most_shared // 256, slots // max(1, blocks))) if n_families else 0
     own_blocks = n_seqs * -(-group // 16) * n_kv_heads
     n_own = max(1, min(32, (table_tokens - (most_shared if n_families else 0)) // 256, _DECODE_SLOTS // max(1, own_blocks)))
     return n_shared, n_own
