@@ -39,8 +39,8 @@ shared_general_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, con
     const int G = p.Hq / p.Hkv;
     Item it;
     pdl_trigger();                                       // (the join waits for this kernel's end)
-    if ((int)blockIdx.x >= shared_blocks) own_item<kRows, kKeys>(p, blockIdx.x - shared_blocks, G, it);
-    else if (!family_item<kRows, kKeys>(p, blockIdx.x, G, it)) return;
+    if ((int)blockIdx.x >= shared_blocks ? !own_item<kRows>(p, blockIdx.x - shared_blocks, G, it)
+                                         : !family_item<kRows, kKeys>(p, blockIdx.x, G, it)) return;
     const int quads = D / 4;
     for (int i = tid; i < kRows * quads; i += kThreads) {
         const int r = i / quads, d = (i - r * quads) * 4;
@@ -166,30 +166,27 @@ __device__ __forceinline__ uint32_t tma_offset(int row, int chunk) {
 
 struct Ring {
     uint64_t full[8], empty[8];
-    int rows[64];                // the item's query rows: sequence * Hq + head, or -1
     int gave_up;
 };
 
-// The warp that fills the ring: a lane per page of a tile.
+// The warp that fills the ring, a lane per page of a tile.  False: a wait ran out.
 template <int D, int STAGES>
-__device__ __forceinline__ void fill(const CUtensorMap* map_k, const CUtensorMap* map_v, const Shared& p, const Item& it, int n_tiles, int kvh,
-                                     int page_shift, const PoolBounds& bounds, uint32_t ring, Ring& sync, unsigned int* error) {
+__device__ __forceinline__ bool fill(const CUtensorMap* map_k, const CUtensorMap* map_v, const Shared& p, const Item& it, int kvh, int page_shift,
+                                     const PoolBounds& bounds, uint32_t ring, Ring& sync) {
     const int lane = threadIdx.x & 31;
-    for (int i = 0; i < n_tiles; ++i) {
-        const int stage = i % STAGES, key0 = it.begin + i * kTile;                // (an item begins with a page)
+    int at = 0;
+    for (int key0 = it.begin; key0 < it.end; key0 += kTile, ++at) {               // (an item begins with a page)
+        const int stage = at % STAGES;
         const int first = key0 >> page_shift, last = (min(it.end, key0 + kTile) - 1) >> page_shift;      // pages of the tile
         int page = first + lane <= last ? it.table[first + lane] : 0;
         if (!page_ok(page, bounds)) page = 0;
         const uint32_t full = smem_addr(&sync.full[stage]);
         bool ok = true;
         if (lane == 0) {
-            ok = mbar_wait(smem_addr(&sync.empty[stage]), ((i / STAGES) & 1) ^ 1, &sync.gave_up);
+            ok = mbar_wait(smem_addr(&sync.empty[stage]), ((at / STAGES) & 1) ^ 1, &sync.gave_up);
             if (ok) mbar_expect_tx(full, (uint32_t)((last - first + 1) << page_shift) * D * 4);
         }
-        if (!__shfl_sync(0xffffffffu, (int)ok, 0)) {
-            if (lane == 0) { *(volatile int*)&sync.gave_up = 1; atomicMax(error, 2u); }
-            return;
-        }
+        if (!__shfl_sync(0xffffffffu, (int)ok, 0)) return false;
         if (first + lane <= last) {
             const uint32_t dst = ring + stage * 2 * kTileBytes<D> + (lane << page_shift) * 128;
             const int row = (page * p.Hkv + kvh) << page_shift;
@@ -201,237 +198,240 @@ __device__ __forceinline__ void fill(const CUtensorMap* map_k, const CUtensorMap
         }
         __syncwarp();
     }
+    return true;
 }
 
+// The four warps that compute meet here.
+__device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
+
+// The warps that compute.  False: a wait ran out (the warps still meet).
 template <int D, int ROW_TILES, int STAGES>
-__device__ __forceinline__ void attend(const bf16* __restrict__ q, const CUtensorMap* map_k, const CUtensorMap* map_v, float* __restrict__ partial,
-                                       const Shared& p, const Item& it, int kvh, int page_shift, const PoolBounds& bounds, unsigned char* smem,
-                                       Ring& sync, unsigned int* error) {
+__device__ __forceinline__ bool attend(const bf16* __restrict__ q, float* __restrict__ partial, const Shared& p, const Item& it, int kvh, int G, uint32_t ring,
+                                       unsigned char* smem, Ring& sync) {
     constexpr int kKSteps = D / 16, kNTiles = D / 8;
     constexpr int kKeyParts = kWarps / ROW_TILES, kGroups = ROW_TILES;           // groups of 16 keys that a warp has of a tile
-    const uint32_t ring = smem_addr(smem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int row_tile = warp % ROW_TILES, key_part = warp / ROW_TILES;
-    const int n_tiles = (it.end - it.begin + kTile - 1) / kTile;
-    float o[kNTiles][4];
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    if (warp == kWarps) {
-        fill<D, STAGES>(map_k, map_v, p, it, n_tiles, kvh, page_shift, bounds, ring, sync, error);
-    } else {
-        // the warp's query rows: row_tile * 16 + g and + 8
-        uint32_t qa[kKSteps][4];
+    // the warp's query rows: row_tile * 16 + g and + 8, as sequence * Hq + head, or -1
+    int rows[2];
+    uint32_t qa[kKSteps][4];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int row = sync.rows[row_tile * 16 + g + 8 * r];
-            const bf16* from = q + (size_t)max(row, 0) * D + 2 * t;
-#pragma unroll
-            for (int ks = 0; ks < kKSteps; ++ks) {
-                qa[ks][r] = row >= 0 ? *reinterpret_cast<const uint32_t*>(from + ks * 16) : 0u;
-                qa[ks][r + 2] = row >= 0 ? *reinterpret_cast<const uint32_t*>(from + ks * 16 + 8) : 0u;
-            }
+    for (int r = 0; r < 2; ++r) {
+        const int i = row_tile * 16 + g + 8 * r;
+        rows[r] = -1;
+        if (i < it.rows) {
+            const int seq = it.seq_of(p, i, G);
+            if (seq >= 0 && seq < p.n_seqs) rows[r] = seq * p.Hq + it.head_of(kvh, i, G);
         }
+        const bf16* from = q + (size_t)max(rows[r], 0) * D + 2 * t;
 #pragma unroll
-        for (int i = 0; i < kNTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-        const bool has_rows = row_tile * 16 < it.rows;
-
-        for (int i = 0; i < n_tiles; ++i) {
-            const int stage = i % STAGES;
-            if (!mbar_wait(smem_addr(&sync.full[stage]), (i / STAGES) & 1, &sync.gave_up)) {
-                if (lane == 0) { *(volatile int*)&sync.gave_up = 1; atomicMax(error, 4u); }
-                break;
-            }
-            __syncwarp();
-            const uint32_t k_s = ring + stage * 2 * kTileBytes<D>, v_s = k_s + kTileBytes<D>;
-            const int in_tile = key_part * kGroups * 16, key0 = it.begin + i * kTile + in_tile;
-            if (has_rows && key0 < it.end) {
-                const bool inside = key0 + kGroups * 16 <= it.end;
-                if (!inside) {
-                    // values of rows without a key become zeros (warps with the same rows write the same)
-                    for (int c = lane; c < kGroups * 16 * (D / 8); c += 32) {
-                        const int row = c / (D / 8);
-                        if (key0 + row >= it.end)
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_s + tma_offset(in_tile + row, c % (D / 8))), "r"(0) : "memory");
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");          // before TMA fills the stage again
-                    __syncwarp();
-                }
-                float s[2 * kGroups][4];
-#pragma unroll
-                for (int n = 0; n < 2 * kGroups; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-#pragma unroll
-                for (int ks = 0; ks < kKSteps; ++ks)
-#pragma unroll
-                    for (int n = 0; n < kGroups; ++n) {
-                        uint32_t kb[4];
-                        ldmatrix_x4(kb, k_s + tma_offset(in_tile + n * 16 + (lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
-                        mma_bf16(s[2 * n], qa[ks], kb[0], kb[1]);
-                        mma_bf16(s[2 * n + 1], qa[ks], kb[2], kb[3]);
-                    }
-                float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                for (int n = 0; n < 2 * kGroups; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = key0 + n * 8 + 2 * t + (e & 1);
-                        s[n][e] = inside || key < it.end ? s[n][e] * p.scale_log2 : -INFINITY;
-                        top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
-                    }
-                float f[2], base[2];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-                    const float m_new = fmaxf(m[r], top[r]);
-                    base[r] = m_new == -INFINITY ? 0.0f : m_new;                  // scores of -inf alone weigh nothing
-                    f[r] = pow2(m[r] - base[r]);
-                    m[r] = m_new;
-                    l[r] *= f[r];
-                }
-#pragma unroll
-                for (int n = 0; n < 2 * kGroups; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[n][e] = pow2(s[n][e] - base[e >> 1]);
-                        l[e >> 1] += s[n][e];
-                    }
-                if (__any_sync(0xffffffffu, f[0] != 1.0f || f[1] != 1.0f)) {      // a maximum rose, which soon is rare
-#pragma unroll
-                    for (int j = 0; j < kNTiles; ++j) { o[j][0] *= f[0]; o[j][1] *= f[0]; o[j][2] *= f[1]; o[j][3] *= f[1]; }
-                }
-#pragma unroll
-                for (int n = 0; n < kGroups; ++n) {
-                    // weights in [0, 1], rounded to bfloat16 for the product (2^-9 of each); their sum is of the unrounded ones
-                    const uint32_t pa[4] = {pack_bf16(s[2 * n][0], s[2 * n][1]), pack_bf16(s[2 * n][2], s[2 * n][3]),
-                                            pack_bf16(s[2 * n + 1][0], s[2 * n + 1][1]), pack_bf16(s[2 * n + 1][2], s[2 * n + 1][3])};
-#pragma unroll
-                    for (int j = 0; j < kNTiles; j += 2) {
-                        uint32_t vb[4];
-                        ldmatrix_x4_trans(vb, v_s + tma_offset(in_tile + n * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), j + (lane >> 4)));
-                        mma_bf16(o[j], pa, vb[0], vb[1]);
-                        mma_bf16(o[j + 1], pa, vb[2], vb[3]);
-                    }
-                }
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_addr(&sync.empty[stage]));
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        for (int ks = 0; ks < kKSteps; ++ks) {
+            qa[ks][r] = rows[r] >= 0 ? *reinterpret_cast<const uint32_t*>(from + ks * 16) : 0u;
+            qa[ks][r + 2] = rows[r] >= 0 ? *reinterpret_cast<const uint32_t*>(from + ks * 16 + 8) : 0u;
         }
     }
-    __syncthreads();                                                              // all tiles have been read
-    if (*(volatile int*)&sync.gave_up) {
-        for (int i = 0; i < 2000; ++i) __nanosleep(1000);                         // copies in flight land before this block's memory is reused
-        return;
+    float o[kNTiles][4];
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < kNTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+    const bool has_rows = row_tile * 16 < it.rows;
+    bool ok = true;
+    int at = 0;
+    for (int tile0 = it.begin; tile0 < it.end; tile0 += kTile, ++at) {
+        const int stage = at % STAGES;
+        ok = mbar_wait(smem_addr(&sync.full[stage]), (at / STAGES) & 1, &sync.gave_up);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint32_t k_s = ring + stage * 2 * kTileBytes<D>, v_s = k_s + kTileBytes<D>;
+        const int in_tile = key_part * kGroups * 16, key0 = tile0 + in_tile;
+        if (has_rows && key0 < it.end) {
+            const bool inside = key0 + kGroups * 16 <= it.end;
+            if (!inside) {
+                // values of rows without a key become zeros (warps with the same rows write the same)
+                for (int c = lane; c < kGroups * 16 * (D / 8); c += 32) {
+                    const int row = c / (D / 8);
+                    if (key0 + row >= it.end)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_s + tma_offset(in_tile + row, c % (D / 8))), "r"(0) : "memory");
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // before TMA fills the stage again
+                __syncwarp();
+            }
+            float s[2 * kGroups][4];
+#pragma unroll
+            for (int n = 0; n < 2 * kGroups; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < kKSteps; ++ks)
+#pragma unroll
+                for (int n = 0; n < kGroups; ++n) {
+                    uint32_t kb[4];
+                    ldmatrix_x4(kb, k_s + tma_offset(in_tile + n * 16 + (lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
+                    mma_bf16(s[2 * n], qa[ks], kb[0], kb[1]);
+                    mma_bf16(s[2 * n + 1], qa[ks], kb[2], kb[3]);
+                }
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int n = 0; n < 2 * kGroups; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int key = key0 + n * 8 + 2 * t + (e & 1);
+                    s[n][e] = inside || key < it.end ? s[n][e] * p.scale_log2 : -INFINITY;
+                    top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+                }
+            float f[2], base[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                const float m_new = fmaxf(m[r], top[r]);
+                base[r] = m_new == -INFINITY ? 0.0f : m_new;                      // scores of -inf alone weigh nothing
+                f[r] = pow2(m[r] - base[r]);
+                m[r] = m_new;
+                l[r] *= f[r];
+            }
+#pragma unroll
+            for (int n = 0; n < 2 * kGroups; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[n][e] = pow2(s[n][e] - base[e >> 1]);
+                    l[e >> 1] += s[n][e];
+                }
+            if (__any_sync(0xffffffffu, f[0] != 1.0f || f[1] != 1.0f)) {          // a maximum rose, which soon is rare
+#pragma unroll
+                for (int j = 0; j < kNTiles; ++j) { o[j][0] *= f[0]; o[j][1] *= f[0]; o[j][2] *= f[1]; o[j][3] *= f[1]; }
+            }
+#pragma unroll
+            for (int n = 0; n < kGroups; ++n) {
+                // weights in [0, 1], rounded to bfloat16 for the product (2^-9 of each); their sum is of the unrounded ones
+                const uint32_t pa[4] = {pack_bf16(s[2 * n][0], s[2 * n][1]), pack_bf16(s[2 * n][2], s[2 * n][3]),
+                                        pack_bf16(s[2 * n + 1][0], s[2 * n + 1][1]), pack_bf16(s[2 * n + 1][2], s[2 * n + 1][3])};
+#pragma unroll
+                for (int j = 0; j < kNTiles; j += 2) {
+                    uint32_t vb[4];
+                    ldmatrix_x4_trans(vb, v_s + tma_offset(in_tile + n * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), j + (lane >> 4)));
+                    mma_bf16(o[j], pa, vb[0], vb[1]);
+                    mma_bf16(o[j + 1], pa, vb[2], vb[3]);
+                }
+            }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&sync.empty[stage]));
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }
     const int stride = D + 2, parts = p.n_shared + p.n_own;
     if (kKeyParts == 1) {
-        if (warp == kWarps) return;
+        if (!ok) return false;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const int row = sync.rows[row_tile * 16 + g + 8 * r];
-            if (row < 0) continue;
-            float* dst = partial + ((size_t)row * parts + it.part) * stride;
+            if (rows[r] < 0) continue;
+            float* dst = partial + ((size_t)rows[r] * parts + it.part) * stride;
 #pragma unroll
             for (int j = 0; j < kNTiles; ++j) *reinterpret_cast<float2*>(dst + j * 8 + 2 * t) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
             if (t == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m[r], l[r]);
         }
-        return;
+        return true;
     }
-    // the warps that had other keys of the same rows meet in shared memory
-    constexpr int kPitch = D + 8;                                                 // floats of a row: eight rows of a warp then meet different banks
-    float* o_s = reinterpret_cast<float*>(smem);                                  // [kWarps][16][kPitch]
-    float* m_s = o_s + kWarps * 16 * kPitch;                                      // [kWarps][16]
-    float* l_s = m_s + kWarps * 16;
-    if (warp < kWarps) {
+    // The warps that had other keys of the same rows meet in shared memory: [row][key part][kPitch] floats of o, then m, l and the row's number.
+    constexpr int kPitch = D + 8;                                                 // eight rows of a warp meet different banks
+    float* merge = reinterpret_cast<float*>(smem);
+    meet();                                                                       // all tiles have been read
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+    for (int r = 0; r < 2; ++r) {
+        const int i = row_tile * 16 + g + 8 * r;
+        if (i < it.rows) {
+            float* at_row = merge + (i * kKeyParts + key_part) * kPitch;
 #pragma unroll
-            for (int j = 0; j < kNTiles; ++j)
-                *reinterpret_cast<float2*>(o_s + (warp * 16 + g + 8 * r) * kPitch + j * 8 + 2 * t) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
-            if (t == 0) { m_s[warp * 16 + g + 8 * r] = m[r]; l_s[warp * 16 + g + 8 * r] = l[r]; }
+            for (int j = 0; j < kNTiles; ++j) *reinterpret_cast<float2*>(at_row + j * 8 + 2 * t) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
+            if (t == 0) *reinterpret_cast<float4*>(at_row + D) = make_float4(m[r], l[r], __int_as_float(rows[r]), 0.0f);
         }
     }
-    __syncthreads();
-    for (int i = tid; i < it.rows * (D / 4); i += kTcThreads) {
-        const int row = i / (D / 4), d = i % (D / 4) * 4;                         // the row's first key part is warp row / 16
-        const int to = sync.rows[row];
+    meet();
+    if (!ok) return false;
+    for (int i = tid; i < it.rows * (D / 4); i += kWarps * 32) {
+        const int row = i / (D / 4), d = i % (D / 4) * 4;
+        const float* from = merge + row * kKeyParts * kPitch;
+        const int to = __float_as_int(from[D + 2]);
         if (to < 0) continue;
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kKeyParts; ++w) top = fmaxf(top, m_s[w * ROW_TILES * 16 + row]);
+        for (int w = 0; w < kKeyParts; ++w) top = fmaxf(top, from[w * kPitch + D]);
         const float base = top == -INFINITY ? 0.0f : top;
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         float sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kKeyParts; ++w) {
-            const int from = w * ROW_TILES * 16 + row;
-            const float f = pow2(m_s[from] - base);
-            const float4 v = *reinterpret_cast<const float4*>(o_s + from * kPitch + d);
+            const float f = pow2(from[w * kPitch + D] - base);
+            const float4 v = *reinterpret_cast<const float4*>(from + w * kPitch + d);
             acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
-            sum = fmaf(l_s[from], f, sum);
+            sum = fmaf(from[w * kPitch + D + 1], f, sum);
         }
         float* dst = partial + ((size_t)to * parts + it.part) * stride;
         *reinterpret_cast<float2*>(dst + d) = make_float2(acc.x, acc.y);
         *reinterpret_cast<float2*>(dst + d + 2) = make_float2(acc.z, acc.w);
         if (d == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(top, sum);
     }
+    return true;
 }
 
-// ROW_TILES: of the shared sides' blocks; a sequence's own keys meet tiles of 16 rows.  beside: the kernel before it on the stream has the
-// shared sides; it was launched the ordinary way, lets this one in at its start, and the two write different parts.
+// ROW_TILES: of the shared sides' items; a sequence's own keys meet tiles of 16 rows.  Blocks in the order of the grid, the kv head fastest:
+// the shared sides', then the first parts of all sequences' own keys, then their second, which many do not have.  (Blocks that walk over items
+// and ask for the next one's tiles ahead were no faster, 75 against 60 us for 101 sequences: the shares come out uneven.)  beside: the kernel
+// before it on the stream has the shared sides; it was launched the ordinary way, lets this one in at its start, and the two write
+// different parts.
 template <int D, int ROW_TILES>
 __global__ void __launch_bounds__(kTcThreads, kBlocks<ROW_TILES>)
 shared_tc_kernel(const bf16* __restrict__ q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                 float* __restrict__ partial, const Shared p, int shared_blocks, int page_shift, const PoolBounds bounds, unsigned int* error, bool beside) {
+                 float* __restrict__ partial, const Shared p, int shared_items, int page_shift, const PoolBounds bounds, unsigned int* error, bool beside) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ Ring sync;
     constexpr int kStages = kRing<ROW_TILES> / (2 * kTileBytes<D>);
     pdl_trigger();                                                                // (the join waits for this kernel's end)
-    const int G = p.Hq / p.Hkv, tid = threadIdx.x;
-    const bool family = (int)blockIdx.x < shared_blocks;
+    const int G = p.Hq / p.Hkv, tid = threadIdx.x, warp = tid >> 5, kvh = blockIdx.x % p.Hkv, block = blockIdx.x / p.Hkv;
+    const bool family = block < shared_items;
     Item it;
-    if (family) {
-        if (!family_item<ROW_TILES * 16, kTile>(p, blockIdx.x, G, it)) return;
-    } else {
-        own_item<16, kTile>(p, blockIdx.x - shared_blocks, G, it);
-    }
-    if (tid == kWarps * 32) {
-        for (int i = 0; i < kStages; ++i) {
-            mbar_init(smem_addr(&sync.full[i]), 1);
-            mbar_init(smem_addr(&sync.empty[i]), kWarps);
+    if (family ? family_item<ROW_TILES * 16, kTile>(p, block, G, it) : own_item<16>(p, block - shared_items, G, it)) {
+        const uint32_t ring = smem_addr(smem);
+        if (tid == 0) {
+            for (int i = 0; i < kStages; ++i) {
+                mbar_init(smem_addr(&sync.full[i]), 1);
+                mbar_init(smem_addr(&sync.empty[i]), kWarps);
+            }
+            sync.gave_up = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
-        sync.gave_up = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    } else if (tid < 64) {
-        int row = -1;
-        if (tid < it.rows) {
-            const int seq = it.seq_of(p, tid, G);
-            if (seq >= 0 && seq < p.n_seqs) row = seq * p.Hq + it.head_of(blockIdx.y, tid, G);
+        __syncthreads();
+        bool ok;
+        if (warp == kWarps) {
+            ok = fill<D, kStages>(&map_k, &map_v, p, it, kvh, page_shift, bounds, ring, sync);
+        } else {
+            ok = family ? attend<D, ROW_TILES, kStages>(q, partial, p, it, kvh, G, ring, smem, sync)
+                        : attend<D, 1, kStages>(q, partial, p, it, kvh, G, ring, smem, sync);
         }
-        sync.rows[tid] = row;
+        if (!ok && (tid & 31) == 0) { *(volatile int*)&sync.gave_up = 1; atomicMax(error, warp == kWarps ? 2u : 4u); }
+        __syncthreads();
+        if (*(volatile int*)&sync.gave_up) {
+            for (int i = 0; i < 2000; ++i) __nanosleep(1000);                     // copies in flight land before this block's memory is reused
+        }
     }
-    __syncthreads();
-    if (family) attend<D, ROW_TILES, kStages>(q, &map_k, &map_v, partial, p, it, blockIdx.y, page_shift, bounds, smem, sync, error);
-    else attend<D, 1, kStages>(q, &map_k, &map_v, partial, p, it, blockIdx.y, page_shift, bounds, smem, sync, error);
     // complete no sooner than the kernel it ran beside: the last block alone waits, the others leave their places to those behind them
-    if (beside && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1) pdl_wait();
+    if (beside && blockIdx.x == gridDim.x - 1) pdl_wait();
 }
 
 // Joins a row's parts: a warp per row, a lane per part for their weights and per four dimensions for the sums.  A sequence outside
 // the families has no shared parts.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-shared_join_kernel(const float* __restrict__ partial, T* __restrict__ out, const int* __restrict__ shared_len, int rows, int Hq, int D, int n_shared,
-                   int n_own) {
+shared_join_kernel(const float* __restrict__ partial, T* __restrict__ out, const Shared p, int rows, int D) {
     const int row = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (row >= rows) return;
-    const int parts = n_shared + n_own, stride = D + 2;
-    const int first = shared_len[row / Hq] > 0 ? 0 : n_shared;                    // (the host wrote it, before the kernel ahead began)
-    const float* base = partial + (size_t)row * parts * stride;
+    const int room = p.n_shared + p.n_own, stride = D + 2, seq = row / p.Hq;
+    // (lengths were there before the kernels ahead began)
+    const int first = p.shared_len[seq] > 0 ? 0 : p.n_shared, parts = p.n_shared + own_parts(p, seq);
+    const float* base = partial + (size_t)row * room * stride;
     pdl_wait();
     float m[2], l[2];                                                             // up to 64 parts
 #pragma unroll
@@ -467,25 +467,15 @@ shared_join_kernel(const float* __restrict__ partial, T* __restrict__ out, const
     }
 }
 
-// Blocks of the shared sides and of all; 0 for all: too many for a grid.
-struct Grid {
-    int shared, all;
-};
-Grid grid_of(const Shared& p, int G, int shared_rows, int own_rows) {
-    const long long shared = (long long)p.n_families * ((p.most_members * G + shared_rows - 1) / shared_rows) * p.n_shared;
-    const long long all = shared + (long long)p.n_seqs * ((G + own_rows - 1) / own_rows) * p.n_own;
-    return all > 0x7fffffff ? Grid{0, 0} : Grid{(int)shared, (int)all};
-}
-
 template <typename T, int QUADS>
 int launch_general(const void* q, const void* k_pool, const void* v_pool, float* partial, const Shared& p, int D, int G, cudaStream_t stream) {
-    const Grid grid = grid_of(p, G, kRows, kRows);
-    if (grid.all == 0) return PB_ERR_TOO_LARGE;
+    const long long shared = family_blocks(p, G, kRows), all = shared + own_blocks(p, G, kRows);
+    if (all > 0x7fffffff) return PB_ERR_TOO_LARGE;
     const size_t smem = (size_t)(kRows * D + kKeys * (D + 4) + kKeys * D) * sizeof(float);
     static SmemLimit limit;
     if (const int rc = limit.allow(shared_general_kernel<T, QUADS>, smem)) return rc;
-    shared_general_kernel<T, QUADS><<<dim3(grid.all, p.Hkv), kThreads, smem, stream>>>((const T*)q, (const T*)k_pool, (const T*)v_pool, partial, p, grid.shared, D,
-                                                                                       pool_bounds_now());
+    shared_general_kernel<T, QUADS><<<dim3((unsigned)all, p.Hkv), kThreads, smem, stream>>>((const T*)q, (const T*)k_pool, (const T*)v_pool, partial, p,
+                                                                                           (int)shared, D, pool_bounds_now());
     return launch_status();
 }
 
@@ -509,15 +499,16 @@ struct Maps {
 
 template <int D, int ROW_TILES>
 int launch_tc(const void* q, const Maps& maps, float* partial, const Shared& p, int G, bool beside, cudaStream_t stream) {
-    const Grid grid = grid_of(p, G, ROW_TILES * 16, 16);
-    if (grid.all == 0) return PB_ERR_TOO_LARGE;
+    const long long shared = family_blocks(p, G, ROW_TILES * 16), items = (shared + own_blocks(p, G, 16)) * p.Hkv;
+    if (items > 0x7fffffff) return PB_ERR_TOO_LARGE;
     constexpr int smem = kRing<ROW_TILES> + 1024;
+    static_assert(kWarps * 16 * (D + 8) * 4 <= kRing<ROW_TILES>, "the warps meet in the ring's memory");
     static SmemLimit limit;
     static DeviceLimit most;
     if (const int rc = limit.allow(shared_tc_kernel<D, ROW_TILES>, smem)) return rc;
     if (const int rc = share_most(most, shared_tc_kernel<D, ROW_TILES>)) return rc;
-    return launch_early(beside, shared_tc_kernel<D, ROW_TILES>, dim3(grid.all, p.Hkv), dim3(kTcThreads), smem, stream, (const bf16*)q, maps.k, maps.v, partial, p,
-                        grid.shared, log2_exact(p.page_size), pool_bounds_now(), maps.error, beside);
+    return launch_early(beside, shared_tc_kernel<D, ROW_TILES>, dim3((unsigned)items), dim3(kTcThreads), smem, stream, (const bf16*)q,
+                        maps.k, maps.v, partial, p, (int)shared, log2_exact(p.page_size), pool_bounds_now(), maps.error, beside);
 }
 
 // Families of up to 16 rows meet their keys as a sequence its own.  Beyond that heads of 128 take the tcgen05 kernel for the shared sides
@@ -562,19 +553,21 @@ PB_EXPORT int pb_shared_rows(int dtype, int rows, int D, int page_size) {
 // q, out [n_seqs, Hq, D], pools [pages, Hkv, page_size, D] (dtype 0 float32, 1 bfloat16); block_table int32 [n_seqs, table_stride];
 // kv_len, shared_len int32 [n_seqs]; members int32 [n_members], family_start int32 [n_families + 1]; partial float32
 // [n_seqs * Hq * (n_shared + n_own) * (D + 2)], all 16-byte aligned; n_pages: of the pools; error: the word that a block sets which gave up
-// a bounded wait; n_shared + n_own <= 64.
+// a bounded wait; own_chunk: keys of a part of a sequence's own, a multiple of 64 and of the page; n_shared + n_own <= 64.
 PB_EXPORT int pb_paged_attention_shared(int dtype, const void* q, const void* k_pool, const void* v_pool, void* out, float* partial,
                                         const int* block_table, int table_stride, const int* kv_len, const int* shared_len, const int* members,
                                         const int* family_start, int n_seqs, int n_members, int n_families, int most_members, int Hq, int Hkv, int D,
-                                        int page_size, float scale, int n_shared, int n_own, int n_pages, unsigned int* error, cudaStream_t stream) {
+                                        int page_size, float scale, int n_shared, int n_own, int own_chunk, int n_pages, unsigned int* error,
+                                        cudaStream_t stream) {
     if (n_seqs <= 0) return 0;
     if (dtype != PB_F32 && dtype != PB_BF16) return PB_ERR_BAD_DTYPE;
     if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || D <= 0 || D % 16 || D > 256 || page_size <= 0 || table_stride <= 0) return PB_ERR_BAD_SIZE;
     if (n_families < 0 || most_members < 0 || n_members < 0 || n_own <= 0 || n_shared < 0 || (n_families > 0 && n_shared == 0)) return PB_ERR_BAD_SIZE;
+    if (own_chunk <= 0 || own_chunk % 64 || own_chunk % page_size) return PB_ERR_BAD_SIZE;
     if (Hkv > 65535 || n_shared + n_own > 64 || (long long)n_seqs * Hq > 0x7fffffff) return PB_ERR_TOO_LARGE;
     const int G = Hq / Hkv;
     Shared p{block_table, kv_len, shared_len, members, family_start, n_seqs, n_members, n_families, most_members, table_stride, Hq, Hkv, page_size, n_shared, n_own,
-             scale * kLog2e};
+             own_chunk, scale * kLog2e};
     int rc;
     if ((((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out | (uintptr_t)partial) & 15) != 0) return PB_ERR_BAD_SIZE;
     if (tc_takes(dtype, D, page_size) && n_pages > 0 && error != nullptr)
@@ -585,8 +578,8 @@ PB_EXPORT int pb_paged_attention_shared(int dtype, const void* q, const void* k_
         rc = D <= 128 ? launch_general<bf16, 1>(q, k_pool, v_pool, partial, p, D, G, stream) : launch_general<bf16, 2>(q, k_pool, v_pool, partial, p, D, G, stream);
     if (rc != 0) return rc;
     const int rows = n_seqs * Hq, blocks = (rows + kThreads / 32 - 1) / (kThreads / 32);
-    if (dtype == PB_F32) return launch_pdl(shared_join_kernel<float>, dim3(blocks), dim3(kThreads), 0, stream, partial, (float*)out, shared_len, rows, Hq, D, n_shared, n_own);
-    return launch_pdl(shared_join_kernel<bf16>, dim3(blocks), dim3(kThreads), 0, stream, partial, (bf16*)out, shared_len, rows, Hq, D, n_shared, n_own);
+    if (dtype == PB_F32) return launch_pdl(shared_join_kernel<float>, dim3(blocks), dim3(kThreads), 0, stream, partial, (float*)out, p, rows, D);
+    return launch_pdl(shared_join_kernel<bf16>, dim3(blocks), dim3(kThreads), 0, stream, partial, (bf16*)out, p, rows, D);
 }
 
 // A new limit of this kernel's bounded waits in clock cycles.

@@ -22,7 +22,8 @@ struct Shared {
     int n_seqs, n_members, n_families, most_members;
     int table_stride;
     int Hq, Hkv, page_size;
-    int n_shared, n_own;        // splits of either side
+    int n_shared, n_own;        // parts that a row has room for, of either side
+    int own_chunk;              // keys of a part of a sequence's own, a multiple of the tiles
     float scale_log2;
 };
 
@@ -38,17 +39,7 @@ struct Item {
     __device__ __forceinline__ int head_of(int kvh, int i, int G) const { return kvh * G + (row0 + i) % G; }
 };
 
-// Split `split` of `splits` of the keys from it.begin on, never beyond the table.
-template <int TILE>
-__device__ __forceinline__ void cut(const Shared& p, Item& it, int keys, int split, int splits) {
-    keys = max(0, min(keys, p.table_stride * p.page_size - it.begin));
-    int chunk = (keys + splits - 1) / splits;
-    chunk = (chunk + TILE - 1) / TILE * TILE;
-    const int end = it.begin + keys;
-    it.begin = min(end, it.begin + split * chunk);
-    it.end = min(end, it.begin + chunk);
-}
-// Block `block` of the shared sides.  False: nothing to do.
+// Block `block` of the shared sides: the family's keys in n_shared parts (those beyond the last key are empty).  False: nothing to do.
 template <int ROWS, int TILE>
 __device__ __forceinline__ bool family_item(const Shared& p, int block, int G, Item& it) {
     const int tiles = (p.most_members * G + ROWS - 1) / ROWS;
@@ -62,24 +53,36 @@ __device__ __forceinline__ bool family_item(const Shared& p, int block, int G, I
     const int first = p.members[it.first_member];
     if (first < 0 || first >= p.n_seqs) return false;
     it.table = p.block_table + (size_t)first * p.table_stride;
-    it.begin = 0;
     it.seq = -1;
     it.part = split;
-    cut<TILE>(p, it, p.shared_len[first], split, p.n_shared);
+    const int keys = max(0, min(p.shared_len[first], p.table_stride * p.page_size));      // never beyond the table
+    int chunk = (keys + p.n_shared - 1) / p.n_shared;
+    chunk = (chunk + TILE - 1) / TILE * TILE;
+    it.begin = min(keys, split * chunk);
+    it.end = min(keys, it.begin + chunk);
     return true;
 }
-// Block `block` of the sequences' own sides.
-template <int ROWS, int TILE>
-__device__ __forceinline__ void own_item(const Shared& p, int block, int G, Item& it) {
-    const int tiles = (G + ROWS - 1) / ROWS, split = block % p.n_own;
-    it.seq = block / p.n_own / tiles;
-    it.row0 = block / p.n_own % tiles * ROWS;
+// The first of a sequence's own keys (its shared pages are whole already, unless the caller erred), and how many parts they make.
+__device__ __forceinline__ int own_begin(const Shared& p, int seq) { return max(0, p.shared_len[seq]) / p.page_size * p.page_size; }
+__device__ __forceinline__ int own_end(const Shared& p, int seq) { return min(p.kv_len[seq], p.table_stride * p.page_size); }
+__device__ __forceinline__ int own_parts(const Shared& p, int seq) {
+    return min(p.n_own, max(0, own_end(p, seq) - own_begin(p, seq) + p.own_chunk - 1) / p.own_chunk);
+}
+// Block `block` of the sequences' own sides, the first parts of all sequences first.  False: the sequence has no such part.
+template <int ROWS>
+__device__ __forceinline__ bool own_item(const Shared& p, int block, int G, Item& it) {
+    const int tiles = (G + ROWS - 1) / ROWS, split = block / (p.n_seqs * tiles);
+    block -= split * p.n_seqs * tiles;
+    it.seq = block / tiles;
+    it.row0 = block % tiles * ROWS;
     it.rows = min(ROWS, G - it.row0);
     it.first_member = 0;
     it.table = p.block_table + (size_t)it.seq * p.table_stride;
-    it.begin = max(0, p.shared_len[it.seq]) / p.page_size * p.page_size;      // (whole pages already, unless the caller erred)
     it.part = p.n_shared + split;
-    cut<TILE>(p, it, p.kv_len[it.seq] - it.begin, split, p.n_own);
+    const int end = own_end(p, it.seq);
+    it.begin = own_begin(p, it.seq) + split * p.own_chunk;
+    it.end = min(end, it.begin + p.own_chunk);
+    return it.begin < end;
 }
 
 // Lets an SM that runs `kernel` have as much of its memory shared as can be, so that a block of another kernel finds room beside it (once per device).
@@ -92,6 +95,8 @@ int share_most(DeviceLimit& done, void (*kernel)(KArgs...)) {
 
 // Blocks of the shared sides.
 inline long long family_blocks(const Shared& p, int G, int rows) { return (long long)p.n_families * ((p.most_members * G + rows - 1) / rows) * p.n_shared; }
+
+inline long long own_blocks(const Shared& p, int G, int rows) { return (long long)p.n_seqs * ((G + rows - 1) / rows) * p.n_own; }
 
 // The shared sides on the fifth-generation tensor cores (attention_shared_tcgen05.cu): head size 128, pages of 8 to 64 keys.
 constexpr int kTcgen05Rows = 128;

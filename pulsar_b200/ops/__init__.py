@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import os
 from typing import Optional, Tuple
 
@@ -141,7 +142,7 @@ _SIGNATURES = {
     "pb_matrix_memory": [_I, _P, _L, _P, _P, _F, _P, _F, _F, _F, _P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "pb_state_space": [_I, _P, _L, _P, _P, _I, _P, _P, _P, _P, _I, _F, _P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "pb_copy_pages": [_I, _P, _P, _P, _P, _P, _I, _P],
-    "pb_paged_attention_shared": [_I] + [_P] * 6 + [_I] + [_P] * 4 + [_I] * 8 + [_F, _I, _I, _I, _P, _P],
+    "pb_paged_attention_shared": [_I] + [_P] * 6 + [_I] + [_P] * 4 + [_I] * 8 + [_F, _I, _I, _I, _I, _P, _P],
     "pb_shared_wait_limit": [ctypes.c_longlong],
     "pb_shared_tcgen05_wait_limit": [ctypes.c_longlong],
     "pb_shared_rows": [_I, _I, _I, _I],
@@ -2057,7 +2058,7 @@ def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     if (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr() | out.data_ptr()) % 16:
         raise KernelError("paged_attention_shared: q, out and the pools must start at a multiple of 16 bytes")
     families = family_start.numel() - 1 if most_members > 0 and most_shared > 0 else 0
-    n_shared, n_own = shared_cut(s, families, int(most_members), int(most_shared), block_table.shape[1] * page_size, hq, hkv, d, page_size, q.dtype)
+    n_shared, n_own, own_chunk = shared_cut(s, families, int(most_members), int(most_shared), block_table.shape[1] * page_size, hq, hkv, d, page_size, q.dtype)
     need = s * hq * (n_shared + n_own) * (d + 2)
     if partial is None:
         partial = torch.empty(need, dtype=torch.float32, device=q.device)
@@ -2065,13 +2066,13 @@ def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
         raise KernelError(f"paged_attention_shared: partial must be float32 of at least {need} elements at a multiple of 16 bytes, found {partial.numel()} of {partial.dtype}")
     check(fn("pb_paged_attention_shared")(kind, _p(q), _p(k_pool), _p(v_pool), _p(out), _p(partial), _p(block_table), block_table.shape[1], _p(kv_len),
                                           _p(shared_len), _p(members), _p(family_start), s, members.numel(), families, int(most_members), hq, hkv, d,
-                                          page_size, float(scale), n_shared, n_own, k_pool.shape[0], wait_word_addresses()[1], stream()), "paged_attention_shared", kernels=2)
+                                          page_size, float(scale), n_shared, n_own, own_chunk, k_pool.shape[0], wait_word_addresses()[1], stream()), "paged_attention_shared", kernels=2)
 
 
 @functools.lru_cache(maxsize=1024)
 def shared_cut(n_seqs: int, n_families: int, most_members: int, most_shared: int, table_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int,
-               page_size: int, dtype: torch.dtype) -> Tuple[int, int]:
-    """(parts of the shared keys, parts of the own keys) that ``paged_attention_shared`` works in."""
+               page_size: int, dtype: torch.dtype) -> Tuple[int, int, int]:
+    """(parts of the shared keys, most parts of a sequence's own keys, keys of one of those) that ``paged_attention_shared`` works in."""
     group = n_heads // n_kv_heads
     rows = most_members * group
     tile = fn("pb_shared_rows")(code(dtype), rows, head_dim, page_size)
@@ -2080,16 +2081,20 @@ def shared_cut(n_seqs: int, n_families: int, most_members: int, most_shared: int
     # rounds, and cutting their keys further only makes more of them.
     slots = _DECODE_SLOTS // 2 if tile == 128 else _DECODE_SLOTS
     n_shared = max(1, min(32, most_shared // 256, slots // max(1, blocks))) if n_families else 0
+    # Own keys: parts of at most 512, so that no block walks much longer than the others, and of fewer where that leaves SMs idle; of more
+    # where a table has more than 32 of them.  Whole tiles of 64, whole pages.
     own_blocks = n_seqs * -(-group // 16) * n_kv_heads
-    n_own = max(1, min(32, (table_tokens - (most_shared if n_families else 0)) // 256, _DECODE_SLOTS // max(1, own_blocks)))
-    return n_shared, n_own
+    chunk = max(128, min(512, table_tokens * own_blocks // (3 * _DECODE_SLOTS // 2)), -(-table_tokens // 32))
+    whole = 64 * page_size // math.gcd(64, page_size)
+    chunk = -(-chunk // whole) * whole
+    return n_shared, max(1, -(-table_tokens // chunk)), chunk
 
 
 def shared_scratch(n_seqs: int, n_families: int, most_members: int, most_shared: int, table_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int,
                    page_size: int, dtype: torch.dtype) -> int:
     """Elements of ``paged_attention_shared``'s scratch."""
-    return n_seqs * n_heads * sum(shared_cut(n_seqs, n_families, most_members, most_shared, table_tokens, n_heads, n_kv_heads, head_dim, page_size,
-                                             dtype)) * (head_dim + 2)
+    n_shared, n_own, _ = shared_cut(n_seqs, n_families, most_members, most_shared, table_tokens, n_heads, n_kv_heads, head_dim, page_size, dtype)
+    return n_seqs * n_heads * (n_shared + n_own) * (head_dim + 2)
 
 
 _LOGITS_AT_ONCE = 1 << 26         # elements of float32 logits that ``head_scores`` keeps where it cannot do without them
