@@ -6,8 +6,13 @@
 // without a word to its neighbours.  A tile leaves three numbers per row; a second kernel joins a row's tiles.
 //
 // Bound: with few rows the bytes of W, with many the products (2 R V K).  The epilogue of a tile costs some 3,000 cycles beside the
-// 32,768 that the products of 256 columns and K = 4096 take (one SM, 8,192 multiply-adds... per cycle), and runs under those of the next
-// tile: there are two accumulators.  Roles, ring of stages and bounded waits are those of gemm_tcgen05.cu.
+// 32,768 that the products of 128 rows, 256 columns and K = 4096 take on one SM, and runs under those of the next tile: there are two
+// accumulators.  Roles, ring of stages and bounded waits are those of gemm_tcgen05.cu.
+//
+// Up to 128 rows a block per SM streams W.  Of h it brings only the rows that there are: the lanes beyond them read what lies behind in
+// shared memory and give sums that nobody reads, and the ring holds that much more of W (17 rows of 4,096 against 151,936: 220 us with
+// tiles of 128 rows of h, 199 without).  More rows go to pairs of blocks on tiles of 256 rows (cta_group::2): each block brings its own 128
+// rows of h and half of the tile's columns of W, which so crosses from L2 once a pair.
 //
 // The width of a tile is chosen so that the tiles fill the SMs in whole rounds (see plan()).
 #include "scores.cuh"
@@ -26,6 +31,7 @@ constexpr int kTmemColumns = 512;
 constexpr int kMostStages = 8;
 constexpr int kABytes = kBM * kBK * 2;
 constexpr int kSmem = 226 * 1024;
+constexpr uint32_t kPeerBitMask = 0xFEFFFFFFu;   // clears the bit in which the two blocks' shared-memory addresses differ: rank 0's barrier
 
 struct HeadArgs {
     const int* tokens;          // [rows]
@@ -35,6 +41,7 @@ struct HeadArgs {
     int rows, vocab, k;
     int columns;                // of a tile
     int m_tiles, n_tiles, stages;
+    int h_bytes, stage_bytes;   // of a stage: the rows of h, and all
     float scale, cap;           // cap 0: none
 };
 
@@ -47,11 +54,41 @@ __device__ __forceinline__ uint64_t umma_desc(uint32_t addr) {      // K-major, 
     d |= (uint64_t)2 << 61;
     return d;
 }
+template <bool PAIR>
 __device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+    if (PAIR)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
 }
+// Arrives on `bar` (of both blocks of a pair) once the products issued so far have retired.
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint32_t bar) {
+    if (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(bar), "h"((unsigned short)3) : "memory");
+    else
+        umma_commit(bar);
+}
+// A box into this block's shared memory; its bytes count on `bar`, in a pair on rank 0's.
+template <bool PAIR>
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+    if (PAIR)
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                     ::"r"(dst), "l"(map), "r"(bar & kPeerBitMask), "r"(c0), "r"(c1) : "memory");
+    else
+        tma_load_2d(dst, map, bar, c0, c1);
+}
+// The same for bytes that are read once and should be the first to leave L2.
+__device__ __forceinline__ void load_box_once(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, uint64_t policy) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "l"(policy) : "memory");
+}
+__device__ __forceinline__ void both_blocks() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // One row's columns [first, first + columns) of an accumulator.
 template <bool CAP>
@@ -81,18 +118,24 @@ __device__ __forceinline__ void score_tile(const HeadArgs& p, uint32_t taddr, in
     }
 }
 
-template <bool CAP>
+// PAIR: a cluster of two blocks per tile of 256 rows; barriers as in gemm_tcgen05.cu: "full" and "accumulator empty" are rank 0's, which
+// issues the products of both.
+template <bool CAP, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 head_scores_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w, const HeadArgs p) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    const int stage_bytes = kABytes + p.columns * kBK * 2;
     __shared__ __align__(8) uint64_t bars[2 * kMostStages + 4];                 // full, empty, accumulator full, accumulator empty
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     volatile int* abort_flag = &abort_word;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint32_t rank = 0;
+    if (PAIR) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const int worker = PAIR ? blockIdx.x >> 1 : blockIdx.x, workers = PAIR ? gridDim.x >> 1 : gridDim.x;
+    constexpr int kRows = PAIR ? 2 * kBM : kBM;                                  // of a tile
+    const int own_columns = PAIR ? p.columns / 2 : p.columns;                    // of W that this block brings
     const int k_tiles = (p.k + kBK - 1) / kBK;
     const int total_tiles = p.m_tiles * p.n_tiles;
     const uint32_t full0 = smem_addr(bars), empty0 = smem_addr(bars + kMostStages);
@@ -100,70 +143,82 @@ head_scores_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_const
 
     if (tid == 0) {
         for (int s = 0; s < p.stages; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
-        for (int a = 0; a < 2; ++a) { mbar_init(acc_full0 + 8 * a, 1); mbar_init(acc_empty0 + 8 * a, 4); }
+        for (int a = 0; a < 2; ++a) { mbar_init(acc_full0 + 8 * a, 1); mbar_init(acc_empty0 + 8 * a, PAIR ? 8 : 4); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(kTmemColumns));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(kTmemColumns));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(kTmemColumns));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (PAIR) both_blocks();                                                     // the peer's barriers exist before anything arrives on them
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = tmem_slot;
 
     if (warp == 0) {
         if (lane == 0) {
+            uint64_t once = 0;
+            if (!PAIR) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
             int s = 0, turn = 0;
             bool ok = true;
-            for (int tile = blockIdx.x; tile < total_tiles && ok; tile += gridDim.x) {
-                const int m0 = (tile % p.m_tiles) * kBM, n0 = (tile / p.m_tiles) * p.columns;
+            for (int tile = worker; tile < total_tiles && ok; tile += workers) {
+                const int m0 = (tile % p.m_tiles) * kRows + (int)rank * kBM, n0 = (tile / p.m_tiles) * p.columns + (int)rank * own_columns;
                 for (int kt = 0; kt < k_tiles; ++kt) {
                     if (!mbar_wait(empty0 + 8 * s, (turn & 1) ^ 1, abort_flag)) { ok = false; break; }
-                    const uint32_t a_dst = smem_addr(smem) + s * stage_bytes;
-                    mbar_expect_tx(full0 + 8 * s, stage_bytes);
-                    tma_load_2d(a_dst, &map_h, full0 + 8 * s, kt * kBK, m0);
-                    tma_load_2d(a_dst + kABytes, &map_w, full0 + 8 * s, kt * kBK, n0);
+                    const uint32_t dst = smem_addr(smem) + s * p.stage_bytes;
+                    const uint32_t bytes = (uint32_t)(p.h_bytes + own_columns * kBK * 2);
+                    if (rank == 0) mbar_expect_tx(full0 + 8 * s, PAIR ? 2 * bytes : bytes);
+                    load_box<PAIR>(dst, &map_h, full0 + 8 * s, kt * kBK, m0);
+                    if (PAIR) load_box<PAIR>(dst + p.h_bytes, &map_w, full0 + 8 * s, kt * kBK, n0);
+                    else load_box_once(dst + p.h_bytes, &map_w, full0 + 8 * s, kt * kBK, n0, once);
                     if (++s == p.stages) { s = 0; ++turn; }
                 }
             }
             if (!ok) { *abort_flag = 1; atomicMax(p.error, 2u); }
         }
     } else if (warp == 1) {
-        const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
-        const uint64_t desc0 = umma_desc(smem_addr(smem));
-        // float32 accumulator, bfloat16 operands, both K-major, columns >> 3, rows >> 4
-        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.columns >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
-        int s = 0, turn = 0, j = 0;
-        bool ok = true;
-        for (int tile = blockIdx.x; tile < total_tiles && ok; tile += gridDim.x, ++j) {
-            const int acc = j & 1;
-            ok = mbar_wait(acc_empty0 + 8 * acc, ((j >> 1) & 1) ^ 1, abort_flag);
-            const uint32_t tmem_d = tmem_u + acc * kMostColumns;
-            for (int kt = 0; kt < k_tiles && ok; ++kt) {
-                if (!mbar_wait(full0 + 8 * s, turn & 1, abort_flag)) { ok = false; break; }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t a_desc = desc0 + (uint64_t)((uint32_t)s * (uint32_t)(stage_bytes >> 4));
-                const uint64_t b_desc = a_desc + (uint64_t)(kABytes >> 4);
-                if (elect_one()) {
+        if (rank == 0) {
+            const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
+            const uint64_t desc0 = umma_desc(smem_addr(smem));
+            // float32 accumulator, bfloat16 operands, both K-major, columns >> 3, rows >> 4
+            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.columns >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+            int s = 0, turn = 0, j = 0;
+            bool ok = true;
+            for (int tile = worker; tile < total_tiles && ok; tile += workers, ++j) {
+                const int acc = j & 1;
+                ok = mbar_wait(acc_empty0 + 8 * acc, ((j >> 1) & 1) ^ 1, abort_flag);
+                const uint32_t tmem_d = tmem_u + acc * kMostColumns;
+                for (int kt = 0; kt < k_tiles && ok; ++kt) {
+                    if (!mbar_wait(full0 + 8 * s, turn & 1, abort_flag)) { ok = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t a_desc = desc0 + (uint64_t)((uint32_t)s * (uint32_t)(p.stage_bytes >> 4));
+                    const uint64_t b_desc = a_desc + (uint64_t)(p.h_bytes >> 4);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < kBK / 16; ++k)
-                        umma_bf16(tmem_d, a_desc + (uint64_t)(k * 2), b_desc + (uint64_t)(k * 2), idesc, (kt > 0 || k > 0) ? 1u : 0u);
-                    umma_commit(empty0 + 8 * s);
-                    if (kt == k_tiles - 1) umma_commit(acc_full0 + 8 * acc);
+                        for (int k = 0; k < kBK / 16; ++k)
+                            umma_bf16<PAIR>(tmem_d, a_desc + (uint64_t)(k * 2), b_desc + (uint64_t)(k * 2), idesc, (kt > 0 || k > 0) ? 1u : 0u);
+                        commit<PAIR>(empty0 + 8 * s);
+                        if (kt == k_tiles - 1) commit<PAIR>(acc_full0 + 8 * acc);
+                    }
+                    __syncwarp();
+                    if (++s == p.stages) { s = 0; ++turn; }
                 }
-                __syncwarp();
-                if (++s == p.stages) { s = 0; ++turn; }
             }
+            if (!ok && lane == 0) { *abort_flag = 1; atomicMax(p.error, 3u); }
         }
-        if (!ok && lane == 0) { *abort_flag = 1; atomicMax(p.error, 3u); }
     } else {
         const int quarter = warp & 3;
         int j = 0;
-        for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, ++j) {
+        for (int tile = worker; tile < total_tiles; tile += workers, ++j) {
             const int acc = j & 1;
-            const int m0 = (tile % p.m_tiles) * kBM, nt = tile / p.m_tiles;
+            const int m0 = (tile % p.m_tiles) * kRows + (int)rank * kBM, nt = tile / p.m_tiles;
             if (!mbar_wait(acc_full0 + 8 * acc, (j >> 1) & 1, abort_flag)) {
                 if (lane == 0) { *abort_flag = 1; atomicMax(p.error, 4u); }
                 break;
@@ -186,7 +241,12 @@ head_scores_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_const
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty0 + 8 * acc);
+            if (lane == 0) {
+                if (PAIR)
+                    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"((acc_empty0 + 8 * acc) & kPeerBitMask) : "memory");
+                else
+                    mbar_arrive(acc_empty0 + 8 * acc);
+            }
         }
     }
     __syncwarp();
@@ -196,7 +256,11 @@ head_scores_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_const
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemColumns));
+    if (PAIR) both_blocks();                                                     // neither leaves while the other may still touch its memory
+    if (warp == 1) {
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemColumns));
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemColumns));
+    }
 }
 
 // Joins the tiles of 32 rows per block: lanes are rows, warps take turns at the tiles.
@@ -235,18 +299,21 @@ int sm_count() {
 }
 
 struct Plan {
+    bool pair;
     int columns, m_tiles, n_tiles;
 };
 
-// The widest tile whose rounds over the SMs come out even: all tiles are as wide, so the time is rounds x (columns + what a tile costs
-// besides, about 16 columns' worth).
+// The widest tile whose rounds over the SMs (pairs of them) come out even: all tiles are as wide, so the time is rounds x (columns + what a
+// tile costs besides, about 16 columns' worth).  (17 rows against 151,936: 731 tiles of 208, five rounds; 594 of 256 would be five too.)
 Plan plan(int rows, int vocab) {
     Plan best = {};
-    best.m_tiles = (rows + kBM - 1) / kBM;
+    best.pair = rows > kBM;
+    const int tile_rows = best.pair ? 2 * kBM : kBM, step = best.pair ? 32 : 16, workers = best.pair ? sm_count() / 2 : sm_count();
+    best.m_tiles = (rows + tile_rows - 1) / tile_rows;
     long long least = 0;
-    for (int columns = kMostColumns; columns >= 16; columns -= 16) {
+    for (int columns = kMostColumns; columns >= step; columns -= step) {
         const long long tiles = (long long)best.m_tiles * ((vocab + columns - 1) / columns);
-        const long long cost = (tiles + sm_count() - 1) / sm_count() * (columns + 16);
+        const long long cost = (tiles + workers - 1) / workers * (columns + 16);
         if (least == 0 || cost < least) {
             least = cost;
             best.columns = columns;
@@ -269,14 +336,24 @@ int make_map(CUtensorMap* map, const void* base, int rows, int k, int box_rows) 
     return rc == CUDA_SUCCESS ? 0 : PB_ERR_BAD_SIZE;
 }
 
-template <bool CAP>
+template <bool CAP, bool PAIR>
 int launch(const CUtensorMap& mh, const CUtensorMap& mw, const HeadArgs& p, cudaStream_t stream) {
-    const int stage_bytes = kABytes + p.columns * kBK * 2, smem = p.stages * stage_bytes + 1024;
     static SmemLimit limit;
-    if (const int rc = limit.allow(head_scores_kernel<CAP>, kSmem)) return rc;
-    const long long tiles = (long long)p.m_tiles * p.n_tiles;
-    head_scores_kernel<CAP><<<(int)(tiles < sm_count() ? tiles : sm_count()), kThreads, smem, stream>>>(mh, mw, p);
-    return launch_status();
+    if (const int rc = limit.allow(head_scores_kernel<CAP, PAIR>, kSmem)) return rc;
+    const long long tiles = (long long)p.m_tiles * p.n_tiles, workers = PAIR ? sm_count() / 2 : sm_count();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles < workers ? tiles : workers) * (PAIR ? 2 : 1));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = p.stages * p.stage_bytes + 1024;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = PAIR ? 2 : 1;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, head_scores_kernel<CAP, PAIR>, mh, mw, p);
 }
 
 }  // namespace
@@ -300,13 +377,19 @@ PB_EXPORT int pb_head_scores(const void* h, const void* w, const int* tokens, fl
                              float cap, float* scratch, unsigned int* error, cudaStream_t stream) {
     if (!pb_head_scores_supported(rows, vocab, k) || (((uintptr_t)h | (uintptr_t)w) & 15) != 0 || error == nullptr || !(cap >= 0.0f)) return PB_ERR_BAD_SIZE;
     const Plan at = plan(rows, vocab);
-    HeadArgs p = {tokens, scratch, scratch + 3 * (size_t)at.n_tiles * rows, error, rows, vocab, k, at.columns, at.m_tiles, at.n_tiles, 0, scale, cap};
-    const int stages = (kSmem - 1024) / (kABytes + at.columns * kBK * 2);
+    HeadArgs p = {tokens, scratch, scratch + 3 * (size_t)at.n_tiles * rows, error, rows, vocab, k, at.columns, at.m_tiles, at.n_tiles, 0, 0, 0, scale, cap};
+    // of a single tile of rows only whole groups of eight are brought; a stage is as long as the 128 that the products read
+    const int h_rows = at.m_tiles == 1 && !at.pair ? (rows + 7) / 8 * 8 : kBM, own_columns = at.pair ? at.columns / 2 : at.columns;
+    p.h_bytes = h_rows * kBK * 2;
+    p.stage_bytes = p.h_bytes + own_columns * kBK * 2;
+    if (p.stage_bytes < kABytes) p.stage_bytes = kABytes;
+    const int stages = (kSmem - 1024) / p.stage_bytes;
     p.stages = stages < kMostStages ? stages : kMostStages;
     CUtensorMap mh, mw;
-    int rc = make_map(&mh, h, rows, k, kBM);
-    if (rc == 0) rc = make_map(&mw, w, vocab, k, at.columns);
-    if (rc == 0) rc = cap > 0.0f ? launch<true>(mh, mw, p, stream) : launch<false>(mh, mw, p, stream);
+    int rc = make_map(&mh, h, rows, k, h_rows);
+    if (rc == 0) rc = make_map(&mw, w, vocab, k, own_columns);
+    if (rc == 0 && at.pair) rc = cap > 0.0f ? launch<true, true>(mh, mw, p, stream) : launch<false, true>(mh, mw, p, stream);
+    else if (rc == 0) rc = cap > 0.0f ? launch<true, false>(mh, mw, p, stream) : launch<false, false>(mh, mw, p, stream);
     if (rc != 0) return rc;
     head_join_kernel<<<(rows + 31) / 32, kJoinWarps * 32, 0, stream>>>(p.part, p.given, tokens, logprob, entropy, rows, at.n_tiles, vocab);
     return launch_status();
