@@ -9,10 +9,9 @@
 // 32,768 that the products of 128 rows, 256 columns and K = 4096 take on one SM, and runs under those of the next tile: there are two
 // accumulators.  Roles, ring of stages and bounded waits are those of gemm_tcgen05.cu.
 //
-// Up to 128 rows a block per SM streams W.  Of h it brings only the rows that there are: the lanes beyond them read what lies behind in
-// shared memory and give sums that nobody reads, and the ring holds that much more of W (17 rows of 4,096 against 151,936: 220 us with
-// tiles of 128 rows of h, 199 without).  More rows go to pairs of blocks on tiles of 256 rows (cta_group::2): each block brings its own 128
-// rows of h and half of the tile's columns of W, which so crosses from L2 once a pair.
+// Up to 128 rows a block per SM streams W (once, so it is the first to leave L2: 201 against 206 us for 17 rows of 4,096 against 151,936,
+// 206 against 216 for 100).  More rows go to pairs of blocks on tiles of 256 rows (cta_group::2): each block brings its own 128 rows of h and
+// half of the tile's columns of W, which so crosses from L2 once a pair (2,048 rows: 1,885 us, single blocks 1,949).
 //
 // The width of a tile is chosen so that the tiles fill the SMs in whole rounds (see plan()).
 #include "scores.cuh"
@@ -41,7 +40,7 @@ struct HeadArgs {
     int rows, vocab, k;
     int columns;                // of a tile
     int m_tiles, n_tiles, stages;
-    int h_bytes, stage_bytes;   // of a stage: the rows of h, and all
+    int stage_bytes;
     float scale, cap;           // cap 0: none
 };
 
@@ -130,6 +129,7 @@ head_scores_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_const
     __shared__ int abort_word;
     volatile int* abort_flag = &abort_word;
 
+    pdl_trigger();                                                               // (what joins the tiles waits for this kernel's end)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint32_t rank = 0;
     if (PAIR) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -173,11 +173,11 @@ head_scores_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_const
                 for (int kt = 0; kt < k_tiles; ++kt) {
                     if (!mbar_wait(empty0 + 8 * s, (turn & 1) ^ 1, abort_flag)) { ok = false; break; }
                     const uint32_t dst = smem_addr(smem) + s * p.stage_bytes;
-                    const uint32_t bytes = (uint32_t)(p.h_bytes + own_columns * kBK * 2);
+                    const uint32_t bytes = (uint32_t)p.stage_bytes;
                     if (rank == 0) mbar_expect_tx(full0 + 8 * s, PAIR ? 2 * bytes : bytes);
                     load_box<PAIR>(dst, &map_h, full0 + 8 * s, kt * kBK, m0);
-                    if (PAIR) load_box<PAIR>(dst + p.h_bytes, &map_w, full0 + 8 * s, kt * kBK, n0);
-                    else load_box_once(dst + p.h_bytes, &map_w, full0 + 8 * s, kt * kBK, n0, once);
+                    if (PAIR) load_box<PAIR>(dst + kABytes, &map_w, full0 + 8 * s, kt * kBK, n0);
+                    else load_box_once(dst + kABytes, &map_w, full0 + 8 * s, kt * kBK, n0, once);
                     if (++s == p.stages) { s = 0; ++turn; }
                 }
             }
@@ -199,7 +199,7 @@ head_scores_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_const
                     if (!mbar_wait(full0 + 8 * s, turn & 1, abort_flag)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint64_t a_desc = desc0 + (uint64_t)((uint32_t)s * (uint32_t)(p.stage_bytes >> 4));
-                    const uint64_t b_desc = a_desc + (uint64_t)(p.h_bytes >> 4);
+                    const uint64_t b_desc = a_desc + (uint64_t)(kABytes >> 4);
                     if (elect_one()) {
 #pragma unroll
                         for (int k = 0; k < kBK / 16; ++k)
@@ -263,26 +263,30 @@ head_scores_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_const
     }
 }
 
-// Joins the tiles of 32 rows per block: lanes are rows, warps take turns at the tiles.
-constexpr int kJoinWarps = 16;
-__global__ void __launch_bounds__(kJoinWarps * 32)
+// Joins the tiles of eight rows per block: 64 threads a row take turns at its tiles.
+constexpr int kJoinRows = 8, kJoinThreads = 512;
+__global__ void __launch_bounds__(kJoinThreads)
 head_join_kernel(const float* __restrict__ part, const float* __restrict__ given, const int* __restrict__ tokens, float* __restrict__ logprob,
                  float* __restrict__ entropy, int rows, int n_tiles, int vocab) {
-    __shared__ Stats st_s[kJoinWarps][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
+    __shared__ Stats st_s[kJoinThreads / 32][kJoinRows];
+    const int tid = threadIdx.x, warp = tid >> 5, i = tid % kJoinRows, row = blockIdx.x * kJoinRows + i;
     const size_t plane = (size_t)n_tiles * rows;
+    pdl_wait();
     Stats st = {-INFINITY, 0.0f, 0.0f};
     if (row < rows) {
 #pragma unroll 4
-        for (int i = warp; i < n_tiles; i += kJoinWarps) {
-            const float* at = part + (size_t)i * rows + row;
+        for (int tile = tid / kJoinRows; tile < n_tiles; tile += kJoinThreads / kJoinRows) {
+            const float* at = part + (size_t)tile * rows + row;
             st = join(st, Stats{at[0], at[plane], at[2 * plane]});
         }
     }
-    st_s[warp][lane] = st;
+#pragma unroll
+    for (int o = kJoinRows; o < 32; o <<= 1)
+        st = join(st, Stats{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.t, o)});
+    if ((tid & 31) < kJoinRows) st_s[warp][i] = st;
     __syncthreads();
-    if (warp != 0 || row >= rows) return;
-    for (int w = 1; w < kJoinWarps; ++w) st = join(st, st_s[w][lane]);
+    if (tid >= kJoinRows || row >= rows) return;
+    for (int w = 1; w < kJoinThreads / 32; ++w) st = join(st, st_s[w][i]);
     const int token = tokens[row];
     const float log_s = logf(st.s);
     logprob[row] = token >= 0 && token < vocab ? (given[row] - st.m) - log_s : nanf("");
@@ -304,7 +308,8 @@ struct Plan {
 };
 
 // The widest tile whose rounds over the SMs (pairs of them) come out even: all tiles are as wide, so the time is rounds x (columns + what a
-// tile costs besides, about 16 columns' worth).  (17 rows against 151,936: 731 tiles of 208, five rounds; 594 of 256 would be five too.)
+// tile costs besides, about 16 columns' worth).  (17 rows against 151,936: 731 tiles of 208 in five rounds, 201 us;
+// 594 of 256 take five as well, 220.)
 Plan plan(int rows, int vocab) {
     Plan best = {};
     best.pair = rows > kBM;
@@ -377,20 +382,17 @@ PB_EXPORT int pb_head_scores(const void* h, const void* w, const int* tokens, fl
                              float cap, float* scratch, unsigned int* error, cudaStream_t stream) {
     if (!pb_head_scores_supported(rows, vocab, k) || (((uintptr_t)h | (uintptr_t)w) & 15) != 0 || error == nullptr || !(cap >= 0.0f)) return PB_ERR_BAD_SIZE;
     const Plan at = plan(rows, vocab);
-    HeadArgs p = {tokens, scratch, scratch + 3 * (size_t)at.n_tiles * rows, error, rows, vocab, k, at.columns, at.m_tiles, at.n_tiles, 0, 0, 0, scale, cap};
-    // of a single tile of rows only whole groups of eight are brought; a stage is as long as the 128 that the products read
-    const int h_rows = at.m_tiles == 1 && !at.pair ? (rows + 7) / 8 * 8 : kBM, own_columns = at.pair ? at.columns / 2 : at.columns;
-    p.h_bytes = h_rows * kBK * 2;
-    p.stage_bytes = p.h_bytes + own_columns * kBK * 2;
-    if (p.stage_bytes < kABytes) p.stage_bytes = kABytes;
+    const int own_columns = at.pair ? at.columns / 2 : at.columns;
+    HeadArgs p = {tokens, scratch, scratch + 3 * (size_t)at.n_tiles * rows, error, rows, vocab, k, at.columns, at.m_tiles, at.n_tiles, 0,
+                  kABytes + own_columns * kBK * 2, scale, cap};
     const int stages = (kSmem - 1024) / p.stage_bytes;
     p.stages = stages < kMostStages ? stages : kMostStages;
     CUtensorMap mh, mw;
-    int rc = make_map(&mh, h, rows, k, h_rows);
+    int rc = make_map(&mh, h, rows, k, kBM);
     if (rc == 0) rc = make_map(&mw, w, vocab, k, own_columns);
     if (rc == 0 && at.pair) rc = cap > 0.0f ? launch<true, true>(mh, mw, p, stream) : launch<false, true>(mh, mw, p, stream);
     else if (rc == 0) rc = cap > 0.0f ? launch<true, false>(mh, mw, p, stream) : launch<false, false>(mh, mw, p, stream);
     if (rc != 0) return rc;
-    head_join_kernel<<<(rows + 31) / 32, kJoinWarps * 32, 0, stream>>>(p.part, p.given, tokens, logprob, entropy, rows, at.n_tiles, vocab);
-    return launch_status();
+    return launch_pdl(head_join_kernel, dim3((rows + kJoinRows - 1) / kJoinRows), dim3(kJoinThreads), 0, stream, (const float*)p.part, (const float*)p.given, tokens,
+                      logprob, entropy, rows, at.n_tiles, vocab);
 }
