@@ -344,6 +344,98 @@ class CacheManager:
         if rc < 0:
             self._raise(rc, rid)
 
+    # ------------------------------------------------------------------ several requests over the same pages
+    def fork(self, rid: Hashable, children: Sequence[Hashable], length: Optional[int] = None) -> None:
+        """New requests that begin as the first ``length`` tokens of ``rid`` (all that it holds, unless given).  Whole pages are shared: they
+        are never written again, and go back to the pool with the last request that holds them.  A page that is filled only in part is copied
+        for each child, and so is a fixed-size state, which is that of all the tokens: such a request is forked at its length only.  Either
+        every child is opened or nothing changes."""
+        children = list(children)
+        nid = self._open_id(rid)
+        held = self.length(rid)
+        length = held if length is None else int(length)
+        if not (0 <= length <= held):
+            raise CacheError(f"request {rid!r} holds {held} tokens: it cannot be forked at {length}")
+        if length != held and any(need.kind == "state" for need in self.needs):
+            raise CacheError(f"request {rid!r} holds fixed-size state of {held} tokens: it cannot be forked at {length}")
+        for i, child in enumerate(children):
+            if self.has(child) or child in children[:i]:
+                raise CacheError(f"request {child!r} is already open")
+        if len(children) > self.n_free_slots():
+            raise OutOfPages(f"{len(children)} new requests but {self.n_free_slots()} free state slots")
+        if length % self.page_size and self.groups and len(children) > min(self.n_free_pages()):
+            raise OutOfPages(f"{len(children)} new requests need a page each, {self.n_free_pages()} pages are free")
+        copies = (ctypes.c_int * max(1, 2 * self._n_groups))()
+        pairs: List[List[Tuple[int, int]]] = [[] for _ in self.groups]
+        slots = []
+        for i, child in enumerate(children):
+            slot = self._lib.ph_fork(self._h, nid, self.native_id(child, create=True), length, copies)
+            if slot < 0:
+                self._forget_if_idle(child)
+                for opened in children[:i]:
+                    self.close(opened)
+                self._raise(slot, rid, f"a page that a query at {length} needs")
+            slots.append(slot)
+            for g in range(self._n_groups):
+                if copies[2 * g] >= 0:
+                    pairs[g].append((copies[2 * g], copies[2 * g + 1]))
+        if self.device is None or not children:
+            return
+        from .. import ops
+        for grp, some in zip(self.groups, pairs):
+            if some:
+                src, dst = torch.tensor(some, dtype=torch.int32).t().contiguous().to(self.device)
+                ops.copy_pages(list(grp.pools.values()), list(grp.pools.values()), src, dst)
+        if self.state:
+            own = self._lib.ph_state_slot(self._h, nid)
+            src, dst = torch.tensor([[own] * len(slots), slots], dtype=torch.int32).to(self.device)
+            states = [t.unsqueeze(0) for t in self.state.values()]
+            ops.copy_pages(states, states, src, dst)
+
+    def page_holders(self, group: int, page: int) -> int:
+        """How many requests hold a page (0: it is free)."""
+        return self._lib.ph_page_holders(self._h, int(group), int(page))
+
+    def n_shared_pages(self) -> List[int]:
+        """Pages of each group that more than one request holds."""
+        return [self._lib.ph_n_shared_pages(self._h, g) for g in range(self._n_groups)]
+
+    def families(self, rids: Sequence[Hashable], group: int) -> Tuple[List[List[int]], List[int]]:
+        """Which of ``rids`` (by their indices) begin with the same pages in ``group``, two at least, and for every request how many keys lie
+        in pages that its whole family shares."""
+        n = len(rids)
+        members, starts, shared, most = (ctypes.c_int * max(1, n))(), (ctypes.c_int * (n + 1))(), (ctypes.c_int * max(1, n))(), (ctypes.c_int * 2)()
+        count = self._lib.ph_families(self._h, int(group), n, host.longs([self._open_id(r) for r in rids]), members, starts, shared, most)
+        return [list(members[starts[f]:starts[f + 1]]) for f in range(count)], list(shared[:n])
+
+    def resize(self, num_pages) -> None:
+        """Give every group ``num_pages`` pages (an int, or a list per group): what is held moves to the front of new pools, and the old pools'
+        memory goes back to PyTorch.  Refused, with nothing changed, where a group holds more pages than that.  While a group moves, its old and
+        its new pools exist side by side.  Whoever keeps the pools' addresses (a captured step) has to forget them."""
+        counts = [int(num_pages)] * self._n_groups if isinstance(num_pages, int) else [int(n) for n in num_pages]
+        if len(counts) != self._n_groups or any(c <= 0 for c in counts):
+            raise CacheError(f"num_pages must give a positive count for each of the {self._n_groups} groups")
+        for g, (grp, n) in enumerate(zip(self.groups, counts)):
+            in_use = grp.allocator.n - grp.allocator.n_free
+            if in_use > n:
+                raise OutOfPages(f"group {g} holds {in_use} pages: it cannot be cut to {n}")
+        for g, (grp, n) in enumerate(zip(self.groups, counts)):
+            pools = None
+            if grp.pools is not None:                       # (memory first: if it cannot be had, this group is as it was)
+                pools = {name: torch.zeros((t.shape[0], n, *t.shape[2:]), dtype=t.dtype, device=t.device) for name, t in grp.pools.items()}
+            moved = (ctypes.c_int * max(1, grp.allocator.n))()
+            live = self._lib.ph_resize(self._h, g, n, moved)
+            if live < 0:
+                raise CacheError(f"group {g}: the host runtime refused {n} pages (code {live})")
+            if pools is not None:
+                if live:
+                    from .. import ops
+                    src = torch.tensor(list(moved[:live]), dtype=torch.int32).to(self.device)
+                    ops.copy_pages(list(grp.pools.values()), list(pools.values()), src, torch.arange(live, dtype=torch.int32, device=self.device))
+                grp.pools = pools
+            grp.allocator = _GroupPages(self, g)
+        self._entry_pools.clear()
+
     # ------------------------------------------------------------------ views for a step
     def table(self, rid: Hashable, group: int) -> List[int]:
         nid = self._open_id(rid)
@@ -404,7 +496,7 @@ class CacheManager:
         return new, True
 
     def check_consistency(self) -> None:
-        """Every page is free or held by exactly one request, every slot likewise; used by tests."""
+        """Every page is free or held by as many requests as name it, every slot is free or held by one; used by tests."""
         if self._lib.ph_check(self._h) != 0:
             raise CacheError("the cache's accounting is inconsistent: a page or slot is lost, held twice or freed twice")
         live = sorted(self._lib.ph_state_slot(self._h, nid) for nid in self._ids.values() if self._lib.ph_has(self._h, nid))

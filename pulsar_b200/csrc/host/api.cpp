@@ -9,6 +9,8 @@
 
 #include <algorithm>
 #include <cstring>
+#include <unordered_map>
+#include <vector>
 
 #define PH_EXPORT extern "C" __attribute__((visibility("default")))
 
@@ -111,6 +113,59 @@ PH_EXPORT int ph_slots(void* h, int64_t rid, int group, int start, int n, int* o
         out[p - start] = page * ps + p % ps;
     }
     return 0;
+}
+
+// A request that starts as the first `length` tokens of another (see Cache::fork); copies: two ints per group.
+PH_EXPORT int ph_fork(void* h, int64_t parent, int64_t child, int length, int* copies) {
+    return static_cast<Cache*>(h)->fork(parent, child, length, copies);
+}
+PH_EXPORT int ph_page_holders(void* h, int group, int page) {
+    const Group& g = static_cast<Cache*>(h)->group(group);
+    return g.pages.held(page) ? g.holders[page] : 0;
+}
+PH_EXPORT int ph_n_shared_pages(void* h, int group) { return static_cast<Cache*>(h)->group(group).n_shared; }
+PH_EXPORT int ph_resize(void* h, int group, int n_pages, int* from) { return static_cast<Cache*>(h)->resize(group, n_pages, from); }
+// The families among requests rids[0 .. n): those whose tables of a group begin with the same page and go on alike.  members [n], starts
+// [n + 1], shared_len [n] (keys in the pages that all members of a request's family share; 0: none) in 32-bit words; most: the largest
+// family's size and the longest shared length.  Returns the number of families (of two requests and more).
+PH_EXPORT int ph_families(void* h, int group, int n, const int64_t* rids, int* members, int* starts, int* shared_len, int* most) {
+    const Cache* c = static_cast<Cache*>(h);
+    std::unordered_map<int, std::vector<int>> by_page;                        // first page -> requests, in their order
+    std::vector<int> order;
+    std::vector<const Request*> reqs(n);
+    for (int i = 0; i < n; ++i) {
+        shared_len[i] = 0;
+        reqs[i] = c->find(rids[i]);
+        if (!reqs[i]) return kUnknownRequest;
+        const std::vector<int>& t = reqs[i]->tables[group];
+        if (t.empty() || t[0] < 0) continue;
+        std::vector<int>& same = by_page[t[0]];
+        if (same.empty()) order.push_back(t[0]);
+        same.push_back(i);
+    }
+    int families = 0, at = 0;
+    most[0] = most[1] = 0;
+    starts[0] = 0;
+    for (int page : order) {
+        const std::vector<int>& same = by_page[page];
+        if (same.size() < 2) continue;
+        const std::vector<int>& first = reqs[same[0]]->tables[group];
+        size_t alike = first.size();
+        for (int i : same) {
+            const std::vector<int>& t = reqs[i]->tables[group];
+            size_t k = 0;
+            while (k < alike && k < t.size() && t[k] >= 0 && t[k] == first[k]) ++k;
+            alike = k;
+        }
+        for (int i : same) {
+            members[at++] = i;
+            shared_len[i] = (int)alike * c->page_size();
+        }
+        starts[++families] = at;
+        most[0] = std::max(most[0], (int)same.size());
+        most[1] = std::max(most[1], (int)alike * c->page_size());
+    }
+    return families;
 }
 
 // ------------------------------------------------------------------ the step packer
@@ -331,6 +386,8 @@ PH_EXPORT int ph_sched_add(void* h, int64_t rid, const int* tokens, int n, int m
 PH_EXPORT int ph_sched_extend(void* h, int64_t rid, const int* tokens, int n, int max_new_tokens) {
     return static_cast<Scheduler*>(h)->extend_request(rid, tokens, n, max_new_tokens);
 }
+// A known request `child` with the first `length` tokens of `parent`, all of them in the cache already (ph_fork).
+PH_EXPORT int ph_sched_fork(void* h, int64_t parent, int64_t child, int length) { return static_cast<Scheduler*>(h)->fork_request(parent, child, length); }
 PH_EXPORT int ph_sched_has_work(void* h) { return static_cast<Scheduler*>(h)->has_work() ? 1 : 0; }
 // Decides a step and keeps it; returns the number of its entries, or kNeedsPreemption.
 PH_EXPORT int ph_sched_schedule(void* h, int allow_preempt) {

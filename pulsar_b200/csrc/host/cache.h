@@ -47,6 +47,12 @@ struct Group {
     int window;                 // keys a query sees at most; <= 0: all of them
     FreeList pages;
     int keep = 0;               // the first `keep` keys of a sequence stay visible below the window: their pages are never given back
+    std::vector<int> holders;   // requests that hold each page (a forked request's whole pages have several); the last one frees it
+    int n_shared = 0;           // pages with several holders
+
+    int take();                 // a page for one request, or kOutOfPages
+    int share(int page);        // one more holder
+    int drop(int page);         // one holder less: 0, or kNotHeld
 };
 
 struct Request {
@@ -74,6 +80,13 @@ public:
     int release_passed(Request& r);
     int append(int64_t rid, int n_new);                         // position of the first new token
     int close(int64_t rid);
+    // A request `child` that starts as the first `length` tokens of `parent`: it shares the whole pages and has a page of its own for what is
+    // left.  copies[2 g], copies[2 g + 1]: the page of group g that the caller copies, and where to (-1 where nothing is left).  The state slot,
+    // or an error that changes nothing.
+    int fork(int64_t parent, int64_t child, int length, int* copies);
+    // Gives group `group` `n_pages` pages: those that are held become the first ones, in the order of their ids, and from[i] is what page i was.
+    // Their number, or kOutOfPages (nothing changes).
+    int resize(int group, int n_pages, int* from);
     int check() const;                                          // 0 or kInconsistent
 
     int page_size() const { return page_size_; }

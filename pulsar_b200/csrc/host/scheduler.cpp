@@ -70,6 +70,20 @@ int Scheduler::extend_request(int64_t rid, const int* tokens, int n, int max_new
     return 0;
 }
 
+// A request that begins as another's first `length` tokens, which the cache holds for it already: known, but not queued before its first turn.
+int Scheduler::fork_request(int64_t parent, int64_t child, int length) {
+    auto it = seqs_.find(parent);
+    if (it == seqs_.end()) return kUnknownRequest;
+    if (seqs_.count(child)) return kAlreadyOpen;
+    const Sequence& p = it->second;
+    if (length < 0 || length > p.n_cached || length > (int)p.tokens.size() - p.unread) return kBadArgument;
+    Sequence s;
+    s.tokens.assign(p.tokens.begin(), p.tokens.begin() + length);
+    s.n_cached = length;
+    seqs_.emplace(child, std::move(s));
+    return 0;
+}
+
 void Scheduler::preempt(int64_t rid) {
     Sequence& s = seqs_.at(rid);
     if (cache_->has(rid)) cache_->close(rid);

@@ -62,6 +62,7 @@ public:
 
     int add_request(int64_t rid, const int* tokens, int n, int max_new_tokens);
     int extend_request(int64_t rid, const int* tokens, int n, int max_new_tokens);
+    int fork_request(int64_t parent, int64_t child, int length);            // the child waits for its first turn (extend_request)
     bool has_work() const { return !waiting_.empty() || !running_.empty(); }
     int schedule(bool allow_preempt, std::vector<PlanEntry>* out);      // 0, or kNeedsPreemption
     void on_step(const std::vector<PlanEntry>& plan);

@@ -57,6 +57,7 @@ _SIGNATURES = {
     "ph_sched_on_sampled": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64]),
     "ph_sched_on_token": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int]),
     "ph_sched_drop_unread": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64]),
+    "ph_sched_fork": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
     "ph_sched_park": (None, [ctypes.c_void_p, ctypes.c_int64]),
     "ph_sched_finish": (None, [ctypes.c_void_p, ctypes.c_int64]),
     "ph_sched_knows": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64]),
@@ -210,6 +211,19 @@ class Scheduler:
             raise SchedulerError(f"request {rid!r}: a further turn needs at least one token to run")
         if rc < 0:
             raise SchedulerError(f"request {rid!r}: the host runtime answered {rc}")
+
+    def fork_request(self, rid: Hashable, child: Hashable, length: int) -> None:
+        """``child`` becomes a known request with the first ``length`` tokens of ``rid``, which the cache holds for it already
+        (``CacheManager.fork``).  It is not queued before ``extend_request`` gives it its first turn."""
+        if rid not in self._known:
+            raise SchedulerError(f"unknown request {rid!r}")
+        if child in self._known:
+            raise SchedulerError(f"request {child!r} is already known")
+        rc = self._lib.ph_sched_fork(self._h, self.cache.native_id(rid), self.cache.pin(child), int(length))
+        if rc < 0:
+            self.cache.unpin(child)
+            raise SchedulerError(f"request {rid!r}: its first {length} tokens are not all cached and read")
+        self._known.add(child)
 
     def has_work(self) -> bool:
         return self._lib.ph_sched_has_work(self._h) == 1
