@@ -12,6 +12,9 @@ def __getattr__(name):
     if name in ("AsyncPulsar", "AsyncSession"):
         from . import aio
         return getattr(aio, name)
+    if name in ("Candidate", "TokenScore"):
+        from .sampling import scores
+        return getattr(scores, name)
     if name in ("Engine",):
         from .engine.engine import Engine
         return Engine

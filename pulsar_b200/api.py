@@ -14,6 +14,7 @@ from typing import Any, Dict, Iterator, List, Optional, Sequence
 import torch
 
 from .engine.engine import Engine
+from .sampling.scores import Candidate, TokenScore
 
 
 class Session:
@@ -54,6 +55,14 @@ class Session:
         (pulsar/src/pulsar/rt/session.py:37-43, without the reference's recall layer)."""
         return self._engine.context_page_ids(self._seq_id), self._engine.context_pages(self._seq_id)
 
+    def fork(self, *, overrides: Optional[Dict[str, Any]] = None, length: Optional[int] = None, scores: Optional[int] = None) -> "Session":
+        """Another session that goes on from here (this one's turn has to be over); see ``Engine.fork``."""
+        return Session(self._engine.fork(self._seq_id, overrides, length, scores), self._engine)
+
+    def scores(self) -> List[TokenScore]:
+        """The scores of the tokens received since the last call, for a session that was created with ``scores``."""
+        return self._engine.scores(self._seq_id)
+
     def destroy(self) -> None:
         self._engine.release(self._seq_id)
 
@@ -73,8 +82,16 @@ class Pulsar:
     def engine(self) -> Engine:
         return self._engine
 
-    def create_session(self, sink: Sequence[int] = (), *, overrides: Optional[Dict[str, Any]] = None) -> Session:
-        return Session(self._engine.create_session(sink, overrides), self._engine)
+    def create_session(self, sink: Sequence[int] = (), *, overrides: Optional[Dict[str, Any]] = None, scores: Optional[int] = None) -> Session:
+        return Session(self._engine.create_session(sink, overrides, scores), self._engine)
+
+    def candidates(self, prompt: Sequence[int], n: int, max_new_tokens: int, **sampling) -> List[Candidate]:
+        """``n`` scored continuations of one prompt, the likeliest first; see ``Engine.candidates``."""
+        return self._engine.candidates(prompt, n, max_new_tokens, **sampling)
+
+    def score(self, prompts: Sequence[Sequence[int]], alternatives: Optional[int] = None) -> List[List[TokenScore]]:
+        """How likely the model finds the tokens of each prompt; see ``Engine.score``."""
+        return self._engine.score(prompts, alternatives)
 
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int, temperature: Optional[float] = None,
                  top_k: Optional[int] = None, top_p: Optional[float] = None, seed: Optional[int] = None

@@ -42,6 +42,8 @@ def parse_args(argv=None) -> argparse.Namespace:
     ap.add_argument("--random_weights", metavar="CONFIG_JSON",
                     help="write --model from this config.json with seeded random weights first")
     ap.add_argument("--weights_seed", type=int, default=0)
+    ap.add_argument("--candidates", type=int, default=1, help="continuations per prompt: each is scored, the likeliest comes first (prompts one "
+                                                              "behind the other; takes that many sessions and one more)")
     ap.add_argument("--json", action="store_true", help="print one JSON object instead of text")
     return ap.parse_args(argv)
 
@@ -81,16 +83,27 @@ def main(argv=None) -> int:
                   top_p=args.top_p, top_k=args.top_k, seed=args.seed)
     if args.max_pages is not None:
         config["num_pages"] = args.max_pages
+    if args.candidates > 1:
+        config["max_sessions"] = max(args.max_sessions, args.candidates + 1)
+        config["max_running"] = max(args.max_running, args.candidates)
+        config.setdefault("num_pages", args.max_sessions * args.active_buffer_size // args.page_size)      # the sessions share their prompt's
     engine = Engine(args.model, config)
     t0 = time.time()
-    outputs = engine.generate(prompts, args.gen_tokens, seed=args.seed)
+    more = {}
+    if args.candidates > 1:
+        found = [engine.candidates(p, args.candidates, args.gen_tokens, seed=args.seed) for p in prompts]
+        outputs = [c.tokens for some in found for c in some]
+        more = {"mean_logprobs": [c.mean_logprob for some in found for c in some]}
+    else:
+        outputs = engine.generate(prompts, args.gen_tokens, seed=args.seed)
     dt = time.time() - t0
     n_new = sum(len(o) for o in outputs)
     if args.json:
-        print(json.dumps({"outputs": outputs, "new_tokens": n_new, "seconds": dt, "forwards": engine.forwards}))
+        print(json.dumps({"outputs": outputs, **more, "new_tokens": n_new, "seconds": dt, "forwards": engine.forwards}))
     else:
         for i, o in enumerate(outputs):
-            print(f"[{i}] " + " ".join(str(t) for t in o))
+            where = f"[{i}] " if not more else f"[{i // args.candidates}.{i % args.candidates}] ({more['mean_logprobs'][i]:.4f}) "
+            print(where + " ".join(str(t) for t in o))
         print(f"{n_new} tokens in {dt:.3f}s ({n_new / max(dt, 1e-9):.1f} tok/s, {engine.forwards} forwards)", file=sys.stderr)
     return 0
 

@@ -17,6 +17,7 @@ from .. import ops, profiling
 from ..cache.manager import CacheManager
 from ..config.engine_config import EngineConfig
 from ..sampling.sampler import GenerationParams, Sampler, draw_uniform, make_generator
+from ..sampling.scores import Candidate, ScoreBoard, TokenScore
 from .loading import load_model, torch_dtype
 from .runner import ModelRunner, StepEntry
 from .scheduler import UNREAD, Scheduled, Scheduler, SchedulerError
@@ -31,6 +32,8 @@ class _Session:
     state: str = "idle"           # "idle", "active", "parked"
     scheduled: bool = False       # known to the scheduler
     ended_on_stop: bool = False   # the last turn ended with the stop token
+    alternatives: Optional[int] = None  # None: tokens are not scored; else so many alternatives go with each score
+    scores: List[TokenScore] = field(default_factory=list)
     redraw: Optional[float] = None      # a number whose draw turned out void: the next draw gives it again
 
     def draw(self) -> float:
@@ -54,6 +57,7 @@ class _Inflight:
     row_of: Dict[int, int]
     report: "ops.Pinned"                   # the kernels' wait error words behind this pass, then its sampled ids
     uniform: List[float]                   # what each row drew (0.0 for greedy sequences)
+    scores: Optional[Tuple["ops.Pinned", int]] = None          # the rows' scores on their way, and the alternatives of each
     void: set = field(default_factory=set)         # sequences that had ended before this pass: its token is dropped
 
 
@@ -111,6 +115,7 @@ class Engine:
         self._unclaimed: List[Tuple[int, int, bool]] = []   # events booked outside ``step``
         self._host_report: List[Optional[ops.Pinned]] = [None, None, None]
         self._host_next = 0
+        self._host_scores: List[Optional[ops.Pinned]] = [None, None, None]
         self._failed: Optional[BaseException] = None
 
     # ------------------------------------------------------------------ sessions
@@ -128,16 +133,59 @@ class Engine:
         if self._failed is not None:
             raise EngineFailed(f"the engine failed earlier and refuses further work: {self._failed}") from self._failed
 
-    def create_session(self, tokens: Sequence[int] = (), overrides: Optional[Dict[str, Any]] = None) -> int:
-        """A new sequence with its first tokens (they are not scheduled before ``feed``)."""
+    def create_session(self, tokens: Sequence[int] = (), overrides: Optional[Dict[str, Any]] = None, scores: Optional[int] = None) -> int:
+        """A new sequence with its first tokens (they are not scheduled before ``feed``).  ``scores``: every token that it emits is scored, with
+        so many alternatives (0 for none); ``scores(seq_id)`` hands the scores out."""
         self._alive()
+        self._check_alternatives(scores)
         if len(self._sessions) >= self.config.max_sessions:
             raise RuntimeError(f"max_sessions ({self.config.max_sessions}) reached")
         params = self._params(overrides)
         sid = self._next_id
         self._next_id += 1
-        self._sessions[sid] = _Session(params, make_generator(params.seed), [int(t) for t in tokens], 0)
+        self._sessions[sid] = _Session(params, make_generator(params.seed), [int(t) for t in tokens], 0, alternatives=scores)
         return sid
+
+    def _check_alternatives(self, scores: Optional[int]) -> None:
+        if scores is not None and not (0 <= scores <= min(ops.MOST_ALTERNATIVES, self.model.spec.vocab_size)):
+            raise ValueError(f"scores come with 0 to {min(ops.MOST_ALTERNATIVES, self.model.spec.vocab_size)} alternatives, found {scores}")
+
+    def fork(self, seq_id: int, overrides: Optional[Dict[str, Any]] = None, length: Optional[int] = None, scores: Optional[int] = None) -> int:
+        """A new sequence that goes on from where ``seq_id``, whose turn has to be over, stands: the pages of the tokens that they have in common
+        are shared.  ``length``: it begins as the first ``length`` tokens only, all of which have to be in the cache, and needs further ones
+        with ``feed``.  Sampling as ``overrides`` and the engine's configuration say, scores as for ``create_session``."""
+        return self._fork(seq_id, [overrides], length, scores)[0]
+
+    def _fork(self, seq_id: int, overrides: Sequence[Optional[Dict[str, Any]]], length: Optional[int], scores: Optional[int]) -> List[int]:
+        self._alive()
+        self._check_alternatives(scores)
+        s = self._session(seq_id)
+        self._drain()
+        if s.state == "active":
+            raise RuntimeError(f"sequence {seq_id} is still generating")
+        if not s.scheduled or not self.cache.has(seq_id):
+            raise ValueError(f"sequence {seq_id} has nothing in the cache that could be shared")
+        if len(self._sessions) + len(overrides) > self.config.max_sessions:
+            raise RuntimeError(f"max_sessions ({self.config.max_sessions}) reached")
+        params = [self._params(o) for o in overrides]
+        held = self.cache.length(seq_id)
+        at = held if length is None else int(length)
+        children = list(range(self._next_id, self._next_id + len(params)))
+        self.cache.fork(seq_id, children, at)
+        self._next_id += len(params)
+        rest = self.scheduler.seqs[seq_id].tokens[at:] + s.pending if length is None else []
+        for sid, p in zip(children, params):
+            self.scheduler.fork_request(seq_id, sid, at)
+            self._sessions[sid] = _Session(p, make_generator(p.seed), list(rest), 0, state="parked", scheduled=True, alternatives=scores)
+        return children
+
+    def scores(self, seq_id: int) -> List[TokenScore]:
+        """The scores of the tokens that the sequence has emitted since the last call, one for each event of ``step``."""
+        s = self._session(seq_id)
+        if s.alternatives is None:
+            raise ValueError(f"sequence {seq_id} was created without scores")
+        out, s.scores = s.scores, []
+        return out
 
     def set_decode_budget(self, seq_id: int, max_tokens: Optional[int] = None) -> None:
         """New tokens allowed in the turns that follow; None: only the stop token ends a turn
@@ -255,6 +303,17 @@ class Engine:
         uniform = [0.0 if s.params.greedy else s.draw() for s in sessions]
         with profiling.scope("launch (sampling)"):
             self.sampler.sample_on_device(logits, [s.params for s in sessions], (), uniform)
+        scores = None
+        top = max((x.alternatives for x in sessions if x.alternatives is not None), default=None)
+        if top is not None:
+            board = ScoreBoard(len(sampled), top, logits.device)
+            board.take(logits, self.sampler.last_ids)
+            n = ScoreBoard.n_words(len(sampled), top)
+            buf = self._host_scores[self._host_next]
+            if buf is None or buf.host.numel() < n:
+                buf = self._host_scores[self._host_next] = ops.Pinned(max(1024, n), torch.float32)
+            buf.from_device(board.words, n)
+            scores = (buf, top)
         # the error words of the kernels with bounded waits travel with the ids, in one copy: no synchronisation of their own
         ops.gather_wait_words(self.sampler.head)
         n_words = Sampler.HEAD + len(sampled)
@@ -265,7 +324,7 @@ class Engine:
         report.from_device(self.sampler.report(len(sampled)), n_words)
         for r in sampled:
             self.scheduler.on_sampled(r)
-        return _Inflight(sampled, {r: i for i, r in enumerate(sampled)}, report, uniform)
+        return _Inflight(sampled, {r: i for i, r in enumerate(sampled)}, report, uniform, scores)
 
     def _collect(self, flight: "_Inflight") -> List[Tuple[int, int, bool]]:
         """Wait for a pass's sampled ids and book them: events ``(seq_id, token, finished)``."""
@@ -279,7 +338,11 @@ class Engine:
             self._inflight = None
             raise EngineFailed(f"a forward pass did not complete: {what}") from self._failed
         events = []
-        for rid, tok in zip(flight.sampled, words[Sampler.HEAD:]):
+        scored: List[TokenScore] = []
+        if flight.scores is not None:
+            board, top = flight.scores              # (copied in front of the report, which has arrived)
+            scored = ScoreBoard.read(board.host, len(flight.sampled), top, words[Sampler.HEAD:])
+        for i, (rid, tok) in enumerate(zip(flight.sampled, words[Sampler.HEAD:])):
             if rid not in self.scheduler.seqs:
                 continue                            # released while the pass was in flight
             if rid in flight.void:
@@ -288,6 +351,9 @@ class Engine:
                 if rid in self._sessions and not self._sessions[rid].params.greedy:
                     self._sessions[rid].redraw = flight.uniform[flight.row_of[rid]]
                 continue
+            if scored and rid in self._sessions and self._sessions[rid].alternatives is not None:
+                del scored[i].alternatives[self._sessions[rid].alternatives:]
+                self._sessions[rid].scores.append(scored[i])
             finished = self.scheduler.on_token(rid, tok, self.eos_id)
             if finished:
                 self.scheduler.park(rid)            # pages stay until release (engine.cpp:770-788)
@@ -383,3 +449,119 @@ class Engine:
                         self.release(sid)
                         del owner[sid]
         return results
+
+    # ------------------------------------------------------------------ several scored continuations, scored prompts
+    def candidates(self, prompt: Sequence[int], n: int, max_new_tokens: int, temperature: Optional[float] = None, top_k: Optional[int] = None,
+                   top_p: Optional[float] = None, seed: Optional[int] = None, alternatives: int = 0) -> List[Candidate]:
+        """``n`` continuations of one prompt, the likeliest (by the mean log probability of its tokens) first.  The prompt goes through the model
+        once; its pages are shared by all continuations, and read once a step for all of them where that pays.  Needs ``n`` + 1 sessions.
+        ``seed``: continuation i draws with seed + i."""
+        self._alive()
+        prompt = [int(t) for t in prompt]
+        if n <= 0 or not prompt:
+            raise ValueError("candidates need a prompt of at least one token, and a number of them above 0")
+        shared = len(prompt) > 1
+        if len(self._sessions) + n + shared > self.config.max_sessions:
+            raise RuntimeError(f"{n} candidates need {n + shared} sessions; max_sessions is {self.config.max_sessions}")
+        common = {k: v for k, v in dict(temperature=temperature, top_k=top_k, top_p=top_p).items() if v is not None}
+        overrides = [dict(common, **({} if seed is None else {"seed": seed + i if seed >= 0 else seed})) for i in range(n)]
+        self._check_alternatives(alternatives)
+        ids: List[int] = []
+        anchor = None
+        try:
+            if shared:
+                # all of the prompt but its last token, through the model once; each continuation runs the last one for itself
+                anchor = self.create_session(prompt[:-1], {"temperature": 0.0})
+                self.feed(anchor, [], 1)
+                self._run_turns({anchor: []})
+                ids = self._fork(anchor, overrides, len(prompt) - 1, alternatives)
+                for sid in ids:
+                    self.feed(sid, prompt[-1:], max_new_tokens)
+                self.release(anchor)
+                anchor = None
+            else:
+                for o in overrides:
+                    ids.append(self.create_session(prompt, o, alternatives))
+                    self.feed(ids[-1], [], max_new_tokens)
+            tokens: Dict[int, List[int]] = {sid: [] for sid in ids}
+            self._run_turns(tokens)
+            found = [Candidate(tokens[sid], self.scores(sid)) for sid in ids]
+        finally:
+            for sid in ids + ([anchor] if anchor is not None else []):
+                self.release(sid)
+        return sorted(found, key=lambda c: -c.mean_logprob)
+
+    def _run_turns(self, tokens: Dict[int, List[int]]) -> None:
+        """Step until the turns of these sequences are over, their tokens appended; what other sequences emit meanwhile waits in the mailbox."""
+        running = set(tokens)
+        while running:
+            events = self.step(1)
+            if not events and not self.has_work():
+                break
+            for sid, tok, finished in events:
+                if sid in tokens:
+                    tokens[sid].append(tok)
+                    if finished:
+                        running.discard(sid)
+                else:
+                    self._mailbox.setdefault(sid, []).append((tok, finished))
+
+    def score(self, prompts: Sequence[Sequence[int]], alternatives: Optional[int] = None) -> List[List[TokenScore]]:
+        """How likely the model finds the tokens of each prompt: the scores of its second token to its last, given those before.  Without
+        ``alternatives`` log probability and entropy come straight from the hidden rows (``ops.head_scores``) and logits are never made; with it
+        (0 for none) ranks and so many alternatives come too.  Prompts run one behind the other in portions of ``max_chunk_size``, each
+        in pages that are given back at its end."""
+        self._alive()
+        self._drain()
+        self._check_alternatives(alternatives)
+        vocab = self.model.spec.vocab_size
+        prompts = [[int(t) for t in p] for p in prompts]
+        for p in prompts:
+            for t in p:
+                if not (0 <= t < vocab):
+                    raise ValueError(f"token id {t} outside the vocabulary [0, {vocab})")
+        results: List[List[TokenScore]] = []
+        portion = self.config.max_chunk_size
+        if alternatives is not None:
+            portion = min(portion, max(1, (1 << 25) // vocab))          # 128 MiB of logits at a time
+        for i, p in enumerate(prompts):
+            rid, out = ("score", i), []
+            try:
+                for at in range(0, len(p) - 1, portion):
+                    some = p[at:min(at + portion, len(p) - 1)]
+                    given = p[at + 1:at + 1 + len(some)]
+                    entry = StepEntry(rid, some, range(len(some)))
+                    if alternatives is None:
+                        logprob, entropy = self.runner.score([entry], given).tolist()
+                        out += [TokenScore(t, a, b) for t, a, b in zip(given, logprob, entropy)]
+                    else:
+                        logits = self.runner.step([entry])
+                        board = ScoreBoard(len(some), alternatives, logits.device)
+                        board.take(logits, torch.tensor(given, dtype=torch.int32, device=logits.device))
+                        out += ScoreBoard.read(board.words.cpu(), len(some), alternatives, given)
+                    self.forwards += 1
+                    try:
+                        ops.check_wait_words()
+                    except ops.DeviceWaitError as e:
+                        self._failed = e
+                        raise EngineFailed(f"a forward pass did not complete: {e}") from e
+            finally:
+                if self.cache.has(rid):
+                    self.cache.close(rid)
+            results.append(out)
+        return results
+
+    def resize_cache(self, num_pages: int) -> None:
+        """Give the cache pools of ``num_pages`` pages: what sequences hold moves into them, the old ones' memory is given back.  Refused where the
+        sequences hold more, or one of them could no longer reach the end of its turn."""
+        self._alive()
+        self._drain()
+        num_pages = int(num_pages)
+        for sid in self.scheduler.seqs:
+            q = self.scheduler.seqs[sid]
+            most = len(q.tokens) + (max(0, q.max_new_tokens - q.n_generated) if self._sessions[sid].state == "active" else 0)
+            if -(-most // self.cache.page_size) > num_pages:
+                raise ValueError(f"sequence {sid} may need {most} tokens: {num_pages} pages of {self.cache.page_size} do not hold them")
+        self.cache.resize(num_pages)
+        self.config.num_pages = num_pages
+        self.runner.forget_addresses()

@@ -21,7 +21,7 @@ import torch
 
 from .. import host, ops, profiling
 from ..cache.manager import CacheManager, OutOfPages
-from ..parts.base import CacheView, HostBatch, StepContext
+from ..parts.base import CacheView, HostBatch, SharedPages, StepContext
 
 
 @dataclass
@@ -86,6 +86,8 @@ class ModelRunner:
         # gained (a few hundred bytes for a decode step instead of the whole [sequences, width] table).
         # PULSAR_RESIDENT_TABLES=0: every step brings whole tables.
         self.resident_tables = os.environ.get("PULSAR_RESIDENT_TABLES", "1") != "0"
+        # Groups whose dense attention reads pages that forked requests share once for all of them (``_find_shared``).
+        self._sharable = [g for g, _ in self._sharing if cache.groups[g].need.window is None]
         # For looking inside a step: called as layer_hook(index in the run order, residual, pending delta) behind every
         # layer call (the stream is residual + delta where a delta is pending).  A step with a hook is never captured.
         self.layer_hook = None
@@ -259,6 +261,8 @@ class ModelRunner:
                 ctx.group_tables.append(table)
             else:
                 ctx.group_tables.append(views[8 + 2 * g])
+        if ctx.all_decode and s > 1 and self._sharable:
+            self._find_shared(ctx, rids)
         if moved:
             ops.move_ids(ctx.token_ids, views[-2], views[-1], sampled_ids)
         if self.position_axes > 1:
@@ -273,6 +277,51 @@ class ModelRunner:
                 at += q
             ctx.position_axes = axes.to(self.device, non_blocking=True)
         return ctx
+
+    # A step takes the attention over shared pages where that saves reading at least so many keys.  (Beside it norm, rotation and cache write are
+    # a launch of their own, and the other finds shared pages in L2.  A step of 12 layers of the 8B sizes, us without and with it: 8 forks of 2,000
+    # tokens, 14,000 keys saved, 3,225 and 3,364; of 4,000 tokens 3,498 and 3,421; of 8,000 4,102 and 3,554; 16 of 2,000 3,919 and 3,751; 32 of
+    # 500, 15,500 saved, 3,572 and 3,782; 32 of 8,000 8,043 and 4,263; 64 of 500 4,305 and 4,048.)
+    SHARED_KEYS_SAVED = 24576
+
+    def _find_shared(self, ctx: StepContext, rids) -> None:
+        """Fill ``ctx.shared_pages``: per group members, starts and shared lengths, in memory that stays where it is (captured steps read it)."""
+        lib, handle, n = self.cache._lib, self.cache._h, ctx.n_seqs
+        for g in self._sharable:
+            if lib.ph_n_shared_pages(handle, g) == 0:
+                continue
+            stage = self._stage(3 * n + 1)
+            words = (ctypes.c_int * (3 * n + 1)).from_address(stage.host.data_ptr())
+            members, starts, shared = (ctypes.cast(ctypes.addressof(words) + 4 * at, host._IP) for at in (0, n, 2 * n + 1))
+            most = (ctypes.c_int * 2)()
+            families = lib.ph_families(handle, g, n, rids, members, starts, shared, most)
+            if families <= 0:
+                continue
+            in_families = starts[families]
+            saved = sum((starts[f + 1] - starts[f] - 1) * shared[members[starts[f]]] for f in range(families))
+            if saved < self.SHARED_KEYS_SAVED:
+                continue
+            room = self.scratch(f"shared.{g}", (3 * self.cache.max_requests + 1,), torch.int32)
+            stage.to_device(room, 3 * n + 1)
+            self.h2d_bytes += 4 * (3 * n + 1)
+            ctx.shared_pages[g] = SharedPages(room[:in_families], room[n:n + families + 1], room[2 * n + 1:3 * n + 1], most[0], most[1])
+
+    def score(self, entries: Sequence[StepEntry], given: Sequence[int]) -> torch.Tensor:
+        """Run the given tokens as ``step`` does and return float32 [2, wanted]: at every wanted position the log probability of that
+        position's token of ``given`` coming next, and the entropy of what may come.  Logits are not made (``ops.head_scores``).  The
+        tensor is scratch memory: it is valid until the next step."""
+        given = [int(t) for t in given]
+        if len(given) != sum(len(e.want) for e in entries):
+            raise StepError(f"{sum(len(e.want) for e in entries)} positions are wanted, {len(given)} tokens given")
+        ctx = self.prepare(entries)
+        stage = self._stage(max(1, len(given)))
+        stage.host[:len(given)] = torch.tensor(given, dtype=torch.int32)
+        ctx.given_tokens = self.scratch("score.given", (len(given),), torch.int32)
+        stage.to_device(ctx.given_tokens, len(given))
+        with torch.cuda.device(self.device):
+            scores = self.model.forward(ctx)
+        self.steps_run += 1
+        return scores
 
     def step(self, entries: Sequence[StepEntry], sampled_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Run the given tokens as one batch from the cache that earlier steps left and
@@ -297,6 +346,7 @@ class ModelRunner:
             self._graph_seen.clear()
             self._graph_epoch = self.scratch_epoch
         key = (ctx.n_tokens, ctx.n_seqs, int(ctx.logit_rows.numel()), ctx.table_widths, ctx.uneven,
+               tuple((g, f.members.numel(), f.family_start.numel(), f.most_members, f.most_shared) for g, f in ctx.shared_pages.items()),
                tuple(int(t.data_ptr()) for t in (ctx.token_ids, ctx.logit_rows)))
         hit = self._graphs.get(key)
         if hit is not None:
@@ -333,6 +383,10 @@ class ModelRunner:
         graph.replay()
         self.graph_replays += 1
         return logits
+
+    def forget_addresses(self) -> None:
+        """The cache's pools are elsewhere: captured steps hold stale addresses."""
+        self.scratch_epoch += 1
 
     def finish(self, rid: Hashable) -> None:
         """The request is over: everything it holds goes back to the pools."""

@@ -148,7 +148,8 @@ class DecoderModel(Part):
         return None
 
     def forward(self, ctx: StepContext) -> torch.Tensor:
-        """Logits float32 [len(ctx.logit_rows), vocab] for the tokens of ``ctx``."""
+        """Logits float32 [len(ctx.logit_rows), vocab] for the tokens of ``ctx``; with ``ctx.given_tokens`` their log probabilities and the
+        entropies, float32 [2, len(ctx.logit_rows)]."""
         s = self.spec
         residual = ctx.scratch("residual", (ctx.n_tokens, s.hidden), torch.float32)
         ops.embed(self.embed, ctx.token_ids, residual, s.embedding_multiplier)
@@ -175,6 +176,12 @@ class DecoderModel(Part):
             if ctx.on_layer is not None:
                 ctx.on_layer(i, residual, delta)
         rows = ctx.logit_rows
+        if ctx.given_tokens is not None:
+            scores = ctx.scratch("scores", (2, rows.numel()), torch.float32)
+            if rows.numel():
+                h = self.final_norm.forward(ctx, residual, delta, rows=rows)
+                ops.head_scores(h, self.head, ctx.given_tokens, scores[0], scores[1], s.logit_scale, s.logit_softcap)
+            return scores
         logits = ctx.scratch("logits", (rows.numel(), s.vocab_size), torch.float32)
         if rows.numel():
             h = self.final_norm.forward(ctx, residual, delta, rows=rows)

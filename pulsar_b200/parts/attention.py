@@ -313,6 +313,19 @@ class Attention(Mixer):
         else:
             cos = sin = ctx.scratch("attn.norope", (n, 0), torch.float32)
             rotary = 0
+        shared = ctx.shared_pages.get(cache.group)
+        if shared is not None and s.window is None:
+            # forked sequences: the pages they share are read once for all of them
+            ops.qk_norm_rope_write(qkv, q, cache.k_pool if n_kv else None, cache.v_pool if n_kv else None, cache.slots if n_kv else None, cos, sin,
+                                   self.q_norm, self.k_norm, s.qk_norm_eps or 0.0, s.n_heads, n_kv, s.head_dim, rotary, cache.page_size)
+            o = ctx.scratch("attn.o", (n, s.n_heads, s.head_dim))
+            n_kv_heads, page_size = cache.k_pool.shape[1], cache.page_size
+            need = ops.shared_scratch(n, shared.family_start.numel() - 1, shared.most_members, shared.most_shared, cache.block_table.shape[1] * page_size,
+                                      s.n_heads, n_kv_heads, s.head_dim, page_size, q.dtype)
+            ops.paged_attention_shared(q, cache.k_pool, cache.v_pool, o, cache.block_table, ctx.kv_len, shared.shared_len, shared.members,
+                                       shared.family_start, shared.most_members, shared.most_shared, s.scale,
+                                       ctx.scratch("attn.partial", (need,), torch.float32))
+            return o
         # (A lone sequence keeps the kernel of its own: its keys are cut into so many splits that every block's share
         # is short, and the norm and rotation in each block's start then cost more than the launch they save:
         # 2.990 against 2.973 ms per step; with two sequences and more the one kernel is ahead by 1.1 to 1.4 %.)

@@ -12,7 +12,7 @@ returns its contribution ``delta`` in the activation dtype and the next norm add
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Callable, Dict, List, Optional, Sequence, Tuple
+from typing import NamedTuple, Callable, Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -65,6 +65,15 @@ class HostBatch:
         return [k - q for q, k in zip(self.q_lens, self.kv_lens)]
 
 
+class SharedPages(NamedTuple):
+    """Families of a step's sequences whose first keys lie in the same pages, as ``ops.paged_attention_shared`` takes them."""
+    members: torch.Tensor           # int32 [members of all families]
+    family_start: torch.Tensor      # int32 [families + 1]
+    shared_len: torch.Tensor        # int32 [S]
+    most_members: int
+    most_shared: int
+
+
 class StepContext:
     """Device arrays of one step plus scratch memory.  Built by the step function."""
 
@@ -88,6 +97,10 @@ class StepContext:
         self.logit_rows = None                                          # [R]
         self.group_tables: List[torch.Tensor] = []                      # per group [S, width]
         self.group_slots: List[torch.Tensor] = []                       # per group [N]
+        # Of a step of single tokens, by group: the sequences that share pages (see ``SharedPages``), where any do.
+        self.shared_pages: Dict[int, SharedPages] = {}
+        # int32 [R]: the tokens whose log probabilities at ``logit_rows`` are asked for instead of logits (see ``ModelRunner.score``)
+        self.given_tokens: Optional[torch.Tensor] = None
         self.shared: Dict[object, object] = {}                          # per-step tables shared by layers
         # What a product has prepared for the norm that follows it, by that norm's id: (residual * norm weight in
         # the activation dtype, parts of the rows' sums of squares).  Valid while nothing else touches the residual.

@@ -1,1 +1,2 @@
 from .sampler import GenerationParams, Sampler, make_generator
+from .scores import Candidate, ScoreBoard, TokenScore
