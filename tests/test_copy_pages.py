@@ -56,8 +56,8 @@ def test_into_other_pools_more_than_one_launch_and_strided_entries():
 
 
 @cuda
-@pytest.mark.parametrize("shift", [1, 2, 4, 8])
-def test_addresses_that_are_no_multiple_of_sixteen(shift):
+@pytest.mark.parametrize("shift", [1, 2, 4, 8, 16, 32])
+def test_addresses_of_any_alignment(shift):
     base = _pool((1 << 14,), torch.uint8, 5)
     pool = base[shift:shift + 3 * 8 * 160].view(3, 8, 160)
     before = base.clone()
