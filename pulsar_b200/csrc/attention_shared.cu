@@ -492,11 +492,6 @@ int make_map(CUtensorMap* map, const void* pool, long long rows, int D, int page
     return rc == CUDA_SUCCESS ? 0 : PB_ERR_BAD_SIZE;
 }
 
-struct Maps {
-    CUtensorMap k, v;
-    unsigned int* error;
-};
-
 template <int D, int ROW_TILES>
 int launch_tc(const void* q, const Maps& maps, float* partial, const Shared& p, int G, bool beside, cudaStream_t stream) {
     const long long shared = family_blocks(p, G, ROW_TILES * 16), items = (shared + own_blocks(p, G, 16)) * p.Hkv;
@@ -527,7 +522,7 @@ int launch_tc(const void* q, const void* k_pool, const void* v_pool, float* part
     if (rc != 0) return rc;
     const int rows = p.n_families > 0 ? p.most_members * G : 0;
     if (tcgen05_takes(rows, D)) {
-        rc = launch_tcgen05(q, k_pool, v_pool, partial, p, n_pages, error, stream);
+        rc = launch_tcgen05(q, maps, partial, p, stream);
         if (rc != 0) return rc;
         p.n_families = 0;                                 // (n_shared stays: it is where a sequence's own parts begin)
         return launch_tc<128, 1>(q, maps, partial, p, G, true, stream);

@@ -3,6 +3,8 @@
 
 #include "common.cuh"
 
+#include <cuda.h>
+
 namespace pb {
 namespace shared_attention {
 
@@ -98,10 +100,15 @@ inline long long family_blocks(const Shared& p, int G, int rows) { return (long 
 
 inline long long own_blocks(const Shared& p, int G, int rows) { return (long long)p.n_seqs * ((G + rows - 1) / rows) * p.n_own; }
 
+// The pools as rows of D dimensions, a box a page of 64 of them with 128-byte swizzle, and the word of waits that ran out.
+struct Maps {
+    CUtensorMap k, v;
+    unsigned int* error;
+};
+
 // The shared sides on the fifth-generation tensor cores (attention_shared_tcgen05.cu): head size 128, pages of 8 to 64 keys.
 constexpr int kTcgen05Rows = 128;
-int launch_tcgen05(const void* q, const void* k_pool, const void* v_pool, float* partial, const Shared& p, int n_pages, unsigned int* error,
-                   cudaStream_t stream);
+int launch_tcgen05(const void* q, const Maps& maps, float* partial, const Shared& p, cudaStream_t stream);
 
 }  // namespace shared_attention
 }  // namespace pb

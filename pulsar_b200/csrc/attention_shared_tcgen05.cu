@@ -287,21 +287,16 @@ shared_tcgen05_kernel(const bf16* __restrict__ q, const __grid_constant__ CUtens
 namespace pb {
 namespace shared_attention {
 
-int launch_tcgen05(const void* q, const void* k_pool, const void* v_pool, float* partial, const Shared& p, int n_pages, unsigned int* error,
-                   cudaStream_t stream) {
-    const long long blocks = family_blocks(p, p.Hq / p.Hkv, kTcgen05Rows), pool_rows = (long long)n_pages * p.Hkv * p.page_size;
-    if (blocks > 0x7fffffff || pool_rows > 0x7fffffff) return PB_ERR_TOO_LARGE;
-    CUtensorMap map_k, map_v;
-    int rc = attn5::make_map(&map_k, k_pool, pool_rows, kD, p.page_size);
-    if (rc == 0) rc = attn5::make_map(&map_v, v_pool, pool_rows, kD, p.page_size);
-    if (rc != 0) return rc;
+int launch_tcgen05(const void* q, const Maps& maps, float* partial, const Shared& p, cudaStream_t stream) {
+    const long long blocks = family_blocks(p, p.Hq / p.Hkv, kTcgen05Rows);
+    if (blocks > 0x7fffffff) return PB_ERR_TOO_LARGE;
     static SmemLimit limit;
     static DeviceLimit most;
-    rc = limit.allow(shared_tcgen05_kernel, kSmemBytes);
+    int rc = limit.allow(shared_tcgen05_kernel, kSmemBytes);
     if (rc == 0) rc = share_most(most, shared_tcgen05_kernel);
     if (rc != 0) return rc;
-    shared_tcgen05_kernel<<<dim3((unsigned)blocks, p.Hkv), kThreads, kSmemBytes, stream>>>((const bf16*)q, map_k, map_v, partial, p, attn5::log2_exact(p.page_size),
-                                                                                           pool_bounds_now(), error);
+    shared_tcgen05_kernel<<<dim3((unsigned)blocks, p.Hkv), kThreads, kSmemBytes, stream>>>((const bf16*)q, maps.k, maps.v, partial, p, attn5::log2_exact(p.page_size),
+                                                                                           pool_bounds_now(), maps.error);
     return launch_status();
 }
 

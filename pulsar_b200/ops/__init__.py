@@ -1933,8 +1933,10 @@ def _page_run(pool: torch.Tensor) -> Tuple[torch.Size, int, int]:
     shape = pool.shape
     if len(shape) < 2:
         raise KernelError(f"copy_pages: a pool is [entries, pages, ...], found {tuple(shape)}")
-    strides, page = pool.stride(), 1
-    fits = True
+    strides = pool.stride()
+    if shape[1] > 1 and pool.is_contiguous():
+        return shape, strides[0], strides[1]
+    page, fits = 1, True
     for size, stride in zip(reversed(shape[2:]), reversed(strides[2:])):
         fits = fits and (size == 1 or stride == page)
         page *= size
