@@ -8,6 +8,10 @@
 // family's sequences there are: bound by the bytes of the keys and values.  (mma.sync takes 2,100 cycles for 32 rows x 64 keys, with two
 // blocks an SM as long as the bytes do, and so many times that for larger families.)
 //
+// A thread takes 128 exponentials a tile, 1,900 cycles with all that goes with them, more than the tile's bytes take where SMs are idle.  So
+// families of up to 64 rows stand in tensor memory twice, of up to 32 four times: each copy has its own half or quarter of a tile's keys,
+// writes zeros for the weights of the others, and the copies' sums are joined at the end (REPEAT).
+//
 // Roles: warps 0-3 softmax (and the gathering of the query rows, which lie with their sequences), warp 4 issues the products, warp 5 brings K
 // and warp 6 V, a lane per half page.  S has two buffers, S of the next tile is issued before O += P V of this one.  The maximum moves only
 // when it grew by more than 2^8; O is rescaled in tensor memory only then, and the sums use the same maximum.
@@ -37,6 +41,10 @@ struct Sync {
     int gave_up;
 };
 
+// The four softmax warps meet here.
+__device__ __forceinline__ void meet() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+template <int REPEAT>
 __global__ void __launch_bounds__(kThreads, 1)
 shared_tcgen05_kernel(const bf16* __restrict__ q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                       float* __restrict__ partial, const Shared p, int page_shift, const PoolBounds bounds, unsigned int* error) {
@@ -48,17 +56,23 @@ shared_tcgen05_kernel(const bf16* __restrict__ q, const __grid_constant__ CUtens
     __shared__ Sync sync;
     pdl_trigger();                               // launched the ordinary way: the sequences' own sides may run beside it
     const int G = p.Hq / p.Hkv, kvh = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    Item it;
-    if (!family_item<kBM, kBN>(p, blockIdx.x, G, it)) return;
-    const int n_tiles = it.begin < it.end ? (it.end - it.begin + kBN - 1) / kBN : 0;          // (a split begins at a multiple of kBN)
-    const int active = (it.rows + 31) / 32;      // softmax warps that have rows
     volatile int* abort_flag = &sync.gave_up;
-
+    if (warp == 4) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sync.tmem)), "r"(kTmemColumns));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    Item it;
+    const bool any = family_item<kBM / REPEAT, kBN>(p, blockIdx.x, G, it);
+    if (!any) it.begin = it.end = it.rows = 0;
+    const int n_tiles = (it.end - it.begin + kBN - 1) / kBN;              // (a split begins at a multiple of kBN)
+    // softmax warp w has rows (w % kGroups) * 32 .. and copy w / kGroups of them
+    constexpr int kGroups = 4 / REPEAT, kKeys = kBN / REPEAT;
+    const int active = (it.rows + 31) / 32 * REPEAT;                      // softmax warps that have rows
     if (tid == 128) {
         mbar_init(smem_addr(&sync.q_full), 4);
         mbar_init(smem_addr(&sync.o_full), 1);
         mbar_init(smem_addr(&sync.o_done), 1);
-        for (int i = 0; i < 2; ++i) { mbar_init(smem_addr(&sync.s_full[i]), 1); mbar_init(smem_addr(&sync.p_full[i]), active); }
+        for (int i = 0; i < 2; ++i) { mbar_init(smem_addr(&sync.s_full[i]), 1); mbar_init(smem_addr(&sync.p_full[i]), max(1, active)); }
         for (int i = 0; i < kStages; ++i) {
             mbar_init(smem_addr(&sync.k_full[i]), 1); mbar_init(smem_addr(&sync.k_empty[i]), 1);
             mbar_init(smem_addr(&sync.v_full[i]), 1); mbar_init(smem_addr(&sync.v_empty[i]), 1);
@@ -73,10 +87,6 @@ shared_tcgen05_kernel(const bf16* __restrict__ q, const __grid_constant__ CUtens
         for (int i = tid; i < (kBN - last_rows) * 16; i += kThreads)
             *reinterpret_cast<uint4*>(tile + (i & 8 ? kHalfBytes : 0) + (last_rows + (i >> 4)) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
-    if (warp == 4) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sync.tmem)), "r"(kTmemColumns));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
     fence_before();
     __syncthreads();
@@ -152,16 +162,17 @@ shared_tcgen05_kernel(const bf16* __restrict__ q, const __grid_constant__ CUtens
         }
         if (!ok && lane == 0) { *abort_flag = 1; atomicMax(error, 3u); }
     } else {
-        // ---------------- softmax: thread r owns query row r
-        const int r = warp * 32 + lane;
-        long long row = -1;                                       // sequence * Hq + head
-        if (r < it.rows) {
-            const int seq = it.seq_of(p, r, G);
-            if (seq >= 0 && seq < p.n_seqs) row = (long long)seq * p.Hq + it.head_of(kvh, r, G);
+        // ---------------- softmax: thread r owns lane r of tensor memory, a copy of a query row
+        const int r = warp * 32 + lane, i = warp % kGroups * 32 + lane, copy = warp / kGroups;
+        const bool has_rows = warp % kGroups * 32 < it.rows;
+        int row = -1;                                             // sequence * Hq + head
+        if (i < it.rows) {
+            const int seq = it.seq_of(p, i, G);
+            if (seq >= 0 && seq < p.n_seqs) row = seq * p.Hq + it.head_of(kvh, i, G);
         }
-        // its query, into the swizzled tile (rows without one stay what they are: they meet nobody else's sums)
+        // its query, into the swizzled tile (lanes without one keep what lies there: they meet nobody else's sums)
         if (row >= 0) {
-            const uint4* from = reinterpret_cast<const uint4*>(q + row * kD);
+            const uint4* from = reinterpret_cast<const uint4*>(q + (size_t)row * kD);
 #pragma unroll
             for (int c = 0; c < kD / 8; ++c)
                 *reinterpret_cast<uint4*>(q_s + (c >> 3) * kHalfBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = from[c];
@@ -172,26 +183,27 @@ shared_tcgen05_kernel(const bf16* __restrict__ q, const __grid_constant__ CUtens
         const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
         float m_used = -INFINITY, l_run = 0.0f;
         bool ok = true;
-        for (int j = 0; j < n_tiles && warp < active; ++j) {
+        for (int j = 0; j < n_tiles && has_rows; ++j) {
             const uint32_t ts = tmem_s + (uint32_t)(j & 1) * kBN + lane_addr;
             ok = mbar_wait(smem_addr(&sync.s_full[j & 1]), (j >> 1) & 1, abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             fence_after();
-            uint32_t v[kBN];
+            // the copy's keys are columns [copy * kKeys, + kKeys)
+            uint32_t v[kKeys];
 #pragma unroll
-            for (int c = 0; c < kBN; c += 32) tmem_ld32_nowait(ts + c, *reinterpret_cast<uint32_t(*)[32]>(&v[c]));
+            for (int c = 0; c < kKeys; c += 32) tmem_ld32_nowait(ts + copy * kKeys + c, *reinterpret_cast<uint32_t(*)[32]>(&v[c]));
             tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < kBN; c += 32) tmem_landed(*reinterpret_cast<uint32_t(*)[32]>(&v[c]));
-            const int valid = it.end - it.begin - j * kBN;
-            if (valid < kBN) {
+            for (int c = 0; c < kKeys; c += 32) tmem_landed(*reinterpret_cast<uint32_t(*)[32]>(&v[c]));
+            const int valid = it.end - it.begin - j * kBN - copy * kKeys;
+            if (valid < kKeys) {
 #pragma unroll
-                for (int i = 0; i < kBN; ++i) v[i] = i < valid ? v[i] : __float_as_uint(-INFINITY);
+                for (int k = 0; k < kKeys; ++k) v[k] = k < valid ? v[k] : __float_as_uint(-INFINITY);
             }
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < kBN; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[i]));
+            for (int k = 0; k < kKeys; ++k) top[k & 3] = fmaxf(top[k & 3], __uint_as_float(v[k]));
             const float highest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
             float f = 1.0f;
             if ((highest - m_used) * p.scale_log2 > kLazyRescale) {       // also the first keys: m_used = -inf
@@ -201,18 +213,26 @@ shared_tcgen05_kernel(const bf16* __restrict__ q, const __grid_constant__ CUtens
             }
             const float lower = m_used == -INFINITY ? 0.0f : -m_used * p.scale_log2;
             float l0 = 0.0f, l1 = 0.0f;
+            // the weights, two a column, over the first half of S; every lane of the warp has read its scores
+            uint32_t pk[16];
 #pragma unroll
-            for (int c = 0; c < kBN; c += 32) {
-                uint32_t pk[16];
+            for (int c = 0; c < kBN / 2; c += 16) {
+                if (c >= copy * kKeys / 2 && c < (copy + 1) * kKeys / 2) continue;
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float p0 = ex2(fmaf(__uint_as_float(v[c + i]), p.scale_log2, lower));
-                    const float p1 = ex2(fmaf(__uint_as_float(v[c + i + 1]), p.scale_log2, lower));
+                for (int k = 0; k < 16; ++k) pk[k] = 0u;
+                tmem_st16(ts + c, pk);
+            }
+#pragma unroll
+            for (int c = 0; c < kKeys; c += 32) {
+#pragma unroll
+                for (int k = 0; k < 32; k += 2) {
+                    const float p0 = ex2(fmaf(__uint_as_float(v[c + k]), p.scale_log2, lower));
+                    const float p1 = ex2(fmaf(__uint_as_float(v[c + k + 1]), p.scale_log2, lower));
                     l0 += p0;
                     l1 += p1;
-                    pk[i >> 1] = pack_bf16x2(p0, p1);
+                    pk[k >> 1] = pack_bf16x2(p0, p1);
                 }
-                tmem_st16(ts + (c >> 1), pk);
+                tmem_st16(ts + copy * (kKeys / 2) + (c >> 1), pk);
             }
             l_run += l0 + l1;
             if (j > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
@@ -234,41 +254,56 @@ shared_tcgen05_kernel(const bf16* __restrict__ q, const __grid_constant__ CUtens
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_addr(&sync.p_full[j & 1]));
         }
-        if (ok && warp < active) {
-            const int parts = p.n_shared + p.n_own;
-            // a thread has a row, a warp writes a row: they change places in shared memory, which the products have done with
-            constexpr int kPitch = kD + 4;
-            float* rows = reinterpret_cast<float*>(k_s) + warp * 32 * kPitch;
-            if (n_tiles > 0) {
-                ok = mbar_wait(smem_addr(&sync.o_done), 0, abort_flag);
-                ok = __all_sync(0xffffffffu, ok);
-                fence_after();
-            }
-            if (ok) {
+        // a thread has a row's copy, a warp writes a row: they meet in shared memory, which the products have done with
+        constexpr int kPitch = kD + 4;
+        float* rows = reinterpret_cast<float*>(k_s);                      // [128][kPitch]
+        float4* ends = reinterpret_cast<float4*>(rows + kBM * kPitch);    // [128]: m, l, the row's number
+        if (n_tiles > 0 && ok) {
+            ok = mbar_wait(smem_addr(&sync.o_done), 0, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            fence_after();
+        }
+        if (has_rows) {
 #pragma unroll 1
-                for (int c = 0; c < kD; c += 32) {
-                    uint32_t o[32];
-                    if (n_tiles > 0) {
-                        tmem_ld32(tmem_o + lane_addr + c, o);
-                    } else {
+            for (int c = 0; c < kD; c += 32) {
+                uint32_t o[32];
+                if (n_tiles > 0) {
+                    tmem_ld32(tmem_o + lane_addr + c, o);
+                } else {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = 0u;
-                    }
+                    for (int k = 0; k < 32; ++k) o[k] = 0u;
+                }
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(rows + lane * kPitch + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4*>(rows + r * kPitch + c + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+            }
+            ends[r] = make_float4(m_used == -INFINITY ? m_used : m_used * p.scale_log2, l_run, __int_as_float(row), 0.0f);
+        }
+        meet();
+        if (ok) {
+            const int parts = p.n_shared + p.n_own;
+            for (int k = warp; k < it.rows; k += 4) {
+                float m = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < REPEAT; ++c) m = fmaxf(m, ends[c * (kBM / REPEAT) + k].x);
+                const float base = m == -INFINITY ? 0.0f : m;
+                float2 a = make_float2(0.0f, 0.0f), b = a;
+                float l = 0.0f;
+#pragma unroll
+                for (int c = 0; c < REPEAT; ++c) {
+                    const int from = c * (kBM / REPEAT) + k;
+                    const float f = ex2(ends[from].x - base);
+                    const float2* o = reinterpret_cast<const float2*>(rows + from * kPitch);
+                    const float2 x = o[lane], y = o[lane + 32];
+                    a.x = fmaf(x.x, f, a.x); a.y = fmaf(x.y, f, a.y);
+                    b.x = fmaf(y.x, f, b.x); b.y = fmaf(y.y, f, b.y);
+                    l = fmaf(ends[from].y, f, l);
                 }
-                __syncwarp();
-                const float m_log2 = m_used == -INFINITY ? m_used : m_used * p.scale_log2;
-                for (int i = 0; i < 32; ++i) {
-                    const long long to = __shfl_sync(0xffffffffu, row, i);
-                    const float m = __shfl_sync(0xffffffffu, m_log2, i), l = __shfl_sync(0xffffffffu, l_run, i);
-                    if (to < 0) continue;
-                    float* dst = partial + (to * parts + it.part) * (kD + 2);
-                    const float2* from = reinterpret_cast<const float2*>(rows + i * kPitch);
-                    reinterpret_cast<float2*>(dst)[lane] = from[lane];
-                    reinterpret_cast<float2*>(dst)[lane + 32] = from[lane + 32];
-                    if (lane == 0) *reinterpret_cast<float2*>(dst + kD) = make_float2(m, l);
-                }
+                const int to = __float_as_int(ends[k].z);
+                if (to < 0) continue;
+                float* dst = partial + ((size_t)to * parts + it.part) * (kD + 2);
+                reinterpret_cast<float2*>(dst)[lane] = a;
+                reinterpret_cast<float2*>(dst)[lane + 32] = b;
+                if (lane == 0) *reinterpret_cast<float2*>(dst + kD) = make_float2(m, l);
             }
         }
         if (!ok && lane == 0) { *abort_flag = 1; atomicMax(error, 4u); }
@@ -282,22 +317,29 @@ shared_tcgen05_kernel(const bf16* __restrict__ q, const __grid_constant__ CUtens
     if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_s), "r"(kTmemColumns));
 }
 
+template <int REPEAT>
+int launch_repeat(const void* q, const Maps& maps, float* partial, const Shared& p, cudaStream_t stream) {
+    const long long blocks = family_blocks(p, p.Hq / p.Hkv, kBM / REPEAT);
+    if (blocks > 0x7fffffff) return PB_ERR_TOO_LARGE;
+    static SmemLimit limit;
+    static DeviceLimit most;
+    int rc = limit.allow(shared_tcgen05_kernel<REPEAT>, kSmemBytes);
+    if (rc == 0) rc = share_most(most, shared_tcgen05_kernel<REPEAT>);
+    if (rc != 0) return rc;
+    shared_tcgen05_kernel<REPEAT><<<dim3((unsigned)blocks, p.Hkv), kThreads, kSmemBytes, stream>>>((const bf16*)q, maps.k, maps.v, partial, p,
+                                                                                                   attn5::log2_exact(p.page_size), pool_bounds_now(), maps.error);
+    return launch_status();
+}
+
 }  // namespace
 
 namespace pb {
 namespace shared_attention {
 
 int launch_tcgen05(const void* q, const Maps& maps, float* partial, const Shared& p, cudaStream_t stream) {
-    const long long blocks = family_blocks(p, p.Hq / p.Hkv, kTcgen05Rows);
-    if (blocks > 0x7fffffff) return PB_ERR_TOO_LARGE;
-    static SmemLimit limit;
-    static DeviceLimit most;
-    int rc = limit.allow(shared_tcgen05_kernel, kSmemBytes);
-    if (rc == 0) rc = share_most(most, shared_tcgen05_kernel);
-    if (rc != 0) return rc;
-    shared_tcgen05_kernel<<<dim3((unsigned)blocks, p.Hkv), kThreads, kSmemBytes, stream>>>((const bf16*)q, maps.k, maps.v, partial, p, attn5::log2_exact(p.page_size),
-                                                                                           pool_bounds_now(), maps.error);
-    return launch_status();
+    const int rows = p.most_members * (p.Hq / p.Hkv);
+    if (rows <= 32) return launch_repeat<4>(q, maps, partial, p, stream);
+    return rows <= 64 ? launch_repeat<2>(q, maps, partial, p, stream) : launch_repeat<1>(q, maps, partial, p, stream);
 }
 
 }  // namespace shared_attention

@@ -280,8 +280,8 @@ class ModelRunner:
 
     # A step takes the attention over shared pages where that saves reading at least so many keys.  (Beside it norm, rotation and cache write are
     # a launch of their own, and the other finds shared pages in L2.  A step of 12 layers of the 8B sizes, us without and with it: 8 forks of 2,000
-    # tokens, 14,000 keys saved, 3,225 and 3,364; of 4,000 tokens 3,498 and 3,421; of 8,000 4,102 and 3,554; 16 of 2,000 3,919 and 3,751; 32 of
-    # 500, 15,500 saved, 3,572 and 3,782; 32 of 8,000 8,043 and 4,263; 64 of 500 4,305 and 4,048.)
+    # tokens, 14,000 keys saved, 3,262 and 3,336; of 4,000 tokens 3,558 and 3,408; of 8,000 4,143 and 3,495; 16 of 2,000 3,941 and 3,741; 32 of
+    # 500, 15,500 saved, 3,591 and 3,829; 32 of 8,000 8,086 and 4,169; 64 of 500 4,353 and 4,111.)
     SHARED_KEYS_SAVED = 24576
 
     def _find_shared(self, ctx: StepContext, rids) -> None:
@@ -304,7 +304,8 @@ class ModelRunner:
             room = self.scratch(f"shared.{g}", (3 * self.cache.max_requests + 1,), torch.int32)
             stage.to_device(room, 3 * n + 1)
             self.h2d_bytes += 4 * (3 * n + 1)
-            ctx.shared_pages[g] = SharedPages(room[:in_families], room[n:n + families + 1], room[2 * n + 1:3 * n + 1], most[0], most[1])
+            most_own = max(length - shared[i] for i, length in enumerate(ctx.host.kv_lens))
+            ctx.shared_pages[g] = SharedPages(room[:in_families], room[n:n + families + 1], room[2 * n + 1:3 * n + 1], most[0], most[1], _align(most_own, 512))
 
     def score(self, entries: Sequence[StepEntry], given: Sequence[int]) -> torch.Tensor:
         """Run the given tokens as ``step`` does and return float32 [2, wanted]: at every wanted position the log probability of that
@@ -346,7 +347,7 @@ class ModelRunner:
             self._graph_seen.clear()
             self._graph_epoch = self.scratch_epoch
         key = (ctx.n_tokens, ctx.n_seqs, int(ctx.logit_rows.numel()), ctx.table_widths, ctx.uneven,
-               tuple((g, f.members.numel(), f.family_start.numel(), f.most_members, f.most_shared) for g, f in ctx.shared_pages.items()),
+               tuple((g, f.members.numel(), f.family_start.numel(), f.most_members, f.most_shared, f.most_own) for g, f in ctx.shared_pages.items()),
                tuple(int(t.data_ptr()) for t in (ctx.token_ids, ctx.logit_rows)))
         hit = self._graphs.get(key)
         if hit is not None:

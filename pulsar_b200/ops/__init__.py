@@ -2025,7 +2025,7 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tens
 
 def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, out: torch.Tensor, block_table: torch.Tensor,
                            kv_len: torch.Tensor, shared_len: torch.Tensor, members: torch.Tensor, family_start: torch.Tensor, most_members: int,
-                           most_shared: int, scale: float, partial: Optional[torch.Tensor] = None) -> None:
+                           most_shared: int, scale: float, partial: Optional[torch.Tensor] = None, most_own: Optional[int] = None) -> None:
     """Attention of one query token per sequence over a cache in which families of sequences share pages: q, out [S, Hq, D], pools
     [pages, Hkv, page, D], ``block_table`` [S, width], ``kv_len`` [S].  Family f is the sequences ``members[family_start[f]:family_start[f + 1]]``;
     they all have the same pages for their first ``shared_len[s]`` keys (whole pages, at most ``kv_len[s]``), which are read once for all
@@ -2033,7 +2033,8 @@ def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     (bfloat16 with pages of 8, 16, 32 or 64 keys and heads of 64 or 128 runs on the tensor cores; a wait that it gives up is reported in
     the tcgen05 attention's error word.)
     ``most_members`` and ``most_shared`` are the largest family's size and the longest shared length as the host knows them (more members
-    than that are not served).  ``partial``: float32 scratch of ``shared_scratch`` elements, made here where it is not given."""
+    than that are not served); ``most_own`` is the most keys that a sequence has beyond its shared ones, where the host knows (keys beyond
+    that are not seen).  ``partial``: float32 scratch of ``shared_scratch`` elements, made here where it is not given."""
     _cuda(q, k_pool, v_pool, out, block_table, kv_len, shared_len, members, family_start, partial)
     _check_against(k_pool)
     if q.dim() != 3 or k_pool.dim() != 4:
@@ -2052,6 +2053,8 @@ def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     if block_table.dim() != 2 or block_table.shape[0] != s or kv_len.numel() != s or shared_len.numel() != s or family_start.numel() == 0:
         raise KernelError(f"paged_attention_shared: {s} sequences need a table row, a length and a shared length each, and family_start one more "
                           "element than there are families")
+    if most_own is not None and most_own < 0:
+        raise KernelError(f"paged_attention_shared: most_own must not be negative, found {most_own}")
     if most_members < 0 or most_shared < 0 or most_members > s:
         raise KernelError(f"paged_attention_shared: most_members must lie in [0, {s}] and most_shared must not be negative, found {most_members}, {most_shared}")
     kind = code(q.dtype)
@@ -2060,7 +2063,10 @@ def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     if (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr() | out.data_ptr()) % 16:
         raise KernelError("paged_attention_shared: q, out and the pools must start at a multiple of 16 bytes")
     families = family_start.numel() - 1 if most_members > 0 and most_shared > 0 else 0
-    n_shared, n_own, own_chunk = shared_cut(s, families, int(most_members), int(most_shared), block_table.shape[1] * page_size, hq, hkv, d, page_size, q.dtype)
+    own_tokens = block_table.shape[1] * page_size
+    if most_own is not None:
+        own_tokens = max(1, min(own_tokens, int(most_own)))
+    n_shared, n_own, own_chunk = shared_cut(s, families, int(most_members), int(most_shared), own_tokens, hq, hkv, d, page_size, q.dtype)
     need = s * hq * (n_shared + n_own) * (d + 2)
     if partial is None:
         partial = torch.empty(need, dtype=torch.float32, device=q.device)
@@ -2072,7 +2078,7 @@ def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
 
 
 @functools.lru_cache(maxsize=1024)
-def shared_cut(n_seqs: int, n_families: int, most_members: int, most_shared: int, table_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int,
+def shared_cut(n_seqs: int, n_families: int, most_members: int, most_shared: int, own_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int,
                page_size: int, dtype: torch.dtype) -> Tuple[int, int, int]:
     """(parts of the shared keys, most parts of a sequence's own keys, keys of one of those) that ``paged_attention_shared`` works in."""
     group = n_heads // n_kv_heads
@@ -2084,20 +2090,20 @@ def shared_cut(n_seqs: int, n_families: int, most_members: int, most_shared: int
     general = not (dtype == torch.bfloat16 and head_dim in (64, 128) and page_size in (8, 16, 32, 64))
     slots, least = (2 * _DECODE_SLOTS, 64) if general else (_DECODE_SLOTS // 2, 256) if tile == 128 else (_DECODE_SLOTS, 256)
     n_shared = max(1, min(32, most_shared // least, slots // max(1, blocks))) if n_families else 0
-    # Own keys: parts of at most 512, so that no block walks much longer than the others, and of fewer where that leaves SMs idle.  But a part
-    # that a sequence does not have costs a block that ends at once, some 1.3 ns: no more than about 5,000 of those (101 sequences of 8 kv heads over
-    # a table of 3,100: 7 parts 52 us, 3 parts 56; 240 over 2,600: 6 parts 58, 2 parts 45), and no more than 32 parts.
+    # Own keys (own_tokens at most): parts of at most 512, so that no block walks much longer than the others, and of fewer where that leaves SMs idle.  But a part
+    # that a sequence does not have costs a block that ends at once, some 1.3 ns: no more than about 5,000 of those (101 sequences of 8 kv heads,
+    # 3,100 at most: 7 parts 52 us, 3 parts 56; 240, 2,600 at most: 6 parts 58, 2 parts 45), and no more than 32 parts.
     own_blocks = n_seqs * -(-group // 16) * n_kv_heads
-    chunk = max(least // 2, min(512, table_tokens * own_blocks // (3 * slots // 2)), -(-table_tokens // min(32, 1 + max(1, 5000 // own_blocks))))
+    chunk = max(least // 2, min(512, own_tokens * own_blocks // (3 * slots // 2)), -(-own_tokens // min(32, 1 + max(1, 5000 // own_blocks))))
     whole = 64 * page_size // math.gcd(64, page_size)
     chunk = -(-chunk // whole) * whole
-    return n_shared, max(1, -(-table_tokens // chunk)), chunk
+    return n_shared, max(1, -(-own_tokens // chunk)), chunk
 
 
-def shared_scratch(n_seqs: int, n_families: int, most_members: int, most_shared: int, table_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int,
+def shared_scratch(n_seqs: int, n_families: int, most_members: int, most_shared: int, own_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int,
                    page_size: int, dtype: torch.dtype) -> int:
-    """Elements of ``paged_attention_shared``'s scratch."""
-    n_shared, n_own, _ = shared_cut(n_seqs, n_families, most_members, most_shared, table_tokens, n_heads, n_kv_heads, head_dim, page_size, dtype)
+    """Elements of ``paged_attention_shared``'s scratch.  ``own_tokens``: the smaller of ``most_own`` and what the table's rows hold."""
+    n_shared, n_own, _ = shared_cut(n_seqs, n_families, most_members, most_shared, own_tokens, n_heads, n_kv_heads, head_dim, page_size, dtype)
     return n_seqs * n_heads * (n_shared + n_own) * (head_dim + 2)
 
 

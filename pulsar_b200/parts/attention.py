@@ -320,11 +320,12 @@ class Attention(Mixer):
                                    self.q_norm, self.k_norm, s.qk_norm_eps or 0.0, s.n_heads, n_kv, s.head_dim, rotary, cache.page_size)
             o = ctx.scratch("attn.o", (n, s.n_heads, s.head_dim))
             n_kv_heads, page_size = cache.k_pool.shape[1], cache.page_size
-            need = ops.shared_scratch(n, shared.family_start.numel() - 1, shared.most_members, shared.most_shared, cache.block_table.shape[1] * page_size,
+            need = ops.shared_scratch(n, shared.family_start.numel() - 1, shared.most_members, shared.most_shared,
+                                      min(shared.most_own, cache.block_table.shape[1] * page_size),
                                       s.n_heads, n_kv_heads, s.head_dim, page_size, q.dtype)
             ops.paged_attention_shared(q, cache.k_pool, cache.v_pool, o, cache.block_table, ctx.kv_len, shared.shared_len, shared.members,
                                        shared.family_start, shared.most_members, shared.most_shared, s.scale,
-                                       ctx.scratch("attn.partial", (need,), torch.float32))
+                                       ctx.scratch("attn.partial", (need,), torch.float32), shared.most_own)
             return o
         # (A lone sequence keeps the kernel of its own: its keys are cut into so many splits that every block's share
         # is short, and the norm and rotation in each block's start then cost more than the launch they save:

@@ -72,6 +72,7 @@ class SharedPages(NamedTuple):
     shared_len: torch.Tensor        # int32 [S]
     most_members: int
     most_shared: int
+    most_own: int                   # keys behind the shared ones, at most (in steps of 512: a captured step serves while it holds)
 
 
 class StepContext:

@@ -144,6 +144,15 @@ def test_wide_tables_scratch_of_the_caller_and_the_same_bits():
 
 
 @cuda
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("families", ["several", "long", "own_empty"])
+def test_the_most_own_keys_are_said(dtype, families):
+    c = Cache(FAMILIES[families], 8, 2, 128, 16, dtype, 13)
+    c.check(width=300, most_own=max(k - s for k, s in zip(c.kv_len, c.shared)))
+    c.check(width=300, most_own=4096)
+
+
+@cuda
 def test_offsets_beyond_32_bits():
     """A pool of 4.6 GB whose last pages are read."""
     pages, hkv, page, dim = 70000, 4, 64, 128
@@ -182,7 +191,7 @@ def test_refusals():
     c = Cache(FAMILIES["pair"], 8, 2, 64, 16, torch.bfloat16, 10)
     k = c.k.cuda()
     for changed, said in ((dict(out=c.q.float().cuda()), "one dtype"), (dict(kv_len=on(c.kv_len).long()), "int32"), (dict(kv_len=on([1])), "a length"),
-                          (dict(most_members=3), "most_members"), (dict(most_shared=-1), "most_members"), (dict(v_pool=k[:, :1].contiguous()), "do not fit"),
+                          (dict(most_members=3), "most_members"), (dict(most_shared=-1), "most_members"), (dict(most_own=-1), "most_own"), (dict(v_pool=k[:, :1].contiguous()), "do not fit"),
                           (dict(out=c.q[:1].cuda()), "do not fit"), (dict(partial=torch.empty(3, device="cuda")), "partial"),
                           (dict(family_start=on([])), "one more"), (dict(k_pool=k.transpose(1, 2)), "contiguous")):
         with pytest.raises(ops.KernelError, match=said):
