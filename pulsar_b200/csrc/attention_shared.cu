@@ -22,7 +22,8 @@ using namespace pb::shared_attention;
 // ---------------------------------------------------------------------------------------------
 // Any head size that is a multiple of 16 (up to 256), any page size, float32 or bfloat16, on the CUDA cores in float32.  Four warps take
 // four rows each of a tile of 16; a tile of 32 keys and its values are brought to shared memory as float32.  Scores: a lane per key; values:
-// a lane per four of the head's dimensions.
+// a lane per four of the head's dimensions.  Bound by what a warp's instructions take, two shared-memory reads per four products: 4 families
+// of 8 over 2,000 keys in float32, heads of 128, take 156 us (their bytes 10), 6 sequences over 700 keys, heads of 96, 33 us.
 constexpr int kRows = 16, kKeys = 32, kThreads = 128;
 constexpr int kWarpRows = kRows / (kThreads / 32);
 
@@ -145,10 +146,11 @@ shared_general_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, con
 // bfloat16, head size 64 or 128, pages of 8, 16, 32 or 64 keys: on the tensor cores (mma.m16n8k16, float32 sums).  Tiles of 64 keys and
 // values come page by page through TMA (boxes of a page x 64 dimensions, 128-byte swizzle) into a ring that a warp of its own fills,
 // two or three blocks an SM: what limits the kernel is bytes in flight, and instructions that gather a tile would cost the other warps as
-// much as its products (cp.async by all warps: 2,300 cycles a tile and block, 77 against 48 us for 101 sequences).  ROW_TILES x 16 query
-// rows meet each tile; the four warps share the work as ROW_TILES row tiles x 4 / ROW_TILES parts of the tile's keys: with one row tile (a
-// sequence's own keys) each warp has 16 keys, with four each has all 64 for its own rows, so that shared memory is read no more often than
-// rows need.
+// much as its products (cp.async by all warps: 2,300 cycles a tile and block; 101 sequences, 96 of them in 12 families over up to 2,600
+// keys: 77 against 66 us).  ROW_TILES x 16 query rows meet each tile; the four warps share the work as ROW_TILES row tiles x 4 / ROW_TILES
+// parts of the tile's keys: with one row tile (a sequence's own keys) each warp has 16 keys, with four each has all 64 for its own rows, so
+// that shared memory is read no more often than rows need.  (The 101 sequences' own keys, up to 500 each, 115 MB: 33 us cold, 44 % of the
+// memory's rate: walks of a few tiles, which their starts and ends bound.)
 //
 // Rows of a tile that no key of the item fills hold what lies in the page, or an earlier tile: their scores are masked, and their values
 // are overwritten with zeros, for zero weights do not silence a NaN.  Every wait is bounded; a block that gives up sets the error
@@ -378,7 +380,8 @@ __device__ __forceinline__ bool attend(const bf16* __restrict__ q, float* __rest
 
 // ROW_TILES: of the shared sides' items; a sequence's own keys meet tiles of 16 rows.  Blocks in the order of the grid, the kv head fastest:
 // the shared sides', then the first parts of all sequences' own keys, then their second, which many do not have.  (Blocks that walk over items
-// and ask for the next one's tiles ahead were no faster, 75 against 60 us for 101 sequences: the shares come out uneven.)  beside: the kernel
+// and ask for the next one's tiles ahead were no faster, 75 against 57 us for the 101
+// sequences above: the shares come out uneven.)  beside: the kernel
 // before it on the stream has the shared sides; it was launched the ordinary way, lets this one in at its start, and the two write
 // different parts.
 template <int D, int ROW_TILES>
@@ -422,7 +425,7 @@ shared_tc_kernel(const bf16* __restrict__ q, const __grid_constant__ CUtensorMap
 }
 
 // Joins a row's parts: a warp per row, a lane per part for their weights and per four dimensions for the sums.  A sequence outside
-// the families has no shared parts.
+// the families has no shared parts.  Latency bounds it: 7 us for 3,232 rows whose parts are cold.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 shared_join_kernel(const float* __restrict__ partial, T* __restrict__ out, const Shared p, int rows, int D) {
@@ -507,7 +510,7 @@ int launch_tc(const void* q, const Maps& maps, float* partial, const Shared& p, 
 }
 
 // Families of up to 16 rows meet their keys as a sequence its own.  Beyond that heads of 128 take the tcgen05 kernel for the shared sides
-// (8 members of 4 heads: 13 against 21 us in all, 64 members: 26 against 104), which takes no other; heads of 64 as many row tiles as the
+// (one family over 4,000 keys, 4 heads a member, us in all: 8 members 15 against 19, 64 members 35 against 104), which takes no other; heads of 64 as many row tiles as the
 // largest family fills.
 bool tcgen05_takes(int rows, int D) { return D == 128 && rows > 16; }
 

@@ -10,7 +10,8 @@
 //
 // A thread takes 128 exponentials a tile, 1,900 cycles with all that goes with them, more than the tile's bytes take where SMs are idle.  So
 // families of up to 64 rows stand in tensor memory twice, of up to 32 four times: each copy has its own half or quarter of a tile's keys,
-// writes zeros for the weights of the others, and the copies' sums are joined at the end (REPEAT).
+// writes zeros for the weights of the others, and the copies' sums are joined at the end (REPEAT).  (12 families of 8, 32 rows per kv head,
+// over up to 2,600 keys, 92 MB: 31 us cold.)
 //
 // Roles: warps 0-3 softmax (and the gathering of the query rows, which lie with their sequences), warp 4 issues the products, warp 5 brings K
 // and warp 6 V, a lane per half page.  S has two buffers, S of the next tile is issued before O += P V of this one.  The maximum moves only

@@ -3,7 +3,9 @@
 // One pass over the row: every thread keeps the maximum and the sums (scores.cuh) of what it has seen, and counts the logits beyond the
 // given token's.  Bound by the bytes of the logits where there are rows enough, by latency where there are few: a row is cut among the
 // blocks of a cluster (up to eight), whose results meet in the first block's hands through distributed shared memory, so there is one
-// launch, no scratch memory and no order of atomics that a result could depend on.
+// launch, no scratch memory and no order of atomics that a result could depend on.  (float32, us, without and with 8 alternatives: 2 rows of
+// 151,936 8 and 11, 64 rows 14 and 17, 2,000 rows 197 and 266, where the bytes take 188; 2,000 rows of 32,000 49 and 74, bytes 40.  bfloat16
+// is bound by instructions: 2,000 rows of 151,936 with 8 take 170, bytes 94.)
 //
 // The n likeliest (n <= 32) cost the pass nothing but the number of the chunk in which a thread's maximum rose last.  A key of 64 bits
 // holds a logit's bits, made to compare as unsigned numbers, above the complement of its index: of equal logits the lower index is the larger
@@ -467,13 +469,17 @@ int launch(const Scores& p, int rows, int cluster, cudaStream_t stream) {
 template <typename T, bool RANK>
 int launch(const Scores& p, int rows, cudaStream_t stream) {
     // What follows the pass over a row costs every block of it the same work: so no more blocks than two of 256 threads an SM, none with
-    // less than 4,096 logits.
+    // less than 4,096 logits.  (64 rows of 151,936 float32 with 8 alternatives, blocks a row x threads: 4 x 256 17 us, 1 x 512 19, 8 x 128 20;
+    // beyond two blocks an SM small ones hide each other's ends: 2,000 rows of 32,000 with 8 alternatives, 128 threads 74 us, 256 82, 512 117.)
     int cluster = 1;
     while (cluster < kMostCluster && (long long)rows * cluster * 2 <= 2 * 148 && p.vocab / (cluster * 2) >= 4096) cluster *= 2;
     const long long blocks = (long long)rows * cluster;
     if (blocks > 0x7fffffff) return PB_ERR_TOO_LARGE;
     if (blocks <= 148) return launch<T, RANK, 512>(p, rows, cluster, stream);
-    if (blocks <= 2 * 148) return launch<T, RANK, 256>(p, rows, cluster, stream);
+    // The elements of a thread in n_top are read once more: of more threads that is a smaller share, which pays where a row is long and its
+    // elements are four bytes (500 rows of 100,352 with 8 alternatives: 51 against 59 us, of 64,000: 39 against 41, of 32,000: 27 against
+    // 25; 2,000 rows of 151,936 bfloat16: 200 against 170).
+    if (blocks <= 2 * 148 || (sizeof(T) == 4 && p.n_top > 0 && p.vocab >= 65536)) return launch<T, RANK, 256>(p, rows, cluster, stream);
     return launch<T, RANK, 128>(p, rows, cluster, stream);
 }
 
