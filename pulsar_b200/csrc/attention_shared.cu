@@ -13,6 +13,8 @@
 #include "mma_common.cuh"
 #include "tcgen05_common.cuh"
 
+#include <type_traits>
+
 namespace {
 
 using namespace pb;
@@ -20,28 +22,81 @@ using namespace pb;
 using namespace pb::shared_attention;
 
 // ---------------------------------------------------------------------------------------------
-// Any head size that is a multiple of 16 (up to 256), any page size, float32 or bfloat16, on the CUDA cores in float32.  Four warps take
-// four rows each of a tile of 16; a tile of 32 keys and its values are brought to shared memory as float32.  Scores: a lane per key; values:
-// a lane per four of the head's dimensions.  Bound by what a warp's instructions take, two shared-memory reads per four products: 4 families
-// of 8 over 2,000 keys in float32, heads of 128, take 156 us (their bytes 10), 6 sequences over 700 keys, heads of 96, 33 us.
-constexpr int kRows = 16, kKeys = 32, kThreads = 128;
-constexpr int kWarpRows = kRows / (kThreads / 32);
+// Any head size that is a multiple of 16 (up to 256), any page size, float32 or bfloat16, on the CUDA cores in float32.  16 rows meet tiles
+// of 64 keys, of which each of four warps has 16, with a maximum, sums and an O of its own; the four are joined at the end.  A warp's scores
+// are 16 rows x 16 keys, four rows and two keys a lane, its O 16 rows x D, four dimensions a lane: shared memory is then read 6 times per 32
+// products of scores and 5 per 64 of O, so the FMA units bound the shared sides; items of up to 4 or 8 rows (a sequence's own) leave out the
+// rest and are bound by bytes.  Keys and values come by cp.async as they lie in the pools, the next tile's keys under this one's values and its
+// values under the next one's scores.  (float32, heads of 128: 4 families of 8 over 2,000 keys 60 us, where a key a lane and four rows a warp,
+// 5 reads per 16 products, took 156; 30 sequences of 2,000 keys that share nothing 83 us, 6.3 TB/s.)
+constexpr int kRows = 16, kKeys = 64, kThreads = 128;
+constexpr int kWarpKeys = kKeys / (kThreads / 32);
+constexpr int kWeightPitch = 20;                         // floats from a key's 16 weights to the next key's: stored and read without bank conflicts
+
+__device__ __forceinline__ void load_eight(const float* p, float (&x)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+__device__ __forceinline__ void load_eight(const bf16* p, float (&x)[8]) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+
+// Shared memory: queries, weights and factors, keys, values.  A row of queries or keys is 16 bytes longer than its elements, so that 8 rows of
+// keys, or 4 of queries, are read without bank conflicts.
+template <typename T> constexpr int kRowPad = 16 / (int)sizeof(T);
+template <typename T>
+size_t general_smem(int D) {
+    return kRows * (D + 4) * sizeof(float) + (kKeys * kWeightPitch + kThreads / 32 * kRows) * sizeof(float) + kKeys * (2 * D + kRowPad<T>) * sizeof(T);
+}
 
 template <typename T, int QUADS /* groups of 128 dimensions */>
 __global__ void __launch_bounds__(kThreads)
 shared_general_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, const T* __restrict__ v_pool, float* __restrict__ partial,
                       const Shared p, int shared_blocks, int D, const PoolBounds bounds) {
     extern __shared__ __align__(16) float smem[];
-    const int row_floats = D + 4;                        // 16-byte reads of 32 neighbouring rows then meet no bank twice
-    float* q_s = smem;                                   // [kRows][D]
-    float* k_s = q_s + kRows * D;                        // [kKeys][row_floats]
-    float* v_s = k_s + kKeys * row_floats;               // [kKeys][D]
-    const int kvh = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __shared__ long long row_s[2][kKeys];                // where in the pools the rows of a tile lie, -1: beyond the item's keys
+    const int q_pitch = D + 4, k_pitch = D + kRowPad<T>;
+    float* q_s = smem;                                   // [kRows][q_pitch]
+    float* weight_s = q_s + kRows * q_pitch;             // [kKeys][kWeightPitch]
+    float* factor_s = weight_s + kKeys * kWeightPitch;   // [warps][kRows]
+    T* k_s = reinterpret_cast<T*>(factor_s + kThreads / 32 * kRows);         // [kKeys][k_pitch]
+    T* v_s = k_s + kKeys * k_pitch;                      // [kKeys][D]
+    const int kvh = blockIdx.x % p.Hkv, block = blockIdx.x / p.Hkv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int G = p.Hq / p.Hkv;
     Item it;
     pdl_trigger();                                       // (the join waits for this kernel's end)
-    if ((int)blockIdx.x >= shared_blocks ? !own_item<kRows>(p, blockIdx.x - shared_blocks, G, it)
-                                         : !family_item<kRows, kKeys>(p, blockIdx.x, G, it)) return;
+    if (block >= shared_blocks ? !own_item<kRows>(p, block - shared_blocks, G, it) : !family_item<kRows, kKeys>(p, block, G, it)) return;
+    auto row_of = [&](int key) {
+        if (key >= it.end) return -1ll;
+        int page = it.table[key / p.page_size];
+        if (!page_ok(page, bounds)) page = 0;
+        return (((long long)page * p.Hkv + kvh) * p.page_size + key % p.page_size) * D;
+    };
+    constexpr int kChunk = 16 / (int)sizeof(T);
+    const int chunks = D / kChunk, first_row = tid / chunks, first_chunk = tid - first_row * chunks;
+    const int row_step = kThreads / chunks, chunk_step = kThreads - row_step * chunks;
+    auto fetch = [&](const T* pool, T* tile, int pitch, const long long* row) {              // rows beyond the item's keys become zeros
+        for (int r = first_row, c = first_chunk; r < kKeys;) {
+            const long long at = row[r];
+            cp_async16(smem_addr(tile + r * pitch + c * kChunk), pool + (at < 0 ? 0 : at) + c * kChunk, at >= 0);
+            r += row_step;
+            c += chunk_step;
+            if (c >= chunks) { c -= chunks; ++r; }
+        }
+        cp_async_commit();
+    };
+    if (tid < kKeys) {
+        row_s[0][tid] = row_of(it.begin + tid);
+        row_s[1][tid] = row_of(it.begin + kKeys + tid);
+    }
+    __syncthreads();
+    if (it.begin < it.end) {
+        fetch(k_pool, k_s, k_pitch, row_s[0]);
+        fetch(v_pool, v_s, D, row_s[0]);
+    }
     const int quads = D / 4;
     for (int i = tid; i < kRows * quads; i += kThreads) {
         const int r = i / quads, d = (i - r * quads) * 4;
@@ -50,95 +105,153 @@ shared_general_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, con
             const int seq = it.seq_of(p, r, G);
             if (seq >= 0 && seq < p.n_seqs) load_quad(q + ((size_t)seq * p.Hq + it.head_of(kvh, r, G)) * D + d, v);
         }
-        store_quad(q_s + r * D + d, v);
+        store_quad(q_s + r * q_pitch + d, v);
     }
-    float m[kWarpRows], l[kWarpRows], o[kWarpRows][QUADS][4];
+    const int key_lane = lane & 7, row_lane = lane >> 3, key_warp = warp * kWarpKeys;        // rows row_lane + 4 i, keys key_lane and + 8
+    float m[4], l[4], o[kRows][QUADS][4];
 #pragma unroll
-    for (int r = 0; r < kWarpRows; ++r) {
-        m[r] = -INFINITY;
-        l[r] = 0.0f;
+    for (int i = 0; i < 4; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.0f;
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
 #pragma unroll
         for (int j = 0; j < QUADS; ++j) o[r][j][0] = o[r][j][1] = o[r][j][2] = o[r][j][3] = 0.0f;
-    }
-    const int row0 = warp * kWarpRows;
-    for (int key0 = it.begin; key0 < it.end; key0 += kKeys) {
-        __syncthreads();
-        for (int i = tid; i < kKeys * quads; i += kThreads) {
-            const int r = i / quads, d = (i - r * quads) * 4, key = key0 + r;
-            float kv[4] = {0.0f, 0.0f, 0.0f, 0.0f}, vv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (key < it.end) {
-                int page = it.table[key / p.page_size];
-                if (!page_ok(page, bounds)) page = 0;
-                const size_t at = (((size_t)page * p.Hkv + kvh) * p.page_size + key % p.page_size) * D + d;
-                load_quad(k_pool + at, kv);
-                load_quad(v_pool + at, vv);
+    cp_async_wait<1>();
+    __syncthreads();                                                          // the first keys, and the queries
+    auto walk = [&](auto quarters) {                     // of the 16 rows: those that the item has
+        constexpr int N = decltype(quarters)::value;
+        int turn = 0;
+        for (int key0 = it.begin; key0 < it.end; key0 += kKeys, ++turn) {
+            const bool more = key0 + kKeys < it.end, mine = key0 + key_warp < it.end;
+            const long long row_later = tid < kKeys ? row_of(key0 + 2 * kKeys + tid) : 0;
+            bool moved = false;
+            if (mine) {
+                float s[4][2] = {};
+                const T* key_a = k_s + (key_warp + key_lane) * k_pitch;
+                const T* key_b = key_a + 8 * k_pitch;
+                const float* query = q_s + row_lane * q_pitch;
+#pragma unroll 2
+                for (int d = 0; d < D; d += 8) {
+                    float a[8], b[8];
+                    load_eight(key_a + d, a);
+                    load_eight(key_b + d, b);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        float x[8];
+                        load_eight(query + 4 * i * q_pitch + d, x);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            s[i][0] = fmaf(x[e], a[e], s[i][0]);
+                            s[i][1] = fmaf(x[e], b[e], s[i][1]);
+                        }
+                    }
+                }
+                const bool in_a = key0 + key_warp + key_lane < it.end, in_b = key0 + key_warp + key_lane + 8 < it.end;
+                float* weight = weight_s + (key_warp + key_lane) * kWeightPitch + row_lane;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float a = in_a ? s[i][0] * p.scale_log2 : -INFINITY, b = in_b ? s[i][1] * p.scale_log2 : -INFINITY;
+                    float top = fmaxf(a, b);
+#pragma unroll
+                    for (int x = 1; x < 8; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                    const float m_new = fmaxf(m[i], top), base = m_new == -INFINITY ? 0.0f : m_new;      // scores of -inf alone weigh nothing
+                    const float f = exp2f(m[i] - base), wa = exp2f(a - base), wb = exp2f(b - base);
+                    l[i] = l[i] * f + (wa + wb);
+                    m[i] = m_new;
+                    weight[4 * i] = wa;
+                    weight[4 * i + 8 * kWeightPitch] = wb;
+                    if (key_lane == 0) factor_s[warp * kRows + row_lane + 4 * i] = f;
+                    moved = moved || f != 1.0f;
+                }
+                moved = __any_sync(0xffffffffu, moved);
             }
-            store_quad(k_s + r * row_floats + d, kv);
-            store_quad(v_s + r * D + d, vv);
-        }
-        __syncthreads();
-        if (row0 >= it.rows) continue;
-        float s[kWarpRows];
+            cp_async_wait<0>();
+            __syncthreads();                                                      // this tile's values; all are done with its keys
+            if (tid < kKeys) row_s[turn & 1][tid] = row_later;
+            if (more) fetch(k_pool, k_s, k_pitch, row_s[(turn + 1) & 1]);
+            if (mine) {
+                if (moved) {
 #pragma unroll
-        for (int r = 0; r < kWarpRows; ++r) s[r] = 0.0f;
-        for (int d = 0; d < D; d += 4) {
-            const float4 k4 = *reinterpret_cast<const float4*>(k_s + lane * row_floats + d);
+                    for (int i = 0; i < N; ++i) {
+                        const float4 f4 = *reinterpret_cast<const float4*>(factor_s + warp * kRows + 4 * i);
+                        const float f[4] = {f4.x, f4.y, f4.z, f4.w};
 #pragma unroll
-            for (int r = 0; r < kWarpRows; ++r) {
-                const float4 q4 = *reinterpret_cast<const float4*>(q_s + (row0 + r) * D + d);
-                s[r] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[r]))));
-            }
-        }
-        const bool in = key0 + lane < it.end;
+                        for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int r = 0; r < kWarpRows; ++r) {
-            s[r] = in ? s[r] * p.scale_log2 : -INFINITY;
-            const float m_new = fmaxf(m[r], warp_max(s[r]));
-            const float base = m_new == -INFINITY ? 0.0f : m_new;             // scores of -inf alone weigh nothing
-            const float f = exp2f(m[r] - base);
-            s[r] = exp2f(s[r] - base);
-            l[r] = l[r] * f + s[r];
-            m[r] = m_new;
+                            for (int j = 0; j < QUADS; ++j)
 #pragma unroll
-            for (int j = 0; j < QUADS; ++j) { o[r][j][0] *= f; o[r][j][1] *= f; o[r][j][2] *= f; o[r][j][3] *= f; }
-        }
-        const int n = min(kKeys, it.end - key0);
-        for (int key = 0; key < n; ++key) {
-            float w[kWarpRows];
+                                for (int e = 0; e < 4; ++e) o[4 * i + r][j][e] *= f[r];
+                    }
+                }
+                const float* weight = weight_s + key_warp * kWeightPitch;
+                const T* value = v_s + key_warp * D + lane * 4;
+#pragma unroll 2
+                for (int key = 0; key < kWarpKeys; ++key) {                       // (weights beyond the item's keys are zeros, and so are the values)
+                    float v[QUADS][4];
 #pragma unroll
-            for (int r = 0; r < kWarpRows; ++r) w[r] = __shfl_sync(0xffffffffu, s[r], key);
+                    for (int j = 0; j < QUADS; ++j) {
+                        v[j][0] = v[j][1] = v[j][2] = v[j][3] = 0.0f;
+                        if ((lane + 32 * j) * 4 < D) load_quad(value + key * D + 128 * j, v[j]);
+                    }
 #pragma unroll
-            for (int j = 0; j < QUADS; ++j) {
-                const int d = (lane + 32 * j) * 4;
-                if (d < D) {
-                    const float4 v4 = *reinterpret_cast<const float4*>(v_s + key * D + d);
+                    for (int i = 0; i < N; ++i) {
+                        const float4 w4 = *reinterpret_cast<const float4*>(weight + key * kWeightPitch + 4 * i);
+                        const float w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-                    for (int r = 0; r < kWarpRows; ++r) {
-                        o[r][j][0] = fmaf(w[r], v4.x, o[r][j][0]);
-                        o[r][j][1] = fmaf(w[r], v4.y, o[r][j][1]);
-                        o[r][j][2] = fmaf(w[r], v4.z, o[r][j][2]);
-                        o[r][j][3] = fmaf(w[r], v4.w, o[r][j][3]);
+                        for (int r = 0; r < 4; ++r)
+#pragma unroll
+                            for (int j = 0; j < QUADS; ++j)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[4 * i + r][j][e] = fmaf(w[r], v[j][e], o[4 * i + r][j][e]);
                     }
                 }
             }
+            cp_async_wait<0>();
+            __syncthreads();                                                      // the next tile's keys; all are done with this one's values
+            if (more) fetch(v_pool, v_s, D, row_s[(turn + 1) & 1]);
         }
+    };
+    if (it.rows <= 4) walk(std::integral_constant<int, 1>());
+    else if (it.rows <= 8) walk(std::integral_constant<int, 2>());
+    else walk(std::integral_constant<int, 4>());
+    // The four warps meet in the memory of keys and values (256 D bytes, which either type's tiles have).
+    float* o_s = reinterpret_cast<float*>(k_s);                               // [warps][kRows][D]
+    float2* ml_s = reinterpret_cast<float2*>(weight_s);                       // [warps][kRows]
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int x = 1; x < 8; x <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
+        if (key_lane == 0) ml_s[warp * kRows + row_lane + 4 * i] = make_float2(m[i], l[i]);
     }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int j = 0; j < QUADS; ++j)
+            if (r < it.rows && (lane + 32 * j) * 4 < D) store_quad(o_s + (warp * kRows + r) * D + (lane + 32 * j) * 4, o[r][j]);
+    __syncthreads();
     const int stride = D + 2, parts = p.n_shared + p.n_own;
-#pragma unroll
-    for (int r = 0; r < kWarpRows; ++r) {
-        if (row0 + r >= it.rows) break;
-        const int seq = it.seq_of(p, row0 + r, G);
+    for (int i = tid; i < it.rows * quads; i += kThreads) {
+        const int r = i / quads, d = (i - r * quads) * 4, seq = it.seq_of(p, r, G);
         if (seq < 0 || seq >= p.n_seqs) continue;
-        float* dst = partial + (((size_t)seq * p.Hq + it.head_of(kvh, row0 + r, G)) * parts + it.part) * stride;
-        const float sum = warp_sum(l[r]);
+        float top = -INFINITY, sum = 0.0f, acc[4] = {};
 #pragma unroll
-        for (int j = 0; j < QUADS; ++j) {
-            const int d = (lane + 32 * j) * 4;
-            if (d < D) {
-                dst[d] = o[r][j][0]; dst[d + 1] = o[r][j][1]; dst[d + 2] = o[r][j][2]; dst[d + 3] = o[r][j][3];
-            }
+        for (int w = 0; w < kThreads / 32; ++w) top = fmaxf(top, ml_s[w * kRows + r].x);
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) {
+            const float2 ml = ml_s[w * kRows + r];
+            const float f = exp2f(ml.x - (top == -INFINITY ? 0.0f : top));
+            float v[4];
+            load_quad(o_s + (w * kRows + r) * D + d, v);
+            sum = fmaf(ml.y, f, sum);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = fmaf(v[e], f, acc[e]);
         }
-        if (lane == 0) { dst[D] = m[r]; dst[D + 1] = sum; }
+        float* dst = partial + (((size_t)seq * p.Hq + it.head_of(kvh, r, G)) * parts + it.part) * stride;
+        *reinterpret_cast<float2*>(dst + d) = make_float2(acc[0], acc[1]);
+        *reinterpret_cast<float2*>(dst + d + 2) = make_float2(acc[2], acc[3]);
+        if (d == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(top, sum);
     }
 }
 
@@ -472,12 +585,12 @@ shared_join_kernel(const float* __restrict__ partial, T* __restrict__ out, const
 
 template <typename T, int QUADS>
 int launch_general(const void* q, const void* k_pool, const void* v_pool, float* partial, const Shared& p, int D, int G, cudaStream_t stream) {
-    const long long shared = family_blocks(p, G, kRows), all = shared + own_blocks(p, G, kRows);
+    const long long shared = family_blocks(p, G, kRows), all = (shared + own_blocks(p, G, kRows)) * p.Hkv;
     if (all > 0x7fffffff) return PB_ERR_TOO_LARGE;
-    const size_t smem = (size_t)(kRows * D + kKeys * (D + 4) + kKeys * D) * sizeof(float);
+    const size_t smem = general_smem<T>(D);
     static SmemLimit limit;
     if (const int rc = limit.allow(shared_general_kernel<T, QUADS>, smem)) return rc;
-    shared_general_kernel<T, QUADS><<<dim3((unsigned)all, p.Hkv), kThreads, smem, stream>>>((const T*)q, (const T*)k_pool, (const T*)v_pool, partial, p,
+    shared_general_kernel<T, QUADS><<<(unsigned)all, kThreads, smem, stream>>>((const T*)q, (const T*)k_pool, (const T*)v_pool, partial, p,
                                                                                            (int)shared, D, pool_bounds_now());
     return launch_status();
 }

@@ -2085,10 +2085,10 @@ def shared_cut(n_seqs: int, n_families: int, most_members: int, most_shared: int
     rows = most_members * group
     tile = fn("pb_shared_rows")(code(dtype), rows, head_dim, page_size)
     blocks = n_families * -(-rows // tile) * n_kv_heads
-    # As many parts as the SMs hold at once (one block of the tcgen05 kernel each, two of the mma.sync kernel, four of the general one,
-    # whose blocks are latency more than bytes); more blocks than that run in rounds, and cutting their keys further only makes more of them.
+    # As many parts as the SMs hold at once (one block of the tcgen05 kernel each, two of the others); more blocks than that run in rounds, and
+    # cutting their keys further only makes more of them.
     general = not (dtype == torch.bfloat16 and head_dim in (64, 128) and page_size in (8, 16, 32, 64))
-    slots, least = (2 * _DECODE_SLOTS, 64) if general else (_DECODE_SLOTS // 2, 256) if tile == 128 else (_DECODE_SLOTS, 256)
+    slots, least = (_DECODE_SLOTS, 64) if general else (_DECODE_SLOTS // 2, 256) if tile == 128 else (_DECODE_SLOTS, 256)
     n_shared = max(1, min(32, most_shared // least, slots // max(1, blocks))) if n_families else 0
     # Own keys (own_tokens at most): parts of at most 512, so that no block walks much longer than the others, and of fewer where that leaves SMs idle.  But a part
     # that a sequence does not have costs a block that ends at once, some 1.3 ns: no more than about 5,000 of those (101 sequences of 8 kv heads,
