@@ -10,6 +10,7 @@ The reference exposes its kernels as ``torch.ops.pulsar.*`` through TorchBind
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 import math
@@ -1972,11 +1973,11 @@ def copy_pages(src_pools, dst_pools, src: torch.Tensor, dst: torch.Tensor) -> No
         shapes += (a_stride * size, b_stride * size, page * size, a_shape[1], b_shape[1], a_shape[0])
     if dst.device != where:
         raise KernelError("copy_pages: pools and page ids must be on one device")
+    of, to, shapes = array.array("q", of), array.array("q", to), array.array("q", shapes)        # (ctypes' arrays take three times as long)
+    of_at, to_at, shapes_at = of.buffer_info()[0], to.buffer_info()[0], shapes.buffer_info()[0]
     for at in range(0, len(of), _MOST_POOLS):
-        n = min(_MOST_POOLS, len(of) - at)
-        pointers, numbers = ctypes.c_void_p * n, ctypes.c_longlong * (6 * n)
-        check(fn("pb_copy_pages")(n, pointers(*of[at:at + n]), pointers(*to[at:at + n]), numbers(*shapes[6 * at:6 * (at + n)]), src.data_ptr(),
-                                  dst.data_ptr(), n_pairs, stream()), "copy_pages")
+        check(fn("pb_copy_pages")(min(_MOST_POOLS, len(of) - at), of_at + 8 * at, to_at + 8 * at, shapes_at + 48 * at, src.data_ptr(), dst.data_ptr(), n_pairs,
+                                  stream()), "copy_pages")
 
 
 MOST_ALTERNATIVES = 32            # one per lane of a warp (csrc/token_scores.cu)
@@ -2037,44 +2038,49 @@ def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     that are not seen).  ``partial``: float32 scratch of ``shared_scratch`` elements, made here where it is not given."""
     _cuda(q, k_pool, v_pool, out, block_table, kv_len, shared_len, members, family_start, partial)
     _check_against(k_pool)
-    if q.dim() != 3 or k_pool.dim() != 4:
-        raise KernelError(f"paged_attention_shared: q is [S, heads, D] and pools [pages, kv heads, page, D], found {tuple(q.shape)}, {tuple(k_pool.shape)}")
-    s, hq, d = q.shape
-    _, hkv, page_size, d2 = k_pool.shape
-    if d2 != d or v_pool.shape != k_pool.shape or out.shape != q.shape or hkv == 0 or hq % hkv:
-        raise KernelError(f"paged_attention_shared: q {tuple(q.shape)}, out {tuple(out.shape)} and pools {tuple(k_pool.shape)}, {tuple(v_pool.shape)} do not fit")
-    if not (q.dtype == k_pool.dtype == v_pool.dtype == out.dtype):
+    q_shape, pool_shape, table_shape, dtype = q.shape, k_pool.shape, block_table.shape, q.dtype
+    if len(q_shape) != 3 or len(pool_shape) != 4:
+        raise KernelError(f"paged_attention_shared: q is [S, heads, D] and pools [pages, kv heads, page, D], found {tuple(q_shape)}, {tuple(pool_shape)}")
+    s, hq, d = q_shape
+    n_pages, hkv, page_size, d2 = pool_shape
+    if d2 != d or v_pool.shape != pool_shape or out.shape != q_shape or hkv == 0 or hq % hkv:
+        raise KernelError(f"paged_attention_shared: q {tuple(q_shape)}, out {tuple(out.shape)} and pools {tuple(pool_shape)}, {tuple(v_pool.shape)} do not fit")
+    if not (dtype == k_pool.dtype == v_pool.dtype == out.dtype):
         raise KernelError("paged_attention_shared: q, out and the pools must have one dtype")
     if d % 16 or d > 256:
         raise KernelError(f"paged_attention_shared: head size {d} must be a multiple of 16, at most 256")
-    for t in (block_table, kv_len, shared_len, members, family_start):
-        if t.dtype != torch.int32:
-            raise KernelError(f"paged_attention_shared: index arrays must be int32, found {t.dtype}")
-    if block_table.dim() != 2 or block_table.shape[0] != s or kv_len.numel() != s or shared_len.numel() != s or family_start.numel() == 0:
+    if not (block_table.dtype == kv_len.dtype == shared_len.dtype == members.dtype == family_start.dtype == torch.int32):
+        raise KernelError("paged_attention_shared: index arrays must be int32, found "
+                          f"{', '.join(str(t.dtype) for t in (block_table, kv_len, shared_len, members, family_start))}")
+    n_starts = family_start.numel()
+    if len(table_shape) != 2 or table_shape[0] != s or kv_len.numel() != s or shared_len.numel() != s or n_starts == 0:
         raise KernelError(f"paged_attention_shared: {s} sequences need a table row, a length and a shared length each, and family_start one more "
                           "element than there are families")
     if most_own is not None and most_own < 0:
         raise KernelError(f"paged_attention_shared: most_own must not be negative, found {most_own}")
     if most_members < 0 or most_shared < 0 or most_members > s:
         raise KernelError(f"paged_attention_shared: most_members must lie in [0, {s}] and most_shared must not be negative, found {most_members}, {most_shared}")
-    kind = code(q.dtype)
+    kind = code(dtype)
     if s == 0:
         return
-    if (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr() | out.data_ptr()) % 16:
+    q_at, k_at, v_at, out_at = q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr()
+    if (q_at | k_at | v_at | out_at) % 16:
         raise KernelError("paged_attention_shared: q, out and the pools must start at a multiple of 16 bytes")
-    families = family_start.numel() - 1 if most_members > 0 and most_shared > 0 else 0
-    own_tokens = block_table.shape[1] * page_size
+    families = n_starts - 1 if most_members > 0 and most_shared > 0 else 0
+    width = table_shape[1]
+    own_tokens = width * page_size
     if most_own is not None:
         own_tokens = max(1, min(own_tokens, int(most_own)))
-    n_shared, n_own, own_chunk = shared_cut(s, families, int(most_members), int(most_shared), own_tokens, hq, hkv, d, page_size, q.dtype)
+    n_shared, n_own, own_chunk = shared_cut(s, families, int(most_members), int(most_shared), own_tokens, hq, hkv, d, page_size, dtype)
     need = s * hq * (n_shared + n_own) * (d + 2)
     if partial is None:
         partial = torch.empty(need, dtype=torch.float32, device=q.device)
     elif partial.dtype != torch.float32 or partial.numel() < need or partial.data_ptr() % 16:
         raise KernelError(f"paged_attention_shared: partial must be float32 of at least {need} elements at a multiple of 16 bytes, found {partial.numel()} of {partial.dtype}")
-    check(fn("pb_paged_attention_shared")(kind, _p(q), _p(k_pool), _p(v_pool), _p(out), _p(partial), _p(block_table), block_table.shape[1], _p(kv_len),
-                                          _p(shared_len), _p(members), _p(family_start), s, members.numel(), families, int(most_members), hq, hkv, d,
-                                          page_size, float(scale), n_shared, n_own, own_chunk, k_pool.shape[0], wait_word_addresses()[1], stream()), "paged_attention_shared", kernels=2)
+    check(fn("pb_paged_attention_shared")(kind, q_at, k_at, v_at, out_at, partial.data_ptr(), block_table.data_ptr(), width, kv_len.data_ptr(),
+                                          shared_len.data_ptr(), members.data_ptr(), family_start.data_ptr(), s, members.numel(), families, int(most_members),
+                                          hq, hkv, d, page_size, scale, n_shared, n_own, own_chunk, n_pages, wait_word_addresses()[1], stream()),
+          "paged_attention_shared", kernels=2)
 
 
 @functools.lru_cache(maxsize=1024)
