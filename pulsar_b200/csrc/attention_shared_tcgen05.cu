@@ -32,7 +32,9 @@ using namespace pb::attn5;
 using namespace pb::shared_attention;
 
 constexpr int kThreads = 224;
-constexpr int kStages = 2;                       // K tiles, and V tiles, on their way: what is left of an SM takes a block of the own sides' kernel
+// K tiles, and V tiles, on their way: what is left of an SM takes a block of the own sides' kernel.  (Three: 47.6 against 48.4 us for 101 sequences with
+// own keys of up to 500, 45.3 against 45.0 for 32 of up to 2,000.)
+constexpr int kStages = 2;
 constexpr int kSmemBytes = (1 + 2 * kStages) * kTileBytes + 1024;
 constexpr int kTmemColumns = 512;                // S[0] | S[1] | O, and what is left of a power of two
 
