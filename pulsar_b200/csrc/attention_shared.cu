@@ -541,19 +541,24 @@ shared_tc_kernel(const bf16* __restrict__ q, const __grid_constant__ CUtensorMap
 // the families has no shared parts.  Latency bounds it: 7 us for 3,232 rows whose parts are cold.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-shared_join_kernel(const float* __restrict__ partial, T* __restrict__ out, const Shared p, int rows, int D) {
+shared_join_kernel(const float* __restrict__ partial, T* __restrict__ out, const Shared p, int rows, int D, int shared_tile) {
     const int row = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (row >= rows) return;
     const int room = p.n_shared + p.n_own, stride = D + 2, seq = row / p.Hq;
     // (lengths were there before the kernels ahead began)
-    const int first = p.shared_len[seq] > 0 ? 0 : p.n_shared, parts = p.n_shared + own_parts(p, seq);
+    int shared = 0;
+    if (p.n_families > 0) {
+        const int keys = shared_keys(p, seq), chunk = shared_chunk(p, keys, shared_tile);
+        shared = (keys + chunk - 1) / chunk;
+    }
+    const int parts = shared + own_parts(p, seq), skipped = p.n_shared - shared;  // part i stands at i, or, of its own, at i + skipped
     const float* base = partial + (size_t)row * room * stride;
     pdl_wait();
     float m[2], l[2];                                                             // up to 64 parts
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int i = first + lane + 32 * h;
-        const float2 ml = i < parts ? *reinterpret_cast<const float2*>(base + (size_t)i * stride + D) : make_float2(-INFINITY, 0.0f);
+        const int i = lane + 32 * h;
+        const float2 ml = i < parts ? *reinterpret_cast<const float2*>(base + (size_t)(i < shared ? i : i + skipped) * stride + D) : make_float2(-INFINITY, 0.0f);
         m[h] = ml.x;
         l[h] = ml.y;
     }
@@ -566,13 +571,23 @@ shared_join_kernel(const float* __restrict__ partial, T* __restrict__ out, const
     for (int d0 = 0; d0 < D; d0 += 128) {
         const int d = d0 + lane * 4;
         float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-        for (int i = first; i < parts; ++i) {
-            const int at = i - first;
-            const float f = __shfl_sync(0xffffffffu, at < 32 ? m[0] : m[1], at & 31);
-            if (d < D) {
-                const float2 a = *reinterpret_cast<const float2*>(base + (size_t)i * stride + d), b = *reinterpret_cast<const float2*>(base + (size_t)i * stride + d + 2);
-                acc[0] = fmaf(a.x, f, acc[0]); acc[1] = fmaf(a.y, f, acc[1]); acc[2] = fmaf(b.x, f, acc[2]); acc[3] = fmaf(b.y, f, acc[3]);
+        for (int i0 = 0; i0 < parts; i0 += 8) {          // eight parts on their way at once (those beyond the last weigh nothing)
+            float2 a[8], b[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int i = i0 + u;
+                const float* part = base + (size_t)(i < shared ? i : i + skipped) * stride + d;
+                a[u] = b[u] = make_float2(0.0f, 0.0f);
+                if (i < parts && d < D) {
+                    a[u] = *reinterpret_cast<const float2*>(part);
+                    b[u] = *reinterpret_cast<const float2*>(part + 2);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int i = i0 + u;
+                const float f = __shfl_sync(0xffffffffu, i < 32 ? m[0] : m[1], i & 31);
+                acc[0] = fmaf(a[u].x, f, acc[0]); acc[1] = fmaf(a[u].y, f, acc[1]); acc[2] = fmaf(b[u].x, f, acc[2]); acc[3] = fmaf(b[u].y, f, acc[3]);
             }
         }
         if (d < D) {
@@ -689,8 +704,10 @@ PB_EXPORT int pb_paged_attention_shared(int dtype, const void* q, const void* k_
         rc = D <= 128 ? launch_general<bf16, 1>(q, k_pool, v_pool, partial, p, D, G, stream) : launch_general<bf16, 2>(q, k_pool, v_pool, partial, p, D, G, stream);
     if (rc != 0) return rc;
     const int rows = n_seqs * Hq, blocks = (rows + kThreads / 32 - 1) / (kThreads / 32);
-    if (dtype == PB_F32) return launch_pdl(shared_join_kernel<float>, dim3(blocks), dim3(kThreads), 0, stream, partial, (float*)out, p, rows, D);
-    return launch_pdl(shared_join_kernel<bf16>, dim3(blocks), dim3(kThreads), 0, stream, partial, (bf16*)out, p, rows, D);
+    static_assert(kKeys == kTile, "the parts of a family's keys are cut by the same tile in both");
+    const int shared_tile = tc_takes(dtype, D, page_size) && tcgen05_takes(most_members * G, D) ? kTcgen05Rows : kTile;
+    if (dtype == PB_F32) return launch_pdl(shared_join_kernel<float>, dim3(blocks), dim3(kThreads), 0, stream, partial, (float*)out, p, rows, D, shared_tile);
+    return launch_pdl(shared_join_kernel<bf16>, dim3(blocks), dim3(kThreads), 0, stream, partial, (bf16*)out, p, rows, D, shared_tile);
 }
 
 // A new limit of this kernel's bounded waits in clock cycles.

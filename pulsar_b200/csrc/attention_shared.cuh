@@ -41,7 +41,13 @@ struct Item {
     __device__ __forceinline__ int head_of(int kvh, int i, int G) const { return kvh * G + (row0 + i) % G; }
 };
 
-// Block `block` of the shared sides: the family's keys in n_shared parts (those beyond the last key are empty).  False: nothing to do.
+// A family's shared keys in at most n_shared parts of whole tiles: the keys of a part, and how many parts they make (short families fewer).
+__device__ __forceinline__ int shared_keys(const Shared& p, int seq) { return max(0, min(p.shared_len[seq], p.table_stride * p.page_size)); }
+__device__ __forceinline__ int shared_chunk(const Shared& p, int keys, int tile) {
+    return max(1, ((keys + p.n_shared - 1) / p.n_shared + tile - 1) / tile) * tile;
+}
+
+// Block `block` of the shared sides.  False: there is no such part.
 template <int ROWS, int TILE>
 __device__ __forceinline__ bool family_item(const Shared& p, int block, int G, Item& it) {
     const int tiles = (p.most_members * G + ROWS - 1) / ROWS;
@@ -57,12 +63,10 @@ __device__ __forceinline__ bool family_item(const Shared& p, int block, int G, I
     it.table = p.block_table + (size_t)first * p.table_stride;
     it.seq = -1;
     it.part = split;
-    const int keys = max(0, min(p.shared_len[first], p.table_stride * p.page_size));      // never beyond the table
-    int chunk = (keys + p.n_shared - 1) / p.n_shared;
-    chunk = (chunk + TILE - 1) / TILE * TILE;
+    const int keys = shared_keys(p, first), chunk = shared_chunk(p, keys, TILE);          // (never beyond the table)
     it.begin = min(keys, split * chunk);
     it.end = min(keys, it.begin + chunk);
-    return true;
+    return it.begin < it.end;
 }
 // The first of a sequence's own keys (its shared pages are whole already, unless the caller erred), and how many parts they make.
 __device__ __forceinline__ int own_begin(const Shared& p, int seq) { return max(0, p.shared_len[seq]) / p.page_size * p.page_size; }

@@ -60,13 +60,12 @@ shared_tcgen05_kernel(const bf16* __restrict__ q, const __grid_constant__ CUtens
     pdl_trigger();                               // launched the ordinary way: the sequences' own sides may run beside it
     const int G = p.Hq / p.Hkv, kvh = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int* abort_flag = &sync.gave_up;
+    Item it;
+    if (!family_item<kBM / REPEAT, kBN>(p, blockIdx.x, G, it)) return;
     if (warp == 4) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sync.tmem)), "r"(kTmemColumns));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
-    Item it;
-    const bool any = family_item<kBM / REPEAT, kBN>(p, blockIdx.x, G, it);
-    if (!any) it.begin = it.end = it.rows = 0;
     const int n_tiles = (it.end - it.begin + kBN - 1) / kBN;              // (a split begins at a multiple of kBN)
     // softmax warp w has rows (w % kGroups) * 32 .. and copy w / kGroups of them
     constexpr int kGroups = 4 / REPEAT, kKeys = kBN / REPEAT;

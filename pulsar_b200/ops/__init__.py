@@ -2091,16 +2091,20 @@ def shared_cut(n_seqs: int, n_families: int, most_members: int, most_shared: int
     rows = most_members * group
     tile = fn("pb_shared_rows")(code(dtype), rows, head_dim, page_size)
     blocks = n_families * -(-rows // tile) * n_kv_heads
-    # As many parts as the SMs hold at once (one block of the tcgen05 kernel each, two of the others); more blocks than that run in rounds, and
-    # cutting their keys further only makes more of them.
+    # As many parts as the SMs hold at once, two blocks each; more blocks than that run in rounds, and cutting their keys further only makes more of
+    # them.  The tcgen05 kernel has an SM to itself but for one block of the own sides, which want room: 120 blocks, or all SMs where that would
+    # be no cut at all (us for 120 and 148: 1 family of 8 over 16,000 keys 20 and 24, 2 over 4,000 14.4 and 16.7, 6 over 4,000 31 and 33, 2 over 30,000 48
+    # and 46; 9 over 12,000 102 uncut, 76 in two parts).  No part of less than two of its tiles, or of the others' (64 keys, general: one).
     general = not (dtype == torch.bfloat16 and head_dim in (64, 128) and page_size in (8, 16, 32, 64))
-    slots, least = (_DECODE_SLOTS, 64) if general else (_DECODE_SLOTS // 2, 256) if tile == 128 else (_DECODE_SLOTS, 256)
-    n_shared = max(1, min(32, most_shared // least, slots // max(1, blocks))) if n_families else 0
+    blocks, least = max(1, blocks), 64 if general else 256 if tile == 128 else 128
+    slots = _DECODE_SLOTS if tile != 128 else 120 if 120 // blocks > 1 else _DECODE_SLOTS // 2
+    n_shared = max(1, min(32, -(-most_shared // least), slots // blocks)) if n_families else 0
     # Own keys (own_tokens at most): parts of at most 512, so that no block walks much longer than the others, and of fewer where that leaves SMs idle.  But a part
     # that a sequence does not have costs a block that ends at once, some 1.3 ns: no more than about 5,000 of those (101 sequences of 8 kv heads,
     # 3,100 at most: 7 parts 52 us, 3 parts 56; 240, 2,600 at most: 6 parts 58, 2 parts 45), and no more than 32 parts.
     own_blocks = n_seqs * -(-group // 16) * n_kv_heads
-    chunk = max(least // 2, min(512, own_tokens * own_blocks // (3 * slots // 2)), -(-own_tokens // min(32, 1 + max(1, 5000 // own_blocks))))
+    own_least, own_slots = 32 if general else 128, 3 * _DECODE_SLOTS // (4 if tile == 128 else 2)
+    chunk = max(own_least, min(512, own_tokens * own_blocks // own_slots), -(-own_tokens // min(32, 1 + max(1, 5000 // own_blocks))))
     whole = 64 * page_size // math.gcd(64, page_size)
     chunk = -(-chunk // whole) * whole
     return n_shared, max(1, -(-own_tokens // chunk)), chunk
