@@ -27,8 +27,8 @@ using namespace pb::shared_attention;
 // are 16 rows x 16 keys, four rows and two keys a lane, its O 16 rows x D, four dimensions a lane: shared memory is then read 6 times per 32
 // products of scores and 5 per 64 of O, so the FMA units bound the shared sides; items of up to 4 or 8 rows (a sequence's own) leave out the
 // rest and are bound by bytes.  Keys and values come by cp.async as they lie in the pools, the next tile's keys under this one's values and its
-// values under the next one's scores.  (float32, heads of 128: 4 families of 8 over 2,000 keys 60 us, where a key a lane and four rows a warp,
-// 5 reads per 16 products, took 156; 30 sequences of 2,000 keys that share nothing 83 us, 6.3 TB/s.)
+// values under the next one's scores.  (float32, heads of 128: 4 families of 8 over 2,000 keys 59 us, where a key a lane and four rows a warp,
+// 5 reads per 16 products, took 156; 30 sequences of 2,000 keys that share nothing 82 us, 6.4 TB/s.)
 constexpr int kRows = 16, kKeys = 64, kThreads = 128;
 constexpr int kWarpKeys = kKeys / (kThreads / 32);
 constexpr int kWeightPitch = 20;                         // floats from a key's 16 weights to the next key's: stored and read without bank conflicts
@@ -638,7 +638,7 @@ int launch_tc(const void* q, const Maps& maps, float* partial, const Shared& p, 
 }
 
 // Families of up to 16 rows meet their keys as a sequence its own.  Beyond that heads of 128 take the tcgen05 kernel for the shared sides
-// (one family over 4,000 keys, 4 heads a member, us in all: 8 members 15 against 19, 64 members 35 against 104), which takes no other; heads of 64 as many row tiles as the
+// (one family over 4,000 keys, 4 heads a member, us in all: 8 members 13 against 20, 64 members 26 against 49), which takes no other; heads of 64 as many row tiles as the
 // largest family fills.
 bool tcgen05_takes(int rows, int D) { return D == 128 && rows > 16; }
 

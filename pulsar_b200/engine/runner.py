@@ -280,8 +280,8 @@ class ModelRunner:
 
     # A step takes the attention over shared pages where that saves reading at least so many keys.  (Beside it norm, rotation and cache write are
     # a launch of their own, and the other finds shared pages in L2.  A step of 12 layers of the 8B sizes, us without and with it: 8 forks of 2,000
-    # tokens, 14,000 keys saved, 3,262 and 3,336; of 4,000 tokens 3,558 and 3,408; of 8,000 4,143 and 3,495; 16 of 2,000 3,941 and 3,741; 32 of
-    # 500, 15,500 saved, 3,591 and 3,829; 32 of 8,000 8,086 and 4,169; 64 of 500 4,353 and 4,111.)
+    # tokens, 14,000 keys saved, 3,236 and 3,218; of 4,000 tokens 3,538 and 3,274; of 8,000 4,126 and 3,385; 16 of 2,000 3,917 and 3,638; 32 of
+    # 500, 15,500 saved, 3,588 and 3,701; 32 of 8,000 8,096 and 3,982; 64 of 500 4,354 and 4,048.)
     SHARED_KEYS_SAVED = 24576
 
     def _find_shared(self, ctx: StepContext, rids) -> None:
