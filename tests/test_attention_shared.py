@@ -211,3 +211,21 @@ def test_no_cpu_path():
     i = torch.zeros(1, dtype=torch.int32)
     with pytest.raises(ops.KernelError, match="no CPU path"):
         ops.paged_attention_shared(z, torch.zeros(1, 1, 4, 16), torch.zeros(1, 1, 4, 16), z, i.view(1, 1), i, i, i, i, 0, 0, 1.0)
+
+
+@cuda
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim,page", [(128, 16), (64, 8), (96, 16)])
+def test_families_of_unlike_length(dtype, dim, page):
+    """The cut of the shared keys follows the longest family: a short one has fewer parts, and nothing is read of those it lacks."""
+    families = [(1200 // page, [3, 70]), (1, [5, 9, 1]), (300 // page, [64]), (0, [17, 400]), (64 // page, [0, 2])]
+    c = Cache(families, 8, 2, dim, page, dtype, dim + page)
+    need = ops.shared_scratch(len(c.shared), len(c.starts) - 1, c.most_members, max(c.shared), max(len(t) for t in c.tables) * page, 8, 2, dim, page, dtype)
+    c.check(partial=torch.full((need,), float("nan"), device="cuda"))
+
+
+@cuda
+@pytest.mark.parametrize("group", [1, 3, 4, 5, 8, 9, 16, 17])
+def test_groups_of_every_size_in_float32(group):
+    """Items of up to 4, 8 and 16 rows take walks of their own, more rows further items."""
+    Cache([(9, [1, 63, 64, 65]), (0, [130, 16])], 2 * group, 2, 48, 16, torch.float32, group).check()

@@ -288,3 +288,22 @@ def test_refusals():
 def test_no_cpu_path():
     with pytest.raises(ops.KernelError, match="no CPU path"):
         ops.token_scores(torch.zeros(1, 4), torch.zeros(1, dtype=torch.int32), torch.zeros(1), torch.zeros(1))
+
+
+@cuda
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab", [(297, 65535), (297, 65536), (310, 70001)])
+def test_many_long_rows(dtype, rows, vocab):
+    """The block's size hangs on the rows, the vocabulary, the type and the alternatives: every row's results, checked on some."""
+    logits, tokens = logits_of(rows, vocab, dtype, vocab)
+    for top in (0, 20):
+        got = run(logits, tokens, top)
+        some = torch.tensor([0, 1, 100, 147, 148, 200, rows - 2, rows - 1], device="cuda")
+        want = plain(logits[some], tokens[some], top)
+        got = {k: v[some] if v is not None else None for k, v in got.items()}
+        near(got["logprob"], want["logprob"], vocab)
+        near(got["entropy"], want["entropy"], vocab)
+        assert torch.equal(got["rank"].long().cpu(), want["rank"])
+        if top:
+            assert torch.equal(got["top_ids"].long().cpu(), want["top_ids"])
+            near(got["top_logprob"], want["top_logprob"], vocab)
