@@ -181,14 +181,16 @@ PH_EXPORT int ph_families(void* h, int group, int n, const int64_t* rids, int* m
 //
 // Phase 2 (ph_step_pack): writes the arrays, each padded to 16 bytes, into `buf`:
 //   token_ids, positions, seq_of_token [N]; cu_q [S+1]; kv_len, state_slots [S]; logit_rows [R];
-//   per group: slots [N], block table [S, width] (-1 where a request has no page);
+//   per group: slots [N]; per group: block table [S, width] (-1 where a request has no page);
 //   if any entry takes its token from the device: move_dst, move_src [number of such entries].
 // With resident tables (ph_set_resident_tables) the device keeps a block-table row per state slot, and the per-group
 // table array is replaced by the page ids the step's requests gained since they were last sent:
-//   updates [1 + 3 * capacity]: the count, then (state slot, logical page, page id) triples; the capacity is the
-//   number of entries for a step of single tokens (a token adds one page at most; the array's length then does not
-//   change from step to step), else the exact count.  Packing marks those pages as sent.
-// offsets/lengths receive where each array starts and how long it is (7 + 2 * groups (+ 2) entries).
+//   updates [1 + 3 * capacity]: the count, then (state slot, logical page, page id) triples.  For a step of single tokens the
+//   capacity is the number of entries at least: a token adds one page at most, but a forked request's first step, or a step after
+//   the pools moved, brings its whole table.  Packing marks those pages as sent.
+// What a captured step reads stands at offsets that N, S, R and the groups alone decide: the tables or updates, whose length may differ from
+// step to step, come behind the slots of all groups.
+// offsets/lengths receive where each array starts and how long it is (7 + 2 * groups (+ 2) entries, a group's slots and its table side by side).
 namespace {
 // Page ids of group g that the entries' requests hold and the device's resident table does not yet.
 int unsynced_pages(const Cache& c, int g, int n_entries, const int64_t* rids) {
@@ -289,19 +291,17 @@ PH_EXPORT int ph_step_pack(void* h, int n_entries, const int64_t* rids, const in
         if (n_tok[i] != 1) all_single = false;
     }
     const bool resident = c->resident_tables();
-    int k = 0, total = 0;
-    auto place = [&](int len) {
+    int total = 0;
+    auto place = [&](int k, int len) {
         offsets[k] = total;
         lengths[k] = len;
-        ++k;
         total += align4(std::max(len, 1));
     };
-    place(n); place(n); place(n); place(S + 1); place(S); place(S); place(rows);
-    for (int g = 0; g < G; ++g) {
-        place(n);
-        place(resident ? 1 + 3 * update_capacity(*c, g, S, rids, all_single) : S * widths[g]);
-    }
-    if (moved) { place(moved); place(moved); }
+    const int fixed[7] = {n, n, n, S + 1, S, S, rows};
+    for (int k = 0; k < 7; ++k) place(k, fixed[k]);
+    for (int g = 0; g < G; ++g) place(7 + 2 * g, n);
+    for (int g = 0; g < G; ++g) place(8 + 2 * g, resident ? 1 + 3 * update_capacity(*c, g, S, rids, all_single) : S * widths[g]);
+    if (moved) { place(7 + 2 * G, moved); place(8 + 2 * G, moved); }
     if (total > capacity) return kTooSmall;
     int* tok = buf + offsets[0];
     int* pos = buf + offsets[1];

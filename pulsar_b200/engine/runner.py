@@ -183,7 +183,7 @@ class ModelRunner:
         # The host runtime checks the whole step's pages and slots before anything changes, grows the
         # requests, and writes the step's index arrays into one pinned buffer:
         # token_ids, positions, seq_of_token [N]; cu_q [S+1]; kv_len, state_slots [S]; logit_rows [R];
-        # per group slots [N] and the block table [S, width]; move_dst, move_src if tokens come from the device.
+        # per group slots [N] and the block table [S, width] (or what it gained); move_dst, move_src if tokens come from the device.
         s = len(entries)
         n_groups = len(cache.groups)
         fresh = [e.rid for e in entries if not cache.has(e.rid)]
@@ -348,7 +348,7 @@ class ModelRunner:
             self._graph_epoch = self.scratch_epoch
         key = (ctx.n_tokens, ctx.n_seqs, int(ctx.logit_rows.numel()), ctx.table_widths, ctx.uneven,
                tuple((g, f.members.numel(), f.family_start.numel(), f.most_members, f.most_shared, f.most_own) for g, f in ctx.shared_pages.items()),
-               tuple(int(t.data_ptr()) for t in (ctx.token_ids, ctx.logit_rows)))
+               tuple(int(t.data_ptr()) for t in (ctx.token_ids, ctx.logit_rows, *ctx.group_slots, *ctx.group_tables)))
         hit = self._graphs.get(key)
         if hit is not None:
             hit[0].replay()
