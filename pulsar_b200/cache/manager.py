@@ -410,31 +410,34 @@ class CacheManager:
 
     def resize(self, num_pages) -> None:
         """Give every group ``num_pages`` pages (an int, or a list per group): what is held moves to the front of new pools, and the old pools'
-        memory goes back to PyTorch.  Refused, with nothing changed, where a group holds more pages than that.  While a group moves, its old and
-        its new pools exist side by side.  Whoever keeps the pools' addresses (a captured step) has to forget them."""
+        memory goes back to PyTorch.  Either all groups move or nothing changes: refused where a group holds more pages than that, and where
+        memory runs out, for the old and the new pools of all groups exist side by side until everything is copied.  Whoever keeps the pools'
+        addresses (a captured step) has to forget them."""
         counts = [int(num_pages)] * self._n_groups if isinstance(num_pages, int) else [int(n) for n in num_pages]
         if len(counts) != self._n_groups or any(c <= 0 for c in counts):
             raise CacheError(f"num_pages must give a positive count for each of the {self._n_groups} groups")
-        for g, (grp, n) in enumerate(zip(self.groups, counts)):
-            in_use = grp.allocator.n - grp.allocator.n_free
-            if in_use > n:
-                raise OutOfPages(f"group {g} holds {in_use} pages: it cannot be cut to {n}")
-        for g, (grp, n) in enumerate(zip(self.groups, counts)):
-            pools = None
-            if grp.pools is not None:                       # (memory first: if it cannot be had, this group is as it was)
-                pools = {name: torch.zeros((t.shape[0], n, *t.shape[2:]), dtype=t.dtype, device=t.device) for name, t in grp.pools.items()}
-            moved = (ctypes.c_int * max(1, grp.allocator.n))()
-            live = self._lib.ph_resize(self._h, g, n, moved)
-            if live < 0:
-                raise CacheError(f"group {g}: the host runtime refused {n} pages (code {live})")
-            if pools is not None:
-                if live:
-                    from .. import ops
-                    src = torch.tensor(list(moved[:live]), dtype=torch.int32).to(self.device)
-                    ops.copy_pages(list(grp.pools.values()), list(pools.values()), src, torch.arange(live, dtype=torch.int32, device=self.device))
-                grp.pools = pools
-            grp.allocator = _GroupPages(self, g)
-        self._entry_pools.clear()
+        held = [grp.allocator.held() for grp in self.groups]
+        for g, (pages, n) in enumerate(zip(held, counts)):
+            if len(pages) > n:
+                raise OutOfPages(f"group {g} holds {len(pages)} pages: it cannot be cut to {n}")
+        # whatever may fail comes before anything is renumbered: the new pools, and the copies of what is held, in the order of its ids
+        pools = [None if grp.pools is None else
+                 {name: torch.zeros((t.shape[0], n, *t.shape[2:]), dtype=t.dtype, device=t.device) for name, t in grp.pools.items()}
+                 for grp, n in zip(self.groups, counts)]
+        for grp, new, pages in zip(self.groups, pools, held):
+            if new is not None and pages:
+                from .. import ops
+                src = torch.tensor(pages, dtype=torch.int32).to(self.device)
+                ops.copy_pages(list(grp.pools.values()), list(new.values()), src, torch.arange(len(pages), dtype=torch.int32, device=self.device))
+        try:
+            for g, (grp, n, new, pages) in enumerate(zip(self.groups, counts, pools, held)):
+                moved = (ctypes.c_int * max(1, len(pages)))()
+                if self._lib.ph_resize(self._h, g, n, moved) != len(pages) or list(moved[:len(pages)]) != pages:
+                    raise CacheError(f"group {g}: the host runtime did not give the held pages the first of {n} numbers")
+                grp.pools, grp.allocator = new, _GroupPages(self, g)
+        finally:
+            self._entry_pools.clear()
+            self.resident.clear()           # rows that ended requests left there name pages that may be no more
 
     # ------------------------------------------------------------------ views for a step
     def table(self, rid: Hashable, group: int) -> List[int]:

@@ -553,7 +553,8 @@ class Engine:
 
     def resize_cache(self, num_pages: int) -> None:
         """Give the cache pools of ``num_pages`` pages: what sequences hold moves into them, the old ones' memory is given back.  Refused where the
-        sequences hold more, or one of them could no longer reach the end of its turn."""
+        sequences hold more, where one of them could no longer reach the end of its turn, or where memory for the old and the new pools
+        together is not to be had; nothing has changed then."""
         self._alive()
         self._drain()
         num_pages = int(num_pages)
@@ -562,6 +563,8 @@ class Engine:
             most = len(q.tokens) + (max(0, q.max_new_tokens - q.n_generated) if self._sessions[sid].state == "active" else 0)
             if -(-most // self.cache.page_size) > num_pages:
                 raise ValueError(f"sequence {sid} may need {most} tokens: {num_pages} pages of {self.cache.page_size} do not hold them")
-        self.cache.resize(num_pages)
+        try:
+            self.cache.resize(num_pages)
+        finally:
+            self.runner.forget_addresses()
         self.config.num_pages = num_pages
-        self.runner.forget_addresses()
