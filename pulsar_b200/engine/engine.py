@@ -9,7 +9,7 @@ nothing is active, a finished sequence is parked with its pages kept until ``rel
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Any, Dict, List, Optional, Sequence, Tuple, Union
+from typing import Any, Callable, Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -483,16 +483,20 @@ class Engine:
                 for o in overrides:
                     ids.append(self.create_session(prompt, o, alternatives))
                     self.feed(ids[-1], [], max_new_tokens)
-            tokens: Dict[int, List[int]] = {sid: [] for sid in ids}
-            self._run_turns(tokens)
-            found = [Candidate(tokens[sid], self.scores(sid)) for sid in ids]
+            found = {sid: Candidate([], []) for sid in ids}
+
+            def over(sid: int) -> None:             # its pages go back at once: another continuation may wait for them
+                found[sid].scores = self.scores(sid)
+                self.release(sid)
+            self._run_turns({sid: c.tokens for sid, c in found.items()}, over)
         finally:
             for sid in ids + ([anchor] if anchor is not None else []):
                 self.release(sid)
-        return sorted(found, key=lambda c: -c.mean_logprob)
+        return sorted(found.values(), key=lambda c: -c.mean_logprob)
 
-    def _run_turns(self, tokens: Dict[int, List[int]]) -> None:
-        """Step until the turns of these sequences are over, their tokens appended; what other sequences emit meanwhile waits in the mailbox."""
+    def _run_turns(self, tokens: Dict[int, List[int]], over: Optional[Callable[[int], None]] = None) -> None:
+        """Step until the turns of these sequences are over, their tokens appended, and call ``over`` for each as it ends; what other sequences
+        emit meanwhile waits in the mailbox."""
         running = set(tokens)
         while running:
             events = self.step(1)
@@ -503,6 +507,8 @@ class Engine:
                     tokens[sid].append(tok)
                     if finished:
                         running.discard(sid)
+                        if over is not None:
+                            over(sid)
                 else:
                     self._mailbox.setdefault(sid, []).append((tok, finished))
 
