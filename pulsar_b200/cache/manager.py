@@ -367,20 +367,25 @@ class CacheManager:
             raise OutOfPages(f"{len(children)} new requests need a page each, {self.n_free_pages()} pages are free")
         copies = (ctypes.c_int * max(1, 2 * self._n_groups))()
         pairs: List[List[Tuple[int, int]]] = [[] for _ in self.groups]
-        slots = []
-        for i, child in enumerate(children):
-            slot = self._lib.ph_fork(self._h, nid, self.native_id(child, create=True), length, copies)
-            if slot < 0:
-                self._forget_if_idle(child)
-                for opened in children[:i]:
-                    self.close(opened)
-                self._raise(slot, rid, f"a page that a query at {length} needs")
-            slots.append(slot)
-            for g in range(self._n_groups):
-                if copies[2 * g] >= 0:
-                    pairs[g].append((copies[2 * g], copies[2 * g + 1]))
-        if self.device is None or not children:
-            return
+        slots: List[int] = []
+        try:
+            for child in children:
+                slot = self._lib.ph_fork(self._h, nid, self.native_id(child, create=True), length, copies)
+                if slot < 0:
+                    self._forget_if_idle(child)
+                    self._raise(slot, rid, f"a page that a query at {length} needs")
+                slots.append(slot)
+                for g in range(self._n_groups):
+                    if copies[2 * g] >= 0:
+                        pairs[g].append((copies[2 * g], copies[2 * g + 1]))
+            if self.device is not None and slots:
+                self._copy_forked(nid, pairs, slots)
+        except BaseException:
+            for child in children[:len(slots)]:
+                self.close(child)
+            raise
+
+    def _copy_forked(self, nid: int, pairs: List[List[Tuple[int, int]]], slots: List[int]) -> None:
         from .. import ops
         for grp, some in zip(self.groups, pairs):
             if some:

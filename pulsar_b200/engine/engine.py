@@ -168,15 +168,20 @@ class Engine:
         if len(self._sessions) + len(overrides) > self.config.max_sessions:
             raise RuntimeError(f"max_sessions ({self.config.max_sessions}) reached")
         params = [self._params(o) for o in overrides]
-        held = self.cache.length(seq_id)
-        at = held if length is None else int(length)
+        at = self.cache.length(seq_id) if length is None else int(length)
+        rest = self.scheduler.seqs[seq_id].tokens[at:] + s.pending if length is None else []
+        sessions = [_Session(p, make_generator(p.seed), list(rest), 0, state="parked", scheduled=True, alternatives=scores) for p in params]
         children = list(range(self._next_id, self._next_id + len(params)))
         self.cache.fork(seq_id, children, at)
+        try:
+            for sid in children:
+                self.scheduler.fork_request(seq_id, sid, at)
+        except BaseException:                       # either every child is there or nothing has changed
+            for sid in children:
+                self.scheduler.finish(sid)
+            raise
         self._next_id += len(params)
-        rest = self.scheduler.seqs[seq_id].tokens[at:] + s.pending if length is None else []
-        for sid, p in zip(children, params):
-            self.scheduler.fork_request(seq_id, sid, at)
-            self._sessions[sid] = _Session(p, make_generator(p.seed), list(rest), 0, state="parked", scheduled=True, alternatives=scores)
+        self._sessions.update(zip(children, sessions))
         return children
 
     def scores(self, seq_id: int) -> List[TokenScore]:
