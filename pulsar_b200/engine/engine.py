@@ -170,7 +170,8 @@ class Engine:
         params = [self._params(o) for o in overrides]
         at = self.cache.length(seq_id) if length is None else int(length)
         rest = self.scheduler.seqs[seq_id].tokens[at:] + s.pending if length is None else []
-        sessions = [_Session(p, make_generator(p.seed), list(rest), 0, state="parked", scheduled=True, alternatives=scores) for p in params]
+        sessions = [_Session(p, make_generator(p.seed), list(rest), 0, state="parked", scheduled=True,
+                             ended_on_stop=s.ended_on_stop and length is None, alternatives=scores) for p in params]
         children = list(range(self._next_id, self._next_id + len(params)))
         self.cache.fork(seq_id, children, at)
         try:
@@ -251,8 +252,8 @@ class Engine:
             if not (0 <= t < self.model.spec.vocab_size):
                 raise ValueError(f"token id {t} outside the vocabulary [0, {self.model.spec.vocab_size})")
         cap = budget if budget < (1 << 30) else 0
-        if s.scheduled and not new and s.ended_on_stop:
-            # Stepping one pass ahead has cached the stop token by now, stepping one pass at a time has not: a
+        if s.scheduled and len(new) == len(s.pending) and s.ended_on_stop:
+            # Stepping one pass ahead has cached the stop token by now, stepping one pass at a time has not (a fork then has it pending): a
             # turn without tokens would run nothing in the one mode and the stop token in the other.  Refused in both.
             raise ValueError(f"sequence {seq_id} ended on the stop token: a further turn needs at least one token")
         if s.scheduled:

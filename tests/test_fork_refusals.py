@@ -70,3 +70,48 @@ def test_a_cache_fork_whose_copy_fails_leaves_nothing_behind(monkeypatch, length
         m.fork("a", ["b", "c"])
     assert (m.n_free_pages(), m.n_free_slots(), m.live_requests(), m.n_shared_pages()) == before
     m.check_consistency()
+
+
+@pytest.mark.parametrize("lookahead", [False, True])
+@pytest.mark.parametrize("generation", [1, 2])
+def test_a_fork_of_a_sequence_that_ended_on_the_stop_token_needs_a_token_too(lookahead, generation):
+    """However the parent was stepped: refused without tokens, and with one the child goes on as the parent does."""
+    stop = rule(rule(rule(36, 36), 37), 38)
+    eng = HostEngine(rule, eos_id=stop)
+    sid = eng.create_session(list(range(37)))
+    eng.feed(sid, [], 40)
+    events = []
+    while eng.has_work():
+        events += eng.step(1, lookahead=lookahead)
+    assert events[-1] == (sid, stop, True)
+    child = sid
+    for _ in range(generation):
+        child = eng.fork(child)
+    for s in (sid, child):
+        with pytest.raises(ValueError, match="stop token"):
+            eng.feed(s, [], 5)
+    out = {sid: [], child: []}
+    for s in out:
+        eng.feed(s, [11], 5)
+    while eng.has_work():
+        for s, token, _ in eng.step(1, lookahead=lookahead):
+            out[s].append(token)
+    assert out[sid] == out[child] and len(out[sid]) == 5
+    assert eng.scheduler.seqs[sid].tokens == eng.scheduler.seqs[child].tokens == [*range(37), rule(36, 36), rule(rule(36, 36), 37), stop, 11, *out[sid]]
+
+
+@pytest.mark.parametrize("lookahead", [False, True])
+def test_a_fork_of_a_sequence_that_spent_its_budget_goes_on_without_tokens(lookahead):
+    eng = HostEngine(rule, eos_id=501)
+    sid = eng.create_session(list(range(37)))
+    eng.feed(sid, [], 6)
+    while eng.has_work():
+        eng.step(1, lookahead=lookahead)
+    child = eng.fork(sid)
+    out = {sid: [], child: []}
+    for s in out:
+        eng.feed(s, [], 4)
+    while eng.has_work():
+        for s, token, _ in eng.step(1, lookahead=lookahead):
+            out[s].append(token)
+    assert out[sid] == out[child] and len(out[sid]) == 4
