@@ -186,11 +186,13 @@ class Engine:
         return children
 
     def scores(self, seq_id: int) -> List[TokenScore]:
-        """The scores of the tokens that the sequence has emitted since the last call, one for each event of ``step``."""
+        """The scores of the tokens that the sequence has emitted since the last call, one for each event of ``step`` (that of an event which
+        still waits to be handed out, here or in a session's ``recv``, waits with it)."""
         s = self._session(seq_id)
         if s.alternatives is None:
             raise ValueError(f"sequence {seq_id} was created without scores")
-        out, s.scores = s.scores, []
+        received = len(s.scores) - sum(sid == seq_id for sid, _, _ in self._unclaimed) - len(self._mailbox.get(seq_id, ()))
+        out, s.scores = s.scores[:received], s.scores[received:]
         return out
 
     def set_decode_budget(self, seq_id: int, max_tokens: Optional[int] = None) -> None:
@@ -502,21 +504,25 @@ class Engine:
 
     def _run_turns(self, tokens: Dict[int, List[int]], over: Optional[Callable[[int], None]] = None) -> None:
         """Step until the turns of these sequences are over, their tokens appended, and call ``over`` for each as it ends; what other sequences
-        emit meanwhile waits in the mailbox."""
+        emit meanwhile is handed out by the next ``step``."""
         running = set(tokens)
-        while running:
-            events = self.step(1)
-            if not events and not self.has_work():
-                break
-            for sid, tok, finished in events:
-                if sid in tokens:
+        others: List[Tuple[int, int, bool]] = []
+        try:
+            while running:
+                events = self.step(1)
+                if not events and not self.has_work():
+                    break
+                for sid, tok, finished in events:
+                    if sid not in tokens:
+                        others.append((sid, tok, finished))
+                        continue
                     tokens[sid].append(tok)
                     if finished:
                         running.discard(sid)
                         if over is not None:
                             over(sid)
-                else:
-                    self._mailbox.setdefault(sid, []).append((tok, finished))
+        finally:
+            self._unclaimed = others + self._unclaimed
 
     def score(self, prompts: Sequence[Sequence[int]], alternatives: Optional[int] = None) -> List[List[TokenScore]]:
         """How likely the model finds the tokens of each prompt: the scores of its second token to its last, given those before.  Without

@@ -48,3 +48,50 @@ def test_a_continuation_that_lost_its_pages_is_what_it_would_have_been(tmp_path,
     assert sorted(c.tokens for c in got) == sorted(want) and eng.scheduler.n_preemptions > 0
     assert all(len(c.scores) == new for c in got) and not eng._sessions
     eng.cache.check_consistency()
+
+
+@pytest.mark.parametrize("lookahead", [False, True])
+def test_other_sequences_events_reach_the_next_step(lookahead):
+    """A scored sequence that runs beside two sets of candidates: every token is an event of ``step`` once and in order, and its score comes with it."""
+    eng = HostEngine(rule)
+    sid = eng.create_session(list(range(20)), scores=0)
+    eng.feed(sid, [], 25)
+    got, scored = [], []
+
+    def take(events):
+        got.extend(tok for s, tok, _ in events if s == sid)
+        scored.extend(eng.scores(sid))
+        assert [s.token for s in scored] == got
+    for _ in range(4):
+        take(eng.step(1, lookahead=lookahead))
+    for prompt in (list(range(30, 70)), [5, 6, 7]):
+        before = len(got)
+        assert [c.tokens for c in eng.candidates(prompt, 3, 6)] == [alone(prompt, 6)] * 3
+        assert eng.scores(sid) == [] and not eng._mailbox
+        take(eng.step(1, lookahead=lookahead))
+        assert len(got) > before + 5
+    while eng.has_work():
+        take(eng.step(1, lookahead=lookahead))
+    assert got == alone(list(range(20)), 25) and eng.session_state(sid) == "parked"
+
+
+def test_events_of_others_outlive_an_exception_between():
+    eng = HostEngine(rule, num_pages=12)
+    sid = eng.create_session(list(range(20)))
+    eng.feed(sid, [], 25)
+    inner, passes = eng._launch, []
+
+    def launch(plan):
+        passes.append(1)
+        if len(passes) == 9:
+            raise RuntimeError("a pass that could not be launched")
+        return inner(plan)
+    eng._launch = launch
+    with pytest.raises(RuntimeError, match="launched"):
+        eng.candidates([1, 2, 3], 2, 20)
+    eng._launch = inner
+    got = []
+    while eng.has_work():
+        got += [tok for s, tok, _ in eng.step(1) if s == sid]
+    assert got == alone(list(range(20)), 25)
+    assert sorted(eng._sessions) == [sid]
