@@ -31,21 +31,21 @@ class Session:
         self._engine.feed(self._seq_id, tokens, max_tokens)
 
     def recv(self) -> Iterator[int]:
-        """Token ids of this turn, as they are decoded (other sessions advance too)."""
-        done = False
-        while not done:
+        """Token ids of this turn, as they are decoded (other sessions advance too).  Those that came while another session streamed come
+        first."""
+        mailbox = self._engine._mailbox
+        while True:
+            while mailbox.get(self._seq_id):
+                tok, finished = mailbox[self._seq_id].pop(0)
+                yield tok
+                if finished:
+                    return
+            mailbox.pop(self._seq_id, None)
             events = self._engine.step(1)
             if not events and not self._engine.has_work():
                 return
             for sid, tok, finished in events:
-                if sid == self._seq_id:
-                    yield tok
-                    done = done or finished
-                else:
-                    self._engine._mailbox.setdefault(sid, []).append((tok, finished))
-            for tok, finished in self._engine._mailbox.pop(self._seq_id, []):
-                yield tok
-                done = done or finished
+                mailbox.setdefault(sid, []).append((tok, finished))
 
     def get_state(self) -> str:
         return self._engine.session_state(self._seq_id)
