@@ -639,8 +639,9 @@ int launch_tc(const void* q, const Maps& maps, float* partial, const Shared& p, 
 
 // Families of up to 16 rows meet their keys as a sequence its own.  Beyond that heads of 128 take the tcgen05 kernel for the shared sides
 // (one family over 4,000 keys, 4 heads a member, us in all: 8 members 13 against 20, 64 members 26 against 49), which takes no other; heads of 64 as many row tiles as the
-// largest family fills.
-bool tcgen05_takes(int rows, int D) { return D == 128 && rows > 16; }
+// largest family fills.  The tcgen05 kernel finds maxima and masks keys before it scales, which is right for a scale above 0 alone: the others
+// take the rest.
+bool tcgen05_takes(int rows, int D, float scale_log2) { return D == 128 && rows > 16 && scale_log2 > 0.0f; }
 
 int launch_tc(const void* q, const void* k_pool, const void* v_pool, float* partial, Shared p, int G, int D, int n_pages, unsigned int* error,
               cudaStream_t stream) {
@@ -652,7 +653,7 @@ int launch_tc(const void* q, const void* k_pool, const void* v_pool, float* part
     if (rc == 0) rc = make_map(&maps.v, v_pool, pool_rows, D, p.page_size);
     if (rc != 0) return rc;
     const int rows = p.n_families > 0 ? p.most_members * G : 0;
-    if (tcgen05_takes(rows, D)) {
+    if (tcgen05_takes(rows, D, p.scale_log2)) {
         rc = launch_tcgen05(q, maps, partial, p, stream);
         if (rc != 0) return rc;
         p.n_families = 0;                                 // (n_shared stays: it is where a sequence's own parts begin)
@@ -670,10 +671,10 @@ bool tc_takes(int dtype, int D, int page_size) {
 
 }  // namespace
 
-// Query rows that a block of the shared sides works on: what the caller cuts the keys by.
+// Query rows that a block of the shared sides works on (for a scale above 0): what the caller cuts the keys by.
 PB_EXPORT int pb_shared_rows(int dtype, int rows, int D, int page_size) {
     if (!tc_takes(dtype, D, page_size)) return kRows;
-    return tcgen05_takes(rows, D) ? kTcgen05Rows : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    return tcgen05_takes(rows, D, 1.0f) ? kTcgen05Rows : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 
 // q, out [n_seqs, Hq, D], pools [pages, Hkv, page_size, D] (dtype 0 float32, 1 bfloat16); block_table int32 [n_seqs, table_stride];
@@ -705,7 +706,7 @@ PB_EXPORT int pb_paged_attention_shared(int dtype, const void* q, const void* k_
     if (rc != 0) return rc;
     const int rows = n_seqs * Hq, blocks = (rows + kThreads / 32 - 1) / (kThreads / 32);
     static_assert(kKeys == kTile, "the parts of a family's keys are cut by the same tile in both");
-    const int shared_tile = tc_takes(dtype, D, page_size) && tcgen05_takes(most_members * G, D) ? kTcgen05Rows : kTile;
+    const int shared_tile = tc_takes(dtype, D, page_size) && tcgen05_takes(most_members * G, D, p.scale_log2) ? kTcgen05Rows : kTile;
     if (dtype == PB_F32) return launch_pdl(shared_join_kernel<float>, dim3(blocks), dim3(kThreads), 0, stream, partial, (float*)out, p, rows, D, shared_tile);
     return launch_pdl(shared_join_kernel<bf16>, dim3(blocks), dim3(kThreads), 0, stream, partial, (bf16*)out, p, rows, D, shared_tile);
 }

@@ -15,7 +15,8 @@
 //
 // Roles: warps 0-3 softmax (and the gathering of the query rows, which lie with their sequences), warp 4 issues the products, warp 5 brings K
 // and warp 6 V, a lane per half page.  S has two buffers, S of the next tile is issued before O += P V of this one.  The maximum moves only
-// when it grew by more than 2^8; O is rescaled in tensor memory only then, and the sums use the same maximum.
+// when it grew by more than 2^8; O is rescaled in tensor memory only then, and the sums use the same maximum.  Maxima and masks are those of
+// unscaled scores: the scale is above 0 (launch_tc sees to it).
 //
 // Shared keys are whole pages, so a page that is read holds nothing but keys.  Where the last tile has fewer pages, the columns of S are
 // masked, and V's buffer is zero or holds an earlier tile's values there.
