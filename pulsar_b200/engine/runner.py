@@ -297,7 +297,6 @@ class ModelRunner:
             families = lib.ph_families(handle, g, n, rids, members, starts, shared, most)
             if families <= 0:
                 continue
-            in_families = starts[families]
             saved = sum((starts[f + 1] - starts[f] - 1) * shared[members[starts[f]]] for f in range(families))
             if saved < self.SHARED_KEYS_SAVED:
                 continue
@@ -305,7 +304,10 @@ class ModelRunner:
             stage.to_device(room, 3 * n + 1)
             self.h2d_bytes += 4 * (3 * n + 1)
             most_own = max(length - shared[i] for i, length in enumerate(ctx.host.kv_lens))
-            ctx.shared_pages[g] = SharedPages(room[:in_families], room[n:n + families + 1], room[2 * n + 1:3 * n + 1], most[0], most[1], _align(most_own, 512))
+            # What a captured step depends on is rounded, so that prompts of many lengths find the same one: the shared length (it decides into how
+            # many parts the keys are cut, nothing else) to the steps in which tables grow wider and no further than cuts differ, a sequence's own keys to 512.
+            most_shared = min(_align(most[1], self.TABLE_BUCKET * self.cache.page_size), ops.SHARED_CUT_KEYS)
+            ctx.shared_pages[g] = SharedPages(room[:n], room[n:n + families + 1], room[2 * n + 1:3 * n + 1], most[0], most_shared, _align(most_own, 512))
 
     def score(self, entries: Sequence[StepEntry], given: Sequence[int]) -> torch.Tensor:
         """Run the given tokens as ``step`` does and return float32 [2, wanted]: at every wanted position the log probability of that
@@ -347,15 +349,19 @@ class ModelRunner:
             self._graph_seen.clear()
             self._graph_epoch = self.scratch_epoch
         key = (ctx.n_tokens, ctx.n_seqs, int(ctx.logit_rows.numel()), ctx.table_widths, ctx.uneven,
-               tuple((g, f.members.numel(), f.family_start.numel(), f.most_members, f.most_shared, f.most_own) for g, f in ctx.shared_pages.items()),
+               tuple((g, f.family_start.numel(), f.most_members, f.most_shared, f.most_own) for g, f in ctx.shared_pages.items()),
                tuple(int(t.data_ptr()) for t in (ctx.token_ids, ctx.logit_rows, *ctx.group_slots, *ctx.group_tables)))
         hit = self._graphs.get(key)
         if hit is not None:
+            if ctx.shared_pages:                          # the one used last is dropped last
+                self._graphs[key] = self._graphs.pop(key)
             hit[0].replay()
             self.graph_replays += 1
             ops.LAUNCHES += hit[2]
             return hit[1]
         seen = self._graph_seen.get(key, 0)
+        if seen == 0 and len(self._graph_seen) > 4096:    # forget those that were never seen a third time
+            self._graph_seen = {k: v for k, v in self._graph_seen.items() if k in self._graphs}
         self._graph_seen[key] = seen + 1
         if seen < 2:                                      # run eagerly first: buffers reach their final size
             return self.model.forward(ctx)
@@ -380,10 +386,25 @@ class ModelRunner:
         if self.scratch_epoch != epoch:                   # grew during capture: do not keep it
             self._graph_epoch = -1
             return self.model.forward(ctx)
-        self._graphs[key] = (graph, logits, launches)
+        self._keep_graph(key, (graph, logits, launches))
         graph.replay()
         self.graph_replays += 1
         return logits
+
+    # Captured steps of forked sequences are as many as there are counts of families and members, which come and go with their users: so many are
+    # kept, those used last.  (The others are as many as batch sizes and table widths.)
+    MOST_SHARED_GRAPHS = 64
+    _SHARED = 5                 # where a graph's key says what is shared
+
+    def _keep_graph(self, key: tuple, entry: tuple) -> None:
+        """Called behind a capture, with nothing in flight on the device."""
+        self._graphs[key] = entry
+        if not key[self._SHARED]:
+            return
+        kept = [k for k in self._graphs if k[self._SHARED]]
+        for k in kept[:max(0, len(kept) - self.MOST_SHARED_GRAPHS)]:
+            del self._graphs[k]
+            self._graph_seen.pop(k, None)
 
     def forget_addresses(self) -> None:
         """The cache's pools are elsewhere: captured steps hold stale addresses."""

@@ -2033,8 +2033,8 @@ def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     of them.  A sequence in no family has ``shared_len`` 0; one with ``kv_len`` 0 gets zeros.  All arrays int32 on the device.
     (bfloat16 with pages of 8, 16, 32 or 64 keys and heads of 64 or 128 runs on the tensor cores; a wait that it gives up is reported in
     the tcgen05 attention's error word.)
-    ``most_members`` and ``most_shared`` are the largest family's size and the longest shared length as the host knows them (more members
-    than that are not served); ``most_own`` is the most keys that a sequence has beyond its shared ones, where the host knows (keys beyond
+    ``most_members`` is the largest family's size as the host knows it (more members than that are not served), ``most_shared`` the longest
+    shared length, about (it decides into how many parts the shared keys are cut; 0: there are no families); ``most_own`` is the most keys that a sequence has beyond its shared ones, where the host knows (keys beyond
     that are not seen).  ``partial``: float32 scratch of ``shared_scratch`` elements, made here where it is not given."""
     _cuda(q, k_pool, v_pool, out, block_table, kv_len, shared_len, members, family_start, partial)
     _check_against(k_pool)
@@ -2081,6 +2081,9 @@ def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
                                           shared_len.data_ptr(), members.data_ptr(), family_start.data_ptr(), s, members.numel(), families, int(most_members),
                                           hq, hkv, d, page_size, scale, n_shared, n_own, own_chunk, n_pages, wait_word_addresses()[1], stream()),
           "paged_attention_shared", kernels=2)
+
+
+SHARED_CUT_KEYS = 32 * 256       # shared keys that are longer than that are cut into as many parts (the most, of the largest least size)
 
 
 @functools.lru_cache(maxsize=1024)

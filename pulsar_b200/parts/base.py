@@ -67,11 +67,11 @@ class HostBatch:
 
 class SharedPages(NamedTuple):
     """Families of a step's sequences whose first keys lie in the same pages, as ``ops.paged_attention_shared`` takes them."""
-    members: torch.Tensor           # int32 [members of all families]
+    members: torch.Tensor           # int32 [S]: the members of all families, and what the place leaves
     family_start: torch.Tensor      # int32 [families + 1]
     shared_len: torch.Tensor        # int32 [S]
     most_members: int
-    most_shared: int
+    most_shared: int                # rounded, as a captured step serves more than one length
     most_own: int                   # keys behind the shared ones, at most (in steps of 512: a captured step serves while it holds)
 
 
