@@ -2043,7 +2043,7 @@ def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
         raise KernelError(f"paged_attention_shared: q is [S, heads, D] and pools [pages, kv heads, page, D], found {tuple(q_shape)}, {tuple(pool_shape)}")
     s, hq, d = q_shape
     n_pages, hkv, page_size, d2 = pool_shape
-    if d2 != d or v_pool.shape != pool_shape or out.shape != q_shape or hkv == 0 or hq % hkv:
+    if d2 != d or v_pool.shape != pool_shape or out.shape != q_shape or hkv == 0 or hq == 0 or hq % hkv or page_size == 0 or d == 0:
         raise KernelError(f"paged_attention_shared: q {tuple(q_shape)}, out {tuple(out.shape)} and pools {tuple(pool_shape)}, {tuple(v_pool.shape)} do not fit")
     if not (dtype == k_pool.dtype == v_pool.dtype == out.dtype):
         raise KernelError("paged_attention_shared: q, out and the pools must have one dtype")
@@ -2062,6 +2062,9 @@ def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
         raise KernelError(f"paged_attention_shared: most_members must lie in [0, {s}] and most_shared must not be negative, found {most_members}, {most_shared}")
     kind = code(dtype)
     if s == 0:
+        return
+    if table_shape[1] == 0 or n_pages == 0:              # nobody has a key
+        out.zero_()
         return
     q_at, k_at, v_at, out_at = q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr()
     if (q_at | k_at | v_at | out_at) % 16:

@@ -24,3 +24,22 @@ def test_any_scale(members, scale, dtype, dim):
         bound = bound + c.value_size * 2.0 ** -8 + want.abs() * 2.0 ** -8
     off = (got - want).abs()
     assert torch.isfinite(got).all() and (off <= bound).all(), float(off.max())
+
+
+@cuda
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sizes_of_zero(dtype):
+    """No pages, or tables without a column: nobody has a key, and everybody gets zeros.  No heads, no dimensions, pages of no keys: refused."""
+    from pulsar_b200 import ops
+    from test_attention_shared import on
+
+    def call(pages=3, hq=8, hkv=2, page=16, d=128, width=2):
+        q = torch.ones(4, hq, d, dtype=dtype, device="cuda")
+        pool, out = torch.zeros(pages, hkv, page, d, dtype=dtype, device="cuda"), torch.full_like(q, 9.0)
+        ops.paged_attention_shared(q, pool, pool, out, torch.zeros(4, width, dtype=torch.int32, device="cuda"), on([0] * 4), on([0] * 4), on([]), on([0]), 0, 0, 0.1)
+        return out
+    for kw in (dict(), dict(pages=0), dict(width=0), dict(pages=0, width=0)):
+        assert not call(**kw).any(), kw
+    for kw in (dict(page=0), dict(hq=0), dict(hkv=0), dict(d=0)):
+        with pytest.raises(ops.KernelError):
+            call(**kw)
