@@ -715,3 +715,13 @@ PB_EXPORT int pb_paged_attention_shared(int dtype, const void* q, const void* k_
 PB_EXPORT int pb_shared_wait_limit(long long limit) {
     return limit > 0 && cudaMemcpyToSymbol(g_wait_limit, &limit, sizeof(limit)) == cudaSuccess ? 0 : -1;
 }
+
+// Lets one of these waits run out: afterwards the error word reads 9.  Set a short limit first.
+namespace {
+struct SharedUnit {};
+}
+PB_EXPORT int pb_shared_wait_selftest(unsigned int* error, cudaStream_t stream) {
+    if (error == nullptr) return PB_ERR_BAD_SIZE;
+    wait_gives_up_kernel<SharedUnit><<<1, 32, 0, stream>>>(error);
+    return launch_status();
+}

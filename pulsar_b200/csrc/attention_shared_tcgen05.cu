@@ -352,3 +352,13 @@ int launch_tcgen05(const void* q, const Maps& maps, float* partial, const Shared
 PB_EXPORT int pb_shared_tcgen05_wait_limit(long long limit) {
     return limit > 0 && cudaMemcpyToSymbol(g_wait_limit, &limit, sizeof(limit)) == cudaSuccess ? 0 : -1;
 }
+
+// Lets one of these waits run out: afterwards the error word reads 9.  Set a short limit first.
+namespace {
+struct SharedTcgen05Unit {};
+}
+PB_EXPORT int pb_shared_tcgen05_wait_selftest(unsigned int* error, cudaStream_t stream) {
+    if (error == nullptr) return PB_ERR_BAD_SIZE;
+    wait_gives_up_kernel<SharedTcgen05Unit><<<1, 32, 0, stream>>>(error);
+    return launch_status();
+}

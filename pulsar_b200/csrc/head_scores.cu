@@ -380,6 +380,16 @@ PB_EXPORT int pb_head_scores_wait_limit(long long limit) {
     return limit > 0 && cudaMemcpyToSymbol(g_wait_limit, &limit, sizeof(limit)) == cudaSuccess ? 0 : -1;
 }
 
+// Lets one of these waits run out: afterwards the error word reads 9.  Set a short limit first.
+namespace {
+struct HeadScoresUnit {};
+}
+PB_EXPORT int pb_head_scores_wait_selftest(unsigned int* error, cudaStream_t stream) {
+    if (error == nullptr) return PB_ERR_BAD_SIZE;
+    wait_gives_up_kernel<HeadScoresUnit><<<1, 32, 0, stream>>>(error);
+    return launch_status();
+}
+
 // h [rows, k], w [vocab, k] bfloat16, 16-byte aligned; tokens int32 [rows]; logprob, entropy float32 [rows]; scratch float32 of
 // pb_head_scores_scratch elements; error: the word that a block sets which gave up a bounded wait.  cap 0: none.
 PB_EXPORT int pb_head_scores(const void* h, const void* w, const int* tokens, float* logprob, float* entropy, int rows, int vocab, int k, float scale,

@@ -44,6 +44,21 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     return true;
 }
 
+// One thread waits, with the limit of this translation unit's bounded waits (Unit: a type of its own), on a barrier that nobody arrives on, gives
+// up and writes 9 to the error word: the give-up path alone (no copy in flight, no tensor memory held).
+template <typename Unit>
+__global__ void wait_gives_up_kernel(unsigned int* error) {
+    __shared__ __align__(8) uint64_t bar;
+    __shared__ int abort_flag;
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        mbar_init(smem_addr(&bar), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (!mbar_wait(smem_addr(&bar), 0, &abort_flag)) atomicMax(error, 9u);
+        asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(smem_addr(&bar)) : "memory");
+    }
+}
+
 // Host side of the bounded waits of one translation unit: a new limit (> 0), a new value of the error word
 // (>= 0; tests and recovery write it), and the word's device address, so that a caller can read it in the
 // stream, beside its results, without a synchronisation of its own.

@@ -145,11 +145,14 @@ _SIGNATURES = {
     "pb_copy_pages": [_I, _P, _P, _P, _P, _P, _I, _P],
     "pb_paged_attention_shared": [_I] + [_P] * 6 + [_I] + [_P] * 4 + [_I] * 8 + [_F, _I, _I, _I, _I, _P, _P],
     "pb_shared_wait_limit": [ctypes.c_longlong],
+    "pb_shared_wait_selftest": [_P, _P],
     "pb_shared_tcgen05_wait_limit": [ctypes.c_longlong],
+    "pb_shared_tcgen05_wait_selftest": [_P, _P],
     "pb_shared_rows": [_I, _I, _I, _I],
     "pb_head_scores_supported": [_I, _I, _I],
     "pb_head_scores_scratch": [_I, _I],
     "pb_head_scores_wait_limit": [ctypes.c_longlong],
+    "pb_head_scores_wait_selftest": [_P, _P],
     "pb_head_scores": [_P] * 5 + [_I, _I, _I, _F, _F, _P, _P, _P],
     "pb_token_scores": [_I, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P],
 }
@@ -715,9 +718,16 @@ def set_wait_words(value: int) -> None:
         raise KernelError("the wait error words could not be written")
 
 
-def wait_selftest() -> None:
-    """One thread waits on a barrier nobody arrives on until the limit runs out and sets the product's error word to 9."""
-    check(fn("pb_gemm_tcgen05_wait_selftest")(stream()), "wait_selftest")
+def wait_selftest(kernel: str = "gemm_tcgen05") -> None:
+    """One thread waits on a barrier nobody arrives on until the limit of ``kernel``'s waits runs out and sets the error word that this kernel
+    reports in to 9: the product's, which is that of "head_scores" too, or the tcgen05 attention's of "shared" and "shared_tcgen05"."""
+    if kernel == "gemm_tcgen05":
+        check(fn("pb_gemm_tcgen05_wait_selftest")(stream()), "wait_selftest")
+        return
+    word = {"head_scores": 0, "shared": 1, "shared_tcgen05": 1}.get(kernel)
+    if word is None:
+        raise ValueError(f"wait_selftest: unknown kernel '{kernel}'")
+    check(fn(f"pb_{kernel}_wait_selftest")(wait_word_addresses()[word], stream()), "wait_selftest")
 
 
 def describe_wait_words(words) -> Optional[str]:
