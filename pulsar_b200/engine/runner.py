@@ -278,11 +278,25 @@ class ModelRunner:
             ctx.position_axes = axes.to(self.device, non_blocking=True)
         return ctx
 
-    # A step takes the attention over shared pages where that saves reading at least so many keys.  (Beside it norm, rotation and cache write are
-    # a launch of their own, and the other finds shared pages in L2.  A step of 12 layers of the 8B sizes, us without and with it: 8 forks of 2,000
-    # tokens, 14,000 keys saved, 3,236 and 3,218; of 4,000 tokens 3,538 and 3,274; of 8,000 4,126 and 3,385; 16 of 2,000 3,917 and 3,638; 32 of
-    # 500, 15,500 saved, 3,588 and 3,701; 32 of 8,000 8,096 and 3,982; 64 of 500 4,354 and 4,048.)
+    # A step takes the attention over shared pages where that saves reading at least so many keys with their values, of 2 KB and more; on the tensor
+    # cores as many more of smaller ones (48 MiB: with few heads the shared keys are in few blocks' hands, and the ordinary attention finds them in
+    # L2).  Beside it norm, rotation and cache write are a launch of their own.  us a layer without and with it, in a captured step, heads as
+    # query / kv / size:
+    #   bfloat16 32/8/128:  8 forks of 2,000 tokens (14,000 keys saved) 29.8, 28.3;  of 3,600  36.2, 29.9;  of 14,000  78.5, 37.4;
+    #                       32 of 450 (13,950)  34.6, 38.2;  of 820 (25,420)  40.0, 40.3;  of 6,000  123.6, 43.5;  64 of 400  45.3, 42.5
+    #   16/8/64:            8 of 3,600  32.2, 23.7;  64 of 400 (25,200)  31.5, 32.3;  32/8/64 there  33.1, 39.1, the worst that is taken
+    #   32/2/128:           8 of 3,600 (25,200)  27.8, 30.0;  of 7,200 (50,400)  30.9, 32.2;  of 14,000  38.0, 35.4
+    #   8/1/64:             8 of 3,600  17.9, 20.8;  of 14,000 (98,000)  22.0, 24.8;  32 of 6,000 (186,000)  32.3, 30.8
+    #   on the CUDA cores it is ahead everywhere: float32 32/8/128, 8 of 3,600  158.7, 79.8;  8/1/64 there  49.7, 37.4;  bfloat16 32/8/96  97.1, 52.9
     SHARED_KEYS_SAVED = 24576
+
+    def _least_saved(self, group: int) -> int:
+        """Keys whose reading ``group``'s attention has to be spared, for the attention over shared pages to be taken."""
+        pools = self.cache.groups[group].pools
+        page_size, dim = pools["k"].shape[3:]
+        per_key = sum(p.shape[2] * p.shape[4] * p.element_size() for p in pools.values())
+        smaller = max(1.0, 2048 / per_key) if ops.shared_on_tensor_cores(pools["k"].dtype, dim, page_size) else 1.0
+        return int(self.SHARED_KEYS_SAVED * smaller)
 
     def _find_shared(self, ctx: StepContext, rids) -> None:
         """Fill ``ctx.shared_pages``: per group members, starts and shared lengths, in memory that stays where it is (captured steps read it)."""
@@ -298,7 +312,7 @@ class ModelRunner:
             if families <= 0:
                 continue
             saved = sum((starts[f + 1] - starts[f] - 1) * shared[members[starts[f]]] for f in range(families))
-            if saved < self.SHARED_KEYS_SAVED:
+            if saved < self._least_saved(g):
                 continue
             room = self.scratch(f"shared.{g}", (3 * self.cache.max_requests + 1,), torch.int32)
             stage.to_device(room, 3 * n + 1)

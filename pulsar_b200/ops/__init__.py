@@ -2096,6 +2096,11 @@ def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
           "paged_attention_shared", kernels=2)
 
 
+def shared_on_tensor_cores(dtype: torch.dtype, head_dim: int, page_size: int) -> bool:
+    """Whether ``paged_attention_shared`` runs on the tensor cores (else on the CUDA cores)."""
+    return dtype == torch.bfloat16 and head_dim in (64, 128) and page_size in (8, 16, 32, 64)
+
+
 SHARED_CUT_KEYS = 32 * 256       # shared keys that are longer than that are cut into as many parts (the most, of the largest least size)
 
 
@@ -2111,7 +2116,7 @@ def shared_cut(n_seqs: int, n_families: int, most_members: int, most_shared: int
     # them.  The tcgen05 kernel has an SM to itself but for one block of the own sides, which want room: 120 blocks, or all SMs where that would
     # be no cut at all (us for 120 and 148: 1 family of 8 over 16,000 keys 20 and 24, 2 over 4,000 14.4 and 16.7, 6 over 4,000 31 and 33, 2 over 30,000 48
     # and 46; 9 over 12,000 102 uncut, 76 in two parts).  No part of less than two of its tiles, or of the others' (64 keys, general: one).
-    general = not (dtype == torch.bfloat16 and head_dim in (64, 128) and page_size in (8, 16, 32, 64))
+    general = not shared_on_tensor_cores(dtype, head_dim, page_size)
     blocks, least = max(1, blocks), 64 if general else 256 if tile == 128 else 128
     slots = _DECODE_SLOTS if tile != 128 else 120 if 120 // blocks > 1 else _DECODE_SLOTS // 2
     n_shared = max(1, min(32, -(-most_shared // least), slots // blocks)) if n_families else 0

@@ -58,3 +58,16 @@ def test_prompts_of_many_lengths_find_the_same_captured_steps(tmp_path):
         got = eng.candidates(prompt, n, 9, temperature=0.9, top_k=40, seed=n)
         assert sorted(c.tokens for c in got) == sorted(plain.generate([prompt] * n, 9, temperature=0.9, top_k=40, seed=n))
         assert len([k for k in eng.runner._graphs if k[5]]) <= 2
+
+
+@pytest.mark.parametrize("heads,dim,page,dtype,keys", [(8, 128, 16, "bfloat16", 24576), (8, 64, 16, "bfloat16", 24576), (2, 128, 16, "bfloat16", 49152), (1, 64, 16, "bfloat16", 196608),
+                                                       (1, 64, 16, "float32", 24576), (1, 96, 16, "bfloat16", 24576), (1, 64, 4, "bfloat16", 24576)])
+def test_small_keys_have_to_be_more(heads, dim, page, dtype, keys):
+    """On the tensor cores 48 MiB of keys and values that need not be read, wherever a key and its value are less than 2 KB."""
+    import torch
+    from pulsar_b200.cache import CacheManager, CacheNeed
+    runner = object.__new__(ModelRunner)
+    runner.cache = CacheManager([CacheNeed.paged_kv(heads, dim)], page, 4, 2, getattr(torch, dtype), "cpu")
+    assert runner._least_saved(0) == keys
+    runner.SHARED_KEYS_SAVED = 1
+    assert runner._least_saved(0) == keys // 24576
