@@ -25,10 +25,10 @@ using namespace pb::shared_attention;
 // Any head size that is a multiple of 16 (up to 256), any page size, float32 or bfloat16, on the CUDA cores in float32.  16 rows meet tiles
 // of 64 keys, of which each of four warps has 16, with a maximum, sums and an O of its own; the four are joined at the end.  A warp's scores
 // are 16 rows x 16 keys, four rows and two keys a lane, its O 16 rows x D, four dimensions a lane: shared memory is then read 6 times per 32
-// products of scores and 5 per 64 of O, so the FMA units bound the shared sides; items of up to 4 or 8 rows (a sequence's own) leave out the
+// products of scores and 5 per 64 of O, and the shared sides are bound by these instructions; items of up to 4 or 8 rows (a sequence's own) leave out the
 // rest and are bound by bytes.  Keys and values come by cp.async as they lie in the pools, the next tile's keys under this one's values and its
-// values under the next one's scores.  (float32, heads of 128: 4 families of 8 over 2,000 keys 59 us, where a key a lane and four rows a warp,
-// 5 reads per 16 products, took 156; 30 sequences of 2,000 keys that share nothing 82 us, 6.4 TB/s.)
+// values under the next one's scores.  (float32, heads of 128: 4 families of 8 over 2,000 keys 59 us, four times what the multiply-adds take at their units' rate, where a key a lane and four rows a
+// warp, 5 reads per 16 products, took 156; 30 sequences of 2,000 keys that share nothing 82 us, 6.4 TB/s.)
 constexpr int kRows = 16, kKeys = 64, kThreads = 128;
 constexpr int kWarpKeys = kKeys / (kThreads / 32);
 constexpr int kWeightPitch = 20;                         // floats from a key's 16 weights to the next key's: stored and read without bank conflicts
@@ -416,7 +416,8 @@ __device__ __forceinline__ bool attend(const bf16* __restrict__ q, float* __rest
             }
 #pragma unroll
             for (int n = 0; n < kGroups; ++n) {
-                // weights in [0, 1], rounded to bfloat16 for the product (2^-9 of each); their sum is of the unrounded ones
+                // weights in [0, 1], rounded to bfloat16 for the product (2^-9 of each, at random: 2.2e-3 of a result, 1.7e-3 of which are the
+                // result's own rounding; float32 weights would take two products); their sum is of the unrounded ones
                 const uint32_t pa[4] = {pack_bf16(s[2 * n][0], s[2 * n][1]), pack_bf16(s[2 * n][2], s[2 * n][3]),
                                         pack_bf16(s[2 * n + 1][0], s[2 * n + 1][1]), pack_bf16(s[2 * n + 1][2], s[2 * n + 1][3])};
 #pragma unroll

@@ -8,7 +8,7 @@
 namespace pb {
 namespace shared_attention {
 
-// 2^x by the special-function unit alone; results below 2^-126 are 0.
+// 2^x by the special-function unit alone, 2 ulp as exp2f has them; results below 2^-126 are 0.
 __device__ __forceinline__ float pow2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

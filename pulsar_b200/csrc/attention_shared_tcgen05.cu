@@ -3,14 +3,15 @@
 //
 // A block has up to 128 query rows of a family (members x the group's heads) and one split of the family's shared keys.  The rows are the
 // lanes of tensor memory: S = Q K^T (tcgen05.mma, 128 x 128 x 16 steps, operands in shared memory), a thread per row takes its row of S,
-// keeps maximum and sum in float32 and writes P = 2^(s c - m c), rounded to bfloat16, over S; O += P V reads P from tensor memory and V as it
+// keeps maximum and sum in float32 and writes P = 2^(s c - m c), rounded to bfloat16 as the product's operand has to be (2^-9 of each weight, the sum is
+// of the unrounded ones), over S; O += P V reads P from tensor memory and V as it
 // lies in the pages.  The product costs the same for one row as for 128, so a key tile passes the tensor cores once however many of the
 // family's sequences there are: bound by the bytes of the keys and values.  (mma.sync takes 2,100 cycles for 32 rows x 64 keys, with two
 // blocks an SM as long as the bytes do, and so many times that for larger families.)
 //
 // A thread takes 128 exponentials a tile, 1,900 cycles with all that goes with them, more than the tile's bytes take where SMs are idle.  So
 // families of up to 64 rows stand in tensor memory twice, of up to 32 four times: each copy has its own half or quarter of a tile's keys,
-// writes zeros for the weights of the others, and the copies' sums are joined at the end (REPEAT).  (12 families of 8, 32 rows per kv head,
+// writes zeros for the weights of the others, and the copies' sums are joined at the end (REPEAT; zero times an infinite value is NaN).  (12 families of 8, 32 rows per kv head,
 // over up to 2,600 keys, 92 MB: 31 us cold.)
 //
 // Roles: warps 0-3 softmax (and the gathering of the query rows, which lie with their sequences), warp 4 issues the products, warp 5 brings K

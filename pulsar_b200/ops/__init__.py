@@ -2040,9 +2040,11 @@ def paged_attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     """Attention of one query token per sequence over a cache in which families of sequences share pages: q, out [S, Hq, D], pools
     [pages, Hkv, page, D], ``block_table`` [S, width], ``kv_len`` [S].  Family f is the sequences ``members[family_start[f]:family_start[f + 1]]``;
     they all have the same pages for their first ``shared_len[s]`` keys (whole pages, at most ``kv_len[s]``), which are read once for all
-    of them.  A sequence in no family has ``shared_len`` 0; one with ``kv_len`` 0 gets zeros.  All arrays int32 on the device.
+    of them.  Page ids of keys that there are have to lie in the pools.  A sequence in no family has ``shared_len`` 0; one with ``kv_len`` 0 gets zeros.  All arrays int32 on the device.
     (bfloat16 with pages of 8, 16, 32 or 64 keys and heads of 64 or 128 runs on the tensor cores; a wait that it gives up is reported in
-    the tcgen05 attention's error word.)
+    the tcgen05 attention's error word.  There the weights, which are at most 1 or, between two moves of the maximum, 2^8, are rounded to bfloat16 for
+    their product with the values, and an infinite value may come out as NaN: a weight of zero, of which there are more than the formula
+    has, makes NaN of it.)
     ``most_members`` is the largest family's size as the host knows it (more members than that are not served), ``most_shared`` the longest
     shared length, about (it decides into how many parts the shared keys are cut; 0: there are no families); ``most_own`` is the most keys that a sequence has beyond its shared ones, where the host knows (keys beyond
     that are not seen).  ``partial``: float32 scratch of ``shared_scratch`` elements, made here where it is not given."""
@@ -2121,8 +2123,9 @@ def shared_cut(n_seqs: int, n_families: int, most_members: int, most_shared: int
     slots = _DECODE_SLOTS if tile != 128 else 120 if 120 // blocks > 1 else _DECODE_SLOTS // 2
     n_shared = max(1, min(32, -(-most_shared // least), slots // blocks)) if n_families else 0
     # Own keys (own_tokens at most): parts of at most 512, so that no block walks much longer than the others, and of fewer where that leaves SMs idle.  But a part
-    # that a sequence does not have costs a block that ends at once, some 1.3 ns: no more than about 5,000 of those (101 sequences of 8 kv heads,
-    # 3,100 at most: 7 parts 52 us, 3 parts 56; 240, 2,600 at most: 6 parts 58, 2 parts 45), and no more than 32 parts.
+    # that a sequence does not have costs a block that ends at once, some 1.3 ns: no more than about 5,000 of those, and no more than 32 parts.  (us in a
+    # graph, 8 kv heads: 101 sequences, 3,100 keys at most as the table has it, up to 1,170 in truth: 7 parts, the rule's, 49, 3 parts 53, one 55; 240, 2,940 at
+    # most, most of them of up to 500: the rule's 3 parts 83, 2 parts 87, 6 parts 89; 240, 236 of them of up to 2,850: 3 parts 220, 2 parts 219, 6 parts 228.)
     own_blocks = n_seqs * -(-group // 16) * n_kv_heads
     own_least, own_slots = 32 if general else 128, 3 * _DECODE_SLOTS // (4 if tile == 128 else 2)
     chunk = max(own_least, min(512, own_tokens * own_blocks // own_slots), -(-own_tokens // min(32, 1 + max(1, 5000 // own_blocks))))
