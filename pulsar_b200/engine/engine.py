@@ -528,7 +528,7 @@ class Engine:
         """How likely the model finds the tokens of each prompt: the scores of its second token to its last, given those before.  Without
         ``alternatives`` log probability and entropy come straight from the hidden rows (``ops.head_scores``) and logits are never made; with it
         (0 for none) ranks and so many alternatives come too.  Prompts run one behind the other in portions of ``max_chunk_size``, each
-        in pages that are given back at its end."""
+        in pages and a state slot that are given back at its end, and that have to be free (OutOfPages)."""
         self._alive()
         self._drain()
         self._check_alternatives(alternatives)
