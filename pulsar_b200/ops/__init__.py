@@ -154,6 +154,9 @@ _SIGNATURES = {
     "pb_head_scores_wait_limit": [ctypes.c_longlong],
     "pb_head_scores_wait_selftest": [_P, _P],
     "pb_head_scores": [_P] * 5 + [_I, _I, _I, _F, _F, _P, _P, _P],
+    "pb_qk_norm_rope_write_4bit": [_I] + [_P] * 11 + [ctypes.c_double] + [_I] * 7 + [_P],
+    "pb_expand_pages_4bit": [_I] + [_P] * 9 + [_I] * 6 + [_P],
+    "pb_paged_attention_4bit": [_I] + [_P] * 7 + [_I, _P, _P] + [_I] * 7 + [_F, _I, _P],
     "pb_token_scores": [_I, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P],
 }
 _RETURNS = {"pb_recurrence_workspace": _L, "pb_head_scores_scratch": _L}        # the others return an int
@@ -168,7 +171,7 @@ _LAUNCHERS = {"embed", "scale_cap", "move_ids", "add_rmsnorm", "rope_table", "qk
               "selective_scan", "selective_scan_prompt", "selective_scan_chunked", "post_norm_add", "clamped_glu",
               "post_norm_add_bias", "glu_bias", "qk_prepare", "qk_prepare_whole", "sigmoid_gate_strided", "add_bias", "moe_route", "moe_gate_up", "moe_up", "moe_down", "moe_grouped",
               "norm_shift", "parallel_add", "activation", "min_gru", "diff_combine", "retention", "scaled_sum", "concat_streams", "normed_sum", "matrix_memory", "state_space",
-              "copy_pages", "token_scores", "paged_attention_shared", "head_scores"}
+              "copy_pages", "token_scores", "paged_attention_shared", "head_scores", "qk_norm_rope_write_4bit", "expand_pages_4bit", "paged_attention_4bit"}
 
 
 class KernelError(RuntimeError):
@@ -2182,3 +2185,154 @@ def head_scores(h: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, logprob:
         if scale != 1.0 or cap is not None:
             scale_cap(logits[:n], scale, cap)
         token_scores(logits[:n], tokens[at:at + n], logprob[at:at + n], entropy[at:at + n])
+
+
+# ------------------------------------------------------------------ keys and values held in 4 bits
+# For every token, kv head and group of 32 neighbouring channels a step and a least value (bfloat16) and 32 codes of 4 bits: value = least +
+# step * code (csrc/cache4.cuh).  Pools are [pages, kv heads, page, width]: codes uint8 of width D / 2, steps bfloat16 of width D / 16.
+GROUP_4BIT = 32
+
+
+def _check_4bit(name: str, pools, n_kv_heads: int, head_dim: int, page_size: int) -> int:
+    """Refuses pools that are not those of a cache of 4 bits with these sizes; pages of the pools."""
+    if head_dim % GROUP_4BIT or not (0 < head_dim <= 256) or n_kv_heads <= 0 or page_size <= 0:
+        raise KernelError(f"{name}: heads of a multiple of {GROUP_4BIT} channels, at most 256, and pages of a key or more, found {head_dim} and {page_size}")
+    n_pages = pools[0].shape[0] if pools[0].dim() else 0
+    for pool, dtype, width in zip(pools, (torch.uint8, torch.bfloat16) * 2, (head_dim // 2, head_dim // 16) * 2):
+        if pool.dtype != dtype or pool.shape != (n_pages, n_kv_heads, page_size, width):
+            raise KernelError(f"{name}: codes are uint8 [pages, {n_kv_heads}, {page_size}, {head_dim // 2}], steps bfloat16 [pages, {n_kv_heads}, {page_size}, "
+                              f"{head_dim // 16}], found {pool.dtype} {tuple(pool.shape)}")
+    return n_pages
+
+
+def _at_16(name: str, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.data_ptr() % 16:
+            raise KernelError(f"{name}: tensors must start at a multiple of 16 bytes")
+
+
+def _elsewhere(name: str, *tensors) -> Optional[torch.device]:
+    """The tensors' device where it is not the current one; refuses tensors of several devices."""
+    where = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != where:
+            raise KernelError(f"{name}: all tensors must be on one device, found {where} and {t.device}")
+    return where if where.index != (torch.cuda.current_device() if _device is None else _device()) else None
+
+
+def qk_norm_rope_write_4bit(qkv: torch.Tensor, q_out: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.Tensor, v_pool: torch.Tensor, v_steps: torch.Tensor,
+                            slots: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                            eps: float, n_heads: int, n_kv_heads: int, head_dim: int, rotary: int, page_size: int) -> None:
+    """``qk_norm_rope_write`` into a cache of 4 bits: per-head RMSNorm (where weights are given) and rotation of the rows ``qkv``
+    [N, (Hq + 2 Hkv) * D] (float32 or bfloat16), q to ``q_out`` [N, Hq, D], k and v, rounded to the rows' dtype as a cache of that dtype would
+    hold them, in 4 bits to ``slots`` (int32 [N], page * page_size + place; no two alike).  A slot outside the pool, -1 for none, is not
+    written.  A group of 32 channels that holds a NaN or a value beyond bfloat16's range comes back as NaN."""
+    name = "qk_norm_rope_write_4bit"
+    tensors = (qkv, q_out, k_pool, k_steps, v_pool, v_steps, slots, cos, sin, q_weight, k_weight)
+    _cuda(*tensors)
+    if (where := _elsewhere(name, *tensors)) is not None:
+        with torch.cuda.device(where):
+            return qk_norm_rope_write_4bit(*tensors, eps, n_heads, n_kv_heads, head_dim, rotary, page_size)
+    n_pages = _check_4bit(name, tensors[2:6], n_kv_heads, head_dim, page_size)
+    kind = code(qkv.dtype)
+    if qkv.dim() != 2 or n_heads < 0 or qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or q_out.shape != (qkv.shape[0], n_heads, head_dim) or q_out.dtype != qkv.dtype:
+        raise KernelError(f"{name}: rows [N, ({n_heads} + 2 * {n_kv_heads}) * {head_dim}] and queries [N, {n_heads}, {head_dim}] of one dtype, found {qkv.dtype} "
+                          f"{tuple(qkv.shape)} and {q_out.dtype} {tuple(q_out.shape)}")
+    n = qkv.shape[0]
+    if slots.dtype != torch.int32 or slots.shape != (n,):
+        raise KernelError(f"{name}: slots must be int32 [{n}], found {slots.dtype} {tuple(slots.shape)}")
+    if rotary < 0 or rotary % 2 or rotary > head_dim or cos.shape != (n, rotary // 2) or sin.shape != cos.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise KernelError(f"{name}: an even number of turned channels, at most {head_dim}, and float32 cosines and sines [{n}, {rotary // 2}], found {rotary}, {cos.dtype} "
+                          f"{tuple(cos.shape)}, {sin.dtype} {tuple(sin.shape)}")
+    for w in (q_weight, k_weight):
+        if w is not None and (w.dtype != torch.float32 or w.shape != (head_dim,)):
+            raise KernelError(f"{name}: norm weights must be float32 [{head_dim}], found {w.dtype} {tuple(w.shape)}")
+    _at_16(name, *tensors[:6])
+    _check_against(k_pool)
+    if n_pages == 0:
+        raise KernelError(f"{name}: pools without a page")
+    if n == 0:
+        return
+    check(fn("pb_qk_norm_rope_write_4bit")(kind, _p(qkv), _p(q_out), _p(k_pool), _p(k_steps), _p(v_pool), _p(v_steps), _p(slots), _p(cos), _p(sin), _p(q_weight), _p(k_weight),
+                                           float(eps), n, n_heads, n_kv_heads, head_dim, rotary, page_size, n_pages, stream()), name)
+
+
+def expand_pages_4bit(k_pool: torch.Tensor, k_steps: torch.Tensor, v_pool: torch.Tensor, v_steps: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor,
+                      k_out: torch.Tensor, v_out: torch.Tensor, table_out: torch.Tensor) -> None:
+    """The values of the pages that sequences hold in a cache of 4 bits, into pages of their own: ``k_out``, ``v_out`` (float32 or bfloat16
+    [S * width pages at least, Hkv, page, D]), where page j of sequence i goes to page i * width + j.  ``block_table`` int32 [S, width],
+    ``kv_len`` int32 [S]; ``table_out`` int32 [S, width] becomes the block table of the new pages.  Places behind a sequence's last key become
+    zeros; pages that hold no key, or whose id lies outside the pool (-1), stay as they were and are -1 in ``table_out``."""
+    name = "expand_pages_4bit"
+    tensors = (k_pool, k_steps, v_pool, v_steps, block_table, kv_len, k_out, v_out, table_out)
+    _cuda(*tensors)
+    if (where := _elsewhere(name, *tensors)) is not None:
+        with torch.cuda.device(where):
+            return expand_pages_4bit(*tensors)
+    if k_out.dim() != 4 or v_out.shape != k_out.shape or v_out.dtype != k_out.dtype:
+        raise KernelError(f"{name}: pages [pages, kv heads, page, D] of one dtype and shape, found {k_out.dtype} {tuple(k_out.shape)} and {v_out.dtype} {tuple(v_out.shape)}")
+    out_pages, hkv, page_size, d = k_out.shape
+    n_pages = _check_4bit(name, tensors[:4], hkv, d, page_size)
+    kind = code(k_out.dtype)
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or table_out.dtype != torch.int32 or table_out.shape != block_table.shape:
+        raise KernelError(f"{name}: block tables must be int32 [S, width], found {block_table.dtype} {tuple(block_table.shape)} and {table_out.dtype} {tuple(table_out.shape)}")
+    s, width = block_table.shape
+    if kv_len.dtype != torch.int32 or kv_len.shape != (s,):
+        raise KernelError(f"{name}: lengths must be int32 [{s}], found {kv_len.dtype} {tuple(kv_len.shape)}")
+    if out_pages < s * width:
+        raise KernelError(f"{name}: {s} sequences of {width} pages need as many pages to go to, found {out_pages}")
+    _at_16(name, *tensors[:4], k_out, v_out)
+    _check_against(k_pool)
+    if s == 0 or width == 0:
+        return
+    if n_pages == 0:
+        table_out.fill_(-1)
+        return
+    check(fn("pb_expand_pages_4bit")(kind, _p(k_pool), _p(k_steps), _p(v_pool), _p(v_steps), _p(block_table), _p(kv_len), _p(k_out), _p(v_out), _p(table_out), s, width,
+                                     hkv, d, page_size, n_pages, stream()), name)
+
+
+def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.Tensor, v_pool: torch.Tensor, v_steps: torch.Tensor, out: torch.Tensor,
+                         block_table: torch.Tensor, kv_len: torch.Tensor, scale: float, window: Optional[int] = None, cu_q: Optional[torch.Tensor] = None,
+                         q_lens=None) -> None:
+    """Attention over a cache of 4 bits: q, out [N, Hq, D] (float32 or bfloat16), ``block_table`` int32 [S, width], ``kv_len`` int32 [S] with
+    the keys of this step in it.  Without ``cu_q`` every sequence has one query token, the last (N = S); else sequence i has the tokens
+    ``cu_q[i]:cu_q[i + 1]`` (int32 [S + 1], from 0, rising), the last of its ``kv_len[i]``, and ``q_lens`` are their numbers as the host knows
+    them.  A query sees the keys up to its own, with ``window`` w the last w of them.  Keys behind the table's row, or whose page id lies
+    outside the pool, are not seen; a query that sees none gets zeros.  Rows of ``out`` behind the last sequence stay as they were."""
+    name = "paged_attention_4bit"
+    tensors = (q, k_pool, k_steps, v_pool, v_steps, out, block_table, kv_len)
+    _cuda(*tensors, cu_q)
+    if (where := _elsewhere(name, *tensors, cu_q)) is not None:
+        with torch.cuda.device(where):
+            return paged_attention_4bit(*tensors, scale, window, cu_q, q_lens)
+    if q.dim() != 3 or out.shape != q.shape or out.dtype != q.dtype or k_pool.dim() != 4:
+        raise KernelError(f"{name}: q and out [N, heads, D] of one dtype, pools [pages, kv heads, page, width], found {q.dtype} {tuple(q.shape)}, {out.dtype} {tuple(out.shape)}, "
+                          f"{tuple(k_pool.shape)}")
+    n, hq, d = q.shape
+    hkv, page_size = k_pool.shape[1:3]
+    n_pages = _check_4bit(name, tensors[1:5], hkv, d, page_size)
+    kind = code(q.dtype)
+    if hq == 0 or hq % hkv:
+        raise KernelError(f"{name}: {hq} query heads cannot be grouped over {hkv} kv heads")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or kv_len.dtype != torch.int32 or kv_len.shape != block_table.shape[:1]:
+        raise KernelError(f"{name}: a block table int32 [S, width] and lengths int32 [S], found {block_table.dtype} {tuple(block_table.shape)} and {kv_len.dtype} {tuple(kv_len.shape)}")
+    s, width = block_table.shape
+    if (cu_q is None) != (q_lens is None):
+        raise KernelError(f"{name}: cu_q and q_lens go together")
+    if cu_q is None:
+        if n != s:
+            raise KernelError(f"{name}: without cu_q every sequence has one query token, found {n} for {s}")
+    elif cu_q.dtype != torch.int32 or cu_q.shape != (s + 1,) or len(q_lens) != s or (s and min(q_lens) < 0) or sum(q_lens) > n:
+        raise KernelError(f"{name}: cu_q int32 [{s + 1}] and {s} numbers of tokens that {n} rows hold, found {cu_q.dtype} {tuple(cu_q.shape)} and {list(q_lens)[:8]}")
+    if window is not None and window <= 0:
+        raise KernelError(f"{name}: a window must be positive, found {window}")
+    _at_16(name, *tensors[:6])
+    _check_against(k_pool)
+    if n == 0 or s == 0:
+        return
+    if width == 0 or n_pages == 0:               # nobody has a key
+        out[:n if q_lens is None else sum(q_lens)].zero_()
+        return
+    check(fn("pb_paged_attention_4bit")(kind, _p(q), _p(k_pool), _p(k_steps), _p(v_pool), _p(v_steps), _p(out), _p(block_table), width, _p(kv_len), _p(cu_q), n, s, hq, hkv, d,
+                                        page_size, n_pages, float(scale), int(window or 0), stream()), name)
