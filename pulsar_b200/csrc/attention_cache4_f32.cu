@@ -1,0 +1,10 @@
+// The float32 kernels of attention over a cache of 4 bits (attention_cache4.cuh).
+#include "attention_cache4.cuh"
+
+namespace pb {
+
+int attend_4bit_f32(const Attend4& a, int groups, int rows, int most_tokens, cudaStream_t stream) {
+    return rows == 8 ? launch_attend_4bit_of<float, 1>(a, groups, most_tokens, stream) : PB_ERR_BAD_SIZE;
+}
+
+}  // namespace pb

@@ -145,15 +145,22 @@ __global__ void qk_norm_rope_write_4bit_kernel(const T* __restrict__ qkv, T* __r
 template <typename T>
 __global__ void expand_pages_4bit_kernel(Pool4 k_pool, Pool4 v_pool, const int* __restrict__ table, const int* __restrict__ kv_len, T* __restrict__ k_out,
                                          T* __restrict__ v_out, int* __restrict__ table_out, int width, int Hkv, int D, int page_size, int n_pages,
-                                         const PoolBounds bounds) {
+                                         const int* __restrict__ cu_q, int window, const PoolBounds bounds) {
     pdl_wait();
-    const int seq = blockIdx.y, logical = blockIdx.x;
-    const int rows = min(page_size, kv_len[seq] - logical * page_size);          // of this page, that hold a key
-    const int page = rows > 0 ? table[(size_t)seq * width + logical] : -1;
-    if (rows > 0 && page >= 0) page_ok(page, bounds);
+    const int seq = blockIdx.y, logical = blockIdx.x, length = kv_len[seq];
     const size_t out_page = (size_t)seq * width + logical;
-    if (blockIdx.z == 0 && threadIdx.x == 0) table_out[out_page] = page_or_none(page, n_pages) < 0 ? -1 : (int)out_page;
-    if (page_or_none(page, n_pages) < 0) return;
+    int rows = min(page_size, length - logical * page_size);                    // of this page, that hold a key
+    int page = rows > 0 ? table[(size_t)seq * width + logical] : -1;
+    if (rows > 0 && page >= 0) page_ok(page, bounds);
+    bool there = page_or_none(page, n_pages) >= 0;
+    if (cu_q != nullptr) {
+        // For attention: what no tile of 128 keys that a query sees touches is left out, and what else is none becomes zeros.
+        const int low = window > 0 ? length - (cu_q[seq + 1] - cu_q[seq]) - window + 1 - 128 : 0;
+        if (!there) rows = min(rows, 0);
+        there = logical * page_size < length && (logical + 1) * page_size > low;
+    }
+    if (blockIdx.z == 0 && threadIdx.x == 0) table_out[out_page] = there ? (int)out_page : -1;
+    if (!there) return;
     const int G = D / kGroup4, octets = D / 8, per_head = page_size * octets, n = 2 * Hkv * per_head;
     for (int i = blockIdx.z * blockDim.x + threadIdx.x; i < n; i += gridDim.z * blockDim.x) {
         const bool is_v = i >= Hkv * per_head;
@@ -208,8 +215,9 @@ PB_EXPORT int pb_qk_norm_rope_write_4bit(int dtype, const void* qkv, void* q_out
 }
 
 PB_EXPORT int pb_expand_pages_4bit(int dtype, void* k_codes, void* k_steps, void* v_codes, void* v_steps, const int* table, const int* kv_len, void* k_out, void* v_out,
-                                   int* table_out, int n_seqs, int width, int Hkv, int D, int page_size, int n_pages, cudaStream_t stream) {
-    if (!sizes_4bit(Hkv, D, page_size, n_pages) || n_seqs < 0 || width < 0) return PB_ERR_BAD_SIZE;
+                                   int* table_out, int n_seqs, int width, int Hkv, int D, int page_size, int n_pages, const int* cu_q, int window,
+                                   cudaStream_t stream) {
+    if (!sizes_4bit(Hkv, D, page_size, n_pages) || n_seqs < 0 || width < 0 || window < 0) return PB_ERR_BAD_SIZE;
     if (n_seqs > 65535 || (long long)n_seqs * width > 0x7fffffffLL || 2LL * Hkv * page_size * (D / 8) > 0x3fffffffLL) return PB_ERR_TOO_LARGE;
     if (n_seqs == 0 || width == 0) return 0;
     const Pool4 k{(uint8_t*)k_codes, (__nv_bfloat16*)k_steps}, v{(uint8_t*)v_codes, (__nv_bfloat16*)v_steps};
@@ -217,9 +225,9 @@ PB_EXPORT int pb_expand_pages_4bit(int dtype, void* k_codes, void* k_steps, void
     const dim3 grid(width, n_seqs, blocks < 64 ? blocks : 64);
     if (dtype == PB_F32)
         return launch_pdl(expand_pages_4bit_kernel<float>, grid, dim3(256), 0, stream, k, v, table, kv_len, (float*)k_out, (float*)v_out, table_out, width, Hkv, D,
-                          page_size, n_pages, pool_bounds_now());
+                          page_size, n_pages, cu_q, window, pool_bounds_now());
     if (dtype == PB_BF16)
         return launch_pdl(expand_pages_4bit_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, k, v, table, kv_len, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out,
-                          table_out, width, Hkv, D, page_size, n_pages, pool_bounds_now());
+                          table_out, width, Hkv, D, page_size, n_pages, cu_q, window, pool_bounds_now());
     return PB_ERR_BAD_DTYPE;
 }

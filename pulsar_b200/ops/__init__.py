@@ -155,8 +155,9 @@ _SIGNATURES = {
     "pb_head_scores_wait_selftest": [_P, _P],
     "pb_head_scores": [_P] * 5 + [_I, _I, _I, _F, _F, _P, _P, _P],
     "pb_qk_norm_rope_write_4bit": [_I] + [_P] * 11 + [ctypes.c_double] + [_I] * 7 + [_P],
-    "pb_expand_pages_4bit": [_I] + [_P] * 9 + [_I] * 6 + [_P],
-    "pb_paged_attention_4bit": [_I] + [_P] * 7 + [_I, _P, _P] + [_I] * 7 + [_F, _I, _P],
+    "pb_expand_pages_4bit": [_I] + [_P] * 9 + [_I] * 6 + [_P, _I, _P],
+    "pb_paged_attention_4bit": [_I] + [_P] * 8 + [_I, _P, _P] + [_I] * 8 + [_F, _I, _I, _I, _P],
+    "pb_attention_4bit_rows": [_I, _I],
     "pb_token_scores": [_I, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P],
 }
 _RETURNS = {"pb_recurrence_workspace": _L, "pb_head_scores_scratch": _L}        # the others return an int
@@ -2289,23 +2290,52 @@ def expand_pages_4bit(k_pool: torch.Tensor, k_steps: torch.Tensor, v_pool: torch
         table_out.fill_(-1)
         return
     check(fn("pb_expand_pages_4bit")(kind, _p(k_pool), _p(k_steps), _p(v_pool), _p(v_steps), _p(block_table), _p(kv_len), _p(k_out), _p(v_out), _p(table_out), s, width,
-                                     hkv, d, page_size, n_pages, stream()), name)
+                                     hkv, d, page_size, n_pages, None, 0, stream()), name)
+
+
+# Rows of a kv head (its query heads times a sequence's tokens) above which portions are attended to in two steps, where a dense kernel of the
+# tensor cores takes their sizes: the sequences' pages as bfloat16 (``expand_pages_4bit``), then that kernel.
+EXPANDED_ROWS_4BIT = 64
+
+
+@functools.lru_cache(maxsize=1024)
+def cut_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads: int, table_tokens: int, window: int, dtype: torch.dtype) -> Tuple[int, int]:
+    """(parts, keys of a part) that ``paged_attention_4bit`` cuts the keys of a sequence into, for sequences of up to ``most_tokens`` tokens."""
+    rows = most_tokens * (n_heads // n_kv_heads)
+    blocks = n_seqs * n_kv_heads * -(-rows // fn("pb_attention_4bit_rows")(code(dtype), rows))
+    keys = min(table_tokens, window + most_tokens + 15) if window else table_tokens
+    part = max(64, min(1024, -(-keys * blocks // (3 * 148)))) if blocks else 64
+    part = -(-part // 64) * 64
+    return -(-keys // part), part
+
+
+def _expanded_4bit(dtype: torch.dtype, rows: int, n_heads: int, n_kv_heads: int, head_dim: int, page_size: int, scale: float) -> Optional[str]:
+    """The dense kernel that attends to portions of so many rows over expanded pages, or None: the kernel on codes does."""
+    if dtype != torch.bfloat16 or rows <= EXPANDED_ROWS_4BIT or not scale > 0.0:
+        return None
+    if ATTENTION_BACKEND != "mma" and prefill_tcgen05_supported(dtype, n_heads, n_kv_heads, head_dim, page_size):
+        return "tcgen05"
+    return "tc" if prefill_tc_supported(dtype, n_heads, n_kv_heads, head_dim, page_size) else None
 
 
 def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.Tensor, v_pool: torch.Tensor, v_steps: torch.Tensor, out: torch.Tensor,
                          block_table: torch.Tensor, kv_len: torch.Tensor, scale: float, window: Optional[int] = None, cu_q: Optional[torch.Tensor] = None,
-                         q_lens=None) -> None:
+                         q_lens=None, scratch=None) -> None:
     """Attention over a cache of 4 bits: q, out [N, Hq, D] (float32 or bfloat16), ``block_table`` int32 [S, width], ``kv_len`` int32 [S] with
     the keys of this step in it.  Without ``cu_q`` every sequence has one query token, the last (N = S); else sequence i has the tokens
     ``cu_q[i]:cu_q[i + 1]`` (int32 [S + 1], from 0, rising), the last of its ``kv_len[i]``, and ``q_lens`` are their numbers as the host knows
-    them.  A query sees the keys up to its own, with ``window`` w the last w of them.  Keys behind the table's row, or whose page id lies
-    outside the pool, are not seen; a query that sees none gets zeros.  Rows of ``out`` behind the last sequence stay as they were."""
+    them.  A query sees the keys up to its own, with ``window`` w the last w of them; those have to lie in pages of the pool (an id that is
+    none is not read).  A query that sees no key gets zeros.  Rows of ``out`` behind the last sequence stay as they were.
+
+    bfloat16 portions of more than 64 rows a kv head (query heads times tokens), where the dense attention of prompt portions has a kernel
+    for their sizes and the scale is above zero, are attended to over expanded pages, which takes room for S * width pages.  (There a value that is NaN also
+    reaches the tokens of its sequence's portion that do not see it.)  ``scratch(tag, shape, dtype)`` gives tensors to work in; without it they are made here."""
     name = "paged_attention_4bit"
     tensors = (q, k_pool, k_steps, v_pool, v_steps, out, block_table, kv_len)
     _cuda(*tensors, cu_q)
     if (where := _elsewhere(name, *tensors, cu_q)) is not None:
         with torch.cuda.device(where):
-            return paged_attention_4bit(*tensors, scale, window, cu_q, q_lens)
+            return paged_attention_4bit(*tensors, scale, window, cu_q, q_lens, scratch)
     if q.dim() != 3 or out.shape != q.shape or out.dtype != q.dtype or k_pool.dim() != 4:
         raise KernelError(f"{name}: q and out [N, heads, D] of one dtype, pools [pages, kv heads, page, width], found {q.dtype} {tuple(q.shape)}, {out.dtype} {tuple(out.shape)}, "
                           f"{tuple(k_pool.shape)}")
@@ -2320,19 +2350,37 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
     s, width = block_table.shape
     if (cu_q is None) != (q_lens is None):
         raise KernelError(f"{name}: cu_q and q_lens go together")
+    most_tokens = 1
     if cu_q is None:
         if n != s:
             raise KernelError(f"{name}: without cu_q every sequence has one query token, found {n} for {s}")
-    elif cu_q.dtype != torch.int32 or cu_q.shape != (s + 1,) or len(q_lens) != s or (s and min(q_lens) < 0) or sum(q_lens) > n:
-        raise KernelError(f"{name}: cu_q int32 [{s + 1}] and {s} numbers of tokens that {n} rows hold, found {cu_q.dtype} {tuple(cu_q.shape)} and {list(q_lens)[:8]}")
+    else:
+        if cu_q.dtype != torch.int32 or cu_q.shape != (s + 1,) or len(q_lens) != s or (s and min(q_lens) < 0) or sum(q_lens) > n:
+            raise KernelError(f"{name}: cu_q int32 [{s + 1}] and {s} numbers of tokens that {n} rows hold, found {cu_q.dtype} {tuple(cu_q.shape)} and {list(q_lens)[:8]}")
+        most_tokens = max(q_lens, default=0)
     if window is not None and window <= 0:
         raise KernelError(f"{name}: a window must be positive, found {window}")
     _at_16(name, *tensors[:6])
     _check_against(k_pool)
-    if n == 0 or s == 0:
+    if n == 0 or s == 0 or most_tokens == 0:
         return
     if width == 0 or n_pages == 0:               # nobody has a key
         out[:n if q_lens is None else sum(q_lens)].zero_()
         return
-    check(fn("pb_paged_attention_4bit")(kind, _p(q), _p(k_pool), _p(k_steps), _p(v_pool), _p(v_steps), _p(out), _p(block_table), width, _p(kv_len), _p(cu_q), n, s, hq, hkv, d,
-                                        page_size, n_pages, float(scale), int(window or 0), stream()), name)
+    if scratch is None:
+        def scratch(tag, shape, dtype):
+            return torch.empty(shape, dtype=dtype, device=q.device)
+    window = int(window or 0)
+    dense = None if cu_q is None else _expanded_4bit(q.dtype, most_tokens * (hq // hkv), hq, hkv, d, page_size, scale)
+    if dense is not None:
+        k_out, v_out = (scratch(f"attn4.{x}", (s * width, hkv, page_size, d), q.dtype) for x in "kv")
+        table_out = scratch("attn4.table", (s, width), torch.int32)
+        check(fn("pb_expand_pages_4bit")(kind, _p(k_pool), _p(k_steps), _p(v_pool), _p(v_steps), _p(block_table), _p(kv_len), _p(k_out), _p(v_out), _p(table_out), s, width,
+                                         hkv, d, page_size, n_pages, _p(cu_q), window, stream()), name)
+        run, tiles = (paged_attention_prefill_tcgen05, prefill_tcgen05_tiles) if dense == "tcgen05" else (paged_attention_prefill_tc, prefill_tc_tiles)
+        run(q, k_out, v_out, out, table_out, cu_q, kv_len, tiles(q_lens), scale, window)
+        return
+    parts, part_keys = cut_4bit(s, most_tokens, hq, hkv, width * page_size, window, q.dtype)
+    sums = scratch("attn4.sums", (n * hq * parts * (d + 2),), torch.float32) if parts > 1 else None
+    check(fn("pb_paged_attention_4bit")(kind, _p(q), _p(k_pool), _p(k_steps), _p(v_pool), _p(v_steps), _p(out), _p(sums), _p(block_table), width, _p(kv_len), _p(cu_q), n,
+                                        most_tokens, s, hq, hkv, d, page_size, n_pages, float(scale), window, parts, part_keys, stream()), name, kernels=1 if parts == 1 else 2)
