@@ -4,15 +4,20 @@
 namespace pb {
 
 int attend_4bit_bf16(const Attend4& a, int groups, int rows, int most_tokens, cudaStream_t stream) {
-    return rows == 8 ? launch_attend_4bit_of<__nv_bfloat16, 1>(a, groups, most_tokens, stream) : launch_attend_4bit_of<__nv_bfloat16, 2>(a, groups, most_tokens, stream);
+    return launch_attend_4bit_of<__nv_bfloat16>(a, groups, rows, most_tokens, stream);
 }
 
 }  // namespace pb
 
 using namespace pb;
 
-// Rows (query heads of a kv head, times tokens) that a block takes: 16 where there are more than 8.
-PB_EXPORT int pb_attention_4bit_rows(int dtype, int rows) { return dtype == PB_BF16 && rows > 8 ? 16 : 8; }
+// Rows that a block takes where a kv head has so many (its query heads times a sequence's tokens): 16 where there are more than 8, 4 and 2 where
+// there are no more and the head's groups of 32 channels can be dealt out to as many copies of them.
+PB_EXPORT int pb_attention_4bit_rows(int dtype, int rows, int D) {
+    if (rows > 8) return dtype == PB_BF16 ? 16 : 8;
+    if (rows <= 2 && D % (4 * kGroup4) == 0) return 2;
+    return rows <= 4 && D % (2 * kGroup4) == 0 ? 4 : 8;
+}
 
 // sums: float32 [n_rows, Hq, parts, D + 2] where there is more than one part; most_tokens: the most that a sequence brings.
 PB_EXPORT int pb_paged_attention_4bit(int dtype, const void* q, void* k_codes, void* k_steps, void* v_codes, void* v_steps, void* out, float* sums, const int* table,
@@ -23,7 +28,7 @@ PB_EXPORT int pb_paged_attention_4bit(int dtype, const void* q, void* k_codes, v
         return PB_ERR_BAD_SIZE;
     if (dtype != PB_F32 && dtype != PB_BF16) return PB_ERR_BAD_DTYPE;
     if (most_tokens == 0 || n_seqs == 0) return 0;
-    const int group = Hq / Hkv, rows = pb_attention_4bit_rows(dtype, most_tokens * group);
+    const int group = Hq / Hkv, rows = pb_attention_4bit_rows(dtype, most_tokens * group, D);
     const long long row_blocks = ((long long)most_tokens * group + rows - 1) / rows;
     if (row_blocks * Hkv > 65535 || n_seqs > 65535 || (long long)most_tokens * Hq > 0x3fffffff || (long long)n_pages * Hkv * page_size >= 0xffffffffLL ||
         (long long)width * page_size > 0x7ffffff0LL)

@@ -4,7 +4,7 @@
 namespace pb {
 
 int attend_4bit_f32(const Attend4& a, int groups, int rows, int most_tokens, cudaStream_t stream) {
-    return rows == 8 ? launch_attend_4bit_of<float, 1>(a, groups, most_tokens, stream) : PB_ERR_BAD_SIZE;
+    return launch_attend_4bit_of<float>(a, groups, rows, most_tokens, stream);
 }
 
 }  // namespace pb
