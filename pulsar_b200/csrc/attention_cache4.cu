@@ -11,29 +11,52 @@ int attend_4bit_bf16(const Attend4& a, int groups, int rows, int most_tokens, cu
 
 using namespace pb;
 
-// Rows that a block takes where a kv head has so many (its query heads times a sequence's tokens): 16 where there are more than 8, 4 and 2 where
-// there are no more and the head's groups of 32 channels can be dealt out to as many copies of them.
+// Rows that a block takes where a kv head has so many (its query heads times a sequence's tokens): 16 of bfloat16 heads of up to 128 where there are
+// more than 8, for which registers suffice, 4 and 2 where there are no more and the head's groups of 32 channels can be dealt out to copies of them.
 PB_EXPORT int pb_attention_4bit_rows(int dtype, int rows, int D) {
-    if (rows > 8) return dtype == PB_BF16 ? 16 : 8;
+    if (rows > 8) return dtype == PB_BF16 && D <= 4 * kGroup4 ? 16 : 8;
     if (rows <= 2 && D % (4 * kGroup4) == 0) return 2;
     return rows <= 4 && D % (2 * kGroup4) == 0 ? 4 : 8;
 }
 
-// sums: float32 [n_rows, Hq, parts, D + 2] where there is more than one part; most_tokens: the most that a sequence brings.
-PB_EXPORT int pb_paged_attention_4bit(int dtype, const void* q, void* k_codes, void* k_steps, void* v_codes, void* v_steps, void* out, float* sums, const int* table,
-                                      int width, const int* kv_len, const int* cu_q, int n_rows, int most_tokens, int n_seqs, int Hq, int Hkv, int D, int page_size, int n_pages,
-                                      float scale, int window, int parts, int part_keys, cudaStream_t stream) {
-    if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || D <= 0 || D > 256 || D % kGroup4 || page_size <= 0 || n_pages <= 0 || width <= 0 || window < 0 || parts <= 0 || part_keys <= 0 ||
-        part_keys % kTile4 || (parts > 1 && sums == nullptr) || most_tokens < 0 || n_seqs < 0 || n_rows < 0)
+namespace {
+int sm_count_4bit() {
+    static DeviceCount count;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+    const int n = count.get(dev, [dev](int* v) { return (int)cudaDeviceGetAttribute(v, cudaDevAttrMultiProcessorCount, dev); });
+    return n > 0 ? n : 148;
+}
+}  // namespace
+
+// Blocks that a call is dealt out to: as many as the SMs hold at once, or as many as the longest sequences that the tables could name would fill.
+PB_EXPORT int pb_attention_4bit_blocks(int dtype, int most_tokens, int n_seqs, int Hq, int Hkv, int D, int width, int page_size, int window) {
+    if (Hkv <= 0 || Hq <= 0 || D <= 0 || most_tokens <= 0 || n_seqs <= 0 || width <= 0 || page_size <= 0) return 1;
+    const int rows = pb_attention_4bit_rows(dtype, most_tokens * (Hq / Hkv), D);
+    const long long row_blocks = ((long long)most_tokens * (Hq / Hkv) + rows - 1) / rows;
+    long long keys = (long long)width * page_size;
+    if (window > 0 && keys > (long long)window + most_tokens + 16) keys = (long long)window + most_tokens + 16;
+    const long long turns = n_seqs * row_blocks * Hkv * ((keys + kTile4 - 1) / kTile4), wanted = (turns + kLeastTurns4 - 1) / kLeastTurns4;
+    const int most = sm_count_4bit() * blocks_4bit(dtype == PB_F32, D / kGroup4, rows);
+    return wanted < most ? (int)wanted : most;
+}
+
+// sums: float32 [blocks, 2, rows, D + 2], rows of attention_4bit_rows; plan: int32 [2 + n_seqs * blocks of rows of most_tokens]; most_tokens: the most
+// that a sequence brings.
+PB_EXPORT int pb_paged_attention_4bit(int dtype, const void* q, void* k_codes, void* k_steps, void* v_codes, void* v_steps, void* out, float* sums, int* plan,
+                                      const int* table, int width, const int* kv_len, const int* cu_q, int n_rows, int most_tokens, int n_seqs, int Hq, int Hkv, int D,
+                                      int page_size, int n_pages, float scale, int window, int blocks, cudaStream_t stream) {
+    if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || D <= 0 || D > 256 || D % kGroup4 || page_size <= 0 || n_pages <= 0 || width <= 0 || window < 0 || blocks <= 0 ||
+        sums == nullptr || plan == nullptr || most_tokens < 0 || n_seqs < 0 || n_rows < 0)
         return PB_ERR_BAD_SIZE;
     if (dtype != PB_F32 && dtype != PB_BF16) return PB_ERR_BAD_DTYPE;
     if (most_tokens == 0 || n_seqs == 0) return 0;
     const int group = Hq / Hkv, rows = pb_attention_4bit_rows(dtype, most_tokens * group, D);
-    const long long row_blocks = ((long long)most_tokens * group + rows - 1) / rows;
-    if (row_blocks * Hkv > 65535 || n_seqs > 65535 || (long long)most_tokens * Hq > 0x3fffffff || (long long)n_pages * Hkv * page_size >= 0xffffffffLL ||
-        (long long)width * page_size > 0x7ffffff0LL)
+    const long long row_blocks = ((long long)most_tokens * group + rows - 1) / rows, keys = (long long)width * page_size;
+    if (n_seqs > 65535 || (long long)most_tokens * Hq > 0x3fffffff || (long long)n_pages * Hkv * page_size >= 0xffffffffLL || keys > 0x7ffffff0LL ||
+        (double)n_seqs * row_blocks * Hkv * (keys / kTile4 + 1) > 2.0e9)
         return PB_ERR_TOO_LARGE;
-    Attend4 a{q, out, {(uint8_t*)k_codes, (__nv_bfloat16*)k_steps}, {(uint8_t*)v_codes, (__nv_bfloat16*)v_steps}, sums, table, kv_len, cu_q, width, n_rows, n_seqs, Hq, Hkv,
-              page_size, log2_exact(page_size), n_pages, parts, part_keys, (int)row_blocks, window, scale * kLog2e, pool_bounds_now()};
+    Attend4 a{q, out, {(uint8_t*)k_codes, (__nv_bfloat16*)k_steps}, {(uint8_t*)v_codes, (__nv_bfloat16*)v_steps}, sums, plan, table, kv_len, cu_q, width, n_rows, n_seqs,
+              Hq, Hkv, page_size, log2_exact(page_size), n_pages, (int)row_blocks, blocks, window, scale * kLog2e, pool_bounds_now()};
     return (dtype == PB_F32 ? attend_4bit_f32 : attend_4bit_bf16)(a, D / kGroup4, rows, most_tokens, stream);
 }

@@ -9,11 +9,11 @@
 //
 //   q.k_j = sum_g s_jg (sum_{i in g} q_i c_ji) + m_jg (sum_{i in g} q_i)          v: sum_j (p_j s'_jg) c'_ji + sum_j p_j m'_jg
 //
-// A code becomes an operand by one logical instruction for two of them: 128 + c is the bits 0x4300 | c in bfloat16, 1,024 + c is 0x6400 | c in
-// float16 and 1,024 + 16 c is 0x6400 | c << 4, which spares a shift: keys are taken in float16, with q scaled to it by a power of two a row.
-// Values stay in bfloat16, whose range a weight times a step needs.  A block takes one sequence, kv head,
-// up to 8 NT rows (query heads of the kv head, tokens) and a part of the keys; its warps take runs of 16 keys in turn, each through a
-// ring of its own in shared memory, so that nobody waits for anybody until the end.  mma.sync m16n8k16 has the keys in its 16 rows for
+// A code becomes an operand by one logical instruction for two of them.  Keys are taken in float16, where the bits of c alone are c 2^-24 and
+// those of c << 4 are c 2^-20 (the products take subnormal numbers as they are), with q scaled to float16 by a power of two a row.  Values are taken in
+// bfloat16, whose range a weight times a step needs: 128 + c is the bits 0x4300 | c.  A block takes one sequence, kv head,
+// up to 8 NT rows (query heads of the kv head, tokens) and a part of the keys; its warps take runs of 32 keys in turn, each through
+// buffers of its own in shared memory, so that nobody waits for anybody until the end.  mma.sync m16n8k16 has the keys in its 16 rows for
 // the scores and the channels for the weighted sum, and the rows of the block in its 8 columns, where rows in its 16 would be mostly empty.
 // A block of 4 rows (2) stands in the columns twice (four times): the products of half (a quarter) of the groups go to each copy, so that no lane
 // computes for an empty column what belongs to a key and column: offsets, steps and least values, weights.  The weights change places
@@ -29,36 +29,64 @@
 
 namespace pb {
 
-constexpr int kTile4 = 16;              // keys of a warp's turn
+constexpr int kTile4 = 32;              // keys of a warp's turn: two halves of 16
 constexpr int kWarps4 = 4;
-constexpr int kStages4 = 4;             // turns in a warp's ring
-constexpr uint32_t kNoRow = 0xffffffffu;
 constexpr float kLowest4 = -3.0e38f;    // a running maximum before the first key
 
 struct Attend4 {
     const void* q;
     void* out;
     Pool4 k, v;
-    float* sums;                        // [rows of q, Hq, parts, D] and behind it [.., 2] (maximum, sum of weights); with more than one part
+    float* sums;                        // [blocks, 2, rows of a block, D] weighted sums, behind them [.., 2] maxima and sums of weights
+    int* plan;                          // turns of a block, then where the turns of every entry begin
     const int* table;
     const int* kv_len;
     const int* cu_q;                    // null: one token each
-    int width, n_rows, n_seqs, Hq, Hkv, page_size, page_shift, n_pages, parts, part_keys, row_blocks, window;
+    int width, n_rows, n_seqs, Hq, Hkv, page_size, page_shift, n_pages, row_blocks, blocks, window;
     float scale_log2;
     PoolBounds bounds;
 };
 
-// The keys [first, last] that any of the block's rows sees, and where the part lies in them.
-struct Span4 {
-    int first, last;
-    __device__ __forceinline__ Span4(const Attend4& a, int kv_len, int n_tokens, int token0, int token1) {
+// The work is dealt out in turns of 32 keys.  An entry is a sequence and as many of its rows (tokens times the query heads of a kv head) as a block
+// takes; the turns of all entries, kv head by kv head, stand in one line, and every block takes the same number of them, one run
+// of the line.  So nobody is left with a long sequence when the others are done, whatever the lengths are, and a block has at most one head that
+// another one began and one that another one ends.  What the lengths are is read here, on the device: a captured call serves any.
+struct Entry4 {
+    int seq, first_token, n_tokens, kv_len, row0, token0, token1;
+    int first, last, turns;             // the keys [first, last] that any of its rows sees; turns begin at first rounded down
+
+    __device__ __forceinline__ Entry4(const Attend4& a, int entry, int rows) {
+        const int group = a.Hq / a.Hkv;
+        seq = entry / a.row_blocks;
+        row0 = (entry - seq * a.row_blocks) * rows;
+        first_token = a.cu_q ? a.cu_q[seq] : seq;
+        n_tokens = a.cu_q ? a.cu_q[seq + 1] - first_token : 1;
+        kv_len = a.kv_len[seq];
+        token0 = row0 / group;
+        token1 = min(n_tokens - 1, (row0 + rows - 1) / group);
         last = min(kv_len - n_tokens + token1, a.width * a.page_size - 1);
         const int low = kv_len - n_tokens + token0 - a.window + 1;
         first = a.window > 0 && low > 0 ? low : 0;
+        turns = row0 < n_tokens * group && last >= first ? (last - start()) / kTile4 + 1 : 0;
     }
-    __device__ __forceinline__ int start() const { return first & ~(kTile4 - 1); }
-    __device__ __forceinline__ int parts(const Attend4& a) const { return last < first ? 0 : min(a.parts, (last - start()) / a.part_keys + 1); }
+    __device__ __forceinline__ int start() const { return first & ~15; }
+    // Where row `local` of the entry stands in q and out, as token * Hq + head; -1 behind the last.
+    __device__ __forceinline__ long row_at(const Attend4& a, int kvh, int local) const {
+        const int group = a.Hq / a.Hkv, row = row0 + local, token = row / group;
+        return token < n_tokens && first_token + token < a.n_rows ? (long)(first_token + token) * a.Hq + kvh * group + (row - token * group) : -1;
+    }
 };
+
+// Blocks of an SM, by what registers allow: of float32 or not, with so many groups and rows of a block.
+constexpr int blocks_4bit(bool exact, int groups, int rows) {
+    return groups * (rows > 8 ? 2 : 1) >= 6 ? 2 : exact || groups * (rows > 8 ? 2 : 1) > 2 ? 3 : 4;
+}
+// Turns of a block where there are so many altogether: no fewer than 8, below which a block's start and end cost more than its turns.
+constexpr int kLeastTurns4 = 8;
+__host__ __device__ inline int turns_of_block(int all, int blocks) {
+    const int n = (all + blocks - 1) / blocks;
+    return n < kLeastTurns4 ? kLeastTurns4 : (n + kWarps4 - 1) / kWarps4 * kWarps4;
+}
 
 __device__ __forceinline__ float exp2_fast(float v) {
     float r;
@@ -80,6 +108,12 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The same from zero.
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 // (word & MASK) | bits in one instruction: `bits` in a register, of two immediate operands the compiler makes two instructions.
 template <uint32_t MASK> __device__ __forceinline__ uint32_t masked_or(uint32_t word, uint32_t bits) {
     uint32_t r;
@@ -89,15 +123,6 @@ template <uint32_t MASK> __device__ __forceinline__ uint32_t masked_or(uint32_t 
 // (128 + c) - 136 = c - 8, exactly.
 __device__ __forceinline__ uint32_t centred(uint32_t raw) {
     const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&raw), __floats2bfloat162_rn(136.0f, 136.0f));
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-// The same of float16's 1,024 + c and 1,024 + 16 c.
-__device__ __forceinline__ uint32_t centred_low(uint32_t raw) {
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&raw), __floats2half2_rn(1032.0f, 1032.0f));
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ uint32_t centred_high(uint32_t raw) {
-    const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&raw), __floats2half2_rn(0.0625f, 0.0625f), __floats2half2_rn(-72.0f, -72.0f));
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
@@ -127,15 +152,21 @@ struct Attend4Block {
     static constexpr int GH = G / COPIES;                   // groups of a copy: copy h has h GH ..
     static constexpr bool kExact = sizeof(T) == 4;          // float32: operands of the products in three bfloat16 terms, codes about zero
     static constexpr int kTerms = kExact ? 3 : 1;
+    // Values keep the offset of their codes, and 136 times the sum of the weights goes through the same products to be taken off at the end: what that
+    // loses of float32 sums 16 times as large as the result is bounded by the length of a part.  Where there are copies, whose weights share a product.
+    static constexpr bool kOffsets = !kExact && COPIES > 1;
     static constexpr int kRow = 16 * G;                     // bytes of a row of codes
-    static constexpr int kKeySteps = kTile4 * kRow, kValues = kKeySteps + kTile4 * 4 * G, kValueSteps = kValues + kTile4 * kRow;
-    static constexpr int kSeen = kValueSteps + kTile4 * 4 * G, kStage = kSeen + 16;
-    static constexpr int kRing = kStages4 * kStage;
+    static constexpr int kBuffers = G <= 4 ? 3 : 2;         // a warp's buffers
+    static constexpr int kHalfStep = 64 * G, kHalf = 256 * G;            // bytes of 16 keys' steps and codes
+    static constexpr int kKeySteps = 2 * kHalf, kValues = kKeySteps + 2 * kHalfStep, kValueSteps = kValues + 2 * kHalf;
+    static constexpr int kStage = kValueSteps + 2 * kHalfStep, kRing = kBuffers * kStage;
     static constexpr int kMerge = (kRows * (D + 2) * 4 + 15) / 16 * 16;
     static constexpr int kPerWarp = kRing > kMerge ? kRing : kMerge;
-    static constexpr int kShared = kWarps4 * kPerWarp;
+    static constexpr int kQ = kWarps4 * kPerWarp;           // q as the second operand: [term][n][g][lane] of 16 bytes
+    static constexpr int kQSums = kTerms * NT * G * 512;    // behind it: [n][g][column] sum, [n][column] factor
+    static constexpr int kQLog2 = kQSums + NT * GH * 32, kShared = kQ + kQLog2 + NT * 32;
 
-    // Row k of 16 keys as the products number them stands in row placed(k) of a stage, and 16-byte chunk c of it at c ^ turned(row): the lanes of
+    // Row k of 16 keys as the products number them stands in row placed(k) of their half of a buffer, and 16-byte chunk c of it at c ^ turned(row): the lanes of
     // either product then read different banks (heads of 128 and 256; the others have some conflicts).
     static __device__ __forceinline__ int placed(int k) { return k ^ ((k >> 1) & 1); }
     static __device__ __forceinline__ int turned(int row) { return G == 4 ? (row >> 1) & 2 : G == 8 ? row & 6 : 0; }
@@ -173,142 +204,158 @@ struct Attend4Block {
     }
 
     // State of a warp.  Lane (r, t) = (lane / 4, lane % 4) holds columns 2 t and 2 t + 1 of 8 for each of NT; they belong to copy t COPIES / 4.
-    uint32_t qb[kTerms][NT][G][2][2];       // q as the second operand: column r, channels 32 g + 8 t + ..
-    float q_sum[NT][GH][2];                 // sum of a column's q over a group of its copy
-    float q_offset[NT][GH][2];              // what the offsets of the codes add to a column's products
+    float q_sum[NT][GH][2];                 // sum of a column's q over a group of its copy, times 2^-24
     float to_log2[NT][2];                   // from a column's sums of products to scores in base 2
-    uint32_t f16_bits, bf16_bits;
+    uint32_t bf16_bits;
     float o[NT][G][2][4];                   // [u]: channels 32 g + 4 r + 2 u, + 1 (elements 0 1, 2 3) of columns 2 t, 2 t + 1; of the columns' copies that have g
     float least_sum[NT][GH][2];             // this lane's part of sum_j p_j (m_j + 8 s_j)
+    float offsets[kOffsets ? GH : 1][4];    // 136 times the sums of the weights of a group of its copy
     float top[NT][2], total[NT][2];
     int pos[NT][2];                         // a column's position
 
-    __device__ __forceinline__ void load_q(const T* const (&src)[NT], float scale_log2, int lane) {
-        asm volatile("mov.b32 %0, 0x64006400;" : "=r"(f16_bits));
-        asm volatile("mov.b32 %0, 0x43004300;" : "=r"(bf16_bits));
-        const int t = lane & 3, copy = (lane >> 2) / kColumns;             // of column r
+    // The block's q, raw: a lane's channels 8 t .. + 7 of column r in every group of its copy.
+    struct RawQ { float v[NT][GH][8]; };
+    static __device__ __forceinline__ void read_q(const T* const (&src)[NT], RawQ& raw, int lane) {
+        const int t = lane & 3, copy = (lane >> 2) / kColumns;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float v[GH][8], most = 0.0f;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int g = 0; g < GH; ++g) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[g][e] = 0.0f;
+                for (int e = 0; e < 8; ++e) raw.v[n][g][e] = 0.0f;
                 if (src[n] != nullptr) {
-                    load_quad(src[n] + 32 * (copy * GH + g) + 8 * t, *reinterpret_cast<float(*)[4]>(v[g]));
-                    load_quad(src[n] + 32 * (copy * GH + g) + 8 * t + 4, *reinterpret_cast<float(*)[4]>(v[g] + 4));
+                    load_quad(src[n] + 32 * (copy * GH + g) + 8 * t, *reinterpret_cast<float(*)[4]>(raw.v[n][g]));
+                    load_quad(src[n] + 32 * (copy * GH + g) + 8 * t + 4, *reinterpret_cast<float(*)[4]>(raw.v[n][g] + 4));
                 }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[g][e]));
             }
+    }
+    // q as an operand to shared memory, with its sums; the warps share the groups.
+    static __device__ __forceinline__ void write_q(RawQ& raw, float scale_log2, uint32_t q_at, int warp, int lane) {
+        const int r = lane >> 2, t = lane & 3, copy = r / kColumns;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float most = 0.0f;
+#pragma unroll
+            for (int g = 0; g < GH; ++g)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(raw.v[n][g][e]));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
             if (COPIES == 4) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
             if (COPIES >= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
-            // the row over 2^k, its largest element in [1, 2); float16 then rounds what is below 2^-14 to 2^-25 of that
-            const int k = most > 0.0f ? min(126, max(-126, ilogbf(most))) : 0;
-            const float down = __int_as_float((127 - k) << 23), up = __int_as_float((127 + k) << 23) * scale_log2;
-            to_log2[n][0] = __shfl_sync(0xffffffffu, up, 8 * t);
-            to_log2[n][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
+            // the row over 2^k, its largest element in [2^14, 2^15): float16 holds 11 bits of all that is above 2^-28 of it
+            const int k = min(126, max(-112, (int)(__float_as_uint(most) >> 23) - 127)) - 14;
+            const float down = __int_as_float((127 - k) << 23);
+            if (warp == 0 && t == 0)
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(q_at + kQLog2 + (n * 8 + r) * 4), "f"(__int_as_float((127 + k) << 23) * 0x1p24f * scale_log2) : "memory");
 #pragma unroll
             for (int g = 0; g < GH; ++g) {
-                float sum = 0.0f, offset = 0.0f;
+                if (g % kWarps4 != warp && GH >= kWarps4) continue;
+                if (GH < kWarps4 && g != warp % GH) continue;
+                float sum = 0.0f, (&v)[8] = raw.v[n][g];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    v[g][e] *= down;
-                    sum += v[g][e];
-                }
+                for (int e = 0; e < 8; ++e) v[e] *= down;
                 // words: pairs of channels (e, 4 + e); those of odd e stand 16 times as high in the codes
-                constexpr float kHigh = kExact ? 1.0f : 0.0625f;
 #pragma unroll
-                for (int term = 0; term < kTerms; ++term)
+                for (int term = 0; term < kTerms; ++term) {
+                    uint32_t words[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float lo = __half2float(__float2half_rn(v[g][e])), hi = __half2float(__float2half_rn(v[g][4 + e])), by = e % 2 ? kHigh : 1.0f;
-                        const uint32_t both = pack_f16(lo * by, hi * by);
-#pragma unroll
-                        for (int h = 0; h < COPIES; ++h) qb[term][n][h * GH + g][e >> 1][e & 1] = copy == h ? both : 0u;
-                        if constexpr (kExact) {
-                            v[g][e] -= lo;
-                            v[g][4 + e] -= hi;
-                        } else {
-                            const float2 held = __half22float2(*reinterpret_cast<const __half2*>(&both));
-                            offset += 1024.0f * (held.x + held.y);
-                        }
+                        const float by = e % 2 ? 0.0625f : 1.0f, back = e % 2 ? 16.0f : 1.0f;
+                        words[e] = pack_f16(v[e] * by, v[4 + e] * by);
+                        const float2 held = __half22float2(*reinterpret_cast<const __half2*>(&words[e]));
+                        v[e] -= held.x * back;
+                        v[4 + e] -= held.y * back;
+                        sum += (held.x + held.y) * back;
                     }
+#pragma unroll
+                    for (int h = 0; h < COPIES; ++h)
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(q_at + ((term * NT + n) * G + h * GH + g) * 512 + lane * 16),
+                                     "r"(copy == h ? words[0] : 0u), "r"(copy == h ? words[1] : 0u), "r"(copy == h ? words[2] : 0u), "r"(copy == h ? words[3] : 0u) : "memory");
+                }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                offset += __shfl_xor_sync(0xffffffffu, offset, 1);
-                offset += __shfl_xor_sync(0xffffffffu, offset, 2);
-                q_sum[n][g][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
-                q_sum[n][g][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
-                q_offset[n][g][0] = __shfl_sync(0xffffffffu, offset, 8 * t);
-                q_offset[n][g][1] = __shfl_sync(0xffffffffu, offset, 8 * t + 4);
+                if (t == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(q_at + kQSums + ((n * GH + g) * 8 + r) * 4), "f"(sum * 0x1p-24f) : "memory");
             }
         }
     }
+    __device__ __forceinline__ void take_q_sums(uint32_t q_at, int lane) {
+        asm volatile("mov.b32 %0, 0x43004300;" : "=r"(bf16_bits));
+        const int t = lane & 3;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(to_log2[n][0]), "=f"(to_log2[n][1]) : "r"(q_at + kQLog2 + (n * 8 + 2 * t) * 4));
+#pragma unroll
+            for (int g = 0; g < GH; ++g)
+                asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(q_sum[n][g][0]), "=f"(q_sum[n][g][1]) : "r"(q_at + kQSums + ((n * GH + g) * 8 + 2 * t) * 4));
+        }
+    }
 
-    // Sixteen keys.  EDGE: some column does not see some of them.
-    template <bool EDGE>
-    __device__ __forceinline__ void turn(uint32_t stage, int key0, uint32_t seen, int window, int lane) {
+    static __device__ __forceinline__ void load_keys(uint32_t half, int row, int t, uint32_t (&w)[G]) {
+        if constexpr (G == 4) {
+            load_shared<16>(half + row * kRow + ((t ^ turned(row)) * 16), w);
+        } else if constexpr (G == 8) {
+            load_shared<16>(half + row * kRow + (((2 * t) ^ turned(row)) * 16), w);
+            load_shared<16>(half + row * kRow + (((2 * t + 1) ^ turned(row)) * 16), w + 4);
+        } else {
+            load_shared<4 * G>(half + row * kRow + t * 4 * G, w);
+        }
+    }
+
+    // Thirty-two keys.  EDGE: some column does not see some of them.  `sees(key, pos)`: whether one does.
+    template <bool EDGE, typename Sees>
+    __device__ __forceinline__ void turn(uint32_t stage, uint32_t q_at, int key0, int lane, Sees sees) {
         const int r = lane >> 2, t = lane & 3, row0 = placed(r), row1 = row0 + 8, copy = t * COPIES / 4;
-        float x[NT][4];
+        float x[2][NT][4];
         {
-            uint32_t w0[G], w1[G], s0[GH], s1[GH];
-            if constexpr (G == 4) {
-                load_shared<16>(stage + row0 * kRow + ((t ^ turned(row0)) * 16), w0);
-                load_shared<16>(stage + row1 * kRow + ((t ^ turned(row1)) * 16), w1);
-            } else if constexpr (G == 8) {
-                load_shared<16>(stage + row0 * kRow + (((2 * t) ^ turned(row0)) * 16), w0);
-                load_shared<16>(stage + row0 * kRow + (((2 * t + 1) ^ turned(row0)) * 16), w0 + 4);
-                load_shared<16>(stage + row1 * kRow + (((2 * t) ^ turned(row1)) * 16), w1);
-                load_shared<16>(stage + row1 * kRow + (((2 * t + 1) ^ turned(row1)) * 16), w1 + 4);
-            } else {
-                load_shared<4 * G>(stage + row0 * kRow + t * 4 * G, w0);
-                load_shared<4 * G>(stage + row1 * kRow + t * 4 * G, w1);
+            uint32_t w[2][2][G], s[2][2][GH];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                load_keys(stage + half * kHalf, row0, t, w[half][0]);
+                load_keys(stage + half * kHalf, row1, t, w[half][1]);
+                load_shared<4 * GH>(stage + kKeySteps + half * kHalfStep + row0 * 4 * G + copy * 4 * GH, s[half][0]);
+                load_shared<4 * GH>(stage + kKeySteps + half * kHalfStep + row1 * 4 * G + copy * 4 * GH, s[half][1]);
             }
-            load_shared<4 * GH>(stage + kKeySteps + row0 * 4 * G + copy * 4 * GH, s0);
-            load_shared<4 * GH>(stage + kKeySteps + row1 * 4 * G + copy * 4 * GH, s1);
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[n][e] = 0.0f;
 #pragma unroll
             for (int j = 0; j < GH; ++j) {
-                float c[NT][4] = {};
+                float c[2][NT][4];
 #pragma unroll
                 for (int h = 0; h < COPIES; ++h) {
                     const int g = h * GH + j;
-                    const uint32_t y[2] = {key_word(w0, g), key_word(w1, g)};
-                    uint32_t ka[2][4];
+                    uint32_t ka[2][2][4];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                    for (int half = 0; half < 2; ++half) {
+                        const uint32_t y[2] = {key_word(w[half][0], g), key_word(w[half][1], g)};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t word = i ? y[e & 1] >> 8 : y[e & 1];
-                            ka[i][e] = e < 2 ? masked_or<0x000f000fu>(word, f16_bits) : masked_or<0x00f000f0u>(word, f16_bits);
-                            if constexpr (kExact) ka[i][e] = e < 2 ? centred_low(ka[i][e]) : centred_high(ka[i][e]);
-                        }
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) ka[half][i][e] = (i ? y[e & 1] >> 8 : y[e & 1]) & (e < 2 ? 0x000f000fu : 0x00f000f0u);
+                    }
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int term = kTerms - 1; term >= 0; --term) {      // the largest terms last
-                            mma_f16(c[n], ka[0], qb[term][n][g][0][0], qb[term][n][g][0][1]);
-                            mma_f16(c[n], ka[1], qb[term][n][g][1][0], qb[term][n][g][1][1]);
+                            uint32_t b[4];
+                            load_shared<16>(q_at + ((term * NT + n) * G + g) * 512 + lane * 16, b);
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                if (h == 0 && term == kTerms - 1) mma_f16_first(c[half][n], ka[half][0], b[0], b[1]);
+                                else mma_f16(c[half][n], ka[half][0], b[0], b[1]);
+                                mma_f16(c[half][n], ka[half][1], b[2], b[3]);
+                            }
                         }
                 }
-                const float step0 = __uint_as_float(s0[j] << 16), step1 = __uint_as_float(s1[j] << 16);
-                float least0 = __uint_as_float(s0[j] & 0xffff0000u), least1 = __uint_as_float(s1[j] & 0xffff0000u);
-                if constexpr (kExact) {
-                    least0 = fmaf(8.0f, step0, least0);
-                    least1 = fmaf(8.0f, step1, least1);
-                }
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int half = 0; half < 2; ++half)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        if constexpr (!kExact) c[n][e] -= q_offset[n][j][e & 1];
-                        x[n][e] = fmaf(e < 2 ? step0 : step1, c[n][e], fmaf(e < 2 ? least0 : least1, q_sum[n][j][e & 1], x[n][e]));
+                        const uint32_t word = s[half][e >> 1][j];
+                        const float step = __uint_as_float(word << 16), least = __uint_as_float(word & 0xffff0000u);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            const float m = j == 0 ? least * q_sum[n][j][e & 1] : fmaf(least, q_sum[n][j][e & 1], x[half][n][e]);
+                            x[half][n][e] = fmaf(step, c[half][n][e], m);
+                        }
                     }
             }
         }
@@ -316,23 +363,22 @@ struct Attend4Block {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[n][e] = over_copies(x[n][e]) * to_log2[n][e & 1];
-                if constexpr (EDGE) {
-                    const int row = e < 2 ? row0 : row1, p = pos[n][e & 1];
-                    const bool sees = ((seen >> row) & 1) && key0 + row <= p && (window == 0 || key0 + row > p - window);
-                    x[n][e] = sees ? x[n][e] : -INFINITY;
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[half][n][e] = over_copies(x[half][n][e]) * to_log2[n][e & 1];
+                    if constexpr (EDGE) x[half][n][e] = sees(key0 + 16 * half + (e < 2 ? row0 : row1), pos[n][e & 1]) ? x[half][n][e] : -INFINITY;
                 }
-            }
             // The maximum moves only when a score passes it by more than 2^8: weights stay below 2^8, float32 and bfloat16 have room for them.
-            rises |= fmaxf(x[n][0], x[n][2]) > top[n][0] + 8.0f || fmaxf(x[n][1], x[n][3]) > top[n][1] + 8.0f;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) rises |= fmaxf(fmaxf(x[0][n][c], x[0][n][c + 2]), fmaxf(x[1][n][c], x[1][n][c + 2])) > top[n][c] + 8.0f;
         }
         if (__any_sync(0xffffffffu, rises)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    float m = fmaxf(x[n][c], x[n][c + 2]);
+                    float m = fmaxf(fmaxf(x[0][n][c], x[0][n][c + 2]), fmaxf(x[1][n][c], x[1][n][c + 2]));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
@@ -341,7 +387,13 @@ struct Attend4Block {
                     top[n][c] = m;
                     total[n][c] *= shrink;
 #pragma unroll
-                    for (int g = 0; g < GH; ++g) least_sum[n][g][c] *= shrink;
+                    for (int g = 0; g < GH; ++g) {
+                        least_sum[n][g][c] *= shrink;
+                        if constexpr (kOffsets) {
+                            offsets[g][c] *= shrink;
+                            offsets[g][c + 2] *= shrink;
+                        }
+                    }
 #pragma unroll
                     for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -354,171 +406,235 @@ struct Attend4Block {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[n][e] = exp2_fast(x[n][e] - top[n][e & 1]);
-            total[n][0] += x[n][0] + x[n][2];
-            total[n][1] += x[n][1] + x[n][3];
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[half][n][e] = exp2_fast(x[half][n][e] - top[n][e & 1]);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) total[n][c] += (x[0][n][c] + x[0][n][c + 2]) + (x[1][n][c] + x[1][n][c + 2]);
         }
-        uint32_t s0[GH], s1[GH], va[G], vb[G], vc[G], vd[G];
-        load_shared<4 * GH>(stage + kValueSteps + row0 * 4 * G + copy * 4 * GH, s0);
-        load_shared<4 * GH>(stage + kValueSteps + row1 * 4 * G + copy * 4 * GH, s1);
-        load_values(stage + kValues, placed(2 * t), r, va);
-        load_values(stage + kValues, placed(2 * t + 1), r, vb);
-        load_values(stage + kValues, placed(2 * t) + 8, r, vc);
-        load_values(stage + kValues, placed(2 * t + 1) + 8, r, vd);
 #pragma unroll
-        for (int j = 0; j < GH; ++j) {
-            const float step0 = __uint_as_float(s0[j] << 16), step1 = __uint_as_float(s1[j] << 16);
-            const float middle0 = fmaf(8.0f, step0, __uint_as_float(s0[j] & 0xffff0000u)), middle1 = fmaf(8.0f, step1, __uint_as_float(s1[j] & 0xffff0000u));
-            uint32_t b0[NT][kTerms], b1[NT][kTerms];
+        for (int half = 0; half < 2; ++half) {
+            uint32_t s[2][GH], va[G], vb[G], vc[G], vd[G];
+            const uint32_t values = stage + kValues + half * kHalf, steps = stage + kValueSteps + half * kHalfStep + copy * 4 * GH;
+            load_shared<4 * GH>(steps + row0 * 4 * G, s[0]);
+            load_shared<4 * GH>(steps + row1 * 4 * G, s[1]);
+            load_values(values, placed(2 * t), r, va);
+            load_values(values, placed(2 * t + 1), r, vb);
+            load_values(values, placed(2 * t) + 8, r, vc);
+            load_values(values, placed(2 * t + 1) + 8, r, vd);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float w[4];
-                // EDGE: a weight of zero is nothing, whatever the value it belongs to
+            for (int j = 0; j < GH; ++j) {
+                float step[2], middle[2];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    w[e] = x[n][e] * (e < 2 ? step0 : step1);
-                    if (EDGE && x[n][e] == 0.0f) w[e] = 0.0f;
-                    else least_sum[n][j][e & 1] = fmaf(x[n][e], e < 2 ? middle0 : middle1, least_sum[n][j][e & 1]);
+                for (int i = 0; i < 2; ++i) {
+                    step[i] = __uint_as_float(s[i][j] << 16);
+                    middle[i] = fmaf(8.0f, step[i], __uint_as_float(s[i][j] & 0xffff0000u));
                 }
+                uint32_t b0[NT][kTerms], b1[NT][kTerms];
 #pragma unroll
-                for (int term = 0; term < kTerms; ++term) {
-                    b0[n][term] = transposed_8x8(pack_bf16(w[0], w[1]));
-                    b1[n][term] = transposed_8x8(pack_bf16(w[2], w[3]));
-                    if constexpr (kExact)
+                for (int n = 0; n < NT; ++n) {
+                    float w[4];
+                    // EDGE: a weight of zero is nothing, whatever the value it belongs to
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] -= __bfloat162float(__float2bfloat16_rn(w[e]));
-                }
-            }
-#pragma unroll
-            for (int h = 0; h < COPIES; ++h) {
-                const int g = h * GH + j;
-                const uint32_t z0 = value_word(va, vb, g), z1 = value_word(vc, vd, g);
-                uint32_t a0[4], a1[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t z = e < 2 ? z0 : z1;
-                    a0[e] = centred(masked_or<0x000f000fu>(e % 2 ? z >> 4 : z, bf16_bits));
-                    a1[e] = centred(masked_or<0x000f000fu>(e % 2 ? z >> 12 : z >> 8, bf16_bits));
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int term = kTerms - 1; term >= 0; --term) {
-                        mma_bf16(o[n][g][0], a0, b0[n][term], b1[n][term]);
-                        mma_bf16(o[n][g][1], a1, b0[n][term], b1[n][term]);
+                    for (int e = 0; e < 4; ++e) {
+                        const float p = x[half][n][e];
+                        w[e] = p * step[e >> 1];
+                        if (EDGE && p == 0.0f) w[e] = 0.0f;
+                        else least_sum[n][j][e & 1] = fmaf(p, middle[e >> 1], least_sum[n][j][e & 1]);
                     }
+#pragma unroll
+                    for (int term = 0; term < kTerms; ++term) {
+                        b0[n][term] = transposed_8x8(pack_bf16(w[0], w[1]));
+                        b1[n][term] = transposed_8x8(pack_bf16(w[2], w[3]));
+                        if constexpr (kExact)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) w[e] -= __bfloat162float(__float2bfloat16_rn(w[e]));
+                    }
+                }
+                if constexpr (kOffsets) {
+                    const uint32_t a[4] = {0x43084308u, 0x43084308u, 0x43084308u, 0x43084308u};
+                    mma_bf16(offsets[j], a, b0[0][0], b1[0][0]);
+                }
+#pragma unroll
+                for (int h = 0; h < COPIES; ++h) {
+                    const int g = h * GH + j;
+                    const uint32_t z[2] = {value_word(va, vb, g), value_word(vc, vd, g)};
+                    uint32_t a[2][4];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            a[u][e] = masked_or<0x000f000fu>(z[e >> 1] >> (8 * u + 4 * (e & 1)), bf16_bits);
+                            if constexpr (!kOffsets) a[u][e] = centred(a[u][e]);
+                        }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int term = kTerms - 1; term >= 0; --term)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) mma_bf16(o[n][g][u], a[u], b0[n][term], b1[n][term]);
+                }
             }
         }
     }
 };
 
-// Which rows of the pools a warp's turns are, and their copies into its ring.  Turn i of a warp is the keys key0 + i * kWarps4 * kTile4 .. + 15.
-// Pages of whole turns: every turn is one run of rows.
+// Which rows of the pools a warp's turns are, and their copies into its buffers.  Turn i of a warp is the keys key0 + i * kWarps4 * kTile4 .. + 31.
+// A key that has no page takes row 0 instead, so that no copy depends on anything; `holes` then says that keys have to be looked at one by one.
+struct Head4 {
+    const int* table;
+    int kvh, key0, own, first, last;    // of a warp: its first key and its turns; the first and last key that are seen at all
+};
+__device__ __forceinline__ int page_of(const Attend4& a, const Head4& head, int key, int& place) {
+    const int logical = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+    place = key - logical * a.page_size;
+    const int page = head.table[logical];
+    page_ok(page, a.bounds);
+    return page_or_none(page, a.n_pages);
+}
+
+// Pages of whole halves of 16 keys: every half is one run of rows.  A lane keeps the run (row / 16) of half lane % 2 of turn 16 n + lane / 2.
 template <typename B>
 struct Turns16 {
-    uint32_t units = kNoRow, units_next = kNoRow;         // of turns (32 n + lane) and the 32 behind them: row / 16
-    uint32_t there = 0;                                   // bit i & 31: turn i has a page
+    uint32_t units, units_next;
+    bool holes = false;
+    const uint8_t *k, *v, *steps;       // a lane's first chunk of 16 bytes: of codes, and of the steps of one of the pools
+    uint32_t code_to, step_to;          // where they go in a buffer
 
-    __device__ __forceinline__ uint32_t unit_of(const Attend4& a, const int* table, int kvh, int key) const {
-        int logical, place;
-        if (a.page_shift >= 0) {
-            logical = key >> a.page_shift;
-            place = key & (a.page_size - 1);
-        } else {
-            logical = key / a.page_size;
-            place = key - logical * a.page_size;
-        }
-        const int page = table[logical];
-        page_ok(page, a.bounds);
-        return page_or_none(page, a.n_pages) < 0 ? kNoRow : (((uint32_t)page * a.Hkv + kvh) * a.page_size + place) / kTile4;
+    __device__ __forceinline__ uint32_t load(const Attend4& a, const Head4& head, int turn, int lane) {
+        const int key = head.key0 + (turn + (lane >> 1)) * (kWarps4 * kTile4) + (lane & 1) * 16;
+        int place, page = 0;
+        if (turn + (lane >> 1) < head.own && key <= head.last) page = page_of(a, head, key, place);
+        else return 0;
+        if (page < 0) holes = true;
+        return page < 0 ? 0 : (((uint32_t)page * a.Hkv + head.kvh) * a.page_size + place) / 16;
     }
-    __device__ __forceinline__ uint32_t load(const Attend4& a, const int* table, int kvh, int key0, int turn, int own) const {
-        return turn < own ? unit_of(a, table, kvh, key0 + turn * (kWarps4 * kTile4)) : kNoRow;
+    __device__ __forceinline__ void begin(const Attend4& a, const Head4& head, int lane) {
+        units_next = load(a, head, 0, lane);
+        k = a.k.codes + lane * 16;
+        v = a.v.codes + lane * 16;
+        steps = reinterpret_cast<const uint8_t*>(lane < 16 ? a.k.steps : a.v.steps) + (lane & 15) * 16;
+        code_to = lane / B::G_ * B::kRow + ((lane % B::G_ ^ B::turned(lane / B::G_)) * 16);
+        step_to = (lane < 16 ? B::kKeySteps : B::kValueSteps) + (lane & 15) * 16;
     }
-    __device__ __forceinline__ void begin(const Attend4& a, const int* table, int kvh, int key0, int own, const Span4&, int lane) {
-        units_next = load(a, table, kvh, key0, lane, own);
-    }
-    // Turn i, in order, into a stage.
-    __device__ __forceinline__ void fill(const Attend4& a, const int* table, int kvh, int key0, int own, const Span4&, int i, uint32_t stage, int lane) {
-        if ((i & 31) == 0) {
+    // Turn i, in order, into a buffer.
+    __device__ __forceinline__ void fill(const Attend4& a, const Head4& head, int i, uint32_t stage, int lane) {
+        if ((i & 15) == 0) {
             units = units_next;
-            units_next = load(a, table, kvh, key0, i + 32 + lane, own);
-        }
-        const uint32_t unit = __shfl_sync(0xffffffffu, units, i & 31);
-        if (unit == kNoRow) {
-            there &= ~(1u << (i & 31));
-            return;
-        }
-        there |= 1u << (i & 31);
-        const uint8_t* k = a.k.codes + (size_t)unit * (kTile4 * B::kRow) + lane * 16;
-        const uint8_t* v = a.v.codes + (size_t)unit * (kTile4 * B::kRow) + lane * 16;
-#pragma unroll
-        for (int it = 0; it < (B::G_ + 1) / 2; ++it) {
-            const int j = it * 32 + lane, key = j / B::G_, c = j - key * B::G_;
-            if (B::G_ % 2 == 0 || j < kTile4 * B::G_) {
-                const uint32_t to = stage + key * B::kRow + ((c ^ B::turned(key)) * 16);
-                cp_async16(to, k + it * 512, true);
-                cp_async16(to + B::kValues, v + it * 512, true);
-            }
+            units_next = load(a, head, i + 16, lane);
+            holes = __any_sync(0xffffffffu, holes);
         }
 #pragma unroll
-        for (int it = 0; it < (8 * B::G_ + 31) / 32; ++it) {
-            const int j = it * 32 + lane;
-            const bool is_v = j >= 4 * B::G_;
-            const int c = is_v ? j - 4 * B::G_ : j;
-            if (8 * B::G_ % 32 == 0 || j < 8 * B::G_) {
-                const uint8_t* steps = reinterpret_cast<const uint8_t*>(is_v ? a.v.steps : a.k.steps) + (size_t)unit * (kTile4 * 4 * B::G_) + c * 16;
-                cp_async16(stage + (is_v ? B::kValueSteps : B::kKeySteps) + c * 16, steps, true);
+        for (int half = 0; half < 2; ++half) {
+            const uint32_t unit = __shfl_sync(0xffffffffu, units, 2 * (i & 15) + half);
+            const uint8_t *kc = k + (size_t)unit * B::kHalf, *vc = v + (size_t)unit * B::kHalf, *st = steps + (size_t)unit * B::kHalfStep;
+            const uint32_t to = stage + half * B::kHalf;
+#pragma unroll
+            for (int it = 0; it < (B::G_ + 1) / 2; ++it) {
+                if constexpr (B::G_ == 4) {             // eight keys an instruction: the second eight stand 512 bytes behind
+                    cp_async16(to + code_to + it * 512, kc + it * 512, true);
+                    cp_async16(to + code_to + B::kValues + it * 512, vc + it * 512, true);
+                } else {
+                    const int j = it * 32 + lane, key = j / B::G_, c = j - key * B::G_;
+                    const uint32_t at = to + key * B::kRow + ((c ^ B::turned(key)) * 16);
+                    if (B::G_ % 2 == 0 || j < 16 * B::G_) {
+                        cp_async16(at, kc + it * 512, true);
+                        cp_async16(at + B::kValues, vc + it * 512, true);
+                    }
+                }
             }
+#pragma unroll
+            for (int it = 0; it < (4 * B::G_ + 15) / 16; ++it)                   // half the warp a pool
+                if (4 * B::G_ % 16 == 0 || it * 16 + (lane & 15) < 4 * B::G_) cp_async16(stage + half * B::kHalfStep + step_to + it * 256, st + it * 256, true);
         }
     }
-    __device__ __forceinline__ uint32_t seen(int i, uint32_t) const { return (there >> (i & 31)) & 1 ? 0xffffu : 0u; }
 };
 
-// Pages of any size: key by key.  `row`: of key (lane & 15) of the next turn.
+// Pages of any size: key by key.  `row`: of key `lane` of the next turn.
 template <typename B>
 struct TurnsAny {
-    uint32_t row = kNoRow;
+    uint32_t row;
+    bool holes = false;
 
-    __device__ __forceinline__ uint32_t row_of(const Attend4& a, const int* table, int kvh, int key, const Span4& span) const {
-        if (key < span.first || key > span.last) return kNoRow;
-        const int logical = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size, page = table[logical];
-        page_ok(page, a.bounds);
-        return page_or_none(page, a.n_pages) < 0 ? kNoRow : ((uint32_t)page * a.Hkv + kvh) * a.page_size + (key - logical * a.page_size);
+    __device__ __forceinline__ uint32_t load(const Attend4& a, const Head4& head, int turn, int lane) {
+        const int key = head.key0 + turn * (kWarps4 * kTile4) + lane;
+        int place, page;
+        if (turn >= head.own || key < head.first || key > head.last) return 0;
+        page = page_of(a, head, key, place);
+        if (page < 0) holes = true;
+        return page < 0 ? 0 : ((uint32_t)page * a.Hkv + head.kvh) * a.page_size + place;
     }
-    __device__ __forceinline__ void begin(const Attend4& a, const int* table, int kvh, int key0, int own, const Span4& span, int lane) {
-        row = own > 0 ? row_of(a, table, kvh, key0 + (lane & 15), span) : kNoRow;
-    }
-    __device__ __forceinline__ void fill(const Attend4& a, const int* table, int kvh, int key0, int own, const Span4& span, int i, uint32_t stage, int lane) {
-        const uint32_t bits = __ballot_sync(0xffffffffu, row != kNoRow) & 0xffffu;
-        if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(stage + B::kSeen), "r"(bits) : "memory");
+    __device__ __forceinline__ void begin(const Attend4& a, const Head4& head, int lane) { row = load(a, head, 0, lane); }
+    __device__ __forceinline__ void fill(const Attend4& a, const Head4& head, int i, uint32_t stage, int lane) {
+        holes = __any_sync(0xffffffffu, holes);
 #pragma unroll
-        for (int it = 0; it < (B::G_ + 1) / 2; ++it) {
+        for (int it = 0; it < B::G_; ++it) {
             const int j = it * 32 + lane, key = j / B::G_, c = j - key * B::G_;
-            const uint32_t from = __shfl_sync(0xffffffffu, row, key & 15);
-            if (B::G_ % 2 == 0 || j < kTile4 * B::G_) {
-                const bool ok = from != kNoRow;
-                const size_t at = ok ? from : 0;
-                const uint32_t to = stage + key * B::kRow + ((c ^ B::turned(key)) * 16);
-                cp_async16(to, a.k.codes + at * B::kRow + c * 16, ok);
-                cp_async16(to + B::kValues, a.v.codes + at * B::kRow + c * 16, ok);
-                cp_async4(stage + B::kKeySteps + j * 4, reinterpret_cast<const uint32_t*>(a.k.steps) + at * B::G_ + c, ok);
-                cp_async4(stage + B::kValueSteps + j * 4, reinterpret_cast<const uint32_t*>(a.v.steps) + at * B::G_ + c, ok);
-            }
+            const size_t at = __shfl_sync(0xffffffffu, row, key);
+            const uint32_t to = stage + key * B::kRow + ((c ^ B::turned(key & 15)) * 16);
+            cp_async16(to, a.k.codes + at * B::kRow + c * 16, true);
+            cp_async16(to + B::kValues, a.v.codes + at * B::kRow + c * 16, true);
+            cp_async4(stage + B::kKeySteps + j * 4, reinterpret_cast<const uint32_t*>(a.k.steps) + at * B::G_ + c, true);
+            cp_async4(stage + B::kValueSteps + j * 4, reinterpret_cast<const uint32_t*>(a.v.steps) + at * B::G_ + c, true);
         }
-        row = i + 1 < own ? row_of(a, table, kvh, key0 + (i + 1) * (kWarps4 * kTile4) + (lane & 15), span) : kNoRow;
-    }
-    __device__ __forceinline__ uint32_t seen(int, uint32_t stage) const {
-        uint32_t bits;
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(bits) : "r"(stage + B::kSeen));
-        return bits;
+        row = load(a, head, i + 1, lane);
     }
 };
 
-// Where row `local` (tokens times the kv head's query heads) of a sequence stands in q and out, as token * Hq + head; -1 behind the last.
-__device__ __forceinline__ long row_at(const Attend4& a, int first_token, int n_tokens, int kvh, int local) {
-    const int group = a.Hq / a.Hkv, token = local / group;
-    return token < n_tokens && first_token + token < a.n_rows ? (long)(first_token + token) * a.Hq + kvh * group + (local - token * group) : -1;
+// Where a block's run of turns begins: every block adds up all entries; block 0 leaves the sums for the kernel that joins.
+struct Run4 {
+    int from, to, entry, offset;        // turns [from, to) of the line, the first of them `offset` into `entry`
+};
+__device__ __forceinline__ Run4 run_of(const Attend4& a, int rows) {
+    __shared__ int sums[kWarps4], found[2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, entries = a.n_seqs * a.row_blocks;
+    int all = 0, mine = 0;
+    for (int e = threadIdx.x; e < entries; e += kWarps4 * 32) {
+        const int n = Entry4(a, e, rows).turns * a.Hkv;
+        if (e < kWarps4 * 32) mine = n;
+        all += n;
+    }
+    all = __reduce_add_sync(0xffffffffu, all);
+    if (lane == 0) sums[warp] = all;
+    __syncthreads();
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps4; ++w) all += sums[w];
+    const int share = turns_of_block(all, a.blocks);
+    Run4 run = {(int)min((long long)all, (long long)blockIdx.x * share), 0, 0, 0};
+    run.to = min(all, run.from + share);
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[0] = share;
+    if (run.from >= run.to && blockIdx.x != 0) return run;
+    int before = 0;
+    for (int e0 = 0; e0 < entries; e0 += kWarps4 * 32) {
+        const int e = e0 + threadIdx.x;
+        const int n = e0 == 0 ? mine : e < entries ? Entry4(a, e, rows).turns * a.Hkv : 0;
+        int upto = n;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, off);
+            if (lane >= off) upto += v;
+        }
+        __syncthreads();                // `sums` have been read
+        if (lane == 31) sums[warp] = upto;
+        __syncthreads();
+        int here = before - n + upto;
+#pragma unroll
+        for (int w = 0; w < kWarps4; ++w) {
+            if (w < warp) here += sums[w];
+            before += sums[w];
+        }
+        if (blockIdx.x == 0 && e < entries) a.plan[1 + e] = here;
+        if (run.from >= here && run.from < here + n) {
+            found[0] = e;
+            found[1] = run.from - here;
+        }
+        if (blockIdx.x != 0 && before > run.from) break;
+    }
+    __syncthreads();
+    run.entry = found[0];
+    run.offset = found[1];
+    return run;
 }
 
 template <typename T, int G, int NT, int COPIES, typename Turns, int BLOCKS>
@@ -528,195 +644,231 @@ __global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_kernel(const
     pdl_wait();
     extern __shared__ __align__(128) uint8_t shared[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, t = lane & 3;
-    const int part = blockIdx.x, kvh = blockIdx.y / a.row_blocks, row_block = blockIdx.y - kvh * a.row_blocks, seq = blockIdx.z;
-    const int group = a.Hq / a.Hkv, row0 = row_block * B::kRows;
-    const int first_token = a.cu_q ? a.cu_q[seq] : seq, n_tokens = a.cu_q ? a.cu_q[seq + 1] - first_token : 1, kv_len = a.kv_len[seq];
-    if (row0 >= n_tokens * group) return;
-    const int token0 = row0 / group, token1 = min(n_tokens - 1, (row0 + B::kRows - 1) / group);
-    const Span4 span(a, kv_len, n_tokens, token0, token1);
-    const int n_parts = span.parts(a);
-    if (part >= n_parts && !(n_parts == 0 && part == 0)) return;
-    const int begin = span.start() + part * a.part_keys, end = min(span.last + 1, begin + a.part_keys);
-    const int tiles = end > begin ? (end - begin + kTile4 - 1) / kTile4 : 0, own = tiles > warp ? (tiles - warp + kWarps4 - 1) / kWarps4 : 0;
-
-    const uint32_t ring = smem_u32(shared) + warp * B::kPerWarp;
-    const int* table = a.table + (size_t)seq * a.width;
-    const int key_first = begin + warp * kTile4;
-    Turns turns;
-    turns.begin(a, table, kvh, key_first, own, span, lane);
-#pragma unroll
-    for (int i = 0; i < kStages4 - 1; ++i) {
-        if (i < own) turns.fill(a, table, kvh, key_first, own, span, i, ring + i * B::kStage, lane);
-        cp_async_commit();
-    }
-
-    B b;
-    const T* src[NT];
-    int lowest = 0x7fffffff, highest = -0x7fffffff;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const long at = row_at(a, first_token, n_tokens, kvh, row0 + 8 * n + r % B::kColumns);
-        src[n] = at < 0 ? nullptr : reinterpret_cast<const T*>(a.q) + at * D;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            b.pos[n][c] = min(span.last, kv_len - n_tokens + min(n_tokens - 1, (row0 + 8 * n + (2 * t + c) % B::kColumns) / group));
-            b.top[n][c] = kLowest4;
-            b.total[n][c] = 0.0f;
-#pragma unroll
-            for (int g = 0; g < B::GH; ++g) b.least_sum[n][g][c] = 0.0f;
-#pragma unroll
-            for (int g = 0; g < G; ++g)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) b.o[n][g][u][c] = b.o[n][g][u][c + 2] = 0.0f;
+    const uint32_t ring = smem_u32(shared) + warp * B::kPerWarp, q_at = smem_u32(shared) + B::kQ;
+    Run4 run = run_of(a, B::kRows);
+    while (run.from < run.to) {
+        const Entry4 entry(a, run.entry, B::kRows);
+        if (run.offset >= entry.turns * a.Hkv) {         // on to the next entry that has turns, 32 looked at together
+            const int entries = a.n_seqs * a.row_blocks;
+            uint32_t some = 0;
+            for (++run.entry; run.entry < entries && some == 0; run.entry += 32)
+                some = __ballot_sync(0xffffffffu, run.entry + lane < entries && Entry4(a, min(run.entry + lane, entries - 1), B::kRows).turns > 0);
+            if (some == 0) break;
+            run.entry += __ffs(some) - 33;
+            run.offset = 0;
+            continue;
         }
-    }
-    lowest = min(span.last, kv_len - n_tokens + token0);
-    highest = kv_len - n_tokens + token1;
-    b.load_q(src, a.scale_log2, lane);
-
-    int stage = 0;
-    for (int i = 0; i < own; ++i) {
-        cp_async_wait<kStages4 - 2>();
-        __syncwarp();
-        const int next = i + kStages4 - 1, to = stage == 0 ? kStages4 - 1 : stage - 1;
-        if (next < own) turns.fill(a, table, kvh, key_first, own, span, next, ring + to * B::kStage, lane);
-        cp_async_commit();
-        const uint32_t at = ring + stage * B::kStage, seen = turns.seen(i, at);
-        const int key0 = key_first + i * (kWarps4 * kTile4);
-        if (seen != 0xffffu || key0 + kTile4 - 1 > lowest || (a.window > 0 && key0 <= highest - a.window)) {
-            if (seen != 0) b.template turn<true>(at, key0, seen, a.window, lane);
-        } else {
-            b.template turn<false>(at, key0, seen, a.window, lane);
+        const int kvh = run.offset / entry.turns, skipped = run.offset - kvh * entry.turns, n_turns = min(entry.turns - skipped, run.to - run.from);
+        const int own = n_turns > warp ? (n_turns - warp + kWarps4 - 1) / kWarps4 : 0;
+        const Head4 head = {a.table + (size_t)entry.seq * a.width, kvh, entry.start() + (skipped + warp) * kTile4, own, entry.first, entry.last};
+        Turns turns;
+        turns.begin(a, head, lane);
+        const T* src[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const long at = entry.row_at(a, kvh, 8 * n + r % B::kColumns);
+            src[n] = at < 0 ? nullptr : reinterpret_cast<const T*>(a.q) + at * D;
         }
-        stage = stage + 1 == kStages4 ? 0 : stage + 1;
+        typename B::RawQ raw;
+        B::read_q(src, raw, lane);
+#pragma unroll
+        for (int i = 0; i < B::kBuffers - 1; ++i) {
+            if (i < own) turns.fill(a, head, i, ring + i * B::kStage, lane);
+            cp_async_commit();
+        }
+        B::write_q(raw, a.scale_log2, q_at, warp, lane);
+
+        B b;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int group = a.Hq / a.Hkv;
+                b.pos[n][c] = min(entry.last, entry.kv_len - entry.n_tokens + min(entry.n_tokens - 1, (entry.row0 + 8 * n + (2 * t + c) % B::kColumns) / group));
+                b.top[n][c] = kLowest4;
+                b.total[n][c] = 0.0f;
+#pragma unroll
+                for (int g = 0; g < B::GH; ++g) {
+                    b.least_sum[n][g][c] = 0.0f;
+                    if (B::kOffsets) b.offsets[g][c] = b.offsets[g][c + 2] = 0.0f;
+                }
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) b.o[n][g][u][c] = b.o[n][g][u][c + 2] = 0.0f;
+            }
+        // turns [inner_from, inner_to) are seen whole by every column
+        const int before = entry.kv_len - entry.n_tokens;
+        const int lowest = min(entry.last, before + entry.token0), above = a.window > 0 ? before + entry.token1 - a.window - head.key0 + 1 : 0;
+        const int inner_from = above > 0 ? (above + kWarps4 * kTile4 - 1) / (kWarps4 * kTile4) : 0;
+        const int inner_to = lowest - head.key0 >= kTile4 - 1 ? (lowest - head.key0 - (kTile4 - 1)) / (kWarps4 * kTile4) + 1 : 0;
+        __syncthreads();
+        b.take_q_sums(q_at, lane);
+
+        uint32_t stage = ring, free = ring + (B::kBuffers - 1) * B::kStage;
+        for (int i = 0; i < own; ++i) {
+            cp_async_wait<B::kBuffers - 2>();
+            __syncwarp();
+            if (i + B::kBuffers - 1 < own) turns.fill(a, head, i + B::kBuffers - 1, free, lane);
+            cp_async_commit();
+            if (i >= inner_from && i < inner_to && !turns.holes)
+                b.template turn<false>(stage, q_at, 0, lane, [](int, int) { return true; });
+            else
+                b.template turn<true>(stage, q_at, head.key0 + i * (kWarps4 * kTile4), lane, [&](int key, int pos) {
+                    int place;
+                    return key <= pos && (a.window == 0 || key > pos - a.window) && (!turns.holes || page_of(a, head, key, place) >= 0);
+                });
+            free = stage;
+            stage = stage == ring + (B::kBuffers - 1) * B::kStage ? ring : stage + B::kStage;
+            __syncwarp();
+        }
+
+        cp_async_wait<0>();
         __syncwarp();
+        // The warp's sums to its own shared memory (the ring is done with): [column][D], then maxima and totals.
+        float* mine = reinterpret_cast<float*>(shared + warp * B::kPerWarp);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int column = 8 * n + (2 * t + c) % B::kColumns, copy = t * COPIES / 4;
+                float total = b.total[n][c];
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+                float least[B::GH];
+#pragma unroll
+                for (int j = 0; j < B::GH; ++j) {
+                    least[j] = b.least_sum[n][j][c];
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) least[j] += __shfl_xor_sync(0xffffffffu, least[j], off);
+                    if (B::kOffsets) least[j] -= b.offsets[j][c];
+                }
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const float m = least[g % B::GH];
+                    if (copy == g / B::GH)
+                        *reinterpret_cast<float4*>(mine + column * D + 32 * g + 4 * r) =
+                            make_float4(b.o[n][g][0][c] + m, b.o[n][g][0][c + 2] + m, b.o[n][g][1][c] + m, b.o[n][g][1][c + 2] + m);
+                }
+                if (r == 0 && copy == 0) {
+                    mine[B::kRows * D + 2 * column] = b.top[n][c];
+                    mine[B::kRows * D + 2 * column + 1] = total;
+                }
+            }
+        __syncthreads();
+        const bool whole = n_turns == entry.turns;
+        const int place = 2 * blockIdx.x + (skipped > 0 ? 0 : 1);        // a head that another block began, or one that another ends
+        for (int i = threadIdx.x; i < B::kRows * (D / 4); i += kWarps4 * 32) {
+            const int column = i / (D / 4), quad = i - column * (D / 4);
+            const long at = entry.row_at(a, kvh, column);
+            if (at < 0) continue;
+            float tops[kWarps4], top = kLowest4, total = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < kWarps4; ++w) {
+                tops[w] = reinterpret_cast<const float*>(shared + w * B::kPerWarp)[B::kRows * D + 2 * column];
+                top = fmaxf(top, tops[w]);
+            }
+#pragma unroll
+            for (int w = 0; w < kWarps4; ++w) {
+                const float* theirs = reinterpret_cast<const float*>(shared + w * B::kPerWarp);
+                const float f = exp2_fast(tops[w] - top);
+                const float4 s = *reinterpret_cast<const float4*>(theirs + column * D + 4 * quad);
+                total += f * theirs[B::kRows * D + 2 * column + 1];
+                v[0] += f * s.x; v[1] += f * s.y; v[2] += f * s.z; v[3] += f * s.w;
+            }
+            if (whole) {
+                const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = total == 0.0f ? 0.0f : v[e] * inverse;
+                store_quad(reinterpret_cast<T*>(a.out) + at * D + 4 * quad, v);
+            } else {
+                store_quad(a.sums + ((size_t)place * B::kRows + column) * D + 4 * quad, v);
+                if (quad == 0) *reinterpret_cast<float2*>(a.sums + (size_t)2 * a.blocks * B::kRows * D + ((size_t)place * B::kRows + column) * 2) = make_float2(top, total);
+            }
+        }
+        __syncthreads();
+        run.from += n_turns;
+        run.offset += n_turns;
     }
-    cp_async_wait<0>();
-    __syncwarp();
     pdl_trigger();
-
-    // The warp's sums to its own shared memory (the ring is done with): [column][D], then maxima and totals.
-    float* mine = reinterpret_cast<float*>(shared + warp * B::kPerWarp);
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int column = 8 * n + (2 * t + c) % B::kColumns, copy = t * COPIES / 4;
-            float total = b.total[n][c];
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-            float least[B::GH];
-#pragma unroll
-            for (int j = 0; j < B::GH; ++j) {
-                least[j] = b.least_sum[n][j][c];
-#pragma unroll
-                for (int off = 4; off < 32; off <<= 1) least[j] += __shfl_xor_sync(0xffffffffu, least[j], off);
-            }
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-                const float m = least[g % B::GH];
-                if (copy == g / B::GH)
-                    *reinterpret_cast<float4*>(mine + column * D + 32 * g + 4 * r) =
-                        make_float4(b.o[n][g][0][c] + m, b.o[n][g][0][c + 2] + m, b.o[n][g][1][c] + m, b.o[n][g][1][c + 2] + m);
-            }
-            if (r == 0 && copy == 0) {
-                mine[B::kRows * D + 2 * column] = b.top[n][c];
-                mine[B::kRows * D + 2 * column + 1] = total;
-            }
-        }
-    __syncthreads();
-    for (int i = threadIdx.x; i < B::kRows * (D / 4); i += kWarps4 * 32) {
-        const int column = i / (D / 4), quad = i - column * (D / 4);
-        const long at = row_at(a, first_token, n_tokens, kvh, row0 + column);
-        if (at < 0) continue;
-        float tops[kWarps4], top = kLowest4, total = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < kWarps4; ++w) {
-            tops[w] = reinterpret_cast<const float*>(shared + w * B::kPerWarp)[B::kRows * D + 2 * column];
-            top = fmaxf(top, tops[w]);
-        }
-#pragma unroll
-        for (int w = 0; w < kWarps4; ++w) {
-            const float* theirs = reinterpret_cast<const float*>(shared + w * B::kPerWarp);
-            const float f = exp2_fast(tops[w] - top);
-            const float4 s = *reinterpret_cast<const float4*>(theirs + column * D + 4 * quad);
-            total += f * theirs[B::kRows * D + 2 * column + 1];
-            v[0] += f * s.x; v[1] += f * s.y; v[2] += f * s.z; v[3] += f * s.w;
-        }
-        if (a.parts == 1) {
-            const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = total == 0.0f ? 0.0f : v[e] * inverse;
-            store_quad(reinterpret_cast<T*>(a.out) + at * D + 4 * quad, v);
-        } else {
-            store_quad(a.sums + (at * a.parts + part) * D + 4 * quad, v);
-            if (quad == 0) {
-                float* ml = a.sums + (size_t)a.n_rows * a.Hq * a.parts * D + (at * a.parts + part) * 2;
-                ml[0] = top;
-                ml[1] = total;
-            }
-        }
-    }
 }
 
-// The parts of a row joined: a warp a row.
+// The rows of heads that several blocks had, joined; zeros where there is no key.  A block a row and head, its warps every fourth part.
 template <typename T>
-__global__ void join_4bit_kernel(const Attend4 a, int D, int rows_of_block) {
+__global__ void __launch_bounds__(128) join_4bit_kernel(const Attend4 a, int D, int rows) {
     pdl_wait();
-    const int lane = threadIdx.x & 31, seq = blockIdx.y;
-    const int first_token = a.cu_q ? a.cu_q[seq] : seq, n_tokens = a.cu_q ? a.cu_q[seq + 1] - first_token : 1;
-    const int index = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), group = a.Hq / a.Hkv;
-    if (index >= n_tokens * a.Hq) return;
-    const int token = index / a.Hq, head = index - token * a.Hq, kvh = head / group, local = token * group + head - kvh * group;
-    const int token0 = local / rows_of_block * rows_of_block / group, token1 = min(n_tokens - 1, (local / rows_of_block * rows_of_block + rows_of_block - 1) / group);
-    const int used = Span4(a, a.kv_len[seq], n_tokens, token0, token1).parts(a);
-    const long at = row_at(a, first_token, n_tokens, kvh, local);
+    __shared__ float shared[4][256];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = a.Hq / a.Hkv, seq = blockIdx.y;
+    const int token = blockIdx.x / a.Hq, head = blockIdx.x - token * a.Hq, kvh = head / group, row = token * group + head - kvh * group;
+    const Entry4 entry(a, seq * a.row_blocks + row / rows, rows);
+    const long at = token < entry.n_tokens ? entry.row_at(a, kvh, row % rows) : -1;
     if (at < 0) return;
-    const float* ml = a.sums + (size_t)a.n_rows * a.Hq * a.parts * D + at * a.parts * 2;
-    float top = kLowest4, total = 0.0f, v[2][4] = {};
-    for (int p = lane; p < used; p += 32) top = fmaxf(top, ml[2 * p]);
-    top = warp_max(top);
-    for (int p = lane; p < used; p += 32) total += exp2_fast(ml[2 * p] - top) * ml[2 * p + 1];
-    total = warp_sum(total);
+    float v[2][4] = {};
+    if (entry.turns > 0) {
+        const int share = a.plan[0], from = a.plan[1 + seq * a.row_blocks + row / rows] + kvh * entry.turns;
+        const int block0 = from / share, parts = (from + entry.turns - 1) / share - block0 + 1;
+        if (parts == 1) return;                          // its block has written it
+        const float* ml = a.sums + (size_t)2 * a.blocks * rows * D;
+        // part p is block0 + p's: the first of them began the head, unless the head's first turn is the first of the block
+        auto place = [&](int p) { return (size_t)(2 * (block0 + p) + (p > 0 ? 0 : 1)) * rows + row % rows; };
+        float top = kLowest4, total = 0.0f;
+        for (int p = lane; p < parts; p += 32) top = fmaxf(top, ml[2 * place(p)]);
+        top = warp_max(top);
+        for (int p = lane; p < parts; p += 32) total += exp2_fast(ml[2 * place(p)] - top) * ml[2 * place(p) + 1];
+        total = warp_sum(total);
+        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll 4
-    for (int p = 0; p < used; ++p) {
-        const float f = exp2_fast(ml[2 * p] - top);
-        const float* s = a.sums + (at * a.parts + p) * D;
+        for (int p = warp; p < parts; p += 4) {
+            const float f = exp2_fast(ml[2 * place(p)] - top);
+            const float* s = a.sums + place(p) * D;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (4 * (lane + 32 * j) < D) {
+                    float w[4];
+                    load_quad(s + 4 * (lane + 32 * j), w);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[j][e] = fmaf(f, w[e], v[j][e]);
+                }
+        }
 #pragma unroll
         for (int j = 0; j < 2; ++j)
             if (4 * (lane + 32 * j) < D) {
-                float w[4];
-                load_quad(s + 4 * (lane + 32 * j), w);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[j][e] = fmaf(f, w[e], v[j][e]);
+                for (int e = 0; e < 4; ++e) v[j][e] = total == 0.0f ? 0.0f : v[j][e] * inverse;
+                *reinterpret_cast<float4*>(shared[warp] + 4 * (lane + 32 * j)) = make_float4(v[j][0], v[j][1], v[j][2], v[j][3]);
             }
+        __syncthreads();
+    } else if (warp == 0) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            if (4 * (lane + 32 * j) < D) store_quad(reinterpret_cast<T*>(a.out) + at * D + 4 * (lane + 32 * j), v[j]);
+        return;
+    } else {
+        return;
     }
-    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    const int quad = threadIdx.x;
+    if (4 * quad < D) {
+        float w[4];
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-        if (4 * (lane + 32 * j) < D) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[j][e] = total == 0.0f ? 0.0f : v[j][e] * inverse;
-            store_quad(reinterpret_cast<T*>(a.out) + at * D + 4 * (lane + 32 * j), v[j]);
-        }
+        for (int e = 0; e < 4; ++e) w[e] = (shared[0][4 * quad + e] + shared[1][4 * quad + e]) + (shared[2][4 * quad + e] + shared[3][4 * quad + e]);
+        store_quad(reinterpret_cast<T*>(a.out) + at * D + 4 * quad, w);
+    }
 }
 
 template <typename T, int G, int NT, int COPIES, template <typename> class Turns>
 int launch_attend_4bit(const Attend4& a, int most_tokens, cudaStream_t stream) {
     using B = Attend4Block<T, G, NT, COPIES>;
-    constexpr int kRegs = G * NT * (4 * B::kTerms + 8) + 6 * NT * B::GH + 66;       // about: q, sums and the rest of a thread
-    constexpr int kBlocks = kRegs <= 150 ? 4 : kRegs <= 180 ? 3 : 2;
+    constexpr int kBlocks = blocks_4bit(sizeof(T) == 4, G, B::kRows);
     auto kernel = attend_4bit_kernel<T, G, NT, COPIES, Turns<B>, kBlocks>;
     static SmemLimit limit;
     if (const int rc = limit.allow(kernel, B::kShared)) return rc;
-    if (const int rc = launch_pdl(kernel, dim3(a.parts, a.Hkv * a.row_blocks, a.n_seqs), dim3(kWarps4 * 32), B::kShared, stream, a)) return rc;
-    if (a.parts == 1) return 0;
-    return launch_pdl(join_4bit_kernel<T>, dim3((most_tokens * a.Hq + 3) / 4, a.n_seqs), dim3(128), 0, stream, a, B::D, B::kRows);
+    if (const int rc = launch_pdl(kernel, dim3(a.blocks), dim3(kWarps4 * 32), B::kShared, stream, a)) return rc;
+    return launch_pdl(join_4bit_kernel<T>, dim3(most_tokens * a.Hq, a.n_seqs), dim3(128), 0, stream, a, B::D, B::kRows);
 }
 
 template <typename T, int G, template <typename> class Turns>
 int launch_attend_4bit_of(const Attend4& a, int rows, int most_tokens, cudaStream_t stream) {
-    if constexpr (sizeof(T) == 2)
+    if constexpr (sizeof(T) == 2 && G <= 4)
         if (rows == 16) return launch_attend_4bit<T, G, 2, 1, Turns>(a, most_tokens, stream);
     if constexpr (G % 4 == 0)
         if (rows == 2) return launch_attend_4bit<T, G, 1, 4, Turns>(a, most_tokens, stream);
@@ -727,7 +879,7 @@ int launch_attend_4bit_of(const Attend4& a, int rows, int most_tokens, cudaStrea
 
 template <typename T, int G>
 int launch_attend_4bit_of(const Attend4& a, int rows, int most_tokens, cudaStream_t stream) {
-    return a.page_size % kTile4 == 0 ? launch_attend_4bit_of<T, G, Turns16>(a, rows, most_tokens, stream) : launch_attend_4bit_of<T, G, TurnsAny>(a, rows, most_tokens, stream);
+    return a.page_size % 16 == 0 ? launch_attend_4bit_of<T, G, Turns16>(a, rows, most_tokens, stream) : launch_attend_4bit_of<T, G, TurnsAny>(a, rows, most_tokens, stream);
 }
 
 template <typename T>

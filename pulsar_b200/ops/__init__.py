@@ -156,7 +156,8 @@ _SIGNATURES = {
     "pb_head_scores": [_P] * 5 + [_I, _I, _I, _F, _F, _P, _P, _P],
     "pb_qk_norm_rope_write_4bit": [_I] + [_P] * 11 + [ctypes.c_double] + [_I] * 7 + [_P],
     "pb_expand_pages_4bit": [_I] + [_P] * 9 + [_I] * 6 + [_P, _I, _P],
-    "pb_paged_attention_4bit": [_I] + [_P] * 8 + [_I, _P, _P] + [_I] * 8 + [_F, _I, _I, _I, _P],
+    "pb_paged_attention_4bit": [_I] + [_P] * 9 + [_I, _P, _P] + [_I] * 8 + [_F, _I, _I, _P],
+    "pb_attention_4bit_blocks": [_I] * 9,
     "pb_attention_4bit_rows": [_I, _I, _I],
     "pb_token_scores": [_I, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P],
 }
@@ -2299,14 +2300,12 @@ EXPANDED_ROWS_4BIT = 64
 
 
 @functools.lru_cache(maxsize=1024)
-def cut_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int, table_tokens: int, window: int, dtype: torch.dtype) -> Tuple[int, int]:
-    """(parts, keys of a part) that ``paged_attention_4bit`` cuts the keys of a sequence into, for sequences of up to ``most_tokens`` tokens."""
-    rows = most_tokens * (n_heads // n_kv_heads)
-    blocks = n_seqs * n_kv_heads * -(-rows // fn("pb_attention_4bit_rows")(code(dtype), rows, head_dim))
-    keys = min(table_tokens, window + most_tokens + 15) if window else table_tokens
-    part = max(64, min(1024, -(-keys * blocks // (3 * 148)))) if blocks else 64
-    part = -(-part // 64) * 64
-    return -(-keys // part), part
+def scratch_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int, width: int, page_size: int, window: int, dtype: torch.dtype) -> Tuple[int, int, int]:
+    """(blocks, float32 elements of sums, int32 elements of the plan) of ``paged_attention_4bit`` for sequences of up to ``most_tokens`` tokens."""
+    rows_all = most_tokens * (n_heads // n_kv_heads)
+    rows = fn("pb_attention_4bit_rows")(code(dtype), rows_all, head_dim)
+    blocks = fn("pb_attention_4bit_blocks")(code(dtype), most_tokens, n_seqs, n_heads, n_kv_heads, head_dim, width, page_size, window)
+    return blocks, blocks * 2 * rows * (head_dim + 2), 2 + n_seqs * -(-rows_all // rows)
 
 
 def _expanded_4bit(dtype: torch.dtype, rows: int, n_heads: int, n_kv_heads: int, head_dim: int, page_size: int, scale: float) -> Optional[str]:
@@ -2380,7 +2379,8 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
         run, tiles = (paged_attention_prefill_tcgen05, prefill_tcgen05_tiles) if dense == "tcgen05" else (paged_attention_prefill_tc, prefill_tc_tiles)
         run(q, k_out, v_out, out, table_out, cu_q, kv_len, tiles(q_lens), scale, window)
         return
-    parts, part_keys = cut_4bit(s, most_tokens, hq, hkv, d, width * page_size, window, q.dtype)
-    sums = scratch("attn4.sums", (n * hq * parts * (d + 2),), torch.float32) if parts > 1 else None
-    check(fn("pb_paged_attention_4bit")(kind, _p(q), _p(k_pool), _p(k_steps), _p(v_pool), _p(v_steps), _p(out), _p(sums), _p(block_table), width, _p(kv_len), _p(cu_q), n,
-                                        most_tokens, s, hq, hkv, d, page_size, n_pages, float(scale), window, parts, part_keys, stream()), name, kernels=1 if parts == 1 else 2)
+    blocks, sums, plan = scratch_4bit(s, most_tokens, hq, hkv, d, width, page_size, window, q.dtype)
+    work = scratch("attn4.work", (sums + plan,), torch.float32)
+    at = work.data_ptr()
+    check(fn("pb_paged_attention_4bit")(kind, _p(q), _p(k_pool), _p(k_steps), _p(v_pool), _p(v_steps), _p(out), at, at + 4 * sums, _p(block_table), width, _p(kv_len),
+                                        _p(cu_q), n, most_tokens, s, hq, hkv, d, page_size, n_pages, float(scale), window, blocks, stream()), name, kernels=2)
