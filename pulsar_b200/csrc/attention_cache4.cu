@@ -36,7 +36,8 @@ PB_EXPORT int pb_attention_4bit_blocks(int dtype, int most_tokens, int n_seqs, i
     const long long row_blocks = ((long long)most_tokens * (Hq / Hkv) + rows - 1) / rows;
     long long keys = (long long)width * page_size;
     if (window > 0 && keys > (long long)window + most_tokens + 16) keys = (long long)window + most_tokens + 16;
-    const long long turns = n_seqs * row_blocks * Hkv * ((keys + kTile4 - 1) / kTile4), wanted = (turns + kLeastTurns4 - 1) / kLeastTurns4;
+    const long long heads = n_seqs * row_blocks * Hkv, turns = heads * ((keys + kTile4 - 1) / kTile4), parts = (turns + kLeastShare4 - 1) / kLeastShare4;
+    const long long wanted = parts > heads ? parts : heads;
     const int most = sm_count_4bit() * blocks_4bit(dtype == PB_F32, D / kGroup4, rows);
     return wanted < most ? (int)wanted : most;
 }
@@ -54,7 +55,7 @@ PB_EXPORT int pb_paged_attention_4bit(int dtype, const void* q, void* k_codes, v
     const int group = Hq / Hkv, rows = pb_attention_4bit_rows(dtype, most_tokens * group, D);
     const long long row_blocks = ((long long)most_tokens * group + rows - 1) / rows, keys = (long long)width * page_size;
     if (n_seqs > 65535 || (long long)most_tokens * Hq > 0x3fffffff || (long long)n_pages * Hkv * page_size >= 0xffffffffLL || keys > 0x7ffffff0LL ||
-        (double)n_seqs * row_blocks * Hkv * (keys / kTile4 + 1) > 2.0e9)
+        (double)n_seqs * row_blocks * Hkv * (keys / kTile4 + 1 + kGap4) > 1.0e9)
         return PB_ERR_TOO_LARGE;
     Attend4 a{q, out, {(uint8_t*)k_codes, (__nv_bfloat16*)k_steps}, {(uint8_t*)v_codes, (__nv_bfloat16*)v_steps}, sums, plan, table, kv_len, cu_q, width, n_rows, n_seqs,
               Hq, Hkv, page_size, log2_exact(page_size), n_pages, (int)row_blocks, blocks, window, scale * kLog2e, pool_bounds_now()};

@@ -48,9 +48,11 @@ struct Attend4 {
 };
 
 // The work is dealt out in turns of 32 keys.  An entry is a sequence and as many of its rows (tokens times the query heads of a kv head) as a block
-// takes; the turns of all entries, kv head by kv head, stand in one line, and every block takes the same number of them, one run
-// of the line.  So nobody is left with a long sequence when the others are done, whatever the lengths are, and a block has at most one head that
-// another one began and one that another one ends.  What the lengths are is read here, on the device: a captured call serves any.
+// takes.  The turns of all entries, kv head by kv head, stand in one line, and every block takes a run of the line of the same length; what
+// the lengths are is read here, on the device: a captured call serves any.  Two ways to lay the line out, whichever ends sooner:
+//   apart    every head begins with a block of its own, and its last block may have less: few heads, as many blocks as there are
+//   packed   a head follows the other, with a gap of kGap4 turns between them that stands for what it costs to begin and end one
+// In either a block has at most one head that another one began and one that another one ends.
 struct Entry4 {
     int seq, first_token, n_tokens, kv_len, row0, token0, token1;
     int first, last, turns;             // the keys [first, last] that any of its rows sees; turns begin at first rounded down
@@ -81,12 +83,27 @@ struct Entry4 {
 constexpr int blocks_4bit(bool exact, int groups, int rows) {
     return groups * (rows > 8 ? 2 : 1) >= 6 ? 2 : exact || groups * (rows > 8 ? 2 : 1) > 2 ? 3 : 4;
 }
-// Turns of a block where there are so many altogether: no fewer than 8, below which a block's start and end cost more than its turns.
-constexpr int kLeastTurns4 = 8;
-__host__ __device__ inline int turns_of_block(int all, int blocks) {
-    const int n = (all + blocks - 1) / blocks;
-    return n < kLeastTurns4 ? kLeastTurns4 : (n + kWarps4 - 1) / kWarps4 * kWarps4;
-}
+constexpr int kLeastShare4 = 8;         // turns of a block, at least
+constexpr int kGap4 = 16;                // turns that a head's start and end are worth
+struct Plan4 {
+    int share;                          // of a block, in turns
+    bool apart;
+    __device__ __forceinline__ int gap() const { return apart ? 0 : kGap4; }
+    __device__ __forceinline__ int line(int turns) const { return turns == 0 ? 0 : apart ? (turns + share - 1) / share * share : turns + kGap4; }
+    // all: turns of all heads; heads: those with turns; most: of one.
+    static __device__ __forceinline__ Plan4 of(int all, int heads, int most, int blocks) {
+        const int packed = (all + heads * kGap4 + blocks - 1) / blocks;
+        int apart = 0x7fffffff;
+        if (heads > 0 && heads <= blocks) {
+            const int each = blocks / heads;
+            apart = (most + each - 1) / each;                                                       // enough blocks for the longest
+            if (blocks > heads) apart = min(apart, (all + blocks - heads - 1) / (blocks - heads));  // enough for whatever they are
+        }
+        const bool is_apart = apart <= packed;
+        const int share = (max(is_apart ? apart : packed, kLeastShare4) + kWarps4 - 1) / kWarps4 * kWarps4;
+        return {share, is_apart};
+    }
+};
 
 __device__ __forceinline__ float exp2_fast(float v) {
     float r;
@@ -302,9 +319,49 @@ struct Attend4Block {
         }
     }
 
-    // Thirty-two keys.  EDGE: some column does not see some of them.  `sees(key, pos)`: whether one does.
-    template <bool EDGE, typename Sees>
-    __device__ __forceinline__ void turn(uint32_t stage, uint32_t q_at, int key0, int lane, Sees sees) {
+    // The keys from key0 on of which some column does not see some, positions [lowest, highest].  Scores of what a column does not see become -inf.
+    // A weight of zero must be nothing whatever the value it belongs to, so steps of values that no column sees, which may be anything, become
+    // zero; so do steps that are no numbers of values that only some columns see, and the sums of those columns are none any more.
+    template <typename There>
+    __device__ __forceinline__ void take_edges(float (&x)[2][NT][4], uint32_t stage, int key0, int lowest, int highest, int window, int lane, There there) {
+        const int r = lane >> 2;
+        const uint32_t pages = __ballot_sync(0xffffffffu, there(key0 + lane));
+        auto sees = [&](int i, int p) { return key0 + i <= p && (window == 0 || key0 + i > p - window) && ((pages >> i) & 1); };
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (!sees(16 * half + placed(r) + (e < 2 ? 0 : 8), pos[n][e & 1])) x[half][n][e] = -INFINITY;
+        const bool any = key0 + lane <= highest && (window == 0 || key0 + lane > lowest - window) && ((pages >> lane) & 1);
+        const bool all = sees(lane, lowest) && sees(lane, highest);
+        const uint32_t steps = stage + kValueSteps + lane * 4 * G;
+        bool bad = false;
+        if (any && !all) {
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                uint32_t word;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(word) : "r"(steps + 4 * g));
+                bad |= (word & 0x7f80u) == 0x7f80u || (word & 0x7f800000u) == 0x7f800000u;
+            }
+        }
+        if (!any || bad) {
+#pragma unroll
+            for (int g = 0; g < G; ++g) asm volatile("st.shared.u32 [%0], %1;" ::"r"(steps + 4 * g), "r"(0) : "memory");
+        }
+        for (uint32_t left = __ballot_sync(0xffffffffu, bad); left != 0; left &= left - 1)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    if (sees(__ffs(left) - 1, pos[n][c])) total[n][c] = __int_as_float(0x7fc00000);
+        __syncwarp();
+    }
+
+    // Thirty-two keys.  `edge`: some column does not see some of them; edges(*this, x) then takes those scores away.
+    template <typename Edges>
+    __device__ __forceinline__ void turn(uint32_t stage, uint32_t q_at, int lane, bool edge, Edges edges) {
         const int r = lane >> 2, t = lane & 3, row0 = placed(r), row1 = row0 + 8, copy = t * COPIES / 4;
         float x[2][NT][4];
         {
@@ -365,10 +422,11 @@ struct Attend4Block {
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[half][n][e] = over_copies(x[half][n][e]) * to_log2[n][e & 1];
-                    if constexpr (EDGE) x[half][n][e] = sees(key0 + 16 * half + (e < 2 ? row0 : row1), pos[n][e & 1]) ? x[half][n][e] : -INFINITY;
-                }
+                for (int e = 0; e < 4; ++e) x[half][n][e] = over_copies(x[half][n][e]) * to_log2[n][e & 1];
+        }
+        if (edge) edges(x);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
             // The maximum moves only when a score passes it by more than 2^8: weights stay below 2^8, float32 and bfloat16 have room for them.
 #pragma unroll
             for (int c = 0; c < 2; ++c) rises |= fmaxf(fmaxf(x[0][n][c], x[0][n][c + 2]), fmaxf(x[1][n][c], x[1][n][c + 2])) > top[n][c] + 8.0f;
@@ -434,13 +492,10 @@ struct Attend4Block {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     float w[4];
-                    // EDGE: a weight of zero is nothing, whatever the value it belongs to
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float p = x[half][n][e];
-                        w[e] = p * step[e >> 1];
-                        if (EDGE && p == 0.0f) w[e] = 0.0f;
-                        else least_sum[n][j][e & 1] = fmaf(p, middle[e >> 1], least_sum[n][j][e & 1]);
+                        w[e] = x[half][n][e] * step[e >> 1];
+                        least_sum[n][j][e & 1] = fmaf(x[half][n][e], middle[e >> 1], least_sum[n][j][e & 1]);
                     }
 #pragma unroll
                     for (int term = 0; term < kTerms; ++term) {
@@ -581,34 +636,44 @@ struct TurnsAny {
     }
 };
 
-// Where a block's run of turns begins: every block adds up all entries; block 0 leaves the sums for the kernel that joins.
+// Where a block's run of the line begins: every block looks at all entries; block 0 leaves the plan for the kernel that joins.
 struct Run4 {
-    int from, to, entry, offset;        // turns [from, to) of the line, the first of them `offset` into `entry`
+    int from, to, entry, offset;        // [from, to) of the line, the first of them `offset` into `entry`
+    Plan4 plan;
 };
 __device__ __forceinline__ Run4 run_of(const Attend4& a, int rows) {
-    __shared__ int sums[kWarps4], found[2];
+    __shared__ int sums[3][kWarps4], found[2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, entries = a.n_seqs * a.row_blocks;
-    int all = 0, mine = 0;
+    int all = 0, heads = 0, most = 0, mine = 0;
     for (int e = threadIdx.x; e < entries; e += kWarps4 * 32) {
-        const int n = Entry4(a, e, rows).turns * a.Hkv;
+        const int n = Entry4(a, e, rows).turns;
         if (e < kWarps4 * 32) mine = n;
         all += n;
+        heads += n > 0;
+        most = max(most, n);
     }
     all = __reduce_add_sync(0xffffffffu, all);
-    if (lane == 0) sums[warp] = all;
-    __syncthreads();
-    all = 0;
+    heads = __reduce_add_sync(0xffffffffu, heads);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (entries > 32) {                 // else the first warp has seen them all
+        if (lane == 0) { sums[0][warp] = all; sums[1][warp] = heads; sums[2][warp] = most; }
+        __syncthreads();
+        all = heads = most = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps4; ++w) all += sums[w];
-    const int share = turns_of_block(all, a.blocks);
-    Run4 run = {(int)min((long long)all, (long long)blockIdx.x * share), 0, 0, 0};
-    run.to = min(all, run.from + share);
-    if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[0] = share;
-    if (run.from >= run.to && blockIdx.x != 0) return run;
+        for (int w = 0; w < kWarps4; ++w) { all += sums[0][w]; heads += sums[1][w]; most = max(most, sums[2][w]); }
+    } else {
+        if (threadIdx.x == 0) { sums[0][0] = all; sums[1][0] = heads; sums[2][0] = most; }
+        __syncthreads();
+        all = sums[0][0]; heads = sums[1][0]; most = sums[2][0];
+    }
+    Run4 run;
+    run.plan = Plan4::of(all * a.Hkv, heads * a.Hkv, most, a.blocks);
+    run.from = (int)min(0x7fffffffLL, (long long)blockIdx.x * run.plan.share);
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[0] = run.plan.apart ? -run.plan.share : run.plan.share;
     int before = 0;
     for (int e0 = 0; e0 < entries; e0 += kWarps4 * 32) {
         const int e = e0 + threadIdx.x;
-        const int n = e0 == 0 ? mine : e < entries ? Entry4(a, e, rows).turns * a.Hkv : 0;
+        const int n = run.plan.line(e0 == 0 ? mine : e < entries ? Entry4(a, e, rows).turns : 0) * a.Hkv;
         int upto = n;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -616,13 +681,13 @@ __device__ __forceinline__ Run4 run_of(const Attend4& a, int rows) {
             if (lane >= off) upto += v;
         }
         __syncthreads();                // `sums` have been read
-        if (lane == 31) sums[warp] = upto;
+        if (lane == 31) sums[0][warp] = upto;
         __syncthreads();
         int here = before - n + upto;
 #pragma unroll
         for (int w = 0; w < kWarps4; ++w) {
-            if (w < warp) here += sums[w];
-            before += sums[w];
+            if (w < warp) here += sums[0][w];
+            before += sums[0][w];
         }
         if (blockIdx.x == 0 && e < entries) a.plan[1 + e] = here;
         if (run.from >= here && run.from < here + n) {
@@ -632,6 +697,8 @@ __device__ __forceinline__ Run4 run_of(const Attend4& a, int rows) {
         if (blockIdx.x != 0 && before > run.from) break;
     }
     __syncthreads();
+    // the line's length is known where it was gone through to the end; who begins before it ends has been found
+    run.to = run.from < before ? run.from + run.plan.share : run.from;
     run.entry = found[0];
     run.offset = found[1];
     return run;
@@ -645,10 +712,12 @@ __global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_kernel(const
     extern __shared__ __align__(128) uint8_t shared[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, t = lane & 3;
     const uint32_t ring = smem_u32(shared) + warp * B::kPerWarp, q_at = smem_u32(shared) + B::kQ;
+    pdl_trigger();                      // all blocks are here at once: what joins may come as they end
     Run4 run = run_of(a, B::kRows);
     while (run.from < run.to) {
         const Entry4 entry(a, run.entry, B::kRows);
-        if (run.offset >= entry.turns * a.Hkv) {         // on to the next entry that has turns, 32 looked at together
+        const int line = run.plan.line(entry.turns);
+        if (run.offset >= line * a.Hkv) {                // on to the next entry that has turns, 32 looked at together
             const int entries = a.n_seqs * a.row_blocks;
             uint32_t some = 0;
             for (++run.entry; run.entry < entries && some == 0; run.entry += 32)
@@ -658,7 +727,12 @@ __global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_kernel(const
             run.offset = 0;
             continue;
         }
-        const int kvh = run.offset / entry.turns, skipped = run.offset - kvh * entry.turns, n_turns = min(entry.turns - skipped, run.to - run.from);
+        // the part [skipped, skipped + n_turns) of a head
+        const int kvh = run.offset / line, at_line = run.offset - kvh * line, taken = min(line - at_line, run.to - run.from);
+        const int skipped = max(0, at_line - run.plan.gap()), n_turns = min(entry.turns, at_line + taken - run.plan.gap()) - skipped;
+        run.from += taken;
+        run.offset += taken;
+        if (n_turns <= 0) continue;
         const int own = n_turns > warp ? (n_turns - warp + kWarps4 - 1) / kWarps4 : 0;
         const Head4 head = {a.table + (size_t)entry.seq * a.width, kvh, entry.start() + (skipped + warp) * kTile4, own, entry.first, entry.last};
         Turns turns;
@@ -699,7 +773,8 @@ __global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_kernel(const
             }
         // turns [inner_from, inner_to) are seen whole by every column
         const int before = entry.kv_len - entry.n_tokens;
-        const int lowest = min(entry.last, before + entry.token0), above = a.window > 0 ? before + entry.token1 - a.window - head.key0 + 1 : 0;
+        const int lowest = min(entry.last, before + entry.token0), highest = min(entry.last, before + entry.token1);
+        const int above = a.window > 0 ? before + entry.token1 - a.window - head.key0 + 1 : 0;
         const int inner_from = above > 0 ? (above + kWarps4 * kTile4 - 1) / (kWarps4 * kTile4) : 0;
         const int inner_to = lowest - head.key0 >= kTile4 - 1 ? (lowest - head.key0 - (kTile4 - 1)) / (kWarps4 * kTile4) + 1 : 0;
         __syncthreads();
@@ -711,13 +786,12 @@ __global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_kernel(const
             __syncwarp();
             if (i + B::kBuffers - 1 < own) turns.fill(a, head, i + B::kBuffers - 1, free, lane);
             cp_async_commit();
-            if (i >= inner_from && i < inner_to && !turns.holes)
-                b.template turn<false>(stage, q_at, 0, lane, [](int, int) { return true; });
-            else
-                b.template turn<true>(stage, q_at, head.key0 + i * (kWarps4 * kTile4), lane, [&](int key, int pos) {
+            b.turn(stage, q_at, lane, i < inner_from || i >= inner_to || turns.holes, [&](auto& x) {
+                b.take_edges(x, stage, head.key0 + i * (kWarps4 * kTile4), lowest, highest, a.window, lane, [&](int key) {
                     int place;
-                    return key <= pos && (a.window == 0 || key > pos - a.window) && (!turns.holes || page_of(a, head, key, place) >= 0);
+                    return !turns.holes || (key >= head.first && key <= head.last && page_of(a, head, key, place) >= 0);
                 });
+            });
             free = stage;
             stage = stage == ring + (B::kBuffers - 1) * B::kStage ? ring : stage + B::kStage;
             __syncwarp();
@@ -787,10 +861,7 @@ __global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_kernel(const
             }
         }
         __syncthreads();
-        run.from += n_turns;
-        run.offset += n_turns;
     }
-    pdl_trigger();
 }
 
 // The rows of heads that several blocks had, joined; zeros where there is no key.  A block a row and head, its warps every fourth part.
@@ -805,8 +876,9 @@ __global__ void __launch_bounds__(128) join_4bit_kernel(const Attend4 a, int D, 
     if (at < 0) return;
     float v[2][4] = {};
     if (entry.turns > 0) {
-        const int share = a.plan[0], from = a.plan[1 + seq * a.row_blocks + row / rows] + kvh * entry.turns;
-        const int block0 = from / share, parts = (from + entry.turns - 1) / share - block0 + 1;
+        const Plan4 plan = {abs(a.plan[0]), a.plan[0] < 0};
+        const int from = a.plan[1 + seq * a.row_blocks + row / rows] + kvh * plan.line(entry.turns) + plan.gap();
+        const int block0 = from / plan.share, parts = (from + entry.turns - 1) / plan.share - block0 + 1;
         if (parts == 1) return;                          // its block has written it
         const float* ml = a.sums + (size_t)2 * a.blocks * rows * D;
         // part p is block0 + p's: the first of them began the head, unless the head's first turn is the first of the block
