@@ -15,9 +15,10 @@
 // up to 8 NT rows (query heads of the kv head, tokens) and a part of the keys; its warps take runs of 32 keys in turn, each through
 // buffers of its own in shared memory, so that nobody waits for anybody until the end.  mma.sync m16n8k16 has the keys in its 16 rows for
 // the scores and the channels for the weighted sum, and the rows of the block in its 8 columns, where rows in its 16 would be mostly empty.
-// A block of 4 rows (2) stands in the columns twice (four times): the products of half (a quarter) of the groups go to each copy, so that no lane
-// computes for an empty column what belongs to a key and column: offsets, steps and least values, weights.  The weights change places
-// between the two products by movmatrix.
+// Where a head has an even number of groups, 4 rows (2) stand in 8 columns twice (four times), and a copy of a row takes every second (fourth) group:
+// no lane computes for an empty column what belongs to a group, key and column, and a 32-bit word of codes, whose halves are two
+// neighbouring groups, is an operand as it is: its halves stand in two places of the sum, of which each copy's other operand has one empty.
+// The weights change places between the two products by movmatrix.
 // (tcgen05 would want codes as bfloat16 in shared memory, which is more traffic there than all the rest; what bounds this kernel are instructions
 // on codes and bytes, not products.)
 #pragma once
@@ -81,7 +82,8 @@ struct Entry4 {
 
 // Blocks of an SM, by what registers allow: of float32 or not, with so many groups and rows of a block.
 constexpr int blocks_4bit(bool exact, int groups, int rows) {
-    return groups * (rows > 8 ? 2 : 1) >= 6 ? 2 : exact || groups * (rows > 8 ? 2 : 1) > 2 ? 3 : 4;
+    const int size = groups * (rows > 8 ? 2 : 1);
+    return size >= 6 ? 2 : exact || size > 2 ? 3 : 4;
 }
 constexpr int kLeastShare4 = 8;         // turns of a block, at least
 constexpr int kGap4 = 16;                // turns that a head's start and end are worth
@@ -162,11 +164,13 @@ template <int BYTES> __device__ __forceinline__ void load_shared(uint32_t addr, 
 
 template <typename T, int G, int NT, int COPIES>
 struct Attend4Block {
-    static_assert(G % COPIES == 0 && (NT == 1 || COPIES == 1), "copies of single columns' groups");
+    static_assert(G % COPIES == 0, "copies take groups in turn");
+    static constexpr bool kPairs = COPIES > 1;              // words of two groups as operands
     static constexpr int D = kGroup4 * G, G_ = G;
     static constexpr int kColumns = 8 / COPIES;             // rows of the block in 8 columns
     static constexpr int kRows = NT * kColumns;
-    static constexpr int GH = G / COPIES;                   // groups of a copy: copy h has h GH ..
+    static constexpr int GH = G / COPIES;                   // groups of a copy: copy h has h, h + COPIES, ..
+    static constexpr int W = kPairs ? G / 2 : G;            // accumulators of 32 channels: of two groups, one for each kind of copy, or of one
     static constexpr bool kExact = sizeof(T) == 4;          // float32: operands of the products in three bfloat16 terms, codes about zero
     static constexpr int kTerms = kExact ? 3 : 1;
     // Values keep the offset of their codes, and 136 times the sum of the weights goes through the same products to be taken off at the end: what that
@@ -224,9 +228,11 @@ struct Attend4Block {
     float q_sum[NT][GH][2];                 // sum of a column's q over a group of its copy, times 2^-24
     float to_log2[NT][2];                   // from a column's sums of products to scores in base 2
     uint32_t bf16_bits;
-    float o[NT][G][2][4];                   // [u]: channels 32 g + 4 r + 2 u, + 1 (elements 0 1, 2 3) of columns 2 t, 2 t + 1; of the columns' copies that have g
+    uint32_t first_of, second_of;           // byte selections: the first (second) of two weights, where column r's copy wants it, beside zero
+    // [w][u]: channels 4 r + 2 u, + 1 (elements 0 1, 2 3) of columns 2 t, 2 t + 1 of group w, or of group 2 w + 1 for odd copies and 2 w for even ones
+    float o[NT][W][2][4];
     float least_sum[NT][GH][2];             // this lane's part of sum_j p_j (m_j + 8 s_j)
-    float offsets[kOffsets ? GH : 1][4];    // 136 times the sums of the weights of a group of its copy
+    float offsets[NT][kOffsets ? GH : 1][4];    // 136 times the sums of the weights of a group of its copy
     float top[NT][2], total[NT][2];
     int pos[NT][2];                         // a column's position
 
@@ -241,8 +247,8 @@ struct Attend4Block {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) raw.v[n][g][e] = 0.0f;
                 if (src[n] != nullptr) {
-                    load_quad(src[n] + 32 * (copy * GH + g) + 8 * t, *reinterpret_cast<float(*)[4]>(raw.v[n][g]));
-                    load_quad(src[n] + 32 * (copy * GH + g) + 8 * t + 4, *reinterpret_cast<float(*)[4]>(raw.v[n][g] + 4));
+                    load_quad(src[n] + 32 * (copy + COPIES * g) + 8 * t, *reinterpret_cast<float(*)[4]>(raw.v[n][g]));
+                    load_quad(src[n] + 32 * (copy + COPIES * g) + 8 * t + 4, *reinterpret_cast<float(*)[4]>(raw.v[n][g] + 4));
                 }
             }
     }
@@ -272,23 +278,35 @@ struct Attend4Block {
                 float sum = 0.0f, (&v)[8] = raw.v[n][g];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] *= down;
-                // words: pairs of channels (e, 4 + e); those of odd e stand 16 times as high in the codes
+                // channels of odd number stand 16 times as high in the codes
 #pragma unroll
                 for (int term = 0; term < kTerms; ++term) {
-                    uint32_t words[4];
+                    uint32_t held[8];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float by = e % 2 ? 0.0625f : 1.0f, back = e % 2 ? 16.0f : 1.0f;
-                        words[e] = pack_f16(v[e] * by, v[4 + e] * by);
-                        const float2 held = __half22float2(*reinterpret_cast<const __half2*>(&words[e]));
-                        v[e] -= held.x * back;
-                        v[4 + e] -= held.y * back;
-                        sum += (held.x + held.y) * back;
+                    for (int e = 0; e < 8; ++e) {
+                        const __half h = __float2half_rn(v[e] * (e % 2 ? 0.0625f : 1.0f));
+                        const float back = __half2float(h) * (e % 2 ? 16.0f : 1.0f);
+                        v[e] -= back;
+                        sum += back;
+                        held[e] = __half_as_ushort(h);
                     }
+                    const uint32_t to = q_at + (term * NT + n) * G * 512 + lane * 16;
+                    if constexpr (kPairs) {
+                        // words (group pair, half of the channels): four channels each, in the half of the operand that is the copy's
 #pragma unroll
-                    for (int h = 0; h < COPIES; ++h)
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(q_at + ((term * NT + n) * G + h * GH + g) * 512 + lane * 16),
-                                     "r"(copy == h ? words[0] : 0u), "r"(copy == h ? words[1] : 0u), "r"(copy == h ? words[2] : 0u), "r"(copy == h ? words[3] : 0u) : "memory");
+                        for (int p = g * COPIES / 2; p < (g + 1) * COPIES / 2; ++p)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                uint32_t word[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) word[e] = (2 * p + (copy & 1)) % COPIES != copy ? 0u : copy & 1 ? held[4 * i + e] << 16 : held[4 * i + e];
+                                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to + (2 * p + i) * 512), "r"(word[0]), "r"(word[1]), "r"(word[2]), "r"(word[3]) : "memory");
+                            }
+                    } else {
+                        // pairs of channels (e, 4 + e)
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to + g * 512), "r"(held[0] | held[4] << 16), "r"(held[1] | held[5] << 16),
+                                     "r"(held[2] | held[6] << 16), "r"(held[3] | held[7] << 16) : "memory");
+                    }
                 }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -299,6 +317,11 @@ struct Attend4Block {
     __device__ __forceinline__ void take_q_sums(uint32_t q_at, int lane) {
         asm volatile("mov.b32 %0, 0x43004300;" : "=r"(bf16_bits));
         const int t = lane & 3;
+        if constexpr (kPairs) {
+            const bool odd = ((lane >> 2) / kColumns) & 1;
+            first_of = odd ? 0x1044u : 0x4410u;
+            second_of = odd ? 0x3244u : 0x4432u;
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(to_log2[n][0]), "=f"(to_log2[n][1]) : "r"(q_at + kQLog2 + (n * 8 + 2 * t) * 4));
@@ -316,6 +339,26 @@ struct Attend4Block {
             load_shared<16>(half + row * kRow + (((2 * t + 1) ^ turned(row)) * 16), w + 4);
         } else {
             load_shared<4 * G>(half + row * kRow + t * 4 * G, w);
+        }
+    }
+
+    // Words of channels 4 r .. + 3 for two columns of the operand: channels 2 u in its rows r, 2 u + 1 in its rows r + 8.
+    __device__ __forceinline__ void value_operands(const uint32_t (&z)[2], uint32_t (&a)[2][4]) const {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                a[u][e] = masked_or<0x000f000fu>(z[e >> 1] >> (8 * u + 4 * (e & 1)), bf16_bits);
+                if constexpr (!kOffsets) a[u][e] = centred(a[u][e]);
+            }
+    }
+    // Steps of a key in a copy's groups.
+    static __device__ __forceinline__ void load_steps(uint32_t at, int copy, uint32_t (&s)[GH]) {
+        if constexpr (kPairs) {
+#pragma unroll
+            for (int j = 0; j < GH; ++j) load_shared<4>(at + (copy + COPIES * j) * 4, s + j);
+        } else {
+            load_shared<4 * G>(at, s);
         }
     }
 
@@ -359,7 +402,7 @@ struct Attend4Block {
         __syncwarp();
     }
 
-    // Thirty-two keys.  `edge`: some column does not see some of them; edges(*this, x) then takes those scores away.
+    // Thirty-two keys.  `edge`: some column does not see some of them; edges(x) then takes those scores away.
     template <typename Edges>
     __device__ __forceinline__ void turn(uint32_t stage, uint32_t q_at, int lane, bool edge, Edges edges) {
         const int r = lane >> 2, t = lane & 3, row0 = placed(r), row1 = row0 + 8, copy = t * COPIES / 4;
@@ -367,22 +410,23 @@ struct Attend4Block {
         {
             uint32_t w[2][2][G], s[2][2][GH];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                load_keys(stage + half * kHalf, row0, t, w[half][0]);
-                load_keys(stage + half * kHalf, row1, t, w[half][1]);
-                load_shared<4 * GH>(stage + kKeySteps + half * kHalfStep + row0 * 4 * G + copy * 4 * GH, s[half][0]);
-                load_shared<4 * GH>(stage + kKeySteps + half * kHalfStep + row1 * 4 * G + copy * 4 * GH, s[half][1]);
-            }
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    load_keys(stage + half * kHalf, i ? row1 : row0, t, w[half][i]);
+                    load_steps(stage + kKeySteps + half * kHalfStep + (i ? row1 : row0) * 4 * G, copy, s[half][i]);
+                }
 #pragma unroll
             for (int j = 0; j < GH; ++j) {
                 float c[2][NT][4];
+                // of words or of groups: those whose products belong to slot j of the copies
 #pragma unroll
-                for (int h = 0; h < COPIES; ++h) {
-                    const int g = h * GH + j;
+                for (int k = kPairs ? j * COPIES : j; k < (kPairs ? (j + 1) * COPIES : j + 1); ++k) {
                     uint32_t ka[2][2][4];
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const uint32_t y[2] = {key_word(w[half][0], g), key_word(w[half][1], g)};
+                        // words: pair k / 2 of groups, half k % 2 of the channels
+                        const uint32_t y[2] = {kPairs ? w[half][0][k / 2 + k % 2 * (G / 2)] : key_word(w[half][0], k), kPairs ? w[half][1][k / 2 + k % 2 * (G / 2)] : key_word(w[half][1], k)};
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -393,10 +437,10 @@ struct Attend4Block {
 #pragma unroll
                         for (int term = kTerms - 1; term >= 0; --term) {      // the largest terms last
                             uint32_t b[4];
-                            load_shared<16>(q_at + ((term * NT + n) * G + g) * 512 + lane * 16, b);
+                            load_shared<16>(q_at + ((term * NT + n) * G + k) * 512 + lane * 16, b);
 #pragma unroll
                             for (int half = 0; half < 2; ++half) {
-                                if (h == 0 && term == kTerms - 1) mma_f16_first(c[half][n], ka[half][0], b[0], b[1]);
+                                if (k == (kPairs ? j * COPIES : j) && term == kTerms - 1) mma_f16_first(c[half][n], ka[half][0], b[0], b[1]);
                                 else mma_f16(c[half][n], ka[half][0], b[0], b[1]);
                                 mma_f16(c[half][n], ka[half][1], b[2], b[3]);
                             }
@@ -416,15 +460,14 @@ struct Attend4Block {
                     }
             }
         }
-        bool rises = false;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[half][n][e] = over_copies(x[half][n][e]) * to_log2[n][e & 1];
-        }
         if (edge) edges(x);
+        bool rises = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             // The maximum moves only when a score passes it by more than 2^8: weights stay below 2^8, float32 and bfloat16 have room for them.
@@ -448,16 +491,16 @@ struct Attend4Block {
                     for (int g = 0; g < GH; ++g) {
                         least_sum[n][g][c] *= shrink;
                         if constexpr (kOffsets) {
-                            offsets[g][c] *= shrink;
-                            offsets[g][c + 2] *= shrink;
+                            offsets[n][g][c] *= shrink;
+                            offsets[n][g][c + 2] *= shrink;
                         }
                     }
 #pragma unroll
-                    for (int g = 0; g < G; ++g)
+                    for (int w = 0; w < W; ++w)
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
-                            o[n][g][u][c] *= shrink;
-                            o[n][g][u][c + 2] *= shrink;
+                            o[n][w][u][c] *= shrink;
+                            o[n][w][u][c + 2] *= shrink;
                         }
                 }
         }
@@ -473,9 +516,9 @@ struct Attend4Block {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             uint32_t s[2][GH], va[G], vb[G], vc[G], vd[G];
-            const uint32_t values = stage + kValues + half * kHalf, steps = stage + kValueSteps + half * kHalfStep + copy * 4 * GH;
-            load_shared<4 * GH>(steps + row0 * 4 * G, s[0]);
-            load_shared<4 * GH>(steps + row1 * 4 * G, s[1]);
+            const uint32_t values = stage + kValues + half * kHalf, steps = stage + kValueSteps + half * kHalfStep;
+            load_steps(steps + row0 * 4 * G, copy, s[0]);
+            load_steps(steps + row1 * 4 * G, copy, s[1]);
             load_values(values, placed(2 * t), r, va);
             load_values(values, placed(2 * t + 1), r, vb);
             load_values(values, placed(2 * t) + 8, r, vc);
@@ -488,7 +531,7 @@ struct Attend4Block {
                     step[i] = __uint_as_float(s[i][j] << 16);
                     middle[i] = fmaf(8.0f, step[i], __uint_as_float(s[i][j] & 0xffff0000u));
                 }
-                uint32_t b0[NT][kTerms], b1[NT][kTerms];
+                uint32_t b0[NT][kTerms], b1[NT][kTerms];          // weights of keys 2 t, 2 t + 1, and of those + 8, for column r
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     float w[4];
@@ -505,29 +548,45 @@ struct Attend4Block {
 #pragma unroll
                             for (int e = 0; e < 4; ++e) w[e] -= __bfloat162float(__float2bfloat16_rn(w[e]));
                     }
+                    if constexpr (kOffsets) {
+                        const uint32_t a[4] = {0x43084308u, 0x43084308u, 0x43084308u, 0x43084308u};
+                        mma_bf16(offsets[n][j], a, b0[n][0], b1[n][0]);
+                    }
                 }
-                if constexpr (kOffsets) {
-                    const uint32_t a[4] = {0x43084308u, 0x43084308u, 0x43084308u, 0x43084308u};
-                    mma_bf16(offsets[j], a, b0[0][0], b1[0][0]);
-                }
+                if constexpr (kPairs) {
 #pragma unroll
-                for (int h = 0; h < COPIES; ++h) {
-                    const int g = h * GH + j;
-                    const uint32_t z[2] = {value_word(va, vb, g), value_word(vc, vd, g)};
-                    uint32_t a[2][4];
+                    for (int k = 0; k < 2; ++k) {                  // keys 2 t and 2 t + 8, then 2 t + 1 and 2 t + 9
+                        uint32_t c0[NT][kTerms], c1[NT][kTerms];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
+                        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            a[u][e] = masked_or<0x000f000fu>(z[e >> 1] >> (8 * u + 4 * (e & 1)), bf16_bits);
-                            if constexpr (!kOffsets) a[u][e] = centred(a[u][e]);
+                            for (int term = 0; term < kTerms; ++term) {
+                                c0[n][term] = __byte_perm(b0[n][term], 0, k ? second_of : first_of);
+                                c1[n][term] = __byte_perm(b1[n][term], 0, k ? second_of : first_of);
+                            }
+#pragma unroll
+                        for (int p = j * COPIES / 2; p < (j + 1) * COPIES / 2; ++p) {
+                            const uint32_t z[2] = {k ? vb[p] : va[p], k ? vd[p] : vc[p]};
+                            uint32_t a[2][4];
+                            value_operands(z, a);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int term = kTerms - 1; term >= 0; --term)
+#pragma unroll
+                                    for (int u = 0; u < 2; ++u) mma_bf16(o[n][p][u], a[u], c0[n][term], c1[n][term]);
                         }
+                    }
+                } else {
+                    const uint32_t z[2] = {value_word(va, vb, j), value_word(vc, vd, j)};
+                    uint32_t a[2][4];
+                    value_operands(z, a);
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int term = kTerms - 1; term >= 0; --term)
 #pragma unroll
-                            for (int u = 0; u < 2; ++u) mma_bf16(o[n][g][u], a[u], b0[n][term], b1[n][term]);
+                            for (int u = 0; u < 2; ++u) mma_bf16(o[n][j][u], a[u], b0[n][term], b1[n][term]);
                 }
             }
         }
@@ -740,7 +799,7 @@ __global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_kernel(const
         const T* src[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const long at = entry.row_at(a, kvh, 8 * n + r % B::kColumns);
+            const long at = entry.row_at(a, kvh, B::kColumns * n + r % B::kColumns);
             src[n] = at < 0 ? nullptr : reinterpret_cast<const T*>(a.q) + at * D;
         }
         typename B::RawQ raw;
@@ -758,18 +817,18 @@ __global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_kernel(const
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int group = a.Hq / a.Hkv;
-                b.pos[n][c] = min(entry.last, entry.kv_len - entry.n_tokens + min(entry.n_tokens - 1, (entry.row0 + 8 * n + (2 * t + c) % B::kColumns) / group));
+                b.pos[n][c] = min(entry.last, entry.kv_len - entry.n_tokens + min(entry.n_tokens - 1, (entry.row0 + B::kColumns * n + (2 * t + c) % B::kColumns) / group));
                 b.top[n][c] = kLowest4;
                 b.total[n][c] = 0.0f;
 #pragma unroll
                 for (int g = 0; g < B::GH; ++g) {
                     b.least_sum[n][g][c] = 0.0f;
-                    if (B::kOffsets) b.offsets[g][c] = b.offsets[g][c + 2] = 0.0f;
+                    if (B::kOffsets) b.offsets[n][g][c] = b.offsets[n][g][c + 2] = 0.0f;
                 }
 #pragma unroll
-                for (int g = 0; g < G; ++g)
+                for (int w = 0; w < B::W; ++w)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) b.o[n][g][u][c] = b.o[n][g][u][c + 2] = 0.0f;
+                    for (int u = 0; u < 2; ++u) b.o[n][w][u][c] = b.o[n][w][u][c + 2] = 0.0f;
             }
         // turns [inner_from, inner_to) are seen whole by every column
         const int before = entry.kv_len - entry.n_tokens;
@@ -796,7 +855,6 @@ __global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_kernel(const
             stage = stage == ring + (B::kBuffers - 1) * B::kStage ? ring : stage + B::kStage;
             __syncwarp();
         }
-
         cp_async_wait<0>();
         __syncwarp();
         // The warp's sums to its own shared memory (the ring is done with): [column][D], then maxima and totals.
@@ -805,7 +863,7 @@ __global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_kernel(const
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const int column = 8 * n + (2 * t + c) % B::kColumns, copy = t * COPIES / 4;
+                const int column = B::kColumns * n + (2 * t + c) % B::kColumns, copy = t * COPIES / 4;
                 float total = b.total[n][c];
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
@@ -815,14 +873,15 @@ __global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_kernel(const
                     least[j] = b.least_sum[n][j][c];
 #pragma unroll
                     for (int off = 4; off < 32; off <<= 1) least[j] += __shfl_xor_sync(0xffffffffu, least[j], off);
-                    if (B::kOffsets) least[j] -= b.offsets[j][c];
+                    if (B::kOffsets) least[j] -= b.offsets[n][j][c];
                 }
 #pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const float m = least[g % B::GH];
-                    if (copy == g / B::GH)
+                for (int w = 0; w < B::W; ++w) {
+                    const int g = B::kPairs ? 2 * w + (copy & 1) : w;
+                    const float m = least[B::kPairs ? 2 * w / COPIES : w];
+                    if (!B::kPairs || g % COPIES == copy)
                         *reinterpret_cast<float4*>(mine + column * D + 32 * g + 4 * r) =
-                            make_float4(b.o[n][g][0][c] + m, b.o[n][g][0][c + 2] + m, b.o[n][g][1][c] + m, b.o[n][g][1][c + 2] + m);
+                            make_float4(b.o[n][w][0][c] + m, b.o[n][w][0][c + 2] + m, b.o[n][w][1][c] + m, b.o[n][w][1][c + 2] + m);
                 }
                 if (r == 0 && copy == 0) {
                     mine[B::kRows * D + 2 * column] = b.top[n][c];
@@ -940,12 +999,12 @@ int launch_attend_4bit(const Attend4& a, int most_tokens, cudaStream_t stream) {
 
 template <typename T, int G, template <typename> class Turns>
 int launch_attend_4bit_of(const Attend4& a, int rows, int most_tokens, cudaStream_t stream) {
-    if constexpr (sizeof(T) == 2 && G <= 4)
-        if (rows == 16) return launch_attend_4bit<T, G, 2, 1, Turns>(a, most_tokens, stream);
     if constexpr (G % 4 == 0)
         if (rows == 2) return launch_attend_4bit<T, G, 1, 4, Turns>(a, most_tokens, stream);
     if constexpr (G % 2 == 0)
         if (rows == 4) return launch_attend_4bit<T, G, 1, 2, Turns>(a, most_tokens, stream);
+    if constexpr (sizeof(T) == 2 && G <= 4)
+        if (rows == 16) return launch_attend_4bit<T, G, 2, 1, Turns>(a, most_tokens, stream);
     return rows == 8 ? launch_attend_4bit<T, G, 1, 1, Turns>(a, most_tokens, stream) : PB_ERR_BAD_SIZE;
 }
 
