@@ -141,12 +141,166 @@ __global__ void qk_norm_rope_write_4bit_kernel(const T* __restrict__ qkv, T* __r
     for (int j = 0; j < QUADS; ++j) quantise_quad(y[j], lane + 32 * j, D / kGroup4, at, is_k ? k_pool : v_pool);
 }
 
-// Eight channels of a row a thread: two words of codes and one of steps, 16 or 32 bytes of values.
-template <typename T>
-__global__ void expand_pages_4bit_kernel(Pool4 k_pool, Pool4 v_pool, const int* __restrict__ table, const int* __restrict__ kv_len, T* __restrict__ k_out,
-                                         T* __restrict__ v_out, int* __restrict__ table_out, int width, int Hkv, int D, int page_size, int n_pages,
-                                         const int* __restrict__ cu_q, int window, const PoolBounds bounds) {
+// qk_norm_rope_write_4bit where a head is 4, 8, 16 or 32 lanes of eight neighbouring channels and all of them turn, or none: as many heads a warp as fit, the other
+// half of a turn L / 2 lanes away, a group in four lanes.  What bounds it are instructions, half of them on the keys' 64-bit arithmetic.
+template <int L> struct Lanes {
+    static __device__ __forceinline__ uint32_t mask(int lane) { return L == 32 ? 0xffffffffu : ((1u << L) - 1u) << (lane & ~(L - 1) & 31); }
+};
+template <int L, typename A> __device__ __forceinline__ A sum_of_lanes(A v, uint32_t mask) {
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
+    return v;
+}
+__device__ __forceinline__ void load_octet(const float* p, float (&v)[8]) {
+    load_quad(p, *reinterpret_cast<float(*)[4]>(v));
+    load_quad(p + 4, *reinterpret_cast<float(*)[4]>(v + 4));
+}
+__device__ __forceinline__ void load_octet(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void store_octet(float* p, const float (&v)[8]) {
+    store_quad(p, *reinterpret_cast<const float(*)[4]>(v));
+    store_quad(p + 4, *reinterpret_cast<const float(*)[4]>(v + 4));
+}
+__device__ __forceinline__ void store_octet(__nv_bfloat16* p, const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename A, int L>
+__device__ __forceinline__ void norm_and_turn_octet(const float (&f)[8], const float* __restrict__ weight, double eps, const float* __restrict__ cos_t,
+                                                    const float* __restrict__ sin_t, bool turns, int l, uint32_t mask, A (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = (A)f[e];
+    if (weight != nullptr) {
+        A ss = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+        const A r = root_inverse(sum_of_lanes<L>(ss, mask) / (A)(8 * L) + (A)eps);
+        float w[8];
+        load_octet(weight + 8 * l, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = x[e] * r * (A)w[e];
+    }
+    if (!turns) return;
+    const int at = 8 * (l & (L / 2 - 1));
+    float c[8], s[8];
+    load_octet(cos_t + at, c);
+    load_octet(sin_t + at, s);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const A other = __shfl_xor_sync(mask, x[e], L / 2), turned = other * (A)s[e];
+        x[e] = l < L / 2 ? x[e] * (A)c[e] - turned : x[e] * (A)c[e] + turned;
+    }
+}
+
+// A lane's eight values of a group, four lanes a group, to codes and steps at row `at` of a pool (quantise_quad has the arithmetic).
+template <int G>
+__device__ __forceinline__ void quantise_octet(const float (&y)[8], int l, uint32_t mask, size_t at, const Pool4& pool) {
+    constexpr float kMost = 3.38953139e38f;
+    float lo = y[0], hi = y[0];
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        lo = fminf(lo, y[e]);
+        hi = fmaxf(hi, y[e]);
+        bad |= !(fabsf(y[e]) <= kMost);
+    }
+    if (bad) hi = __int_as_float(0x7f800000);
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
+    }
+    bad = hi > kMost;
+    const double m = (double)__bfloat162float(__float2bfloat16_rd(lo));
+    const float step = __bfloat162float(__float2bfloat16_ru(__double2float_ru(((double)hi - m) / 15.0)));
+    const double s = (double)step, inverse = step > 0.0f ? 1.0 / s : 0.0;
+    uint32_t words = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const double d = (double)y[e] - m;
+        double c = d * inverse;
+        c = fma(fma(-c, s, d), inverse, c);              // the quotient as a division would round it
+        words |= (uint32_t)min(15, __double2int_rn(c)) << (4 * e);
+    }
+    if (bad) words = 0;
+    const int g = l >> 2, t = l & 3;
+    uint16_t* row = reinterpret_cast<uint16_t*>(pool.codes) + at * (size_t)(8 * G) + g;
+    row[2 * t * G] = (uint16_t)words;
+    row[(2 * t + 1) * G] = (uint16_t)(words >> 16);
+    if (t == 0) {
+        const uint32_t two = (__float_as_uint(step) >> 16) | (__float_as_uint((float)m) & 0xffff0000u);
+        reinterpret_cast<uint32_t*>(pool.steps)[at * (size_t)G + g] = bad ? 0x7fc07fc0u : two;
+    }
+}
+
+template <typename T, int G>
+__global__ void __launch_bounds__(128) write_lanes_4bit_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, Pool4 k_pool, Pool4 v_pool, const int* __restrict__ slots,
+                                                               const float* __restrict__ cos_t, const float* __restrict__ sin_t, const float* __restrict__ q_weight,
+                                                               const float* __restrict__ k_weight, double eps, int Hq, int Hkv, int turns, int page_size, int n_pages,
+                                                               const PoolBounds bounds) {
     pdl_wait();
+    constexpr int D = kGroup4 * G, L = D / 8;
+    const int lane = threadIdx.x & 31, l = lane & (L - 1), t = blockIdx.x;
+    const int head = blockIdx.y * (128 / L) + threadIdx.x / L;
+    if (head >= Hq + 2 * Hkv) return;
+    const uint32_t mask = Lanes<L>::mask(lane);
+    const float *c = cos_t + (size_t)t * (D / 2) * turns, *s = sin_t + (size_t)t * (D / 2) * turns;
+    float y[8];
+    load_octet(qkv + ((size_t)t * (Hq + 2 * Hkv) + head) * D + 8 * l, y);
+    if (head < Hq) {
+        float x[8];
+        norm_and_turn_octet<float, L>(y, q_weight, eps, c, s, turns, l, mask, x);
+        store_octet(q_out + ((size_t)t * Hq + head) * D + 8 * l, x);
+        return;
+    }
+    const int slot = slots[t];
+    if (slot < 0 || !slot_ok(slot, page_size, bounds) || page_or_none(slot / page_size, n_pages) < 0) return;
+    const bool is_k = head < Hq + Hkv;
+    const int h = is_k ? head - Hq : head - Hq - Hkv;
+    const size_t at = ((size_t)(slot / page_size) * Hkv + h) * page_size + slot % page_size;
+    if (is_k) {
+        double x[8];
+        norm_and_turn_octet<double, L>(y, k_weight, eps, c, s, turns, l, mask, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = to_float(from_float<T>((float)x[e]));
+    }
+    quantise_octet<G>(y, l, mask, at, is_k ? k_pool : v_pool);
+}
+
+// N neighbouring words, aligned to as many of them as make 16, 8 or 4 bytes.
+template <int N> __device__ __forceinline__ void load_words(const uint32_t* __restrict__ p, uint32_t (&w)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) *reinterpret_cast<uint4*>(w + 4 * i) = *reinterpret_cast<const uint4*>(p + 4 * i);
+    } else if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) *reinterpret_cast<uint2*>(w + 2 * i) = *reinterpret_cast<const uint2*>(p + 2 * i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = p[i];
+    }
+}
+
+// A lane takes the codes of channels 8 t .. + 7 of all groups of a row, side by side in the pool, and writes eight values of every group.
+template <typename T, int G>
+__global__ void __launch_bounds__(256) expand_pages_4bit_kernel(Pool4 k_pool, Pool4 v_pool, const int* __restrict__ table, const int* __restrict__ kv_len,
+                                                                T* __restrict__ k_out, T* __restrict__ v_out, int* __restrict__ table_out, int width, int Hkv,
+                                                                int page_size, int n_pages, const int* __restrict__ cu_q, int window, const PoolBounds bounds) {
+    pdl_wait();
+    constexpr int D = kGroup4 * G;
     const int seq = blockIdx.y, logical = blockIdx.x, length = kv_len[seq];
     const size_t out_page = (size_t)seq * width + logical;
     int rows = min(page_size, length - logical * page_size);                    // of this page, that hold a key
@@ -161,25 +315,34 @@ __global__ void expand_pages_4bit_kernel(Pool4 k_pool, Pool4 v_pool, const int* 
     }
     if (blockIdx.z == 0 && threadIdx.x == 0) table_out[out_page] = there ? (int)out_page : -1;
     if (!there) return;
-    const int G = D / kGroup4, octets = D / 8, per_head = page_size * octets, n = 2 * Hkv * per_head;
+    const int per_pool = Hkv * page_size, n = 2 * per_pool * 4;
+    const bool partly = rows < page_size;
     for (int i = blockIdx.z * blockDim.x + threadIdx.x; i < n; i += gridDim.z * blockDim.x) {
-        const bool is_v = i >= Hkv * per_head;
-        const int rest = is_v ? i - Hkv * per_head : i, row = rest / octets, o = rest - row * octets;      // row: head * page_size + place
+        const int t = i & 3, both = i >> 2;
+        const bool is_v = both >= per_pool;
+        const int row = is_v ? both - per_pool : both;                          // head * page_size + place
         const Pool4& pool = is_v ? v_pool : k_pool;
-        const int g = o >> 2, r = (o & 3) * 2;
-        const size_t in_pool = (size_t)page * Hkv * page_size + row;
-        float y[2][4] = {};
-        if (row % page_size < rows) {
-            const uint16_t* codes = reinterpret_cast<const uint16_t*>(pool.codes) + in_pool * (size_t)(8 * G);
-            const uint32_t two = reinterpret_cast<const uint32_t*>(pool.steps)[in_pool * (size_t)G + g];
-            const float step = __uint_as_float(two << 16), least = __uint_as_float(two & 0xffff0000u);
-            const uint32_t words = codes[r * G + g] | (uint32_t)codes[(r + 1) * G + g] << 16;
+        T* dst = (is_v ? v_out : k_out) + (out_page * per_pool + row) * D + 8 * t;
+        if (partly && row % page_size >= rows) {
+            const float zero[8] = {};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e >> 2][e & 3] = fmaf(step, (float)((words >> (4 * e)) & 15), least);
+            for (int g = 0; g < G; ++g) store_octet(dst + 32 * g, zero);
+            continue;
         }
-        T* dst = (is_v ? v_out : k_out) + (out_page * Hkv * page_size + row) * D + 8 * o;
-        store_quad(dst, y[0]);
-        store_quad(dst + 4, y[1]);
+        const size_t in_pool = (size_t)page * per_pool + row;
+        uint32_t w[G], two[G];
+        load_words<G>(reinterpret_cast<const uint32_t*>(pool.codes) + (in_pool * 4 + t) * G, w);
+        load_words<G>(reinterpret_cast<const uint32_t*>(pool.steps) + in_pool * G, two);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const float step = __uint_as_float(two[g] << 16), least = __uint_as_float(two[g] & 0xffff0000u);
+            // 16-bit words g and G + g of the lane's 2 G
+            const uint32_t sel = ((g & 1) ? 0x0032u : 0x0010u) | (((G + g) & 1) ? 0x7600u : 0x5400u), word = __byte_perm(w[g >> 1], w[(G + g) >> 1], sel);
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = fmaf(step, __uint_as_float(((word >> (4 * e)) & 15) | 0x4b000000u) - 8388608.0f, least);
+            store_octet(dst + 32 * g, y);
+        }
     }
 }
 
@@ -189,9 +352,34 @@ int launch_write(const void* qkv, void* q_out, const Pool4& k, const Pool4& v, c
     constexpr int kWarps = 4;
     const dim3 grid(n, (Hq + 2 * Hkv + kWarps - 1) / kWarps);
     const size_t smem = (size_t)kWarps * D * sizeof(double);
+    const bool whole = rotary == 0 || rotary == D, aligned = (((size_t)cos_t | (size_t)sin_t | (size_t)qw | (size_t)kw) & 15) == 0;
+    if ((D & (D - 1)) == 0 && whole && aligned) {
+        auto lanes = D == 32 ? write_lanes_4bit_kernel<T, 1> : D == 64 ? write_lanes_4bit_kernel<T, 2> : D == 128 ? write_lanes_4bit_kernel<T, 4> : write_lanes_4bit_kernel<T, 8>;
+        const int heads = 128 / (D / 8);
+        return launch_pdl(lanes, dim3(n, (Hq + 2 * Hkv + heads - 1) / heads), dim3(128), 0, stream, (const T*)qkv, (T*)q_out, k, v, slots, cos_t, sin_t, qw, kw, eps, Hq, Hkv,
+                          rotary > 0 ? 1 : 0, page_size, n_pages, pool_bounds_now());
+    }
     auto kernel = D <= 128 ? qk_norm_rope_write_4bit_kernel<T, 1> : qk_norm_rope_write_4bit_kernel<T, 2>;
     return launch_pdl(kernel, grid, dim3(kWarps * 32), smem, stream, (const T*)qkv, (T*)q_out, k, v, slots, cos_t, sin_t, qw, kw, eps, Hq, Hkv, D, rotary, page_size,
                       n_pages, pool_bounds_now());
+}
+
+template <typename T, int G>
+int launch_expand_of(const Pool4& k, const Pool4& v, const int* table, const int* kv_len, void* k_out, void* v_out, int* table_out, int n_seqs, int width, int Hkv,
+                     int page_size, int n_pages, const int* cu_q, int window, cudaStream_t stream) {
+    const int units = 2 * Hkv * page_size * 4, blocks = (units + 511) / 512;
+    return launch_pdl(expand_pages_4bit_kernel<T, G>, dim3(width, n_seqs, blocks < 64 ? blocks : 64), dim3(256), 0, stream, k, v, table, kv_len, (T*)k_out, (T*)v_out,
+                      table_out, width, Hkv, page_size, n_pages, cu_q, window, pool_bounds_now());
+}
+template <typename T>
+int launch_expand(int groups, const Pool4& k, const Pool4& v, const int* table, const int* kv_len, void* k_out, void* v_out, int* table_out, int n_seqs, int width, int Hkv,
+                  int page_size, int n_pages, const int* cu_q, int window, cudaStream_t stream) {
+    switch (groups) {
+#define PB_EXPAND(g) case g: return launch_expand_of<T, g>(k, v, table, kv_len, k_out, v_out, table_out, n_seqs, width, Hkv, page_size, n_pages, cu_q, window, stream);
+        PB_EXPAND(1) PB_EXPAND(2) PB_EXPAND(3) PB_EXPAND(4) PB_EXPAND(5) PB_EXPAND(6) PB_EXPAND(7) PB_EXPAND(8)
+#undef PB_EXPAND
+    }
+    return PB_ERR_BAD_SIZE;
 }
 
 bool sizes_4bit(int Hkv, int D, int page_size, int n_pages) {
@@ -218,16 +406,12 @@ PB_EXPORT int pb_expand_pages_4bit(int dtype, void* k_codes, void* k_steps, void
                                    int* table_out, int n_seqs, int width, int Hkv, int D, int page_size, int n_pages, const int* cu_q, int window,
                                    cudaStream_t stream) {
     if (!sizes_4bit(Hkv, D, page_size, n_pages) || n_seqs < 0 || width < 0 || window < 0) return PB_ERR_BAD_SIZE;
-    if (n_seqs > 65535 || (long long)n_seqs * width > 0x7fffffffLL || 2LL * Hkv * page_size * (D / 8) > 0x3fffffffLL) return PB_ERR_TOO_LARGE;
+    if (n_seqs > 65535 || (long long)n_seqs * width > 0x7fffffffLL || 8LL * Hkv * page_size > 0x3fffffffLL) return PB_ERR_TOO_LARGE;
     if (n_seqs == 0 || width == 0) return 0;
     const Pool4 k{(uint8_t*)k_codes, (__nv_bfloat16*)k_steps}, v{(uint8_t*)v_codes, (__nv_bfloat16*)v_steps};
-    const int units = 2 * Hkv * page_size * (D / 8), blocks = (units + 1023) / 1024;
-    const dim3 grid(width, n_seqs, blocks < 64 ? blocks : 64);
     if (dtype == PB_F32)
-        return launch_pdl(expand_pages_4bit_kernel<float>, grid, dim3(256), 0, stream, k, v, table, kv_len, (float*)k_out, (float*)v_out, table_out, width, Hkv, D,
-                          page_size, n_pages, cu_q, window, pool_bounds_now());
+        return launch_expand<float>(D / kGroup4, k, v, table, kv_len, k_out, v_out, table_out, n_seqs, width, Hkv, page_size, n_pages, cu_q, window, stream);
     if (dtype == PB_BF16)
-        return launch_pdl(expand_pages_4bit_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, k, v, table, kv_len, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out,
-                          table_out, width, Hkv, D, page_size, n_pages, cu_q, window, pool_bounds_now());
+        return launch_expand<__nv_bfloat16>(D / kGroup4, k, v, table, kv_len, k_out, v_out, table_out, n_seqs, width, Hkv, page_size, n_pages, cu_q, window, stream);
     return PB_ERR_BAD_DTYPE;
 }
