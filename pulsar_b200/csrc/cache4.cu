@@ -64,7 +64,7 @@ __device__ __forceinline__ void norm_and_turn(const T* __restrict__ src, const f
 
 // A lane's four values of a group, eight lanes a group, to codes and steps at row `at` of a pool.  The steps and codes are found in 64 bits: a
 // value next to the border of two codes falls where the formula has it.
-__device__ __forceinline__ void quantise_quad(const float (&y)[4], int quad, int groups, size_t at, const Pool4& pool) {
+__device__ __forceinline__ void quantise_quad(const float (&y)[4], int quad, int own, int groups, size_t at, const Pool4& pool) {
     float lo = fminf(fminf(y[0], y[1]), fminf(y[2], y[3])), hi = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
     constexpr float kMost = 3.38953139e38f;          // the largest bfloat16
 #pragma unroll
@@ -75,7 +75,7 @@ __device__ __forceinline__ void quantise_quad(const float (&y)[4], int quad, int
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
-    if (4 * quad >= kGroup4 * groups) return;
+    if (4 * quad >= kGroup4 * own) return;              // a lane without channels
     const bool bad = hi > kMost;
     const double m = (double)__bfloat162float(__float2bfloat16_rd(lo));
     const float step = __bfloat162float(__float2bfloat16_ru(__double2float_ru(((double)hi - m) / 15.0)));
@@ -124,7 +124,8 @@ __global__ void qk_norm_rope_write_4bit_kernel(const T* __restrict__ qkv, T* __r
     const bool is_k = head < Hq + Hkv;
     const int h = is_k ? head - Hq : head - Hq - Hkv;
     const size_t at = ((size_t)(slot / page_size) * Hkv + h) * page_size + slot % page_size;
-    float y[QUADS][4];
+    const Pool4 pool = {is_k ? k_pool.codes : v_pool.codes, is_k ? k_pool.steps : v_pool.steps};
+    float y[QUADS][4] = {};
     if (is_k) {
         double x[QUADS][4];
         norm_and_turn<double>(src, k_weight, eps, c, s, D, rotary, lane, shared + (size_t)warp * D, x);
@@ -138,35 +139,20 @@ __global__ void qk_norm_rope_write_4bit_kernel(const T* __restrict__ qkv, T* __r
             if (4 * (lane + 32 * j) < D) load_quad(src + 4 * (lane + 32 * j), y[j]);
     }
 #pragma unroll
-    for (int j = 0; j < QUADS; ++j) quantise_quad(y[j], lane + 32 * j, D / kGroup4, at, is_k ? k_pool : v_pool);
+    for (int j = 0; j < QUADS; ++j) quantise_quad(y[j], lane + 32 * j, D / kGroup4, D / kGroup4, at, pool);
 }
 
-// qk_norm_rope_write_4bit where a head is 4, 8, 16 or 32 lanes of eight neighbouring channels and all of them turn, or none: as many heads a warp as fit, the other
-// half of a turn L / 2 lanes away, a group in four lanes.  What bounds it are instructions, half of them on the keys' 64-bit arithmetic.
-template <int L> struct Lanes {
-    static __device__ __forceinline__ uint32_t mask(int lane) { return L == 32 ? 0xffffffffu : ((1u << L) - 1u) << (lane & ~(L - 1) & 31); }
-};
-template <int L, typename A> __device__ __forceinline__ A sum_of_lanes(A v, uint32_t mask) {
+// qk_norm_rope_write_4bit where a head is 8, 16 or 32 lanes of four channels of its first half and the same four of its second, and all of them turn, or
+// none: both ends of a turn are in one lane, as many heads a warp as fit, a group in eight lanes.  What bounds it are instructions, half of
+// them on the keys' 64-bit arithmetic.
+template <int L, typename A> __device__ __forceinline__ A sum_of_lanes(A v) {
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
+    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-__device__ __forceinline__ void load_octet(const float* p, float (&v)[8]) {
-    load_quad(p, *reinterpret_cast<float(*)[4]>(v));
-    load_quad(p + 4, *reinterpret_cast<float(*)[4]>(v + 4));
-}
-__device__ __forceinline__ void load_octet(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-}
 __device__ __forceinline__ void store_octet(float* p, const float (&v)[8]) {
-    store_quad(p, *reinterpret_cast<const float(*)[4]>(v));
-    store_quad(p + 4, *reinterpret_cast<const float(*)[4]>(v + 4));
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
 }
 __device__ __forceinline__ void store_octet(__nv_bfloat16* p, const float (&v)[8]) {
     uint32_t w[4];
@@ -178,106 +164,94 @@ __device__ __forceinline__ void store_octet(__nv_bfloat16* p, const float (&v)[8
     *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+struct Turn4 {
+    float w[2][4], c[4], s[4];
+    bool norm, turns;
+    template <int L> __device__ __forceinline__ void load_weight(const float* __restrict__ weight, int l) {
+        norm = weight != nullptr;
+        if (norm) {
+            load_quad(weight + 4 * l, w[0]);
+            load_quad(weight + 4 * (L + l), w[1]);
+        }
+    }
+};
 template <typename A, int L>
-__device__ __forceinline__ void norm_and_turn_octet(const float (&f)[8], const float* __restrict__ weight, double eps, const float* __restrict__ cos_t,
-                                                    const float* __restrict__ sin_t, bool turns, int l, uint32_t mask, A (&x)[8]) {
+__device__ __forceinline__ void norm_and_turn_pair(const float (&f)[2][4], const Turn4& t, double eps, A (&x)[2][4]) {
+    A ss = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = (A)f[e];
-    if (weight != nullptr) {
-        A ss = 0;
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
-        const A r = root_inverse(sum_of_lanes<L>(ss, mask) / (A)(8 * L) + (A)eps);
-        float w[8];
-        load_octet(weight + 8 * l, w);
+        for (int e = 0; e < 4; ++e) {
+            x[i][e] = (A)f[i][e];
+            if (t.norm) ss += x[i][e] * x[i][e];
+        }
+    if (t.norm) {
+        const A r = root_inverse(sum_of_lanes<L>(ss) / (A)(8 * L) + (A)eps);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * r * (A)w[e];
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[i][e] = x[i][e] * r * (A)t.w[i][e];
     }
-    if (!turns) return;
-    const int at = 8 * (l & (L / 2 - 1));
-    float c[8], s[8];
-    load_octet(cos_t + at, c);
-    load_octet(sin_t + at, s);
+    if (!t.turns) return;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const A other = __shfl_xor_sync(mask, x[e], L / 2), turned = other * (A)s[e];
-        x[e] = l < L / 2 ? x[e] * (A)c[e] - turned : x[e] * (A)c[e] + turned;
-    }
-}
-
-// A lane's eight values of a group, four lanes a group, to codes and steps at row `at` of a pool (quantise_quad has the arithmetic).
-template <int G>
-__device__ __forceinline__ void quantise_octet(const float (&y)[8], int l, uint32_t mask, size_t at, const Pool4& pool) {
-    constexpr float kMost = 3.38953139e38f;
-    float lo = y[0], hi = y[0];
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        lo = fminf(lo, y[e]);
-        hi = fmaxf(hi, y[e]);
-        bad |= !(fabsf(y[e]) <= kMost);
-    }
-    if (bad) hi = __int_as_float(0x7f800000);
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
-    }
-    bad = hi > kMost;
-    const double m = (double)__bfloat162float(__float2bfloat16_rd(lo));
-    const float step = __bfloat162float(__float2bfloat16_ru(__double2float_ru(((double)hi - m) / 15.0)));
-    const double s = (double)step, inverse = step > 0.0f ? 1.0 / s : 0.0;
-    uint32_t words = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const double d = (double)y[e] - m;
-        double c = d * inverse;
-        c = fma(fma(-c, s, d), inverse, c);              // the quotient as a division would round it
-        words |= (uint32_t)min(15, __double2int_rn(c)) << (4 * e);
-    }
-    if (bad) words = 0;
-    const int g = l >> 2, t = l & 3;
-    uint16_t* row = reinterpret_cast<uint16_t*>(pool.codes) + at * (size_t)(8 * G) + g;
-    row[2 * t * G] = (uint16_t)words;
-    row[(2 * t + 1) * G] = (uint16_t)(words >> 16);
-    if (t == 0) {
-        const uint32_t two = (__float_as_uint(step) >> 16) | (__float_as_uint((float)m) & 0xffff0000u);
-        reinterpret_cast<uint32_t*>(pool.steps)[at * (size_t)G + g] = bad ? 0x7fc07fc0u : two;
+    for (int e = 0; e < 4; ++e) {
+        const A u = x[0][e], v = x[1][e];
+        x[0][e] = u * (A)t.c[e] - v * (A)t.s[e];
+        x[1][e] = v * (A)t.c[e] + u * (A)t.s[e];
     }
 }
 
 template <typename T, int G>
-__global__ void __launch_bounds__(128) write_lanes_4bit_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, Pool4 k_pool, Pool4 v_pool, const int* __restrict__ slots,
+__global__ void __launch_bounds__(128, 10) write_lanes_4bit_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, Pool4 k_pool, Pool4 v_pool, const int* __restrict__ slots,
                                                                const float* __restrict__ cos_t, const float* __restrict__ sin_t, const float* __restrict__ q_weight,
                                                                const float* __restrict__ k_weight, double eps, int Hq, int Hkv, int turns, int page_size, int n_pages,
                                                                const PoolBounds bounds) {
     pdl_wait();
     constexpr int D = kGroup4 * G, L = D / 8;
-    const int lane = threadIdx.x & 31, l = lane & (L - 1), t = blockIdx.x;
-    const int head = blockIdx.y * (128 / L) + threadIdx.x / L;
-    if (head >= Hq + 2 * Hkv) return;
-    const uint32_t mask = Lanes<L>::mask(lane);
-    const float *c = cos_t + (size_t)t * (D / 2) * turns, *s = sin_t + (size_t)t * (D / 2) * turns;
-    float y[8];
-    load_octet(qkv + ((size_t)t * (Hq + 2 * Hkv) + head) * D + 8 * l, y);
-    if (head < Hq) {
-        float x[8];
-        norm_and_turn_octet<float, L>(y, q_weight, eps, c, s, turns, l, mask, x);
-        store_octet(q_out + ((size_t)t * Hq + head) * D + 8 * l, x);
+    const int l = threadIdx.x & (L - 1);
+    // a block is of queries, keys or values alone; lanes of heads that there are not only keep their neighbours company
+    constexpr int kHeads = 128 / L;
+    const int kv_blocks = (Hkv + kHeads - 1) / kHeads;                  // keys first: their blocks take longest
+    const int section = (int)blockIdx.y < kv_blocks ? 1 : (int)blockIdx.y < 2 * kv_blocks ? 2 : 0;
+    const int h = ((int)blockIdx.y - (section == 1 ? 0 : section == 2 ? kv_blocks : 2 * kv_blocks)) * kHeads + threadIdx.x / L;
+    const bool there = h < (section == 0 ? Hq : Hkv);
+    const int head = (there ? h : 0) + (section == 0 ? 0 : section == 1 ? Hq : Hq + Hkv);
+    const Pool4 pool = {section == 1 ? k_pool.codes : v_pool.codes, section == 1 ? k_pool.steps : v_pool.steps};
+    Turn4 turn;
+    turn.turns = section < 2 && turns;
+    turn.load_weight<L>(section == 0 ? q_weight : section == 1 ? k_weight : nullptr, l);
+    const int t = blockIdx.x;
+    float y[2][4];
+    const T* src = qkv + ((size_t)t * (Hq + 2 * Hkv) + head) * D + 4 * l;
+    load_quad(src, y[0]);
+    load_quad(src + D / 2, y[1]);
+    if (turn.turns) {
+        load_quad(cos_t + (size_t)t * (D / 2) + 4 * l, turn.c);
+        load_quad(sin_t + (size_t)t * (D / 2) + 4 * l, turn.s);
+    }
+    if (section == 0) {
+        float x[2][4];
+        norm_and_turn_pair<float, L>(y, turn, eps, x);
+        T* dst = q_out + ((size_t)t * Hq + h) * D + 4 * l;
+        if (there) {
+            store_quad(dst, x[0]);
+            store_quad(dst + D / 2, x[1]);
+        }
         return;
     }
     const int slot = slots[t];
     if (slot < 0 || !slot_ok(slot, page_size, bounds) || page_or_none(slot / page_size, n_pages) < 0) return;
-    const bool is_k = head < Hq + Hkv;
-    const int h = is_k ? head - Hq : head - Hq - Hkv;
     const size_t at = ((size_t)(slot / page_size) * Hkv + h) * page_size + slot % page_size;
-    if (is_k) {
-        double x[8];
-        norm_and_turn_octet<double, L>(y, k_weight, eps, c, s, turns, l, mask, x);
+    if (section == 1) {
+        double x[2][4];
+        norm_and_turn_pair<double, L>(y, turn, eps, x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = to_float(from_float<T>((float)x[e]));
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[i][e] = to_float(from_float<T>((float)x[i][e]));
     }
-    quantise_octet<G>(y, l, mask, at, is_k ? k_pool : v_pool);
+    quantise_quad(y[0], l, there ? G : 0, G, at, pool);
+    quantise_quad(y[1], L + l, there ? G : 0, G, at, pool);
 }
 
 // N neighbouring words, aligned to as many of them as make 16, 8 or 4 bytes.
@@ -321,7 +295,7 @@ __global__ void __launch_bounds__(256) expand_pages_4bit_kernel(Pool4 k_pool, Po
         const int t = i & 3, both = i >> 2;
         const bool is_v = both >= per_pool;
         const int row = is_v ? both - per_pool : both;                          // head * page_size + place
-        const Pool4& pool = is_v ? v_pool : k_pool;
+        const Pool4 pool = {is_v ? v_pool.codes : k_pool.codes, is_v ? v_pool.steps : k_pool.steps};
         T* dst = (is_v ? v_out : k_out) + (out_page * per_pool + row) * D + 8 * t;
         if (partly && row % page_size >= rows) {
             const float zero[8] = {};
@@ -353,10 +327,10 @@ int launch_write(const void* qkv, void* q_out, const Pool4& k, const Pool4& v, c
     const dim3 grid(n, (Hq + 2 * Hkv + kWarps - 1) / kWarps);
     const size_t smem = (size_t)kWarps * D * sizeof(double);
     const bool whole = rotary == 0 || rotary == D, aligned = (((size_t)cos_t | (size_t)sin_t | (size_t)qw | (size_t)kw) & 15) == 0;
-    if ((D & (D - 1)) == 0 && whole && aligned) {
-        auto lanes = D == 32 ? write_lanes_4bit_kernel<T, 1> : D == 64 ? write_lanes_4bit_kernel<T, 2> : D == 128 ? write_lanes_4bit_kernel<T, 4> : write_lanes_4bit_kernel<T, 8>;
-        const int heads = 128 / (D / 8);
-        return launch_pdl(lanes, dim3(n, (Hq + 2 * Hkv + heads - 1) / heads), dim3(128), 0, stream, (const T*)qkv, (T*)q_out, k, v, slots, cos_t, sin_t, qw, kw, eps, Hq, Hkv,
+    if ((D == 64 || D == 128 || D == 256) && whole && aligned) {
+        auto lanes = D == 64 ? write_lanes_4bit_kernel<T, 2> : D == 128 ? write_lanes_4bit_kernel<T, 4> : write_lanes_4bit_kernel<T, 8>;
+        const int heads = 128 / (D / 8), sections = (Hq + heads - 1) / heads + 2 * ((Hkv + heads - 1) / heads);
+        return launch_pdl(lanes, dim3(n, sections), dim3(128), 0, stream, (const T*)qkv, (T*)q_out, k, v, slots, cos_t, sin_t, qw, kw, eps, Hq, Hkv,
                           rotary > 0 ? 1 : 0, page_size, n_pages, pool_bounds_now());
     }
     auto kernel = D <= 128 ? qk_norm_rope_write_4bit_kernel<T, 1> : qk_norm_rope_write_4bit_kernel<T, 2>;
