@@ -71,7 +71,8 @@ class Pulsar:
     """``Pulsar(model_dir, config, dtype=torch.bfloat16)``: ``config`` is the flat engine
     dictionary of the reference (``page_size``, ``max_sessions``, ``active_buffer_size``,
     ``max_running``, ``max_chunk_size``, ``eos_id``, ``temperature``, ``top_p``, ``top_k``,
-    ``seed``, ``device``; unknown keys are rejected) plus ``num_pages``."""
+    ``seed``, ``device``; unknown keys are rejected) plus ``num_pages`` and ``cache_bits`` (4: keys and
+    values are cached in 4 bits)."""
 
     def __init__(self, model_dir: str, config: Optional[Dict[str, Any]] = None, *, dtype=torch.bfloat16):
         cfg = dict(config or {})

@@ -39,6 +39,8 @@ def parse_args(argv=None) -> argparse.Namespace:
     ap.add_argument("--max_pages", type=int, default=None, help="pages of the cache pool (overrides "
                                                                 "max_sessions * active_buffer_size / page_size)")
     ap.add_argument("--page_size", type=int, default=16)
+    ap.add_argument("--cache_bits", type=int, default=0, choices=[0, 4], help="bits of a cached key or value: 0 those of --dtype, 4 for three times "
+                                                                              "the tokens in the same memory")
     ap.add_argument("--random_weights", metavar="CONFIG_JSON",
                     help="write --model from this config.json with seeded random weights first")
     ap.add_argument("--weights_seed", type=int, default=0)
@@ -80,7 +82,7 @@ def main(argv=None) -> int:
     config = dict(device=args.device, dtype=args.dtype, page_size=args.page_size, max_sessions=args.max_sessions,
                   active_buffer_size=args.active_buffer_size, max_running=args.max_running,
                   max_chunk_size=args.max_chunk_size, eos_id=int(eos), temperature=args.temperature,
-                  top_p=args.top_p, top_k=args.top_k, seed=args.seed)
+                  top_p=args.top_p, top_k=args.top_k, seed=args.seed, cache_bits=args.cache_bits)
     if args.max_pages is not None:
         config["num_pages"] = args.max_pages
     if args.candidates > 1:

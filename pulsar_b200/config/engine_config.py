@@ -33,6 +33,7 @@ class EngineConfig:
     top_k: int = 0
     seed: int = -1
     cuda_graphs: bool = True
+    cache_bits: int = 0              # bits of a cached key or value: 0 those of dtype, or 4 (dense attention with heads of a multiple of 32 channels)
 
     @classmethod
     def from_dict(cls, raw: Dict[str, Any]) -> "EngineConfig":
@@ -48,6 +49,8 @@ class EngineConfig:
         if self.dtype not in _DTYPES:
             raise ConfigError(f"EngineConfig: dtype '{self.dtype}' is not one of {sorted(set(_DTYPES))}")
         self.dtype = _DTYPES[self.dtype]
+        if self.cache_bits not in (0, 4):
+            raise ConfigError(f"EngineConfig: cache_bits must be 0 (those of dtype) or 4, found {self.cache_bits!r}")
         if self.page_size <= 0:
             raise ConfigError("EngineConfig: page_size must be > 0")
         if self.num_pages is None:

@@ -80,6 +80,7 @@ class MixerSpec:
     value_position: Optional[PositionSpec] = None
     sigmoid_weights: bool = False    # no softmax: a visible key's weight is sigmoid(score), not normalised over the keys
     score_bias: bool = False         # with sigmoid_weights: a learned number per head joins the score (tensor role "score_bias")
+    cache_bits: int = 0              # 4: keys and values are cached in 4 bits; 0: in the activation dtype
     extra: Tuple[Tuple[str, object], ...] = ()   # free-form parameters of other kinds
 
     def option(self, name, default=None):

@@ -69,7 +69,7 @@ class Engine:
     def __init__(self, model_dir: str, config: Union[EngineConfig, Dict[str, Any], None] = None):
         cfg = self._config(config)
         self._check_device(cfg)
-        model_config, model = load_model(model_dir, cfg.dtype, cfg.device)
+        model_config, model = load_model(model_dir, cfg.dtype, cfg.device, cfg.cache_bits)
         self._init(model_config, model, cfg)
 
     @classmethod
@@ -79,6 +79,8 @@ class Engine:
         cls._check_device(cfg)
         if model.dtype != torch_dtype(cfg.dtype):
             raise ValueError(f"the model computes in {model.dtype}, the engine was configured for {cfg.dtype}")
+        if getattr(model, "cache_bits", 0) != cfg.cache_bits:
+            raise ValueError(f"the model caches keys and values in {getattr(model, 'cache_bits', 0)} bits, the engine was configured for {cfg.cache_bits} (0: those of dtype)")
         self._init(model_config, model, cfg)
         return self
 

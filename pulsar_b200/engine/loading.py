@@ -20,9 +20,9 @@ def torch_dtype(name) -> torch.dtype:
         raise ValueError(f"dtype '{name}' is not one of {sorted(DTYPES)}") from None
 
 
-def load_model(model_dir: str, dtype, device):
-    """(typed config, model) for the folder; the model class is chosen by ``config.json``."""
+def load_model(model_dir: str, dtype, device, cache_bits: int = 0):
+    """(typed config, model) for the folder; the model class is chosen by ``config.json``.  ``cache_bits``: see ``build_model``."""
     config = config_from_dict(read_config_json(model_dir))
-    model = build_model(config, torch_dtype(dtype))
+    model = build_model(config, torch_dtype(dtype), cache_bits)
     load_weights(model, model_dir, device)
     return config, model

@@ -87,6 +87,11 @@ class DecoderModel(Part):
         return list(self._needs)
 
     @property
+    def cache_bits(self) -> int:
+        """Bits in which the layers cache keys and values; 0: those of the dtype."""
+        return max((b.mixer.cache_bits for b in self.spec.blocks), default=0)
+
+    @property
     def graph_safe(self) -> bool:
         """Whether a step of this model may be captured into a CUDA graph (every part says so)."""
         return all(getattr(b, "graph_safe", True) for b in self.blocks) and getattr(self.final_norm, "graph_safe", True)

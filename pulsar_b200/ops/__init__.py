@@ -2322,9 +2322,9 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
                          q_lens=None, scratch=None) -> None:
     """Attention over a cache of 4 bits: q, out [N, Hq, D] (float32 or bfloat16), ``block_table`` int32 [S, width], ``kv_len`` int32 [S] with
     the keys of this step in it.  Without ``cu_q`` every sequence has one query token, the last (N = S); else sequence i has the tokens
-    ``cu_q[i]:cu_q[i + 1]`` (int32 [S + 1], from 0, rising), the last of its ``kv_len[i]``, and ``q_lens`` are their numbers as the host knows
+    ``cu_q[i]:cu_q[i + 1]`` (int32 [S + 1], rising, rows of q), the last of its ``kv_len[i]``, and ``q_lens`` are their numbers as the host knows
     them.  A query sees the keys up to its own, with ``window`` w the last w of them; those have to lie in pages of the pool (an id that is
-    none is not read).  A query that sees no key gets zeros.  Rows of ``out`` behind the last sequence stay as they were.
+    none is not read).  A query that sees no key gets zeros.  Rows of ``out`` that are no sequence's stay as they were.
 
     bfloat16 portions of more than 64 rows a kv head (query heads times tokens), where the dense attention of prompt portions has a kernel
     for their sizes and the scale is above zero, are attended to over expanded pages, which takes room for S * width pages.  (There a value that is NaN also
@@ -2364,7 +2364,8 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
     if n == 0 or s == 0 or most_tokens == 0:
         return
     if width == 0 or n_pages == 0:               # nobody has a key
-        out[:n if q_lens is None else sum(q_lens)].zero_()
+        rows = torch.arange(n, device=q.device)
+        out.zero_() if cu_q is None else out.masked_fill_(((rows >= cu_q[0]) & (rows < cu_q[-1])).view(n, 1, 1), 0.0)
         return
     if scratch is None:
         def scratch(tag, shape, dtype):
@@ -2384,3 +2385,21 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
     at = work.data_ptr()
     check(fn("pb_paged_attention_4bit")(kind, _p(q), _p(k_pool), _p(k_steps), _p(v_pool), _p(v_steps), _p(out), at, at + 4 * sums, _p(block_table), width, _p(kv_len),
                                         _p(cu_q), n, most_tokens, s, hq, hkv, d, page_size, n_pages, float(scale), window, blocks, stream()), name, kernels=2)
+
+
+def attention_4bit(ctx, q: torch.Tensor, pools, block_table: torch.Tensor, out: torch.Tensor, scale: float, window: Optional[int]) -> None:
+    """``attention`` over a cache of 4 bits: the step's query tokens over their pages, ``pools`` as ``paged_attention_4bit`` takes them.  The decoded
+    tokens of a mixed step, which come first, are a call of their own."""
+    if ctx.all_decode:
+        paged_attention_4bit(q, *pools, out, block_table, ctx.kv_len, scale, window, scratch=ctx.scratch)
+        return
+    q_lens = ctx.host.q_lens
+    n_dec = 0
+    while n_dec < len(q_lens) and q_lens[n_dec] == 1:
+        n_dec += 1
+    if n_dec > 0:
+        paged_attention_4bit(q[:n_dec], *pools, out[:n_dec], block_table[:n_dec], ctx.kv_len[:n_dec], scale, window, scratch=ctx.scratch)
+    if n_dec == len(q_lens):
+        return
+    # (the rows' alignment: the portions take the whole of q and out, their places say which rows are theirs)
+    paged_attention_4bit(q, *pools, out, block_table[n_dec:], ctx.kv_len[n_dec:], scale, window, ctx.cu_q[n_dec:], q_lens[n_dec:], scratch=ctx.scratch)

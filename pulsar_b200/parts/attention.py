@@ -55,6 +55,8 @@ class Attention(Mixer):
     every head's output turns back by the query's, inside the attention kernels (``ops.qk_prepare_whole``, ``turn_back``).
     ``sigmoid_weights``: the weight of a visible key is sigmoid(score + score_bias[head]) and nothing is normalised.
 
+    With ``spec.cache_bits`` 4 the dense form caches keys and values in 4 bits (``ops.qk_norm_rope_write_4bit``, ``ops.attention_4bit``).
+
     ``output_bias`` is the output projection's bias (or None).  ``forward`` adds it unless the block has set
     ``defer_output_bias`` because the kernel behind the mixer takes it along.
     """
@@ -89,7 +91,13 @@ class Attention(Mixer):
                             or spec.keep_first or spec.softcap is not None or spec.sinks or spec.fixed_sink is not None
                             or spec.output_gate or self.prepared or self.whole or spec.sigmoid_weights
                             or self.maps > 1 or spec.q_temperature is not None)
-        self.shares_keys = not self.general
+        # keys and values in 4 bits: the dense form alone
+        self.four_bit = spec.cache_bits == 4
+        if spec.cache_bits not in (0, 4):
+            raise ValueError(f"attention: keys and values are cached in the activation dtype (0) or in 4 bits, found {spec.cache_bits}")
+        if self.four_bit and (self.general or spec.head_dim % ops.GROUP_4BIT):
+            raise ValueError(f"attention: a cache of 4 bits goes with the dense form and heads of a multiple of {ops.GROUP_4BIT} channels")
+        self.shares_keys = not self.general and not self.four_bit
         if (self.maps > 1 or spec.q_temperature is not None) and (self.prepared or not spec.own_kv):
             raise ValueError("attention: the differential form and the query temperature go with plain projections of its own keys")
         if spec.q_temperature is not None and not (int(spec.q_temperature[1]) > 0):
@@ -215,6 +223,10 @@ class Attention(Mixer):
         if s.value_dim != s.head_dim or self.maps > 1:
             return CacheNeed.paged((CachedTensor("k", s.n_kv_heads * self.maps, s.head_dim), CachedTensor("v", s.n_kv_heads, s.value_dim)),
                                    s.window, s.keep_first)
+        if self.four_bit:
+            codes, steps = s.head_dim // 2, s.head_dim // 16
+            return CacheNeed.paged((CachedTensor("k", s.n_kv_heads, codes, torch.uint8), CachedTensor("k_steps", s.n_kv_heads, steps, torch.bfloat16),
+                                    CachedTensor("v", s.n_kv_heads, codes, torch.uint8), CachedTensor("v_steps", s.n_kv_heads, steps, torch.bfloat16)), s.window)
         return CacheNeed.paged_kv(s.n_kv_heads, s.head_dim, s.window, s.keep_first)
 
     # ---------------------------------------------------------------- one step
@@ -313,6 +325,16 @@ class Attention(Mixer):
         else:
             cos = sin = ctx.scratch("attn.norope", (n, 0), torch.float32)
             rotary = 0
+        if self.four_bit:
+            pools = [cache.pools[name] for name in ("k", "k_steps", "v", "v_steps")]
+            if n_kv:
+                ops.qk_norm_rope_write_4bit(qkv, q, *pools, cache.slots, cos, sin, self.q_norm, self.k_norm, s.qk_norm_eps or 0.0, s.n_heads, n_kv, s.head_dim, rotary,
+                                            cache.page_size)
+            else:
+                ops.qk_norm_rope_write(qkv, q, None, None, None, cos, sin, self.q_norm, self.k_norm, s.qk_norm_eps or 0.0, s.n_heads, 0, s.head_dim, rotary, cache.page_size)
+            o = ctx.scratch("attn.o", (n, s.n_heads, s.head_dim))
+            ops.attention_4bit(ctx, q, pools, cache.block_table, o, s.scale, s.window)
+            return o
         shared = ctx.shared_pages.get(cache.group)
         if shared is not None and s.window is None:
             # forked sequences: the pages they share are read once for all of them

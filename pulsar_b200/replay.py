@@ -17,11 +17,11 @@ class Replay:
     runner that generation uses, driven by given tokens instead of sampled ones."""
 
     def __init__(self, model_dir: str, dtype: str, max_tokens: int, page_size: int = 16, max_running: int = 8,
-                 device: str = "cuda:0"):
+                 device: str = "cuda:0", cache_bits: int = 0):
         if not torch.cuda.is_available():
             raise RuntimeError("trace replay needs a CUDA device: the engine has no CPU path")
         torch.cuda.set_device(device)
-        self.config, self.model = load_model(model_dir, dtype, device)
+        self.config, self.model = load_model(model_dir, dtype, device, cache_bits)
         num_pages = max(1, -(-int(max_tokens) // page_size))
         self.cache = CacheManager(self.model.cache_needs(), page_size, num_pages, max_running, self.model.dtype, device)
         self.runner = ModelRunner(self.model, self.cache, device)
