@@ -44,9 +44,24 @@ PB_EXPORT int pb_attention_4bit_blocks(int dtype, int most_tokens, int n_seqs, i
 
 // sums: float32 [blocks, 2, rows, D + 2], rows of attention_4bit_rows; plan: int32 [2 + n_seqs * blocks of rows of most_tokens]; most_tokens: the most
 // that a sequence brings.
-PB_EXPORT int pb_paged_attention_4bit(int dtype, const void* q, void* k_codes, void* k_steps, void* v_codes, void* v_steps, void* out, float* sums, int* plan,
-                                      const int* table, int width, const int* kv_len, const int* cu_q, int n_rows, int most_tokens, int n_seqs, int Hq, int Hkv, int D,
-                                      int page_size, int n_pages, float scale, int window, int blocks, cudaStream_t stream) {
+// Words: dtype, q, k codes, k steps, v codes, v steps, out, sums, plan, table, kv_len, cu_q (or 0), width, n_rows, most_tokens, n_seqs, Hq, Hkv, D, page_size,
+// n_pages, scale, window, blocks.
+PB_EXPORT int pb_paged_attention_4bit(const long long* words, cudaStream_t stream) {
+    Words4 w{words};
+    const int dtype = w.num();
+    const void* q = w.ptr<const void>();
+    Pool4 k, v;
+    k.codes = w.ptr<uint8_t>();
+    k.steps = w.ptr<__nv_bfloat16>();
+    v.codes = w.ptr<uint8_t>();
+    v.steps = w.ptr<__nv_bfloat16>();
+    void* out = w.ptr<void>();
+    float* sums = w.ptr<float>();
+    int* plan = w.ptr<int>();
+    const int *table = w.ptr<const int>(), *kv_len = w.ptr<const int>(), *cu_q = w.ptr<const int>();
+    const int width = w.num(), n_rows = w.num(), most_tokens = w.num(), n_seqs = w.num(), Hq = w.num(), Hkv = w.num(), D = w.num(), page_size = w.num(), n_pages = w.num();
+    const float scale = (float)w.real();
+    const int window = w.num(), blocks = w.num();
     if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || D <= 0 || D > 256 || D % kGroup4 || page_size <= 0 || n_pages <= 0 || width <= 0 || window < 0 || blocks <= 0 ||
         sums == nullptr || plan == nullptr || most_tokens < 0 || n_seqs < 0 || n_rows < 0)
         return PB_ERR_BAD_SIZE;
@@ -57,7 +72,7 @@ PB_EXPORT int pb_paged_attention_4bit(int dtype, const void* q, void* k_codes, v
     if (n_seqs > 65535 || (long long)most_tokens * Hq > 0x3fffffff || (long long)n_pages * Hkv * page_size >= 0xffffffffLL || keys > 0x7ffffff0LL ||
         (double)n_seqs * row_blocks * Hkv * (keys / kTile4 + 1 + kGap4) > 1.0e9)
         return PB_ERR_TOO_LARGE;
-    Attend4 a{q, out, {(uint8_t*)k_codes, (__nv_bfloat16*)k_steps}, {(uint8_t*)v_codes, (__nv_bfloat16*)v_steps}, sums, plan, table, kv_len, cu_q, width, n_rows, n_seqs,
+    Attend4 a{q, out, k, v, sums, plan, table, kv_len, cu_q, width, n_rows, n_seqs,
               Hq, Hkv, page_size, log2_exact(page_size), n_pages, (int)row_blocks, blocks, window, scale * kLog2e, pool_bounds_now()};
     return (dtype == PB_F32 ? attend_4bit_f32 : attend_4bit_bf16)(a, D / kGroup4, rows, most_tokens, stream);
 }

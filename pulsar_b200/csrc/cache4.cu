@@ -362,13 +362,24 @@ bool sizes_4bit(int Hkv, int D, int page_size, int n_pages) {
 
 }  // namespace
 
-PB_EXPORT int pb_qk_norm_rope_write_4bit(int dtype, const void* qkv, void* q_out, void* k_codes, void* k_steps, void* v_codes, void* v_steps, const int* slots,
-                                         const float* cos_t, const float* sin_t, const float* q_weight, const float* k_weight, double eps, int n, int Hq, int Hkv, int D,
-                                         int rotary, int page_size, int n_pages, cudaStream_t stream) {
+// dtype, qkv, q_out, k codes, k steps, v codes, v steps, slots, cos, sin, q weight, k weight, eps, n, Hq, Hkv, D, rotary, page_size, n_pages
+PB_EXPORT int pb_qk_norm_rope_write_4bit(const long long* words, cudaStream_t stream) {
+    Words4 w{words};
+    const int dtype = w.num();
+    const void* qkv = w.ptr<const void>();
+    void* q_out = w.ptr<void>();
+    Pool4 k, v;
+    k.codes = w.ptr<uint8_t>();
+    k.steps = w.ptr<__nv_bfloat16>();
+    v.codes = w.ptr<uint8_t>();
+    v.steps = w.ptr<__nv_bfloat16>();
+    const int* slots = w.ptr<const int>();
+    const float *cos_t = w.ptr<const float>(), *sin_t = w.ptr<const float>(), *q_weight = w.ptr<const float>(), *k_weight = w.ptr<const float>();
+    const double eps = w.real();
+    const int n = w.num(), Hq = w.num(), Hkv = w.num(), D = w.num(), rotary = w.num(), page_size = w.num(), n_pages = w.num();
     if (!sizes_4bit(Hkv, D, page_size, n_pages) || Hq < 0 || n < 0 || rotary < 0 || rotary > D || rotary % 2) return PB_ERR_BAD_SIZE;
-    if ((Hq + 2 * Hkv + 3) / 4 > 65535) return PB_ERR_TOO_LARGE;
+    if (Hq + 2LL * Hkv > 65535) return PB_ERR_TOO_LARGE;
     if (n == 0) return 0;
-    const Pool4 k{(uint8_t*)k_codes, (__nv_bfloat16*)k_steps}, v{(uint8_t*)v_codes, (__nv_bfloat16*)v_steps};
     if (dtype == PB_F32)
         return launch_write<float>(qkv, q_out, k, v, slots, cos_t, sin_t, q_weight, k_weight, eps, n, Hq, Hkv, D, rotary, page_size, n_pages, stream);
     if (dtype == PB_BF16)
@@ -376,13 +387,24 @@ PB_EXPORT int pb_qk_norm_rope_write_4bit(int dtype, const void* qkv, void* q_out
     return PB_ERR_BAD_DTYPE;
 }
 
-PB_EXPORT int pb_expand_pages_4bit(int dtype, void* k_codes, void* k_steps, void* v_codes, void* v_steps, const int* table, const int* kv_len, void* k_out, void* v_out,
-                                   int* table_out, int n_seqs, int width, int Hkv, int D, int page_size, int n_pages, const int* cu_q, int window,
-                                   cudaStream_t stream) {
+// dtype, k codes, k steps, v codes, v steps, table, kv_len, k out, v out, table out, n_seqs, width, Hkv, D, page_size, n_pages, cu_q (or 0), window
+PB_EXPORT int pb_expand_pages_4bit(const long long* words, cudaStream_t stream) {
+    Words4 w{words};
+    const int dtype = w.num();
+    Pool4 k, v;
+    k.codes = w.ptr<uint8_t>();
+    k.steps = w.ptr<__nv_bfloat16>();
+    v.codes = w.ptr<uint8_t>();
+    v.steps = w.ptr<__nv_bfloat16>();
+    const int *table = w.ptr<const int>(), *kv_len = w.ptr<const int>();
+    void *k_out = w.ptr<void>(), *v_out = w.ptr<void>();
+    int* table_out = w.ptr<int>();
+    const int n_seqs = w.num(), width = w.num(), Hkv = w.num(), D = w.num(), page_size = w.num(), n_pages = w.num();
+    const int* cu_q = w.ptr<const int>();
+    const int window = w.num();
     if (!sizes_4bit(Hkv, D, page_size, n_pages) || n_seqs < 0 || width < 0 || window < 0) return PB_ERR_BAD_SIZE;
-    if (n_seqs > 65535 || (long long)n_seqs * width > 0x7fffffffLL || 8LL * Hkv * page_size > 0x3fffffffLL) return PB_ERR_TOO_LARGE;
+    if (n_seqs > 65535 || (long long)n_seqs * width > 0x7fffffffLL || (long long)width * page_size > 0x7fffffffLL || 8LL * Hkv * page_size > 0x3fffffffLL) return PB_ERR_TOO_LARGE;
     if (n_seqs == 0 || width == 0) return 0;
-    const Pool4 k{(uint8_t*)k_codes, (__nv_bfloat16*)k_steps}, v{(uint8_t*)v_codes, (__nv_bfloat16*)v_steps};
     if (dtype == PB_F32)
         return launch_expand<float>(D / kGroup4, k, v, table, kv_len, k_out, v_out, table_out, n_seqs, width, Hkv, page_size, n_pages, cu_q, window, stream);
     if (dtype == PB_BF16)

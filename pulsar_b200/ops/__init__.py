@@ -15,6 +15,7 @@ import ctypes
 import functools
 import math
 import os
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -154,9 +155,9 @@ _SIGNATURES = {
     "pb_head_scores_wait_limit": [ctypes.c_longlong],
     "pb_head_scores_wait_selftest": [_P, _P],
     "pb_head_scores": [_P] * 5 + [_I, _I, _I, _F, _F, _P, _P, _P],
-    "pb_qk_norm_rope_write_4bit": [_I] + [_P] * 11 + [ctypes.c_double] + [_I] * 7 + [_P],
-    "pb_expand_pages_4bit": [_I] + [_P] * 9 + [_I] * 6 + [_P, _I, _P],
-    "pb_paged_attention_4bit": [_I] + [_P] * 9 + [_I, _P, _P] + [_I] * 8 + [_F, _I, _I, _P],
+    "pb_qk_norm_rope_write_4bit": [ctypes.c_char_p, _P],
+    "pb_expand_pages_4bit": [ctypes.c_char_p, _P],
+    "pb_paged_attention_4bit": [ctypes.c_char_p, _P],
     "pb_attention_4bit_blocks": [_I] * 9,
     "pb_attention_4bit_rows": [_I, _I, _I],
     "pb_token_scores": [_I, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P],
@@ -641,6 +642,7 @@ BOUNDS_CODES = {2: "a block table named a page outside its pool (the access was 
 _bounds_words = {}
 
 
+@functools.lru_cache(maxsize=1)
 def bounds_checked() -> bool:
     """Whether the loaded library is the debug build whose kernels check page ids and slots
     (built with PULSAR_CHECK_BOUNDS=1)."""
@@ -2195,31 +2197,42 @@ def head_scores(h: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, logprob:
 GROUP_4BIT = 32
 
 
-def _check_4bit(name: str, pools, n_kv_heads: int, head_dim: int, page_size: int) -> int:
-    """Refuses pools that are not those of a cache of 4 bits with these sizes; pages of the pools."""
-    if head_dim % GROUP_4BIT or not (0 < head_dim <= 256) or n_kv_heads <= 0 or page_size <= 0:
-        raise KernelError(f"{name}: heads of a multiple of {GROUP_4BIT} channels, at most 256, and pages of a key or more, found {head_dim} and {page_size}")
-    n_pages = pools[0].shape[0] if pools[0].dim() else 0
-    for pool, dtype, width in zip(pools, (torch.uint8, torch.bfloat16) * 2, (head_dim // 2, head_dim // 16) * 2):
-        if pool.dtype != dtype or pool.shape != (n_pages, n_kv_heads, page_size, width):
-            raise KernelError(f"{name}: codes are uint8 [pages, {n_kv_heads}, {page_size}, {head_dim // 2}], steps bfloat16 [pages, {n_kv_heads}, {page_size}, "
-                              f"{head_dim // 16}], found {pool.dtype} {tuple(pool.shape)}")
-    return n_pages
+# The arguments of the kernels' entry points, as one row of 64-bit words (csrc/cache4.cuh).
+_WRITE_4BIT, _EXPAND_4BIT, _ATTEND_4BIT = struct.Struct("=12qd7q"), struct.Struct("=18q"), struct.Struct("=21qd2q")
 
 
-def _at_16(name: str, *tensors) -> None:
+def _on_one_device(name: str, tensors) -> int:
+    """The device of contiguous CUDA tensors; refuses others, and tensors of several devices."""
+    where = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.data_ptr() % 16:
-            raise KernelError(f"{name}: tensors must start at a multiple of 16 bytes")
+        if t is not None and (t.get_device() != where or not t.is_contiguous()):
+            where = -1
+            break
+    if where < 0:
+        _cuda(*tensors)
+        raise KernelError(f"{name}: all tensors must be on one device, found {sorted({str(t.device) for t in tensors if t is not None})}")
+    return where
 
 
-def _elsewhere(name: str, *tensors) -> Optional[torch.device]:
-    """The tensors' device where it is not the current one; refuses tensors of several devices."""
-    where = tensors[0].device
-    for t in tensors:
-        if t is not None and t.device != where:
-            raise KernelError(f"{name}: all tensors must be on one device, found {where} and {t.device}")
-    return where if where.index != (torch.cuda.current_device() if _device is None else _device()) else None
+def _current_device() -> int:
+    return torch.cuda.current_device() if _device is None else _device()
+
+
+def _pools_4bit(name: str, k_pool, k_steps, v_pool, v_steps, head_dim: int):
+    """The shape (pages, kv heads, page, D / 2) of pools of a cache of 4 bits with heads of ``head_dim``; refuses others."""
+    shape = k_pool.shape
+    if head_dim % GROUP_4BIT or not 0 < head_dim <= 256:
+        raise KernelError(f"{name}: heads of a multiple of {GROUP_4BIT} channels, at most 256, found {head_dim}")
+    if len(shape) != 4 or shape[3] * 2 != head_dim or shape[1] == 0 or shape[2] == 0 or v_pool.shape != shape or not (k_pool.dtype == v_pool.dtype == torch.uint8):
+        raise KernelError(f"{name}: codes are uint8 [pages, kv heads, page, {head_dim // 2}], found {k_pool.dtype} {tuple(shape)} and {v_pool.dtype} {tuple(v_pool.shape)}")
+    steps = (*shape[:3], head_dim // 16)
+    if k_steps.shape != steps or v_steps.shape != steps or not (k_steps.dtype == v_steps.dtype == torch.bfloat16):
+        raise KernelError(f"{name}: steps bfloat16 {steps} beside codes {tuple(shape)}, found {k_steps.dtype} {tuple(k_steps.shape)} and {v_steps.dtype} {tuple(v_steps.shape)}")
+    return shape
+
+
+def _refuse_16(name: str) -> None:
+    raise KernelError(f"{name}: tensors must start at a multiple of 16 bytes")
 
 
 def qk_norm_rope_write_4bit(qkv: torch.Tensor, q_out: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.Tensor, v_pool: torch.Tensor, v_steps: torch.Tensor,
@@ -2231,32 +2244,38 @@ def qk_norm_rope_write_4bit(qkv: torch.Tensor, q_out: torch.Tensor, k_pool: torc
     written.  A group of 32 channels that holds a NaN or a value beyond bfloat16's range comes back as NaN."""
     name = "qk_norm_rope_write_4bit"
     tensors = (qkv, q_out, k_pool, k_steps, v_pool, v_steps, slots, cos, sin, q_weight, k_weight)
-    _cuda(*tensors)
-    if (where := _elsewhere(name, *tensors)) is not None:
+    if (where := _on_one_device(name, tensors)) != _current_device():
         with torch.cuda.device(where):
             return qk_norm_rope_write_4bit(*tensors, eps, n_heads, n_kv_heads, head_dim, rotary, page_size)
-    n_pages = _check_4bit(name, tensors[2:6], n_kv_heads, head_dim, page_size)
-    kind = code(qkv.dtype)
-    if qkv.dim() != 2 or n_heads < 0 or qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or q_out.shape != (qkv.shape[0], n_heads, head_dim) or q_out.dtype != qkv.dtype:
-        raise KernelError(f"{name}: rows [N, ({n_heads} + 2 * {n_kv_heads}) * {head_dim}] and queries [N, {n_heads}, {head_dim}] of one dtype, found {qkv.dtype} "
-                          f"{tuple(qkv.shape)} and {q_out.dtype} {tuple(q_out.shape)}")
-    n = qkv.shape[0]
+    dtype, rows = qkv.dtype, qkv.shape
+    kind = code(dtype)
+    n_pages, hkv, page, _ = _pools_4bit(name, k_pool, k_steps, v_pool, v_steps, head_dim)
+    if hkv != n_kv_heads or page != page_size:
+        raise KernelError(f"{name}: pools of {n_kv_heads} kv heads and pages of {page_size}, found codes {tuple(k_pool.shape)}")
+    n = rows[0] if len(rows) == 2 else -1
+    if n < 0 or n_heads < 0 or rows[1] != (n_heads + 2 * hkv) * head_dim or q_out.shape != (n, n_heads, head_dim) or q_out.dtype != dtype:
+        raise KernelError(f"{name}: rows [N, ({n_heads} + 2 * {n_kv_heads}) * {head_dim}] and queries [N, {n_heads}, {head_dim}] of one dtype, found {dtype} "
+                          f"{tuple(rows)} and {q_out.dtype} {tuple(q_out.shape)}")
     if slots.dtype != torch.int32 or slots.shape != (n,):
         raise KernelError(f"{name}: slots must be int32 [{n}], found {slots.dtype} {tuple(slots.shape)}")
-    if rotary < 0 or rotary % 2 or rotary > head_dim or cos.shape != (n, rotary // 2) or sin.shape != cos.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+    turned = (n, rotary // 2)
+    if rotary < 0 or rotary % 2 or rotary > head_dim or cos.shape != turned or sin.shape != turned or not (cos.dtype == sin.dtype == torch.float32):
         raise KernelError(f"{name}: an even number of turned channels, at most {head_dim}, and float32 cosines and sines [{n}, {rotary // 2}], found {rotary}, {cos.dtype} "
                           f"{tuple(cos.shape)}, {sin.dtype} {tuple(sin.shape)}")
     for w in (q_weight, k_weight):
         if w is not None and (w.dtype != torch.float32 or w.shape != (head_dim,)):
             raise KernelError(f"{name}: norm weights must be float32 [{head_dim}], found {w.dtype} {tuple(w.shape)}")
-    _at_16(name, *tensors[:6])
-    _check_against(k_pool)
     if n_pages == 0:
         raise KernelError(f"{name}: pools without a page")
     if n == 0:
         return
-    check(fn("pb_qk_norm_rope_write_4bit")(kind, _p(qkv), _p(q_out), _p(k_pool), _p(k_steps), _p(v_pool), _p(v_steps), _p(slots), _p(cos), _p(sin), _p(q_weight), _p(k_weight),
-                                           float(eps), n, n_heads, n_kv_heads, head_dim, rotary, page_size, n_pages, stream()), name)
+    _check_against(k_pool)
+    at = qkv.data_ptr(), q_out.data_ptr(), k_pool.data_ptr(), k_steps.data_ptr(), v_pool.data_ptr(), v_steps.data_ptr()
+    if (at[0] | at[1] | at[2] | at[3] | at[4] | at[5]) % 16:
+        _refuse_16(name)
+    words = _WRITE_4BIT.pack(kind, *at, slots.data_ptr(), cos.data_ptr(), sin.data_ptr(), 0 if q_weight is None else q_weight.data_ptr(),
+                             0 if k_weight is None else k_weight.data_ptr(), eps, n, n_heads, hkv, head_dim, rotary, page, n_pages)
+    check(fn("pb_qk_norm_rope_write_4bit")(words, stream()), name)
 
 
 def expand_pages_4bit(k_pool: torch.Tensor, k_steps: torch.Tensor, v_pool: torch.Tensor, v_steps: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor,
@@ -2267,31 +2286,38 @@ def expand_pages_4bit(k_pool: torch.Tensor, k_steps: torch.Tensor, v_pool: torch
     zeros; pages that hold no key, or whose id lies outside the pool (-1), stay as they were and are -1 in ``table_out``."""
     name = "expand_pages_4bit"
     tensors = (k_pool, k_steps, v_pool, v_steps, block_table, kv_len, k_out, v_out, table_out)
-    _cuda(*tensors)
-    if (where := _elsewhere(name, *tensors)) is not None:
+    if (where := _on_one_device(name, tensors)) != _current_device():
         with torch.cuda.device(where):
             return expand_pages_4bit(*tensors)
-    if k_out.dim() != 4 or v_out.shape != k_out.shape or v_out.dtype != k_out.dtype:
-        raise KernelError(f"{name}: pages [pages, kv heads, page, D] of one dtype and shape, found {k_out.dtype} {tuple(k_out.shape)} and {v_out.dtype} {tuple(v_out.shape)}")
-    out_pages, hkv, page_size, d = k_out.shape
-    n_pages = _check_4bit(name, tensors[:4], hkv, d, page_size)
-    kind = code(k_out.dtype)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or table_out.dtype != torch.int32 or table_out.shape != block_table.shape:
-        raise KernelError(f"{name}: block tables must be int32 [S, width], found {block_table.dtype} {tuple(block_table.shape)} and {table_out.dtype} {tuple(table_out.shape)}")
-    s, width = block_table.shape
+    out_shape, dtype, table_shape = k_out.shape, k_out.dtype, block_table.shape
+    if len(out_shape) != 4 or v_out.shape != out_shape or v_out.dtype != dtype:
+        raise KernelError(f"{name}: pages [pages, kv heads, page, D] of one dtype and shape, found {dtype} {tuple(out_shape)} and {v_out.dtype} {tuple(v_out.shape)}")
+    kind = code(dtype)
+    out_pages, hkv, page_size, d = out_shape
+    shape = _pools_4bit(name, k_pool, k_steps, v_pool, v_steps, d)
+    if shape[1:3] != out_shape[1:3]:
+        raise KernelError(f"{name}: pages of {hkv} kv heads and {page_size} places to go to, found codes {tuple(shape)}")
+    if len(table_shape) != 2 or table_out.shape != table_shape or not (block_table.dtype == table_out.dtype == torch.int32):
+        raise KernelError(f"{name}: block tables must be int32 [S, width], found {block_table.dtype} {tuple(table_shape)} and {table_out.dtype} {tuple(table_out.shape)}")
+    s, width = table_shape
     if kv_len.dtype != torch.int32 or kv_len.shape != (s,):
         raise KernelError(f"{name}: lengths must be int32 [{s}], found {kv_len.dtype} {tuple(kv_len.shape)}")
     if out_pages < s * width:
         raise KernelError(f"{name}: {s} sequences of {width} pages need as many pages to go to, found {out_pages}")
-    _at_16(name, *tensors[:4], k_out, v_out)
-    _check_against(k_pool)
     if s == 0 or width == 0:
         return
-    if n_pages == 0:
+    if shape[0] == 0:
         table_out.fill_(-1)
         return
-    check(fn("pb_expand_pages_4bit")(kind, _p(k_pool), _p(k_steps), _p(v_pool), _p(v_steps), _p(block_table), _p(kv_len), _p(k_out), _p(v_out), _p(table_out), s, width,
-                                     hkv, d, page_size, n_pages, None, 0, stream()), name)
+    _check_against(k_pool)
+    _launch_expand(name, kind, (k_pool.data_ptr(), k_steps.data_ptr(), v_pool.data_ptr(), v_steps.data_ptr()), block_table.data_ptr(), kv_len.data_ptr(), k_out.data_ptr(),
+                   v_out.data_ptr(), table_out.data_ptr(), s, width, hkv, d, page_size, shape[0], 0, 0)
+
+
+def _launch_expand(name: str, kind: int, pools, table: int, kv_len: int, k_out: int, v_out: int, table_out: int, *sizes) -> None:
+    if (pools[0] | pools[1] | pools[2] | pools[3] | k_out | v_out) % 16:
+        _refuse_16(name)
+    check(fn("pb_expand_pages_4bit")(_EXPAND_4BIT.pack(kind, *pools, table, kv_len, k_out, v_out, table_out, *sizes), stream()), name)
 
 
 # Rows of a kv head (its query heads times a sequence's tokens) above which portions are attended to in two steps, where a dense kernel of the
@@ -2331,60 +2357,64 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
     reaches the tokens of its sequence's portion that do not see it.)  ``scratch(tag, shape, dtype)`` gives tensors to work in; without it they are made here."""
     name = "paged_attention_4bit"
     tensors = (q, k_pool, k_steps, v_pool, v_steps, out, block_table, kv_len)
-    _cuda(*tensors, cu_q)
-    if (where := _elsewhere(name, *tensors, cu_q)) is not None:
+    if (where := _on_one_device(name, (*tensors, cu_q))) != _current_device():
         with torch.cuda.device(where):
             return paged_attention_4bit(*tensors, scale, window, cu_q, q_lens, scratch)
-    if q.dim() != 3 or out.shape != q.shape or out.dtype != q.dtype or k_pool.dim() != 4:
-        raise KernelError(f"{name}: q and out [N, heads, D] of one dtype, pools [pages, kv heads, page, width], found {q.dtype} {tuple(q.shape)}, {out.dtype} {tuple(out.shape)}, "
-                          f"{tuple(k_pool.shape)}")
-    n, hq, d = q.shape
-    hkv, page_size = k_pool.shape[1:3]
-    n_pages = _check_4bit(name, tensors[1:5], hkv, d, page_size)
-    kind = code(q.dtype)
+    q_shape, dtype, table_shape = q.shape, q.dtype, block_table.shape
+    if len(q_shape) != 3 or out.shape != q_shape or out.dtype != dtype:
+        raise KernelError(f"{name}: q and out [N, heads, D] of one dtype, found {dtype} {tuple(q_shape)} and {out.dtype} {tuple(out.shape)}")
+    kind = code(dtype)
+    n, hq, d = q_shape
+    n_pages, hkv, page_size, _ = _pools_4bit(name, k_pool, k_steps, v_pool, v_steps, d)
     if hq == 0 or hq % hkv:
         raise KernelError(f"{name}: {hq} query heads cannot be grouped over {hkv} kv heads")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or kv_len.dtype != torch.int32 or kv_len.shape != block_table.shape[:1]:
-        raise KernelError(f"{name}: a block table int32 [S, width] and lengths int32 [S], found {block_table.dtype} {tuple(block_table.shape)} and {kv_len.dtype} {tuple(kv_len.shape)}")
-    s, width = block_table.shape
-    if (cu_q is None) != (q_lens is None):
-        raise KernelError(f"{name}: cu_q and q_lens go together")
+    if len(table_shape) != 2 or kv_len.shape != table_shape[:1] or not (block_table.dtype == kv_len.dtype == torch.int32):
+        raise KernelError(f"{name}: a block table int32 [S, width] and lengths int32 [S], found {block_table.dtype} {tuple(table_shape)} and {kv_len.dtype} {tuple(kv_len.shape)}")
+    s, width = table_shape
     most_tokens = 1
     if cu_q is None:
+        if q_lens is not None:
+            raise KernelError(f"{name}: cu_q and q_lens go together")
         if n != s:
             raise KernelError(f"{name}: without cu_q every sequence has one query token, found {n} for {s}")
     else:
+        if q_lens is None:
+            raise KernelError(f"{name}: cu_q and q_lens go together")
         if cu_q.dtype != torch.int32 or cu_q.shape != (s + 1,) or len(q_lens) != s or (s and min(q_lens) < 0) or sum(q_lens) > n:
             raise KernelError(f"{name}: cu_q int32 [{s + 1}] and {s} numbers of tokens that {n} rows hold, found {cu_q.dtype} {tuple(cu_q.shape)} and {list(q_lens)[:8]}")
         most_tokens = max(q_lens, default=0)
-    if window is not None and window <= 0:
+    if window is None:
+        window = 0
+    elif window <= 0:
         raise KernelError(f"{name}: a window must be positive, found {window}")
-    _at_16(name, *tensors[:6])
-    _check_against(k_pool)
     if n == 0 or s == 0 or most_tokens == 0:
         return
     if width == 0 or n_pages == 0:               # nobody has a key
         rows = torch.arange(n, device=q.device)
         out.zero_() if cu_q is None else out.masked_fill_(((rows >= cu_q[0]) & (rows < cu_q[-1])).view(n, 1, 1), 0.0)
         return
-    if scratch is None:
-        def scratch(tag, shape, dtype):
-            return torch.empty(shape, dtype=dtype, device=q.device)
-    window = int(window or 0)
-    dense = None if cu_q is None else _expanded_4bit(q.dtype, most_tokens * (hq // hkv), hq, hkv, d, page_size, scale)
+    _check_against(k_pool)
+    pools = k_pool.data_ptr(), k_steps.data_ptr(), v_pool.data_ptr(), v_steps.data_ptr()
+    dense = None if cu_q is None else _expanded_4bit(dtype, most_tokens * (hq // hkv), hq, hkv, d, page_size, scale)
     if dense is not None:
-        k_out, v_out = (scratch(f"attn4.{x}", (s * width, hkv, page_size, d), q.dtype) for x in "kv")
-        table_out = scratch("attn4.table", (s, width), torch.int32)
-        check(fn("pb_expand_pages_4bit")(kind, _p(k_pool), _p(k_steps), _p(v_pool), _p(v_steps), _p(block_table), _p(kv_len), _p(k_out), _p(v_out), _p(table_out), s, width,
-                                         hkv, d, page_size, n_pages, _p(cu_q), window, stream()), name)
+        shapes = ((s * width, hkv, page_size, d), dtype), ((s * width, hkv, page_size, d), dtype), ((s, width), torch.int32)
+        if scratch is None:
+            k_out, v_out, table_out = (torch.empty(shape, dtype=kept, device=q.device) for shape, kept in shapes)
+        else:
+            k_out, v_out, table_out = (scratch(f"attn4.{what}", shape, kept) for what, (shape, kept) in zip(("k", "v", "table"), shapes))
+        _launch_expand(name, kind, pools, block_table.data_ptr(), kv_len.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), table_out.data_ptr(), s, width, hkv, d, page_size,
+                       n_pages, cu_q.data_ptr(), window)
         run, tiles = (paged_attention_prefill_tcgen05, prefill_tcgen05_tiles) if dense == "tcgen05" else (paged_attention_prefill_tc, prefill_tc_tiles)
         run(q, k_out, v_out, out, table_out, cu_q, kv_len, tiles(q_lens), scale, window)
         return
-    blocks, sums, plan = scratch_4bit(s, most_tokens, hq, hkv, d, width, page_size, window, q.dtype)
-    work = scratch("attn4.work", (sums + plan,), torch.float32)
-    at = work.data_ptr()
-    check(fn("pb_paged_attention_4bit")(kind, _p(q), _p(k_pool), _p(k_steps), _p(v_pool), _p(v_steps), _p(out), at, at + 4 * sums, _p(block_table), width, _p(kv_len),
-                                        _p(cu_q), n, most_tokens, s, hq, hkv, d, page_size, n_pages, float(scale), window, blocks, stream()), name, kernels=2)
+    blocks, sums, plan = scratch_4bit(s, most_tokens, hq, hkv, d, width, page_size, window, dtype)
+    work = torch.empty(sums + plan, dtype=torch.float32, device=q.device) if scratch is None else scratch("attn4.work", (sums + plan,), torch.float32)
+    work_at, q_at, out_at = work.data_ptr(), q.data_ptr(), out.data_ptr()
+    if (q_at | out_at | work_at | pools[0] | pools[1] | pools[2] | pools[3]) % 16:
+        _refuse_16(name)
+    words = _ATTEND_4BIT.pack(kind, q_at, *pools, out_at, work_at, work_at + 4 * sums, block_table.data_ptr(), kv_len.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
+                              width, n, most_tokens, s, hq, hkv, d, page_size, n_pages, scale, window, blocks)
+    check(fn("pb_paged_attention_4bit")(words, stream()), name, 2)
 
 
 def attention_4bit(ctx, q: torch.Tensor, pools, block_table: torch.Tensor, out: torch.Tensor, scale: float, window: Optional[int]) -> None:
