@@ -23,6 +23,7 @@
 // on codes and bytes, not products.)
 #pragma once
 
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include "cache4.cuh"
@@ -166,7 +167,7 @@ template <typename T, int G, int NT, int COPIES>
 struct Attend4Block {
     static_assert(G % COPIES == 0, "copies take groups in turn");
     static constexpr bool kPairs = COPIES > 1;              // words of two groups as operands
-    static constexpr int D = kGroup4 * G, G_ = G;
+    static constexpr int D = kGroup4 * G, G_ = G, NT_ = NT, COPIES_ = COPIES;
     static constexpr int kColumns = 8 / COPIES;             // rows of the block in 8 columns
     static constexpr int kRows = NT * kColumns;
     static constexpr int GH = G / COPIES;                   // groups of a copy: copy h has h, h + COPIES, ..
@@ -763,14 +764,146 @@ __device__ __forceinline__ Run4 run_of(const Attend4& a, int rows) {
     return run;
 }
 
+// Turns [skipped, skipped + n_turns) of a head by the warps of a block.  Afterwards every warp's sums stand in its shared memory: [row][D], then
+// (maximum, sum of weights) of each row; block_sum adds them up.
+template <typename T, typename B, typename Turns>
+__device__ __forceinline__ void attend_part(const Attend4& a, const Entry4& entry, int kvh, int skipped, int n_turns, uint8_t* shared) {
+    constexpr int D = B::D, NT = B::NT_, COPIES = B::COPIES_;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, t = lane & 3;
+    const uint32_t ring = smem_u32(shared) + warp * B::kPerWarp, q_at = smem_u32(shared) + B::kQ;
+    const int own = n_turns > warp ? (n_turns - warp + kWarps4 - 1) / kWarps4 : 0;
+    const Head4 head = {a.table + (size_t)entry.seq * a.width, kvh, entry.start() + (skipped + warp) * kTile4, own, entry.first, entry.last};
+    Turns turns;
+    turns.begin(a, head, lane);
+    const T* src[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const long at = entry.row_at(a, kvh, B::kColumns * n + r % B::kColumns);
+        src[n] = at < 0 ? nullptr : reinterpret_cast<const T*>(a.q) + at * D;
+    }
+    typename B::RawQ raw;
+    B::read_q(src, raw, lane);
+#pragma unroll
+    for (int i = 0; i < B::kBuffers - 1; ++i) {
+        if (i < own) turns.fill(a, head, i, ring + i * B::kStage, lane);
+        cp_async_commit();
+    }
+    B::write_q(raw, a.scale_log2, q_at, warp, lane);
+
+    B b;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int group = a.Hq / a.Hkv;
+            b.pos[n][c] = min(entry.last, entry.kv_len - entry.n_tokens + min(entry.n_tokens - 1, (entry.row0 + B::kColumns * n + (2 * t + c) % B::kColumns) / group));
+            b.top[n][c] = kLowest4;
+            b.total[n][c] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < B::GH; ++g) {
+                b.least_sum[n][g][c] = 0.0f;
+                if (B::kOffsets) b.offsets[n][g][c] = b.offsets[n][g][c + 2] = 0.0f;
+            }
+#pragma unroll
+            for (int w = 0; w < B::W; ++w)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) b.o[n][w][u][c] = b.o[n][w][u][c + 2] = 0.0f;
+        }
+    // turns [inner_from, inner_to) are seen whole by every column
+    const int before = entry.kv_len - entry.n_tokens;
+    const int lowest = min(entry.last, before + entry.token0), highest = min(entry.last, before + entry.token1);
+    const int above = a.window > 0 ? before + entry.token1 - a.window - head.key0 + 1 : 0;
+    const int inner_from = above > 0 ? (above + kWarps4 * kTile4 - 1) / (kWarps4 * kTile4) : 0;
+    const int inner_to = lowest - head.key0 >= kTile4 - 1 ? (lowest - head.key0 - (kTile4 - 1)) / (kWarps4 * kTile4) + 1 : 0;
+    __syncthreads();
+    b.take_q_sums(q_at, lane);
+
+    uint32_t stage = ring, free = ring + (B::kBuffers - 1) * B::kStage;
+    for (int i = 0; i < own; ++i) {
+        cp_async_wait<B::kBuffers - 2>();
+        __syncwarp();
+        if (i + B::kBuffers - 1 < own) turns.fill(a, head, i + B::kBuffers - 1, free, lane);
+        cp_async_commit();
+        b.turn(stage, q_at, lane, i < inner_from || i >= inner_to || turns.holes, [&](auto& x) {
+            b.take_edges(x, stage, head.key0 + i * (kWarps4 * kTile4), lowest, highest, a.window, lane, [&](int key) {
+                int place;
+                return !turns.holes || (key >= head.first && key <= head.last && page_of(a, head, key, place) >= 0);
+            });
+        });
+        free = stage;
+        stage = stage == ring + (B::kBuffers - 1) * B::kStage ? ring : stage + B::kStage;
+        __syncwarp();
+    }
+    cp_async_wait<0>();
+    __syncwarp();
+    // The warp's sums to its own shared memory (the ring is done with): [column][D], then maxima and totals.
+    float* mine = reinterpret_cast<float*>(shared + warp * B::kPerWarp);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int column = B::kColumns * n + (2 * t + c) % B::kColumns, copy = t * COPIES / 4;
+            float total = b.total[n][c];
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+            float least[B::GH];
+#pragma unroll
+            for (int j = 0; j < B::GH; ++j) {
+                least[j] = b.least_sum[n][j][c];
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) least[j] += __shfl_xor_sync(0xffffffffu, least[j], off);
+                if (B::kOffsets) least[j] -= b.offsets[n][j][c];
+            }
+#pragma unroll
+            for (int w = 0; w < B::W; ++w) {
+                const int g = B::kPairs ? 2 * w + (copy & 1) : w;
+                const float m = least[B::kPairs ? 2 * w / COPIES : w];
+                if (!B::kPairs || g % COPIES == copy)
+                    *reinterpret_cast<float4*>(mine + column * D + 32 * g + 4 * r) =
+                        make_float4(b.o[n][w][0][c] + m, b.o[n][w][0][c + 2] + m, b.o[n][w][1][c] + m, b.o[n][w][1][c + 2] + m);
+            }
+            if (r == 0 && copy == 0) {
+                mine[B::kRows * D + 2 * column] = b.top[n][c];
+                mine[B::kRows * D + 2 * column + 1] = total;
+            }
+        }
+    __syncthreads();
+}
+// Four channels of a row, the warps' parts together: not divided by the sum of weights.
+template <typename B>
+__device__ __forceinline__ void block_sum(const uint8_t* shared, int column, int quad, float& top, float& total, float (&v)[4]) {
+    constexpr int D = B::D;
+    float tops[kWarps4];
+    top = kLowest4;
+    total = v[0] = v[1] = v[2] = v[3] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps4; ++w) {
+        tops[w] = reinterpret_cast<const float*>(shared + w * B::kPerWarp)[B::kRows * D + 2 * column];
+        top = fmaxf(top, tops[w]);
+    }
+#pragma unroll
+    for (int w = 0; w < kWarps4; ++w) {
+        const float* theirs = reinterpret_cast<const float*>(shared + w * B::kPerWarp);
+        const float f = exp2_fast(tops[w] - top);
+        const float4 s = *reinterpret_cast<const float4*>(theirs + column * D + 4 * quad);
+        total += f * theirs[B::kRows * D + 2 * column + 1];
+        v[0] += f * s.x; v[1] += f * s.y; v[2] += f * s.z; v[3] += f * s.w;
+    }
+}
+template <typename T> __device__ __forceinline__ void store_weighed(T* out, float total, float (&v)[4]) {
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = total == 0.0f ? 0.0f : v[e] * inverse;
+    store_quad(out, v);
+}
+
 template <typename T, int G, int NT, int COPIES, typename Turns, int BLOCKS>
 __global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_kernel(const Attend4 a) {
     using B = Attend4Block<T, G, NT, COPIES>;
     constexpr int D = B::D;
     pdl_wait();
     extern __shared__ __align__(128) uint8_t shared[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, t = lane & 3;
-    const uint32_t ring = smem_u32(shared) + warp * B::kPerWarp, q_at = smem_u32(shared) + B::kQ;
+    const int lane = threadIdx.x & 31;
     pdl_trigger();                      // all blocks are here at once: what joins may come as they end
     Run4 run = run_of(a, B::kRows);
     while (run.from < run.to) {
@@ -792,128 +925,17 @@ __global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_kernel(const
         run.from += taken;
         run.offset += taken;
         if (n_turns <= 0) continue;
-        const int own = n_turns > warp ? (n_turns - warp + kWarps4 - 1) / kWarps4 : 0;
-        const Head4 head = {a.table + (size_t)entry.seq * a.width, kvh, entry.start() + (skipped + warp) * kTile4, own, entry.first, entry.last};
-        Turns turns;
-        turns.begin(a, head, lane);
-        const T* src[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const long at = entry.row_at(a, kvh, B::kColumns * n + r % B::kColumns);
-            src[n] = at < 0 ? nullptr : reinterpret_cast<const T*>(a.q) + at * D;
-        }
-        typename B::RawQ raw;
-        B::read_q(src, raw, lane);
-#pragma unroll
-        for (int i = 0; i < B::kBuffers - 1; ++i) {
-            if (i < own) turns.fill(a, head, i, ring + i * B::kStage, lane);
-            cp_async_commit();
-        }
-        B::write_q(raw, a.scale_log2, q_at, warp, lane);
-
-        B b;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int group = a.Hq / a.Hkv;
-                b.pos[n][c] = min(entry.last, entry.kv_len - entry.n_tokens + min(entry.n_tokens - 1, (entry.row0 + B::kColumns * n + (2 * t + c) % B::kColumns) / group));
-                b.top[n][c] = kLowest4;
-                b.total[n][c] = 0.0f;
-#pragma unroll
-                for (int g = 0; g < B::GH; ++g) {
-                    b.least_sum[n][g][c] = 0.0f;
-                    if (B::kOffsets) b.offsets[n][g][c] = b.offsets[n][g][c + 2] = 0.0f;
-                }
-#pragma unroll
-                for (int w = 0; w < B::W; ++w)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) b.o[n][w][u][c] = b.o[n][w][u][c + 2] = 0.0f;
-            }
-        // turns [inner_from, inner_to) are seen whole by every column
-        const int before = entry.kv_len - entry.n_tokens;
-        const int lowest = min(entry.last, before + entry.token0), highest = min(entry.last, before + entry.token1);
-        const int above = a.window > 0 ? before + entry.token1 - a.window - head.key0 + 1 : 0;
-        const int inner_from = above > 0 ? (above + kWarps4 * kTile4 - 1) / (kWarps4 * kTile4) : 0;
-        const int inner_to = lowest - head.key0 >= kTile4 - 1 ? (lowest - head.key0 - (kTile4 - 1)) / (kWarps4 * kTile4) + 1 : 0;
-        __syncthreads();
-        b.take_q_sums(q_at, lane);
-
-        uint32_t stage = ring, free = ring + (B::kBuffers - 1) * B::kStage;
-        for (int i = 0; i < own; ++i) {
-            cp_async_wait<B::kBuffers - 2>();
-            __syncwarp();
-            if (i + B::kBuffers - 1 < own) turns.fill(a, head, i + B::kBuffers - 1, free, lane);
-            cp_async_commit();
-            b.turn(stage, q_at, lane, i < inner_from || i >= inner_to || turns.holes, [&](auto& x) {
-                b.take_edges(x, stage, head.key0 + i * (kWarps4 * kTile4), lowest, highest, a.window, lane, [&](int key) {
-                    int place;
-                    return !turns.holes || (key >= head.first && key <= head.last && page_of(a, head, key, place) >= 0);
-                });
-            });
-            free = stage;
-            stage = stage == ring + (B::kBuffers - 1) * B::kStage ? ring : stage + B::kStage;
-            __syncwarp();
-        }
-        cp_async_wait<0>();
-        __syncwarp();
-        // The warp's sums to its own shared memory (the ring is done with): [column][D], then maxima and totals.
-        float* mine = reinterpret_cast<float*>(shared + warp * B::kPerWarp);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int column = B::kColumns * n + (2 * t + c) % B::kColumns, copy = t * COPIES / 4;
-                float total = b.total[n][c];
-#pragma unroll
-                for (int off = 4; off < 32; off <<= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-                float least[B::GH];
-#pragma unroll
-                for (int j = 0; j < B::GH; ++j) {
-                    least[j] = b.least_sum[n][j][c];
-#pragma unroll
-                    for (int off = 4; off < 32; off <<= 1) least[j] += __shfl_xor_sync(0xffffffffu, least[j], off);
-                    if (B::kOffsets) least[j] -= b.offsets[n][j][c];
-                }
-#pragma unroll
-                for (int w = 0; w < B::W; ++w) {
-                    const int g = B::kPairs ? 2 * w + (copy & 1) : w;
-                    const float m = least[B::kPairs ? 2 * w / COPIES : w];
-                    if (!B::kPairs || g % COPIES == copy)
-                        *reinterpret_cast<float4*>(mine + column * D + 32 * g + 4 * r) =
-                            make_float4(b.o[n][w][0][c] + m, b.o[n][w][0][c + 2] + m, b.o[n][w][1][c] + m, b.o[n][w][1][c + 2] + m);
-                }
-                if (r == 0 && copy == 0) {
-                    mine[B::kRows * D + 2 * column] = b.top[n][c];
-                    mine[B::kRows * D + 2 * column + 1] = total;
-                }
-            }
-        __syncthreads();
+        attend_part<T, B, Turns>(a, entry, kvh, skipped, n_turns, shared);
         const bool whole = n_turns == entry.turns;
         const int place = 2 * blockIdx.x + (skipped > 0 ? 0 : 1);        // a head that another block began, or one that another ends
         for (int i = threadIdx.x; i < B::kRows * (D / 4); i += kWarps4 * 32) {
             const int column = i / (D / 4), quad = i - column * (D / 4);
             const long at = entry.row_at(a, kvh, column);
             if (at < 0) continue;
-            float tops[kWarps4], top = kLowest4, total = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int w = 0; w < kWarps4; ++w) {
-                tops[w] = reinterpret_cast<const float*>(shared + w * B::kPerWarp)[B::kRows * D + 2 * column];
-                top = fmaxf(top, tops[w]);
-            }
-#pragma unroll
-            for (int w = 0; w < kWarps4; ++w) {
-                const float* theirs = reinterpret_cast<const float*>(shared + w * B::kPerWarp);
-                const float f = exp2_fast(tops[w] - top);
-                const float4 s = *reinterpret_cast<const float4*>(theirs + column * D + 4 * quad);
-                total += f * theirs[B::kRows * D + 2 * column + 1];
-                v[0] += f * s.x; v[1] += f * s.y; v[2] += f * s.z; v[3] += f * s.w;
-            }
+            float top, total, v[4];
+            block_sum<B>(shared, column, quad, top, total, v);
             if (whole) {
-                const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = total == 0.0f ? 0.0f : v[e] * inverse;
-                store_quad(reinterpret_cast<T*>(a.out) + at * D + 4 * quad, v);
+                store_weighed(reinterpret_cast<T*>(a.out) + at * D + 4 * quad, total, v);
             } else {
                 store_quad(a.sums + ((size_t)place * B::kRows + column) * D + 4 * quad, v);
                 if (quad == 0) *reinterpret_cast<float2*>(a.sums + (size_t)2 * a.blocks * B::kRows * D + ((size_t)place * B::kRows + column) * 2) = make_float2(top, total);
@@ -921,6 +943,63 @@ __global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_kernel(const
         }
         __syncthreads();
     }
+}
+
+// A head a cluster (of one block: a block): its parts are joined through the blocks' shared memory, and nothing needs to be known of the others.
+template <typename T, int G, int NT, int COPIES, typename Turns, int BLOCKS>
+__global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_cluster_kernel(const Attend4 a) {
+    namespace cg = cooperative_groups;
+    using B = Attend4Block<T, G, NT, COPIES>;
+    constexpr int D = B::D;
+    pdl_wait();
+    extern __shared__ __align__(128) uint8_t shared[];
+    const int parts = gridDim.x, part = blockIdx.x, kvh = blockIdx.y / a.row_blocks;
+    const Entry4 entry(a, blockIdx.z * a.row_blocks + blockIdx.y - kvh * a.row_blocks, B::kRows);
+    if (entry.row0 >= entry.n_tokens * (a.Hq / a.Hkv)) return;                   // the whole cluster
+    const int share = (entry.turns + parts - 1) / parts, skipped = part * share;
+    attend_part<T, B, Turns>(a, entry, kvh, skipped, max(0, min(share, entry.turns - skipped)), shared);
+    pdl_trigger();
+    float* mine = reinterpret_cast<float*>(shared + B::kShared);                 // [row][D], then (maximum, sum of weights) of each
+    for (int i = threadIdx.x; i < B::kRows * (D / 4); i += kWarps4 * 32) {
+        const int column = i / (D / 4), quad = i - column * (D / 4);
+        float top, total, v[4];
+        block_sum<B>(shared, column, quad, top, total, v);
+        if (parts == 1) {
+            const long at = entry.row_at(a, kvh, column);
+            if (at >= 0) store_weighed(reinterpret_cast<T*>(a.out) + at * D + 4 * quad, total, v);
+        } else {
+            *reinterpret_cast<float4*>(mine + column * D + 4 * quad) = make_float4(v[0], v[1], v[2], v[3]);
+            if (quad == 0) *reinterpret_cast<float2*>(mine + B::kRows * D + 2 * column) = make_float2(top, total);
+        }
+    }
+    if (parts == 1) return;
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    for (int i = part * kWarps4 * 32 + threadIdx.x; i < B::kRows * (D / 4); i += parts * kWarps4 * 32) {
+        const int column = i / (D / 4), quad = i - column * (D / 4);
+        const long at = entry.row_at(a, kvh, column);
+        if (at < 0) continue;
+        float2 ml[8];
+        float4 s[8];
+        float top = kLowest4, total = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
+            if (p < parts) {
+                const float* theirs = cluster.map_shared_rank(mine, p);
+                ml[p] = *reinterpret_cast<const float2*>(theirs + B::kRows * D + 2 * column);
+                s[p] = *reinterpret_cast<const float4*>(theirs + column * D + 4 * quad);
+                top = fmaxf(top, ml[p].x);
+            }
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
+            if (p < parts) {
+                const float f = exp2_fast(ml[p].x - top);
+                total += f * ml[p].y;
+                v[0] += f * s[p].x; v[1] += f * s[p].y; v[2] += f * s[p].z; v[3] += f * s[p].w;
+            }
+        store_weighed(reinterpret_cast<T*>(a.out) + at * D + 4 * quad, total, v);
+    }
+    cluster.sync();                     // nobody leaves while its shared memory is read
 }
 
 // The rows of heads that several blocks had, joined; zeros where there is no key.  A block a row and head, its warps every fourth part.
@@ -991,6 +1070,26 @@ int launch_attend_4bit(const Attend4& a, int most_tokens, cudaStream_t stream) {
     using B = Attend4Block<T, G, NT, COPIES>;
     constexpr int kBlocks = blocks_4bit(sizeof(T) == 4, G, B::kRows);
     auto kernel = attend_4bit_kernel<T, G, NT, COPIES, Turns<B>, kBlocks>;
+    if (a.blocks < 0) {                 // clusters of -blocks
+        auto clusters = attend_4bit_cluster_kernel<T, G, NT, COPIES, Turns<B>, kBlocks>;
+        constexpr int kBytes = B::kShared + B::kRows * (B::D + 2) * 4;
+        static SmemLimit limit;
+        if (const int rc = limit.allow(clusters, kBytes)) return rc;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(-a.blocks, a.Hkv * a.row_blocks, a.n_seqs);
+        cfg.blockDim = dim3(kWarps4 * 32);
+        cfg.dynamicSmemBytes = kBytes;
+        cfg.stream = stream;
+        cudaLaunchAttribute attrs[2];
+        attrs[0].id = cudaLaunchAttributeClusterDimension;
+        attrs[0].val.clusterDim.x = -a.blocks;
+        attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+        attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attrs[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attrs;
+        cfg.numAttrs = pdl_enabled() ? 2 : 1;
+        return (int)cudaLaunchKernelEx(&cfg, clusters, a);
+    }
     static SmemLimit limit;
     if (const int rc = limit.allow(kernel, B::kShared)) return rc;
     if (const int rc = launch_pdl(kernel, dim3(a.blocks), dim3(kWarps4 * 32), B::kShared, stream, a)) return rc;

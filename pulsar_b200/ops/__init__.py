@@ -2327,10 +2327,13 @@ EXPANDED_ROWS_4BIT = 64
 
 @functools.lru_cache(maxsize=1024)
 def scratch_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int, width: int, page_size: int, window: int, dtype: torch.dtype) -> Tuple[int, int, int]:
-    """(blocks, float32 elements of sums, int32 elements of the plan) of ``paged_attention_4bit`` for sequences of up to ``most_tokens`` tokens."""
+    """(blocks, float32 elements of sums, int32 elements of the plan) of ``paged_attention_4bit`` for sequences of up to ``most_tokens`` tokens; blocks below
+    zero: clusters of so many, which need no room."""
     rows_all = most_tokens * (n_heads // n_kv_heads)
     rows = fn("pb_attention_4bit_rows")(code(dtype), rows_all, head_dim)
     blocks = fn("pb_attention_4bit_blocks")(code(dtype), most_tokens, n_seqs, n_heads, n_kv_heads, head_dim, width, page_size, window)
+    if blocks < 0:
+        return blocks, 0, 0
     return blocks, blocks * 2 * rows * (head_dim + 2), 2 + n_seqs * -(-rows_all // rows)
 
 
@@ -2408,13 +2411,15 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
         run(q, k_out, v_out, out, table_out, cu_q, kv_len, tiles(q_lens), scale, window)
         return
     blocks, sums, plan = scratch_4bit(s, most_tokens, hq, hkv, d, width, page_size, window, dtype)
-    work = torch.empty(sums + plan, dtype=torch.float32, device=q.device) if scratch is None else scratch("attn4.work", (sums + plan,), torch.float32)
-    work_at, q_at, out_at = work.data_ptr(), q.data_ptr(), out.data_ptr()
+    work_at, q_at, out_at = 0, q.data_ptr(), out.data_ptr()
+    if sums:
+        work = torch.empty(sums + plan, dtype=torch.float32, device=q.device) if scratch is None else scratch("attn4.work", (sums + plan,), torch.float32)
+        work_at = work.data_ptr()
     if (q_at | out_at | work_at | pools[0] | pools[1] | pools[2] | pools[3]) % 16:
         _refuse_16(name)
     words = _ATTEND_4BIT.pack(kind, q_at, *pools, out_at, work_at, work_at + 4 * sums, block_table.data_ptr(), kv_len.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
                               width, n, most_tokens, s, hq, hkv, d, page_size, n_pages, scale, window, blocks)
-    check(fn("pb_paged_attention_4bit")(words, stream()), name, 2)
+    check(fn("pb_paged_attention_4bit")(words, stream()), name, 2 if sums else 1)
 
 
 def attention_4bit(ctx, q: torch.Tensor, pools, block_table: torch.Tensor, out: torch.Tensor, scale: float, window: Optional[int]) -> None:
