@@ -46,7 +46,7 @@ PB_EXPORT int pb_attention_4bit_blocks(int dtype, int most_tokens, int n_seqs, i
         long long best = turns / sms + kApart4 + 1;
         int cluster = 0;
         for (int n = 8; n >= 1; n /= 2) {
-            if (n > 1 && (heads * n > most || of_head < 2 * kWarps4 * n)) continue;          // one wave of blocks, two turns a warp
+            if (n > 1 && (heads * n > most || of_head < 3 * n)) continue;          // one wave of blocks, a turn for most of their warps
             const long long fullest = (heads * n + sms - 1) / sms * ((of_head + n - 1) / n);
             if (fullest < best) {
                 best = fullest;

@@ -103,7 +103,7 @@ struct Plan4 {
             if (blocks > heads) apart = min(apart, (all + blocks - heads - 1) / (blocks - heads));  // enough for whatever they are
         }
         const bool is_apart = apart <= packed;
-        const int share = (max(is_apart ? apart : packed, kLeastShare4) + kWarps4 - 1) / kWarps4 * kWarps4;
+        const int share = max(is_apart ? apart : packed, kLeastShare4);
         return {share, is_apart};
     }
 };
@@ -227,7 +227,7 @@ struct Attend4Block {
 
     // State of a warp.  Lane (r, t) = (lane / 4, lane % 4) holds columns 2 t and 2 t + 1 of 8 for each of NT; they belong to copy t COPIES / 4.
     float q_sum[NT][GH][2];                 // sum of a column's q over a group of its copy, times 2^-24
-    float to_log2[NT][2];                   // from a column's sums of products to scores in base 2
+    float to_log2[NT][2];                   // from a column's sums of products to scores in base 2; above zero (a scale's sign is q's)
     uint32_t bf16_bits;
     uint32_t first_of, second_of;           // byte selections: the first (second) of two weights, where column r's copy wants it, beside zero
     // [w][u]: channels 4 r + 2 u, + 1 (elements 0 1, 2 3) of columns 2 t, 2 t + 1 of group w, or of group 2 w + 1 for odd copies and 2 w for even ones
@@ -269,9 +269,9 @@ struct Attend4Block {
             if (COPIES >= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
             // the row over 2^k, its largest element in [2^14, 2^15): float16 holds 11 bits of all that is above 2^-28 of it
             const int k = min(126, max(-112, (int)(__float_as_uint(most) >> 23) - 127)) - 14;
-            const float down = __int_as_float((127 - k) << 23);
+            const float down = copysignf(__int_as_float((127 - k) << 23), scale_log2);
             if (warp == 0 && t == 0)
-                asm volatile("st.shared.f32 [%0], %1;" ::"r"(q_at + kQLog2 + (n * 8 + r) * 4), "f"(__int_as_float((127 + k) << 23) * 0x1p24f * scale_log2) : "memory");
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(q_at + kQLog2 + (n * 8 + r) * 4), "f"(fmaxf(1.2e-38f, __int_as_float((127 + k) << 23) * 0x1p24f * fabsf(scale_log2))) : "memory");      // -inf stays so times it
 #pragma unroll
             for (int g = 0; g < GH; ++g) {
                 if (g % kWarps4 != warp && GH >= kWarps4) continue;
@@ -466,14 +466,14 @@ struct Attend4Block {
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[half][n][e] = over_copies(x[half][n][e]) * to_log2[n][e & 1];
+                for (int e = 0; e < 4; ++e) x[half][n][e] = over_copies(x[half][n][e]);
         if (edge) edges(x);
         bool rises = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             // The maximum moves only when a score passes it by more than 2^8: weights stay below 2^8, float32 and bfloat16 have room for them.
 #pragma unroll
-            for (int c = 0; c < 2; ++c) rises |= fmaxf(fmaxf(x[0][n][c], x[0][n][c + 2]), fmaxf(x[1][n][c], x[1][n][c + 2])) > top[n][c] + 8.0f;
+            for (int c = 0; c < 2; ++c) rises |= fmaxf(fmaxf(x[0][n][c], x[0][n][c + 2]), fmaxf(x[1][n][c], x[1][n][c + 2])) * to_log2[n][c] > top[n][c] + 8.0f;
         }
         if (__any_sync(0xffffffffu, rises)) {
 #pragma unroll
@@ -484,7 +484,7 @@ struct Attend4Block {
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                    m = fmaxf(m, top[n][c]);
+                    m = fmaxf(m * to_log2[n][c], top[n][c]);
                     const float shrink = exp2_fast(top[n][c] - m);
                     top[n][c] = m;
                     total[n][c] *= shrink;
@@ -510,7 +510,7 @@ struct Attend4Block {
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[half][n][e] = exp2_fast(x[half][n][e] - top[n][e & 1]);
+                for (int e = 0; e < 4; ++e) x[half][n][e] = exp2_fast(fmaf(x[half][n][e], to_log2[n][e & 1], -top[n][e & 1]));
 #pragma unroll
             for (int c = 0; c < 2; ++c) total[n][c] += (x[0][n][c] + x[0][n][c + 2]) + (x[1][n][c] + x[1][n][c + 2]);
         }
