@@ -30,26 +30,29 @@ int sm_count_4bit() {
 }  // namespace
 
 // How a call is dealt out, by the longest sequences that the tables could name: n > 0 blocks in even shares whose parts a second kernel joins (as many
-// as the SMs hold at once, or as many as there are heads or least shares), or -n: a cluster of n blocks a head.  The second kernel and
-// the look at all lengths take some 4 us, which is what a block needs for kApart4 turns; clusters are taken where the fullest SM has no more
-// turns than that above an even share.
-constexpr int kApart4 = 25;
+// as the SMs hold at once, or as many as there are heads or least shares), or -n: a cluster of n blocks a head.  What ends first, by what was measured
+// of heads of 128: with b blocks an SM a warp's turn takes 0.35 + 0.5 b us and a block's start and end 1 us more for each, and even shares 4 us for the
+// second kernel and the look at all lengths.  (us, clusters of 1, 2, 4, 8 and even shares, 32 / 8 heads; sequences of half to all of so many keys:
+// 1 of 900  9.0, 7.3, 6.2, 5.4, 9.9;  8 of 1,024  9.0, 7.8, 8.6, 12.5, 12.7;  8 of 4,096  26, 17.3, 14.8, 18.6, 17.4;  16 of 8,000  49, 36.3, 40, 42, 36.4;
+// 64 of 1,024  23.6, 29, 39, 68, 30;  64 of 8,192  161, -, -, -, 106.)
 PB_EXPORT int pb_attention_4bit_blocks(int dtype, int most_tokens, int n_seqs, int Hq, int Hkv, int D, int width, int page_size, int window) {
     if (Hkv <= 0 || Hq <= 0 || D <= 0 || most_tokens <= 0 || n_seqs <= 0 || width <= 0 || page_size <= 0) return 1;
-    const int rows = pb_attention_4bit_rows(dtype, most_tokens * (Hq / Hkv), D), sms = sm_count_4bit();
+    const int rows = pb_attention_4bit_rows(dtype, most_tokens * (Hq / Hkv), D), sms = sm_count_4bit(), held = blocks_4bit(dtype == PB_F32, D / kGroup4, rows);
     const long long row_blocks = ((long long)most_tokens * (Hq / Hkv) + rows - 1) / rows;
     long long keys = (long long)width * page_size;
     if (window > 0 && keys > (long long)window + most_tokens + 16) keys = (long long)window + most_tokens + 16;
     const long long heads = n_seqs * row_blocks * Hkv, of_head = (keys + kTile4 - 1) / kTile4, turns = heads * of_head, parts = (turns + kLeastShare4 - 1) / kLeastShare4;
-    const int most = sms * blocks_4bit(dtype == PB_F32, D / kGroup4, rows);
+    const int most = sms * held;
     if (row_blocks * Hkv <= 65535) {
-        long long best = turns / sms + kApart4 + 1;
+        // in twentieths of a microsecond
+        long long best = (turns + most * kWarps4 - 1) / (most * kWarps4) * (7 + 10 * held) + 20 * held + 80;
         int cluster = 0;
-        for (int n = 8; n >= 1; n /= 2) {
-            if (n > 1 && (heads * n > most || of_head < 3 * n)) continue;          // one wave of blocks, a turn for most of their warps
-            const long long fullest = (heads * n + sms - 1) / sms * ((of_head + n - 1) / n);
-            if (fullest < best) {
-                best = fullest;
+        for (int n = 1; n <= 8; n *= 2) {
+            if (n > 1 && (heads * n > most || of_head < 3 * n)) continue;        // one wave of blocks, a turn for most of their warps
+            const long long blocks = (heads * n + sms - 1) / sms, a_warp = (of_head + n * kWarps4 - 1) / (n * kWarps4);
+            const long long takes = a_warp * (blocks <= held ? 7 + 10 * blocks : (7 + 10 * held) * blocks / held) + 20 * blocks;
+            if (takes < best) {
+                best = takes;
                 cluster = n;
             }
         }

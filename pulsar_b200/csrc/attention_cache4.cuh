@@ -33,6 +33,7 @@ namespace pb {
 
 constexpr int kTile4 = 32;              // keys of a warp's turn: two halves of 16
 constexpr int kWarps4 = 4;
+constexpr int kFold4 = 4;               // turns after which values' offsets are taken off (a power of two)
 constexpr float kLowest4 = -3.0e38f;    // a running maximum before the first key
 
 struct Attend4 {
@@ -145,8 +146,16 @@ __device__ __forceinline__ uint32_t centred(uint32_t raw) {
     const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&raw), __floats2bfloat162_rn(136.0f, 136.0f));
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    const __half2 v = __floats2half2_rn(lo, hi);
+// c - 8 in float16's normal numbers, exactly, of the bits of c and of c << 4.  (float32: the products line subnormal numbers up by the exponent that they
+// would have if they were normal, and lose up to ten bits of what they cut off: 1.5e-6 of an output, as it is 3e-7.)
+__device__ __forceinline__ uint32_t centred_low(uint32_t bits) {
+    const uint32_t raw = bits | 0x64006400u;                    // 1,024 + c
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&raw), __floats2half2_rn(1032.0f, 1032.0f));
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t centred_high(uint32_t bits) {
+    const uint32_t raw = bits | 0x64006400u;                    // 1,024 + 16 c
+    const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&raw), __floats2half2_rn(0.0625f, 0.0625f), __floats2half2_rn(-72.0f, -72.0f));
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 template <int BYTES> __device__ __forceinline__ void load_shared(uint32_t addr, uint32_t* v) {
@@ -174,8 +183,10 @@ struct Attend4Block {
     static constexpr int W = kPairs ? G / 2 : G;            // accumulators of 32 channels: of two groups, one for each kind of copy, or of one
     static constexpr bool kExact = sizeof(T) == 4;          // float32: operands of the products in three bfloat16 terms, codes about zero
     static constexpr int kTerms = kExact ? 3 : 1;
-    // Values keep the offset of their codes, and 136 times the sum of the weights goes through the same products to be taken off at the end: what that
-    // loses of float32 sums 16 times as large as the result is bounded by the length of a part.  Where there are copies, whose weights share a product.
+    static constexpr float kCodeUp = kExact ? 1.0f : 0x1p24f;           // a code over the operand that stands for it
+    // Values keep the offset of their codes, and 136 times the sum of the weights goes through the same products to be taken off every kFold4 turns: the
+    // sums are some 16 times as large as the result meanwhile, and the products cut off where float32 rounds (taken off at the end only, outputs
+    // of 8,192 keys were 3.0e-3 off, as they are 2.3e-3).  Where there are copies, whose weights share a product.
     static constexpr bool kOffsets = !kExact && COPIES > 1;
     static constexpr int kRow = 16 * G;                     // bytes of a row of codes
     static constexpr int kBuffers = G <= 4 ? 3 : 2;         // a warp's buffers
@@ -226,7 +237,7 @@ struct Attend4Block {
     }
 
     // State of a warp.  Lane (r, t) = (lane / 4, lane % 4) holds columns 2 t and 2 t + 1 of 8 for each of NT; they belong to copy t COPIES / 4.
-    float q_sum[NT][GH][2];                 // sum of a column's q over a group of its copy, times 2^-24
+    float q_sum[NT][GH][2];                 // sum of a column's q over a group of its copy, over kCodeUp
     float to_log2[NT][2];                   // from a column's sums of products to scores in base 2; above zero (a scale's sign is q's)
     uint32_t bf16_bits;
     uint32_t first_of, second_of;           // byte selections: the first (second) of two weights, where column r's copy wants it, beside zero
@@ -271,7 +282,7 @@ struct Attend4Block {
             const int k = min(126, max(-112, (int)(__float_as_uint(most) >> 23) - 127)) - 14;
             const float down = copysignf(__int_as_float((127 - k) << 23), scale_log2);
             if (warp == 0 && t == 0)
-                asm volatile("st.shared.f32 [%0], %1;" ::"r"(q_at + kQLog2 + (n * 8 + r) * 4), "f"(fmaxf(1.2e-38f, __int_as_float((127 + k) << 23) * 0x1p24f * fabsf(scale_log2))) : "memory");      // -inf stays so times it
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(q_at + kQLog2 + (n * 8 + r) * 4), "f"(fmaxf(1.2e-38f, __int_as_float((127 + k) << 23) * kCodeUp * fabsf(scale_log2))) : "memory");      // -inf stays so times it
 #pragma unroll
             for (int g = 0; g < GH; ++g) {
                 if (g % kWarps4 != warp && GH >= kWarps4) continue;
@@ -279,14 +290,15 @@ struct Attend4Block {
                 float sum = 0.0f, (&v)[8] = raw.v[n][g];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] *= down;
-                // channels of odd number stand 16 times as high in the codes
+                // channels of odd number stand 16 times as high in the codes, unless those are made normal numbers
+                constexpr float kDown = kExact ? 1.0f : 0.0625f, kUp = kExact ? 1.0f : 16.0f;
 #pragma unroll
                 for (int term = 0; term < kTerms; ++term) {
                     uint32_t held[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const __half h = __float2half_rn(v[e] * (e % 2 ? 0.0625f : 1.0f));
-                        const float back = __half2float(h) * (e % 2 ? 16.0f : 1.0f);
+                        const __half h = __float2half_rn(v[e] * (e % 2 ? kDown : 1.0f));
+                        const float back = __half2float(h) * (e % 2 ? kUp : 1.0f);
                         v[e] -= back;
                         sum += back;
                         held[e] = __half_as_ushort(h);
@@ -311,7 +323,7 @@ struct Attend4Block {
                 }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                if (t == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(q_at + kQSums + ((n * GH + g) * 8 + r) * 4), "f"(sum * 0x1p-24f) : "memory");
+                if (t == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(q_at + kQSums + ((n * GH + g) * 8 + r) * 4), "f"(sum / kCodeUp) : "memory");
             }
         }
     }
@@ -343,6 +355,21 @@ struct Attend4Block {
         }
     }
 
+    __device__ __forceinline__ void fold_offsets() {
+        if constexpr (kOffsets) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+#pragma unroll
+                    for (int w = 0; w < W; ++w)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) o[n][w][u][c] -= offsets[n][2 * w / COPIES][c];
+#pragma unroll
+                    for (int j = 0; j < GH; ++j) offsets[n][j][c] = 0.0f;
+                }
+        }
+    }
     // Words of channels 4 r .. + 3 for two columns of the operand: channels 2 u in its rows r, 2 u + 1 in its rows r + 8.
     __device__ __forceinline__ void value_operands(const uint32_t (&z)[2], uint32_t (&a)[2][4]) const {
 #pragma unroll
@@ -431,7 +458,10 @@ struct Attend4Block {
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) ka[half][i][e] = (i ? y[e & 1] >> 8 : y[e & 1]) & (e < 2 ? 0x000f000fu : 0x00f000f0u);
+                            for (int e = 0; e < 4; ++e) {
+                                ka[half][i][e] = (i ? y[e & 1] >> 8 : y[e & 1]) & (e < 2 ? 0x000f000fu : 0x00f000f0u);
+                                if constexpr (kExact) ka[half][i][e] = e < 2 ? centred_low(ka[half][i][e]) : centred_high(ka[half][i][e]);
+                            }
                     }
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
@@ -452,7 +482,9 @@ struct Attend4Block {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const uint32_t word = s[half][e >> 1][j];
-                        const float step = __uint_as_float(word << 16), least = __uint_as_float(word & 0xffff0000u);
+                        const float step = __uint_as_float(word << 16);
+                        float least = __uint_as_float(word & 0xffff0000u);
+                        if constexpr (kExact) least = fmaf(8.0f, step, least);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             const float m = j == 0 ? least * q_sum[n][j][e & 1] : fmaf(least, q_sum[n][j][e & 1], x[half][n][e]);
@@ -830,10 +862,12 @@ __device__ __forceinline__ void attend_part(const Attend4& a, const Entry4& entr
                 return !turns.holes || (key >= head.first && key <= head.last && page_of(a, head, key, place) >= 0);
             });
         });
+        if ((i & (kFold4 - 1)) == kFold4 - 1) b.fold_offsets();
         free = stage;
         stage = stage == ring + (B::kBuffers - 1) * B::kStage ? ring : stage + B::kStage;
         __syncwarp();
     }
+    b.fold_offsets();
     cp_async_wait<0>();
     __syncwarp();
     // The warp's sums to its own shared memory (the ring is done with): [column][D], then maxima and totals.
@@ -852,7 +886,6 @@ __device__ __forceinline__ void attend_part(const Attend4& a, const Entry4& entr
                 least[j] = b.least_sum[n][j][c];
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) least[j] += __shfl_xor_sync(0xffffffffu, least[j], off);
-                if (B::kOffsets) least[j] -= b.offsets[n][j][c];
             }
 #pragma unroll
             for (int w = 0; w < B::W; ++w) {
