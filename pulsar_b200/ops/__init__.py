@@ -2320,11 +2320,6 @@ def _launch_expand(name: str, kind: int, pools, table: int, kv_len: int, k_out: 
     check(fn("pb_expand_pages_4bit")(_EXPAND_4BIT.pack(kind, *pools, table, kv_len, k_out, v_out, table_out, *sizes), stream()), name)
 
 
-# Rows of a kv head (its query heads times a sequence's tokens) above which portions are attended to in two steps, where a dense kernel of the
-# tensor cores takes their sizes: the sequences' pages as bfloat16 (``expand_pages_4bit``), then that kernel.
-EXPANDED_ROWS_4BIT = 64
-
-
 @functools.lru_cache(maxsize=1024)
 def scratch_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int, width: int, page_size: int, window: int, dtype: torch.dtype) -> Tuple[int, int, int]:
     """(blocks, float32 elements of sums, int32 elements of the plan) of ``paged_attention_4bit`` for sequences of up to ``most_tokens`` tokens; blocks below
@@ -2337,13 +2332,31 @@ def scratch_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads: int, h
     return blocks, blocks * 2 * rows * (head_dim + 2), 2 + n_seqs * -(-rows_all // rows)
 
 
-def _expanded_4bit(dtype: torch.dtype, rows: int, n_heads: int, n_kv_heads: int, head_dim: int, page_size: int, scale: float) -> Optional[str]:
-    """The dense kernel that attends to portions of so many rows over expanded pages, or None: the kernel on codes does."""
-    if dtype != torch.bfloat16 or rows <= EXPANDED_ROWS_4BIT or not scale > 0.0:
+@functools.lru_cache(maxsize=1024)
+def expanded_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int, width: int, page_size: int, window: int, dtype: torch.dtype) -> Optional[str]:
+    """The dense kernel of the tensor cores ("tcgen05" or "tc") that attends to portions over expanded pages, or None: the kernel on codes does.
+
+    The kernel on codes takes what its blocks' turns take: 0.235 us a turn of 32 keys and 16 rows and SM (heads of 64: two thirds of that), and 16 turns'
+    time for a block's start and end.  Expanded pages cost their bytes twice, and the dense kernels some 13.5 ns a key for as many tiles of query
+    tokens as there are SMs.  (us on codes and expanded, heads 32 / 8 of 128, sequences of 0.7 to all of so many keys, 16 / 128 / 512 rows a kv head:
+    1 of 1,000  8.8, 24;  12.4, 24;  20, 25;    1 of 8,000  16, 122;  33, 123;  113, 124;    8 of 1,000  13, 29;  57, 30;  179, 32;
+    8 of 4,000  20, 90;  115, 91;  409, 93;    1 of 6,000 with 2,048 rows  318, 97.)"""
+    if dtype != torch.bfloat16:
         return None
+    kernel = None
     if ATTENTION_BACKEND != "mma" and prefill_tcgen05_supported(dtype, n_heads, n_kv_heads, head_dim, page_size):
-        return "tcgen05"
-    return "tc" if prefill_tc_supported(dtype, n_heads, n_kv_heads, head_dim, page_size) else None
+        kernel = "tcgen05"
+    elif prefill_tc_supported(dtype, n_heads, n_kv_heads, head_dim, page_size):
+        kernel = "tc"
+    if kernel is None:
+        return None
+    keys = min(width * page_size, window + most_tokens) if window else width * page_size
+    rows = most_tokens * (n_heads // n_kv_heads)
+    blocks = n_seqs * n_kv_heads * -(-rows // fn("pb_attention_4bit_rows")(code(dtype), rows, head_dim))
+    on_codes = 7 + blocks * (keys / 32 + 16) / 148 * 0.235 * (0.67 if head_dim <= 64 else 1.0)
+    tiles = n_seqs * -(-most_tokens // 128) * n_heads / 2 / 148
+    expanded = 12 + n_seqs * keys * n_kv_heads * head_dim * 5.25 / 6.2e6 + keys * 0.0135 * max(1.0, tiles)
+    return kernel if expanded < on_codes else None
 
 
 def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.Tensor, v_pool: torch.Tensor, v_steps: torch.Tensor, out: torch.Tensor,
@@ -2355,9 +2368,9 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
     them.  A query sees the keys up to its own, with ``window`` w the last w of them; those have to lie in pages of the pool (an id that is
     none is not read).  A query that sees no key gets zeros.  Rows of ``out`` that are no sequence's stay as they were.
 
-    bfloat16 portions of more than 64 rows a kv head (query heads times tokens), where the dense attention of prompt portions has a kernel
-    for their sizes and the scale is above zero, are attended to over expanded pages, which takes room for S * width pages.  (There a value that is NaN also
-    reaches the tokens of its sequence's portion that do not see it.)  ``scratch(tag, shape, dtype)`` gives tensors to work in; without it they are made here."""
+    bfloat16 portions of many tokens, where the dense attention of prompt portions has a kernel for their sizes, are attended to over expanded
+    pages (``expanded_4bit``), which takes room for S * width pages.  (There values are rounded to bfloat16, and a value that is NaN also reaches the tokens of its
+    sequence's portion that do not see it.)  ``scratch(tag, shape, dtype)`` gives tensors to work in; without it they are made here."""
     name = "paged_attention_4bit"
     tensors = (q, k_pool, k_steps, v_pool, v_steps, out, block_table, kv_len)
     if (where := _on_one_device(name, (*tensors, cu_q))) != _current_device():
@@ -2398,7 +2411,7 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
         return
     _check_against(k_pool)
     pools = k_pool.data_ptr(), k_steps.data_ptr(), v_pool.data_ptr(), v_steps.data_ptr()
-    dense = None if cu_q is None else _expanded_4bit(dtype, most_tokens * (hq // hkv), hq, hkv, d, page_size, scale)
+    dense = None if cu_q is None or not scale > 0.0 else expanded_4bit(s, most_tokens, hq, hkv, d, width, page_size, window, dtype)
     if dense is not None:
         shapes = ((s * width, hkv, page_size, d), dtype), ((s * width, hkv, page_size, d), dtype), ((s, width), torch.int32)
         if scratch is None:

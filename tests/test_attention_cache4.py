@@ -176,6 +176,47 @@ def test_wide_tables_and_the_same_bits():
     c.check(block_table=c.table(width=700).cuda())
 
 
+# (lengths, tokens or None, query and kv heads, head_dim, page, window, how a call of bfloat16 is dealt out: -n for a cluster of n blocks a head, 0 for even shares)
+DEALT = [([30], None, 8, 2, 128, 16, None, -1),
+         ([1090, 33, 0], None, 8, 2, 128, 16, None, -8),
+         ([2050, 0, 5, 1, 700, 31, 32, 33, 257], None, 36, 9, 64, 3, None, -4),
+         ([1500, 40], None, 12, 4, 96, 5, 200, -2),
+         ([107 * i + 7 for i in range(18)], None, 16, 8, 128, 16, None, -2),
+         ([490, 0, 100, 27] * 10, [5, 0, 3, 5] * 10, 8, 2, 96, 7, None, -1),
+         ([1600, 77, 900, 4], [5, 1, 5, 4], 24, 2, 128, 16, None, -4),
+         ([14399, 3, 0, 450, 1], None, 8, 1, 128, 16, None, 0),
+         ([11000, 2500, 20], [20, 1, 20], 24, 2, 128, 8, None, 0),
+         ([11000, 2500, 9000, 20], [20, 1, 3, 20], 24, 2, 128, 8, 5000, 0),
+         ([(331 * i) % 1920 for i in range(150)], None, 8, 2, 64, 16, None, 0)]
+
+
+def dealt_out(case, dtype):
+    most = max(case.q_lens)
+    return ops.scratch_4bit(len(case.q_lens), most, case.q.shape[1], case.cache.hkv, case.cache.dim, case.table().shape[1], case.cache.page, case.window or 0, dtype)[0]
+
+
+@cuda
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("lens,q_lens,hq,hkv,dim,page,window,how", DEALT)
+def test_every_way_to_deal_a_call_out(dtype, lens, q_lens, hq, hkv, dim, page, window, how):
+    c = Case(lens, hq, hkv, dim, page, dtype, len(lens) + dim, q_lens, window=window)
+    if dtype == torch.bfloat16:
+        assert min(dealt_out(c, dtype), 0) == how
+    c.check()
+    table = c.cache.table().cuda()
+    short = on([n // 3 if q_lens is None else min(n, count + n // 3) for n, count in zip(lens, c.q_lens)])            # the lengths alone say what is read
+    few = Case(short.tolist(), hq, hkv, dim, page, dtype, len(lens) + dim, q_lens)
+    few.cache.tables, few.cache.pools, few.q, few.window = c.cache.tables, c.cache.pools, c.q, window
+    few.check(block_table=table)
+
+
+def test_portions_of_many_rows_take_expanded_pages():
+    for tokens, width, want in ((1, 128, None), (4, 250, None), (64, 250, True), (512, 500, True)):
+        assert (ops.expanded_4bit(8, tokens, 32, 8, 128, width, 16, 0, torch.bfloat16) is not None) == bool(want)
+        assert ops.expanded_4bit(8, tokens, 32, 8, 128, width, 16, 0, torch.float32) is None
+        assert ops.expanded_4bit(8, tokens, 32, 8, 96, width, 6, 0, torch.bfloat16) is None
+
+
 @cuda
 def test_many_sequences_of_unlike_length():
     lens = [(37 * i) % 900 for i in range(150)]
