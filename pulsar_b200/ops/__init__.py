@@ -2333,30 +2333,34 @@ def scratch_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads: int, h
 
 
 @functools.lru_cache(maxsize=1024)
-def expanded_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int, width: int, page_size: int, window: int, dtype: torch.dtype) -> Optional[str]:
-    """The dense kernel of the tensor cores ("tcgen05" or "tc") that attends to portions over expanded pages, or None: the kernel on codes does.
+def _expanded_pays_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int, width: int, page_size: int, window: int) -> bool:
+    """Whether bfloat16 portions end sooner over expanded pages, by what is measured of either way.
 
     The kernel on codes takes what its blocks' turns take: 0.235 us a turn of 32 keys and 16 rows and SM (heads of 64: two thirds of that), and 16 turns'
     time for a block's start and end.  Expanded pages cost their bytes twice, and the dense kernels some 13.5 ns a key for as many tiles of query
     tokens as there are SMs.  (us on codes and expanded, heads 32 / 8 of 128, sequences of 0.7 to all of so many keys, 16 / 128 / 512 rows a kv head:
     1 of 1,000  8.8, 24;  12.4, 24;  20, 25;    1 of 8,000  16, 122;  33, 123;  113, 124;    8 of 1,000  13, 29;  57, 30;  179, 32;
     8 of 4,000  20, 90;  115, 91;  409, 93;    1 of 6,000 with 2,048 rows  318, 97.)"""
-    if dtype != torch.bfloat16:
-        return None
-    kernel = None
-    if ATTENTION_BACKEND != "mma" and prefill_tcgen05_supported(dtype, n_heads, n_kv_heads, head_dim, page_size):
-        kernel = "tcgen05"
-    elif prefill_tc_supported(dtype, n_heads, n_kv_heads, head_dim, page_size):
-        kernel = "tc"
-    if kernel is None:
-        return None
     keys = min(width * page_size, window + most_tokens) if window else width * page_size
     rows = most_tokens * (n_heads // n_kv_heads)
-    blocks = n_seqs * n_kv_heads * -(-rows // fn("pb_attention_4bit_rows")(code(dtype), rows, head_dim))
+    blocks = n_seqs * n_kv_heads * -(-rows // fn("pb_attention_4bit_rows")(code(torch.bfloat16), rows, head_dim))
     on_codes = 7 + blocks * (keys / 32 + 16) / 148 * 0.235 * (0.67 if head_dim <= 64 else 1.0)
     tiles = n_seqs * -(-most_tokens // 128) * n_heads / 2 / 148
     expanded = 12 + n_seqs * keys * n_kv_heads * head_dim * 5.25 / 6.2e6 + keys * 0.0135 * max(1.0, tiles)
-    return kernel if expanded < on_codes else None
+    return expanded < on_codes
+
+
+# Bytes that expanded pages may take, unless one sequence's alone are more: portions of more sequences than that holds are runs of calls.
+EXPANDED_ROOM_4BIT = 1 << 30
+
+
+def expanded_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int, width: int, page_size: int, window: int, dtype: torch.dtype) -> Optional[str]:
+    """The dense kernel of the tensor cores ("tcgen05" or "tc") that attends to portions over expanded pages, or None: the kernel on codes does."""
+    if dtype != torch.bfloat16 or not _expanded_pays_4bit(n_seqs, most_tokens, n_heads, n_kv_heads, head_dim, width, page_size, window):
+        return None
+    if ATTENTION_BACKEND != "mma" and prefill_tcgen05_supported(dtype, n_heads, n_kv_heads, head_dim, page_size):
+        return "tcgen05"
+    return "tc" if prefill_tc_supported(dtype, n_heads, n_kv_heads, head_dim, page_size) else None
 
 
 def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.Tensor, v_pool: torch.Tensor, v_steps: torch.Tensor, out: torch.Tensor,
@@ -2366,10 +2370,11 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
     the keys of this step in it.  Without ``cu_q`` every sequence has one query token, the last (N = S); else sequence i has the tokens
     ``cu_q[i]:cu_q[i + 1]`` (int32 [S + 1], rising, rows of q), the last of its ``kv_len[i]``, and ``q_lens`` are their numbers as the host knows
     them.  A query sees the keys up to its own, with ``window`` w the last w of them; those have to lie in pages of the pool (an id that is
-    none is not read).  A query that sees no key gets zeros.  Rows of ``out`` that are no sequence's stay as they were.
+    none is not read).  (``kv_len[i]`` is no more than the table's width holds.)  A query that sees no key gets zeros.  Rows of ``out`` that are no sequence's stay as
+    they were.
 
     bfloat16 portions of many tokens, where the dense attention of prompt portions has a kernel for their sizes, are attended to over expanded
-    pages (``expanded_4bit``), which takes room for S * width pages.  (There values are rounded to bfloat16, and a value that is NaN also reaches the tokens of its
+    pages (``expanded_4bit``), which takes room for S * width pages, of as many sequences at a time as 1 GiB holds.  (There values are rounded to bfloat16, and a value that is NaN also reaches the tokens of its
     sequence's portion that do not see it.)  ``scratch(tag, shape, dtype)`` gives tensors to work in; without it they are made here."""
     name = "paged_attention_4bit"
     tensors = (q, k_pool, k_steps, v_pool, v_steps, out, block_table, kv_len)
@@ -2411,24 +2416,35 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
         return
     _check_against(k_pool)
     pools = k_pool.data_ptr(), k_steps.data_ptr(), v_pool.data_ptr(), v_steps.data_ptr()
-    dense = None if cu_q is None or not scale > 0.0 else expanded_4bit(s, most_tokens, hq, hkv, d, width, page_size, window, dtype)
-    if dense is not None:
-        shapes = ((s * width, hkv, page_size, d), dtype), ((s * width, hkv, page_size, d), dtype), ((s, width), torch.int32)
-        if scratch is None:
-            k_out, v_out, table_out = (torch.empty(shape, dtype=kept, device=q.device) for shape, kept in shapes)
-        else:
-            k_out, v_out, table_out = (scratch(f"attn4.{what}", shape, kept) for what, (shape, kept) in zip(("k", "v", "table"), shapes))
-        _launch_expand(name, kind, pools, block_table.data_ptr(), kv_len.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), table_out.data_ptr(), s, width, hkv, d, page_size,
-                       n_pages, cu_q.data_ptr(), window)
-        run, tiles = (paged_attention_prefill_tcgen05, prefill_tcgen05_tiles) if dense == "tcgen05" else (paged_attention_prefill_tc, prefill_tc_tiles)
-        run(q, k_out, v_out, out, table_out, cu_q, kv_len, tiles(q_lens), scale, window)
-        return
+    q_at, out_at = q.data_ptr(), out.data_ptr()
+    if (q_at | out_at | pools[0] | pools[1] | pools[2] | pools[3]) % 16:
+        _refuse_16(name)
+    if cu_q is not None and scale > 0.0:
+        run_of = min(s, max(1, EXPANDED_ROOM_4BIT // (4 * width * hkv * page_size * d)))
+        dense = expanded_4bit(run_of, most_tokens, hq, hkv, d, width, page_size, window, dtype)
+        if dense is not None:
+            run, tiles = (paged_attention_prefill_tcgen05, prefill_tcgen05_tiles) if dense == "tcgen05" else (paged_attention_prefill_tc, prefill_tc_tiles)
+            shapes = ((run_of * width, hkv, page_size, d), dtype), ((run_of * width, hkv, page_size, d), dtype), ((run_of, width), torch.int32)
+            if scratch is None:
+                k_out, v_out, table_out = (torch.empty(shape, dtype=kept, device=q.device) for shape, kept in shapes)
+            else:
+                k_out, v_out, table_out = (scratch(f"attn4.{what}", shape, kept) for what, (shape, kept) in zip(("k", "v", "table"), shapes))
+            for first in range(0, s, run_of):
+                end = min(first + run_of, s)
+                lens = q_lens[first:end]
+                if not any(lens):
+                    continue
+                table, kv, cu = block_table[first:end], kv_len[first:end], cu_q[first:end + 1]
+                _launch_expand(name, kind, pools, table.data_ptr(), kv.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), table_out.data_ptr(), end - first, width, hkv, d,
+                               page_size, n_pages, cu.data_ptr(), window)
+                run(q, k_out, v_out, out, table_out[:end - first], cu, kv, tiles(lens), scale, window)
+            return
     blocks, sums, plan = scratch_4bit(s, most_tokens, hq, hkv, d, width, page_size, window, dtype)
-    work_at, q_at, out_at = 0, q.data_ptr(), out.data_ptr()
+    work_at = 0
     if sums:
         work = torch.empty(sums + plan, dtype=torch.float32, device=q.device) if scratch is None else scratch("attn4.work", (sums + plan,), torch.float32)
         work_at = work.data_ptr()
-    if (q_at | out_at | work_at | pools[0] | pools[1] | pools[2] | pools[3]) % 16:
+    if work_at % 16:
         _refuse_16(name)
     words = _ATTEND_4BIT.pack(kind, q_at, *pools, out_at, work_at, work_at + 4 * sums, block_table.data_ptr(), kv_len.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
                               width, n, most_tokens, s, hq, hkv, d, page_size, n_pages, scale, window, blocks)

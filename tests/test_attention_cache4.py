@@ -218,6 +218,33 @@ def test_portions_of_many_rows_take_expanded_pages():
 
 
 @cuda
+@pytest.mark.parametrize("window", [None, 100])
+@pytest.mark.parametrize("room", [1, 3 * 4 * 25 * 2 * 16 * 128])
+def test_expanded_pages_of_a_few_sequences_at_a_time(room, window, monkeypatch):
+    """Sequences over whose pages too much room would go are taken in runs; rows of none stay."""
+    c = Case([400, 130, 0, 390, 64, 100, 40], 8, 2, 128, 16, torch.bfloat16, 31, [300, 130, 0, 260, 0, 100, 33], window=window)
+    monkeypatch.setattr(ops, "_expanded_pays_4bit", lambda *a: True)
+    want = c.check()
+    monkeypatch.setattr(ops, "EXPANDED_ROOM_4BIT", room)
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got = c.run()
+    assert torch.equal(got.double().cpu(), want)
+    assert torch.cuda.max_memory_allocated() - before < max(room, 4 * 25 * 2 * 16 * 128) + 8 * c.q.numel() + (4 << 20)
+
+
+@cuda
+@pytest.mark.parametrize("lens,q_lens,window", [([400, 130], [5, 130], None), ([300, 1, 20], [3, 1, 20], 7), ([64], [64], None), ([1], [1], None)])
+@pytest.mark.parametrize("hq,hkv,dim,page", [(32, 8, 128, 16), (8, 1, 64, 8), (4, 4, 128, 64)])
+def test_either_way_of_portions(lens, q_lens, window, hq, hkv, dim, page, monkeypatch):
+    """Short portions over expanded pages, long ones on codes: whichever way a rule takes, the sums are the formula's."""
+    c = Case(lens, hq, hkv, dim, page, torch.bfloat16, 32, q_lens, window=window)
+    for pays in (True, False):
+        monkeypatch.setattr(ops, "_expanded_pays_4bit", lambda *a: pays)
+        c.check()
+
+
+@cuda
 def test_many_sequences_of_unlike_length():
     lens = [(37 * i) % 900 for i in range(150)]
     Case(lens, 8, 2, 64, 16, torch.bfloat16, 14).check()
