@@ -2306,6 +2306,8 @@ def expand_pages_4bit(k_pool: torch.Tensor, k_steps: torch.Tensor, v_pool: torch
         raise KernelError(f"{name}: {s} sequences of {width} pages need as many pages to go to, found {out_pages}")
     if s == 0 or width == 0:
         return
+    if abs(table_out.data_ptr() - block_table.data_ptr()) < 4 * s * width:
+        raise KernelError(f"{name}: the new block table must not lie over the old one")
     if shape[0] == 0:
         table_out.fill_(-1)
         return
@@ -2408,6 +2410,8 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
         window = 0
     elif window <= 0:
         raise KernelError(f"{name}: a window must be positive, found {window}")
+    elif window >= width * page_size:            # as wide as all keys
+        window = 0
     if n == 0 or s == 0 or most_tokens == 0:
         return
     if width == 0 or n_pages == 0:               # nobody has a key

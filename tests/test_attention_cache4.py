@@ -234,6 +234,18 @@ def test_expanded_pages_of_a_few_sequences_at_a_time(room, window, monkeypatch):
 
 
 @cuda
+@pytest.mark.parametrize("q_lens", [None, [90, 33, 200]])
+def test_windows_as_wide_as_all_keys_and_queries_as_outputs(q_lens):
+    c = Case([90, 33, 400], 8, 2, 128, 16, torch.bfloat16, 33, q_lens)
+    want = c.run()
+    for window in (401, (1 << 31) - 1, 1 << 40):
+        assert torch.equal(c.run(window=window), want)
+    if q_lens is None:                         # a row of q is read before anything is written to it
+        q = c.q.cuda()
+        assert torch.equal(c.run(q=q, out=q), want)
+
+
+@cuda
 @pytest.mark.parametrize("lens,q_lens,window", [([400, 130], [5, 130], None), ([300, 1, 20], [3, 1, 20], 7), ([64], [64], None), ([1], [1], None)])
 @pytest.mark.parametrize("hq,hkv,dim,page", [(32, 8, 128, 16), (8, 1, 64, 8), (4, 4, 128, 64)])
 def test_either_way_of_portions(lens, q_lens, window, hq, hkv, dim, page, monkeypatch):

@@ -236,6 +236,9 @@ def test_refusals_of_the_expansion():
                           (dict(k_steps=c.pools[1][:3].cuda()), "steps bfloat16"), (dict(k_out=small.half(), v_out=small.half()), "float32 or bfloat16")):
         with pytest.raises(ops.KernelError, match=said):
             run(**changed)
+    table = c.table().cuda()
+    with pytest.raises(ops.KernelError, match="lie over"):
+        run(block_table=table, table_out=table)
     run(block_table=c.table()[:0].cuda(), kv_len=on([]), table_out=c.table()[:0].cuda())
     table_out = c.table().cuda()
     run(k_pool=c.pools[0][:0].cuda(), k_steps=c.pools[1][:0].cuda(), v_pool=c.pools[2][:0].cuda(), v_steps=c.pools[3][:0].cuda(), table_out=table_out)
