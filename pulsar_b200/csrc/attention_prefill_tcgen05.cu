@@ -457,18 +457,19 @@ PB_EXPORT int pb_prefill_tcgen05_wait_control(long long limit, int error, void**
 }
 
 // q, out [N, Hq, D] bfloat16; pools [n_pages, Hkv, page_size, D] bfloat16 with finite contents;
-// n_q_tiles = sum over sequences of ceil(q_len / pb_prefill_tcgen05_tile()).
+// n_q_tiles = sum over sequences of ceil(q_len / pb_prefill_tcgen05_tile()); heads: query heads a block takes where their kv head has an even
+// number, 0 for two (or what PULSAR_ATTENTION_HEADS says).
 PB_EXPORT int pb_paged_attention_prefill_tcgen05(int dtype, const void* q, const void* k_pool, const void* v_pool, void* out,
                                                  const int* block_table, int table_stride, const int* cu_q,
                                                  const int* kv_len, int n_tokens, int n_seqs, int n_q_tiles, int n_pages,
                                                  int Hq, int Hkv, int D, int page_size, float scale, int window,
-                                                 cudaStream_t stream) {
+                                                 int heads, cudaStream_t stream) {
     if (n_seqs <= 0 || n_q_tiles <= 0 || n_tokens <= 0) return 0;
     if (!pb_prefill_tcgen05_supported(dtype, Hq, Hkv, D, page_size)) return PB_ERR_BAD_SIZE;
     const long long items = (long long)n_q_tiles * Hq;
     if (items >= (1LL << 30)) return PB_ERR_TOO_LARGE;
     if ((((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out) & 15) != 0) return PB_ERR_BAD_SIZE;
-    if (heads_per_block() == 2 && dual_supported(Hq, Hkv))
+    if ((heads > 0 ? heads : heads_per_block()) == 2 && dual_supported(Hq, Hkv))
         return launch_dual(q, k_pool, v_pool, out, block_table, table_stride, cu_q, kv_len, n_tokens, n_seqs, n_q_tiles, n_pages, Hq,
                            Hkv, page_size, scale, window, stream);
     const long long pool_rows = (long long)n_pages * Hkv * page_size;

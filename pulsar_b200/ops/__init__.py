@@ -61,7 +61,7 @@ _SIGNATURES = {
     "pb_paged_attention_prefill_tc": [_I, _P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P],
     "pb_prefill_tc_supported": [_I, _I, _I, _I, _I],
     "pb_prefill_tc_tile": [],
-    "pb_paged_attention_prefill_tcgen05": [_I, _P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P],
+    "pb_paged_attention_prefill_tcgen05": [_I, _P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P],
     "pb_prefill_tcgen05_supported": [_I, _I, _I, _I, _I],
     "pb_prefill_tcgen05_tile": [],
     "pb_prefill_tcgen05_error": [],
@@ -1049,9 +1049,9 @@ def prefill_tcgen05_error() -> int:
 
 def paged_attention_prefill_tcgen05(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, out: torch.Tensor,
                                     block_table: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor, n_q_tiles: int,
-                                    scale: float, window: Optional[int]) -> None:
+                                    scale: float, window: Optional[int], heads: int = 0) -> None:
     """tcgen05 attention for a ragged batch of portions (bfloat16, head size 128, pages of 8 or more
-    tokens).  Pool rows that were never written must hold finite values."""
+    tokens).  Pool rows that were never written must hold finite values.  ``heads``: query heads of a block, 1 or 2 (0: two where they pair up)."""
     _cuda(q, k_pool, v_pool, out, block_table, cu_q, kv_len)
     _check_against(k_pool)
     n, hq, d = q.shape
@@ -1064,7 +1064,7 @@ def paged_attention_prefill_tcgen05(q: torch.Tensor, k_pool: torch.Tensor, v_poo
     assert cu_q.numel() == s + 1 and block_table.shape[0] == s
     check(fn("pb_paged_attention_prefill_tcgen05")(code(q.dtype), _p(q), _p(k_pool), _p(v_pool), _p(out), _p(block_table),
                                                    block_table.shape[1], _p(cu_q), _p(kv_len), n, s, n_q_tiles, pages, hq,
-                                                   hkv, d, page_size, float(scale), int(window or 0), stream()),
+                                                   hkv, d, page_size, float(scale), int(window or 0), heads, stream()),
           "paged_attention_prefill_tcgen05")
 
 
@@ -2334,21 +2334,28 @@ def scratch_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads: int, h
     return blocks, blocks * 2 * rows * (head_dim + 2), 2 + n_seqs * -(-rows_all // rows)
 
 
+def _one_head_a_block(head_dim: int, heads: int) -> bool:
+    """Whether the tcgen05 attention of portions takes its query heads (of all tiles of tokens) one a block: where every one has an SM of its own, two a block, which
+    share what they load, take longer for being two.  (us, two and one a block, 6,000 keys: 128 heads 89.6, 56.3; 160 heads 89.7, 100; the same bits.)"""
+    return head_dim == 128 and heads <= 148
+
+
 @functools.lru_cache(maxsize=1024)
 def _expanded_pays_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int, width: int, page_size: int, window: int) -> bool:
     """Whether bfloat16 portions end sooner over expanded pages, by what is measured of either way.
 
     The kernel on codes takes what its blocks' turns take: 0.235 us a turn of 32 keys and 16 rows and SM (heads of 64: two thirds of that), and 16 turns'
-    time for a block's start and end.  Expanded pages cost their bytes twice, and the dense kernels some 13.5 ns a key for as many tiles of query
-    tokens as there are SMs.  (us on codes and expanded, heads 32 / 8 of 128, sequences of 0.7 to all of so many keys, 16 / 128 / 512 rows a kv head:
-    1 of 1,000  8.8, 24;  12.4, 24;  20, 25;    1 of 8,000  16, 122;  33, 123;  113, 124;    8 of 1,000  13, 29;  57, 30;  179, 32;
-    8 of 4,000  20, 90;  115, 91;  409, 93;    1 of 6,000 with 2,048 rows  318, 97.)"""
+    time for a block's start and end.  Expanded pages cost their bytes twice, and the dense kernels 8 ns a key where a block takes one head, else 13 for as
+    many pairs of heads and tiles of query tokens as there are SMs.  (us on codes and expanded, heads 32 / 8 of 128, sequences of 0.7 to all of so many keys,
+    16 / 128 / 512 rows a kv head: 1 of 1,000  8.7, 17;  12, 17;  20, 19;    1 of 8,000  15, 78;  33, 78;  113, 80;    8 of 1,000  13, 29;  57, 31;
+    179, 32;    8 of 4,000  21, 90;  115, 92;  409, 93;    1 of 6,000 with 2,048 rows  318, 62.  The slower side is taken by up to 30 % between them.)"""
     keys = min(width * page_size, window + most_tokens) if window else width * page_size
     rows = most_tokens * (n_heads // n_kv_heads)
     blocks = n_seqs * n_kv_heads * -(-rows // fn("pb_attention_4bit_rows")(code(torch.bfloat16), rows, head_dim))
     on_codes = 7 + blocks * (keys / 32 + 16) / 148 * 0.235 * (0.67 if head_dim <= 64 else 1.0)
-    tiles = n_seqs * -(-most_tokens // 128) * n_heads / 2 / 148
-    expanded = 12 + n_seqs * keys * n_kv_heads * head_dim * 5.25 / 6.2e6 + keys * 0.0135 * max(1.0, tiles)
+    heads = n_seqs * -(-most_tokens // 128) * n_heads
+    a_key = 0.0081 if _one_head_a_block(head_dim, heads) else 0.0133 * max(1.0, heads / 2 / 148)
+    expanded = 11 + n_seqs * keys * n_kv_heads * head_dim * 5.25 / 6.2e6 + keys * a_key
     return expanded < on_codes
 
 
@@ -2376,8 +2383,9 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
     they were.
 
     bfloat16 portions of many tokens, where the dense attention of prompt portions has a kernel for their sizes, are attended to over expanded
-    pages (``expanded_4bit``), which takes room for S * width pages, of as many sequences at a time as 1 GiB holds.  (There values are rounded to bfloat16, and a value that is NaN also reaches the tokens of its
-    sequence's portion that do not see it.)  ``scratch(tag, shape, dtype)`` gives tensors to work in; without it they are made here."""
+    pages (``expanded_4bit``), which takes room for S * width pages, of as many sequences at a time as 1 GiB holds.  (There keys and values are operands rounded to bfloat16, as a cache
+    of bfloat16 holds them: over 6,000 keys outputs are 3.7e-3 off, 2.3e-3 on codes and 1.7e-3 by their own rounding alone; and a value that is NaN also reaches
+    the tokens of its sequence's portion that do not see it.)  ``scratch(tag, shape, dtype)`` gives tensors to work in; without it they are made here."""
     name = "paged_attention_4bit"
     tensors = (q, k_pool, k_steps, v_pool, v_steps, out, block_table, kv_len)
     if (where := _on_one_device(name, (*tensors, cu_q))) != _current_device():
@@ -2438,10 +2446,14 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
                 lens = q_lens[first:end]
                 if not any(lens):
                     continue
+                if first > 0:
+                    _check_against(k_pool)               # the dense kernel has its own pool checked against
                 table, kv, cu = block_table[first:end], kv_len[first:end], cu_q[first:end + 1]
                 _launch_expand(name, kind, pools, table.data_ptr(), kv.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), table_out.data_ptr(), end - first, width, hkv, d,
                                page_size, n_pages, cu.data_ptr(), window)
-                run(q, k_out, v_out, out, table_out[:end - first], cu, kv, tiles(lens), scale, window)
+                n_tiles = tiles(lens)
+                one = (1,) if dense == "tcgen05" and _one_head_a_block(d, n_tiles * hq) else ()
+                run(q, k_out, v_out, out, table_out[:end - first], cu, kv, n_tiles, scale, window, *one)
             return
     blocks, sums, plan = scratch_4bit(s, most_tokens, hq, hkv, d, width, page_size, window, dtype)
     work_at = 0

@@ -257,6 +257,17 @@ def test_either_way_of_portions(lens, q_lens, window, hq, hkv, dim, page, monkey
 
 
 @cuda
+def test_one_and_two_heads_a_block_give_the_same_bits(monkeypatch):
+    c = Case([700, 260], 16, 4, 128, 16, torch.bfloat16, 34, [333, 260])
+    monkeypatch.setattr(ops, "_expanded_pays_4bit", lambda *a: True)
+    got = []
+    for one in (True, False):
+        monkeypatch.setattr(ops, "_one_head_a_block", lambda *a: one)
+        got.append(c.check())
+    assert torch.equal(*got)
+
+
+@cuda
 def test_many_sequences_of_unlike_length():
     lens = [(37 * i) % 900 for i in range(150)]
     Case(lens, 8, 2, 64, 16, torch.bfloat16, 14).check()
