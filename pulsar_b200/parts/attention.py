@@ -95,8 +95,8 @@ class Attention(Mixer):
         self.four_bit = spec.cache_bits == 4
         if spec.cache_bits not in (0, 4):
             raise ValueError(f"attention: keys and values are cached in the activation dtype (0) or in 4 bits, found {spec.cache_bits}")
-        if self.four_bit and (self.general or spec.head_dim % ops.GROUP_4BIT):
-            raise ValueError(f"attention: a cache of 4 bits goes with the dense form and heads of a multiple of {ops.GROUP_4BIT} channels")
+        if self.four_bit and (self.general or spec.head_dim % ops.GROUP_4BIT or spec.head_dim > 256):
+            raise ValueError(f"attention: a cache of 4 bits goes with the dense form and heads of a multiple of {ops.GROUP_4BIT} channels, at most 256")
         self.shares_keys = not self.general and not self.four_bit
         if (self.maps > 1 or spec.q_temperature is not None) and (self.prepared or not spec.own_kv):
             raise ValueError("attention: the differential form and the query temperature go with plain projections of its own keys")

@@ -188,6 +188,8 @@ def test_what_has_no_cache_of_4_bits_is_refused():
     from pulsar_b200.models import build_model
     with pytest.raises(ConfigError, match="multiple of 32"):
         build_model(config_from_dict(helpers.TINY_A), torch.float32, 4)                     # heads of 16
+    with pytest.raises(ConfigError, match="at most 256"):
+        build_model(config_from_dict(dict(helpers.TINY_B, head_dim=288)), torch.float32, 4)
     with pytest.raises(ConfigError, match="0 .* or 4"):
         EngineConfig.from_dict(dict(cache_bits=8))
     with pytest.raises(ConfigError, match="in 4 bits, found 2"):
