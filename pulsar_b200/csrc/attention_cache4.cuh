@@ -19,8 +19,14 @@
 // no lane computes for an empty column what belongs to a group, key and column, and a 32-bit word of codes, whose halves are two
 // neighbouring groups, is an operand as it is: its halves stand in two places of the sum, of which each copy's other operand has one empty.
 // The weights change places between the two products by movmatrix.
-// (tcgen05 would want codes as bfloat16 in shared memory, which is more traffic there than all the rest; what bounds this kernel are instructions
-// on codes and bytes, not products.)
+//
+// What bounds it: instructions.  4 query heads a kv head, heads of 128, bfloat16: 317 warp instructions for 16 keys (a third of them shifts and masks of codes,
+// 18 products), issue slots 54 % full with the three blocks an SM that registers allow, ALU 51, products 24, and the same time when all pages lie
+// in L2.  64 sequences of 4,096 to 8,192 keys take 108 us (507 MB: 4.7 TB/s; keys beyond the first thousands come at 5.4), 8 of 4,096 take
+// 17, one of 900 takes 5.5.  16 rows of a block take 588 instructions for 16 keys, less than twice as many for four times the
+// rows: 12 portions of 7 tokens over 1,300 to 2,600 keys take 39 us.  (tcgen05 would want codes as bfloat16 in shared memory, which is more traffic there
+// than all the rest.  Tried: keys and values refilled apart, 111 us instead of 108 at the time; four blocks of two buffers an SM, 111; five warps a block, 145;
+// copies of columns for 8 and 16 rows too, 56 instead of 44 for the portions.)
 #pragma once
 
 #include <cooperative_groups.h>
@@ -45,14 +51,18 @@ struct Attend4 {
     const int* table;
     const int* kv_len;
     const int* cu_q;                    // null: one token each
-    int width, n_rows, n_seqs, Hq, Hkv, page_size, page_shift, n_pages, row_blocks, blocks, window;
+    int width, n_rows, n_seqs, Hq, Hkv, page_size, page_shift, n_pages, row_blocks;     // row_blocks: entries of a sequence
+    int blocks;                         // of even shares; below 0: clusters of -blocks
+    int window;
     float scale_log2;
     PoolBounds bounds;
 };
 
 // The work is dealt out in turns of 32 keys.  An entry is a sequence and as many of its rows (tokens times the query heads of a kv head) as a block
-// takes.  The turns of all entries, kv head by kv head, stand in one line, and every block takes a run of the line of the same length; what
-// the lengths are is read here, on the device: a captured call serves any.  Two ways to lay the line out, whichever ends sooner:
+// takes; what the lengths are is read here, on the device: a captured call serves any.  Either an entry and kv head is a cluster's, whose blocks take
+// equal parts (attend_4bit_cluster_kernel); or the turns of all entries, kv head by kv head, stand in one line, and every block takes a run of the
+// line of the same length (attend_4bit_kernel, then join_4bit_kernel).  Which of them: pb_attention_4bit_blocks.  Two ways to lay the line out,
+// whichever ends sooner:
 //   apart    every head begins with a block of its own, and its last block may have less: few heads, as many blocks as there are
 //   packed   a head follows the other, with a gap of kGap4 turns between them that stands for what it costs to begin and end one
 // In either a block has at most one head that another one began and one that another one ends.
