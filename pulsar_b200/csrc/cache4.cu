@@ -11,7 +11,7 @@ namespace {
 using namespace pb;
 
 __device__ __forceinline__ float root_inverse(float v) { return rsqrtf(v); }
-__device__ __forceinline__ double root_inverse(double v) { return 1.0 / sqrt(v); }
+__device__ __forceinline__ double root_inverse(double v) { return rsqrt(v); }
 template <typename A> __device__ __forceinline__ A sum_of_warp(A v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -78,15 +78,23 @@ __device__ __forceinline__ void quantise_quad(const float (&y)[4], int quad, int
     if (4 * quad >= kGroup4 * own) return;              // a lane without channels
     const bool bad = hi > kMost;
     const double m = (double)__bfloat162float(__float2bfloat16_rd(lo));
-    const float step = __bfloat162float(__float2bfloat16_ru(__double2float_ru(((double)hi - m) / 15.0)));
-    const double s = (double)step, inverse = step > 0.0f ? 1.0 / s : 0.0;
+    // A quotient is a product with the reciprocal r and Newton's step for what is left, q + (d - q b) r, which leaves the square of r's error: below what 64
+    // bits hold, so that a quotient that they hold exactly (a tie between two codes) comes out as that.  The reciprocal of a step is that of 32 bits after one
+    // such step of its own; of steps whose reciprocal 32 bits do not hold, a division's.
+    constexpr double kFifteenth = 1.0 / 15.0;
+    const double range = (double)hi - m, rough = range * kFifteenth;
+    const float step = __bfloat162float(__float2bfloat16_ru(__double2float_ru(fma(fma(-rough, 15.0, range), kFifteenth, rough))));
+    const double s = (double)step;
+    double inverse = (double)__frcp_rn(step);
+    inverse = fma(fma(-s, inverse, 1.0), inverse, inverse);
+    if (!(step > 1e-37f && step < 1e37f)) inverse = step > 0.0f ? 1.0 / s : 0.0;
     uint32_t word = 0;
     if (!bad) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const double d = (double)y[e] - m;
             double c = d * inverse;
-            c = fma(fma(-c, s, d), inverse, c);          // the quotient as a division would round it
+            c = fma(fma(-c, s, d), inverse, c);
             word |= (uint32_t)min(15, __double2int_rn(c)) << (4 * e);
         }
     }
@@ -144,8 +152,8 @@ __global__ void qk_norm_rope_write_4bit_kernel(const T* __restrict__ qkv, T* __r
 
 // qk_norm_rope_write_4bit where a head is 8, 16 or 32 lanes of four channels of its first half and the same four of its second, and all of them turn, or
 // none: both ends of a turn are in one lane, as many heads a warp as fit, a group in eight lanes.  What bounds it are instructions (issue slots 71 % full,
-// conversions to and from 64 bits 40 % of their unit): 2,048 bfloat16 tokens of 32 / 8 heads of 128 take 19 us, where their bytes would take 7; one token
-// 2.6.  The kernel above, which takes every other size, takes 41 and 3.3 for them.  (Tried: several tokens a block, 24 where it was 19; twelve blocks an SM
+// conversions to and from 64 bits 40 % of their unit): 2,048 bfloat16 tokens of 32 / 8 heads of 128 take 18.5 us, where their bytes would take 7; one
+// token 2.3.  The kernel above, which takes every other size, takes 41 and 3.3 for them.  (Tried: several tokens a block, 24 where it was 19; twelve blocks an SM
 // instead of ten, 20.)
 template <int L, typename A> __device__ __forceinline__ A sum_of_lanes(A v) {
 #pragma unroll

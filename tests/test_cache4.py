@@ -126,6 +126,20 @@ def test_a_group_with_a_value_that_is_no_number_comes_back_as_nan(dtype, value):
 
 
 @cuda
+def test_halves_between_two_codes_of_every_step():
+    """Steps of 8 bits from 2^-126 to 2^124, with values on every code and halfway between every two: float32 holds them, and so does the quotient."""
+    n = 257
+    r = Rows(n, 1, 2, 64, 4, torch.float32, rotary=0, norm=False, seed=35)
+    g = torch.Generator().manual_seed(36)
+    step = torch.ldexp(torch.randint(128, 256, (n, 5, 2), generator=g).double(), (torch.arange(n) - 140).clamp(-133, 116).view(n, 1, 1))
+    x = (step.unsqueeze(-1) * torch.arange(31).double() / 2).float()                                # 0, s / 2, .. 15 s
+    least = torch.where(torch.rand(n, 5, 2, 1, generator=g) < 0.5, 0.0, (-step.unsqueeze(-1) * 7).float())
+    x = torch.cat([x, x[..., :1]], -1) + least
+    r.qkv = x.flatten(1)
+    r.check()
+
+
+@cuda
 def test_float32_values_beyond_bfloat16_are_infinite():
     r = Rows(1, 1, 1, 32, 4, torch.float32, rotary=0, norm=False, seed=6)
     r.qkv[0, 40] = 3.4e38
