@@ -125,6 +125,26 @@ def test_captured_steps_give_the_same_tokens(folders, name):
 
 
 @cuda
+def test_the_command_line_and_the_python_entry_point(folders, capsys):
+    import json
+
+    from pulsar_b200 import cli
+    from pulsar_b200.api import Pulsar
+    raw, _, page = TINY["D"]
+    prompt = helpers.random_tokens(random.Random(3), 70, raw["vocab_size"])
+    want = engine(folders["D"], page).generate([prompt], 8)[0]
+    args = ["--model", folders["D"], "--prompt_ids", ",".join(map(str, prompt)), "--gen_tokens", "8", "--dtype", "bfloat16", "--page_size", str(page), "--max_pages", "64",
+            "--eos_id", "-1", "--cache_bits", "4", "--json"]
+    assert cli.main(args) == 0
+    assert json.loads(capsys.readouterr().out)["outputs"] == [want]
+    p = Pulsar(folders["D"], dict(page_size=page, num_pages=64, max_sessions=4, max_running=4, eos_id=-1, cache_bits=4))
+    assert {t.dtype for g in p.engine.cache.groups for t in g.pools.values()} == {torch.uint8, torch.bfloat16}
+    s = p.create_session(prompt[:50])
+    s.send(prompt[50:], 8)
+    assert list(s.recv()) == want
+
+
+@cuda
 def test_forked_sequences_go_on_as_their_parent(folders):
     """A fork in the middle of a page: the children's greedy tokens are the parent's, on pages shared and copied in 4 bits."""
     raw, _, page = TINY["D"]
