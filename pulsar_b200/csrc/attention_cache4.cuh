@@ -707,23 +707,25 @@ struct Turns16 {
     }
 };
 
-// Pages of any size: key by key.  `row`: of key `lane` of the next turn.
+// Pages of any size: key by key.  `row`: of key `lane` of the next turn, `hole`: that key's page is none.  The whole warp has to take a turn's edges or none of
+// it, so `holes` is what the warp has voted of the turns that were filled; a lane's own find waits for the fill that needs its row.
 template <typename B>
 struct TurnsAny {
     uint32_t row;
-    bool holes = false;
+    bool hole = false, holes = false;
 
     __device__ __forceinline__ uint32_t load(const Attend4& a, const Head4& head, int turn, int lane) {
         const int key = head.key0 + turn * (kWarps4 * kTile4) + lane;
         int place, page;
+        hole = false;
         if (turn >= head.own || key < head.first || key > head.last) return 0;
         page = page_of(a, head, key, place);
-        if (page < 0) holes = true;
+        hole = page < 0;
         return page < 0 ? 0 : ((uint32_t)page * a.Hkv + head.kvh) * a.page_size + place;
     }
     __device__ __forceinline__ void begin(const Attend4& a, const Head4& head, int lane) { row = load(a, head, 0, lane); }
     __device__ __forceinline__ void fill(const Attend4& a, const Head4& head, int i, uint32_t stage, int lane) {
-        holes = __any_sync(0xffffffffu, holes);
+        holes = __any_sync(0xffffffffu, hole) || holes;
 #pragma unroll
         for (int it = 0; it < B::G_; ++it) {
             const int j = it * 32 + lane, key = j / B::G_, c = j - key * B::G_;
