@@ -144,7 +144,8 @@ __device__ __forceinline__ bool next_item(Work& w, const Args& a, const Seqs& se
     w.pos_last = ctx0 + m0 + w.rows - 1;
     w.lo = (a.window > 0 && w.pos_first - a.window + 1 > 0) ? w.pos_first - a.window + 1 : 0;
     w.kt0 = w.lo / kBN;
-    w.n_tiles = w.pos_last / kBN - w.kt0 + 1;
+    // (rows that all lie before the sequence's first key, as those of a padded portion do: one tile, of which they see nothing)
+    w.n_tiles = max(w.pos_last, 0) / kBN - w.kt0 + 1;
     w.table = a.block_table + (size_t)s * a.table_stride;
     w.t = k + 1;
     return true;
