@@ -424,7 +424,7 @@ struct Attend4Block {
             for (int g = 0; g < G; ++g) {
                 uint32_t word;
                 asm volatile("ld.shared.u32 %0, [%1];" : "=r"(word) : "r"(steps + 4 * g));
-                bad |= (word & 0x7f80u) == 0x7f80u || (word & 0x7f800000u) == 0x7f800000u;
+                bad |= no_number(word);
             }
         }
         if (!any || bad) {

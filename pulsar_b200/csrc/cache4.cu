@@ -66,17 +66,16 @@ __device__ __forceinline__ void norm_and_turn(const T* __restrict__ src, const f
 // value next to the border of two codes falls where the formula has it.
 __device__ __forceinline__ void quantise_quad(const float (&y)[4], int quad, int own, int groups, size_t at, const Pool4& pool) {
     float lo = fminf(fminf(y[0], y[1]), fminf(y[2], y[3])), hi = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
-    constexpr float kMost = 3.38953139e38f;          // the largest bfloat16
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (!(fabsf(y[e]) <= kMost)) hi = __int_as_float(0x7f800000);
+        if (!(fabsf(y[e]) <= kMost4)) hi = __int_as_float(0x7f800000);
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
     if (4 * quad >= kGroup4 * own) return;              // a lane without channels
-    const bool bad = hi > kMost;
+    const bool bad = hi > kMost4;
     const double m = (double)__bfloat162float(__float2bfloat16_rd(lo));
     // A quotient is a product with the reciprocal r and Newton's step for what is left, q + (d - q b) r, which leaves the square of r's error: below what 64
     // bits hold, so that a quotient that they hold exactly (a tie between two codes) comes out as that.  The reciprocal of a step is that of 32 bits after one
@@ -293,7 +292,10 @@ __global__ void __launch_bounds__(256) expand_pages_4bit_kernel(Pool4 k_pool, Po
     if (rows > 0 && page >= 0) page_ok(page, bounds);
     bool there = page_or_none(page, n_pages) >= 0;
     if (cu_q != nullptr) {
-        // For attention: what no tile of 128 keys that a query sees touches is left out, and what else is none becomes zeros.
+        // For attention: what no tile of 128 keys that a query sees touches is left out, and what else is none becomes zeros.  The dense kernels want
+        // every value finite, seen or not, for a weight of zero times a NaN is one, in every row of the tile and of the tiles that find it in their
+        // buffers later; scores of keys that a row does not see they take away whatever those are.  So the key of a value that is no number
+        // becomes NaN and the value finite: who sees it gets NaN, and nobody else.
         const int low = window > 0 ? length - (cu_q[seq + 1] - cu_q[seq]) - window + 1 - 128 : 0;
         if (!there) rows = min(rows, 0);
         there = logical * page_size < length && (logical + 1) * page_size > low;
@@ -318,6 +320,14 @@ __global__ void __launch_bounds__(256) expand_pages_4bit_kernel(Pool4 k_pool, Po
         uint32_t w[G], two[G];
         load_words<G>(reinterpret_cast<const uint32_t*>(pool.codes) + (in_pool * 4 + t) * G, w);
         load_words<G>(reinterpret_cast<const uint32_t*>(pool.steps) + in_pool * G, two);
+        if (cu_q != nullptr && !is_v) {
+            uint32_t of_value[G];
+            load_words<G>(reinterpret_cast<const uint32_t*>(v_pool.steps) + in_pool * G, of_value);
+            bool lost = false;
+#pragma unroll
+            for (int g = 0; g < G; ++g) lost |= no_number(of_value[g]);
+            if (lost) two[0] = 0x7fc07fc0u;
+        }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             const float step = __uint_as_float(two[g] << 16), least = __uint_as_float(two[g] & 0xffff0000u);
@@ -326,6 +336,10 @@ __global__ void __launch_bounds__(256) expand_pages_4bit_kernel(Pool4 k_pool, Po
             float y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = fmaf(step, __uint_as_float(((word >> (4 * e)) & 15) | 0x4b000000u) - 8388608.0f, least);
+            if (cu_q != nullptr && is_v && !(fmaf(15.0f, fabsf(step), fabsf(least)) <= kMost4)) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = fminf(fmaxf(y[e], -kMost4), kMost4);
+            }
             store_octet(dst + 32 * g, y);
         }
     }

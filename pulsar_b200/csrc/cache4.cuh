@@ -21,6 +21,7 @@
 namespace pb {
 
 constexpr int kGroup4 = 32;
+constexpr float kMost4 = 3.38953139e38f;          // the largest bfloat16
 
 struct Pool4 {
     uint8_t* codes;             // [pages, heads, page, D / 2]
@@ -29,6 +30,9 @@ struct Pool4 {
 
 // A page of a block table as the kernels of this cache take it: -1 where it is not a page of the pool (nothing is read or written there).
 __device__ __forceinline__ int page_or_none(int page, int n_pages) { return (unsigned)page < (unsigned)n_pages ? page : -1; }
+
+// Whether a word of a step and a least value holds a NaN or an infinity.
+__device__ __forceinline__ bool no_number(uint32_t word) { return (word & 0x7f80u) == 0x7f80u || (word & 0x7f800000u) == 0x7f800000u; }
 
 // The arguments of the entry points of this cache come as one row of 64-bit words (a pointer, a whole number or a double each), which the host fills in
 // a sixth of the time that as many arguments of a call take it.

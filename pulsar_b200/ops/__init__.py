@@ -2384,8 +2384,8 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
 
     bfloat16 portions of many tokens, where the dense attention of prompt portions has a kernel for their sizes, are attended to over expanded
     pages (``expanded_4bit``), which takes room for S * width pages, of as many sequences at a time as 1 GiB holds.  (There keys and values are operands rounded to bfloat16, as a cache
-    of bfloat16 holds them: over 6,000 keys outputs are 3.7e-3 off, 2.3e-3 on codes and 1.7e-3 by their own rounding alone; and a value that is NaN also reaches
-    the tokens of its sequence's portion that do not see it.)  ``scratch(tag, shape, dtype)`` gives tensors to work in; without it they are made here."""
+    of bfloat16 holds them: over 6,000 keys outputs are 3.7e-3 off, 2.3e-3 on codes and 1.7e-3 by their own rounding alone.)  A key or a value that is NaN makes NaN of what the queries
+    that see it get from its kv head, a value's of its group's channels at least; no other query's changes.  ``scratch(tag, shape, dtype)`` gives tensors to work in; without it they are made here."""
     name = "paged_attention_4bit"
     tensors = (q, k_pool, k_steps, v_pool, v_steps, out, block_table, kv_len)
     if (where := _on_one_device(name, (*tensors, cu_q))) != _current_device():
