@@ -277,29 +277,43 @@ template <int N> __device__ __forceinline__ void load_words(const uint32_t* __re
     }
 }
 
+// A lane's 8 G codes of a row, channels 8 t .. + 7 of every group, as values that lie at most `most` from zero.
+template <bool BOUNDED, typename T, int G>
+__device__ __forceinline__ void store_values(const uint32_t (&w)[G], const uint32_t (&two)[G], T* dst, float most) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        const float step = __uint_as_float(two[g] << 16), least = __uint_as_float(two[g] & 0xffff0000u);
+        // 16-bit words g and G + g of the lane's 2 G
+        const uint32_t sel = ((g & 1) ? 0x0032u : 0x0010u) | (((G + g) & 1) ? 0x7600u : 0x5400u), word = __byte_perm(w[g >> 1], w[(G + g) >> 1], sel);
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            y[e] = fmaf(step, __uint_as_float(((word >> (4 * e)) & 15) | 0x4b000000u) - 8388608.0f, least);
+            if (BOUNDED) y[e] = fminf(fmaxf(y[e], -most), most);
+        }
+        store_octet(dst + 32 * g, y);
+    }
+}
+template <typename T, int G> __device__ __forceinline__ void store_zeros(T* dst) {
+    const float zero[8] = {};
+#pragma unroll
+    for (int g = 0; g < G; ++g) store_octet(dst + 32 * g, zero);
+}
+
 // A lane takes the codes of channels 8 t .. + 7 of all groups of a row, side by side in the pool, and writes eight values of every group.  Bytes bound it: 5
 // sequences of 15,000 to 30,000 bfloat16 keys, 8 heads of 128, take 95 us at 6.1 TB/s, three quarters of them written.
 template <typename T, int G>
 __global__ void __launch_bounds__(256) expand_pages_4bit_kernel(Pool4 k_pool, Pool4 v_pool, const int* __restrict__ table, const int* __restrict__ kv_len,
                                                                 T* __restrict__ k_out, T* __restrict__ v_out, int* __restrict__ table_out, int width, int Hkv,
-                                                                int page_size, int n_pages, const int* __restrict__ cu_q, int window, const PoolBounds bounds) {
+                                                                int page_size, int n_pages, const PoolBounds bounds) {
     pdl_wait();
     constexpr int D = kGroup4 * G;
     const int seq = blockIdx.y, logical = blockIdx.x, length = kv_len[seq];
     const size_t out_page = (size_t)seq * width + logical;
-    int rows = min(page_size, length - logical * page_size);                    // of this page, that hold a key
-    int page = rows > 0 ? table[(size_t)seq * width + logical] : -1;
+    const int rows = min(page_size, length - logical * page_size);              // of this page, that hold a key
+    const int page = rows > 0 ? table[(size_t)seq * width + logical] : -1;
     if (rows > 0 && page >= 0) page_ok(page, bounds);
-    bool there = page_or_none(page, n_pages) >= 0;
-    if (cu_q != nullptr) {
-        // For attention: what no tile of 128 keys that a query sees touches is left out, and what else is none becomes zeros.  The dense kernels want
-        // every value finite, seen or not, for a weight of zero times a NaN is one, in every row of the tile and of the tiles that find it in their
-        // buffers later; scores of keys that a row does not see they take away whatever those are.  So the key of a value that is no number
-        // becomes NaN and the value finite: who sees it gets NaN, and nobody else.
-        const int low = window > 0 ? length - (cu_q[seq + 1] - cu_q[seq]) - window + 1 - 128 : 0;
-        if (!there) rows = min(rows, 0);
-        there = logical * page_size < length && (logical + 1) * page_size > low;
-    }
+    const bool there = page_or_none(page, n_pages) >= 0;
     if (blockIdx.z == 0 && threadIdx.x == 0) table_out[out_page] = there ? (int)out_page : -1;
     if (!there) return;
     const int per_pool = Hkv * page_size, n = 2 * per_pool * 4;
@@ -311,37 +325,66 @@ __global__ void __launch_bounds__(256) expand_pages_4bit_kernel(Pool4 k_pool, Po
         const Pool4 pool = {is_v ? v_pool.codes : k_pool.codes, is_v ? v_pool.steps : k_pool.steps};
         T* dst = (is_v ? v_out : k_out) + (out_page * per_pool + row) * D + 8 * t;
         if (partly && row % page_size >= rows) {
-            const float zero[8] = {};
-#pragma unroll
-            for (int g = 0; g < G; ++g) store_octet(dst + 32 * g, zero);
+            store_zeros<T, G>(dst);
             continue;
         }
         const size_t in_pool = (size_t)page * per_pool + row;
         uint32_t w[G], two[G];
         load_words<G>(reinterpret_cast<const uint32_t*>(pool.codes) + (in_pool * 4 + t) * G, w);
         load_words<G>(reinterpret_cast<const uint32_t*>(pool.steps) + in_pool * G, two);
-        if (cu_q != nullptr && !is_v) {
-            uint32_t of_value[G];
-            load_words<G>(reinterpret_cast<const uint32_t*>(v_pool.steps) + in_pool * G, of_value);
-            bool lost = false;
-#pragma unroll
-            for (int g = 0; g < G; ++g) lost |= no_number(of_value[g]);
-            if (lost) two[0] = 0x7fc07fc0u;
+        store_values<false, T, G>(w, two, dst, 0.0f);
+    }
+}
+
+// The same for the dense attention kernels: a page that no tile of 128 keys touches which a query sees is left out, and what else is none becomes zeros.
+// Those kernels want every value finite, seen or not, for a weight of zero times a NaN is one, in every row of the tile and of the tiles that find it
+// in their buffers later; scores of keys that a row does not see they take away whatever those are.  So the key of a value that is no number becomes NaN
+// and the value finite: who sees it gets NaN, and nobody else.  A lane takes a key and its value.
+template <int G>
+__global__ void __launch_bounds__(256) expand_for_attention_4bit_kernel(Pool4 k_pool, Pool4 v_pool, const int* __restrict__ table, const int* __restrict__ kv_len,
+                                                                        __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out,
+                                                                        int* __restrict__ table_out, int width, int Hkv, int page_size, int n_pages,
+                                                                        const int* __restrict__ cu_q, int window, const PoolBounds bounds) {
+    pdl_wait();
+    constexpr int D = kGroup4 * G;
+    const int seq = blockIdx.y, logical = blockIdx.x, length = kv_len[seq];
+    const size_t out_page = (size_t)seq * width + logical;
+    const int low = window > 0 ? length - (cu_q[seq + 1] - cu_q[seq]) - window + 1 - 128 : 0;
+    const bool there = logical * page_size < length && (logical + 1) * page_size > low;
+    if (blockIdx.z == 0 && threadIdx.x == 0) table_out[out_page] = there ? (int)out_page : -1;
+    if (!there) return;
+    const int page = table[out_page];
+    if (page >= 0) page_ok(page, bounds);
+    const int rows = page_or_none(page, n_pages) >= 0 ? min(page_size, length - logical * page_size) : 0;      // of this page, that hold a key
+    const int per_pool = Hkv * page_size, n = per_pool * 4;
+    const bool partly = rows < page_size;
+    for (int i = blockIdx.z * blockDim.x + threadIdx.x; i < n; i += gridDim.z * blockDim.x) {
+        const int t = i & 3, row = i >> 2;                                      // head * page_size + place
+        const size_t to = (out_page * per_pool + row) * D + 8 * t;
+        if (partly && row % page_size >= rows) {
+            store_zeros<__nv_bfloat16, G>(k_out + to);
+            store_zeros<__nv_bfloat16, G>(v_out + to);
+            continue;
         }
+        const size_t in_pool = (size_t)page * per_pool + row;
+        uint32_t k[G], v[G], k_two[G], v_two[G];
+        load_words<G>(reinterpret_cast<const uint32_t*>(k_pool.codes) + (in_pool * 4 + t) * G, k);
+        load_words<G>(reinterpret_cast<const uint32_t*>(k_pool.steps) + in_pool * G, k_two);
+        load_words<G>(reinterpret_cast<const uint32_t*>(v_pool.codes) + (in_pool * 4 + t) * G, v);
+        load_words<G>(reinterpret_cast<const uint32_t*>(v_pool.steps) + in_pool * G, v_two);
+        bool bounded = false;                   // a value passes the end of bfloat16's range, or is none
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const float step = __uint_as_float(two[g] << 16), least = __uint_as_float(two[g] & 0xffff0000u);
-            // 16-bit words g and G + g of the lane's 2 G
-            const uint32_t sel = ((g & 1) ? 0x0032u : 0x0010u) | (((G + g) & 1) ? 0x7600u : 0x5400u), word = __byte_perm(w[g >> 1], w[(G + g) >> 1], sel);
-            float y[8];
+        for (int g = 0; g < G; ++g)
+            bounded |= !(fmaf(15.0f, fabsf(__uint_as_float(v_two[g] << 16)), fabsf(__uint_as_float(v_two[g] & 0xffff0000u))) <= kMost4);
+        if (bounded) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = fmaf(step, __uint_as_float(((word >> (4 * e)) & 15) | 0x4b000000u) - 8388608.0f, least);
-            if (cu_q != nullptr && is_v && !(fmaf(15.0f, fabsf(step), fabsf(least)) <= kMost4)) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = fminf(fmaxf(y[e], -kMost4), kMost4);
-            }
-            store_octet(dst + 32 * g, y);
+            for (int g = 0; g < G; ++g)
+                if (no_number(v_two[g])) k_two[0] = 0x7fc07fc0u;
+            store_values<true, __nv_bfloat16, G>(v, v_two, v_out + to, kMost4);
+        } else {
+            store_values<false, __nv_bfloat16, G>(v, v_two, v_out + to, 0.0f);
         }
+        store_values<false, __nv_bfloat16, G>(k, k_two, k_out + to, 0.0f);
     }
 }
 
@@ -363,18 +406,28 @@ int launch_write(const void* qkv, void* q_out, const Pool4& k, const Pool4& v, c
                       n_pages, pool_bounds_now());
 }
 
-template <typename T, int G>
-int launch_expand_of(const Pool4& k, const Pool4& v, const int* table, const int* kv_len, void* k_out, void* v_out, int* table_out, int n_seqs, int width, int Hkv,
-                     int page_size, int n_pages, const int* cu_q, int window, cudaStream_t stream) {
-    const int units = 2 * Hkv * page_size * 4, blocks = (units + 511) / 512;
-    return launch_pdl(expand_pages_4bit_kernel<T, G>, dim3(width, n_seqs, blocks < 64 ? blocks : 64), dim3(256), 0, stream, k, v, table, kv_len, (T*)k_out, (T*)v_out,
-                      table_out, width, Hkv, page_size, n_pages, cu_q, window, pool_bounds_now());
+// Arguments of an expansion; cu_q (and window): for attention.
+struct Expand4 {
+    Pool4 k, v;
+    const int *table, *kv_len, *cu_q;
+    void *k_out, *v_out;
+    int* table_out;
+    int n_seqs, width, Hkv, page_size, n_pages, window;
+};
+template <typename T, int G> int launch_expand_of(const Expand4& x, cudaStream_t stream) {
+    const int units = 2 * x.Hkv * x.page_size * 4, blocks = (units + 511) / 512;         // two units a thread
+    const dim3 grid(x.width, x.n_seqs, blocks < 64 ? blocks : 64);
+    if (x.cu_q == nullptr)
+        return launch_pdl(expand_pages_4bit_kernel<T, G>, grid, dim3(256), 0, stream, x.k, x.v, x.table, x.kv_len, (T*)x.k_out, (T*)x.v_out, x.table_out, x.width, x.Hkv,
+                          x.page_size, x.n_pages, pool_bounds_now());
+    if constexpr (sizeof(T) == 2 && (G == 2 || G == 4))                                  // what the dense kernels take
+        return launch_pdl(expand_for_attention_4bit_kernel<G>, grid, dim3(256), 0, stream, x.k, x.v, x.table, x.kv_len, (T*)x.k_out, (T*)x.v_out, x.table_out, x.width, x.Hkv,
+                          x.page_size, x.n_pages, x.cu_q, x.window, pool_bounds_now());
+    return PB_ERR_BAD_SIZE;
 }
-template <typename T>
-int launch_expand(int groups, const Pool4& k, const Pool4& v, const int* table, const int* kv_len, void* k_out, void* v_out, int* table_out, int n_seqs, int width, int Hkv,
-                  int page_size, int n_pages, const int* cu_q, int window, cudaStream_t stream) {
+template <typename T> int launch_expand(int groups, const Expand4& x, cudaStream_t stream) {
     switch (groups) {
-#define PB_EXPAND(g) case g: return launch_expand_of<T, g>(k, v, table, kv_len, k_out, v_out, table_out, n_seqs, width, Hkv, page_size, n_pages, cu_q, window, stream);
+#define PB_EXPAND(g) case g: return launch_expand_of<T, g>(x, stream);
         PB_EXPAND(1) PB_EXPAND(2) PB_EXPAND(3) PB_EXPAND(4) PB_EXPAND(5) PB_EXPAND(6) PB_EXPAND(7) PB_EXPAND(8)
 #undef PB_EXPAND
     }
@@ -416,23 +469,29 @@ PB_EXPORT int pb_qk_norm_rope_write_4bit(const long long* words, cudaStream_t st
 PB_EXPORT int pb_expand_pages_4bit(const long long* words, cudaStream_t stream) {
     Words4 w{words};
     const int dtype = w.num();
-    Pool4 k, v;
-    k.codes = w.ptr<uint8_t>();
-    k.steps = w.ptr<__nv_bfloat16>();
-    v.codes = w.ptr<uint8_t>();
-    v.steps = w.ptr<__nv_bfloat16>();
-    const int *table = w.ptr<const int>(), *kv_len = w.ptr<const int>();
-    void *k_out = w.ptr<void>(), *v_out = w.ptr<void>();
-    int* table_out = w.ptr<int>();
-    const int n_seqs = w.num(), width = w.num(), Hkv = w.num(), D = w.num(), page_size = w.num(), n_pages = w.num();
-    const int* cu_q = w.ptr<const int>();
-    const int window = w.num();
-    if (!sizes_4bit(Hkv, D, page_size, n_pages) || n_seqs < 0 || width < 0 || window < 0) return PB_ERR_BAD_SIZE;
-    if (n_seqs > 65535 || (long long)n_seqs * width > 0x7fffffffLL || (long long)width * page_size > 0x7fffffffLL || 8LL * Hkv * page_size > 0x3fffffffLL) return PB_ERR_TOO_LARGE;
-    if (n_seqs == 0 || width == 0) return 0;
-    if (dtype == PB_F32)
-        return launch_expand<float>(D / kGroup4, k, v, table, kv_len, k_out, v_out, table_out, n_seqs, width, Hkv, page_size, n_pages, cu_q, window, stream);
-    if (dtype == PB_BF16)
-        return launch_expand<__nv_bfloat16>(D / kGroup4, k, v, table, kv_len, k_out, v_out, table_out, n_seqs, width, Hkv, page_size, n_pages, cu_q, window, stream);
+    Expand4 x;
+    x.k.codes = w.ptr<uint8_t>();
+    x.k.steps = w.ptr<__nv_bfloat16>();
+    x.v.codes = w.ptr<uint8_t>();
+    x.v.steps = w.ptr<__nv_bfloat16>();
+    x.table = w.ptr<const int>();
+    x.kv_len = w.ptr<const int>();
+    x.k_out = w.ptr<void>();
+    x.v_out = w.ptr<void>();
+    x.table_out = w.ptr<int>();
+    x.n_seqs = w.num();
+    x.width = w.num();
+    x.Hkv = w.num();
+    const int D = w.num();
+    x.page_size = w.num();
+    x.n_pages = w.num();
+    x.cu_q = w.ptr<const int>();
+    x.window = w.num();
+    if (!sizes_4bit(x.Hkv, D, x.page_size, x.n_pages) || x.n_seqs < 0 || x.width < 0 || x.window < 0) return PB_ERR_BAD_SIZE;
+    if (x.n_seqs > 65535 || (long long)x.n_seqs * x.width > 0x7fffffffLL || (long long)x.width * x.page_size > 0x7fffffffLL || 8LL * x.Hkv * x.page_size > 0x3fffffffLL)
+        return PB_ERR_TOO_LARGE;
+    if (x.n_seqs == 0 || x.width == 0) return 0;
+    if (dtype == PB_F32) return launch_expand<float>(D / kGroup4, x, stream);
+    if (dtype == PB_BF16) return launch_expand<__nv_bfloat16>(D / kGroup4, x, stream);
     return PB_ERR_BAD_DTYPE;
 }
