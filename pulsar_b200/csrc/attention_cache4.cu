@@ -62,36 +62,79 @@ PB_EXPORT int pb_attention_4bit_blocks(int dtype, int most_tokens, int n_seqs, i
     return wanted < most ? (int)wanted : most;
 }
 
+namespace {
 // Words: dtype, q, k codes, k steps, v codes, v steps, out, sums, plan, table, kv_len, cu_q (or 0), width, n_rows, most_tokens, n_seqs, Hq, Hkv, D, page_size,
 // n_pages, scale, window, blocks (of attention_4bit_blocks; sums and plan only where it is above 0).
+struct Call4 {
+    Attend4 a;
+    int dtype, D, most_tokens;
+    // 0, or the error; `rows` of a block: 0 for attention_4bit_rows
+    int read(const long long* words, int& rows) {
+        Words4 w{words};
+        dtype = w.num();
+        a.q = w.ptr<const void>();
+        a.k.codes = w.ptr<uint8_t>();
+        a.k.steps = w.ptr<__nv_bfloat16>();
+        a.v.codes = w.ptr<uint8_t>();
+        a.v.steps = w.ptr<__nv_bfloat16>();
+        a.out = w.ptr<void>();
+        a.sums = w.ptr<float>();
+        a.plan = w.ptr<int>();
+        a.table = w.ptr<const int>();
+        a.kv_len = w.ptr<const int>();
+        a.cu_q = w.ptr<const int>();
+        a.width = w.num();
+        a.n_rows = w.num();
+        most_tokens = w.num();
+        a.n_seqs = w.num();
+        a.Hq = w.num();
+        a.Hkv = w.num();
+        D = w.num();
+        a.page_size = w.num();
+        a.n_pages = w.num();
+        a.scale_log2 = (float)w.real() * kLog2e;
+        a.window = w.num();
+        a.blocks = w.num();
+        if (a.Hkv <= 0 || a.Hq <= 0 || a.Hq % a.Hkv || D <= 0 || D > 256 || D % kGroup4 || a.page_size <= 0 || a.n_pages <= 0 || a.width <= 0 || a.window < 0 || most_tokens < 0 ||
+            a.n_seqs < 0 || a.n_rows < 0)
+            return PB_ERR_BAD_SIZE;
+        if (dtype != PB_F32 && dtype != PB_BF16) return PB_ERR_BAD_DTYPE;
+        const int group = a.Hq / a.Hkv;
+        if (rows == 0) rows = pb_attention_4bit_rows(dtype, most_tokens * group, D);
+        const long long row_blocks = ((long long)most_tokens * group + rows - 1) / rows, keys = (long long)a.width * a.page_size;
+        if (a.n_seqs > 65535 || (long long)most_tokens * a.Hq > 0x3fffffff || (long long)a.n_pages * a.Hkv * a.page_size >= 0xffffffffLL || keys > 0x7ffffff0LL ||
+            (double)a.n_seqs * row_blocks * a.Hkv * (keys / kTile4 + 1 + kGap4) > 1.0e9)
+            return PB_ERR_TOO_LARGE;
+        a.page_shift = log2_exact(a.page_size);
+        a.row_blocks = (int)row_blocks;
+        a.bounds = pool_bounds_now();
+        return 0;
+    }
+};
+}  // namespace
+
 PB_EXPORT int pb_paged_attention_4bit(const long long* words, cudaStream_t stream) {
-    Words4 w{words};
-    const int dtype = w.num();
-    const void* q = w.ptr<const void>();
-    Pool4 k, v;
-    k.codes = w.ptr<uint8_t>();
-    k.steps = w.ptr<__nv_bfloat16>();
-    v.codes = w.ptr<uint8_t>();
-    v.steps = w.ptr<__nv_bfloat16>();
-    void* out = w.ptr<void>();
-    float* sums = w.ptr<float>();
-    int* plan = w.ptr<int>();
-    const int *table = w.ptr<const int>(), *kv_len = w.ptr<const int>(), *cu_q = w.ptr<const int>();
-    const int width = w.num(), n_rows = w.num(), most_tokens = w.num(), n_seqs = w.num(), Hq = w.num(), Hkv = w.num(), D = w.num(), page_size = w.num(), n_pages = w.num();
-    const float scale = (float)w.real();
-    const int window = w.num(), blocks = w.num();
-    if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || D <= 0 || D > 256 || D % kGroup4 || page_size <= 0 || n_pages <= 0 || width <= 0 || window < 0 || blocks == 0 || blocks < -8 ||
-        (blocks > 0 && (sums == nullptr || plan == nullptr)) || most_tokens < 0 || n_seqs < 0 || n_rows < 0)
-        return PB_ERR_BAD_SIZE;
-    if (dtype != PB_F32 && dtype != PB_BF16) return PB_ERR_BAD_DTYPE;
-    if (most_tokens == 0 || n_seqs == 0) return 0;
-    const int group = Hq / Hkv, rows = pb_attention_4bit_rows(dtype, most_tokens * group, D);
-    const long long row_blocks = ((long long)most_tokens * group + rows - 1) / rows, keys = (long long)width * page_size;
-    if (n_seqs > 65535 || (long long)most_tokens * Hq > 0x3fffffff || (long long)n_pages * Hkv * page_size >= 0xffffffffLL || keys > 0x7ffffff0LL ||
-        (double)n_seqs * row_blocks * Hkv * (keys / kTile4 + 1 + kGap4) > 1.0e9)
-        return PB_ERR_TOO_LARGE;
-    if (blocks < 0 && row_blocks * Hkv > 65535) return PB_ERR_TOO_LARGE;
-    Attend4 a{q, out, k, v, sums, plan, table, kv_len, cu_q, width, n_rows, n_seqs,
-              Hq, Hkv, page_size, log2_exact(page_size), n_pages, (int)row_blocks, blocks, window, scale * kLog2e, pool_bounds_now()};
-    return (dtype == PB_F32 ? attend_4bit_f32 : attend_4bit_bf16)(a, D / kGroup4, rows, most_tokens, stream);
+    Call4 c;
+    int rows = 0;
+    if (const int rc = c.read(words, rows)) return rc;
+    const Attend4& a = c.a;
+    if (a.blocks == 0 || a.blocks < -8 || (a.blocks > 0 && (a.sums == nullptr || a.plan == nullptr))) return PB_ERR_BAD_SIZE;
+    if (c.most_tokens == 0 || a.n_seqs == 0) return 0;
+    if (a.blocks < 0 && (long long)a.row_blocks * a.Hkv > 65535) return PB_ERR_TOO_LARGE;
+    return (c.dtype == PB_F32 ? attend_4bit_f32 : attend_4bit_bf16)(a, c.D / kGroup4, rows, c.most_tokens, stream);
+}
+
+// Portions that a dense kernel has attended to over expanded pages: those that see keys of pages that are none.  Words as above, without sums, plan and
+// blocks; bfloat16, heads of 64 or 128 (of which the dense kernels are).
+PB_EXPORT int pb_paged_attention_4bit_holes(const long long* words, cudaStream_t stream) {
+    Call4 c;
+    int rows = 16;
+    if (const int rc = c.read(words, rows)) return rc;
+    if (c.dtype != PB_BF16 || c.a.cu_q == nullptr) return PB_ERR_BAD_DTYPE;
+    if (c.most_tokens == 0 || c.a.n_seqs == 0) return 0;
+    const bool by_16 = c.a.page_size % 16 == 0;
+    const int sms = sm_count_4bit();
+    if (c.D == 64) return by_16 ? launch_attend_4bit_holes<__nv_bfloat16, 2, 2, Turns16>(c.a, sms, stream) : launch_attend_4bit_holes<__nv_bfloat16, 2, 2, TurnsAny>(c.a, sms, stream);
+    if (c.D == 128) return by_16 ? launch_attend_4bit_holes<__nv_bfloat16, 4, 2, Turns16>(c.a, sms, stream) : launch_attend_4bit_holes<__nv_bfloat16, 4, 2, TurnsAny>(c.a, sms, stream);
+    return PB_ERR_BAD_SIZE;
 }

@@ -1110,6 +1110,52 @@ __global__ void __launch_bounds__(128) join_4bit_kernel(const Attend4 a, int D, 
     }
 }
 
+// Behind a dense kernel over expanded pages, where pages that are none stand as keys of zeros: the rows of sequences that see such, once more on codes.
+// A row of blocks a sequence; all others' have nothing to do but to look at the table, which they do while the dense kernel runs: that one was launched
+// behind everything that writes tables and lengths.  (us without such pages, without this launch and with it: 512 tokens over 6,000 keys 63.0, 64.2; 2,048 tokens
+// 150.9, 151.7.  All behind pdl_wait 62.6, 65.5.)
+template <typename T, int G, int NT, typename Turns, int BLOCKS>
+__global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_holes_kernel(const Attend4 a) {
+    using B = Attend4Block<T, G, NT, 1>;
+    constexpr int D = B::D;
+    extern __shared__ __align__(128) uint8_t shared[];
+    const int seq = blockIdx.y, n_tokens = a.cu_q[seq + 1] - a.cu_q[seq], kv_len = a.kv_len[seq];
+    const int low = kv_len - n_tokens - a.window + 1, first = a.window > 0 && low > 0 ? low : 0, last = min(kv_len, a.width * a.page_size) - 1;
+    bool hole = false;
+    if (n_tokens > 0 && last >= first)
+        for (int page = first / a.page_size + threadIdx.x; page <= last / a.page_size; page += kWarps4 * 32)
+            hole |= page_or_none(a.table[(size_t)seq * a.width + page], a.n_pages) < 0;
+    hole = __syncthreads_or(hole);
+    pdl_trigger();
+    pdl_wait();                         // the dense kernel has written its rows
+    if (!hole) return;
+    for (int item = blockIdx.x; item < a.Hkv * a.row_blocks; item += gridDim.x) {
+        const int kvh = item / a.row_blocks;
+        const Entry4 entry(a, seq * a.row_blocks + item - kvh * a.row_blocks, B::kRows);
+        if (entry.row0 >= n_tokens * (a.Hq / a.Hkv)) continue;
+        attend_part<T, B, Turns>(a, entry, kvh, 0, entry.turns, shared);
+        for (int i = threadIdx.x; i < B::kRows * (D / 4); i += kWarps4 * 32) {
+            const int column = i / (D / 4), quad = i - column * (D / 4);
+            const long at = entry.row_at(a, kvh, column);
+            if (at < 0) continue;
+            float top, total, v[4];
+            block_sum<B>(shared, column, quad, top, total, v);
+            store_weighed(reinterpret_cast<T*>(a.out) + at * D + 4 * quad, total, v);
+        }
+        __syncthreads();
+    }
+}
+template <typename T, int G, int NT, template <typename> class Turns>
+int launch_attend_4bit_holes(const Attend4& a, int sms, cudaStream_t stream) {
+    using B = Attend4Block<T, G, NT, 1>;
+    constexpr int kBlocks = blocks_4bit(sizeof(T) == 4, G, B::kRows);
+    auto kernel = attend_4bit_holes_kernel<T, G, NT, Turns<B>, kBlocks>;
+    static SmemLimit limit;
+    if (const int rc = limit.allow(kernel, B::kShared)) return rc;
+    const long long items = (long long)a.Hkv * a.row_blocks, each = sms / a.n_seqs;           // a block an SM
+    return launch_pdl(kernel, dim3((unsigned)(items < each ? items : each > 0 ? each : 1), a.n_seqs), dim3(kWarps4 * 32), B::kShared, stream, a);
+}
+
 template <typename T, int G, int NT, int COPIES, template <typename> class Turns>
 int launch_attend_4bit(const Attend4& a, int most_tokens, cudaStream_t stream) {
     using B = Attend4Block<T, G, NT, COPIES>;

@@ -158,6 +158,7 @@ _SIGNATURES = {
     "pb_qk_norm_rope_write_4bit": [ctypes.c_char_p, _P],
     "pb_expand_pages_4bit": [ctypes.c_char_p, _P],
     "pb_paged_attention_4bit": [ctypes.c_char_p, _P],
+    "pb_paged_attention_4bit_holes": [ctypes.c_char_p, _P],
     "pb_attention_4bit_blocks": [_I] * 9,
     "pb_attention_4bit_rows": [_I, _I, _I],
     "pb_token_scores": [_I, _P, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P],
@@ -174,7 +175,7 @@ _LAUNCHERS = {"embed", "scale_cap", "move_ids", "add_rmsnorm", "rope_table", "qk
               "selective_scan", "selective_scan_prompt", "selective_scan_chunked", "post_norm_add", "clamped_glu",
               "post_norm_add_bias", "glu_bias", "qk_prepare", "qk_prepare_whole", "sigmoid_gate_strided", "add_bias", "moe_route", "moe_gate_up", "moe_up", "moe_down", "moe_grouped",
               "norm_shift", "parallel_add", "activation", "min_gru", "diff_combine", "retention", "scaled_sum", "concat_streams", "normed_sum", "matrix_memory", "state_space",
-              "copy_pages", "token_scores", "paged_attention_shared", "head_scores", "qk_norm_rope_write_4bit", "expand_pages_4bit", "paged_attention_4bit"}
+              "copy_pages", "token_scores", "paged_attention_shared", "head_scores", "qk_norm_rope_write_4bit", "expand_pages_4bit", "paged_attention_4bit", "paged_attention_4bit_holes"}
 
 
 class KernelError(RuntimeError):
@@ -2378,8 +2379,8 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
     """Attention over a cache of 4 bits: q, out [N, Hq, D] (float32 or bfloat16), ``block_table`` int32 [S, width], ``kv_len`` int32 [S] with
     the keys of this step in it.  Without ``cu_q`` every sequence has one query token, the last (N = S); else sequence i has the tokens
     ``cu_q[i]:cu_q[i + 1]`` (int32 [S + 1], rising, rows of q), the last of its ``kv_len[i]``, and ``q_lens`` are their numbers as the host knows
-    them.  A query sees the keys up to its own, with ``window`` w the last w of them; those have to lie in pages of the pool (an id that is
-    none is not read).  (``kv_len[i]`` is no more than the table's width holds.)  A query that sees no key gets zeros.  Rows of ``out`` that are no sequence's stay as
+    them.  A query sees the keys up to its own, with ``window`` w the last w of them, but none whose page is not one of the pool (-1, say).
+    (``kv_len[i]`` is no more than the table's width holds.)  A query that sees no key gets zeros.  Rows of ``out`` that are no sequence's stay as
     they were.
 
     bfloat16 portions of many tokens, where the dense attention of prompt portions has a kernel for their sizes, are attended to over expanded
@@ -2454,6 +2455,11 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
                 n_tiles = tiles(lens)
                 one = (1,) if dense == "tcgen05" and _one_head_a_block(d, n_tiles * hq) else ()
                 run(q, k_out, v_out, out, table_out[:end - first], cu, kv, n_tiles, scale, window, *one)
+            # a page that is none is a key of zeros to the dense kernels: sequences that have one where a query sees it are taken once more, on codes
+            _check_against(k_pool)
+            words = _ATTEND_4BIT.pack(kind, q_at, *pools, out_at, 0, 0, block_table.data_ptr(), kv_len.data_ptr(), cu_q.data_ptr(), width, n, most_tokens, s, hq, hkv, d, page_size,
+                                      n_pages, scale, window, 0)
+            check(fn("pb_paged_attention_4bit_holes")(words, stream()), name)
             return
     blocks, sums, plan = scratch_4bit(s, most_tokens, hq, hkv, d, width, page_size, window, dtype)
     work_at = 0

@@ -60,3 +60,63 @@ def test_a_sequence_of_holes_alone_gives_zeros(page):
     assert (got[0] == 0).all() and torch.equal(got[1], c.run()[1])
     short = c.run(block_table=table.cuda(), kv_len=on([0, 300]))
     assert torch.equal(short, got)
+
+
+def both_ways(monkeypatch, case, holes):
+    """The way on codes and the one over expanded pages, with one and two heads a block where it has both: what sequences without holes get does not change."""
+    for expanded, one in ((False, False), (True, False), (True, True)):
+        monkeypatch.setattr(ops, "_expanded_pays_4bit", lambda *a: expanded)
+        monkeypatch.setattr(ops, "_one_head_a_block", lambda *a: one and case.cache.dim == 128)
+        whole = case.run().cpu()
+        got = case.run(block_table=with_holes(case, holes).cuda()).cpu()
+        want, most = expected(case.cache, case.q, case.q_lens, case.scale, case.window, pages_hidden(case.cache, holes), expanded)
+        assert beyond(got, want, most) == 0, (expanded, one, float((got.double() - want).abs().max()))
+        at = 0
+        for i, count in enumerate(case.q_lens):
+            if not holes.get(i):
+                assert torch.equal(got[at:at + count], whole[at:at + count])
+            at += count
+
+
+@cuda
+@pytest.mark.parametrize("window", [None, 300])
+@pytest.mark.parametrize("hq,hkv,dim,page", [(8, 2, 128, 16), (3, 3, 128, 8), (32, 4, 64, 4), (8, 2, 64, 16), (4, 2, 128, 64)])
+def test_holes_that_portions_meet_either_way(monkeypatch, hq, hkv, dim, page, window):
+    lens, q_lens = [700, 40, 333, 0, 520, 300], [150, 40, 1, 0, 200, 260]
+    c = Case(lens, hq, hkv, dim, page, torch.bfloat16, 80 + page, q_lens, window=window)
+    both_ways(monkeypatch, c, {0: [470 // page, 480 // page + 1, 699 // page], 4: [500 // page], 5: [0, 128 // page, 299 // page]})
+
+
+@cuda
+def test_holes_that_no_query_sees_change_nothing(monkeypatch):
+    """Behind the last key, before the window."""
+    c = Case([700, 130], 8, 2, 128, 16, torch.bfloat16, 90, [100, 130], window=64)
+    monkeypatch.setattr(ops, "_expanded_pays_4bit", lambda *a: True)
+    table = c.cache.table(width=60)
+    want = c.run(block_table=table.cuda())
+    table[0, :33], table[0, 44:], table[1, 9:] = -1, -1, 1 << 30
+    assert torch.equal(c.run(block_table=table.cuda()), want)
+
+
+@cuda
+def test_holes_in_runs_of_sequences_and_in_a_captured_call(monkeypatch):
+    lens, q_lens = [400, 130, 0, 390, 64, 100, 40], [300, 130, 0, 260, 0, 100, 33]
+    c = Case(lens, 8, 2, 128, 16, torch.bfloat16, 91, q_lens)
+    monkeypatch.setattr(ops, "EXPANDED_ROOM_4BIT", 2 * 4 * 25 * 2 * 16 * 128)
+    holes = {0: [3, 10], 3: [20], 5: [0]}
+    both_ways(monkeypatch, c, holes)
+    args = c.args(block_table=with_holes(c, holes).cuda())
+    ops.paged_attention_4bit(**args)
+    want = args["out"].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.paged_attention_4bit(**args)
+    args["out"].zero_()
+    args["block_table"].copy_(c.table())                 # the lengths and tables that a replay finds are the ones that count
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(args["out"], c.run())
+    args["block_table"].copy_(with_holes(c, holes))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(args["out"], want)
