@@ -2376,6 +2376,13 @@ def expanded_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads: int, 
 def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.Tensor, v_pool: torch.Tensor, v_steps: torch.Tensor, out: torch.Tensor,
                          block_table: torch.Tensor, kv_len: torch.Tensor, scale: float, window: Optional[int] = None, cu_q: Optional[torch.Tensor] = None,
                          q_lens=None, scratch=None) -> None:
+def _expanded_room(scratch, tag: str, shape, dtype: torch.dtype) -> torch.Tensor:
+    """Room for expanded pages from a caller's ``scratch``, asked for in powers of two: one that doubles what it keeps when it has to grow then grows to what is
+    asked for, and keys and values together never hold more than the room (or twice what one sequence takes that needs more)."""
+    numel = math.prod(shape)
+    return scratch(tag, (1 << (numel - 1).bit_length(),), dtype)[:numel].view(shape)
+
+
     """Attention over a cache of 4 bits: q, out [N, Hq, D] (float32 or bfloat16), ``block_table`` int32 [S, width], ``kv_len`` int32 [S] with
     the keys of this step in it.  Without ``cu_q`` every sequence has one query token, the last (N = S); else sequence i has the tokens
     ``cu_q[i]:cu_q[i + 1]`` (int32 [S + 1], rising, rows of q), the last of its ``kv_len[i]``, and ``q_lens`` are their numbers as the host knows
@@ -2441,7 +2448,8 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
             if scratch is None:
                 k_out, v_out, table_out = (torch.empty(shape, dtype=kept, device=q.device) for shape, kept in shapes)
             else:
-                k_out, v_out, table_out = (scratch(f"attn4.{what}", shape, kept) for what, (shape, kept) in zip(("k", "v", "table"), shapes))
+                k_out, v_out = (_expanded_room(scratch, f"attn4.{what}", *kept) for what, kept in zip(("k", "v"), shapes))
+                table_out = scratch("attn4.table", *shapes[2])
             for first in range(0, s, run_of):
                 end = min(first + run_of, s)
                 lens = q_lens[first:end]
