@@ -2236,6 +2236,14 @@ def _refuse_16(name: str) -> None:
     raise KernelError(f"{name}: tensors must start at a multiple of 16 bytes")
 
 
+def _check_steps(name: str, k_steps: int, v_steps: int, head_dim: int, page_size: int) -> None:
+    """Steps may start where a row of steps may in a pool that starts at a multiple of 16 bytes: a layer's part of a cache's pool does."""
+    groups = head_dim // GROUP_4BIT
+    least = 16 if page_size % 16 == 0 else min(16, 4 * (groups & -groups))
+    if (k_steps | v_steps) % least:
+        raise KernelError(f"{name}: steps of {groups} groups in pages of {page_size} must start at a multiple of {least} bytes")
+
+
 def qk_norm_rope_write_4bit(qkv: torch.Tensor, q_out: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.Tensor, v_pool: torch.Tensor, v_steps: torch.Tensor,
                             slots: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
                             eps: float, n_heads: int, n_kv_heads: int, head_dim: int, rotary: int, page_size: int) -> None:
@@ -2272,8 +2280,10 @@ def qk_norm_rope_write_4bit(qkv: torch.Tensor, q_out: torch.Tensor, k_pool: torc
         return
     _check_against(k_pool)
     at = qkv.data_ptr(), q_out.data_ptr(), k_pool.data_ptr(), k_steps.data_ptr(), v_pool.data_ptr(), v_steps.data_ptr()
-    if (at[0] | at[1] | at[2] | at[3] | at[4] | at[5]) % 16:
+    if (at[0] | at[1] | at[2] | at[4]) % 16:
         _refuse_16(name)
+    if (at[3] | at[5]) % 16:
+        _check_steps(name, at[3], at[5], head_dim, page_size)
     words = _WRITE_4BIT.pack(kind, *at, slots.data_ptr(), cos.data_ptr(), sin.data_ptr(), 0 if q_weight is None else q_weight.data_ptr(),
                              0 if k_weight is None else k_weight.data_ptr(), eps, n, n_heads, hkv, head_dim, rotary, page, n_pages)
     check(fn("pb_qk_norm_rope_write_4bit")(words, stream()), name)
@@ -2318,8 +2328,10 @@ def expand_pages_4bit(k_pool: torch.Tensor, k_steps: torch.Tensor, v_pool: torch
 
 
 def _launch_expand(name: str, kind: int, pools, table: int, kv_len: int, k_out: int, v_out: int, table_out: int, *sizes) -> None:
-    if (pools[0] | pools[1] | pools[2] | pools[3] | k_out | v_out) % 16:
+    if (pools[0] | pools[2] | k_out | v_out) % 16:
         _refuse_16(name)
+    if (pools[1] | pools[3]) % 16:
+        _check_steps(name, pools[1], pools[3], sizes[3], sizes[4])
     check(fn("pb_expand_pages_4bit")(_EXPAND_4BIT.pack(kind, *pools, table, kv_len, k_out, v_out, table_out, *sizes), stream()), name)
 
 
@@ -2360,8 +2372,15 @@ def _expanded_pays_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads:
     return expanded < on_codes
 
 
-# Bytes that expanded pages may take, unless one sequence's alone are more: portions of more sequences than that holds are runs of calls.
+# Bytes that expanded pages may take, unless one sequence's alone are more: portions of more sequences than that holds are runs of calls.  A power of two.
 EXPANDED_ROOM_4BIT = 1 << 30
+
+
+def _expanded_room(scratch, tag: str, shape, dtype: torch.dtype) -> torch.Tensor:
+    """Room for expanded pages from a caller's ``scratch``, asked for in powers of two: one that doubles what it keeps when it has to grow then grows to what is
+    asked for, and keys and values together never hold more than the room (or twice what one sequence takes that needs more)."""
+    numel = math.prod(shape)
+    return scratch(tag, (1 << (numel - 1).bit_length(),), dtype)[:numel].view(shape)
 
 
 def expanded_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int, width: int, page_size: int, window: int, dtype: torch.dtype) -> Optional[str]:
@@ -2376,13 +2395,6 @@ def expanded_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads: int, 
 def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.Tensor, v_pool: torch.Tensor, v_steps: torch.Tensor, out: torch.Tensor,
                          block_table: torch.Tensor, kv_len: torch.Tensor, scale: float, window: Optional[int] = None, cu_q: Optional[torch.Tensor] = None,
                          q_lens=None, scratch=None) -> None:
-def _expanded_room(scratch, tag: str, shape, dtype: torch.dtype) -> torch.Tensor:
-    """Room for expanded pages from a caller's ``scratch``, asked for in powers of two: one that doubles what it keeps when it has to grow then grows to what is
-    asked for, and keys and values together never hold more than the room (or twice what one sequence takes that needs more)."""
-    numel = math.prod(shape)
-    return scratch(tag, (1 << (numel - 1).bit_length(),), dtype)[:numel].view(shape)
-
-
     """Attention over a cache of 4 bits: q, out [N, Hq, D] (float32 or bfloat16), ``block_table`` int32 [S, width], ``kv_len`` int32 [S] with
     the keys of this step in it.  Without ``cu_q`` every sequence has one query token, the last (N = S); else sequence i has the tokens
     ``cu_q[i]:cu_q[i + 1]`` (int32 [S + 1], rising, rows of q), the last of its ``kv_len[i]``, and ``q_lens`` are their numbers as the host knows
@@ -2437,8 +2449,10 @@ def _expanded_room(scratch, tag: str, shape, dtype: torch.dtype) -> torch.Tensor
     _check_against(k_pool)
     pools = k_pool.data_ptr(), k_steps.data_ptr(), v_pool.data_ptr(), v_steps.data_ptr()
     q_at, out_at = q.data_ptr(), out.data_ptr()
-    if (q_at | out_at | pools[0] | pools[1] | pools[2] | pools[3]) % 16:
+    if (q_at | out_at | pools[0] | pools[2]) % 16:
         _refuse_16(name)
+    if (pools[1] | pools[3]) % 16:
+        _check_steps(name, pools[1], pools[3], d, page_size)
     if cu_q is not None and scale > 0.0:
         run_of = min(s, max(1, EXPANDED_ROOM_4BIT // (4 * width * hkv * page_size * d)))
         dense = expanded_4bit(run_of, most_tokens, hq, hkv, d, width, page_size, window, dtype)
