@@ -20,9 +20,9 @@
 // neighbouring groups, is an operand as it is: its halves stand in two places of the sum, of which each copy's other operand has one empty.
 // The weights change places between the two products by movmatrix.
 //
-// What bounds it: instructions.  4 query heads a kv head, heads of 128, bfloat16: 317 warp instructions for 16 keys (a third of them shifts and masks of codes,
-// 18 products), issue slots 54 % full with the three blocks an SM that registers allow, ALU 51, products 24, and the same time when all pages lie
-// in L2.  64 sequences of 4,096 to 8,192 keys take 108 us (507 MB: 4.7 TB/s; keys beyond the first thousands come at 5.4), 8 of 4,096 take
+// What bounds it: the latency of a turn, one chain of products, shuffles, exponentials and products.  4 query heads a kv head, heads of 128, bfloat16: 317 warp
+// instructions for 16 keys (a third of them shifts and masks of codes, 18 products) fill 54 % of the issue slots with the three blocks an SM that registers
+// allow, 10.6 warps, ALU 51, products 24, and it takes the same time when all pages lie in L2.  64 sequences of 4,096 to 8,192 keys take 108 us (507 MB: 4.7 TB/s; keys beyond the first thousands come at 5.4), 8 of 4,096 take
 // 17, one of 900 takes 5.5.  16 rows of a block take 588 instructions for 16 keys, less than twice as many for four times the
 // rows: 12 portions of 7 tokens over 1,300 to 2,600 keys take 39 us.  (tcgen05 would want codes as bfloat16 in shared memory, which is more traffic there
 // than all the rest.  Tried: keys and values refilled apart, 111 us instead of 108 at the time; four blocks of two buffers an SM, 111; five warps a block, 145;
@@ -1112,8 +1112,8 @@ __global__ void __launch_bounds__(128) join_4bit_kernel(const Attend4 a, int D, 
 
 // Behind a dense kernel over expanded pages, where pages that are none stand as keys of zeros: the rows of sequences that see such, once more on codes.
 // A row of blocks a sequence; all others' have nothing to do but to look at the table, which they do while the dense kernel runs: that one was launched
-// behind everything that writes tables and lengths.  (us without such pages, without this launch and with it: 512 tokens over 6,000 keys 63.0, 64.2; 2,048 tokens
-// 150.9, 151.7.  All behind pdl_wait 62.6, 65.5.)
+// behind everything that writes tables and lengths.  (us without such pages, without this launch and with it, of two runs: 512 tokens over 6,000 keys
+// 63.0, 64.2 and 64.0, 65.7; 2,048 tokens 150.9, 151.7 and 151.2, 152.2.  All behind pdl_wait 62.6, 65.5.)
 template <typename T, int G, int NT, typename Turns, int BLOCKS>
 __global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_holes_kernel(const Attend4 a) {
     using B = Attend4Block<T, G, NT, 1>;

@@ -2,7 +2,8 @@
 //
 //   qk_norm_rope_write_4bit   per (token, head) of a projection row [q: Hq*D | k: Hkv*D | v: Hkv*D]: q and k are normed (x / sqrt(mean(x^2) + eps) * w,
 //                             where weights are given) and their first `rotary` channels turned, (u, v) -> (u cos - v sin, v cos + u sin)
-//                             with v half a turn's width behind u; q is rounded to T, k and v to T and then to 4 bits, at their slots.
+//                             with v half a turn's width behind u; q is rounded to T, k and v to T and then to 4 bits, at their slots.  (q in 32 bits, as
+//                             much as its scores have; k in 64, because a rounding more may move a code.)
 //   expand_pages_4bit         the values of the pages that sequences hold, as T, into pages of their own.
 #include "cache4.cuh"
 

@@ -2359,7 +2359,7 @@ def _expanded_pays_4bit(n_seqs: int, most_tokens: int, n_heads: int, n_kv_heads:
 
     The kernel on codes takes what its blocks' turns take: 0.235 us a turn of 32 keys and 16 rows and SM (heads of 64: two thirds of that), and 16 turns'
     time for a block's start and end.  Expanded pages cost their bytes twice, and the dense kernels 8 ns a key where a block takes one head, else 13 for as
-    many pairs of heads and tiles of query tokens as there are SMs.  (us on codes and expanded, heads 32 / 8 of 128, sequences of 0.7 to all of so many keys,
+    many pairs of heads and tiles of query tokens as there are SMs (148).  (us on codes and expanded, heads 32 / 8 of 128, sequences of 0.7 to all of so many keys,
     16 / 128 / 512 rows a kv head: 1 of 1,000  8.7, 17;  12, 17;  20, 19;    1 of 8,000  15, 78;  33, 78;  113, 80;    8 of 1,000  13, 29;  57, 31;
     179, 32;    8 of 4,000  21, 90;  115, 92;  409, 93;    1 of 6,000 with 2,048 rows  318, 62.  The slower side is taken by up to 30 % between them.)"""
     keys = min(width * page_size, window + most_tokens) if window else width * page_size
@@ -2399,13 +2399,13 @@ def paged_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, k_steps: torch.T
     the keys of this step in it.  Without ``cu_q`` every sequence has one query token, the last (N = S); else sequence i has the tokens
     ``cu_q[i]:cu_q[i + 1]`` (int32 [S + 1], rising, rows of q), the last of its ``kv_len[i]``, and ``q_lens`` are their numbers as the host knows
     them.  A query sees the keys up to its own, with ``window`` w the last w of them, but none whose page is not one of the pool (-1, say).
-    (``kv_len[i]`` is no more than the table's width holds.)  A query that sees no key gets zeros.  Rows of ``out`` that are no sequence's stay as
-    they were.
+    (``kv_len[i]`` is no more than the table's width holds.)  A query that sees no key, as one that stands before its sequence's
+    first (a padded portion's), gets zeros.  Rows of ``out`` that are no sequence's stay as they were.
 
     bfloat16 portions of many tokens, where the dense attention of prompt portions has a kernel for their sizes, are attended to over expanded
     pages (``expanded_4bit``), which takes room for S * width pages, of as many sequences at a time as 1 GiB holds.  (There keys and values are operands rounded to bfloat16, as a cache
     of bfloat16 holds them: over 6,000 keys outputs are 3.7e-3 off, 2.3e-3 on codes and 1.7e-3 by their own rounding alone.)  A key or a value that is NaN makes NaN of what the queries
-    that see it get from its kv head, a value's of its group's channels at least; no other query's changes.  ``scratch(tag, shape, dtype)`` gives tensors to work in; without it they are made here."""
+    that see it get from its kv head, a value's of its group's channels at least, and reaches no other query.  ``scratch(tag, shape, dtype)`` gives tensors to work in; without it they are made here."""
     name = "paged_attention_4bit"
     tensors = (q, k_pool, k_steps, v_pool, v_steps, out, block_table, kv_len)
     if (where := _on_one_device(name, (*tensors, cu_q))) != _current_device():
