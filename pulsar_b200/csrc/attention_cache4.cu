@@ -68,6 +68,7 @@ namespace {
 struct Call4 {
     Attend4 a;
     int dtype, D, most_tokens;
+    double turns;                       // of all heads, at most
     // 0, or the error; `rows` of a block: 0 for attention_4bit_rows
     int read(const long long* words, int& rows) {
         Words4 w{words};
@@ -102,9 +103,8 @@ struct Call4 {
         const int group = a.Hq / a.Hkv;
         if (rows == 0) rows = pb_attention_4bit_rows(dtype, most_tokens * group, D);
         const long long row_blocks = ((long long)most_tokens * group + rows - 1) / rows, keys = (long long)a.width * a.page_size;
-        if (a.n_seqs > 65535 || (long long)most_tokens * a.Hq > 0x3fffffff || (long long)a.n_pages * a.Hkv * a.page_size >= 0xffffffffLL || keys > 0x7ffffff0LL ||
-            (double)a.n_seqs * row_blocks * a.Hkv * (keys / kTile4 + 1 + kGap4) > 1.0e9)
-            return PB_ERR_TOO_LARGE;
+        if (a.n_seqs > 65535 || (long long)most_tokens * a.Hq > 0x3fffffff || (long long)a.n_pages * a.Hkv * a.page_size >= 0xffffffffLL || keys > 0x7ffffff0LL) return PB_ERR_TOO_LARGE;
+        turns = (double)a.n_seqs * row_blocks * a.Hkv * (keys / kTile4 + 1 + kGap4);
         a.page_shift = log2_exact(a.page_size);
         a.row_blocks = (int)row_blocks;
         a.bounds = pool_bounds_now();
@@ -120,7 +120,7 @@ PB_EXPORT int pb_paged_attention_4bit(const long long* words, cudaStream_t strea
     const Attend4& a = c.a;
     if (a.blocks == 0 || a.blocks < -8 || (a.blocks > 0 && (a.sums == nullptr || a.plan == nullptr))) return PB_ERR_BAD_SIZE;
     if (c.most_tokens == 0 || a.n_seqs == 0) return 0;
-    if (a.blocks < 0 && (long long)a.row_blocks * a.Hkv > 65535) return PB_ERR_TOO_LARGE;
+    if (c.turns > 1.0e9 || (a.blocks < 0 && (long long)a.row_blocks * a.Hkv > 65535)) return PB_ERR_TOO_LARGE;
     return (c.dtype == PB_F32 ? attend_4bit_f32 : attend_4bit_bf16)(a, c.D / kGroup4, rows, c.most_tokens, stream);
 }
 

@@ -70,10 +70,11 @@ struct Entry4 {
     int seq, first_token, n_tokens, kv_len, row0, token0, token1;
     int first, last, turns;             // the keys [first, last] that any of its rows sees; turns begin at first rounded down
 
-    __device__ __forceinline__ Entry4(const Attend4& a, int entry, int rows) {
+    __device__ __forceinline__ Entry4(const Attend4& a, int entry, int rows) : Entry4(a, entry / a.row_blocks, entry % a.row_blocks, rows) {}
+    __device__ __forceinline__ Entry4(const Attend4& a, int sequence, int row_block, int rows) {
         const int group = a.Hq / a.Hkv;
-        seq = entry / a.row_blocks;
-        row0 = (entry - seq * a.row_blocks) * rows;
+        seq = sequence;
+        row0 = row_block * rows;
         first_token = a.cu_q ? a.cu_q[seq] : seq;
         n_tokens = a.cu_q ? a.cu_q[seq + 1] - first_token : 1;
         kv_len = a.kv_len[seq];
@@ -1131,7 +1132,7 @@ __global__ void __launch_bounds__(kWarps4 * 32, BLOCKS) attend_4bit_holes_kernel
     if (!hole) return;
     for (int item = blockIdx.x; item < a.Hkv * a.row_blocks; item += gridDim.x) {
         const int kvh = item / a.row_blocks;
-        const Entry4 entry(a, seq * a.row_blocks + item - kvh * a.row_blocks, B::kRows);
+        const Entry4 entry(a, seq, item - kvh * a.row_blocks, B::kRows);
         if (entry.row0 >= n_tokens * (a.Hq / a.Hkv)) continue;
         attend_part<T, B, Turns>(a, entry, kvh, 0, entry.turns, shared);
         for (int i = threadIdx.x; i < B::kRows * (D / 4); i += kWarps4 * 32) {

@@ -123,3 +123,19 @@ def test_holes_in_runs_of_sequences_and_in_a_captured_call(monkeypatch):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(args["out"], want)
+
+
+@cuda
+def test_many_sequences_under_a_wide_table(monkeypatch):
+    """One long portion among 250, a table of 131,072 keys: more turns than the kernel on codes can deal out, which a look for holes does not do."""
+    lens, q_lens = [2000] + [3 + i % 20 for i in range(249)], [2000] + [1 + i % 3 for i in range(249)]
+    c = Case(lens, 8, 1, 64, 16, torch.bfloat16, 92, q_lens)
+    monkeypatch.setattr(ops, "_expanded_pays_4bit", lambda *a: True)
+    holes = {0: [5, 60], 7: [0]}
+    wide = torch.full((len(lens), 8192), -1, dtype=torch.int32)
+    table = with_holes(c, holes)
+    wide[:, :table.shape[1]] = table
+    got = c.run(block_table=wide.cuda()).cpu()
+    want, most = expected(c.cache, c.q, q_lens, c.scale, None, pages_hidden(c.cache, holes), True)
+    _, on_codes = expected(c.cache, c.q, q_lens, c.scale, None, pages_hidden(c.cache, holes))
+    assert beyond(got, want, torch.maximum(most, on_codes)) == 0
